@@ -235,6 +235,124 @@ int wf_qlinear_allgather(int64_t ctx, int64_t comm, int64_t weight, const void* 
 int wf_qlinear_noalloc(int64_t ctx, int64_t weight, int64_t x_dev, int x_dtype, int64_t m, int64_t y_dev,
                        int64_t stream);
 
+/* ---- attention over a paged cache ------------------------------------------------------
+ * What lies between the projections of a decoder layer.  (No counterpart in the reference: its custom_call kernels end
+ * with softmax, nvidia/ops/CudaCustomCallKernel.java:50-59, and its graph holds attention as dot_general, softmax and
+ * dot_general on whole score matrices.)  q, k, v come from the projections, wf_qk_norm_rope norms and rotates them and
+ * brings k and v into the cache, wf_prompt_attention (prompts) or wf_tree_attention (one or a few tokens per sequence)
+ * reads it, and its bf16 rows are what wf_qlinear takes for the output projection.
+ *
+ * The arguments that belong to buffers are passed as structs by address, so that a caller fills them in once; all
+ * addresses in them are device addresses held in 64-bit integers.  A struct is read during the call only.  Every call
+ * enqueues on `stream` and returns; nothing is read from or copied to the host.  Lengths, tables and masks are read on
+ * the device when the kernel runs, so that a recorded graph serves every step of a growing cache; what they may hold is
+ * checked there (a page, a slot, a position or a count outside its range is skipped and makes the next wf_stream_sync
+ * return WF_ERR_INDEX), never followed.
+ *
+ * wf_kv_cache: keys and values are bf16 [layers][pages][kv_heads][page_tokens][head_dim], both 16-byte aligned.
+ * page_tokens is a power of two from 16 to 1024, head_dim a multiple of 8 from 8 to 128.  Token t of a sequence lies in row
+ * t % page_tokens of page table[t / page_tokens].  page_tokens == 1 is a packed tensor [tokens][kv_heads][head_dim]: a
+ * prompt's keys and values one behind the other, without a cache (layers 1, pages = tokens). */
+typedef struct wf_kv_cache {
+    int64_t keys_dev, values_dev;
+    int64_t pages;
+    int32_t layers, kv_heads, page_tokens, head_dim;
+} wf_kv_cache;
+
+/* For every token and head: x' = x / sqrt(mean(x^2) + eps) * gamma (WF_QK_NORM; q and k only), then the rotation of the first
+ * rot_dim elements, pairs (i, i + rot_dim/2) or, with WF_ROPE_ADJACENT, (2i, 2i + 1):
+ *     (a, b) -> (a c - b s, b c + a s)      c, s = rope[position][i]
+ * in fp32, rounded once to bf16.  v is rounded only.
+ *   q_dev, k_dev, v_dev   [tokens][heads * head_dim] of x_dtype, *_stride elements from one token to the next
+ *   gamma_*_dev           fp32 [head_dim], 0 = ones
+ *   rope_dev              fp32 [rope_rows][rot_dim / 2][2], cosine and sine; rot_dim a multiple of 8, 0 = no rotation
+ *   positions_dev         int32 [tokens], rows of rope (not read when rot_dim is 0)
+ *   slots_dev             int64 [tokens]: where k and v go, page * page_tokens + row; negative = nowhere; 0 (no array) = slot i
+ *                         for token i.  Two tokens must not share a slot.
+ *   q_out_dev             bf16 [tokens][q_heads][head_dim]
+ * q_dev or k_dev with v_dev may be 0 (that part is not wanted).  A token whose position or slot is outside its range gets zeros in
+ * q_out and is not stored. */
+#define WF_QK_NORM 1
+#define WF_ROPE_ADJACENT 2
+typedef struct wf_qk_norm_rope_args {
+    int64_t q_dev, k_dev, v_dev;
+    int64_t q_stride, k_stride, v_stride;
+    int64_t gamma_q_dev, gamma_k_dev;
+    int64_t rope_dev, rope_rows;
+    int64_t positions_dev, slots_dev;
+    int64_t q_out_dev;
+    int64_t tokens;
+    int32_t x_dtype, q_heads, rot_dim, flags;
+    float eps;
+} wf_qk_norm_rope_args;
+int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* args, const wf_kv_cache* cache, int layer, int64_t stream);
+
+/* Causal attention over whole prompts, packed one behind the other: sequence s has the rows [q_offsets[s], q_offsets[s+1]) of q and
+ * k_lens[s] keys, of which its rows are the last; row r sees the keys 0 .. k_lens[s] - rows + r.  Query head h reads the keys of
+ * head h / (q_heads / kv_heads).   out = softmax(scale q k^T) v, a row that sees no key is zeros.
+ *   q_dev, out_dev   bf16 [tokens][q_heads][head_dim]; q_stride elements (a multiple of 8) from one token of q to the next, 16-byte
+ *                    aligned; out without gaps
+ *   q_offsets_dev    int32 [seqs + 1], ascending, the last at most `tokens`
+ *   cache            with page_tokens == 1: packed keys and values, sequence s has the same rows of them as of q (tables_dev and k_lens_dev
+ *                    are 0); else pages by tables_dev int32 [seqs][table_stride] and k_lens_dev int32 [seqs]
+ * Products are bf16, scores, sums and the running maximum fp32; the weights exp(score - m) are rounded to bf16 for the second
+ * product.  A key that a row does not see has no influence on it, whatever it and its value hold (Inf and NaN too). */
+typedef struct wf_prompt_attention_args {
+    int64_t q_dev, out_dev;
+    int64_t q_stride;
+    int64_t q_offsets_dev;
+    int64_t tables_dev, table_stride;
+    int64_t k_lens_dev;
+    int64_t tokens;
+    int32_t seqs, q_heads;
+    float scale;
+} wf_prompt_attention_args;
+int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* args, const wf_kv_cache* cache, int layer, int64_t stream);
+
+/* Attention of a few new tokens per sequence over a long cache: a decoded token, or the nodes of a tree of drafted ones.  Sequence s
+ * has context[s] tokens in its pages and behind them the keys and values of its new tokens, row i of them at position
+ * context[s] + i.  Row i sees the whole context and the new token j where bit j of ancestors[row] is set.
+ *   q_dev, out_dev   as above, the new tokens of all sequences one behind the other
+ *   q_offsets_dev    int32 [seqs + 1]; 0 (no array) = max_drafts tokens for each
+ *   max_drafts       most new tokens of a sequence, 1 .. 64; max_context: most context of one (what the work is cut by; a longer
+ *                    one is WF_ERR_INDEX and its row zeros)
+ *   ancestors_dev    uint64 [tokens]; 0 (no array) = a chain, each sees those before it and itself
+ * The same sums and types; a long context is cut over the device and its parts are joined in a fixed order, so the result is the same
+ * from call to call. */
+typedef struct wf_tree_attention_args {
+    int64_t q_dev, out_dev;
+    int64_t q_stride;
+    int64_t q_offsets_dev;
+    int64_t tables_dev, table_stride;
+    int64_t context_dev;
+    int64_t ancestors_dev;
+    int64_t tokens, max_context;
+    int32_t seqs, q_heads, max_drafts;
+    float scale;
+} wf_tree_attention_args;
+int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* args, const wf_kv_cache* cache, int layer, int64_t stream);
+
+/* Pages copied to other pages in every layer: pairs_dev int32 [n][2] (from, to); rows_dev int32 [n], the rows of each that are in
+ * use, 0 (no array) = all.  No page may be the target of two pairs or source and target at once. */
+int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev, int64_t rows_dev, int64_t n, int64_t stream);
+/* After drafting: in every layer, token context[s] + kept[s][i] of sequence s becomes token context[s] + i, for i < counts[s].
+ * kept int32 [seqs][kept_stride] ascending; counts int32 [seqs]; tables and context as in wf_tree_attention. */
+int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, int64_t table_stride, int64_t context_dev, int64_t kept_dev,
+                     int64_t kept_stride, int64_t counts_dev, int64_t seqs, int64_t stream);
+
+/* Who holds which page: a count of holders per page, in host memory.  Process-wide handles that need no device, any thread may call.
+ * wf_pages_take: n free pages, each with one holder, lowest numbers first; all or none (WF_ERR_TOO_LARGE).  wf_pages_share: one
+ * holder more for each (a fork reads the pages of what it was forked from).  wf_pages_release: one fewer; a page without holders
+ * is free again.  A page that is not held, or named more often than it is held, is WF_ERR_INDEX and nothing is changed.  wf_pages_info:
+ * pages in all, free ones; wf_pages_holders: how many hold page id. */
+int wf_pages_create(int64_t pages, int64_t* pool);
+int wf_pages_destroy(int64_t pool);
+int wf_pages_take(int64_t pool, int64_t n, int32_t* ids);
+int wf_pages_share(int64_t pool, int64_t n, const int32_t* ids);
+int wf_pages_release(int64_t pool, int64_t n, const int32_t* ids);
+int wf_pages_info(int64_t pool, int64_t* pages, int64_t* free_pages);
+int wf_pages_holders(int64_t pool, int32_t id, int64_t* holders);
+
 /* ---- collectives --------------------------------------------------------------------
  * Replaces CollectiveApi.allGather(Tensor input, Tensor output)
  * (warpforge-io/src/main/java/io/surfworks/warpforge/io/collective/CollectiveApi.java:137-146,

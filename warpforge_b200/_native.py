@@ -19,6 +19,30 @@ c_int, c_i64, c_vp, c_f32 = ctypes.c_int, ctypes.c_int64, ctypes.c_void_p, ctype
 c_char_p = ctypes.c_char_p
 P = ctypes.POINTER
 
+
+class KvCacheArgs(ctypes.Structure):  # wf_kv_cache
+    _fields_ = [("keys_dev", c_i64), ("values_dev", c_i64), ("pages", c_i64),
+                ("layers", ctypes.c_int32), ("kv_heads", ctypes.c_int32), ("page_tokens", ctypes.c_int32), ("head_dim", ctypes.c_int32)]
+
+
+class QkNormRopeArgs(ctypes.Structure):  # wf_qk_norm_rope_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "k_dev", "v_dev", "q_stride", "k_stride", "v_stride", "gamma_q_dev", "gamma_k_dev", "rope_dev", "rope_rows",
+                                     "positions_dev", "slots_dev", "q_out_dev", "tokens")] + [
+        (n, ctypes.c_int32) for n in ("x_dtype", "q_heads", "rot_dim", "flags")] + [("eps", c_f32)]
+
+
+class PromptAttentionArgs(ctypes.Structure):  # wf_prompt_attention_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "out_dev", "q_stride", "q_offsets_dev", "tables_dev", "table_stride", "k_lens_dev", "tokens")] + [
+        ("seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("scale", c_f32)]
+
+
+class TreeAttentionArgs(ctypes.Structure):  # wf_tree_attention_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "out_dev", "q_stride", "q_offsets_dev", "tables_dev", "table_stride", "context_dev", "ancestors_dev", "tokens",
+                                     "max_context")] + [("seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_drafts", ctypes.c_int32), ("scale", c_f32)]
+
+
+c_i32 = ctypes.c_int32
+
 # name -> (restype, argtypes); must list every function declared in include/wfb200.h
 SIGNATURES = {
     "wf_version": (c_int, []),
@@ -60,6 +84,18 @@ SIGNATURES = {
     "wf_qlinear": (c_int, [c_i64, c_i64, c_vp, c_int, c_int, c_i64, c_vp, c_int, c_i64]),
     "wf_qlinear_noalloc": (c_int, [c_i64, c_i64, c_i64, c_int, c_i64, c_i64, c_i64]),
     "wf_qlinear_allgather": (c_int, [c_i64, c_i64, c_i64, c_vp, c_int, c_i64, c_vp, c_i64]),
+    "wf_qk_norm_rope": (c_int, [c_i64, P(QkNormRopeArgs), P(KvCacheArgs), c_int, c_i64]),
+    "wf_prompt_attention": (c_int, [c_i64, P(PromptAttentionArgs), P(KvCacheArgs), c_int, c_i64]),
+    "wf_tree_attention": (c_int, [c_i64, P(TreeAttentionArgs), P(KvCacheArgs), c_int, c_i64]),
+    "wf_cache_copy_pages": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64]),
+    "wf_cache_compact": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "wf_pages_create": (c_int, [c_i64, P(c_i64)]),
+    "wf_pages_destroy": (c_int, [c_i64]),
+    "wf_pages_take": (c_int, [c_i64, c_i64, P(c_i32)]),
+    "wf_pages_share": (c_int, [c_i64, c_i64, P(c_i32)]),
+    "wf_pages_release": (c_int, [c_i64, c_i64, P(c_i32)]),
+    "wf_pages_info": (c_int, [c_i64, P(c_i64), P(c_i64)]),
+    "wf_pages_holders": (c_int, [c_i64, c_i32, P(c_i64)]),
     "wf_comm_get_unique_id": (c_int, [c_vp]),
     "wf_comm_init": (c_int, [c_i64, c_vp, c_int, c_int, P(c_i64)]),
     "wf_comm_destroy": (c_int, [c_i64, c_i64]),
@@ -103,6 +139,7 @@ WF_X_BF16, WF_X_F32, WF_X_RMSNORM_F32, WF_X_SWIGLU_F32 = 0, 1, 2, 3
 WF_Q4_0_ORDER_REFERENCE, WF_Q4_0_ORDER_GGML = 0, 1
 WF_DTYPE_F32, WF_DTYPE_BF16 = 0, 1
 WF_OP_NEW_X, WF_OP_DEPENDS = 1, 2
+WF_QK_NORM, WF_ROPE_ADJACENT = 1, 2
 
 
 class NativeLibraryMissing(RuntimeError):

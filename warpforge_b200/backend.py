@@ -88,18 +88,21 @@ class Tensor:
 
 @dataclass
 class DeviceTensor:
-    """Device-resident tensor: raw pointer + shape + dtype.  ``owner`` keeps whatever
-    allocated the memory alive (a CudaContext allocation or, e.g., a torch tensor)."""
+    """Device-resident tensor: raw pointer + shape + dtype ('f32', 'bf16', 'i32' or 'i64').  ``owner`` keeps whatever
+    allocated the memory alive (a CudaContext allocation or, e.g., a torch tensor).  ``row_stride``: elements from one
+    entry of the first dimension to the next where they lie further apart than they are long; 0 = no gaps (only the
+    operators of ``attention`` look at it)."""
     ptr: int
     shape_: Sequence[int]
     dtype: str = "f32"
     owner: object = None
+    row_stride: int = 0
 
     def shape(self):
         return tuple(self.shape_)
 
     def nbytes(self) -> int:
-        return int(np.prod(self.shape_)) * (4 if self.dtype == "f32" else 2)
+        return int(np.prod(self.shape_)) * {"f32": 4, "i32": 4, "i64": 8}.get(self.dtype, 2)
 
 
 class CudaContext:

@@ -1,0 +1,179 @@
+// Attention over a paged cache: wf_prompt_attention and wf_tree_attention.
+//   out = softmax(scale q k^T) v   over the keys that a row sees, with base-2 exponentials: softmax(x) = 2^(x log2 e - m) / sum
+#include "wf_attention.cuh"
+
+namespace wf {
+
+// A warp per row and head, key by key.
+__global__ void __launch_bounds__(128) prompt_rows_kernel(const __grid_constant__ PromptParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t n = p.tokens * p.q_heads;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); i < n; i += (int64_t)gridDim.x * 4) {
+        const int row = (int)(i / p.q_heads), head = (int)(i % p.q_heads);
+        int s = 0;
+        while (s < p.seqs && !(row >= p.q_offsets[s] && row < p.q_offsets[s + 1])) s++;
+        if (s == p.seqs) continue;
+        const PromptSeq q = prompt_seq(p, s);
+        if (row >= q.row0 + q.rows) continue;
+        const int last = q.keys - q.rows + (row - q.row0);
+        attend_row(p.cache, q.place, p.q + (size_t)row * p.q_stride + (size_t)head * p.cache.dim, p.out + ((size_t)row * p.q_heads + head) * p.cache.dim,
+                   head / p.group, min(q.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
+    }
+}
+__global__ void __launch_bounds__(128) tree_rows_kernel(const __grid_constant__ TreeParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int64_t n = (int64_t)p.seqs * p.max_drafts * p.q_heads;
+    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); i < n; i += (int64_t)gridDim.x * 4) {
+        const int head = (int)(i % p.q_heads), draft = (int)(i / p.q_heads % p.max_drafts), s = (int)(i / p.q_heads / p.max_drafts);
+        const TreeSeq q = tree_seq(p, s);
+        if (draft >= q.rows) continue;
+        const int row = q.row0 + draft;
+        attend_row(p.cache, q.place, p.q + (size_t)row * p.q_stride + (size_t)head * p.cache.dim, p.out + ((size_t)row * p.q_heads + head) * p.cache.dim,
+                   head / p.group, q.context < 0 ? 0 : q.context + q.rows, p.scale_log2, p.status, SeesAncestors{q.context, ancestors_of(p, row, draft)});
+    }
+}
+
+}  // namespace wf
+
+using namespace wf;
+
+static int check_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too) {
+    if (!cache) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null cache", what);
+    if (!cache->keys_dev || !cache->values_dev || (cache->keys_dev | cache->values_dev) & 15)
+        return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: keys and values must be 16-byte aligned device addresses", what);
+    if (cache->layers < 1 || layer < 0 || layer >= cache->layers) return set_error(c, WF_ERR_SHAPE, "%s: layer %d of %d", what, layer, cache->layers);
+    if (cache->head_dim < 8 || cache->head_dim > ATTN_MAX_DIM || cache->head_dim % 8)
+        return set_error(c, WF_ERR_SHAPE, "%s: head_dim %d is not a multiple of 8 from 8 to %d", what, cache->head_dim, ATTN_MAX_DIM);
+    const int p = cache->page_tokens;
+    if (!(packed_too && p == 1 && cache->layers == 1) && (p < 16 || p > 1024 || (p & (p - 1))))
+        return set_error(c, WF_ERR_SHAPE, "%s: page_tokens %d is not a power of two from 16 to 1024", what, p);
+    if (cache->kv_heads < 1 || cache->kv_heads > 1024 || cache->pages < 0 || cache->pages > (1LL << 31) - 1 ||
+        cache->pages * cache->kv_heads * p > (1LL << 31) - 1024)
+        return set_error(c, WF_ERR_SHAPE, "%s: bad cache, pages=%lld kv_heads=%d", what, (long long)cache->pages, cache->kv_heads);
+    return WF_OK;
+}
+namespace wf {
+CacheView cache_layer(const wf_kv_cache& cache, int layer) {
+    CacheView v;
+    v.pages = cache.pages;
+    v.kv_heads = cache.kv_heads;
+    v.dim = cache.head_dim;
+    v.page_shift = __builtin_ctz((unsigned)cache.page_tokens);
+    const size_t skip = (size_t)layer * cache.pages * cache.kv_heads * cache.page_tokens * cache.head_dim;
+    v.keys = reinterpret_cast<bf16*>(cache.keys_dev) + skip;
+    v.values = reinterpret_cast<bf16*>(cache.values_dev) + skip;
+    return v;
+}
+int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too) { return check_cache(c, what, cache, layer, packed_too); }
+}  // namespace wf
+static int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
+    if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
+    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192)
+        return set_error(c, WF_ERR_SHAPE, "%s: bad shape tokens=%lld seqs=%d q_heads=%d", what, (long long)tokens, seqs, q_heads);
+    if (q_heads % cache->kv_heads) return set_error(c, WF_ERR_SHAPE, "%s: %d query heads over %d kv heads", what, q_heads, cache->kv_heads);
+    if (q_heads / cache->kv_heads > 128) return set_error(c, WF_ERR_TOO_LARGE, "%s: more than 128 query heads for each kv head", what);
+    if (q_stride < (int64_t)q_heads * cache->head_dim || q_stride % 8) return set_error(c, WF_ERR_SHAPE, "%s: q_stride %lld", what, (long long)q_stride);
+    return WF_OK;
+}
+template <class Params>
+static int launch_attention(Context* c, const char* what, void (*kernel)(Params), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const Params& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess) return cuda_status(c, e, what);
+    c->launches++;
+    return WF_OK;
+}
+
+#define ATTENTION_ENTER(ctxh)                                              \
+    Context* c = get_context(ctxh);                                        \
+    if (!c) return WF_ERR_INVALID_HANDLE;                                  \
+    ScopedLock _lk(c);                                                     \
+    if (!_lk.ok) return WF_ERR_BUSY;                                       \
+    WF_CUDA(c, cudaSetDevice(c->device));                                  \
+    cudaStream_t s = resolve_stream(c, stream)
+
+extern "C" {
+
+int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
+    ATTENTION_ENTER(ctx);
+    const char* what = "prompt_attention";
+    if (!a) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    int rc = check_cache(c, what, cache, layer, true);
+    if (rc == WF_OK) rc = check_queries(c, what, a->q_dev, a->out_dev, a->q_stride, a->tokens, a->seqs, a->q_heads, cache);
+    if (rc != WF_OK) return rc;
+    const bool packed = cache->page_tokens == 1;
+    if (!a->q_offsets_dev || a->q_offsets_dev & 3 || a->tables_dev & 3 || a->k_lens_dev & 3)
+        return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q_offsets, tables and k_lens are 4-byte aligned device arrays", what);
+    if (packed ? a->tables_dev || a->k_lens_dev : !a->tables_dev || !a->k_lens_dev)
+        return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: pages need tables and k_lens, packed keys take neither", what);
+    if (!packed && (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1))
+        return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld", what, (long long)a->table_stride);
+    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
+    PromptParams p{};
+    p.cache = cache_layer(*cache, layer);
+    p.q = reinterpret_cast<const bf16*>(a->q_dev);
+    p.out = reinterpret_cast<bf16*>(a->out_dev);
+    p.q_stride = a->q_stride;
+    p.q_offsets = reinterpret_cast<const int*>(a->q_offsets_dev);
+    p.tables = reinterpret_cast<const int*>(a->tables_dev);
+    p.table_stride = a->table_stride;
+    p.k_lens = reinterpret_cast<const int*>(a->k_lens_dev);
+    p.tokens = a->tokens;
+    p.seqs = a->seqs;
+    p.q_heads = a->q_heads;
+    p.group = a->q_heads / cache->kv_heads;
+    p.scale_log2 = a->scale * 1.44269504f;
+    p.status = c->d_status;
+    const int64_t want = (a->tokens * a->q_heads + 3) / 4;
+    return launch_attention(c, what, prompt_rows_kernel, (unsigned)std::min<int64_t>(want, c->sm_count * 16), 128, 0, s, p);
+}
+
+int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
+    ATTENTION_ENTER(ctx);
+    const char* what = "tree_attention";
+    if (!a) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    int rc = check_cache(c, what, cache, layer, false);
+    if (rc == WF_OK) rc = check_queries(c, what, a->q_dev, a->out_dev, a->q_stride, a->tokens, a->seqs, a->q_heads, cache);
+    if (rc != WF_OK) return rc;
+    if (!a->tables_dev || !a->context_dev || (a->tables_dev | a->context_dev | a->q_offsets_dev) & 3 || a->ancestors_dev & 7)
+        return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: tables and context are 4-byte aligned device arrays, ancestors 8-byte aligned", what);
+    if (a->max_drafts < 1 || a->max_drafts > TREE_MAX_DRAFTS) return set_error(c, WF_ERR_TOO_LARGE, "%s: max_drafts %d is not 1 .. %d", what, a->max_drafts, TREE_MAX_DRAFTS);
+    if (!a->q_offsets_dev && a->tokens != (int64_t)a->seqs * a->max_drafts)
+        return set_error(c, WF_ERR_SHAPE, "%s: %lld tokens are not %d for each of %d sequences", what, (long long)a->tokens, a->max_drafts, a->seqs);
+    if (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1 || a->max_context < 0 || a->max_context > (1LL << 31) - 1024)
+        return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld, max_context %lld", what, (long long)a->table_stride, (long long)a->max_context);
+    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
+    TreeParams p{};
+    p.cache = cache_layer(*cache, layer);
+    p.q = reinterpret_cast<const bf16*>(a->q_dev);
+    p.out = reinterpret_cast<bf16*>(a->out_dev);
+    p.q_stride = a->q_stride;
+    p.q_offsets = reinterpret_cast<const int*>(a->q_offsets_dev);
+    p.tables = reinterpret_cast<const int*>(a->tables_dev);
+    p.table_stride = a->table_stride;
+    p.context = reinterpret_cast<const int*>(a->context_dev);
+    p.ancestors = reinterpret_cast<const uint64_t*>(a->ancestors_dev);
+    p.tokens = a->tokens;
+    p.max_context = a->max_context;
+    p.seqs = a->seqs;
+    p.q_heads = a->q_heads;
+    p.group = a->q_heads / cache->kv_heads;
+    p.max_drafts = a->max_drafts;
+    p.scale_log2 = a->scale * 1.44269504f;
+    p.status = c->d_status;
+    const int64_t want = ((int64_t)a->seqs * a->max_drafts * a->q_heads + 3) / 4;
+    return launch_attention(c, what, tree_rows_kernel, (unsigned)std::min<int64_t>(want, c->sm_count * 16), 128, 0, s, p);
+}
+
+}  // extern "C"

@@ -1,0 +1,315 @@
+// The pages of a key/value cache: who holds them (host), copies of pages and the move of kept tokens (device).
+#include <algorithm>
+#include <mutex>
+#include <new>
+#include <queue>
+#include <unordered_set>
+
+#include "wf_attention.cuh"
+
+namespace wf {
+
+CacheView cache_layer(const wf_kv_cache& cache, int layer);
+int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too);
+
+// ---------------------------------------------------------------- who holds which page
+struct PagePool {
+    std::mutex mu;
+    std::vector<int64_t> holders;
+    std::priority_queue<int32_t, std::vector<int32_t>, std::greater<int32_t>> free_ids;  // lowest first: a cache stays dense at its start
+};
+static std::mutex g_pools_mu;
+static std::unordered_set<PagePool*> g_pools;
+
+// The pool stays locked, and in the registry, while `f` works on it.  Nothing may leave a C entry as an exception.
+template <class F> static int with_pool(int64_t handle, F f) {
+    try {
+        std::lock_guard<std::mutex> lk(g_pools_mu);
+        PagePool* p = reinterpret_cast<PagePool*>(handle);
+        if (!p || !g_pools.count(p)) return WF_ERR_INVALID_HANDLE;
+        std::lock_guard<std::mutex> in(p->mu);
+        return f(*p);
+    } catch (const std::bad_alloc&) {
+        return WF_ERR_CUDA_BASE + (int)cudaErrorMemoryAllocation;
+    } catch (...) {
+        return WF_ERR_INVALID_ARGUMENT;
+    }
+}
+
+// ---------------------------------------------------------------- copies
+struct CopyParams {
+    CacheView cache;
+    size_t layer_elements;
+    int layers;
+    const int2* pairs;
+    const int* rows;
+    int64_t n;
+    int* status;
+};
+// A unit is one head of one page in one layer, keys or values: contiguous on both sides.  COPY_DEPTH 16-byte pieces a thread in flight.
+// Bound by HBM.
+constexpr int COPY_THREADS = 256, COPY_DEPTH = 4;
+__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int heads = p.cache.kv_heads, page_tokens = 1 << p.cache.page_shift;
+    const int64_t units = (int64_t)p.layers * 2 * p.n * heads;
+    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
+        const int head = (int)(u % heads);
+        const int64_t i = u / heads % p.n, of = u / heads / p.n;  // keys of layer 0, values of layer 0, keys of layer 1 ..
+        const int2 pair = p.pairs[i];
+        const int rows = p.rows ? p.rows[i] : page_tokens;
+        const bool bad = pair.x < 0 || pair.y < 0 || pair.x >= p.cache.pages || pair.y >= p.cache.pages || rows < 0 || rows > page_tokens;
+        if (bad && threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
+        if (bad || pair.x == pair.y) continue;
+        bf16* base = (of & 1 ? p.cache.values : p.cache.keys) + (size_t)(of >> 1) * p.layer_elements;
+        const uint4* from = reinterpret_cast<const uint4*>(base + p.cache.at(pair.x, head, 0));
+        uint4* to = reinterpret_cast<uint4*>(base + p.cache.at(pair.y, head, 0));
+        const int pieces = rows * p.cache.dim / 8;
+        for (int j0 = threadIdx.x; j0 < pieces; j0 += COPY_DEPTH * COPY_THREADS) {
+            uint4 v[COPY_DEPTH];
+#pragma unroll
+            for (int e = 0; e < COPY_DEPTH; e++)
+                if (j0 + e * COPY_THREADS < pieces) v[e] = from[j0 + e * COPY_THREADS];
+#pragma unroll
+            for (int e = 0; e < COPY_DEPTH; e++)
+                if (j0 + e * COPY_THREADS < pieces) to[j0 + e * COPY_THREADS] = v[e];
+        }
+    }
+}
+
+struct CompactParams {
+    CacheView cache;
+    size_t layer_elements;
+    int layers;
+    const int* tables;
+    int64_t table_stride;
+    const int* context;
+    const int* kept;
+    int64_t kept_stride;
+    const int* counts;
+    int64_t seqs;
+    int* status;
+};
+// A thread has one 16-byte piece of every kept token of a (layer, keys or values, sequence, head) and takes them in order, COMPACT_DEPTH
+// at a time: all loads, then all stores.  kept ascends, so kept[i] >= i and token i is stored to a place that only an earlier
+// token (or itself) came from: no load of a later batch can find it overwritten, and no two threads touch the same piece.
+constexpr int COMPACT_THREADS = 128, COMPACT_DEPTH = 8;
+__global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const __grid_constant__ CompactParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int pieces = p.cache.dim / 8, heads = p.cache.kv_heads, shift = p.cache.page_shift;
+    const int64_t n = (int64_t)p.layers * 2 * p.seqs * heads * pieces;
+    for (int64_t u = (int64_t)blockIdx.x * COMPACT_THREADS + threadIdx.x; u < n; u += (int64_t)gridDim.x * COMPACT_THREADS) {
+        const int piece = (int)(u % pieces), head = (int)(u / pieces % heads);
+        const int64_t s = u / pieces / heads % p.seqs, of = u / pieces / heads / p.seqs;
+        bf16* base = (of & 1 ? p.cache.values : p.cache.keys) + (size_t)(of >> 1) * p.layer_elements;
+        const int* table = p.tables + s * p.table_stride;
+        const int* kept = p.kept + s * p.kept_stride;
+        const int64_t start = p.context[s], most = p.table_stride << shift;
+        const int count = p.counts[s];
+        bool bad = start < 0 || count < 0 || count > p.kept_stride;
+        auto place = [&](int64_t t) -> uint4* {
+            const int64_t page = table[t >> shift];
+            if (page < 0 || page >= p.cache.pages) return nullptr;
+            return reinterpret_cast<uint4*>(base + p.cache.at(page, head, (int)(t & ((1 << shift) - 1)))) + piece;
+        };
+        int before = -1;
+        for (int i0 = 0; i0 < count && !bad; i0 += COMPACT_DEPTH) {
+            uint4 v[COMPACT_DEPTH];
+            uint4* to[COMPACT_DEPTH];
+#pragma unroll
+            for (int e = 0; e < COMPACT_DEPTH; e++) {
+                to[e] = nullptr;
+                if (i0 + e >= count || bad) continue;
+                const int j = kept[i0 + e];
+                if (j <= before || start + j >= most) {
+                    bad = true;
+                    continue;
+                }
+                before = j;
+                if (j == i0 + e) continue;  // where it belongs already
+                const uint4* from = place(start + j);
+                to[e] = place(start + i0 + e);
+                if (!from || !to[e]) {
+                    bad = true;
+                    to[e] = nullptr;
+                    continue;
+                }
+                v[e] = *from;
+            }
+#pragma unroll
+            for (int e = 0; e < COMPACT_DEPTH; e++)
+                if (to[e]) *to[e] = v[e];
+        }
+        if (bad) report_status(p.status, STATUS_BAD_INDEX);
+    }
+}
+
+}  // namespace wf
+
+using namespace wf;
+
+template <class Params> static int launch_cache(Context* c, const char* what, void (*kernel)(Params), int64_t want, unsigned threads, cudaStream_t s, const Params& p) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)c->sm_count * (2048 / threads))));
+    cfg.blockDim = dim3(threads);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    if (e != cudaSuccess) return cuda_status(c, e, what);
+    c->launches++;
+    return WF_OK;
+}
+
+#define CACHE_ENTER(ctxh)                                                  \
+    Context* c = get_context(ctxh);                                        \
+    if (!c) return WF_ERR_INVALID_HANDLE;                                  \
+    ScopedLock _lk(c);                                                     \
+    if (!_lk.ok) return WF_ERR_BUSY;                                       \
+    WF_CUDA(c, cudaSetDevice(c->device));                                  \
+    cudaStream_t s = resolve_stream(c, stream)
+
+extern "C" {
+
+int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev, int64_t rows_dev, int64_t n, int64_t stream) {
+    CACHE_ENTER(ctx);
+    const char* what = "cache_copy_pages";
+    const int rc = check_kv_cache(c, what, cache, 0, false);
+    if (rc != WF_OK) return rc;
+    if (n < 0 || n > (1LL << 31) - 1) return set_error(c, WF_ERR_SHAPE, "%s: %lld pairs", what, (long long)n);
+    if (n == 0) return WF_OK;
+    if (!pairs_dev || pairs_dev & 7 || rows_dev & 3) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: pairs is an 8-byte aligned device array, rows a 4-byte aligned one", what);
+    CopyParams p{};
+    p.cache = cache_layer(*cache, 0);
+    p.layer_elements = (size_t)cache->pages * cache->kv_heads * cache->page_tokens * cache->head_dim;
+    p.layers = cache->layers;
+    p.pairs = reinterpret_cast<const int2*>(pairs_dev);
+    p.rows = reinterpret_cast<const int*>(rows_dev);
+    p.n = n;
+    p.status = c->d_status;
+    return launch_cache(c, what, copy_pages_kernel, (int64_t)cache->layers * 2 * n * cache->kv_heads, COPY_THREADS, s, p);
+}
+
+int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, int64_t table_stride, int64_t context_dev, int64_t kept_dev, int64_t kept_stride,
+                     int64_t counts_dev, int64_t seqs, int64_t stream) {
+    CACHE_ENTER(ctx);
+    const char* what = "cache_compact";
+    const int rc = check_kv_cache(c, what, cache, 0, false);
+    if (rc != WF_OK) return rc;
+    if (seqs < 0 || seqs > (1LL << 31) - 1 || kept_stride < 0 || kept_stride > (1LL << 31) - 1 || table_stride < 1 || table_stride > (1LL << 31) / cache->page_tokens - 1)
+        return set_error(c, WF_ERR_SHAPE, "%s: seqs=%lld kept_stride=%lld table_stride=%lld", what, (long long)seqs, (long long)kept_stride, (long long)table_stride);
+    if (seqs == 0 || kept_stride == 0) return WF_OK;
+    if (!tables_dev || !context_dev || !kept_dev || !counts_dev || (tables_dev | context_dev | kept_dev | counts_dev) & 3)
+        return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: tables, context, kept and counts are 4-byte aligned device arrays", what);
+    CompactParams p{};
+    p.cache = cache_layer(*cache, 0);
+    p.layer_elements = (size_t)cache->pages * cache->kv_heads * cache->page_tokens * cache->head_dim;
+    p.layers = cache->layers;
+    p.tables = reinterpret_cast<const int*>(tables_dev);
+    p.table_stride = table_stride;
+    p.context = reinterpret_cast<const int*>(context_dev);
+    p.kept = reinterpret_cast<const int*>(kept_dev);
+    p.kept_stride = kept_stride;
+    p.counts = reinterpret_cast<const int*>(counts_dev);
+    p.seqs = seqs;
+    p.status = c->d_status;
+    const int64_t threads = (int64_t)cache->layers * 2 * seqs * cache->kv_heads * (cache->head_dim / 8);
+    return launch_cache(c, what, compact_kernel, (threads + COMPACT_THREADS - 1) / COMPACT_THREADS, COMPACT_THREADS, s, p);
+}
+
+int wf_pages_create(int64_t pages, int64_t* pool) {
+    if (!pool) return WF_ERR_INVALID_ARGUMENT;
+    *pool = 0;
+    if (pages < 0 || pages > (1LL << 31) - 1) return WF_ERR_SHAPE;
+    try {
+        std::unique_ptr<PagePool> p(new PagePool);
+        p->holders.assign((size_t)pages, 0);
+        std::vector<int32_t> ids((size_t)pages);
+        for (int64_t i = 0; i < pages; i++) ids[(size_t)i] = (int32_t)i;
+        p->free_ids = decltype(p->free_ids)(std::greater<int32_t>(), std::move(ids));
+        std::lock_guard<std::mutex> lk(g_pools_mu);
+        g_pools.insert(p.get());
+        *pool = reinterpret_cast<int64_t>(p.release());
+        return WF_OK;
+    } catch (...) {
+        return WF_ERR_CUDA_BASE + (int)cudaErrorMemoryAllocation;
+    }
+}
+
+int wf_pages_destroy(int64_t pool) {
+    PagePool* p = reinterpret_cast<PagePool*>(pool);
+    std::lock_guard<std::mutex> lk(g_pools_mu);
+    if (!p || !g_pools.erase(p)) return WF_ERR_INVALID_HANDLE;
+    delete p;
+    return WF_OK;
+}
+
+int wf_pages_take(int64_t pool, int64_t n, int32_t* ids) {
+    return with_pool(pool, [&](PagePool& p) {
+        if (n < 0 || (n > 0 && !ids)) return WF_ERR_INVALID_ARGUMENT;
+        if (n > (int64_t)p.free_ids.size()) return WF_ERR_TOO_LARGE;
+        for (int64_t i = 0; i < n; i++) {
+            ids[i] = p.free_ids.top();
+            p.free_ids.pop();
+            p.holders[(size_t)ids[i]] = 1;
+        }
+        return WF_OK;
+    });
+}
+
+int wf_pages_share(int64_t pool, int64_t n, const int32_t* ids) {
+    return with_pool(pool, [&](PagePool& p) {
+        if (n < 0 || (n > 0 && !ids)) return WF_ERR_INVALID_ARGUMENT;
+        for (int64_t i = 0; i < n; i++)
+            if (ids[i] < 0 || (size_t)ids[i] >= p.holders.size() || p.holders[(size_t)ids[i]] < 1) return WF_ERR_INDEX;
+        for (int64_t i = 0; i < n; i++) p.holders[(size_t)ids[i]]++;
+        return WF_OK;
+    });
+}
+
+int wf_pages_release(int64_t pool, int64_t n, const int32_t* ids) {
+    return with_pool(pool, [&](PagePool& p) {
+        if (n < 0 || (n > 0 && !ids)) return WF_ERR_INVALID_ARGUMENT;
+        int64_t done = 0;
+        for (; done < n; done++) {
+            if (ids[done] < 0 || (size_t)ids[done] >= p.holders.size() || p.holders[(size_t)ids[done]] < 1) break;
+            p.holders[(size_t)ids[done]]--;
+        }
+        if (done < n) {  // nothing is changed
+            while (done-- > 0) p.holders[(size_t)ids[done]]++;
+            return WF_ERR_INDEX;
+        }
+        for (int64_t i = 0; i < n; i++)
+            if (p.holders[(size_t)ids[i]] == 0) {
+                p.holders[(size_t)ids[i]] = -1;  // named twice: freed once
+                p.free_ids.push(ids[i]);
+            }
+        for (int64_t i = 0; i < n; i++)
+            if (p.holders[(size_t)ids[i]] < 0) p.holders[(size_t)ids[i]] = 0;
+        return WF_OK;
+    });
+}
+
+int wf_pages_info(int64_t pool, int64_t* pages, int64_t* free_pages) {
+    return with_pool(pool, [&](PagePool& p) {
+        if (pages) *pages = (int64_t)p.holders.size();
+        if (free_pages) *free_pages = (int64_t)p.free_ids.size();
+        return WF_OK;
+    });
+}
+
+int wf_pages_holders(int64_t pool, int32_t id, int64_t* holders) {
+    return with_pool(pool, [&](PagePool& p) {
+        if (!holders) return WF_ERR_INVALID_ARGUMENT;
+        if (id < 0 || (size_t)id >= p.holders.size()) return WF_ERR_INDEX;
+        *holders = p.holders[(size_t)id];
+        return WF_OK;
+    });
+}
+
+}  // extern "C"
