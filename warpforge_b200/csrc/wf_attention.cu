@@ -1,26 +1,12 @@
 // Attention over a paged cache: wf_prompt_attention and wf_tree_attention.
 //   out = softmax(scale q k^T) v   over the keys that a row sees, with base-2 exponentials: softmax(x) = 2^(x log2 e - m) / sum
-#include "wf_attention.cuh"
+#include <algorithm>
+#include <atomic>
+
+#include "wf_attention_prompt.cuh"
 
 namespace wf {
 
-// A warp per row and head, key by key.
-__global__ void __launch_bounds__(128) prompt_rows_kernel(const __grid_constant__ PromptParams p) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t n = p.tokens * p.q_heads;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); i < n; i += (int64_t)gridDim.x * 4) {
-        const int row = (int)(i / p.q_heads), head = (int)(i % p.q_heads);
-        int s = 0;
-        while (s < p.seqs && !(row >= p.q_offsets[s] && row < p.q_offsets[s + 1])) s++;
-        if (s == p.seqs) continue;
-        const PromptSeq q = prompt_seq(p, s);
-        if (row >= q.row0 + q.rows) continue;
-        const int last = q.keys - q.rows + (row - q.row0);
-        attend_row(p.cache, q.place, p.q + (size_t)row * p.q_stride + (size_t)head * p.cache.dim, p.out + ((size_t)row * p.q_heads + head) * p.cache.dim,
-                   head / p.group, min(q.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
-    }
-}
 __global__ void __launch_bounds__(128) tree_rows_kernel(const __grid_constant__ TreeParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
@@ -77,8 +63,8 @@ static int check_queries(Context* c, const char* what, int64_t q, int64_t out, i
     if (q_stride < (int64_t)q_heads * cache->head_dim || q_stride % 8) return set_error(c, WF_ERR_SHAPE, "%s: q_stride %lld", what, (long long)q_stride);
     return WF_OK;
 }
-template <class Params>
-static int launch_attention(Context* c, const char* what, void (*kernel)(Params), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const Params& p) {
+template <class... Params, class... Args>
+static int launch_attention(Context* c, const char* what, void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = dim3(grid);
     cfg.blockDim = dim3(threads);
@@ -89,10 +75,57 @@ static int launch_attention(Context* c, const char* what, void (*kernel)(Params)
     attr[0].val.programmaticStreamSerializationAllowed = 1;
     cfg.attrs = attr;
     cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) return cuda_status(c, e, what);
     c->launches++;
     return WF_OK;
+}
+
+// bf16 [z][y][x] with the given distances (elements) between y and z; boxes of 64 elements x by x bz, 128-byte swizzle, zeros outside
+static int encode_rows(Context* c, CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z, int64_t y_apart, int64_t z_apart, int by, int bz) {
+    const cuuint64_t dims[3] = {(cuuint64_t)x, (cuuint64_t)y, (cuuint64_t)z}, strides[2] = {(cuuint64_t)y_apart * 2, (cuuint64_t)z_apart * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)by, (cuuint32_t)bz}, step[3] = {1, 1, 1};
+    const EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return set_error(c, WF_ERR_NO_DEVICE, "the driver has no cuTensorMapEncodeTiled");
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(c, WF_ERR_CUDA_BASE + (int)cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed: %d", (int)r);
+    return WF_OK;
+}
+static int encode_cache(Context* c, CUtensorMap* map, const bf16* base, const CacheView& v, int box_rows) {
+    if (v.page_shift == 0) return encode_rows(c, map, base, v.dim, v.kv_heads, v.pages, v.dim, (int64_t)v.kv_heads * v.dim, 1, box_rows);
+    return encode_rows(c, map, base, v.dim, 1, (v.pages * v.kv_heads) << v.page_shift, v.dim, v.dim, 1, box_rows);
+}
+static int dim_chunks(int dim) { return (dim + 63) / 64; }
+
+template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p, cudaStream_t s) {
+    const char* what = "prompt_attention";
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    GemvScratch& scratch = c->gemv_scratch[s];
+    if (!scratch.d_attn_sched) {
+        const int rc = refuse_allocation_while_recording(c, s, "the counters of prompt_attention");
+        if (rc != WF_OK) return rc;
+        std::shared_ptr<unsigned int> sched;
+        WF_CUDA(c, make_shared_device(c, sched, 2 * sizeof(unsigned int)));
+        WF_CUDA(c, cudaMemsetAsync(sched.get(), 0, 2 * sizeof(unsigned int), s));
+        scratch.d_attn_sched = sched;
+    }
+    PromptTiles t{};
+    t.p = p;
+    t.tile_tokens = PA_ROWS / p.group;
+    t.box_rows = p.tables ? std::min(PA_KEYS, 1 << p.cache.page_shift) : PA_KEYS;
+    t.sched = scratch.d_attn_sched.get();
+    CUtensorMap q, k, v;
+    int rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
+    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
+    if (rc != WF_OK) return rc;
+    const int64_t items = (p.tokens / (2 * t.tile_tokens) + p.seqs) * p.cache.kv_heads;
+    return launch_attention(c, what, prompt_tiles_kernel<CHUNKS>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
 
 #define ATTENTION_ENTER(ctxh)                                              \
@@ -119,7 +152,9 @@ int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf
         return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: pages need tables and k_lens, packed keys take neither", what);
     if (!packed && (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1))
         return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld", what, (long long)a->table_stride);
+    if (!(a->scale > 0.f) || a->scale > 1e30f) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: scale %g", what, (double)a->scale);
     if (a->tokens == 0 || a->seqs == 0) return WF_OK;
+    if (cache->pages < 1) return set_error(c, WF_ERR_SHAPE, "%s: a cache without pages", what);
     PromptParams p{};
     p.cache = cache_layer(*cache, layer);
     p.q = reinterpret_cast<const bf16*>(a->q_dev);
@@ -135,8 +170,7 @@ int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf
     p.group = a->q_heads / cache->kv_heads;
     p.scale_log2 = a->scale * 1.44269504f;
     p.status = c->d_status;
-    const int64_t want = (a->tokens * a->q_heads + 3) / 4;
-    return launch_attention(c, what, prompt_rows_kernel, (unsigned)std::min<int64_t>(want, c->sm_count * 16), 128, 0, s, p);
+    return dim_chunks(cache->head_dim) == 1 ? launch_prompt<1>(c, p, s) : launch_prompt<2>(c, p, s);
 }
 
 int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
@@ -153,7 +187,9 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
         return set_error(c, WF_ERR_SHAPE, "%s: %lld tokens are not %d for each of %d sequences", what, (long long)a->tokens, a->max_drafts, a->seqs);
     if (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1 || a->max_context < 0 || a->max_context > (1LL << 31) - 1024)
         return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld, max_context %lld", what, (long long)a->table_stride, (long long)a->max_context);
+    if (!(a->scale > 0.f) || a->scale > 1e30f) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: scale %g", what, (double)a->scale);
     if (a->tokens == 0 || a->seqs == 0) return WF_OK;
+    if (cache->pages < 1) return set_error(c, WF_ERR_SHAPE, "%s: a cache without pages", what);
     TreeParams p{};
     p.cache = cache_layer(*cache, layer);
     p.q = reinterpret_cast<const bf16*>(a->q_dev);

@@ -1,0 +1,602 @@
+// Attention over whole prompts on the 5th-generation tensor cores.
+//
+//   S = Q K^T   [128 rows x 128 keys] fp32 in TMEM, Q and K in shared memory
+//   P = 2^(S scale log2 e - m)        bf16, written over S in TMEM
+//   O += P V    [128 rows x dim] fp32 in TMEM, P in TMEM, V in shared memory
+//
+// A CTA works on two tiles of rows of one kv head at a time, so that the tensor core has the one tile's products to do while the other
+// tile's exponentials are taken.  The rows of a tile are the heads of the group for some tokens, token by token: keys and values are read once
+// for the whole group.  A thread of the softmax warps has a row: its maximum and sum need no exchange.
+#pragma once
+#include "wf_attention.cuh"
+#include "wf_gemm_core.cuh"
+
+namespace wf {
+
+constexpr int PA_ROWS = 128, PA_KEYS = 128;  // of a tile
+constexpr int PA_SOFTMAX_WARPS = 8;          // four a tile
+constexpr int PA_LOAD_WARP = 8, PA_MMA_WARP = 9, PA_SCHED_WARP = 10;  // and one that has nothing to do: setmaxnreg wants four
+constexpr int PA_THREADS = 12 * 32;
+// Registers: 168 a thread at launch; the softmax warps, which hold a row of S, take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int PA_SOFTMAX_REGS = 216, PA_OTHER_REGS = 72;
+constexpr int PA_CHUNK = PA_KEYS * 128;      // bytes of 128 rows x 64 elements
+constexpr int PA_ITEMS = 2;                  // items announced ahead
+constexpr float PA_RESCALE = 8.f;            // the running maximum is followed when it has grown by this many powers of two
+constexpr int PA_MAX_STAGES = 12;
+template <int CHUNKS> struct PromptShape {  // by the head's dimension in 64 elements, rounded up
+    static constexpr int STAGES = CHUNKS == 2 ? 5 : 12, STAGE_BYTES = CHUNKS * PA_CHUNK, Q_BYTES = 2 * CHUNKS * PA_CHUNK;
+    static constexpr int SMEM = Q_BYTES + STAGES * STAGE_BYTES + 1024;
+};
+
+// Two tiles of rows of one sequence and kv head.
+struct PromptItem {
+    int seq, head;
+    int row0, rows, keys;  // of the sequence
+    int token0;            // first token of tile 0
+    int n0, n1;            // key tiles that the tiles see
+    int last;              // no more work (1), or a wait ran out
+};
+
+struct PromptTiles {
+    PromptParams p;
+    int tile_tokens;   // tokens of a tile: 128 / group
+    int box_rows;      // rows of keys that one TMA load brings: those of a page, at most 128
+    unsigned int* sched;  // [0] items taken beyond the first of each CTA, [1] CTAs that are done
+};
+
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, void* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+                 "r"(y), "r"(z), "r"(g_smem_u32(bar))
+                 : "memory");
+}
+// Operand of 16-bit elements with the other dimension contiguous (V: a row is a key, its elements run along N), 128-byte swizzle: 64 elements x 8
+// rows are 1024 bytes, the next 8 rows follow, the next 64 elements lie `chunk` bytes on.
+__device__ __forceinline__ uint64_t smem_desc_sw128_n(uint32_t saddr, uint32_t chunk) {
+    return (uint64_t)((saddr & 0x3FFFF) >> 4) | (uint64_t)(chunk >> 4) << 16 | (uint64_t)(1024 >> 4) << 32 | (uint64_t)1 << 46 | (uint64_t)2 << 61;
+}
+// Four MMAs over 64 elements of the heads: both operands in shared memory, 32 bytes apart in the swizzled rows.
+__device__ __forceinline__ void pa_mma_qk(uint32_t d, uint64_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred p, e, t;\n\t.reg .b64 a1, a2, a3, b1, b2, b3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "add.s64 a1, %1, 2;\n\tadd.s64 a2, %1, 4;\n\tadd.s64 a3, %1, 6;\n\t"
+        "add.s64 b1, %2, 2;\n\tadd.s64 b2, %2, 4;\n\tadd.s64 b3, %2, 6;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], %1, %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a1, b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a2, b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], a3, b3, %3, t;\n\t}" ::"r"(d),
+        "l"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(issue)
+        : "memory");
+}
+// Four MMAs over 64 keys: weights in TMEM, eight columns each; values 16 rows (2048 bytes) apart.
+__device__ __forceinline__ void pa_mma_pv(uint32_t d, uint32_t a, uint64_t b, uint32_t idesc, uint32_t accumulate, uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred p, e, t;\n\t.reg .b32 a1, a2, a3;\n\t.reg .b64 b1, b2, b3;\n\t"
+        "setp.ne.b32 p, %4, 0;\n\tsetp.ne.b32 e, %5, 0;\n\tsetp.eq.b32 t, 0, 0;\n\t"
+        "add.s32 a1, %1, 8;\n\tadd.s32 a2, %1, 16;\n\tadd.s32 a3, %1, 24;\n\t"
+        "add.s64 b1, %2, 128;\n\tadd.s64 b2, %2, 256;\n\tadd.s64 b3, %2, 384;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [%1], %2, %3, p;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a1], b1, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a2], b2, %3, t;\n\t"
+        "@e tcgen05.mma.cta_group::1.kind::f16 [%0], [a3], b3, %3, t;\n\t}" ::"r"(d),
+        "r"(a), "l"(b), "r"(idesc), "r"(accumulate), "r"(issue)
+        : "memory");
+}
+__device__ __forceinline__ void tc_commit_if(void* bar, uint32_t issue) {
+    asm volatile(
+        "{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %1, 0;\n\t"
+        "@e tcgen05.commit.cta_group::1.mbarrier::arrive::one.shared::cluster.b64 [%0];\n\t}" ::"r"(g_smem_u32(bar)),
+        "r"(issue)
+        : "memory");
+}
+// 32 columns of this warp's 32 lanes, without the wait
+__device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t* r) {
+    asm volatile(
+        "tcgen05.ld.sync.aligned.32x32b.x32.b32 "
+        "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31}, [%32];"
+        : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]),
+          "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15]), "=r"(r[16]), "=r"(r[17]), "=r"(r[18]),
+          "=r"(r[19]), "=r"(r[20]), "=r"(r[21]), "=r"(r[22]), "=r"(r[23]), "=r"(r[24]), "=r"(r[25]), "=r"(r[26]), "=r"(r[27]),
+          "=r"(r[28]), "=r"(r[29]), "=r"(r[30]), "=r"(r[31])
+        : "r"(taddr)
+        : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+__device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
+    asm volatile(
+        "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
+        "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16,%17,%18,%19,%20,%21,%22,%23,%24,%25,%26,%27,%28,%29,%30,%31,%32};" ::"r"(taddr),
+        "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]), "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]),
+        "r"(r[13]), "r"(r[14]), "r"(r[15]), "r"(r[16]), "r"(r[17]), "r"(r[18]), "r"(r[19]), "r"(r[20]), "r"(r[21]), "r"(r[22]), "r"(r[23]), "r"(r[24]),
+        "r"(r[25]), "r"(r[26]), "r"(r[27]), "r"(r[28]), "r"(r[29]), "r"(r[30]), "r"(r[31])
+        : "memory");
+}
+__device__ __forceinline__ float ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+__device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
+    return d;
+}
+__device__ __forceinline__ float2 add2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
+
+// Waits for a barrier, the whole warp with one answer.
+__device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, g_mbar_wait(bar, parity)); }
+
+struct PromptShared {
+    uint64_t q_full[2], q_empty[2];
+    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t kv_full[PA_MAX_STAGES], kv_empty[PA_MAX_STAGES];
+    uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
+    PromptItem items[PA_ITEMS];
+    int bad_page;  // an item of this number and before has pages outside the cache
+    uint32_t tmem;
+};
+
+// The next item of the ring; false: no more, or a wait ran out.
+struct ItemCursor {
+    int slot = 0;
+    uint32_t phase = 0;
+    __device__ __forceinline__ bool next(PromptShared* sh, PromptItem& it, bool& failed) {
+        if (!pa_wait(&sh->item_full[slot], phase)) {
+            failed = true;
+            return false;
+        }
+        it = sh->items[slot];
+        __syncwarp();
+        if ((threadIdx.x & 31) == 0) g_mbar_arrive(&sh->item_empty[slot]);
+        if (++slot == PA_ITEMS) slot = 0, phase ^= 1;
+        return it.last == 0;
+    }
+};
+
+// Which items there are, the longest first: tiles of a sequence count from where its past ends, v = block + past / block tokens, and v goes down
+// over all sequences at once.  Every lane has every 32nd sequence.
+struct PromptSchedule {
+    const PromptTiles& t;
+    int block;       // tokens of an item
+    int v;           // where the cursor is
+    int64_t before;  // items with a larger v
+    int count;       // sequences that have this v
+    __device__ __forceinline__ void span(int s, int& lo, int& hi) const {  // a sequence's v: [lo, hi)
+        const PromptSeq q = prompt_seq(t.p, s);
+        const int past = max(0, q.keys - q.rows);
+        lo = past / block;
+        hi = lo + (q.rows + block - 1) / block;
+    }
+    __device__ __forceinline__ int have(int value) const {
+        int n = 0;
+        for (int s0 = 0; s0 < t.p.seqs; s0 += 32) {
+            int lo = 0, hi = 0;
+            if (s0 + (int)(threadIdx.x & 31) < t.p.seqs) span(s0 + (threadIdx.x & 31), lo, hi);
+            n += __popc(__ballot_sync(0xFFFFFFFFu, value >= lo && value < hi));
+        }
+        return n;
+    }
+    __device__ __forceinline__ void begin() {
+        block = 2 * t.tile_tokens;
+        int top = 0;
+        for (int s = threadIdx.x & 31; s < t.p.seqs; s += 32) {
+            int lo, hi;
+            span(s, lo, hi);
+            top = max(top, hi);
+        }
+        v = __reduce_max_sync(0xFFFFFFFFu, top) - 1;
+        before = 0;
+        count = v >= 0 ? have(v) : 0;
+    }
+    // item i (they come in ascending order); false: there is none
+    __device__ __forceinline__ bool find(int64_t i, PromptItem& it) {
+        const int heads = t.p.cache.kv_heads;
+        while (v >= 0 && i >= before + (int64_t)count * heads) {
+            before += (int64_t)count * heads;
+            if (--v >= 0) count = have(v);
+        }
+        if (v < 0) return false;
+        int nth = (int)((i - before) / heads);
+        it.head = (int)((i - before) % heads);
+        for (int s0 = 0; s0 < t.p.seqs; s0 += 32) {
+            int lo = 0, hi = 0;
+            if (s0 + (int)(threadIdx.x & 31) < t.p.seqs) span(s0 + (threadIdx.x & 31), lo, hi);
+            uint32_t with = __ballot_sync(0xFFFFFFFFu, v >= lo && v < hi);
+            const int n = __popc(with);
+            if (nth >= n) {
+                nth -= n;
+                continue;
+            }
+            for (; nth > 0; nth--) with &= with - 1;
+            const int lane = __ffs(with) - 1;
+            it.seq = s0 + lane;
+            lo = __shfl_sync(0xFFFFFFFFu, lo, lane);
+            break;
+        }
+        const PromptSeq q = prompt_seq(t.p, it.seq);
+        it.row0 = q.row0;
+        it.rows = q.rows;
+        it.keys = q.keys;
+        it.token0 = (v - max(0, q.keys - q.rows) / block) * block;
+        auto tiles = [&](int token) {  // key tiles that a tile of rows starting at this token sees
+            if (token >= q.rows) return 0;
+            const int last = q.keys - q.rows + min(q.rows, token + t.tile_tokens) - 1;
+            return last < 0 ? 0 : last / PA_KEYS + 1;
+        };
+        it.n0 = tiles(it.token0);
+        it.n1 = tiles(it.token0 + t.tile_tokens);
+        it.last = 0;
+        return true;
+    }
+};
+
+template <int CHUNKS>
+__global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __grid_constant__ PromptTiles t, const __grid_constant__ CUtensorMap q_map,
+                                                                    const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    constexpr int DIM = CHUNKS * 64, STAGES = PromptShape<CHUNKS>::STAGES, STAGE_BYTES = PromptShape<CHUNKS>::STAGE_BYTES;
+    constexpr uint32_t IDESC = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(PA_ROWS / 16) << 24;  // fp32 += bf16 x bf16, 128 rows
+    constexpr uint32_t IDESC_QK = IDESC | (uint32_t)(PA_KEYS / 8) << 17, IDESC_PV = IDESC | 1u << 16 | (uint32_t)(DIM / 8) << 17;
+    constexpr uint32_t O_COLUMN = 2 * PA_KEYS;  // TMEM: S of tile 0, S of tile 1, O of tile 0, O of tile 1
+    extern __shared__ uint8_t raw[];
+    __shared__ PromptShared sh_;
+    PromptShared* const sh = &sh_;
+    const uint32_t smem = (g_smem_u32(raw) + 1023u) & ~1023u, kv_smem = smem + PromptShape<CHUNKS>::Q_BYTES;
+    const PromptParams& p = t.p;
+    const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
+    if (warp == PA_LOAD_WARP && lane == 0) {
+        for (int g = 0; g < 2; g++) {
+            g_mbar_init(&sh->q_full[g], 1);
+            g_mbar_init(&sh->q_empty[g], 1);
+            g_mbar_init(&sh->s_full[g], 1);
+            g_mbar_init(&sh->p_full[g], 4);
+            g_mbar_init(&sh->o_full[g], 1);
+        }
+        for (int i = 0; i < STAGES; i++) {
+            g_mbar_init(&sh->kv_full[i], 1);
+            g_mbar_init(&sh->kv_empty[i], 1);
+        }
+        for (int i = 0; i < PA_ITEMS; i++) {
+            g_mbar_init(&sh->item_full[i], 1);
+            g_mbar_init(&sh->item_empty[i], PA_SOFTMAX_WARPS + 2);
+        }
+        sh->bad_page = -1;
+        asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+        prefetch_tensormap(&q_map);
+        prefetch_tensormap(&k_map);
+        prefetch_tensormap(&v_map);
+    }
+    if (warp == PA_MMA_WARP) tmem_alloc(&sh->tmem, 512);
+    tc_fence_before();
+    __syncthreads();
+    tc_fence_after();
+    const uint32_t tmem = sh->tmem;
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+
+    bool failed = false;
+    PromptItem it;
+    ItemCursor items;
+    if (warp < PA_SOFTMAX_WARPS) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(PA_SOFTMAX_REGS));
+    else asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(PA_OTHER_REGS));
+    if (warp < PA_SOFTMAX_WARPS) {
+        const int g = warp >> 2, r = (warp & 3) * 32 + lane;  // the tile, the row of it
+        const uint32_t lanes = (uint32_t)((warp & 3) * 32) << 16, s_at = tmem + lanes + (uint32_t)(g * PA_KEYS), o_at = tmem + lanes + O_COLUMN + (uint32_t)(g * DIM);
+        const int group = p.group, tile_tokens = t.tile_tokens;
+        const int my_token = r / group, my_head = r % group;
+        const float scale = p.scale_log2;
+        uint32_t s_phase = 0, o_phase = 0;
+        for (int number = 0; items.next(sh, it, failed); number++) {
+            const int n = g ? it.n1 : it.n0, first = it.token0 + g * tile_tokens, token = first + my_token;
+            const bool mine = r < group * tile_tokens && token < it.rows;
+            const int last_key = it.keys - it.rows + token;  // that the row sees
+            const int all_see = it.keys - it.rows + first + (warp & 3) * 32 / group;  // that every row of this warp sees
+            float m = -INFINITY, l = 0.f;
+            for (int j = 0; j < n; j++) {
+                if (!pa_wait(&sh->s_full[g], s_phase)) {
+                    failed = true;
+                    break;
+                }
+                s_phase ^= 1;
+                tc_fence_after();
+                uint32_t s[PA_KEYS];
+#pragma unroll
+                for (int c = 0; c < 4; c++) tmem_ld32_start(s_at + 32 * c, s + 32 * c);
+                tmem_wait_ld();
+                if (j * PA_KEYS + PA_KEYS - 1 > all_see) {  // keys that some row of the warp does not see
+                    const int limit = last_key - j * PA_KEYS;
+#pragma unroll
+                    for (int i = 0; i < PA_KEYS; i++)
+                        if (i > limit) s[i] = 0xFF800000u;
+                }
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+                for (int i = 0; i < PA_KEYS; i += 8)
+#pragma unroll
+                    for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[i + 2 * e])), __uint_as_float(s[i + 2 * e + 1]));
+                const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                if (j == 0) {
+                    m = tile_top;
+                } else if (__any_sync(0xFFFFFFFFu, (tile_top - m) * scale > PA_RESCALE)) {
+                    // O is at rest: the MMAs that made it ran before those that made S
+                    const float grown = fmaxf(m, tile_top), ref = grown == -INFINITY ? 0.f : grown;
+                    const float keep = ex2((m - ref) * scale);
+                    m = grown;
+                    l *= keep;
+#pragma unroll
+                    for (int c = 0; c < DIM; c += 32) {
+                        uint32_t o[32];
+                        tmem_ld32_start(o_at + c, o);
+                        tmem_wait_ld();
+#pragma unroll
+                        for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
+                        tmem_st32(o_at + c, o);
+                    }
+                }
+                const float ref = m == -INFINITY ? 0.f : m * scale;
+                const float2 sc = make_float2(scale, scale), off = make_float2(-ref, -ref);
+                float2 sum[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+                uint32_t w[32];
+#pragma unroll
+                for (int h = 0; h < 2; h++) {
+#pragma unroll
+                    for (int i = 0; i < 32; i++) {
+                        const int k = 64 * h + 2 * i;
+                        float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sc, off);
+                        x.x = ex2(x.x);
+                        x.y = ex2(x.y);
+                        sum[i & 1] = add2(sum[i & 1], x);
+                        w[i] = pack_bf16(x.x, x.y);
+                    }
+                    tmem_st32(s_at + 32 * h, w);
+                }
+                const float2 both = add2(sum[0], sum[1]);
+                l += both.x + both.y;
+                tmem_wait_st();
+                tc_fence_before();
+                if (lane == 0) g_mbar_arrive(&sh->p_full[g]);
+            }
+            if (failed) break;
+            const int row = it.row0 + token, head = it.head * group + my_head;
+            bf16* const to = p.out + ((size_t)row * p.q_heads + head) * p.cache.dim;
+            const int d = p.cache.dim;
+            bool odd = false;  // something is not finite
+            if (n > 0) {
+                if (!pa_wait(&sh->o_full[g], o_phase)) {
+                    failed = true;
+                    break;
+                }
+                o_phase ^= 1;
+                tc_fence_after();
+                const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+                odd = !(l < INFINITY);
+#pragma unroll
+                for (int c = 0; c < DIM; c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_start(o_at + c, o);
+                    tmem_wait_ld();
+                    uint32_t largest = 0;
+#pragma unroll
+                    for (int i = 0; i < 32; i++) largest = max(largest, o[i] & 0x7FFFFFFFu);
+                    odd |= largest >= 0x7F800000u;
+#pragma unroll
+                    for (int i = 0; i < 32; i += 8) {
+                        uint4 v;
+                        v.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
+                        v.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
+                        v.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
+                        v.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
+                        if (mine && c + i < d) *reinterpret_cast<uint4*>(to + c + i) = v;
+                    }
+                }
+                tc_fence_before();
+            } else if (mine) {
+                for (int i = 0; i < d; i += 8) *reinterpret_cast<uint4*>(to + i) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            // Rows with an Inf or a NaN in their sums, and rows whose pages are not in the cache, go key by key: the first may have
+            // come from a key that the row does not see (0 x Inf), the second's keys were not read.
+            odd |= *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
+            uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && odd);
+            while (again) {
+                const int l2 = __ffs(again) - 1;
+                again &= again - 1;
+                const int tok = __shfl_sync(0xFFFFFFFFu, token, l2), hd = __shfl_sync(0xFFFFFFFFu, head, l2), last = it.keys - it.rows + tok;
+                KeyPlace place;
+                place.table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
+                place.first = it.row0;
+                attend_row(p.cache, place, p.q + (size_t)(it.row0 + tok) * p.q_stride + (size_t)hd * d, p.out + ((size_t)(it.row0 + tok) * p.q_heads + hd) * d,
+                           it.head, min(it.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
+            }
+        }
+    } else if (warp == PA_LOAD_WARP) {
+        StageCursor ring;
+        uint32_t q_phase[2] = {1, 1};
+        for (int number = 0; items.next(sh, it, failed); number++) {
+            const int n = max(it.n0, it.n1);
+            const int* table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
+            const int boxes = PA_KEYS / t.box_rows;
+            for (int j = 0; j < n && !failed; j++) {
+                // the rows of this tile's boxes, a lane each
+                int z = it.row0 + j * PA_KEYS, valid = 1;
+                const int y = table ? 0 : it.head;
+                if (table) {
+                    const int key = j * PA_KEYS + lane * t.box_rows;
+                    valid = 0;
+                    if (lane < boxes && key < it.keys) {
+                        int page = table[key >> p.cache.page_shift];
+                        if (page < 0 || page >= p.cache.pages) {  // never followed: these rows go key by key
+                            report_status(p.status, STATUS_BAD_INDEX);
+                            *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                            page = 0;
+                        }
+                        z = (int)((((int64_t)page * p.cache.kv_heads + it.head) << p.cache.page_shift) + (key & ((1 << p.cache.page_shift) - 1)));
+                        valid = 1;
+                    }
+                } else if (lane > 0) valid = 0;
+                const int loads = __popc(__ballot_sync(0xFFFFFFFFu, valid));
+                if (j == 0)
+                    for (int g = 0; g < 2; g++) {
+                        if ((g ? it.n1 : it.n0) == 0) continue;
+                        if (!pa_wait(&sh->q_empty[g], q_phase[g])) failed = true;
+                        q_phase[g] ^= 1;
+                        if (failed) break;
+                        if (lane == 0) {
+                            g_mbar_expect_tx(&sh->q_full[g], (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens));
+                            for (int c = 0; c < CHUNKS; c++)
+                                tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, it.row0 + it.token0 + g * t.tile_tokens, &sh->q_full[g]);
+                        }
+                        __syncwarp();
+                    }
+                for (int kv = 0; kv < 2 && !failed; kv++) {
+                    if (!pa_wait(&sh->kv_empty[ring.s], ring.phase ^ 1)) {
+                        failed = true;
+                        break;
+                    }
+                    if (lane == 0) g_mbar_expect_tx(&sh->kv_full[ring.s], (uint32_t)(loads * CHUNKS * 128 * t.box_rows));
+                    __syncwarp();
+                    if (valid)
+                        for (int c = 0; c < CHUNKS; c++)
+                            tma_load_3d(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + lane * t.box_rows * 128), kv ? &v_map : &k_map, 64 * c, y, z, &sh->kv_full[ring.s]);
+                    ring.advance(STAGES);
+                }
+            }
+            if (failed) break;
+        }
+    } else if (warp == PA_MMA_WARP) {
+        const uint32_t issue = elect_one();
+        StageCursor ring;
+        uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
+        auto after = [](StageCursor c) {
+            c.advance(STAGES);
+            return c;
+        };
+        auto scores = [&](int g, int stage) {
+            const uint64_t a = smem_desc_sw128(smem + (uint32_t)(g * CHUNKS * PA_CHUNK)), b = smem_desc_sw128(kv_smem + (uint32_t)(stage * STAGE_BYTES));
+#pragma unroll
+            for (int c = 0; c < CHUNKS; c++)
+                pa_mma_qk(tmem + (uint32_t)(g * PA_KEYS), a + (uint64_t)(c * (PA_CHUNK >> 4)), b + (uint64_t)(c * (PA_CHUNK >> 4)), IDESC_QK, c > 0, issue);
+            tc_commit_if(&sh->s_full[g], issue);
+        };
+        while (items.next(sh, it, failed)) {
+            const int n = max(it.n0, it.n1), nt[2] = {it.n0, it.n1};
+            const bool tail = n > 0 && n * PA_KEYS > it.keys;
+            if (n == 0) continue;
+            // ring: keys of tile 0, values of tile 0, keys of tile 1, values of tile 1, ...
+            if (!pa_wait(&sh->kv_full[ring.s], ring.phase)) failed = true;
+            for (int g = 0; g < 2 && !failed; g++) {
+                if (nt[g] == 0) continue;
+                if (!pa_wait(&sh->q_full[g], q_phase[g])) {
+                    failed = true;
+                    break;
+                }
+                q_phase[g] ^= 1;
+                tc_fence_after();
+                scores(g, ring.s);
+                if (nt[g] == 1) tc_commit_if(&sh->q_empty[g], issue);
+            }
+            if (failed) break;
+            tc_commit_if(&sh->kv_empty[ring.s], issue);
+            ring.advance(STAGES);
+            for (int j = 0; j < n && !failed; j++) {
+                const StageCursor v = ring, k = after(v);
+                bool have_v = false, have_k = false;
+                for (int g = 0; g < 2; g++) {
+                    if (j >= nt[g]) continue;
+                    if (!have_v) {
+                        have_v = true;
+                        if (!pa_wait(&sh->kv_full[v.s], v.phase)) {
+                            failed = true;
+                            break;
+                        }
+                        if (tail && j == n - 1) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
+                            for (int c = 0; c < CHUNKS; c++)
+                                for (int i = (it.keys - j * PA_KEYS) * 8 + lane; i < PA_KEYS * 8; i += 32)
+                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv_smem + (uint32_t)(v.s * STAGE_BYTES + c * PA_CHUNK + i * 16)), "r"(0) : "memory");
+                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                            __syncwarp();
+                        }
+                    }
+                    if (!pa_wait(&sh->p_full[g], p_phase[g])) {
+                        failed = true;
+                        break;
+                    }
+                    p_phase[g] ^= 1;
+                    tc_fence_after();
+                    const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(v.s * STAGE_BYTES), PA_CHUNK);
+#pragma unroll
+                    for (int h = 0; h < 2; h++)
+                        pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, (j | h) > 0, issue);
+                    if (j + 1 == nt[g]) {
+                        tc_commit_if(&sh->o_full[g], issue);
+                        continue;
+                    }
+                    if (!have_k) {
+                        have_k = true;
+                        if (!pa_wait(&sh->kv_full[k.s], k.phase)) {
+                            failed = true;
+                            break;
+                        }
+                        tc_fence_after();
+                    }
+                    scores(g, k.s);
+                    if (j + 2 == nt[g]) tc_commit_if(&sh->q_empty[g], issue);
+                }
+                if (failed) break;
+                tc_commit_if(&sh->kv_empty[v.s], issue);
+                ring.advance(STAGES);
+                if (j + 1 < n) {
+                    tc_commit_if(&sh->kv_empty[k.s], issue);
+                    ring.advance(STAGES);
+                }
+            }
+            if (failed) break;
+        }
+    } else if (warp == PA_SCHED_WARP) {
+        PromptSchedule schedule{t};
+        schedule.begin();
+        int64_t i = blockIdx.x;
+        int slot = 0;
+        uint32_t phase = 1;
+        for (bool more = true; more;) {
+            it = PromptItem{};
+            it.last = 1;
+            more = schedule.find(i, it);
+            unsigned int ahead = 0;
+            if (more && lane == 0) ahead = atomicAdd(&t.sched[0], 1u);
+            if (!pa_wait(&sh->item_empty[slot], phase)) {
+                failed = true;
+                break;
+            }
+            if (lane == 0) {
+                sh->items[slot] = it;
+                g_mbar_arrive(&sh->item_full[slot]);
+            }
+            if (++slot == PA_ITEMS) slot = 0, phase ^= 1;
+            i = (int64_t)gridDim.x + __shfl_sync(0xFFFFFFFFu, ahead, 0);
+        }
+        __threadfence();
+        if (lane == 0 && atomicAdd(&t.sched[1], 1u) == gridDim.x - 1) {  // the last one leaves the counters as it found them
+            t.sched[0] = 0;
+            t.sched[1] = 0;
+        }
+    }
+    if (failed) {
+        if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
+        drain_after_abort();
+    }
+    tc_fence_before();
+    __syncthreads();
+    if (warp == PA_MMA_WARP) {
+        tc_fence_after();
+        tmem_dealloc(tmem, 512);
+    }
+}
+
+}  // namespace wf

@@ -113,6 +113,8 @@ struct GemvScratch {
     int64_t x16_bytes = 0;
     std::shared_ptr<float> d_gemm_partial;  // [sm_count][256][128] pieces of tiles cut by a share boundary
     std::shared_ptr<unsigned int> d_gemm_ready;  // [sm_count][4] generation whose piece is complete, per 32-row quarter; then {generation, CTAs out}
+    // attention
+    std::shared_ptr<unsigned int> d_attn_sched;  // counters of the prompt kernel, 0 between launches
 };
 // cudaMalloc for everything that a context allocates: where memory is short, its kept tile buffers go first.
 cudaError_t device_alloc(Context* c, void** p, size_t bytes);

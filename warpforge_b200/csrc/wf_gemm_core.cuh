@@ -10,6 +10,11 @@
 
 namespace wf {
 
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_tiled_fn();  // the driver's cuTensorMapEncodeTiled, null if there is none (wf_gemm.cu)
+
 constexpr int GEMM_BN = 128;             // weight rows per CTA and tile (UMMA M per CTA)
 constexpr int GEMM_BK = 128;             // k per unit of the work split
 constexpr int GEMM_DEQUANT_WARPS = 8;    // of a set: a 16-row weight tile each
