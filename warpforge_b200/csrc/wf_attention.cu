@@ -4,22 +4,9 @@
 #include <atomic>
 
 #include "wf_attention_prompt.cuh"
+#include "wf_attention_tree.cuh"
 
 namespace wf {
-
-__global__ void __launch_bounds__(128) tree_rows_kernel(const __grid_constant__ TreeParams p) {
-    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-    asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t n = (int64_t)p.seqs * p.max_drafts * p.q_heads;
-    for (int64_t i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 5); i < n; i += (int64_t)gridDim.x * 4) {
-        const int head = (int)(i % p.q_heads), draft = (int)(i / p.q_heads % p.max_drafts), s = (int)(i / p.q_heads / p.max_drafts);
-        const TreeSeq q = tree_seq(p, s);
-        if (draft >= q.rows) continue;
-        const int row = q.row0 + draft;
-        attend_row(p.cache, q.place, p.q + (size_t)row * p.q_stride + (size_t)head * p.cache.dim, p.out + ((size_t)row * p.q_heads + head) * p.cache.dim,
-                   head / p.group, q.context < 0 ? 0 : q.context + q.rows, p.scale_log2, p.status, SeesAncestors{q.context, ancestors_of(p, row, draft)});
-    }
-}
 
 }  // namespace wf
 
@@ -128,6 +115,37 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     return launch_attention(c, what, prompt_tiles_kernel<CHUNKS>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
 
+template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const TreeParams& p, cudaStream_t s) {
+    const char* what = "tree_attention";
+    typedef TreeShape<CHUNKS, MT, WM> Shape;
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    GemvScratch& scratch = c->gemv_scratch[s];
+    if (!scratch.d_attn_pieces) {
+        const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
+        if (rc != WF_OK) return rc;
+        std::shared_ptr<float> pieces;  // and behind them the counters
+        const size_t bytes = (size_t)c->sm_count * (2 * TA_MAX_PIECE * sizeof(float) + sizeof(unsigned int));
+        WF_CUDA(c, make_shared_device(c, pieces, bytes));
+        WF_CUDA(c, cudaMemsetAsync(pieces.get(), 0, bytes, s));
+        scratch.d_attn_pieces = pieces;
+    }
+    TreeTiles t{};
+    t.p = p;
+    t.pieces = scratch.d_attn_pieces.get();
+    t.count = reinterpret_cast<unsigned int*>(t.pieces + (size_t)c->sm_count * 2 * TA_MAX_PIECE);
+    CUtensorMap k, v;
+    int rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
+    if (rc != WF_OK) return rc;
+    const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
+    const int64_t most = std::min<int64_t>(p.seqs * blocks * p.cache.kv_heads, c->sm_count) * tiles;  // tiles, where there are fewer than SMs
+    return launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, WM>, (unsigned)std::min<int64_t>(most, c->sm_count), TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
+}
+
 #define ATTENTION_ENTER(ctxh)                                              \
     Context* c = get_context(ctxh);                                        \
     if (!c) return WF_ERR_INVALID_HANDLE;                                  \
@@ -141,7 +159,8 @@ extern "C" {
 int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
     ATTENTION_ENTER(ctx);
     const char* what = "prompt_attention";
-    if (!a) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (!a || !cache) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
     int rc = check_cache(c, what, cache, layer, true);
     if (rc == WF_OK) rc = check_queries(c, what, a->q_dev, a->out_dev, a->q_stride, a->tokens, a->seqs, a->q_heads, cache);
     if (rc != WF_OK) return rc;
@@ -153,7 +172,6 @@ int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf
     if (!packed && (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1))
         return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld", what, (long long)a->table_stride);
     if (!(a->scale > 0.f) || a->scale > 1e30f) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: scale %g", what, (double)a->scale);
-    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
     if (cache->pages < 1) return set_error(c, WF_ERR_SHAPE, "%s: a cache without pages", what);
     PromptParams p{};
     p.cache = cache_layer(*cache, layer);
@@ -176,7 +194,8 @@ int wf_prompt_attention(int64_t ctx, const wf_prompt_attention_args* a, const wf
 int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
     ATTENTION_ENTER(ctx);
     const char* what = "tree_attention";
-    if (!a) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (!a || !cache) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
     int rc = check_cache(c, what, cache, layer, false);
     if (rc == WF_OK) rc = check_queries(c, what, a->q_dev, a->out_dev, a->q_stride, a->tokens, a->seqs, a->q_heads, cache);
     if (rc != WF_OK) return rc;
@@ -188,7 +207,6 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     if (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1 || a->max_context < 0 || a->max_context > (1LL << 31) - 1024)
         return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld, max_context %lld", what, (long long)a->table_stride, (long long)a->max_context);
     if (!(a->scale > 0.f) || a->scale > 1e30f) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: scale %g", what, (double)a->scale);
-    if (a->tokens == 0 || a->seqs == 0) return WF_OK;
     if (cache->pages < 1) return set_error(c, WF_ERR_SHAPE, "%s: a cache without pages", what);
     TreeParams p{};
     p.cache = cache_layer(*cache, layer);
@@ -208,8 +226,9 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     p.max_drafts = a->max_drafts;
     p.scale_log2 = a->scale * 1.44269504f;
     p.status = c->d_status;
-    const int64_t want = ((int64_t)a->seqs * a->max_drafts * a->q_heads + 3) / 4;
-    return launch_attention(c, what, tree_rows_kernel, (unsigned)std::min<int64_t>(want, c->sm_count * 16), 128, 0, s, p);
+    const int rows = a->max_drafts * p.group;  // of a sequence and kv head: the smallest block of rows that holds them, 64 at most
+    if (dim_chunks(cache->head_dim) == 1) return rows <= 16 ? launch_tree<1, 1, 1>(c, p, s) : rows <= 32 ? launch_tree<1, 2, 1>(c, p, s) : launch_tree<1, 2, 2>(c, p, s);
+    return rows <= 16 ? launch_tree<2, 1, 1>(c, p, s) : rows <= 32 ? launch_tree<2, 2, 1>(c, p, s) : launch_tree<2, 2, 2>(c, p, s);
 }
 
 }  // extern "C"

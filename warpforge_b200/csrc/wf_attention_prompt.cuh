@@ -376,7 +376,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 o_phase ^= 1;
                 tc_fence_after();
                 const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-                odd = !(l < INFINITY);
+                odd = !(l < INFINITY) || (l == 0.f && m > -INFINITY);  // scores so large that rounding m scale alone moves a weight out of range
 #pragma unroll
                 for (int c = 0; c < DIM; c += 32) {
                     uint32_t o[32];

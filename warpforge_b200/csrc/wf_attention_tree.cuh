@@ -1,0 +1,552 @@
+// Attention of a few new tokens per sequence over a long cache.
+//
+// Bound by HBM: every key and value is read once, 4 dim bytes for 4 dim flops a row.  The rows of a sequence and kv head (its new tokens times the
+// heads of the group) are padded to 16 .. 64 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
+// one decoded token fills one to eight.
+//
+// All (sequence, kv head, rows) units, each so many tiles of 16 keys long, form one line that is cut evenly over the SMs.  A CTA's share crosses
+// units; the pieces of a unit that is cut between CTAs are joined by the last of them to finish, in the order of the line.  Inside a CTA one warp
+// walks the line and has TMA fill a ring of tiles ahead, across the ends of units too; teams of warps take the tiles of a piece in turn.
+#pragma once
+#include "wf_attention.cuh"
+#include "wf_gemm_core.cuh"
+
+namespace wf {
+
+constexpr int TA_KEYS = 16;  // of a tile
+constexpr int TA_WARPS = 8;  // that multiply; one more walks, and three have nothing to do: setmaxnreg wants four
+constexpr int TA_THREADS = (TA_WARPS + 4) * 32;
+// Registers: 168 a thread at launch; the warps that multiply take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
+constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
+constexpr int TA_MERGE_BYTES = 64 * 1024;
+constexpr int TA_SEGMENTS = 2;     // announced ahead
+constexpr int TA_UNIT_TILES = 8;   // what a unit costs beyond its tiles, in tiles
+constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
+// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows a warp, WM warps a team
+template <int CHUNKS, int MT, int WM> struct TreeShape {
+    static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT * WM, TEAMS = TA_WARPS / WM;
+    static constexpr int SLOT_BYTES = 2 * CHUNKS * TA_KEYS * 128;  // keys and values of a tile
+    static constexpr int Q_BYTES = ROWS * DIM * 2;
+    static constexpr int FIT = (227 * 1024 - TA_MERGE_BYTES - TA_SEGMENTS * Q_BYTES - 4 * 1024) / SLOT_BYTES, SLOTS = FIT > 32 ? 32 : FIT;
+    static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TEAMS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TEAMS;  // teams whose sums lie in shared memory at a time
+    static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
+    static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory: sums, then maxima, then weights
+    static_assert(SETS == TEAMS || 2 * SETS == TEAMS, "one round of folding");
+    static_assert(SLOTS >= TEAMS, "a slot for every team");
+};
+constexpr int TA_MAX_PIECE = 64 * (128 + 2);
+
+// What a CTA has of a unit.
+struct TreeSegment {
+    int row0, rows, context, seq;  // of the sequence; context < 0: a sequence that cannot be, its rows are zeros
+    int head, first;               // first of the sequence's rows * group that the unit has
+    int from, to, tiles;           // of the unit
+    int slot, phase;               // of the first tile in the ring
+    int first_cta, last_cta;       // that have pieces of it
+    int last;                      // no more work
+};
+
+struct TreeTiles {
+    TreeParams p;
+    float* pieces;        // [CTAs][2]: the piece a CTA's share begins with, one that starts later in it
+    unsigned int* count;  // [CTAs]: pieces done of the cut unit that begins in this CTA's share; 0 between launches
+};
+
+__device__ __forceinline__ void ta_load(uint32_t dst, const CUtensorMap* map, int x, int z, void* bar) {
+    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
+                 "r"(0), "r"(z), "r"(g_smem_u32(bar))
+                 : "memory");
+}
+__device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void ldmatrix4_trans(uint32_t addr, uint32_t (&r)[4]) {
+    asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
+}
+__device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ta_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+__device__ __forceinline__ void ta_copy16(uint32_t dst, const void* src, bool real) {  // zeros where there is nothing
+    asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
+}
+__device__ __forceinline__ void ta_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(TA_WARPS * 32) : "memory"); }
+__device__ __forceinline__ bool ta_sync_or(bool v) {  // the same answer for all warps that multiply
+    uint32_t r;
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)v), "n"(TA_WARPS * 32) : "memory");
+    return r != 0;
+}
+
+template <int CHUNKS, int MT, int WM> struct TreeShared {
+    typedef TreeShape<CHUNKS, MT, WM> Shape;
+    uint64_t full[Shape::SLOTS], empty[Shape::SLOTS];
+    uint64_t seg_full[TA_SEGMENTS], seg_empty[TA_SEGMENTS];
+    TreeSegment segments[TA_SEGMENTS];
+    float team_max[Shape::SETS][Shape::ROWS], team_sum[Shape::SETS][Shape::ROWS];
+    unsigned long long odd_rows;
+    int last_one;
+    int bad_page;  // the segment of this number and those before it have pages outside the cache
+};
+
+// The warp that walks the line: announces this CTA's segments with their queries, and has their tiles loaded.  True: all went well.
+template <int CHUNKS, int MT, int WM>
+__device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem) {
+    typedef TreeShape<CHUNKS, MT, WM> Shape;
+    constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
+    const TreeParams& p = t.p;
+    const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
+    auto tiles_of = [&](const TreeSeq& q) { return max(1, (q.context + q.rows + TA_KEYS - 1) / TA_KEYS); };
+    auto units_of = [&](const TreeSeq& q) { return heads * ((q.rows * group + ROWS - 1) / ROWS); };
+    auto line_of = [&](const TreeSeq& q) { return q.rows == 0 ? 0 : (int64_t)(tiles_of(q) + TA_UNIT_TILES) * units_of(q); };
+    auto info = [&](int s) {
+        TreeSeq q;
+        q.rows = 0;
+        if (s < p.seqs) q = tree_seq(p, s);
+        return q;
+    };
+    // a lane has a sequence at a time
+    TreeSeq mine = info(lane);
+    int64_t line = line_of(mine), total = line;
+#pragma unroll 1
+    for (int s0 = 32; s0 < p.seqs; s0 += 32) total += line_of(info(s0 + lane));
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
+    const int64_t share = total / gridDim.x, more = total % gridDim.x;  // the first `more` CTAs have one position more
+    const int64_t begin = blockIdx.x * share + min((int64_t)blockIdx.x, more), end = begin + share + ((int64_t)blockIdx.x < more);
+    auto cta_of = [&](int64_t x) { return (int)(x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share); };
+    int seg = 0, slot = 0, number = 0;
+    uint32_t seg_phase = 1, phase = 1;
+    int64_t at = 0;  // where the sequence begins on the line
+    bool ok = true;
+#pragma unroll 1
+    for (int s0 = 0; s0 < p.seqs && at < end && ok; s0 += 32) {
+        if (s0) {
+            mine = info(s0 + lane);
+            line = line_of(mine);
+        }
+        int64_t to_here = line;  // of the sequences up to this lane's
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int64_t v = __shfl_up_sync(0xFFFFFFFFu, to_here, o);
+            if (lane >= o) to_here += v;
+        }
+        const int64_t base = at;
+        at += __shfl_sync(0xFFFFFFFFu, to_here, 31);
+        uint32_t ours = __ballot_sync(0xFFFFFFFFu, line > 0 && base + to_here > begin && base + to_here - line < end);  // sequences that the share touches
+#pragma unroll 1
+        for (; ours && ok; ours &= ours - 1) {
+            const int l = __ffs(ours) - 1;
+            TreeSeq q;
+            q.row0 = __shfl_sync(0xFFFFFFFFu, mine.row0, l);
+            q.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, l);
+            q.context = __shfl_sync(0xFFFFFFFFu, mine.context, l);
+            const int64_t start = base + __shfl_sync(0xFFFFFFFFu, to_here - line, l);
+            const int tiles = tiles_of(q), units = units_of(q), length = tiles + TA_UNIT_TILES, blocks = units / heads, keys = q.context < 0 ? 0 : q.context + q.rows;
+            const int* table = p.tables + (size_t)(s0 + l) * p.table_stride;
+            int unit = begin > start ? (int)((begin - start) / length) : 0;
+#pragma unroll 1
+            for (int64_t u_at = start + (int64_t)unit * length; unit < units && u_at < end; unit++, u_at += length) {
+                // a unit begins with TA_UNIT_TILES positions that stand for what it costs in any case
+                const int from = (int)max((int64_t)0, begin - u_at - TA_UNIT_TILES), to = (int)min((int64_t)tiles, end - u_at - TA_UNIT_TILES);
+                if (to <= from) continue;
+                const int head = unit / blocks, first = (unit - head * blocks) * ROWS;
+                // the page of a lane's tile, asked for before anything is waited for
+                int tile = from + lane, page = 0;
+                if (tile < to && keys > 0) page = table[tile * TA_KEYS >> p.cache.page_shift];
+                if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
+                const int count = min(ROWS, q.rows * group - first);
+                if (lane == 0) {
+                    TreeSegment& d = sh->segments[seg];
+                    const bool whole = from == 0 && to == tiles;
+                    d.row0 = q.row0, d.rows = q.rows, d.context = q.context, d.seq = s0 + l, d.head = head, d.first = first;
+                    d.from = from, d.to = to, d.tiles = tiles, d.slot = slot, d.phase = (int)phase ^ 1, d.last = 0;
+                    d.first_cta = whole ? 0 : cta_of(u_at + TA_UNIT_TILES);
+                    d.last_cta = whole ? 0 : cta_of(u_at + length - 1);
+                    g_mbar_arrive(&sh->seg_full[seg]);
+                }
+                __syncwarp();
+                auto queries = [&] {  // rows of 16-byte pieces, swizzled by the row
+                    const bf16* q0 = p.q + (size_t)q.row0 * p.q_stride + (size_t)head * group * p.cache.dim;
+#pragma unroll 1
+                    for (int i = lane; i < ROWS * (DIM / 8); i += 32) {
+                        const int r = i / (DIM / 8), piece = i % (DIM / 8), token = (first + r) / group;
+                        const bool real = r < count && piece * 8 < p.cache.dim;
+                        ta_copy16(q_smem + (uint32_t)(seg * Shape::Q_BYTES + r * DIM * 2 + ((piece ^ (r & 7)) << 4)),
+                                  real ? q0 + (size_t)token * p.q_stride + (size_t)((first + r) - token * group) * p.cache.dim + piece * 8 : p.q, real);
+                    }
+                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(g_smem_u32(&sh->seg_full[seg])) : "memory");
+                };
+#pragma unroll 1
+                for (int t0 = from; t0 < to; t0 += 32) {
+                    if (t0 > from) {
+                        tile = t0 + lane;
+                        page = tile < to && keys > 0 ? table[tile * TA_KEYS >> p.cache.page_shift] : 0;
+                    }
+                    if (page < 0 || page >= p.cache.pages) {  // never followed: the unit's rows go key by key
+                        *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                        page = 0;
+                    }
+                    const int z = ((page * heads + head) << p.cache.page_shift) + (tile * TA_KEYS & ((1 << p.cache.page_shift) - 1));  // below 2^31: check_cache
+                    const int n = min(32, to - t0);
+#pragma unroll 1
+                    for (int i = 0; i < n; i++) {
+                        const int row = __shfl_sync(0xFFFFFFFFu, z, i);
+                        if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
+                        if (lane == 0) g_mbar_expect_tx(&sh->full[slot], Shape::SLOT_BYTES);
+                        __syncwarp();
+                        if (lane < 2 * CHUNKS)
+                            ta_load(ring + (uint32_t)(slot * Shape::SLOT_BYTES + lane * TA_KEYS * 128), lane < CHUNKS ? k_map : v_map, 64 * (lane % CHUNKS), row, &sh->full[slot]);
+                        if (++slot == Shape::SLOTS) slot = 0, phase ^= 1;
+                        if (t0 == from && i == min(n, Shape::TEAMS) - 1) queries();  // behind the first tiles, which take longer
+                    }
+                }
+                number++;
+                if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
+            }
+        }
+    }
+    if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
+    if (lane == 0) sh->segments[seg].last = 1;
+    __syncwarp();
+    if (lane == 0) g_mbar_arrive(&sh->seg_full[seg]);
+    g_mbar_arrive(&sh->seg_full[seg]);
+    return true;
+}
+
+template <int CHUNKS, int MT, int WM>
+__global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
+                                                                   const __grid_constant__ CUtensorMap v_map) {
+    typedef TreeShape<CHUNKS, MT, WM> Shape;
+    constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, TEAMS = Shape::TEAMS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
+    constexpr bool Q_KEPT = MT * CHUNKS <= 2;  // queries stay in registers; else they are read again with every tile
+    extern __shared__ uint8_t raw[];
+    __shared__ TreeShared<CHUNKS, MT, WM> sh_;
+    TreeShared<CHUNKS, MT, WM>* const sh = &sh_;
+    const TreeParams& p = t.p;
+    const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, quad = lane & 3;
+    const uint32_t ring = (g_smem_u32(raw) + 1023u) & ~1023u, q_smem = ring + SLOTS * SLOT_BYTES;
+    float* const merge = reinterpret_cast<float*>(raw + (ring - g_smem_u32(raw)) + SLOTS * SLOT_BYTES + TA_SEGMENTS * Shape::Q_BYTES);
+    if (tid < SLOTS) {
+        g_mbar_init(&sh->full[tid], 1);
+        g_mbar_init(&sh->empty[tid], WM);
+    } else if (tid >= 32 && tid < 32 + TA_SEGMENTS) {
+        g_mbar_init(&sh->seg_full[tid - 32], 33);  // every lane's copies of queries, and the words
+        g_mbar_init(&sh->seg_empty[tid - 32], TA_WARPS);
+    } else if (tid == 64) {
+        sh->odd_rows = 0;
+        sh->bad_page = -1;
+        prefetch_tensormap(&k_map);
+        prefetch_tensormap(&v_map);
+    }
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    __syncthreads();
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    if (warp >= TA_WARPS) {
+        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
+        if (warp == TA_WARPS && !tree_walk<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem)) {
+            if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
+            drain_after_abort();
+        }
+        return;
+    }
+
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_MULTIPLY_REGS));
+    const int team = warp / WM, part = warp % WM;  // the team, which rows of it
+    const float scale = p.scale_log2;
+    const int d = p.cache.dim, group = p.group;
+    // ldmatrix: a lane's row and 16-byte piece, swizzled
+    const int matrix = lane >> 3, mrow = lane & 7;
+    const uint32_t k_row = (uint32_t)(((matrix >> 1) * 8 + mrow) * 128), v_row = (uint32_t)(((matrix & 1) * 8 + mrow) * 128) + CHUNKS * TA_KEYS * 128;
+    const uint32_t q_row = (uint32_t)((part * MT * 16 + (matrix & 1) * 8 + mrow) * DIM * 2);
+    int seg = 0;
+    uint32_t seg_phase = 0;
+    bool failed = false;
+#pragma unroll 1
+    for (int number = 0;; number++) {
+        failed |= !g_mbar_wait(&sh->seg_full[seg], seg_phase);
+        if (ta_sync_or(failed)) {  // `merge` is free again, too
+            failed = true;
+            break;
+        }
+        const TreeSegment w = sh->segments[seg];
+        if (w.last) break;
+        const int keys = w.context < 0 ? 0 : w.context + w.rows, count = min(ROWS, w.rows * group - w.first);
+        const uint32_t q_at = q_smem + (uint32_t)(seg * Shape::Q_BYTES) + q_row;
+        auto load_q = [&](int i, int k, uint32_t(&a)[4]) { ldmatrix4(q_at + (uint32_t)(i * 16 * DIM * 2) + (uint32_t)(((2 * k + (matrix >> 1)) ^ mrow) << 4), a); };
+        uint32_t q[MT][Q_KEPT ? DIM / 16 : 1][4];
+        if (Q_KEPT)
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int k = 0; k < DIM / 16; k++) load_q(i, k, q[i][Q_KEPT ? k : 0]);
+        float o[MT][N_TILES][4], m[MT][2], l[MT][2];
+#pragma unroll
+        for (int i = 0; i < MT; i++) {
+            m[i][0] = m[i][1] = -INFINITY;
+            l[i][0] = l[i][1] = 0.f;
+#pragma unroll
+            for (int n = 0; n < N_TILES; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
+        }
+        int slot = w.slot + team;
+        uint32_t phase = (uint32_t)w.phase;
+        if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+#pragma unroll 1
+        for (int tile = w.from + team; tile < w.to; tile += TEAMS) {
+            if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->full[slot], phase))) {
+                failed = true;
+                break;
+            }
+            const uint32_t base = ring + (uint32_t)(slot * SLOT_BYTES);
+            float s[MT][2][4] = {};
+#pragma unroll
+            for (int k0 = 0; k0 < DIM / 16; k0 += 4) {
+                uint32_t b[4][4];
+#pragma unroll
+                for (int k = 0; k < 4; k++) ldmatrix4(base + (uint32_t)(k0 / 4 * TA_KEYS * 128) + k_row + (uint32_t)(((2 * k + (matrix & 1)) ^ mrow) << 4), b[k]);
+#pragma unroll
+                for (int k = 0; k < 4; k++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        if (!Q_KEPT) load_q(i, k0 + k, q[i][0]);
+                        mma_bf16(s[i][0], q[i][Q_KEPT ? k0 + k : 0], b[k][0], b[k][1]);
+                        mma_bf16(s[i][1], q[i][Q_KEPT ? k0 + k : 0], b[k][2], b[k][3]);
+                    }
+            }
+            const int key0 = tile * TA_KEYS;
+            if (key0 + TA_KEYS > w.context) {  // new tokens, or none
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = (part * MT + i) * 16 + g + 8 * e, token = (w.first + r) / group;
+                        const uint64_t sees = r < count && keys > 0 ? ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows)) : 0;
+#pragma unroll
+                        for (int c = 0; c < 4; c++) {
+                            const int j = key0 + 8 * (c >> 1) + 2 * quad + (c & 1) - w.context;
+                            if (!(w.context >= 0 && (j < 0 || (j < TREE_MAX_DRAFTS && (sees >> j & 1))))) s[i][c >> 1][2 * e + (c & 1)] = -INFINITY;
+                        }
+                    }
+                if (key0 + TA_KEYS > keys) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
+#pragma unroll 1
+                    for (int e = max(0, keys - key0) * 8 * CHUNKS + lane; e < TA_KEYS * 8 * CHUNKS; e += 32) {
+                        const int row = e / (8 * CHUNKS), piece = e % (8 * CHUNKS);
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(base + (uint32_t)((CHUNKS + piece / 8) * TA_KEYS * 128 + row * 128 + piece % 8 * 16)), "r"(0) : "memory");
+                    }
+                    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                    __syncwarp();
+                }
+            }
+            bool grows = false;
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++)
+                    grows |= (fmaxf(fmaxf(s[i][0][2 * e], s[i][0][2 * e + 1]), fmaxf(s[i][1][2 * e], s[i][1][2 * e + 1])) - m[i][e]) * scale > TA_RESCALE;
+            if (__any_sync(0xFFFFFFFFu, grows)) {
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        float top = fmaxf(fmaxf(s[i][0][2 * e], s[i][0][2 * e + 1]), fmaxf(s[i][1][2 * e], s[i][1][2 * e + 1]));
+                        top = fmaxf(m[i][e], top);
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
+                        top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
+                        const float keep = ta_ex2((m[i][e] - (top == -INFINITY ? 0.f : top)) * scale);
+                        m[i][e] = top;
+                        l[i][e] *= keep;
+#pragma unroll
+                        for (int n = 0; n < N_TILES; n++) {
+                            o[i][n][2 * e] *= keep;
+                            o[i][n][2 * e + 1] *= keep;
+                        }
+                    }
+            }
+            uint32_t a[MT][4];
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const float ref = m[i][e] == -INFINITY ? 0.f : m[i][e] * scale;
+#pragma unroll
+                    for (int n = 0; n < 2; n++) {
+                        const float x = ta_ex2(fmaf(s[i][n][2 * e], scale, -ref)), y = ta_ex2(fmaf(s[i][n][2 * e + 1], scale, -ref));
+                        l[i][e] += x + y;
+                        a[i][2 * n + e] = pack_bf16(x, y);
+                    }
+                }
+#pragma unroll
+            for (int n0 = 0; n0 < N_TILES / 2; n0 += 4) {
+                uint32_t b[4][4];
+#pragma unroll
+                for (int n = 0; n < 4; n++) ldmatrix4_trans(base + (uint32_t)(n0 / 4 * TA_KEYS * 128) + v_row + (uint32_t)(((2 * n + (matrix >> 1)) ^ mrow) << 4), b[n]);
+#pragma unroll
+                for (int n = 0; n < 4; n++)
+#pragma unroll
+                    for (int i = 0; i < MT; i++) {
+                        mma_bf16(o[i][2 * (n0 + n)], a[i], b[n][0], b[n][1]);
+                        mma_bf16(o[i][2 * (n0 + n) + 1], a[i], b[n][2], b[n][3]);
+                    }
+            }
+            __syncwarp();
+            if (lane == 0) g_mbar_arrive(&sh->empty[slot]);
+            slot += TEAMS;
+            if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
+        }
+        __syncwarp();
+        if (lane == 0) g_mbar_arrive(&sh->seg_empty[seg]);  // the queries
+        if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
+        if (*reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l[0][0] = l[0][1] = l[MT - 1][0] = l[MT - 1][1] = __uint_as_float(0x7FC00000u);
+
+        // The teams' sums together.  Where they do not all fit shared memory the upper half hands its to the lower half first.
+        auto write_sums = [&](int set) {
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    // the threads of a row have followed the same maximum
+                    l[i][e] += __shfl_xor_sync(0xFFFFFFFFu, l[i][e], 1);
+                    l[i][e] += __shfl_xor_sync(0xFFFFFFFFu, l[i][e], 2);
+                    const int r = (part * MT + i) * 16 + g + 8 * e;
+                    if (quad == 0) {
+                        sh->team_max[set][r] = m[i][e];
+                        sh->team_sum[set][r] = l[i][e];
+                    }
+                    float2* row = reinterpret_cast<float2*>(merge + (size_t)(set * ROWS + r) * DIM);
+#pragma unroll
+                    for (int n = 0; n < N_TILES; n++) row[(n ^ (r & 3)) * 4 + quad] = make_float2(o[i][n][2 * e], o[i][n][2 * e + 1]);
+                }
+        };
+        if (SETS < TEAMS) {
+            if (team >= SETS) write_sums(team - SETS);
+            ta_sync();
+            if (team < SETS) {
+#pragma unroll
+                for (int i = 0; i < MT; i++)
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int r = (part * MT + i) * 16 + g + 8 * e;
+                        const float other = sh->team_max[team][r], top = fmaxf(m[i][e], other), ref = top == -INFINITY ? 0.f : top;
+                        const float keep = ta_ex2((m[i][e] - ref) * scale), take = ta_ex2((other - ref) * scale);
+                        m[i][e] = top;
+                        l[i][e] = l[i][e] * keep + (quad == 0 ? sh->team_sum[team][r] * take : 0.f);
+                        const float2* row = reinterpret_cast<const float2*>(merge + (size_t)(team * ROWS + r) * DIM);
+#pragma unroll
+                        for (int n = 0; n < N_TILES; n++) {
+                            const float2 v = row[(n ^ (r & 3)) * 4 + quad];
+                            o[i][n][2 * e] = o[i][n][2 * e] * keep + v.x * take;
+                            o[i][n][2 * e + 1] = o[i][n][2 * e + 1] * keep + v.y * take;
+                        }
+                    }
+            }
+            ta_sync();
+        }
+        if (team < SETS) write_sums(team);
+        ta_sync();
+        const bool whole = w.from == 0 && w.to == w.tiles;
+        // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
+        float* const piece = t.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
+        auto store = [&](int r, int col, const float(&x)[8], float sum, float top) {  // eight elements of a row, or zeros where it sees nothing
+            const float inv = sum == 0.f ? 0.f : 1.f / sum;
+            // a sum of 0 under a maximum: scores so large that rounding m scale alone moves a weight out of range
+            uint32_t largest = sum < INFINITY && !(sum == 0.f && top > -INFINITY) ? 0 : 0x7F800000u;
+#pragma unroll
+            for (int e = 0; e < 8; e++) largest = max(largest, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+            if (largest >= 0x7F800000u) atomicOr(&sh->odd_rows, 1ull << r);
+            const int token = (w.first + r) / group;
+            bf16* to = p.out + ((size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group) * d + col;
+            *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv), pack_bf16(x[4] * inv, x[5] * inv),
+                                                       pack_bf16(x[6] * inv, x[7] * inv));
+        };
+        constexpr int PER_ROW = DIM / 8;  // threads of a row
+#pragma unroll 1
+        for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
+            const int r = i / PER_ROW, n = i % PER_ROW;
+            float top = -INFINITY, sum = 0.f, x[8] = {};
+#pragma unroll
+            for (int c = 0; c < SETS; c++) top = fmaxf(top, sh->team_max[c][r]);
+            const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll
+            for (int c = 0; c < SETS; c++) {
+                const float keep = ta_ex2((sh->team_max[c][r] - ref) * scale);
+                sum += sh->team_sum[c][r] * keep;
+                const float4* from = reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + (n ^ (r & 3)) * 8);
+                const float4 u = from[0], v = from[1];
+                x[0] += u.x * keep, x[1] += u.y * keep, x[2] += u.z * keep, x[3] += u.w * keep;
+                x[4] += v.x * keep, x[5] += v.y * keep, x[6] += v.z * keep, x[7] += v.w * keep;
+            }
+            if (whole) {
+                if (8 * n < d) store(r, 8 * n, x, sum, top);
+            } else {
+                float4* to = reinterpret_cast<float4*>(piece + r * DIM + 8 * n);
+                __stcg(to, make_float4(x[0], x[1], x[2], x[3]));
+                __stcg(to + 1, make_float4(x[4], x[5], x[6], x[7]));
+                if (n == 0) {
+                    __stcg(piece + ROWS * DIM + r, top);
+                    __stcg(piece + ROWS * (DIM + 1) + r, sum);
+                }
+            }
+        }
+        if (!whole) {
+            __threadfence();
+            ta_sync();
+            if (tid == 0) {
+                sh->last_one = atomicAdd(&t.count[w.first_cta], 1u) == (unsigned)(w.last_cta - w.first_cta);
+                if (sh->last_one) t.count[w.first_cta] = 0;
+                __threadfence();
+            }
+            ta_sync();
+            if (sh->last_one) {
+                auto piece_of = [&](int c) { return t.pieces + ((size_t)c * 2 + (c == w.first_cta)) * Shape::PIECE; };
+#pragma unroll 1
+                for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
+                    const int r = i / PER_ROW, n = i % PER_ROW;
+                    float top = -INFINITY, sum = 0.f, x[8] = {};
+#pragma unroll 8
+                    for (int c = w.first_cta; c <= w.last_cta; c++) top = fmaxf(top, __ldcg(piece_of(c) + ROWS * DIM + r));
+                    const float ref = top == -INFINITY ? 0.f : top;
+#pragma unroll 4
+                    for (int c = w.first_cta; c <= w.last_cta; c++) {
+                        const float* from = piece_of(c);
+                        const float keep = ta_ex2((__ldcg(from + ROWS * DIM + r) - ref) * scale);
+                        sum += __ldcg(from + ROWS * (DIM + 1) + r) * keep;
+                        const float4 u = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 8 * n)), v = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 8 * n) + 1);
+                        x[0] += u.x * keep, x[1] += u.y * keep, x[2] += u.z * keep, x[3] += u.w * keep;
+                        x[4] += v.x * keep, x[5] += v.y * keep, x[6] += v.z * keep, x[7] += v.w * keep;
+                    }
+                    if (8 * n < d) store(r, 8 * n, x, sum, top);
+                }
+            }
+        }
+        ta_sync();
+        const unsigned long long odd = sh->odd_rows;
+        if (odd) {
+            // An Inf or a NaN in a row's sums may have come from a key that it does not see (0 x Inf), or from a page that is not in the cache: key by key.
+            ta_sync();
+            if (tid == 0) sh->odd_rows = 0;
+            KeyPlace place;
+            place.table = p.tables + (size_t)w.seq * p.table_stride;
+            place.first = 0;
+#pragma unroll 1
+            for (int r = warp; r < count; r += TA_WARPS) {
+                if (!(odd >> r & 1)) continue;
+                const int token = (w.first + r) / group, h = w.head * group + (w.first + r) - token * group;
+                attend_row(p.cache, place, p.q + (size_t)(w.row0 + token) * p.q_stride + (size_t)h * d, p.out + ((size_t)(w.row0 + token) * p.q_heads + h) * d, w.head, keys,
+                           scale, p.status, SeesAncestors{w.context, ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows))});
+            }
+        }
+    }
+    if (failed) {
+        if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
+        drain_after_abort();
+    }
+}
+
+}  // namespace wf

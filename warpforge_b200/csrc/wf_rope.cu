@@ -147,7 +147,8 @@ extern "C" int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* a, const
     WF_CUDA(c, cudaSetDevice(c->device));
     cudaStream_t s = resolve_stream(c, stream);
     const char* what = "qk_norm_rope";
-    if (!a) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (!a || !cache) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null arguments", what);
+    if (a->tokens == 0) return WF_OK;
     const int rc = check_kv_cache(c, what, cache, layer, true);
     if (rc != WF_OK) return rc;
     if (a->x_dtype != WF_DTYPE_F32 && a->x_dtype != WF_DTYPE_BF16) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: x_dtype %d", what, a->x_dtype);
@@ -164,7 +165,6 @@ extern "C" int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* a, const
         return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: a rotation needs a 16-byte aligned table and positions", what);
     if ((a->gamma_q_dev | a->gamma_k_dev) & 3 || a->slots_dev & 7) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: misaligned gamma or slots", what);
     if (a->flags & ~(WF_QK_NORM | WF_ROPE_ADJACENT)) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: unknown flags %d", what, a->flags);
-    if (a->tokens == 0) return WF_OK;
     RopeParams p{};
     p.q = reinterpret_cast<const void*>(a->q_dev), p.k = reinterpret_cast<const void*>(a->k_dev), p.v = reinterpret_cast<const void*>(a->v_dev);
     p.q_stride = a->q_stride, p.k_stride = a->k_stride, p.v_stride = a->v_stride;
