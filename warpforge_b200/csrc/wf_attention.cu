@@ -224,6 +224,7 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     p.q_heads = a->q_heads;
     p.group = a->q_heads / cache->kv_heads;
     p.max_drafts = a->max_drafts;
+    p.group_inverse = p.group == 1 ? 0 : (uint32_t)(((1ull << 32) + p.group - 1) / p.group);
     p.scale_log2 = a->scale * 1.44269504f;
     p.status = c->d_status;
     const int rows = a->max_drafts * p.group;  // of a sequence and kv head: the smallest block of rows that holds them, 64 at most

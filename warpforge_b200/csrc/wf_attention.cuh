@@ -59,8 +59,13 @@ struct TreeParams {
     const uint64_t* ancestors;
     int64_t tokens, max_context;
     int seqs, q_heads, group, max_drafts;
+    uint32_t group_inverse;  // 2^32 / group, rounded up; 0 for a group of one
     float scale_log2;
     int* status;
+#ifdef __CUDACC__
+    // row / group, for the rows of a sequence (64 x 128 at most)
+    __device__ __forceinline__ int token_of(int row) const { return group_inverse ? (int)__umulhi((uint32_t)row, group_inverse) : row; }
+#endif
 };
 
 #ifdef __CUDACC__

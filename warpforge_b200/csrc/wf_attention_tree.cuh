@@ -5,8 +5,8 @@
 // one decoded token fills one to eight.
 //
 // All (sequence, kv head, rows) units, each so many tiles of 16 keys long, form one line that is cut evenly over the SMs.  A CTA's share crosses
-// units; the pieces of a unit that is cut between CTAs are joined by the last of them to finish, in the order of the line.  Inside a CTA one warp
-// walks the line and has TMA fill a ring of tiles ahead, across the ends of units too; teams of warps take the tiles of a piece in turn.
+// units; the pieces of a unit that is cut between CTAs are joined by the last of them to finish, in the order of the line.  Inside a CTA four warps
+// walk the line and have TMA fill a ring of tiles ahead, across the ends of units too; teams of eight others take the tiles of a piece in turn.
 #pragma once
 #include "wf_attention.cuh"
 #include "wf_gemm_core.cuh"
@@ -14,8 +14,8 @@
 namespace wf {
 
 constexpr int TA_KEYS = 16;  // of a tile
-constexpr int TA_WARPS = 8;  // that multiply; one more walks, and three have nothing to do: setmaxnreg wants four
-constexpr int TA_THREADS = (TA_WARPS + 4) * 32;
+constexpr int TA_WARPS = 8, TA_LOADERS = 4;  // warps that multiply, warps that walk and load
+constexpr int TA_THREADS = (TA_WARPS + TA_LOADERS) * 32;
 // Registers: 168 a thread at launch; the warps that multiply take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
 constexpr int TA_MERGE_BYTES = 64 * 1024;
@@ -27,17 +27,19 @@ template <int CHUNKS, int MT, int WM> struct TreeShape {
     static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT * WM, TEAMS = TA_WARPS / WM;
     static constexpr int SLOT_BYTES = 2 * CHUNKS * TA_KEYS * 128;  // keys and values of a tile
     static constexpr int Q_BYTES = ROWS * DIM * 2;
-    static constexpr int FIT = (227 * 1024 - TA_MERGE_BYTES - TA_SEGMENTS * Q_BYTES - 4 * 1024) / SLOT_BYTES, SLOTS = FIT > 32 ? 32 : FIT;
+    static constexpr int FIT = (227 * 1024 - TA_MERGE_BYTES - TA_SEGMENTS * Q_BYTES - 4 * 1024) / SLOT_BYTES;
+    // A slot belongs to one loader, and within a segment to one team, lap after lap: a barrier's parity tells the lap apart only for those that wait for every one.
+    static constexpr int TURN = TEAMS > TA_LOADERS ? TEAMS : TA_LOADERS, SLOTS = FIT > 32 ? 32 : FIT / TURN * TURN;
     static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TEAMS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TEAMS;  // teams whose sums lie in shared memory at a time
     static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
     static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory: sums, then maxima, then weights
     static_assert(SETS == TEAMS || 2 * SETS == TEAMS, "one round of folding");
-    static_assert(SLOTS >= TEAMS, "a slot for every team");
+    static_assert(SLOTS >= TEAMS && SLOTS % TEAMS == 0 && SLOTS % TA_LOADERS == 0, "slots for every team and loader");
 };
 constexpr int TA_MAX_PIECE = 64 * (128 + 2);
 
 // What a CTA has of a unit.
-struct TreeSegment {
+struct alignas(16) TreeSegment {
     int row0, rows, context, seq;  // of the sequence; context < 0: a sequence that cannot be, its rows are zeros
     int head, first;               // first of the sequence's rows * group that the unit has
     int from, to, tiles;           // of the unit
@@ -52,10 +54,16 @@ struct TreeTiles {
     unsigned int* count;  // [CTAs]: pieces done of the cut unit that begins in this CTA's share; 0 between launches
 };
 
-__device__ __forceinline__ void ta_load(uint32_t dst, const CUtensorMap* map, int x, int z, void* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
-                 "r"(0), "r"(z), "r"(g_smem_u32(bar))
+// By the thread whose `issue` is non-zero; the whole warp comes here with the same operands, which then sit in uniform registers (issued by four
+// lanes with operands of their own, the loads of a tile took 670 cycles and set the pace; HBM gives an SM a tile in 345).
+__device__ __forceinline__ void ta_load(uint32_t dst, const CUtensorMap* map, int x, int z, uint32_t bar, uint32_t issue) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+                 "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(0), "r"(z), "r"(bar), "r"(issue)
                  : "memory");
+}
+__device__ __forceinline__ void ta_expect(uint32_t bar, uint32_t bytes, uint32_t issue) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(issue) : "memory");
 }
 __device__ __forceinline__ void ldmatrix4(uint32_t addr, uint32_t (&r)[4]) {
     asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0, %1, %2, %3}, [%4];" : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(addr));
@@ -95,9 +103,10 @@ template <int CHUNKS, int MT, int WM> struct TreeShared {
     int bad_page;  // the segment of this number and those before it have pages outside the cache
 };
 
-// The warp that walks the line: announces this CTA's segments with their queries, and has their tiles loaded.  True: all went well.
+// The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
+// well.
 template <int CHUNKS, int MT, int WM>
-__device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem) {
+__device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
     typedef TreeShape<CHUNKS, MT, WM> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
     const TreeParams& p = t.p;
@@ -121,6 +130,7 @@ __device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS,
     const int64_t share = total / gridDim.x, more = total % gridDim.x;  // the first `more` CTAs have one position more
     const int64_t begin = blockIdx.x * share + min((int64_t)blockIdx.x, more), end = begin + share + ((int64_t)blockIdx.x < more);
     auto cta_of = [&](int64_t x) { return (int)(x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share); };
+    const uint32_t issue = elect_one();
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
     int64_t at = 0;  // where the sequence begins on the line
@@ -162,7 +172,7 @@ __device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS,
                 if (tile < to && keys > 0) page = table[tile * TA_KEYS >> p.cache.page_shift];
                 if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
                 const int count = min(ROWS, q.rows * group - first);
-                if (lane == 0) {
+                if (loader == 0 && lane == 0) {
                     TreeSegment& d = sh->segments[seg];
                     const bool whole = from == 0 && to == tiles;
                     d.row0 = q.row0, d.rows = q.rows, d.context = q.context, d.seq = s0 + l, d.head = head, d.first = first;
@@ -175,8 +185,8 @@ __device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS,
                 auto queries = [&] {  // rows of 16-byte pieces, swizzled by the row
                     const bf16* q0 = p.q + (size_t)q.row0 * p.q_stride + (size_t)head * group * p.cache.dim;
 #pragma unroll 1
-                    for (int i = lane; i < ROWS * (DIM / 8); i += 32) {
-                        const int r = i / (DIM / 8), piece = i % (DIM / 8), token = (first + r) / group;
+                    for (int i = loader * 32 + lane; i < ROWS * (DIM / 8); i += 32 * TA_LOADERS) {
+                        const int r = i / (DIM / 8), piece = i % (DIM / 8), token = p.token_of(first + r);
                         const bool real = r < count && piece * 8 < p.cache.dim;
                         ta_copy16(q_smem + (uint32_t)(seg * Shape::Q_BYTES + r * DIM * 2 + ((piece ^ (r & 7)) << 4)),
                                   real ? q0 + (size_t)token * p.q_stride + (size_t)((first + r) - token * group) * p.cache.dim + piece * 8 : p.q, real);
@@ -198,11 +208,13 @@ __device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS,
 #pragma unroll 1
                     for (int i = 0; i < n; i++) {
                         const int row = __shfl_sync(0xFFFFFFFFu, z, i);
-                        if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
-                        if (lane == 0) g_mbar_expect_tx(&sh->full[slot], Shape::SLOT_BYTES);
-                        __syncwarp();
-                        if (lane < 2 * CHUNKS)
-                            ta_load(ring + (uint32_t)(slot * Shape::SLOT_BYTES + lane * TA_KEYS * 128), lane < CHUNKS ? k_map : v_map, 64 * (lane % CHUNKS), row, &sh->full[slot]);
+                        if (slot % TA_LOADERS == loader) {
+                            if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
+                            const uint32_t bar = g_smem_u32(&sh->full[slot]), to_slot = ring + (uint32_t)(slot * Shape::SLOT_BYTES);
+                            ta_expect(bar, Shape::SLOT_BYTES, issue);
+#pragma unroll
+                            for (int c = 0; c < 2 * CHUNKS; c++) ta_load(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue);
+                        }
                         if (++slot == Shape::SLOTS) slot = 0, phase ^= 1;
                         if (t0 == from && i == min(n, Shape::TEAMS) - 1) queries();  // behind the first tiles, which take longer
                     }
@@ -213,9 +225,10 @@ __device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS,
         }
     }
     if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
-    if (lane == 0) sh->segments[seg].last = 1;
-    __syncwarp();
-    if (lane == 0) g_mbar_arrive(&sh->seg_full[seg]);
+    if (loader == 0 && lane == 0) {
+        sh->segments[seg].last = 1;
+        g_mbar_arrive(&sh->seg_full[seg]);
+    }
     g_mbar_arrive(&sh->seg_full[seg]);
     return true;
 }
@@ -237,7 +250,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         g_mbar_init(&sh->full[tid], 1);
         g_mbar_init(&sh->empty[tid], WM);
     } else if (tid >= 32 && tid < 32 + TA_SEGMENTS) {
-        g_mbar_init(&sh->seg_full[tid - 32], 33);  // every lane's copies of queries, and the words
+        g_mbar_init(&sh->seg_full[tid - 32], 32 * TA_LOADERS + 1);  // every lane's copies of queries, and the words
         g_mbar_init(&sh->seg_empty[tid - 32], TA_WARPS);
     } else if (tid == 64) {
         sh->odd_rows = 0;
@@ -251,7 +264,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= TA_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (warp == TA_WARPS && !tree_walk<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem)) {
+        if (!tree_walk<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
@@ -326,7 +339,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const int r = (part * MT + i) * 16 + g + 8 * e, token = (w.first + r) / group;
+                        const int r = (part * MT + i) * 16 + g + 8 * e, token = p.token_of(w.first + r);
                         const uint64_t sees = r < count && keys > 0 ? ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows)) : 0;
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
@@ -453,41 +466,36 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         const bool whole = w.from == 0 && w.to == w.tiles;
         // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
         float* const piece = t.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
-        auto store = [&](int r, int col, const float(&x)[8], float sum, float top) {  // eight elements of a row, or zeros where it sees nothing
+        auto store = [&](int r, int col, const float4& x, float sum, float top) {  // four elements of a row, or zeros where it sees nothing
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             // a sum of 0 under a maximum: scores so large that rounding m scale alone moves a weight out of range
             uint32_t largest = sum < INFINITY && !(sum == 0.f && top > -INFINITY) ? 0 : 0x7F800000u;
-#pragma unroll
-            for (int e = 0; e < 8; e++) largest = max(largest, __float_as_uint(x[e]) & 0x7FFFFFFFu);
+            largest = max(max(largest, __float_as_uint(x.x) & 0x7FFFFFFFu), max(__float_as_uint(x.y) & 0x7FFFFFFFu, max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu)));
             if (largest >= 0x7F800000u) atomicOr(&sh->odd_rows, 1ull << r);
-            const int token = (w.first + r) / group;
+            const int token = p.token_of(w.first + r);
             bf16* to = p.out + ((size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group) * d + col;
-            *reinterpret_cast<uint4*>(to) = make_uint4(pack_bf16(x[0] * inv, x[1] * inv), pack_bf16(x[2] * inv, x[3] * inv), pack_bf16(x[4] * inv, x[5] * inv),
-                                                       pack_bf16(x[6] * inv, x[7] * inv));
+            *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
         };
-        constexpr int PER_ROW = DIM / 8;  // threads of a row
+        constexpr int PER_ROW = DIM / 4;  // threads of a row
 #pragma unroll 1
         for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
             const int r = i / PER_ROW, n = i % PER_ROW;
-            float top = -INFINITY, sum = 0.f, x[8] = {};
+            float top = -INFINITY, sum = 0.f, tops[SETS];
+            float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < SETS; c++) top = fmaxf(top, sh->team_max[c][r]);
+            for (int c = 0; c < SETS; c++) top = fmaxf(top, tops[c] = sh->team_max[c][r]);
             const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int c = 0; c < SETS; c++) {
-                const float keep = ta_ex2((sh->team_max[c][r] - ref) * scale);
+                const float keep = ta_ex2((tops[c] - ref) * scale);
                 sum += sh->team_sum[c][r] * keep;
-                const float4* from = reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + (n ^ (r & 3)) * 8);
-                const float4 u = from[0], v = from[1];
-                x[0] += u.x * keep, x[1] += u.y * keep, x[2] += u.z * keep, x[3] += u.w * keep;
-                x[4] += v.x * keep, x[5] += v.y * keep, x[6] += v.z * keep, x[7] += v.w * keep;
+                const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
+                x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
             }
             if (whole) {
-                if (8 * n < d) store(r, 8 * n, x, sum, top);
+                if (4 * n < d) store(r, 4 * n, x, sum, top);
             } else {
-                float4* to = reinterpret_cast<float4*>(piece + r * DIM + 8 * n);
-                __stcg(to, make_float4(x[0], x[1], x[2], x[3]));
-                __stcg(to + 1, make_float4(x[4], x[5], x[6], x[7]));
+                __stcg(reinterpret_cast<float4*>(piece + r * DIM + 4 * n), x);
                 if (n == 0) {
                     __stcg(piece + ROWS * DIM + r, top);
                     __stcg(piece + ROWS * (DIM + 1) + r, sum);
@@ -508,20 +516,20 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll 1
                 for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
                     const int r = i / PER_ROW, n = i % PER_ROW;
-                    float top = -INFINITY, sum = 0.f, x[8] = {};
-#pragma unroll 8
-                    for (int c = w.first_cta; c <= w.last_cta; c++) top = fmaxf(top, __ldcg(piece_of(c) + ROWS * DIM + r));
-                    const float ref = top == -INFINITY ? 0.f : top;
+                    float top = -INFINITY, sum = 0.f;
+                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll 4
-                    for (int c = w.first_cta; c <= w.last_cta; c++) {
+                    for (int c = w.first_cta; c <= w.last_cta; c++) {  // the maximum followed on the way: all loads of a few pieces in flight at once
                         const float* from = piece_of(c);
-                        const float keep = ta_ex2((__ldcg(from + ROWS * DIM + r) - ref) * scale);
-                        sum += __ldcg(from + ROWS * (DIM + 1) + r) * keep;
-                        const float4 u = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 8 * n)), v = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 8 * n) + 1);
-                        x[0] += u.x * keep, x[1] += u.y * keep, x[2] += u.z * keep, x[3] += u.w * keep;
-                        x[4] += v.x * keep, x[5] += v.y * keep, x[6] += v.z * keep, x[7] += v.w * keep;
+                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 4 * n));
+                        const float m_c = __ldcg(from + ROWS * DIM + r), l_c = __ldcg(from + ROWS * (DIM + 1) + r);
+                        const float grown = fmaxf(top, m_c), ref = grown == -INFINITY ? 0.f : grown;
+                        const float keep = ta_ex2((top - ref) * scale), take = ta_ex2((m_c - ref) * scale);
+                        top = grown;
+                        sum = sum * keep + l_c * take;
+                        x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
                     }
-                    if (8 * n < d) store(r, 8 * n, x, sum, top);
+                    if (4 * n < d) store(r, 4 * n, x, sum, top);
                 }
             }
         }
@@ -537,7 +545,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll 1
             for (int r = warp; r < count; r += TA_WARPS) {
                 if (!(odd >> r & 1)) continue;
-                const int token = (w.first + r) / group, h = w.head * group + (w.first + r) - token * group;
+                const int token = p.token_of(w.first + r), h = w.head * group + (w.first + r) - token * group;
                 attend_row(p.cache, place, p.q + (size_t)(w.row0 + token) * p.q_stride + (size_t)h * d, p.out + ((size_t)(w.row0 + token) * p.q_heads + h) * d, w.head, keys,
                            scale, p.status, SeesAncestors{w.context, ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows))});
             }
