@@ -51,9 +51,9 @@ static int check_queries(Context* c, const char* what, int64_t q, int64_t out, i
     return WF_OK;
 }
 template <class... Params, class... Args>
-static int launch_attention(Context* c, const char* what, void (*kernel)(Params...), unsigned grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
+static int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3(grid);
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
@@ -115,6 +115,25 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     return launch_attention(c, what, prompt_tiles_kernel<CHUNKS>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
 
+// Where the pieces of cut units go.
+static int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cuts) {
+    GemvScratch& scratch = c->gemv_scratch[s];
+    const int64_t head = (c->sm_count * (int64_t)sizeof(TreeCut) + 255) & ~255LL, bytes = head + floats * (int64_t)sizeof(float);
+    if (bytes > scratch.attn_bytes) {
+        const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
+        if (rc != WF_OK) return rc;
+        scratch.d_attn.reset();
+        scratch.attn_bytes = 0;
+        WF_CUDA(c, make_shared_device(c, scratch.d_attn, (size_t)bytes));
+        scratch.attn_bytes = bytes;
+    }
+    cuts->cuts = reinterpret_cast<TreeCut*>(scratch.d_attn.get());
+    cuts->pieces = reinterpret_cast<float*>(scratch.d_attn.get() + head);
+    return WF_OK;
+}
+static int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
+    return launch_attention(c, "tree_attention", tree_join_kernel, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
+}
 template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const TreeParams& p, cudaStream_t s) {
     const char* what = "tree_attention";
     typedef TreeShape<CHUNKS, MT, WM> Shape;
@@ -123,27 +142,21 @@ template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const T
         WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
-    GemvScratch& scratch = c->gemv_scratch[s];
-    if (!scratch.d_attn_pieces) {
-        const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
-        if (rc != WF_OK) return rc;
-        std::shared_ptr<float> pieces;  // and behind them the counters
-        const size_t bytes = (size_t)c->sm_count * (2 * TA_MAX_PIECE * sizeof(float) + sizeof(unsigned int));
-        WF_CUDA(c, make_shared_device(c, pieces, bytes));
-        WF_CUDA(c, cudaMemsetAsync(pieces.get(), 0, bytes, s));
-        scratch.d_attn_pieces = pieces;
-    }
+    const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
     TreeTiles t{};
     t.p = p;
-    t.pieces = scratch.d_attn_pieces.get();
-    t.count = reinterpret_cast<unsigned int*>(t.pieces + (size_t)c->sm_count * 2 * TA_MAX_PIECE);
+    t.c.may_cut = tiles > TA_WHOLE_TILES;
+    t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
+    t.c.dim = Shape::DIM;
+    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
     CUtensorMap k, v;
-    int rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
+    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
     if (rc != WF_OK) return rc;
-    const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
-    const int64_t most = std::min<int64_t>(p.seqs * blocks * p.cache.kv_heads, c->sm_count) * tiles;  // tiles, where there are fewer than SMs
-    return launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, WM>, (unsigned)std::min<int64_t>(most, c->sm_count), TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    const int64_t units = p.seqs * blocks * p.cache.kv_heads, most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
+    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, WM>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, Shape::ROWS, s) : rc;
 }
 
 #define ATTENTION_ENTER(ctxh)                                              \

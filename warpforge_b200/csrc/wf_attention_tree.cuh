@@ -4,11 +4,10 @@
 // heads of the group) are padded to 16 .. 64 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
 // one decoded token fills one to eight.
 //
-// All (sequence, kv head, rows) units, each so many tiles of 16 keys long, form one line that is cut evenly over the SMs.  A CTA's share crosses
-// units; the pieces of a unit that is cut between CTAs are joined by the last of them to finish, in the order of the line.  Inside a CTA four warps
-// walk the line and have TMA fill a ring of tiles ahead, across the ends of units too; teams of eight others take the tiles of a piece in turn.
+// The units are cut as wf_attention_line.cuh says.  Inside a CTA four warps walk its share and have TMA fill a ring of tiles ahead, across the ends of
+// units too; teams of eight others take the tiles of a piece in turn.
 #pragma once
-#include "wf_attention.cuh"
+#include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
 
 namespace wf {
@@ -21,6 +20,7 @@ constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
 constexpr int TA_MERGE_BYTES = 64 * 1024;
 constexpr int TA_SEGMENTS = 2;     // announced ahead
 constexpr int TA_UNIT_TILES = 8;   // what a unit costs beyond its tiles, in tiles
+constexpr int TA_WHOLE_TILES = 40; // units of no more tiles are never cut
 constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
 // CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows a warp, WM warps a team
 template <int CHUNKS, int MT, int WM> struct TreeShape {
@@ -32,26 +32,22 @@ template <int CHUNKS, int MT, int WM> struct TreeShape {
     static constexpr int TURN = TEAMS > TA_LOADERS ? TEAMS : TA_LOADERS, SLOTS = FIT > 32 ? 32 : FIT / TURN * TURN;
     static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TEAMS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TEAMS;  // teams whose sums lie in shared memory at a time
     static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
-    static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory: sums, then maxima, then weights
+    static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory
     static_assert(SETS == TEAMS || 2 * SETS == TEAMS, "one round of folding");
     static_assert(SLOTS >= TEAMS && SLOTS % TEAMS == 0 && SLOTS % TA_LOADERS == 0, "slots for every team and loader");
 };
-constexpr int TA_MAX_PIECE = 64 * (128 + 2);
-
 // What a CTA has of a unit.
 struct alignas(16) TreeSegment {
     int row0, rows, context, seq;  // of the sequence; context < 0: a sequence that cannot be, its rows are zeros
     int head, first;               // first of the sequence's rows * group that the unit has
     int from, to, tiles;           // of the unit
     int slot, phase;               // of the first tile in the ring
-    int first_cta, last_cta;       // that have pieces of it
     int last;                      // no more work
 };
 
 struct TreeTiles {
     TreeParams p;
-    float* pieces;        // [CTAs][2]: the piece a CTA's share begins with, one that starts later in it
-    unsigned int* count;  // [CTAs]: pieces done of the cut unit that begins in this CTA's share; 0 between launches
+    TreeCuts c;
 };
 
 // By the thread whose `issue` is non-zero; the whole warp comes here with the same operands, which then sit in uniform registers (issued by four
@@ -76,12 +72,6 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ta_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 __device__ __forceinline__ void ta_copy16(uint32_t dst, const void* src, bool real) {  // zeros where there is nothing
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
@@ -99,133 +89,79 @@ template <int CHUNKS, int MT, int WM> struct TreeShared {
     TreeSegment segments[TA_SEGMENTS];
     float team_max[Shape::SETS][Shape::ROWS], team_sum[Shape::SETS][Shape::ROWS];
     unsigned long long odd_rows;
-    int last_one;
     int bad_page;  // the segment of this number and those before it have pages outside the cache
 };
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
 template <int CHUNKS, int MT, int WM>
-__device__ __forceinline__ bool tree_walk(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
+__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
     typedef TreeShape<CHUNKS, MT, WM> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
     const TreeParams& p = t.p;
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
-    auto tiles_of = [&](const TreeSeq& q) { return max(1, (q.context + q.rows + TA_KEYS - 1) / TA_KEYS); };
-    auto units_of = [&](const TreeSeq& q) { return heads * ((q.rows * group + ROWS - 1) / ROWS); };
-    auto line_of = [&](const TreeSeq& q) { return q.rows == 0 ? 0 : (int64_t)(tiles_of(q) + TA_UNIT_TILES) * units_of(q); };
-    auto info = [&](int s) {
-        TreeSeq q;
-        q.rows = 0;
-        if (s < p.seqs) q = tree_seq(p, s);
-        return q;
-    };
-    // a lane has a sequence at a time
-    TreeSeq mine = info(lane);
-    int64_t line = line_of(mine), total = line;
-#pragma unroll 1
-    for (int s0 = 32; s0 < p.seqs; s0 += 32) total += line_of(info(s0 + lane));
-#pragma unroll
-    for (int o = 16; o > 0; o >>= 1) total += __shfl_xor_sync(0xFFFFFFFFu, total, o);
-    const int64_t share = total / gridDim.x, more = total % gridDim.x;  // the first `more` CTAs have one position more
-    const int64_t begin = blockIdx.x * share + min((int64_t)blockIdx.x, more), end = begin + share + ((int64_t)blockIdx.x < more);
-    auto cta_of = [&](int64_t x) { return (int)(x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share); };
     const uint32_t issue = elect_one();
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
-    int64_t at = 0;  // where the sequence begins on the line
-    bool ok = true;
-#pragma unroll 1
-    for (int s0 = 0; s0 < p.seqs && at < end && ok; s0 += 32) {
-        if (s0) {
-            mine = info(s0 + lane);
-            line = line_of(mine);
+    bool cut = false;  // a unit that begins here goes on in the next share
+    const bool ok = walk_line<TA_KEYS>(p, ROWS, TA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+        const int keys = u.q.context < 0 ? 0 : u.q.context + u.q.rows, count = min(ROWS, u.q.rows * group - u.first);
+        // the page of a lane's tile, asked for before anything is waited for
+        const int* const table = u.q.place.table;
+        int tile = u.from + lane, page = 0;
+        if (tile < u.to && keys > 0) page = table[tile * TA_KEYS >> p.cache.page_shift];
+        if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
+        if (loader == 0 && lane == 0) {
+            TreeSegment& d = sh->segments[seg];
+            d.row0 = u.q.row0, d.rows = u.q.rows, d.context = u.q.context, d.seq = u.seq, d.head = u.head, d.first = u.first;
+            d.from = u.from, d.to = u.to, d.tiles = u.tiles, d.slot = slot, d.phase = (int)phase ^ 1, d.last = 0;
+            g_mbar_arrive(&sh->seg_full[seg]);
+            if (u.from == 0 && u.to < u.tiles) leave_cut(t.c, u, count);
         }
-        int64_t to_here = line;  // of the sequences up to this lane's
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int64_t v = __shfl_up_sync(0xFFFFFFFFu, to_here, o);
-            if (lane >= o) to_here += v;
+        cut |= u.from == 0 && u.to < u.tiles;
+        __syncwarp();
+        // the queries: rows of 16-byte pieces, swizzled by the row
+        const bf16* q0 = p.q + (size_t)u.q.row0 * p.q_stride + (size_t)u.head * group * p.cache.dim;
+#pragma unroll 1
+        for (int i = loader * 32 + lane; i < ROWS * (DIM / 8); i += 32 * TA_LOADERS) {
+            const int r = i / (DIM / 8), piece = i % (DIM / 8), token = p.token_of(u.first + r);
+            const bool real = r < count && piece * 8 < p.cache.dim;
+            ta_copy16(q_smem + (uint32_t)(seg * Shape::Q_BYTES + r * DIM * 2 + ((piece ^ (r & 7)) << 4)),
+                      real ? q0 + (size_t)token * p.q_stride + (size_t)((u.first + r) - token * group) * p.cache.dim + piece * 8 : p.q, real);
         }
-        const int64_t base = at;
-        at += __shfl_sync(0xFFFFFFFFu, to_here, 31);
-        uint32_t ours = __ballot_sync(0xFFFFFFFFu, line > 0 && base + to_here > begin && base + to_here - line < end);  // sequences that the share touches
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(g_smem_u32(&sh->seg_full[seg])) : "memory");
 #pragma unroll 1
-        for (; ours && ok; ours &= ours - 1) {
-            const int l = __ffs(ours) - 1;
-            TreeSeq q;
-            q.row0 = __shfl_sync(0xFFFFFFFFu, mine.row0, l);
-            q.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, l);
-            q.context = __shfl_sync(0xFFFFFFFFu, mine.context, l);
-            const int64_t start = base + __shfl_sync(0xFFFFFFFFu, to_here - line, l);
-            const int tiles = tiles_of(q), units = units_of(q), length = tiles + TA_UNIT_TILES, blocks = units / heads, keys = q.context < 0 ? 0 : q.context + q.rows;
-            const int* table = p.tables + (size_t)(s0 + l) * p.table_stride;
-            int unit = begin > start ? (int)((begin - start) / length) : 0;
+        for (int t0 = u.from; t0 < u.to; t0 += 32) {
+            if (t0 > u.from) {
+                tile = t0 + lane;
+                page = tile < u.to && keys > 0 ? table[tile * TA_KEYS >> p.cache.page_shift] : 0;
+            }
+            if (page < 0 || page >= p.cache.pages) {  // never followed: the unit's rows go key by key
+                *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                page = 0;
+            }
+            const int z = ((page * heads + u.head) << p.cache.page_shift) + (tile * TA_KEYS & ((1 << p.cache.page_shift) - 1));  // below 2^31: check_cache
+            const int n = min(32, u.to - t0);
 #pragma unroll 1
-            for (int64_t u_at = start + (int64_t)unit * length; unit < units && u_at < end; unit++, u_at += length) {
-                // a unit begins with TA_UNIT_TILES positions that stand for what it costs in any case
-                const int from = (int)max((int64_t)0, begin - u_at - TA_UNIT_TILES), to = (int)min((int64_t)tiles, end - u_at - TA_UNIT_TILES);
-                if (to <= from) continue;
-                const int head = unit / blocks, first = (unit - head * blocks) * ROWS;
-                // the page of a lane's tile, asked for before anything is waited for
-                int tile = from + lane, page = 0;
-                if (tile < to && keys > 0) page = table[tile * TA_KEYS >> p.cache.page_shift];
-                if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
-                const int count = min(ROWS, q.rows * group - first);
-                if (loader == 0 && lane == 0) {
-                    TreeSegment& d = sh->segments[seg];
-                    const bool whole = from == 0 && to == tiles;
-                    d.row0 = q.row0, d.rows = q.rows, d.context = q.context, d.seq = s0 + l, d.head = head, d.first = first;
-                    d.from = from, d.to = to, d.tiles = tiles, d.slot = slot, d.phase = (int)phase ^ 1, d.last = 0;
-                    d.first_cta = whole ? 0 : cta_of(u_at + TA_UNIT_TILES);
-                    d.last_cta = whole ? 0 : cta_of(u_at + length - 1);
-                    g_mbar_arrive(&sh->seg_full[seg]);
-                }
-                __syncwarp();
-                auto queries = [&] {  // rows of 16-byte pieces, swizzled by the row
-                    const bf16* q0 = p.q + (size_t)q.row0 * p.q_stride + (size_t)head * group * p.cache.dim;
-#pragma unroll 1
-                    for (int i = loader * 32 + lane; i < ROWS * (DIM / 8); i += 32 * TA_LOADERS) {
-                        const int r = i / (DIM / 8), piece = i % (DIM / 8), token = p.token_of(first + r);
-                        const bool real = r < count && piece * 8 < p.cache.dim;
-                        ta_copy16(q_smem + (uint32_t)(seg * Shape::Q_BYTES + r * DIM * 2 + ((piece ^ (r & 7)) << 4)),
-                                  real ? q0 + (size_t)token * p.q_stride + (size_t)((first + r) - token * group) * p.cache.dim + piece * 8 : p.q, real);
-                    }
-                    asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(g_smem_u32(&sh->seg_full[seg])) : "memory");
-                };
-#pragma unroll 1
-                for (int t0 = from; t0 < to; t0 += 32) {
-                    if (t0 > from) {
-                        tile = t0 + lane;
-                        page = tile < to && keys > 0 ? table[tile * TA_KEYS >> p.cache.page_shift] : 0;
-                    }
-                    if (page < 0 || page >= p.cache.pages) {  // never followed: the unit's rows go key by key
-                        *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
-                        page = 0;
-                    }
-                    const int z = ((page * heads + head) << p.cache.page_shift) + (tile * TA_KEYS & ((1 << p.cache.page_shift) - 1));  // below 2^31: check_cache
-                    const int n = min(32, to - t0);
-#pragma unroll 1
-                    for (int i = 0; i < n; i++) {
-                        const int row = __shfl_sync(0xFFFFFFFFu, z, i);
-                        if (slot % TA_LOADERS == loader) {
-                            if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
-                            const uint32_t bar = g_smem_u32(&sh->full[slot]), to_slot = ring + (uint32_t)(slot * Shape::SLOT_BYTES);
-                            ta_expect(bar, Shape::SLOT_BYTES, issue);
+            for (int i = 0; i < n; i++) {
+                const int row = __shfl_sync(0xFFFFFFFFu, z, i);
+                if (slot % TA_LOADERS == loader) {
+                    if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
+                    const uint32_t bar = g_smem_u32(&sh->full[slot]), to_slot = ring + (uint32_t)(slot * Shape::SLOT_BYTES);
+                    ta_expect(bar, Shape::SLOT_BYTES, issue);
 #pragma unroll
-                            for (int c = 0; c < 2 * CHUNKS; c++) ta_load(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue);
-                        }
-                        if (++slot == Shape::SLOTS) slot = 0, phase ^= 1;
-                        if (t0 == from && i == min(n, Shape::TEAMS) - 1) queries();  // behind the first tiles, which take longer
-                    }
+                    for (int c = 0; c < 2 * CHUNKS; c++) ta_load(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue);
                 }
-                number++;
-                if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
+                if (++slot == Shape::SLOTS) slot = 0, phase ^= 1;
             }
         }
-    }
-    if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
+        number++;
+        if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
+        return true;
+    });
+    if (!ok || !__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
     if (loader == 0 && lane == 0) {
+        if (t.c.may_cut && !cut) t.c.cuts[blockIdx.x].first_cta = -1;
         sh->segments[seg].last = 1;
         g_mbar_arrive(&sh->seg_full[seg]);
     }
@@ -264,7 +200,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= TA_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_walk<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
+        if (!tree_load<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
@@ -372,7 +308,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                         top = fmaxf(m[i][e], top);
                         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 1));
                         top = fmaxf(top, __shfl_xor_sync(0xFFFFFFFFu, top, 2));
-                        const float keep = ta_ex2((m[i][e] - (top == -INFINITY ? 0.f : top)) * scale);
+                        const float keep = line_ex2((m[i][e] - (top == -INFINITY ? 0.f : top)) * scale);
                         m[i][e] = top;
                         l[i][e] *= keep;
 #pragma unroll
@@ -390,7 +326,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                     const float ref = m[i][e] == -INFINITY ? 0.f : m[i][e] * scale;
 #pragma unroll
                     for (int n = 0; n < 2; n++) {
-                        const float x = ta_ex2(fmaf(s[i][n][2 * e], scale, -ref)), y = ta_ex2(fmaf(s[i][n][2 * e + 1], scale, -ref));
+                        const float x = line_ex2(fmaf(s[i][n][2 * e], scale, -ref)), y = line_ex2(fmaf(s[i][n][2 * e + 1], scale, -ref));
                         l[i][e] += x + y;
                         a[i][2 * n + e] = pack_bf16(x, y);
                     }
@@ -447,7 +383,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                     for (int e = 0; e < 2; e++) {
                         const int r = (part * MT + i) * 16 + g + 8 * e;
                         const float other = sh->team_max[team][r], top = fmaxf(m[i][e], other), ref = top == -INFINITY ? 0.f : top;
-                        const float keep = ta_ex2((m[i][e] - ref) * scale), take = ta_ex2((other - ref) * scale);
+                        const float keep = line_ex2((m[i][e] - ref) * scale), take = line_ex2((other - ref) * scale);
                         m[i][e] = top;
                         l[i][e] = l[i][e] * keep + (quad == 0 ? sh->team_sum[team][r] * take : 0.f);
                         const float2* row = reinterpret_cast<const float2*>(merge + (size_t)(team * ROWS + r) * DIM);
@@ -465,7 +401,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         ta_sync();
         const bool whole = w.from == 0 && w.to == w.tiles;
         // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
-        float* const piece = t.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
+        float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
         auto store = [&](int r, int col, const float4& x, float sum, float top) {  // four elements of a row, or zeros where it sees nothing
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             // a sum of 0 under a maximum: scores so large that rounding m scale alone moves a weight out of range
@@ -487,7 +423,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int c = 0; c < SETS; c++) {
-                const float keep = ta_ex2((tops[c] - ref) * scale);
+                const float keep = line_ex2((tops[c] - ref) * scale);
                 sum += sh->team_sum[c][r] * keep;
                 const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
                 x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
@@ -495,41 +431,10 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             if (whole) {
                 if (4 * n < d) store(r, 4 * n, x, sum, top);
             } else {
-                __stcg(reinterpret_cast<float4*>(piece + r * DIM + 4 * n), x);
+                *reinterpret_cast<float4*>(piece + r * DIM + 4 * n) = x;
                 if (n == 0) {
-                    __stcg(piece + ROWS * DIM + r, top);
-                    __stcg(piece + ROWS * (DIM + 1) + r, sum);
-                }
-            }
-        }
-        if (!whole) {
-            __threadfence();
-            ta_sync();
-            if (tid == 0) {
-                sh->last_one = atomicAdd(&t.count[w.first_cta], 1u) == (unsigned)(w.last_cta - w.first_cta);
-                if (sh->last_one) t.count[w.first_cta] = 0;
-                __threadfence();
-            }
-            ta_sync();
-            if (sh->last_one) {
-                auto piece_of = [&](int c) { return t.pieces + ((size_t)c * 2 + (c == w.first_cta)) * Shape::PIECE; };
-#pragma unroll 1
-                for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
-                    const int r = i / PER_ROW, n = i % PER_ROW;
-                    float top = -INFINITY, sum = 0.f;
-                    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll 4
-                    for (int c = w.first_cta; c <= w.last_cta; c++) {  // the maximum followed on the way: all loads of a few pieces in flight at once
-                        const float* from = piece_of(c);
-                        const float4 v = __ldcg(reinterpret_cast<const float4*>(from + r * DIM + 4 * n));
-                        const float m_c = __ldcg(from + ROWS * DIM + r), l_c = __ldcg(from + ROWS * (DIM + 1) + r);
-                        const float grown = fmaxf(top, m_c), ref = grown == -INFINITY ? 0.f : grown;
-                        const float keep = ta_ex2((top - ref) * scale), take = ta_ex2((m_c - ref) * scale);
-                        top = grown;
-                        sum = sum * keep + l_c * take;
-                        x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
-                    }
-                    if (4 * n < d) store(r, 4 * n, x, sum, top);
+                    piece[ROWS * DIM + r] = top;
+                    piece[ROWS * (DIM + 1) + r] = sum;
                 }
             }
         }

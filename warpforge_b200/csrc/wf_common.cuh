@@ -115,7 +115,8 @@ struct GemvScratch {
     std::shared_ptr<unsigned int> d_gemm_ready;  // [sm_count][4] generation whose piece is complete, per 32-row quarter; then {generation, CTAs out}
     // attention
     std::shared_ptr<unsigned int> d_attn_sched;  // counters of the prompt kernel, 0 between launches
-    std::shared_ptr<float> d_attn_pieces;        // tree kernel: sums of units that are cut between CTAs, and counters, 0 between launches
+    std::shared_ptr<uint8_t> d_attn;             // tree kernels: units that are cut between CTAs, and their pieces
+    int64_t attn_bytes = 0;
 };
 // cudaMalloc for everything that a context allocates: where memory is short, its kept tile buffers go first.
 cudaError_t device_alloc(Context* c, void** p, size_t bytes);
