@@ -274,6 +274,23 @@ def test_tree_drafts(backend, drafts, page):
     run_tree(backend, [1037, 20, 3], drafts, 4, 4, 64, page, shape="chain")
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(8, 1, 128), (16, 2, 64), (3, 1, 96), (64, 1, 128)])
+@pytest.mark.parametrize("lens,drafts", [([3000, 700], [64, 40]), ([255, 128, 0, 1100], [9, 33, 17, 1]), ([129], [64])])
+def test_tree_many_rows(backend, q_heads, kv_heads, dim, lens, drafts):
+    """More rows than one tile, cut units and whole ones, key tiles that two groups share."""
+    run_tree(backend, lens, drafts, q_heads, kv_heads, dim, 32)
+
+
+def test_tree_many_rows_long_context(backend):
+    run_tree(backend, [70001], [7], 8, 1, 128, 128)
+    run_tree(backend, [9000, 8000], [20, 64], 4, 1, 64, 16)
+
+
+def test_tree_many_units_of_many_rows(backend):
+    rng = np.random.default_rng(15)
+    run_tree(backend, [int(n) for n in rng.integers(0, 400, 60)], [int(n) for n in rng.integers(1, 65, 60)], 8, 2, 64, 16)
+
+
 def test_tree_defaults(backend):
     """Without offsets and words: every sequence has max_drafts tokens, a chain."""
     run_tree(backend, [100, 333, 5], [4, 4, 4], 4, 2, 64, 16, shape="chain", arrays=False)

@@ -89,7 +89,7 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     const char* what = "prompt_attention";
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
+        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
     GemvScratch& scratch = c->gemv_scratch[s];
@@ -112,7 +112,7 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
     if (rc != WF_OK) return rc;
     const int64_t items = (p.tokens / (2 * t.tile_tokens) + p.seqs) * p.cache.kv_heads;
-    return launch_attention(c, what, prompt_tiles_kernel<CHUNKS>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
+    return launch_attention(c, what, prompt_tiles_kernel<CHUNKS, false>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
 
 // Where the pieces of cut units go.
@@ -157,6 +157,41 @@ template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const T
     const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
     rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, WM>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
     return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, Shape::ROWS, s) : rc;
+}
+
+// The prompt kernel on the rows of trees.
+template <int CHUNKS> static int launch_wide_tree(Context* c, const TreeParams& p, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    PromptTiles t{};
+    t.tree = p;
+    t.p.cache = p.cache;
+    t.p.q = p.q, t.p.out = p.out, t.p.q_stride = p.q_stride;
+    t.p.tables = p.tables, t.p.table_stride = p.table_stride;
+    t.p.q_heads = p.q_heads, t.p.group = p.group;
+    t.p.scale_log2 = p.scale_log2;
+    t.p.status = p.status;
+    t.tile_tokens = PA_ROWS / p.group;
+    t.box_rows = std::min(PA_KEYS, 1 << p.cache.page_shift);
+    const int64_t blocks = (p.max_drafts + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens), tiles = (p.max_context + p.max_drafts + PA_KEYS - 1) / PA_KEYS;
+    t.c.may_cut = tiles > PA_WHOLE_TILES;
+    t.c.piece_rows = p.max_drafts <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;
+    t.c.tile_rows = t.tile_tokens * p.group;
+    t.c.tile_room = PA_ROWS;
+    t.c.dim = CHUNKS * 64;
+    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * t.c.piece_rows * (t.c.dim + 2) : 0, &t.c);
+    CUtensorMap q, k, v;
+    if (rc == WF_OK) rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
+    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
+    if (rc != WF_OK) return rc;
+    const int64_t units = p.seqs * blocks * p.cache.kv_heads, most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
+    rc = launch_attention(c, "tree_attention", prompt_tiles_kernel<CHUNKS, true>, grid, PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, std::min(p.max_drafts, 2 * t.tile_tokens) * p.group, s) : rc;
 }
 
 #define ATTENTION_ENTER(ctxh)                                              \
@@ -240,9 +275,10 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     p.group_inverse = p.group == 1 ? 0 : (uint32_t)(((1ull << 32) + p.group - 1) / p.group);
     p.scale_log2 = a->scale * 1.44269504f;
     p.status = c->d_status;
-    const int rows = a->max_drafts * p.group;  // of a sequence and kv head: the smallest block of rows that holds them, 64 at most
-    if (dim_chunks(cache->head_dim) == 1) return rows <= 16 ? launch_tree<1, 1, 1>(c, p, s) : rows <= 32 ? launch_tree<1, 2, 1>(c, p, s) : launch_tree<1, 2, 2>(c, p, s);
-    return rows <= 16 ? launch_tree<2, 1, 1>(c, p, s) : rows <= 32 ? launch_tree<2, 2, 1>(c, p, s) : launch_tree<2, 2, 2>(c, p, s);
+    const int rows = a->max_drafts * p.group, chunks = dim_chunks(cache->head_dim);  // rows of a sequence and kv head
+    if (rows > 32) return chunks == 1 ? launch_wide_tree<1>(c, p, s) : launch_wide_tree<2>(c, p, s);
+    if (chunks == 1) return rows <= 16 ? launch_tree<1, 1, 1>(c, p, s) : launch_tree<1, 2, 1>(c, p, s);
+    return rows <= 16 ? launch_tree<2, 1, 1>(c, p, s) : launch_tree<2, 2, 1>(c, p, s);
 }
 
 }  // extern "C"

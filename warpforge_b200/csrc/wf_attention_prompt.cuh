@@ -1,14 +1,14 @@
-// Attention over whole prompts on the 5th-generation tensor cores.
+// Attention on the 5th-generation tensor cores: whole prompts, and trees of drafted tokens with many rows.
 //
 //   S = Q K^T   [128 rows x 128 keys] fp32 in TMEM, Q and K in shared memory
 //   P = 2^(S scale log2 e - m)        bf16, written over S in TMEM
 //   O += P V    [128 rows x dim] fp32 in TMEM, P in TMEM, V in shared memory
 //
 // A CTA works on two tiles of rows of one kv head at a time, so that the tensor core has the one tile's products to do while the other
-// tile's exponentials are taken.  The rows of a tile are the heads of the group for some tokens, token by token: keys and values are read once
+// tile's exponentials are taken; where there is one tile of rows, on every other tile of keys of it in turn.  The rows of a tile are the heads of the group for some tokens, token by token: keys and values are read once
 // for the whole group.  A thread of the softmax warps has a row: its maximum and sum need no exchange.
 #pragma once
-#include "wf_attention.cuh"
+#include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
 
 namespace wf {
@@ -33,21 +33,34 @@ struct PromptItem {
     int seq, head;
     int row0, rows, keys;  // of the sequence
     int token0;            // first token of tile 0
-    int n0, n1;            // key tiles that the tiles see
+    int from, n0, n1;      // key tiles: the first, and where the tiles of rows end
+    int split;             // one tile of rows: both groups work on it, n0 is where it ends, group g takes the key tiles from + g, from + g + 2, ..
+    int context;           // tree: tokens before the new ones, -1: a sequence that cannot be
+    int piece;             // tree: the unit is cut; 1: this piece is not the one it begins with, 2: it is
     int last;              // no more work (1), or a wait ran out
+    // key tiles of group g
+    __device__ __forceinline__ int tiles(int g) const { return split ? (n0 - from - g + 1) >> 1 : max(0, (g ? n1 : n0) - from); }
+    __device__ __forceinline__ int all() const { return max(n0, n1) - from; }
 };
 
 struct PromptTiles {
     PromptParams p;
     int tile_tokens;   // tokens of a tile: 128 / group
     int box_rows;      // rows of keys that one TMA load brings: those of a page, at most 128
-    unsigned int* sched;  // [0] items taken beyond the first of each CTA, [1] CTAs that are done
+    unsigned int* sched;  // prompt: [0] items taken beyond the first of each CTA, [1] CTAs that are done
+    TreeParams tree;
+    TreeCuts c;
 };
 
-__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, void* bar) {
-    asm volatile("cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];" ::"r"(dst), "l"(map), "r"(x),
-                 "r"(y), "r"(z), "r"(g_smem_u32(bar))
+// By the thread whose `issue` is non-zero; the whole warp comes here with the same operands, which then sit in uniform registers.
+__device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar, uint32_t issue) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+                 "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(bar), "r"(issue)
                  : "memory");
+}
+__device__ __forceinline__ void mbar_expect_if(uint32_t bar, uint32_t bytes, uint32_t issue) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %2, 0;\n\t@e mbarrier.arrive.expect_tx.shared::cta.b64 _, [%0], %1;\n\t}" ::"r"(bar), "r"(bytes), "r"(issue) : "memory");
 }
 // Operand of 16-bit elements with the other dimension contiguous (V: a row is a key, its elements run along N), 128-byte swizzle: 64 elements x 8
 // rows are 1024 bytes, the next 8 rows follow, the next 64 elements lie `chunk` bytes on.
@@ -137,6 +150,8 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) { return
 struct PromptShared {
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t half_ready, half_taken;  // tree, one tile of rows: the second group's maxima and sums lie in half_max and half_sum; they and its O have been read
+    float half_max[PA_ROWS], half_sum[PA_ROWS];
     uint64_t kv_full[PA_MAX_STAGES], kv_empty[PA_MAX_STAGES];
     uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
     PromptItem items[PA_ITEMS];
@@ -231,6 +246,7 @@ struct PromptSchedule {
             const int last = q.keys - q.rows + min(q.rows, token + t.tile_tokens) - 1;
             return last < 0 ? 0 : last / PA_KEYS + 1;
         };
+        it.from = it.split = it.piece = 0;
         it.n0 = tiles(it.token0);
         it.n1 = tiles(it.token0 + t.tile_tokens);
         it.last = 0;
@@ -238,7 +254,33 @@ struct PromptSchedule {
     }
 };
 
-template <int CHUNKS>
+// The items of a CTA's share of a tree call.
+constexpr int PA_UNIT_TILES = 2;    // what a unit costs beyond its key tiles, in key tiles
+constexpr int PA_WHOLE_TILES = 5;   // units of no more key tiles are never cut
+template <class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
+    const TreeParams& p = t.tree;
+    bool cut = false;
+    const bool ok = walk_line<PA_KEYS>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+        PromptItem it{};
+        it.seq = u.seq, it.head = u.head, it.row0 = u.q.row0, it.rows = u.q.rows, it.context = u.q.context;
+        it.keys = u.q.context < 0 ? 0 : u.q.context + u.q.rows;
+        it.token0 = u.first / p.group;
+        it.from = u.from;
+        it.n0 = u.to;
+        it.split = it.rows - it.token0 <= t.tile_tokens;
+        it.n1 = it.split ? u.from : u.to;
+        it.piece = u.from == 0 && u.to == u.tiles ? 0 : u.from == 0 ? 2 : 1;
+        if (it.piece == 2) {
+            cut = true;
+            if ((threadIdx.x & 31) == 0) leave_cut(t.c, u, min(2 * t.tile_tokens, it.rows - it.token0) * p.group);
+        }
+        return f(it);
+    });
+    if (t.c.may_cut && !cut && (threadIdx.x & 31) == 0) t.c.cuts[blockIdx.x].first_cta = -1;
+    return ok;
+}
+
+template <int CHUNKS, bool TREE>
 __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __grid_constant__ PromptTiles t, const __grid_constant__ CUtensorMap q_map,
                                                                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
     constexpr int DIM = CHUNKS * 64, STAGES = PromptShape<CHUNKS>::STAGES, STAGE_BYTES = PromptShape<CHUNKS>::STAGE_BYTES;
@@ -259,6 +301,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             g_mbar_init(&sh->p_full[g], 4);
             g_mbar_init(&sh->o_full[g], 1);
         }
+        g_mbar_init(&sh->half_ready, 4);
+        g_mbar_init(&sh->half_taken, 4);
         for (int i = 0; i < STAGES; i++) {
             g_mbar_init(&sh->kv_full[i], 1);
             g_mbar_init(&sh->kv_empty[i], 1);
@@ -292,14 +336,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         const int group = p.group, tile_tokens = t.tile_tokens;
         const int my_token = r / group, my_head = r % group;
         const float scale = p.scale_log2;
-        uint32_t s_phase = 0, o_phase = 0;
+        uint32_t s_phase = 0, o_phase[2] = {0, 0}, half_phase = 0;
         for (int number = 0; items.next(sh, it, failed); number++) {
-            const int n = g ? it.n1 : it.n0, first = it.token0 + g * tile_tokens, token = first + my_token;
+            const int n = it.tiles(g), step = TREE && it.split ? 2 : 1;
+            const int first = it.token0 + (TREE && it.split ? 0 : g * tile_tokens), token = first + my_token;
             const bool mine = r < group * tile_tokens && token < it.rows;
-            const int last_key = it.keys - it.rows + token;  // that the row sees
-            const int all_see = it.keys - it.rows + first + (warp & 3) * 32 / group;  // that every row of this warp sees
+            const int last_key = it.keys - it.rows + token;  // prompt: that the row sees
+            const int all_see = TREE ? it.context - 1 : it.keys - it.rows + first + (warp & 3) * 32 / group;  // that every row of this warp sees
+            const uint64_t word = TREE && mine && it.keys > 0 ? ancestors_of(t.tree, it.row0 + token, token) & ((uint64_t)-1 >> (64 - it.rows)) : 0;
             float m = -INFINITY, l = 0.f;
-            for (int j = 0; j < n; j++) {
+            int j = it.from + (TREE && it.split ? g : 0);  // the key tile
+            for (int i_tile = 0; i_tile < n; i_tile++, j += step) {
                 if (!pa_wait(&sh->s_full[g], s_phase)) {
                     failed = true;
                     break;
@@ -311,10 +358,24 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 for (int c = 0; c < 4; c++) tmem_ld32_start(s_at + 32 * c, s + 32 * c);
                 tmem_wait_ld();
                 if (j * PA_KEYS + PA_KEYS - 1 > all_see) {  // keys that some row of the warp does not see
-                    const int limit = last_key - j * PA_KEYS;
+                    if (TREE) {
+                        // bit i of the four words: the row sees key i of the tile.  Below `old` it does, from there on the ancestors say so.
+                        const int old = it.context - j * PA_KEYS;
 #pragma unroll
-                    for (int i = 0; i < PA_KEYS; i++)
-                        if (i > limit) s[i] = 0xFF800000u;
+                        for (int c = 0; c < 4; c++) {
+                            const int at = old - 32 * c;  // where the word begins, seen from this one
+                            uint32_t bits = it.context < 0 || at <= 0 ? 0u : at >= 32 ? 0xFFFFFFFFu : (1u << at) - 1;
+                            if (at > -64 && at < 32) bits |= at >= 0 ? (uint32_t)(word << at) : (uint32_t)(word >> -at);
+#pragma unroll
+                            for (int i = 0; i < 32; i++)
+                                if (!(bits >> i & 1)) s[32 * c + i] = 0xFF800000u;
+                        }
+                    } else {
+                        const int limit = last_key - j * PA_KEYS;
+#pragma unroll
+                        for (int i = 0; i < PA_KEYS; i++)
+                            if (i > limit) s[i] = 0xFF800000u;
+                    }
                 }
                 float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
@@ -322,7 +383,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
 #pragma unroll
                     for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[i + 2 * e])), __uint_as_float(s[i + 2 * e + 1]));
                 const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
-                if (j == 0) {
+                if (i_tile == 0) {
                     m = tile_top;
                 } else if (__any_sync(0xFFFFFFFFu, (tile_top - m) * scale > PA_RESCALE)) {
                     // O is at rest: the MMAs that made it ran before those that made S
@@ -368,20 +429,80 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             bf16* const to = p.out + ((size_t)row * p.q_heads + head) * p.cache.dim;
             const int d = p.cache.dim;
             bool odd = false;  // something is not finite
-            if (n > 0) {
-                if (!pa_wait(&sh->o_full[g], o_phase)) {
+            const bool halves = TREE && it.split && it.tiles(1) > 0;
+            if (n > 0 || (halves && g == 0)) {
+                if (!pa_wait(&sh->o_full[g], o_phase[g])) {
                     failed = true;
                     break;
                 }
-                o_phase ^= 1;
+                o_phase[g] ^= 1;
                 tc_fence_after();
+            }
+            if (TREE && g == 0 && !halves && it.tiles(1) > 0) o_phase[1] ^= 1;  // the other group's
+            if (TREE && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l = __uint_as_float(0x7FC00000u);
+            if (halves && g == 1) {  // the first group adds both halves up
+                sh->half_max[r] = m;
+                sh->half_sum[r] = l;
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(&sh->half_ready);
+                if (!pa_wait(&sh->half_taken, half_phase)) {
+                    failed = true;
+                    break;
+                }
+                half_phase ^= 1;
+                continue;
+            }
+            float keep = 1.f, take = 0.f, top = m;
+            if (halves) {
+                if (!pa_wait(&sh->half_ready, half_phase) || !pa_wait(&sh->o_full[1], o_phase[1])) {
+                    failed = true;
+                    break;
+                }
+                half_phase ^= 1;
+                o_phase[1] ^= 1;
+                tc_fence_after();
+                const float m1 = sh->half_max[r];
+                top = fmaxf(m, m1);
+                const float ref = top == -INFINITY ? 0.f : top;
+                keep = ex2((m - ref) * scale), take = ex2((m1 - ref) * scale);
+                l = l * keep + sh->half_sum[r] * take;
+            }
+            // the row's sums, 32 at a time
+            auto sums = [&](int c, uint32_t(&o)[32]) {
+                tmem_ld32_start(o_at + c, o);
+                tmem_wait_ld();
+                if (halves) {
+                    uint32_t o1[32];
+                    tmem_ld32_start(o_at + DIM + c, o1);
+                    tmem_wait_ld();
+#pragma unroll
+                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep + __uint_as_float(o1[i]) * take);
+                }
+            };
+            if (TREE && it.piece && (n > 0 || !it.split)) {
+                const int rows = t.c.piece_rows, at = (it.split ? 0 : g * PA_ROWS) + r;
+                float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
+                if (r < group * tile_tokens) {
+                    piece[rows * DIM + at] = n > 0 ? top : -INFINITY;
+                    piece[rows * (DIM + 1) + at] = n > 0 ? l : 0.f;
+                }
+#pragma unroll 1
+                for (int c = 0; c < DIM; c += 32) {
+                    uint32_t o[32];
+                    sums(c, o);
+                    if (mine)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<float4*>(piece + (size_t)at * DIM + c + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
+                }
+                tc_fence_before();
+            } else if (n > 0) {
                 const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-                odd = !(l < INFINITY) || (l == 0.f && m > -INFINITY);  // scores so large that rounding m scale alone moves a weight out of range
+                odd = !(l < INFINITY) || (l == 0.f && top > -INFINITY);  // the latter: scores so large that rounding m scale alone moves a weight out of range
 #pragma unroll
                 for (int c = 0; c < DIM; c += 32) {
                     uint32_t o[32];
-                    tmem_ld32_start(o_at + c, o);
-                    tmem_wait_ld();
+                    sums(c, o);
                     uint32_t largest = 0;
 #pragma unroll
                     for (int i = 0; i < 32; i++) largest = max(largest, o[i] & 0x7FFFFFFFu);
@@ -397,12 +518,16 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     }
                 }
                 tc_fence_before();
-            } else if (mine) {
+            } else if (!TREE && mine) {
                 for (int i = 0; i < d; i += 8) *reinterpret_cast<uint4*>(to + i) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (halves) {
+                __syncwarp();
+                if (lane == 0) g_mbar_arrive(&sh->half_taken);
             }
             // Rows with an Inf or a NaN in their sums, and rows whose pages are not in the cache, go key by key: the first may have
             // come from a key that the row does not see (0 x Inf), the second's keys were not read.
-            odd |= *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
+            if (!TREE) odd |= *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
             uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && odd);
             while (again) {
                 const int l2 = __ffs(again) - 1;
@@ -411,72 +536,82 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 KeyPlace place;
                 place.table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
                 place.first = it.row0;
-                attend_row(p.cache, place, p.q + (size_t)(it.row0 + tok) * p.q_stride + (size_t)hd * d, p.out + ((size_t)(it.row0 + tok) * p.q_heads + hd) * d,
-                           it.head, min(it.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
+                const bf16* q_row = p.q + (size_t)(it.row0 + tok) * p.q_stride + (size_t)hd * d;
+                bf16* out_row = p.out + ((size_t)(it.row0 + tok) * p.q_heads + hd) * d;
+                if (TREE)
+                    attend_row(p.cache, place, q_row, out_row, it.head, it.keys, p.scale_log2, p.status,
+                               SeesAncestors{it.context, ancestors_of(t.tree, it.row0 + tok, tok) & ((uint64_t)-1 >> (64 - it.rows))});
+                else attend_row(p.cache, place, q_row, out_row, it.head, min(it.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
             }
         }
     } else if (warp == PA_LOAD_WARP) {
+        const uint32_t issue = elect_one();
         StageCursor ring;
         uint32_t q_phase[2] = {1, 1};
+        const int boxes = PA_KEYS / t.box_rows;
         for (int number = 0; items.next(sh, it, failed); number++) {
-            const int n = max(it.n0, it.n1);
+            const int n = it.all();
             const int* table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
-            const int boxes = PA_KEYS / t.box_rows;
-            for (int j = 0; j < n && !failed; j++) {
-                // the rows of this tile's boxes, a lane each
-                int z = it.row0 + j * PA_KEYS, valid = 1;
-                const int y = table ? 0 : it.head;
-                if (table) {
-                    const int key = j * PA_KEYS + lane * t.box_rows;
-                    valid = 0;
-                    if (lane < boxes && key < it.keys) {
-                        int page = table[key >> p.cache.page_shift];
-                        if (page < 0 || page >= p.cache.pages) {  // never followed: these rows go key by key
-                            report_status(p.status, STATUS_BAD_INDEX);
-                            *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
-                            page = 0;
-                        }
-                        z = (int)((((int64_t)page * p.cache.kv_heads + it.head) << p.cache.page_shift) + (key & ((1 << p.cache.page_shift) - 1)));
-                        valid = 1;
-                    }
-                } else if (lane > 0) valid = 0;
-                const int loads = __popc(__ballot_sync(0xFFFFFFFFu, valid));
+            // the rows of a key tile's boxes, a lane each, and how many there are
+            auto find = [&](int j, int& z) {
+                if (!table) {
+                    z = it.row0 + j * PA_KEYS;
+                    return 1;
+                }
+                const int key = j * PA_KEYS + lane * t.box_rows;
+                int page = 0;
+                const bool valid = lane < boxes && (key < it.keys || (TREE && lane == 0));  // a sequence that cannot be reads something, and sees nothing
+                if (valid && key < it.keys) page = table[key >> p.cache.page_shift];
+                if (page < 0 || page >= p.cache.pages) {  // never followed: these rows go key by key
+                    report_status(p.status, STATUS_BAD_INDEX);
+                    *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                    page = 0;
+                }
+                z = (int)((((int64_t)page * p.cache.kv_heads + it.head) << p.cache.page_shift) + (key & ((1 << p.cache.page_shift) - 1)));
+                return __popc(__ballot_sync(0xFFFFFFFFu, valid));
+            };
+            auto load = [&](const CUtensorMap* map, int z, int loads) {
+                if (!pa_wait(&sh->kv_empty[ring.s], ring.phase ^ 1)) {
+                    failed = true;
+                    return;
+                }
+                const uint32_t bar = g_smem_u32(&sh->kv_full[ring.s]);
+                mbar_expect_if(bar, (uint32_t)(loads * CHUNKS * 128 * t.box_rows), issue);
+                for (int i = 0; i < loads; i++) {
+                    const int row = __shfl_sync(0xFFFFFFFFu, z, i);
+#pragma unroll
+                    for (int c = 0; c < CHUNKS; c++)
+                        tma_load_3d(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + i * t.box_rows * 128), map, 64 * c, table ? 0 : it.head, row, bar, issue);
+                }
+                ring.advance(STAGES);
+            };
+            int z = 0, z_before = 0, loads = 0, loads_before = 0;
+            for (int j = 0; j < n && !failed; j++) {  // keys 0, keys 1, values 0, keys 2, values 1, ..
+                loads = find(it.from + j, z);
                 if (j == 0)
                     for (int g = 0; g < 2; g++) {
-                        if ((g ? it.n1 : it.n0) == 0) continue;
+                        if (it.tiles(g) == 0) continue;
                         if (!pa_wait(&sh->q_empty[g], q_phase[g])) failed = true;
                         q_phase[g] ^= 1;
                         if (failed) break;
-                        if (lane == 0) {
-                            g_mbar_expect_tx(&sh->q_full[g], (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens));
-                            for (int c = 0; c < CHUNKS; c++)
-                                tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, it.row0 + it.token0 + g * t.tile_tokens, &sh->q_full[g]);
-                        }
-                        __syncwarp();
+                        const uint32_t bar = g_smem_u32(&sh->q_full[g]);
+                        mbar_expect_if(bar, (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens), issue);
+                        const int first = it.row0 + it.token0 + (TREE && it.split ? 0 : g * t.tile_tokens);
+#pragma unroll
+                        for (int c = 0; c < CHUNKS; c++) tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, first, bar, issue);
                     }
-                for (int kv = 0; kv < 2 && !failed; kv++) {
-                    if (!pa_wait(&sh->kv_empty[ring.s], ring.phase ^ 1)) {
-                        failed = true;
-                        break;
-                    }
-                    if (lane == 0) g_mbar_expect_tx(&sh->kv_full[ring.s], (uint32_t)(loads * CHUNKS * 128 * t.box_rows));
-                    __syncwarp();
-                    if (valid)
-                        for (int c = 0; c < CHUNKS; c++)
-                            tma_load_3d(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + lane * t.box_rows * 128), kv ? &v_map : &k_map, 64 * c, y, z, &sh->kv_full[ring.s]);
-                    ring.advance(STAGES);
-                }
+                if (!failed) load(&k_map, z, loads);
+                if (j > 0 && !failed) load(&v_map, z_before, loads_before);
+                z_before = z;
+                loads_before = loads;
             }
+            if (n > 0 && !failed) load(&v_map, z_before, loads_before);
             if (failed) break;
         }
     } else if (warp == PA_MMA_WARP) {
         const uint32_t issue = elect_one();
-        StageCursor ring;
         uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-        auto after = [](StageCursor c) {
-            c.advance(STAGES);
-            return c;
-        };
+        int base = 0;  // loads before this item, modulo two laps of the ring
         auto scores = [&](int g, int stage) {
             const uint64_t a = smem_desc_sw128(smem + (uint32_t)(g * CHUNKS * PA_CHUNK)), b = smem_desc_sw128(kv_smem + (uint32_t)(stage * STAGE_BYTES));
 #pragma unroll
@@ -485,106 +620,130 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             tc_commit_if(&sh->s_full[g], issue);
         };
         while (items.next(sh, it, failed)) {
-            const int n = max(it.n0, it.n1), nt[2] = {it.n0, it.n1};
-            const bool tail = n > 0 && n * PA_KEYS > it.keys;
+            const int n = it.all(), nt[2] = {it.tiles(0), it.tiles(1)};
             if (n == 0) continue;
-            // ring: keys of tile 0, values of tile 0, keys of tile 1, values of tile 1, ...
-            if (!pa_wait(&sh->kv_full[ring.s], ring.phase)) failed = true;
-            for (int g = 0; g < 2 && !failed; g++) {
-                if (nt[g] == 0) continue;
-                if (!pa_wait(&sh->q_full[g], q_phase[g])) {
-                    failed = true;
-                    break;
-                }
+            const bool split = TREE && it.split, tail = max(it.n0, it.n1) * PA_KEYS > it.keys;
+            // the stage of the keys or values of key tile j, once they are there; -1: the wait ran out
+            auto stage_of = [&](bool values, int j) {
+                const int at = base + (values ? (j + 1 < n ? 2 * j + 2 : 2 * n - 1) : (j ? 2 * j - 1 : 0)), stage = at % STAGES;
+                if (!pa_wait(&sh->kv_full[stage], (uint32_t)(at / STAGES) & 1)) failed = true;
+                tc_fence_after();
+                return stage;
+            };
+            auto queries = [&](int g) {
+                if (!pa_wait(&sh->q_full[g], q_phase[g])) failed = true;
                 q_phase[g] ^= 1;
                 tc_fence_after();
-                scores(g, ring.s);
+            };
+            auto products = [&](int g, int stage, bool accumulate) {  // O += P V
+                if (!pa_wait(&sh->p_full[g], p_phase[g])) {
+                    failed = true;
+                    return;
+                }
+                p_phase[g] ^= 1;
+                tc_fence_after();
+                const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(stage * STAGE_BYTES), PA_CHUNK);
+#pragma unroll
+                for (int h = 0; h < 2; h++)
+                    pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, accumulate || h > 0, issue);
+            };
+            auto zero_tail = [&](int stage, int j) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
+                if (!tail || j != n - 1) return;
+                for (int c = 0; c < CHUNKS; c++)
+                    for (int i = max(0, it.keys - (it.from + j) * PA_KEYS) * 8 + lane; i < PA_KEYS * 8; i += 32)
+                        asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv_smem + (uint32_t)(stage * STAGE_BYTES + c * PA_CHUNK + i * 16)), "r"(0) : "memory");
+                asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+                __syncwarp();
+            };
+            const int first_keys = stage_of(false, 0);
+            for (int g = 0; g < 2 && !failed; g++) {
+                if (nt[g] == 0) continue;
+                queries(g);
+                const int stage = split && g ? stage_of(false, 1) : first_keys;
+                if (failed) break;
+                scores(g, stage);
                 if (nt[g] == 1) tc_commit_if(&sh->q_empty[g], issue);
+                if (split) tc_commit_if(&sh->kv_empty[stage], issue);
             }
             if (failed) break;
-            tc_commit_if(&sh->kv_empty[ring.s], issue);
-            ring.advance(STAGES);
+            if (!split) tc_commit_if(&sh->kv_empty[first_keys], issue);
             for (int j = 0; j < n && !failed; j++) {
-                const StageCursor v = ring, k = after(v);
-                bool have_v = false, have_k = false;
+                const int values = stage_of(true, j);
+                if (failed) break;
+                zero_tail(values, j);
+                if (split) {  // group j & 1 alone, whose next key tile is j + 2
+                    const int g = j & 1;
+                    products(g, values, j >= 2);
+                    if (failed) break;
+                    tc_commit_if(&sh->kv_empty[values], issue);
+                    if (j + 2 >= n) {
+                        tc_commit_if(&sh->o_full[g], issue);
+                        continue;
+                    }
+                    const int keys = stage_of(false, j + 2);
+                    if (failed) break;
+                    scores(g, keys);
+                    tc_commit_if(&sh->kv_empty[keys], issue);
+                    if (j + 4 >= n) tc_commit_if(&sh->q_empty[g], issue);
+                    continue;
+                }
+                int keys = -1;
                 for (int g = 0; g < 2; g++) {
                     if (j >= nt[g]) continue;
-                    if (!have_v) {
-                        have_v = true;
-                        if (!pa_wait(&sh->kv_full[v.s], v.phase)) {
-                            failed = true;
-                            break;
-                        }
-                        if (tail && j == n - 1) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
-                            for (int c = 0; c < CHUNKS; c++)
-                                for (int i = (it.keys - j * PA_KEYS) * 8 + lane; i < PA_KEYS * 8; i += 32)
-                                    asm volatile("st.shared.v4.b32 [%0], {%1, %1, %1, %1};" ::"r"(kv_smem + (uint32_t)(v.s * STAGE_BYTES + c * PA_CHUNK + i * 16)), "r"(0) : "memory");
-                            asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-                            __syncwarp();
-                        }
-                    }
-                    if (!pa_wait(&sh->p_full[g], p_phase[g])) {
-                        failed = true;
-                        break;
-                    }
-                    p_phase[g] ^= 1;
-                    tc_fence_after();
-                    const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(v.s * STAGE_BYTES), PA_CHUNK);
-#pragma unroll
-                    for (int h = 0; h < 2; h++)
-                        pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, (j | h) > 0, issue);
+                    products(g, values, j > 0);
+                    if (failed) break;
                     if (j + 1 == nt[g]) {
                         tc_commit_if(&sh->o_full[g], issue);
                         continue;
                     }
-                    if (!have_k) {
-                        have_k = true;
-                        if (!pa_wait(&sh->kv_full[k.s], k.phase)) {
-                            failed = true;
-                            break;
-                        }
-                        tc_fence_after();
-                    }
-                    scores(g, k.s);
+                    if (keys < 0) keys = stage_of(false, j + 1);
+                    if (failed) break;
+                    scores(g, keys);
                     if (j + 2 == nt[g]) tc_commit_if(&sh->q_empty[g], issue);
                 }
                 if (failed) break;
-                tc_commit_if(&sh->kv_empty[v.s], issue);
-                ring.advance(STAGES);
-                if (j + 1 < n) {
-                    tc_commit_if(&sh->kv_empty[k.s], issue);
-                    ring.advance(STAGES);
-                }
+                tc_commit_if(&sh->kv_empty[values], issue);
+                if (keys >= 0) tc_commit_if(&sh->kv_empty[keys], issue);
             }
             if (failed) break;
+            base = (base + 2 * n) % (2 * STAGES);
         }
     } else if (warp == PA_SCHED_WARP) {
-        PromptSchedule schedule{t};
-        schedule.begin();
-        int64_t i = blockIdx.x;
         int slot = 0;
         uint32_t phase = 1;
-        for (bool more = true; more;) {
-            it = PromptItem{};
-            it.last = 1;
-            more = schedule.find(i, it);
-            unsigned int ahead = 0;
-            if (more && lane == 0) ahead = atomicAdd(&t.sched[0], 1u);
+        auto announce = [&](const PromptItem& item) {
             if (!pa_wait(&sh->item_empty[slot], phase)) {
                 failed = true;
-                break;
+                return false;
             }
             if (lane == 0) {
-                sh->items[slot] = it;
+                sh->items[slot] = item;
                 g_mbar_arrive(&sh->item_full[slot]);
             }
             if (++slot == PA_ITEMS) slot = 0, phase ^= 1;
-            i = (int64_t)gridDim.x + __shfl_sync(0xFFFFFFFFu, ahead, 0);
+            return true;
+        };
+        if (TREE) {
+            tree_items(t, announce);
+        } else {
+            PromptSchedule schedule{t};
+            schedule.begin();
+            for (int64_t i = blockIdx.x; schedule.find(i, it);) {
+                unsigned int ahead = 0;
+                if (lane == 0) ahead = atomicAdd(&t.sched[0], 1u);
+                if (!announce(it)) break;
+                i = (int64_t)gridDim.x + __shfl_sync(0xFFFFFFFFu, ahead, 0);
+            }
+            __threadfence();
+            if (lane == 0 && atomicAdd(&t.sched[1], 1u) == gridDim.x - 1) {  // the last one leaves the counters as it found them
+                t.sched[0] = 0;
+                t.sched[1] = 0;
+            }
         }
-        __threadfence();
-        if (lane == 0 && atomicAdd(&t.sched[1], 1u) == gridDim.x - 1) {  // the last one leaves the counters as it found them
-            t.sched[0] = 0;
-            t.sched[1] = 0;
+        if (!failed) {
+            it = PromptItem{};
+            it.last = 1;
+            announce(it);
         }
     }
     if (failed) {
