@@ -16,7 +16,7 @@ static int check_cache(Context* c, const char* what, const wf_kv_cache* cache, i
     if (!cache) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: null cache", what);
     if (!cache->keys_dev || !cache->values_dev || (cache->keys_dev | cache->values_dev) & 15)
         return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: keys and values must be 16-byte aligned device addresses", what);
-    if (cache->layers < 1 || layer < 0 || layer >= cache->layers) return set_error(c, WF_ERR_SHAPE, "%s: layer %d of %d", what, layer, cache->layers);
+    if (cache->layers < 1 || cache->layers > 32767 || layer < 0 || layer >= cache->layers) return set_error(c, WF_ERR_SHAPE, "%s: layer %d of %d", what, layer, cache->layers);
     if (cache->head_dim < 8 || cache->head_dim > ATTN_MAX_DIM || cache->head_dim % 8)
         return set_error(c, WF_ERR_SHAPE, "%s: head_dim %d is not a multiple of 8 from 8 to %d", what, cache->head_dim, ATTN_MAX_DIM);
     const int p = cache->page_tokens;

@@ -46,34 +46,38 @@ struct CopyParams {
     int64_t n;
     int* status;
 };
-// A unit is one head of one page in one layer, keys or values: contiguous on both sides.  COPY_DEPTH 16-byte pieces a thread in flight.
-// Bound by HBM.
+// A unit is one head of one page in one layer, keys or values: contiguous on both sides.  A CTA has a unit at a time, COPY_DEPTH 16-byte pieces a thread in flight,
+// and knows where the next one lies before it copies.  Bound by HBM.
 constexpr int COPY_THREADS = 256, COPY_DEPTH = 4;
 __global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const __grid_constant__ CopyParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int heads = p.cache.kv_heads, page_tokens = 1 << p.cache.page_shift;
-    const int64_t units = (int64_t)p.layers * 2 * p.n * heads;
-    for (int64_t u = blockIdx.x; u < units; u += gridDim.x) {
-        const int head = (int)(u % heads);
-        const int64_t i = u / heads % p.n, of = u / heads / p.n;  // keys of layer 0, values of layer 0, keys of layer 1 ..
-        const int2 pair = p.pairs[i];
-        const int rows = p.rows ? p.rows[i] : page_tokens;
+    const unsigned heads = (unsigned)p.cache.kv_heads, n = (unsigned)p.n, units = n * heads;  // of a layer's keys or values
+    const int page_tokens = 1 << p.cache.page_shift;
+    bf16* const base = (blockIdx.y & 1 ? p.cache.values : p.cache.keys) + (size_t)(blockIdx.y >> 1) * p.layer_elements;  // keys of layer 0, values of layer 0, keys of layer 1 ..
+    int2 pair;
+    int rows;
+    auto look = [&](unsigned u) {
+        pair = p.pairs[u / heads];
+        rows = p.rows ? p.rows[u / heads] : page_tokens;
+    };
+    unsigned u = blockIdx.x;
+    if (u < units) look(u);
+    for (; u < units; u += gridDim.x) {
         const bool bad = pair.x < 0 || pair.y < 0 || pair.x >= p.cache.pages || pair.y >= p.cache.pages || rows < 0 || rows > page_tokens;
         if (bad && threadIdx.x == 0) report_status(p.status, STATUS_BAD_INDEX);
-        if (bad || pair.x == pair.y) continue;
-        bf16* base = (of & 1 ? p.cache.values : p.cache.keys) + (size_t)(of >> 1) * p.layer_elements;
+        const int head = (int)(u % heads), pieces = bad || pair.x == pair.y ? 0 : rows * p.cache.dim / 8;
         const uint4* from = reinterpret_cast<const uint4*>(base + p.cache.at(pair.x, head, 0));
         uint4* to = reinterpret_cast<uint4*>(base + p.cache.at(pair.y, head, 0));
-        const int pieces = rows * p.cache.dim / 8;
+        if (u + gridDim.x < units) look(u + gridDim.x);
         for (int j0 = threadIdx.x; j0 < pieces; j0 += COPY_DEPTH * COPY_THREADS) {
             uint4 v[COPY_DEPTH];
 #pragma unroll
             for (int e = 0; e < COPY_DEPTH; e++)
-                if (j0 + e * COPY_THREADS < pieces) v[e] = from[j0 + e * COPY_THREADS];
+                if (j0 + e * COPY_THREADS < pieces) v[e] = __ldcs(from + j0 + e * COPY_THREADS);
 #pragma unroll
             for (int e = 0; e < COPY_DEPTH; e++)
-                if (j0 + e * COPY_THREADS < pieces) to[j0 + e * COPY_THREADS] = v[e];
+                if (j0 + e * COPY_THREADS < pieces) __stcs(to + j0 + e * COPY_THREADS, v[e]);
         }
     }
 }
@@ -98,12 +102,11 @@ constexpr int COMPACT_THREADS = 128, COMPACT_DEPTH = 8;
 __global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const __grid_constant__ CompactParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int pieces = p.cache.dim / 8, heads = p.cache.kv_heads, shift = p.cache.page_shift;
-    const int64_t n = (int64_t)p.layers * 2 * p.seqs * heads * pieces;
-    for (int64_t u = (int64_t)blockIdx.x * COMPACT_THREADS + threadIdx.x; u < n; u += (int64_t)gridDim.x * COMPACT_THREADS) {
-        const int piece = (int)(u % pieces), head = (int)(u / pieces % heads);
-        const int64_t s = u / pieces / heads % p.seqs, of = u / pieces / heads / p.seqs;
-        bf16* base = (of & 1 ? p.cache.values : p.cache.keys) + (size_t)(of >> 1) * p.layer_elements;
+    const unsigned pieces = (unsigned)p.cache.dim / 8, columns = pieces * p.cache.kv_heads, u = blockIdx.x * COMPACT_THREADS + threadIdx.x;
+    if (u >= columns) return;
+    const int piece = (int)(u % pieces), head = (int)(u / pieces), shift = p.cache.page_shift;
+    bf16* const base = (blockIdx.z & 1 ? p.cache.values : p.cache.keys) + (size_t)(blockIdx.z >> 1) * p.layer_elements;
+    for (int64_t s = blockIdx.y; s < p.seqs; s += gridDim.y) {
         const int* table = p.tables + s * p.table_stride;
         const int* kept = p.kept + s * p.kept_stride;
         const int64_t start = p.context[s], most = p.table_stride << shift;
@@ -118,11 +121,14 @@ __global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const __grid_c
         for (int i0 = 0; i0 < count && !bad; i0 += COMPACT_DEPTH) {
             uint4 v[COMPACT_DEPTH];
             uint4* to[COMPACT_DEPTH];
+            int next[COMPACT_DEPTH];
+#pragma unroll
+            for (int e = 0; e < COMPACT_DEPTH; e++) next[e] = i0 + e < count ? kept[i0 + e] : 0;
 #pragma unroll
             for (int e = 0; e < COMPACT_DEPTH; e++) {
                 to[e] = nullptr;
                 if (i0 + e >= count || bad) continue;
-                const int j = kept[i0 + e];
+                const int j = next[e];
                 if (j <= before || start + j >= most) {
                     bad = true;
                     continue;
@@ -150,9 +156,9 @@ __global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const __grid_c
 
 using namespace wf;
 
-template <class Params> static int launch_cache(Context* c, const char* what, void (*kernel)(Params), int64_t want, unsigned threads, cudaStream_t s, const Params& p) {
+template <class Params> static int launch_cache(Context* c, const char* what, void (*kernel)(Params), dim3 grid, unsigned threads, cudaStream_t s, const Params& p) {
     cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = dim3((unsigned)std::max<int64_t>(1, std::min<int64_t>(want, (int64_t)c->sm_count * (2048 / threads))));
+    cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.stream = s;
     cudaLaunchAttribute attr[1];
@@ -181,7 +187,7 @@ int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev
     const char* what = "cache_copy_pages";
     const int rc = check_kv_cache(c, what, cache, 0, false);
     if (rc != WF_OK) return rc;
-    if (n < 0 || n > (1LL << 31) - 1) return set_error(c, WF_ERR_SHAPE, "%s: %lld pairs", what, (long long)n);
+    if (n < 0 || n > (1LL << 31) / cache->kv_heads - 1) return set_error(c, WF_ERR_SHAPE, "%s: %lld pairs", what, (long long)n);
     if (n == 0) return WF_OK;
     if (!pairs_dev || pairs_dev & 7 || rows_dev & 3) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: pairs is an 8-byte aligned device array, rows a 4-byte aligned one", what);
     CopyParams p{};
@@ -192,7 +198,9 @@ int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev
     p.rows = reinterpret_cast<const int*>(rows_dev);
     p.n = n;
     p.status = c->d_status;
-    return launch_cache(c, what, copy_pages_kernel, (int64_t)cache->layers * 2 * n * cache->kv_heads, COPY_THREADS, s, p);
+    const int64_t units = n * cache->kv_heads, wave = (int64_t)c->sm_count * (2048 / COPY_THREADS);  // CTAs that the device holds
+    const int64_t x = std::min<int64_t>(units, std::max<int64_t>(1, wave / (2 * cache->layers)));
+    return launch_cache(c, what, copy_pages_kernel, dim3((unsigned)x, 2 * (unsigned)cache->layers), COPY_THREADS, s, p);
 }
 
 int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, int64_t table_stride, int64_t context_dev, int64_t kept_dev, int64_t kept_stride,
@@ -218,8 +226,8 @@ int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, 
     p.counts = reinterpret_cast<const int*>(counts_dev);
     p.seqs = seqs;
     p.status = c->d_status;
-    const int64_t threads = (int64_t)cache->layers * 2 * seqs * cache->kv_heads * (cache->head_dim / 8);
-    return launch_cache(c, what, compact_kernel, (threads + COMPACT_THREADS - 1) / COMPACT_THREADS, COMPACT_THREADS, s, p);
+    const unsigned columns = (unsigned)cache->kv_heads * (unsigned)(cache->head_dim / 8);  // 16-byte pieces of a token
+    return launch_cache(c, what, compact_kernel, dim3((columns + COMPACT_THREADS - 1) / COMPACT_THREADS, (unsigned)std::min<int64_t>(seqs, 65535), 2 * (unsigned)cache->layers), COMPACT_THREADS, s, p);
 }
 
 int wf_pages_create(int64_t pages, int64_t* pool) {

@@ -24,114 +24,130 @@ struct RopeParams {
     int64_t tokens;
     int q_heads, k_heads, v_heads;  // 0: that part is not wanted
     int rot, norm, adjacent;
+    int sets, batches;  // warps of a token, batches of heads of a warp
     float eps;
     int* status;
 };
 
-template <class X, bool VEC> __device__ __forceinline__ void load_x(const void* base, size_t i, float (&f)[4]) {
+// Two neighbouring elements.
+template <class X, bool VEC> __device__ __forceinline__ float2 load_pair(const void* base, size_t i) {
     const X* p = static_cast<const X*>(base) + i;
-    if (VEC && sizeof(X) == 4) {
-        const float4 v = ld_once(reinterpret_cast<const float4*>(p));
-        f[0] = v.x, f[1] = v.y, f[2] = v.z, f[3] = v.w;
-    } else if (VEC) {
-        load4(reinterpret_cast<const bf16*>(p), f);
-    } else {
-#pragma unroll
-        for (int e = 0; e < 4; e++) f[e] = (float)p[e];
+    if (!VEC) return make_float2((float)p[0], (float)p[1]);
+    float2 v;
+    if (sizeof(X) == 4) {
+        asm volatile("ld.global.cs.v2.f32 {%0, %1}, [%2];" : "=f"(v.x), "=f"(v.y) : "l"(p));
+        return v;
     }
+    uint32_t w;
+    asm volatile("ld.global.cs.u32 %0, [%1];" : "=r"(w) : "l"(p));
+    return make_float2(__uint_as_float(w << 16), __uint_as_float(w & 0xFFFF0000u));
 }
 
-// A group of LANES lanes has a head, four elements a lane; a warp takes HEADS heads of one token at a time, all requested before the
-// first is used.  The partner of a pair (i, i + rot/2) lies rot / 8 lanes away (rot is a multiple of 8).
-constexpr int ROPE_WARPS = 4, ROPE_UNROLL = 4;
+// A group of LANES lanes has a head, four elements a lane: two pairs that are rotated, (i, i + rot/2) and (i + 1, i + 1 + rot/2) or two adjacent ones, so
+// that no lane needs another's, or four that are not. A warp takes HEADS heads of one token at a time, and asks for the next ones before it works on them.
+constexpr int ROPE_WARPS = 4, ROPE_UNROLL = 4, ROPE_WARPS_PER_SM = 48, ROPE_MOST_BATCHES = 5;
 template <class X, bool VEC, int LANES> __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
-    constexpr int SIDE = 32 / LANES, HEADS = ROPE_UNROLL * SIDE;  // heads beside one another in a warp, heads of a warp
+    constexpr int SIDE = 32 / LANES, HEADS = ROPE_UNROLL * SIDE;  // heads beside one another in a warp, heads of a batch
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const int lane = threadIdx.x & (LANES - 1), side = (threadIdx.x & 31) / LANES;
-    const int d = p.cache.dim, i = 4 * lane, heads = p.q_heads + p.k_heads + p.v_heads, sets = (heads + HEADS - 1) / HEADS;
-    const bool mine = i < d;
+    const int d = p.cache.dim, heads = p.q_heads + p.k_heads + p.v_heads, rotated = p.q_heads + p.k_heads;
+    const bool mine = 4 * lane < d;
     const int64_t unit = (int64_t)blockIdx.x * ROPE_WARPS + (threadIdx.x >> 5);
-    const int64_t t = unit / sets;
+    const int64_t t = unit / p.sets;
     if (t >= p.tokens) return;
-    const int h0 = (int)(unit % sets) * HEADS + side;
-    float x[ROPE_UNROLL][4] = {};
+    const int set = (int)(unit - t * p.sets), h_first = set * p.batches * HEADS + side;
+    const int h_end = min(heads, (set + 1) * p.batches * HEADS);
+    // the elements: a0, a0 + 1 and b0, b0 + 1
+    const bool turns = 4 * lane < p.rot, apart = turns && !p.adjacent;
+    const int a0 = apart ? 2 * lane : 4 * lane, b0 = apart ? p.rot / 2 + 2 * lane : 4 * lane + 2;
+    auto ask = [&](int h0, float2 (&x)[ROPE_UNROLL][2]) {
 #pragma unroll
-    for (int u = 0; u < ROPE_UNROLL; u++) {
-        const int h = h0 + u * SIDE;
-        if (h >= heads || !mine) continue;
-        if (h < p.q_heads) load_x<X, VEC>(p.q, t * p.q_stride + (size_t)h * d + i, x[u]);
-        else if (h < p.q_heads + p.k_heads) load_x<X, VEC>(p.k, t * p.k_stride + (size_t)(h - p.q_heads) * d + i, x[u]);
-        else load_x<X, VEC>(p.v, t * p.v_stride + (size_t)(h - p.q_heads - p.k_heads) * d + i, x[u]);
-    }
+        for (int u = 0; u < ROPE_UNROLL; u++) {
+            const int h = h0 + u * SIDE;
+            x[u][0] = x[u][1] = make_float2(0.f, 0.f);
+            if (h >= h_end || !mine) continue;
+            const void* base = h < p.q_heads ? p.q : h < rotated ? p.k : p.v;
+            const size_t at = h < p.q_heads  ? t * p.q_stride + (size_t)h * d
+                              : h < rotated ? t * p.k_stride + (size_t)(h - p.q_heads) * d
+                                            : t * p.v_stride + (size_t)(h - rotated) * d;
+            x[u][0] = load_pair<X, VEC>(base, at + a0);
+            x[u][1] = load_pair<X, VEC>(base, at + b0);
+        }
+    };
+    float2 x[ROPE_UNROLL][2];
+    ask(h_first, x);
     int64_t slot = p.slots ? p.slots[t] : t;
     int64_t pos = p.rot ? p.positions[t] : 0;
+    float2 gq[2] = {make_float2(1.f, 1.f), make_float2(1.f, 1.f)}, gk[2] = {make_float2(1.f, 1.f), make_float2(1.f, 1.f)};
+    if (p.norm && mine) {
+        if (p.gamma_q) gq[0] = make_float2(p.gamma_q[a0], p.gamma_q[a0 + 1]), gq[1] = make_float2(p.gamma_q[b0], p.gamma_q[b0 + 1]);
+        if (p.gamma_k) gk[0] = make_float2(p.gamma_k[a0], p.gamma_k[a0 + 1]), gk[1] = make_float2(p.gamma_k[b0], p.gamma_k[b0 + 1]);
+    }
     const bool bad = (p.rot && (pos < 0 || pos >= p.rope_rows)) || (p.k_heads && slot >= p.cache.pages << p.cache.page_shift);
     if (bad) {
         if ((threadIdx.x & 31) == 0) report_status(p.status, STATUS_BAD_INDEX);
         slot = -1;
         pos = 0;
     }
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, s[4] = {};
-    const int half = p.rot / 2;
-    const bool upper = !p.adjacent && i >= half;  // the second of its pairs
-    if (i < p.rot) {  // rows of the table are rot * 4 bytes: 16-byte pieces
-        if (p.adjacent) {
-            const float4 w = *reinterpret_cast<const float4*>(p.rope + (size_t)pos * half + i / 2);
-            c[0] = c[1] = w.x, s[0] = s[1] = w.y, c[2] = c[3] = w.z, s[2] = s[3] = w.w;
-        } else {
-            const float4* row = reinterpret_cast<const float4*>(p.rope + (size_t)pos * half + (upper ? i - half : i));
-            const float4 a = row[0], b = row[1];
-            c[0] = a.x, s[0] = a.y, c[1] = a.z, s[1] = a.w, c[2] = b.x, s[2] = b.y, c[3] = b.z, s[3] = b.w;
-        }
-    }
-    float gq[4] = {1.f, 1.f, 1.f, 1.f}, gk[4] = {1.f, 1.f, 1.f, 1.f};
-    if (p.norm && mine) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            if (p.gamma_q) gq[e] = p.gamma_q[i + e];
-            if (p.gamma_k) gk[e] = p.gamma_k[i + e];
-        }
-    }
+    float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);  // cosine and sine of the lane's two pairs: 16 bytes of the row either way
+    if (turns) cs = *reinterpret_cast<const float4*>(p.rope + (size_t)pos * (p.rot / 2) + 2 * lane);
     const int64_t page = slot >> p.cache.page_shift;
     const int row = (int)(slot & ((1 << p.cache.page_shift) - 1));
-    const int away = p.rot / 8;
-#pragma unroll
-    for (int u = 0; u < ROPE_UNROLL; u++) {
-        const int h = h0 + u * SIDE;
-        const bool is_q = h < p.q_heads, turned = h < p.q_heads + p.k_heads;  // the same for the lanes of a head, not for a warp's
-        float y[4];
-        float inv = 1.f;
+    for (int h0 = h_first; h0 - side < h_end; h0 += HEADS) {
+        float2 next[ROPE_UNROLL][2];
+        if (h0 - side + HEADS < h_end) ask(h0 + HEADS, next);
+        float inv[ROPE_UNROLL];
         if (p.norm) {
-            float sum = x[u][0] * x[u][0] + x[u][1] * x[u][1] + x[u][2] * x[u][2] + x[u][3] * x[u][3];
+            // The sums of squares of four heads in ten exchanges instead of twenty: with every exchange at a distance a lane passes on half of the sums that it has and adds
+            // to the others, until it has one; that one is then brought to all lanes of the head.
+            float s[ROPE_UNROLL];
 #pragma unroll
-            for (int o = LANES / 2; o > 0; o >>= 1) sum += __shfl_xor_sync(0xFFFFFFFFu, sum, o);
-            if (turned) inv = rsqrtf(sum / (float)d + p.eps);
+            for (int u = 0; u < ROPE_UNROLL; u++) s[u] = x[u][0].x * x[u][0].x + x[u][0].y * x[u][0].y + x[u][1].x * x[u][1].x + x[u][1].y * x[u][1].y;
+            const bool hi = lane & (LANES / 2), hi2 = lane & (LANES / 4);
+            float t0 = hi ? s[2] : s[0], t1 = hi ? s[3] : s[1];
+            t0 += __shfl_xor_sync(0xFFFFFFFFu, hi ? s[0] : s[2], LANES / 2);
+            t1 += __shfl_xor_sync(0xFFFFFFFFu, hi ? s[1] : s[3], LANES / 2);
+            float r = hi2 ? t1 : t0;
+            r += __shfl_xor_sync(0xFFFFFFFFu, hi2 ? t0 : t1, LANES / 4);
+#pragma unroll
+            for (int o = LANES / 8; o > 0; o >>= 1) r += __shfl_xor_sync(0xFFFFFFFFu, r, o);
+            r = rsqrtf(r / (float)d + p.eps);
+#pragma unroll
+            for (int u = 0; u < ROPE_UNROLL; u++) inv[u] = __shfl_sync(0xFFFFFFFFu, r, (u >> 1) * (LANES / 2) + (u & 1) * (LANES / 4), LANES);
         }
 #pragma unroll
-        for (int e = 0; e < 4; e++) y[e] = turned && p.norm ? x[u][e] * inv * (is_q ? gq[e] : gk[e]) : x[u][e];
-        if (p.rot) {
-            float other[4];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const float far = __shfl_sync(0xFFFFFFFFu, y[e], upper ? lane - away : lane + away, LANES);
-                other[e] = p.adjacent ? y[e ^ 1] : far;
-            }
-            if (turned && i < p.rot) {
-#pragma unroll
-                for (int e = 0; e < 4; e++) {
-                    const bool second = p.adjacent ? e & 1 : upper;
-                    y[e] = second ? y[e] * c[e] + other[e] * s[e] : y[e] * c[e] - other[e] * s[e];
+        for (int u = 0; u < ROPE_UNROLL; u++) {
+            const int h = h0 + u * SIDE;
+            if (h >= h_end || !mine) continue;
+            float2 a = x[u][0], b = x[u][1];
+            if (h < rotated) {
+                if (p.norm) {
+                    const bool is_q = h < p.q_heads;
+                    const float2 ga = is_q ? gq[0] : gk[0], gb = is_q ? gq[1] : gk[1];
+                    a = make_float2(a.x * inv[u] * ga.x, a.y * inv[u] * ga.y);
+                    b = make_float2(b.x * inv[u] * gb.x, b.y * inv[u] * gb.y);
+                }
+                if (apart) {
+                    const float2 a1 = make_float2(a.x * cs.x - b.x * cs.y, a.y * cs.z - b.y * cs.w);
+                    b = make_float2(b.x * cs.x + a.x * cs.y, b.y * cs.z + a.y * cs.w);
+                    a = a1;
+                } else if (turns) {
+                    a = make_float2(a.x * cs.x - a.y * cs.y, a.y * cs.x + a.x * cs.y);
+                    b = make_float2(b.x * cs.z - b.y * cs.w, b.y * cs.z + b.x * cs.w);
                 }
             }
+            const uint32_t wa = bad ? 0u : pack_bf16(a.x, a.y), wb = bad ? 0u : pack_bf16(b.x, b.y);
+            bf16* to = nullptr;
+            if (h < p.q_heads) to = p.q_out + ((size_t)t * p.q_heads + h) * d;
+            else if (slot >= 0) to = h < rotated ? p.cache.keys + p.cache.at(page, h - p.q_heads, row) : p.cache.values + p.cache.at(page, h - rotated, row);
+            if (to) {
+                *reinterpret_cast<uint32_t*>(to + a0) = wa;
+                *reinterpret_cast<uint32_t*>(to + b0) = wb;
+            }
         }
-        if (h >= heads || !mine) continue;
-        const uint2 w = bad ? make_uint2(0u, 0u) : make_uint2(pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3]));
-        if (is_q) *reinterpret_cast<uint2*>(p.q_out + ((size_t)t * p.q_heads + h) * d + i) = w;
-        else if (slot >= 0) {
-            bf16* to = turned ? p.cache.keys + p.cache.at(page, h - p.q_heads, row) : p.cache.values + p.cache.at(page, h - p.q_heads - p.k_heads, row);
-            *reinterpret_cast<uint2*>(to + i) = w;
-        }
+#pragma unroll
+        for (int u = 0; u < ROPE_UNROLL; u++) x[u][0] = next[u][0], x[u][1] = next[u][1];
     }
 }
 
@@ -181,11 +197,14 @@ extern "C" int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* a, const
     p.rot = a->rot_dim, p.norm = a->flags & WF_QK_NORM, p.adjacent = (a->flags & WF_ROPE_ADJACENT) != 0;
     p.eps = a->eps;
     p.status = c->d_status;
-    // 16-byte (bf16: 8-byte) loads where every head of every token allows them; head_dim is a multiple of 8
-    const int64_t piece = 4 * size;
-    const bool vec = ((a->q_dev | a->k_dev | a->v_dev) % piece) == 0 && (!a->q_dev || a->q_stride % 4 == 0) && (!a->k_dev || (a->k_stride % 4 == 0 && a->v_stride % 4 == 0));
-    const int heads = p.q_heads + p.k_heads + p.v_heads, side = d <= 64 ? 2 : 1, sets = (heads + ROPE_UNROLL * side - 1) / (ROPE_UNROLL * side);
-    const int64_t grid = (a->tokens * sets + ROPE_WARPS - 1) / ROPE_WARPS;
+    // 8-byte (bf16: 4-byte) loads where every head of every token allows them; head_dim is a multiple of 8
+    const int64_t piece = 2 * size;
+    const bool vec = ((a->q_dev | a->k_dev | a->v_dev) % piece) == 0 && (!a->q_dev || a->q_stride % 2 == 0) && (!a->k_dev || (a->k_stride % 2 == 0 && a->v_stride % 2 == 0));
+    // Batches of heads of a warp: as many warps as the device holds come first, then fewer that share a token's table row and scales.
+    const int heads = p.q_heads + p.k_heads + p.v_heads, side = d <= 64 ? 2 : 1, all = (heads + ROPE_UNROLL * side - 1) / (ROPE_UNROLL * side);
+    p.batches = (int)std::max<int64_t>(1, std::min<int64_t>({a->tokens * all / ((int64_t)c->sm_count * ROPE_WARPS_PER_SM), all, ROPE_MOST_BATCHES}));
+    p.sets = (all + p.batches - 1) / p.batches;
+    const int64_t grid = (a->tokens * p.sets + ROPE_WARPS - 1) / ROPE_WARPS;
     if (grid > (1LL << 31) - 1) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens of %d heads", what, (long long)a->tokens, heads);
     void (*kernel)(RopeParams);
 #define WF_ROPE_PICK(X, V) (side == 2 ? qk_norm_rope_kernel<X, V, 16> : qk_norm_rope_kernel<X, V, 32>)
