@@ -126,6 +126,10 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
     return r;
 }
 
+// The kernels take a weight as 2^fma(s, scale, -(m scale)): for the largest score that is 2 to what rounding m scale has left, at most 2^-24 of it.  From 2^20 on
+// that may matter, and rows go key by key.
+__device__ __forceinline__ bool scores_too_large(float m, float scale) { return m > -INFINITY && fabsf(m * scale) >= 1048576.f; }
+
 // One row by one warp, key by key: lane l has elements 4 l .. 4 l + 3.  softmax(s) v = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m) with the
 // running maximum m; keys that are not seen are not read.
 template <class Seen>

@@ -165,10 +165,9 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid
     const int d = p.cache.dim, token = p.token_of(cut.first + row), head = cut.head * p.group + cut.first + row - token * p.group;
     bf16* const to = p.out + ((size_t)(cut.row0 + token) * p.q_heads + head) * d;
     if (4 * lane < d) *reinterpret_cast<uint2*>(to + 4 * lane) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
-    // Key by key where an Inf or a NaN may have come from a key that the row does not see, or from a page that is not in the cache; a sum of 0 under a
-    // maximum: scores so large that rounding m scale alone moves a weight out of range.
+    // Key by key where an Inf or a NaN may have come from a key that the row does not see, or from a page that is not in the cache.
     const float largest = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
-    const bool odd = !(sum < INFINITY) || (sum == 0.f && top > -INFINITY) || !(largest < INFINITY) || x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
+    const bool odd = !(sum < INFINITY) || scores_too_large(top, p.scale_log2) || !(largest < INFINITY) || x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
     if (__any_sync(0xFFFFFFFFu, odd)) {
         KeyPlace place;
         place.table = p.tables + (size_t)cut.seq * p.table_stride;

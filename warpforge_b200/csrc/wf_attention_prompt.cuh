@@ -21,6 +21,8 @@ constexpr int PA_THREADS = 12 * 32;
 constexpr int PA_SOFTMAX_REGS = 216, PA_OTHER_REGS = 72;
 constexpr int PA_CHUNK = PA_KEYS * 128;      // bytes of 128 rows x 64 elements
 constexpr int PA_ITEMS = 2;                  // items announced ahead
+// Which of the 32 pairs of weights of 64 keys are taken by the cubic: two in five, so that the special function unit and the fp32 units are through at about the same time.
+__host__ __device__ constexpr bool PA_CUBIC(int pair) { return pair % 5 == 1 || pair % 5 == 3; }
 constexpr float PA_RESCALE = 8.f;            // the running maximum is followed when it has grown by this many powers of two
 constexpr int PA_MAX_STAGES = 12;
 template <int CHUNKS> struct PromptShape {  // by the head's dimension in 64 elements, rounded up
@@ -114,7 +116,15 @@ __device__ __forceinline__ void tmem_ld32_start(uint32_t taddr, uint32_t* r) {
         : "r"(taddr)
         : "memory");
 }
-__device__ __forceinline__ void tmem_wait_ld() { asm volatile("tcgen05.wait::ld.sync.aligned;" ::: "memory"); }
+// ... and the wait: what uses the columns stays behind it
+__device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]),
+                   "+r"(r[10]), "+r"(r[11]), "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15]), "+r"(r[16]), "+r"(r[17]), "+r"(r[18]), "+r"(r[19]),
+                   "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
+                 :
+                 : "memory");
+}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -136,6 +146,20 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
         : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y), "f"(c.x), "f"(c.y));
     return d;
 }
+// 2^x for x <= PA_RESCALE without the special function unit, which has 16 of them a cycle and would be what a tile waits for: x = n + f with n the nearest
+// integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a cubic on [-1/2, 1/2], 1 at 0, with the smallest largest relative error (1.0e-4, 1/38 of
+// what a weight may be off by its rounding to bf16), n added to the exponent.  0 from -127 on.
+__device__ __forceinline__ float2 add2(float2 a, float2 b);
+__device__ __forceinline__ float2 ex2_by_cubic(float2 x) {
+    x.x = fmaxf(x.x, -127.f);
+    x.y = fmaxf(x.y, -127.f);
+    const float2 big = make_float2(12582912.f, 12582912.f), less = make_float2(-12582912.f, -12582912.f);
+    const float2 t = add2(x, big), n = add2(t, less), f = fma2(n, make_float2(-1.f, -1.f), x);
+    float2 y = fma2(f, make_float2(0.05500893f, 0.05500893f), make_float2(0.24221095f, 0.24221095f));
+    y = fma2(y, f, make_float2(0.6932829f, 0.6932829f));
+    y = fma2(y, f, make_float2(1.f, 1.f));
+    return make_float2(__uint_as_float(__float_as_uint(y.x) + (__float_as_uint(t.x) << 23)), __uint_as_float(__float_as_uint(y.y) + (__float_as_uint(t.y) << 23)));
+}
 __device__ __forceinline__ float2 add2(float2 a, float2 b) {
     float2 d;
     asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tadd.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
@@ -149,7 +173,7 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) { return
 
 struct PromptShared {
     uint64_t q_full[2], q_empty[2];
-    uint64_t s_full[2], p_full[2], o_full[2];
+    uint64_t s_full[2], p_half[2], p_full[2], o_full[2];  // scores; weights of the first 64 keys, of all; sums
     uint64_t half_ready, half_taken;  // tree, one tile of rows: the second group's maxima and sums lie in half_max and half_sum; they and its O have been read
     float half_max[PA_ROWS], half_sum[PA_ROWS];
     uint64_t kv_full[PA_MAX_STAGES], kv_empty[PA_MAX_STAGES];
@@ -298,6 +322,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             g_mbar_init(&sh->q_full[g], 1);
             g_mbar_init(&sh->q_empty[g], 1);
             g_mbar_init(&sh->s_full[g], 1);
+            g_mbar_init(&sh->p_half[g], 4);
             g_mbar_init(&sh->p_full[g], 4);
             g_mbar_init(&sh->o_full[g], 1);
         }
@@ -354,10 +379,23 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 s_phase ^= 1;
                 tc_fence_after();
                 uint32_t s[PA_KEYS];
+                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+                auto maxima = [&](int c) {  // of 32 keys
 #pragma unroll
-                for (int c = 0; c < 4; c++) tmem_ld32_start(s_at + 32 * c, s + 32 * c);
-                tmem_wait_ld();
-                if (j * PA_KEYS + PA_KEYS - 1 > all_see) {  // keys that some row of the warp does not see
+                    for (int i = 32 * c; i < 32 * c + 32; i += 8)
+#pragma unroll
+                        for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[i + 2 * e])), __uint_as_float(s[i + 2 * e + 1]));
+                };
+                tmem_ld32_start(s_at, s);
+                tmem_wait_ld32(s);
+                const bool masked = j * PA_KEYS + PA_KEYS - 1 > all_see;  // keys that some row of the warp does not see
+#pragma unroll
+                for (int c = 1; c < 4; c++) {
+                    tmem_ld32_start(s_at + 32 * c, s + 32 * c);
+                    if (!masked) maxima(c - 1);  // under the load
+                    tmem_wait_ld32(s + 32 * c);
+                }
+                if (masked) {
                     if (TREE) {
                         // bit i of the four words: the row sees key i of the tile.  Below `old` it does, from there on the ancestors say so.
                         const int old = it.context - j * PA_KEYS;
@@ -376,12 +414,10 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                         for (int i = 0; i < PA_KEYS; i++)
                             if (i > limit) s[i] = 0xFF800000u;
                     }
+#pragma unroll
+                    for (int c = 0; c < 3; c++) maxima(c);
                 }
-                float top[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
-#pragma unroll
-                for (int i = 0; i < PA_KEYS; i += 8)
-#pragma unroll
-                    for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[i + 2 * e])), __uint_as_float(s[i + 2 * e + 1]));
+                maxima(3);
                 const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
                 if (i_tile == 0) {
                     m = tile_top;
@@ -395,7 +431,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     for (int c = 0; c < DIM; c += 32) {
                         uint32_t o[32];
                         tmem_ld32_start(o_at + c, o);
-                        tmem_wait_ld();
+                        tmem_wait_ld32(o);
 #pragma unroll
                         for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep);
                         tmem_st32(o_at + c, o);
@@ -411,12 +447,21 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     for (int i = 0; i < 32; i++) {
                         const int k = 64 * h + 2 * i;
                         float2 x = fma2(make_float2(__uint_as_float(s[k]), __uint_as_float(s[k + 1])), sc, off);
-                        x.x = ex2(x.x);
-                        x.y = ex2(x.y);
+                        if (PA_CUBIC(i)) {
+                            x = ex2_by_cubic(x);
+                        } else {
+                            x.x = ex2(x.x);
+                            x.y = ex2(x.y);
+                        }
                         sum[i & 1] = add2(sum[i & 1], x);
                         w[i] = pack_bf16(x.x, x.y);
                     }
                     tmem_st32(s_at + 32 * h, w);
+                    if (h == 0) {  // the products of these keys may begin
+                        tmem_wait_st();
+                        tc_fence_before();
+                        if (lane == 0) g_mbar_arrive(&sh->p_half[g]);
+                    }
                 }
                 const float2 both = add2(sum[0], sum[1]);
                 l += both.x + both.y;
@@ -470,11 +515,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             // the row's sums, 32 at a time
             auto sums = [&](int c, uint32_t(&o)[32]) {
                 tmem_ld32_start(o_at + c, o);
-                tmem_wait_ld();
+                tmem_wait_ld32(o);
                 if (halves) {
                     uint32_t o1[32];
                     tmem_ld32_start(o_at + DIM + c, o1);
-                    tmem_wait_ld();
+                    tmem_wait_ld32(o1);
 #pragma unroll
                     for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep + __uint_as_float(o1[i]) * take);
                 }
@@ -498,7 +543,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 tc_fence_before();
             } else if (n > 0) {
                 const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-                odd = !(l < INFINITY) || (l == 0.f && top > -INFINITY);  // the latter: scores so large that rounding m scale alone moves a weight out of range
+                odd = !(l < INFINITY) || scores_too_large(top, scale);
 #pragma unroll
                 for (int c = 0; c < DIM; c += 32) {
                     uint32_t o[32];
@@ -636,16 +681,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 tc_fence_after();
             };
             auto products = [&](int g, int stage, bool accumulate) {  // O += P V
-                if (!pa_wait(&sh->p_full[g], p_phase[g])) {
-                    failed = true;
-                    return;
-                }
-                p_phase[g] ^= 1;
-                tc_fence_after();
                 const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(stage * STAGE_BYTES), PA_CHUNK);
 #pragma unroll
-                for (int h = 0; h < 2; h++)
+                for (int h = 0; h < 2; h++) {
+                    if (!pa_wait(h ? &sh->p_full[g] : &sh->p_half[g], p_phase[g])) {
+                        failed = true;
+                        return;
+                    }
+                    tc_fence_after();
                     pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, accumulate || h > 0, issue);
+                }
+                p_phase[g] ^= 1;
             };
             auto zero_tail = [&](int stage, int j) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
                 if (!tail || j != n - 1) return;

@@ -404,8 +404,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
         auto store = [&](int r, int col, const float4& x, float sum, float top) {  // four elements of a row, or zeros where it sees nothing
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
-            // a sum of 0 under a maximum: scores so large that rounding m scale alone moves a weight out of range
-            uint32_t largest = sum < INFINITY && !(sum == 0.f && top > -INFINITY) ? 0 : 0x7F800000u;
+            uint32_t largest = sum < INFINITY && !scores_too_large(top, scale) ? 0 : 0x7F800000u;
             largest = max(max(largest, __float_as_uint(x.x) & 0x7FFFFFFFu), max(__float_as_uint(x.y) & 0x7FFFFFFFu, max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu)));
             if (largest >= 0x7F800000u) atomicOr(&sh->odd_rows, 1ull << r);
             const int token = p.token_of(w.first + r);

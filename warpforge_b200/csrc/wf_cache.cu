@@ -48,8 +48,8 @@ struct CopyParams {
 };
 // A unit is one head of one page in one layer, keys or values: contiguous on both sides.  A CTA has a unit at a time, COPY_DEPTH 16-byte pieces a thread in flight,
 // and knows where the next one lies before it copies.  Bound by HBM.
-constexpr int COPY_THREADS = 256, COPY_DEPTH = 4;
-__global__ void __launch_bounds__(COPY_THREADS) copy_pages_kernel(const __grid_constant__ CopyParams p) {
+constexpr int COPY_THREADS = 128, COPY_DEPTH = 8, COPY_CTAS = 8;  // CTAs of an SM
+__global__ void __launch_bounds__(COPY_THREADS, COPY_CTAS) copy_pages_kernel(const __grid_constant__ CopyParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const unsigned heads = (unsigned)p.cache.kv_heads, n = (unsigned)p.n, units = n * heads;  // of a layer's keys or values
@@ -198,7 +198,7 @@ int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev
     p.rows = reinterpret_cast<const int*>(rows_dev);
     p.n = n;
     p.status = c->d_status;
-    const int64_t units = n * cache->kv_heads, wave = (int64_t)c->sm_count * (2048 / COPY_THREADS);  // CTAs that the device holds
+    const int64_t units = n * cache->kv_heads, wave = (int64_t)c->sm_count * COPY_CTAS;  // CTAs that the device holds
     const int64_t x = std::min<int64_t>(units, std::max<int64_t>(1, wave / (2 * cache->layers)));
     return launch_cache(c, what, copy_pages_kernel, dim3((unsigned)x, 2 * (unsigned)cache->layers), COPY_THREADS, s, p);
 }

@@ -30,8 +30,7 @@ struct RopeParams {
 };
 
 // Two neighbouring elements.
-template <class X, bool VEC> __device__ __forceinline__ float2 load_pair(const void* base, size_t i) {
-    const X* p = static_cast<const X*>(base) + i;
+template <class X, bool VEC> __device__ __forceinline__ float2 load_pair(const X* p) {
     if (!VEC) return make_float2((float)p[0], (float)p[1]);
     float2 v;
     if (sizeof(X) == 4) {
@@ -44,7 +43,7 @@ template <class X, bool VEC> __device__ __forceinline__ float2 load_pair(const v
 }
 
 // A group of LANES lanes has a head, four elements a lane: two pairs that are rotated, (i, i + rot/2) and (i + 1, i + 1 + rot/2) or two adjacent ones, so
-// that no lane needs another's, or four that are not. A warp takes HEADS heads of one token at a time, and asks for the next ones before it works on them.
+// that no lane needs another's, or four that are not. A warp takes HEADS heads of one token at a time.
 constexpr int ROPE_WARPS = 4, ROPE_UNROLL = 4, ROPE_WARPS_PER_SM = 48, ROPE_MOST_BATCHES = 5;
 template <class X, bool VEC, int LANES> __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     constexpr int SIDE = 32 / LANES, HEADS = ROPE_UNROLL * SIDE;  // heads beside one another in a warp, heads of a batch
@@ -61,18 +60,19 @@ template <class X, bool VEC, int LANES> __global__ void __launch_bounds__(ROPE_W
     // the elements: a0, a0 + 1 and b0, b0 + 1
     const bool turns = 4 * lane < p.rot, apart = turns && !p.adjacent;
     const int a0 = apart ? 2 * lane : 4 * lane, b0 = apart ? p.rot / 2 + 2 * lane : 4 * lane + 2;
+    // where the token's heads lie, as if all were heads of one tensor: head h is h * d elements on
+    const X* const in_q = static_cast<const X*>(p.q) + t * p.q_stride;
+    const X* const in_k = static_cast<const X*>(p.k) + t * p.k_stride - (int64_t)p.q_heads * d;
+    const X* const in_v = static_cast<const X*>(p.v) + t * p.v_stride - (int64_t)rotated * d;
     auto ask = [&](int h0, float2 (&x)[ROPE_UNROLL][2]) {
 #pragma unroll
         for (int u = 0; u < ROPE_UNROLL; u++) {
             const int h = h0 + u * SIDE;
             x[u][0] = x[u][1] = make_float2(0.f, 0.f);
             if (h >= h_end || !mine) continue;
-            const void* base = h < p.q_heads ? p.q : h < rotated ? p.k : p.v;
-            const size_t at = h < p.q_heads  ? t * p.q_stride + (size_t)h * d
-                              : h < rotated ? t * p.k_stride + (size_t)(h - p.q_heads) * d
-                                            : t * p.v_stride + (size_t)(h - rotated) * d;
-            x[u][0] = load_pair<X, VEC>(base, at + a0);
-            x[u][1] = load_pair<X, VEC>(base, at + b0);
+            const X* const from = (h < p.q_heads ? in_q : h < rotated ? in_k : in_v) + h * d;
+            x[u][0] = load_pair<X, VEC>(from + a0);
+            x[u][1] = load_pair<X, VEC>(from + b0);
         }
     };
     float2 x[ROPE_UNROLL][2];
@@ -92,11 +92,11 @@ template <class X, bool VEC, int LANES> __global__ void __launch_bounds__(ROPE_W
     }
     float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);  // cosine and sine of the lane's two pairs: 16 bytes of the row either way
     if (turns) cs = *reinterpret_cast<const float4*>(p.rope + (size_t)pos * (p.rot / 2) + 2 * lane);
-    const int64_t page = slot >> p.cache.page_shift;
-    const int row = (int)(slot & ((1 << p.cache.page_shift) - 1));
+    bf16* const out_q = p.q_out + t * p.q_heads * d;
+    const int64_t place = slot < 0 ? 0 : (int64_t)p.cache.at(slot >> p.cache.page_shift, 0, (int)(slot & ((1 << p.cache.page_shift) - 1)));
+    const int apart_heads = d << p.cache.page_shift;  // elements between heads of the cache
     for (int h0 = h_first; h0 - side < h_end; h0 += HEADS) {
-        float2 next[ROPE_UNROLL][2];
-        if (h0 - side + HEADS < h_end) ask(h0 + HEADS, next);
+        if (h0 > h_first) ask(h0, x);
         float inv[ROPE_UNROLL];
         if (p.norm) {
             // The sums of squares of four heads in ten exchanges instead of twenty: with every exchange at a distance a lane passes on half of the sums that it has and adds
@@ -138,16 +138,13 @@ template <class X, bool VEC, int LANES> __global__ void __launch_bounds__(ROPE_W
                 }
             }
             const uint32_t wa = bad ? 0u : pack_bf16(a.x, a.y), wb = bad ? 0u : pack_bf16(b.x, b.y);
-            bf16* to = nullptr;
-            if (h < p.q_heads) to = p.q_out + ((size_t)t * p.q_heads + h) * d;
-            else if (slot >= 0) to = h < rotated ? p.cache.keys + p.cache.at(page, h - p.q_heads, row) : p.cache.values + p.cache.at(page, h - rotated, row);
-            if (to) {
+            bf16* to = out_q + h * d;
+            if (h >= p.q_heads) to = (h < rotated ? p.cache.keys + (int64_t)(h - p.q_heads) * apart_heads : p.cache.values + (int64_t)(h - rotated) * apart_heads) + place;
+            if (h < p.q_heads || slot >= 0) {
                 *reinterpret_cast<uint32_t*>(to + a0) = wa;
                 *reinterpret_cast<uint32_t*>(to + b0) = wb;
             }
         }
-#pragma unroll
-        for (int u = 0; u < ROPE_UNROLL; u++) x[u][0] = next[u][0], x[u][1] = next[u][1];
     }
 }
 
