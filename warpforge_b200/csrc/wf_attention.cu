@@ -111,7 +111,10 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
     if (rc != WF_OK) return rc;
-    const int64_t items = (p.tokens / (2 * t.tile_tokens) + p.seqs) * p.cache.kv_heads;
+    // Items of two tiles of rows; of one, on which both groups of a CTA work, where that many would leave half of the device idle.
+    const int64_t pairs = (p.tokens + (int64_t)p.seqs * (2 * t.tile_tokens - 1)) / (2 * t.tile_tokens) * p.cache.kv_heads;
+    t.split = 2 * pairs <= c->sm_count;
+    const int64_t items = t.split ? (p.tokens + (int64_t)p.seqs * (t.tile_tokens - 1)) / t.tile_tokens * p.cache.kv_heads : pairs;
     return launch_attention(c, what, prompt_tiles_kernel<CHUNKS, false>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
 

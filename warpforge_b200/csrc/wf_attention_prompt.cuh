@@ -49,6 +49,7 @@ struct PromptTiles {
     PromptParams p;
     int tile_tokens;   // tokens of a tile: 128 / group
     int box_rows;      // rows of keys that one TMA load brings: those of a page, at most 128
+    int split;         // prompt: items have one tile of rows
     unsigned int* sched;  // prompt: [0] items taken beyond the first of each CTA, [1] CTAs that are done
     TreeParams tree;
     TreeCuts c;
@@ -124,6 +125,33 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
                    "+r"(r[20]), "+r"(r[21]), "+r"(r[22]), "+r"(r[23]), "+r"(r[24]), "+r"(r[25]), "+r"(r[26]), "+r"(r[27]), "+r"(r[28]), "+r"(r[29]), "+r"(r[30]), "+r"(r[31])
                  :
                  : "memory");
+}
+// 16 rows x 32 columns: a lane has the columns 8 x + 2 q and 8 x + 2 q + 1 (q = lane % 4, x = 0 .. 3) of the rows lane / 4 (r[4 x], r[4 x + 1]) and lane / 4 + 8
+// (r[4 x + 2], r[4 x + 3])
+__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
+    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
+                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
+                 : "r"(taddr)
+                 : "memory");
+}
+__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
+    asm volatile("tcgen05.wait::ld.sync.aligned;"
+                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
+                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
+                 :
+                 : "memory");
+}
+// Lane q of four has word x of column x of a 4 x 4 matrix in w[x]; afterwards its row q.
+__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
+    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
+    // exchange with the neighbour, then two on: blocks of one, then of two
+    const uint32_t a = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[0] : w[1], 1), b = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[2] : w[3], 1);
+    if (odd) w[0] = a, w[2] = b;
+    else w[1] = a, w[3] = b;
+    const uint32_t c = __shfl_xor_sync(0xFFFFFFFFu, high ? w[0] : w[2], 2), d = __shfl_xor_sync(0xFFFFFFFFu, high ? w[1] : w[3], 2);
+    if (high) w[0] = c, w[1] = d;
+    else w[2] = c, w[3] = d;
 }
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
@@ -208,27 +236,39 @@ struct PromptSchedule {
     int v;           // where the cursor is
     int64_t before;  // items with a larger v
     int count;       // sequences that have this v
-    __device__ __forceinline__ void span(int s, int& lo, int& hi) const {  // a sequence's v: [lo, hi)
-        const PromptSeq q = prompt_seq(t.p, s);
-        const int past = max(0, q.keys - q.rows);
-        lo = past / block;
+    PromptSeq mine;  // of the first 32 sequences, this lane's; the others are looked up when they are needed
+    int mine_lo, mine_hi;
+    __device__ __forceinline__ PromptSeq look(int s, int& lo, int& hi) const {  // a sequence and its v: [lo, hi)
+        PromptSeq q{};
+        lo = hi = 0;
+        if (s >= t.p.seqs) return q;
+        q = prompt_seq(t.p, s);
+        lo = max(0, q.keys - q.rows) / block;
         hi = lo + (q.rows + block - 1) / block;
+        return q;
+    }
+    __device__ __forceinline__ uint32_t with(int s0, int value, int& lo, PromptSeq& q) const {  // which of 32 sequences have it
+        int hi = mine_hi;
+        lo = mine_lo;
+        q = mine;
+        if (s0) q = look(s0 + (threadIdx.x & 31), lo, hi);
+        return __ballot_sync(0xFFFFFFFFu, value >= lo && value < hi);
     }
     __device__ __forceinline__ int have(int value) const {
-        int n = 0;
-        for (int s0 = 0; s0 < t.p.seqs; s0 += 32) {
-            int lo = 0, hi = 0;
-            if (s0 + (int)(threadIdx.x & 31) < t.p.seqs) span(s0 + (threadIdx.x & 31), lo, hi);
-            n += __popc(__ballot_sync(0xFFFFFFFFu, value >= lo && value < hi));
-        }
+        int n = 0, lo;
+        PromptSeq q;
+#pragma unroll 1
+        for (int s0 = 0; s0 < t.p.seqs; s0 += 32) n += __popc(with(s0, value, lo, q));
         return n;
     }
     __device__ __forceinline__ void begin() {
-        block = 2 * t.tile_tokens;
-        int top = 0;
-        for (int s = threadIdx.x & 31; s < t.p.seqs; s += 32) {
+        block = (t.split ? 1 : 2) * t.tile_tokens;
+        mine = look(threadIdx.x & 31, mine_lo, mine_hi);
+        int top = mine_hi;
+#pragma unroll 1
+        for (int s = 32 + (threadIdx.x & 31); s < t.p.seqs; s += 32) {
             int lo, hi;
-            span(s, lo, hi);
+            look(s, lo, hi);
             top = max(top, hi);
         }
         v = __reduce_max_sync(0xFFFFFFFFu, top) - 1;
@@ -238,42 +278,42 @@ struct PromptSchedule {
     // item i (they come in ascending order); false: there is none
     __device__ __forceinline__ bool find(int64_t i, PromptItem& it) {
         const int heads = t.p.cache.kv_heads;
+#pragma unroll 1
         while (v >= 0 && i >= before + (int64_t)count * heads) {
             before += (int64_t)count * heads;
             if (--v >= 0) count = have(v);
         }
         if (v < 0) return false;
-        int nth = (int)((i - before) / heads);
-        it.head = (int)((i - before) % heads);
+        int nth = (int)(i - before) / heads;
+        it.head = (int)(i - before) - nth * heads;
+#pragma unroll 1
         for (int s0 = 0; s0 < t.p.seqs; s0 += 32) {
-            int lo = 0, hi = 0;
-            if (s0 + (int)(threadIdx.x & 31) < t.p.seqs) span(s0 + (threadIdx.x & 31), lo, hi);
-            uint32_t with = __ballot_sync(0xFFFFFFFFu, v >= lo && v < hi);
-            const int n = __popc(with);
+            int lo;
+            PromptSeq q;
+            uint32_t which = with(s0, v, lo, q);
+            const int n = __popc(which);
             if (nth >= n) {
                 nth -= n;
                 continue;
             }
-            for (; nth > 0; nth--) with &= with - 1;
-            const int lane = __ffs(with) - 1;
+            for (; nth > 0; nth--) which &= which - 1;
+            const int lane = __ffs(which) - 1;
             it.seq = s0 + lane;
-            lo = __shfl_sync(0xFFFFFFFFu, lo, lane);
+            it.row0 = __shfl_sync(0xFFFFFFFFu, q.row0, lane);
+            it.rows = __shfl_sync(0xFFFFFFFFu, q.rows, lane);
+            it.keys = __shfl_sync(0xFFFFFFFFu, q.keys, lane);
+            it.token0 = (v - __shfl_sync(0xFFFFFFFFu, lo, lane)) * block;
             break;
         }
-        const PromptSeq q = prompt_seq(t.p, it.seq);
-        it.row0 = q.row0;
-        it.rows = q.rows;
-        it.keys = q.keys;
-        it.token0 = (v - max(0, q.keys - q.rows) / block) * block;
         auto tiles = [&](int token) {  // key tiles that a tile of rows starting at this token sees
-            if (token >= q.rows) return 0;
-            const int last = q.keys - q.rows + min(q.rows, token + t.tile_tokens) - 1;
+            if (token >= it.rows) return 0;
+            const int last = it.keys - it.rows + min(it.rows, token + t.tile_tokens) - 1;
             return last < 0 ? 0 : last / PA_KEYS + 1;
         };
-        it.from = it.split = it.piece = 0;
+        it.from = it.piece = it.last = 0;
+        it.split = t.split;
         it.n0 = tiles(it.token0);
-        it.n1 = tiles(it.token0 + t.tile_tokens);
-        it.last = 0;
+        it.n1 = t.split ? 0 : tiles(it.token0 + t.tile_tokens);
         return true;
     }
 };
@@ -363,14 +403,14 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         const float scale = p.scale_log2;
         uint32_t s_phase = 0, o_phase[2] = {0, 0}, half_phase = 0;
         for (int number = 0; items.next(sh, it, failed); number++) {
-            const int n = it.tiles(g), step = TREE && it.split ? 2 : 1;
-            const int first = it.token0 + (TREE && it.split ? 0 : g * tile_tokens), token = first + my_token;
+            const int n = it.tiles(g), step = it.split ? 2 : 1;
+            const int first = it.token0 + (it.split ? 0 : g * tile_tokens), token = first + my_token;
             const bool mine = r < group * tile_tokens && token < it.rows;
             const int last_key = it.keys - it.rows + token;  // prompt: that the row sees
             const int all_see = TREE ? it.context - 1 : it.keys - it.rows + first + (warp & 3) * 32 / group;  // that every row of this warp sees
             const uint64_t word = TREE && mine && it.keys > 0 ? ancestors_of(t.tree, it.row0 + token, token) & ((uint64_t)-1 >> (64 - it.rows)) : 0;
             float m = -INFINITY, l = 0.f;
-            int j = it.from + (TREE && it.split ? g : 0);  // the key tile
+            int j = it.from + (it.split ? g : 0);  // the key tile
             for (int i_tile = 0; i_tile < n; i_tile++, j += step) {
                 if (!pa_wait(&sh->s_full[g], s_phase)) {
                     failed = true;
@@ -474,7 +514,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             bf16* const to = p.out + ((size_t)row * p.q_heads + head) * p.cache.dim;
             const int d = p.cache.dim;
             bool odd = false;  // something is not finite
-            const bool halves = TREE && it.split && it.tiles(1) > 0;
+            const bool halves = it.split && it.tiles(1) > 0;
             if (n > 0 || (halves && g == 0)) {
                 if (!pa_wait(&sh->o_full[g], o_phase[g])) {
                     failed = true;
@@ -483,7 +523,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 o_phase[g] ^= 1;
                 tc_fence_after();
             }
-            if (TREE && g == 0 && !halves && it.tiles(1) > 0) o_phase[1] ^= 1;  // the other group's
+            if (g == 0 && !halves && it.tiles(1) > 0) o_phase[1] ^= 1;  // the other group's
             if (TREE && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l = __uint_as_float(0x7FC00000u);
             if (halves && g == 1) {  // the first group adds both halves up
                 sh->half_max[r] = m;
@@ -512,58 +552,75 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 keep = ex2((m - ref) * scale), take = ex2((m1 - ref) * scale);
                 l = l * keep + sh->half_sum[r] * take;
             }
-            // the row's sums, 32 at a time
-            auto sums = [&](int c, uint32_t(&o)[32]) {
-                tmem_ld32_start(o_at + c, o);
-                tmem_wait_ld32(o);
-                if (halves) {
-                    uint32_t o1[32];
-                    tmem_ld32_start(o_at + DIM + c, o1);
-                    tmem_wait_ld32(o1);
+            // The sums leave by 16 rows and 32 columns: a lane has rows 16 b + lane / 4 and 8 on, so that what four lanes store is contiguous.  (A thread
+            // storing its own row touches 32 rows with every store.)
+            const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+            const bool whole = !(TREE && it.piece);
+            if (whole && n > 0) odd = !(l < INFINITY) || scores_too_large(top, scale);
+            const int rows = t.c.piece_rows, at = it.split ? 0 : g * PA_ROWS;
+            float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
+            if (!whole && n > 0 && r < group * tile_tokens) {
+                piece[rows * DIM + at + r] = top;
+                piece[rows * (DIM + 1) + at + r] = l;
+            }
+            if (n > 0) {
+                const float factor = whole ? inv : 1.f;  // of this thread's row
+                uint32_t strange = 0;                    // rows with something that is not finite: bit b * 2 + e, rows 16 b + 8 e + lane / 4
 #pragma unroll
-                    for (int i = 0; i < 32; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * keep + __uint_as_float(o1[i]) * take);
-                }
-            };
-            if (TREE && it.piece && (n > 0 || !it.split)) {
-                const int rows = t.c.piece_rows, at = (it.split ? 0 : g * PA_ROWS) + r;
-                float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
-                if (r < group * tile_tokens) {
-                    piece[rows * DIM + at] = n > 0 ? top : -INFINITY;
-                    piece[rows * (DIM + 1) + at] = n > 0 ? l : 0.f;
-                }
+                for (int b = 0; b < 2; b++) {
+                    float f0[2], f1[2];
+                    bf16* out[2];
+                    float* part[2];
+#pragma unroll
+                    for (int e = 0; e < 2; e++) {
+                        const int from = 16 * b + 8 * e + (lane >> 2);  // the lane that has the row
+                        f0[e] = __shfl_sync(0xFFFFFFFFu, factor * (halves ? keep : 1.f), from);
+                        f1[e] = __shfl_sync(0xFFFFFFFFu, factor * take, from);
+                        const bool real = __shfl_sync(0xFFFFFFFFu, mine, from);
+                        const int row_at = __shfl_sync(0xFFFFFFFFu, row, from), head_at = __shfl_sync(0xFFFFFFFFu, head, from);
+                        out[e] = real && whole ? p.out + ((size_t)row_at * p.q_heads + head_at) * d : nullptr;
+                        part[e] = real && !whole ? piece + (size_t)(at + (warp & 3) * 32 + from) * DIM : nullptr;
+                    }
 #pragma unroll 1
-                for (int c = 0; c < DIM; c += 32) {
-                    uint32_t o[32];
-                    sums(c, o);
-                    if (mine)
+                    for (int c = 0; c < DIM; c += 32) {
+                        uint32_t o[16];
+                        tmem_ld_16x32(o_at + (uint32_t)(16 * b << 16) + c, o);
+                        tmem_wait_ld16(o);
+                        if (halves) {
+                            uint32_t o1[16];
+                            tmem_ld_16x32(o_at + (uint32_t)(16 * b << 16) + DIM + c, o1);
+                            tmem_wait_ld16(o1);
 #pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<float4*>(piece + (size_t)at * DIM + c + i) = make_float4(__uint_as_float(o[i]), __uint_as_float(o[i + 1]), __uint_as_float(o[i + 2]), __uint_as_float(o[i + 3]));
-                }
-                tc_fence_before();
-            } else if (n > 0) {
-                const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-                odd = !(l < INFINITY) || scores_too_large(top, scale);
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0[i >> 1 & 1] + __uint_as_float(o1[i]) * f1[i >> 1 & 1]);
+                        } else {
 #pragma unroll
-                for (int c = 0; c < DIM; c += 32) {
-                    uint32_t o[32];
-                    sums(c, o);
-                    uint32_t largest = 0;
+                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0[i >> 1 & 1]);
+                        }
 #pragma unroll
-                    for (int i = 0; i < 32; i++) largest = max(largest, o[i] & 0x7FFFFFFFu);
-                    odd |= largest >= 0x7F800000u;
+                        for (int e = 0; e < 2; e++) {
+                            uint32_t largest = 0, w[4];
 #pragma unroll
-                    for (int i = 0; i < 32; i += 8) {
-                        uint4 v;
-                        v.x = pack_bf16(__uint_as_float(o[i]) * inv, __uint_as_float(o[i + 1]) * inv);
-                        v.y = pack_bf16(__uint_as_float(o[i + 2]) * inv, __uint_as_float(o[i + 3]) * inv);
-                        v.z = pack_bf16(__uint_as_float(o[i + 4]) * inv, __uint_as_float(o[i + 5]) * inv);
-                        v.w = pack_bf16(__uint_as_float(o[i + 6]) * inv, __uint_as_float(o[i + 7]) * inv);
-                        if (mine && c + i < d) *reinterpret_cast<uint4*>(to + c + i) = v;
+                            for (int x = 0; x < 4; x++) {
+                                const uint32_t u = o[4 * x + 2 * e], v = o[4 * x + 2 * e + 1];
+                                largest = max(largest, max(u & 0x7FFFFFFFu, v & 0x7FFFFFFFu));
+                                if (TREE && part[e]) *reinterpret_cast<uint2*>(part[e] + c + 8 * x + 2 * (lane & 3)) = make_uint2(u, v);
+                                w[x] = pack_bf16(__uint_as_float(u), __uint_as_float(v));
+                            }
+                            if (largest >= 0x7F800000u) strange |= 1u << (2 * b + e);
+                            quad_transpose(w);
+                            if (out[e] && c + 8 * (lane & 3) < d) *reinterpret_cast<uint4*>(out[e] + c + 8 * (lane & 3)) = make_uint4(w[0], w[1], w[2], w[3]);
+                        }
                     }
                 }
                 tc_fence_before();
-            } else if (!TREE && mine) {
+                if (__any_sync(0xFFFFFFFFu, strange)) {  // to the lanes that have the rows
+#pragma unroll
+                    for (int k = 0; k < 4; k++) {
+                        const uint32_t by = __ballot_sync(0xFFFFFFFFu, strange >> k & 1);
+                        if (lane >> 3 == k && (by >> (4 * (lane & 7)) & 15)) odd = whole;
+                    }
+                }
+            } else if (!TREE && mine && !(it.split && g)) {
                 for (int i = 0; i < d; i += 8) *reinterpret_cast<uint4*>(to + i) = make_uint4(0u, 0u, 0u, 0u);
             }
             if (halves) {
@@ -572,7 +629,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             }
             // Rows with an Inf or a NaN in their sums, and rows whose pages are not in the cache, go key by key: the first may have
             // come from a key that the row does not see (0 x Inf), the second's keys were not read.
-            if (!TREE) odd |= *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
+            if (!TREE) odd |= !(it.split && g) && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
             uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && odd);
             while (again) {
                 const int l2 = __ffs(again) - 1;
@@ -641,7 +698,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                         if (failed) break;
                         const uint32_t bar = g_smem_u32(&sh->q_full[g]);
                         mbar_expect_if(bar, (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens), issue);
-                        const int first = it.row0 + it.token0 + (TREE && it.split ? 0 : g * t.tile_tokens);
+                        const int first = it.row0 + it.token0 + (it.split ? 0 : g * t.tile_tokens);
 #pragma unroll
                         for (int c = 0; c < CHUNKS; c++) tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, first, bar, issue);
                     }
@@ -654,45 +711,63 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             if (failed) break;
         }
     } else if (warp == PA_MMA_WARP) {
+        // Everything here is laid out for the pace of the issuing thread: the group is a constant in every place (as a variable the kernel lost 10 %).
         const uint32_t issue = elect_one();
         uint32_t q_phase[2] = {0, 0}, p_phase[2] = {0, 0};
-        int base = 0;  // loads before this item, modulo two laps of the ring
-        auto scores = [&](int g, int stage) {
+        struct Place {  // in the ring
+            int s = 0;
+            uint32_t phase = 0;
+            __device__ __forceinline__ void advance(int by) {
+                s += by;
+                if (s >= STAGES) s -= STAGES, phase ^= 1;
+            }
+        } begin;
+        typedef std::integral_constant<int, 0> Group0;
+        typedef std::integral_constant<int, 1> Group1;
+        auto there = [&](const Place& at) {  // its keys or values have arrived
+            if (!pa_wait(&sh->kv_full[at.s], at.phase)) failed = true;
+            tc_fence_after();
+            return !failed;
+        };
+        auto scores = [&](auto group, int stage) {  // S = Q K^T
+            constexpr int g = decltype(group)::value;
             const uint64_t a = smem_desc_sw128(smem + (uint32_t)(g * CHUNKS * PA_CHUNK)), b = smem_desc_sw128(kv_smem + (uint32_t)(stage * STAGE_BYTES));
 #pragma unroll
             for (int c = 0; c < CHUNKS; c++)
                 pa_mma_qk(tmem + (uint32_t)(g * PA_KEYS), a + (uint64_t)(c * (PA_CHUNK >> 4)), b + (uint64_t)(c * (PA_CHUNK >> 4)), IDESC_QK, c > 0, issue);
             tc_commit_if(&sh->s_full[g], issue);
         };
+        auto first_scores = [&](auto group, int stage, int tiles) {
+            constexpr int g = decltype(group)::value;
+            if (!pa_wait(&sh->q_full[g], q_phase[g])) {
+                failed = true;
+                return false;
+            }
+            q_phase[g] ^= 1;
+            tc_fence_after();
+            scores(group, stage);
+            if (tiles == 1) tc_commit_if(&sh->q_empty[g], issue);
+            return true;
+        };
+        auto products = [&](auto group, int stage, bool accumulate) {  // O += P V
+            constexpr int g = decltype(group)::value;
+            const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(stage * STAGE_BYTES), PA_CHUNK);
+#pragma unroll
+            for (int h = 0; h < 2; h++) {
+                if (!pa_wait(h ? &sh->p_full[g] : &sh->p_half[g], p_phase[g])) {
+                    failed = true;
+                    return false;
+                }
+                tc_fence_after();
+                pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, accumulate || h > 0, issue);
+            }
+            p_phase[g] ^= 1;
+            return true;
+        };
         while (items.next(sh, it, failed)) {
             const int n = it.all(), nt[2] = {it.tiles(0), it.tiles(1)};
             if (n == 0) continue;
-            const bool split = TREE && it.split, tail = max(it.n0, it.n1) * PA_KEYS > it.keys;
-            // the stage of the keys or values of key tile j, once they are there; -1: the wait ran out
-            auto stage_of = [&](bool values, int j) {
-                const int at = base + (values ? (j + 1 < n ? 2 * j + 2 : 2 * n - 1) : (j ? 2 * j - 1 : 0)), stage = at % STAGES;
-                if (!pa_wait(&sh->kv_full[stage], (uint32_t)(at / STAGES) & 1)) failed = true;
-                tc_fence_after();
-                return stage;
-            };
-            auto queries = [&](int g) {
-                if (!pa_wait(&sh->q_full[g], q_phase[g])) failed = true;
-                q_phase[g] ^= 1;
-                tc_fence_after();
-            };
-            auto products = [&](int g, int stage, bool accumulate) {  // O += P V
-                const uint64_t b = smem_desc_sw128_n(kv_smem + (uint32_t)(stage * STAGE_BYTES), PA_CHUNK);
-#pragma unroll
-                for (int h = 0; h < 2; h++) {
-                    if (!pa_wait(h ? &sh->p_full[g] : &sh->p_half[g], p_phase[g])) {
-                        failed = true;
-                        return;
-                    }
-                    tc_fence_after();
-                    pa_mma_pv(tmem + O_COLUMN + (uint32_t)(g * DIM), tmem + (uint32_t)(g * PA_KEYS + 32 * h), b + (uint64_t)(h * 512), IDESC_PV, accumulate || h > 0, issue);
-                }
-                p_phase[g] ^= 1;
-            };
+            const bool tail = max(it.n0, it.n1) * PA_KEYS > it.keys;
             auto zero_tail = [&](int stage, int j) {  // values behind the last key: their weights are 0, and 0 x whatever lies there has to be 0
                 if (!tail || j != n - 1) return;
                 for (int c = 0; c < CHUNKS; c++)
@@ -701,58 +776,69 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
                 __syncwarp();
             };
-            const int first_keys = stage_of(false, 0);
-            for (int g = 0; g < 2 && !failed; g++) {
-                if (nt[g] == 0) continue;
-                queries(g);
-                const int stage = split && g ? stage_of(false, 1) : first_keys;
-                if (failed) break;
-                scores(g, stage);
-                if (nt[g] == 1) tc_commit_if(&sh->q_empty[g], issue);
-                if (split) tc_commit_if(&sh->kv_empty[stage], issue);
+            Place keys = begin, values = begin;  // keys 0, keys 1, values 0, keys 2, values 1, .., the last two values
+            values.advance(n > 1 ? 2 : 1);
+            if (!there(keys)) break;
+            if (!it.split) {
+                if ((nt[0] && !first_scores(Group0{}, keys.s, nt[0])) || (nt[1] && !first_scores(Group1{}, keys.s, nt[1]))) break;
+                tc_commit_if(&sh->kv_empty[keys.s], issue);
+                keys.advance(1);
+                for (int j = 0; j < n; j++) {
+                    if (!there(values)) break;
+                    zero_tail(values.s, j);
+                    bool more = false;
+                    auto step = [&](auto group) {
+                        constexpr int g = decltype(group)::value;
+                        if (!products(group, values.s, j > 0)) return;
+                        if (j + 1 == nt[g]) return tc_commit_if(&sh->o_full[g], issue);
+                        if (!more && !there(keys)) return;
+                        more = true;
+                        scores(group, keys.s);
+                        if (j + 2 == nt[g]) tc_commit_if(&sh->q_empty[g], issue);
+                    };
+                    if (j < nt[0]) step(Group0{});
+                    if (j < nt[1] && !failed) step(Group1{});
+                    if (failed) break;
+                    tc_commit_if(&sh->kv_empty[values.s], issue);
+                    if (more) {
+                        tc_commit_if(&sh->kv_empty[keys.s], issue);
+                        keys.advance(2);
+                    }
+                    values.advance(j + 2 < n ? 2 : 1);
+                }
+            } else {  // a key tile is one group's, and the next one the other's
+                if (!first_scores(Group0{}, keys.s, nt[0])) break;
+                tc_commit_if(&sh->kv_empty[keys.s], issue);
+                keys.advance(1);
+                if (n > 1) {
+                    if (!there(keys) || !first_scores(Group1{}, keys.s, nt[1])) break;
+                    tc_commit_if(&sh->kv_empty[keys.s], issue);
+                    keys.advance(2);
+                }
+                for (int j = 0; j < n; j++) {
+                    if (!there(values)) break;
+                    zero_tail(values.s, j);
+                    auto step = [&](auto group) {
+                        constexpr int g = decltype(group)::value;
+                        if (!products(group, values.s, j >= 2)) return;
+                        tc_commit_if(&sh->kv_empty[values.s], issue);
+                        if (j + 2 >= n) return tc_commit_if(&sh->o_full[g], issue);
+                        if (!there(keys)) return;
+                        scores(group, keys.s);
+                        tc_commit_if(&sh->kv_empty[keys.s], issue);
+                        keys.advance(2);
+                        if (j + 4 >= n) tc_commit_if(&sh->q_empty[g], issue);
+                    };
+                    if (j & 1) step(Group1{});
+                    else step(Group0{});
+                    if (failed) break;
+                    values.advance(j + 2 < n ? 2 : 1);
+                }
             }
             if (failed) break;
-            if (!split) tc_commit_if(&sh->kv_empty[first_keys], issue);
-            for (int j = 0; j < n && !failed; j++) {
-                const int values = stage_of(true, j);
-                if (failed) break;
-                zero_tail(values, j);
-                if (split) {  // group j & 1 alone, whose next key tile is j + 2
-                    const int g = j & 1;
-                    products(g, values, j >= 2);
-                    if (failed) break;
-                    tc_commit_if(&sh->kv_empty[values], issue);
-                    if (j + 2 >= n) {
-                        tc_commit_if(&sh->o_full[g], issue);
-                        continue;
-                    }
-                    const int keys = stage_of(false, j + 2);
-                    if (failed) break;
-                    scores(g, keys);
-                    tc_commit_if(&sh->kv_empty[keys], issue);
-                    if (j + 4 >= n) tc_commit_if(&sh->q_empty[g], issue);
-                    continue;
-                }
-                int keys = -1;
-                for (int g = 0; g < 2; g++) {
-                    if (j >= nt[g]) continue;
-                    products(g, values, j > 0);
-                    if (failed) break;
-                    if (j + 1 == nt[g]) {
-                        tc_commit_if(&sh->o_full[g], issue);
-                        continue;
-                    }
-                    if (keys < 0) keys = stage_of(false, j + 1);
-                    if (failed) break;
-                    scores(g, keys);
-                    if (j + 2 == nt[g]) tc_commit_if(&sh->q_empty[g], issue);
-                }
-                if (failed) break;
-                tc_commit_if(&sh->kv_empty[values], issue);
-                if (keys >= 0) tc_commit_if(&sh->kv_empty[keys], issue);
-            }
-            if (failed) break;
-            base = (base + 2 * n) % (2 * STAGES);
+            const int on = begin.s + 2 * n;
+            begin.s = on % STAGES;
+            begin.phase ^= (uint32_t)(on / STAGES) & 1;
         }
     } else if (warp == PA_SCHED_WARP) {
         int slot = 0;
