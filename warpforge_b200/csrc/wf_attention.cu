@@ -43,7 +43,7 @@ int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int l
 }  // namespace wf
 static int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
     if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
-    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192)
+    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
         return set_error(c, WF_ERR_SHAPE, "%s: bad shape tokens=%lld seqs=%d q_heads=%d", what, (long long)tokens, seqs, q_heads);
     if (q_heads % cache->kv_heads) return set_error(c, WF_ERR_SHAPE, "%s: %d query heads over %d kv heads", what, q_heads, cache->kv_heads);
     if (q_heads / cache->kv_heads > 128) return set_error(c, WF_ERR_TOO_LARGE, "%s: more than 128 query heads for each kv head", what);
@@ -113,6 +113,7 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     if (rc != WF_OK) return rc;
     // Items of two tiles of rows; of one, on which both groups of a CTA work, where that many would leave half of the device idle.
     const int64_t pairs = (p.tokens + (int64_t)p.seqs * (2 * t.tile_tokens - 1)) / (2 * t.tile_tokens) * p.cache.kv_heads;
+    if (pairs > (1LL << 31) - 65536) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens of %d heads", what, (long long)p.tokens, p.q_heads);
     t.split = 2 * pairs <= c->sm_count;
     const int64_t items = t.split ? (p.tokens + (int64_t)p.seqs * (t.tile_tokens - 1)) / t.tile_tokens * p.cache.kv_heads : pairs;
     return launch_attention(c, what, prompt_tiles_kernel<CHUNKS, false>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);

@@ -17,18 +17,14 @@ constexpr int PA_ROWS = 128, PA_KEYS = 128;  // of a tile
 constexpr int PA_SOFTMAX_WARPS = 8;          // four a tile
 constexpr int PA_LOAD_WARP = 8, PA_MMA_WARP = 9, PA_SCHED_WARP = 10;  // and one that has nothing to do: setmaxnreg wants four
 constexpr int PA_THREADS = 12 * 32;
-// Registers: 168 a thread at launch; the softmax warps, which hold a row of S, take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
-constexpr int PA_SOFTMAX_REGS = 216, PA_OTHER_REGS = 72;
+// Registers: 168 a thread at launch; the softmax warps, which hold a row of S, take what the others give back (256 x 224 + 128 x 56 = 384 x 168).
+constexpr int PA_SOFTMAX_REGS = 224, PA_OTHER_REGS = 56;
 constexpr int PA_CHUNK = PA_KEYS * 128;      // bytes of 128 rows x 64 elements
 constexpr int PA_ITEMS = 2;                  // items announced ahead
 // Which of the 32 pairs of weights of 64 keys are taken by the cubic: two in five, so that the special function unit and the fp32 units are through at about the same time.
 __host__ __device__ constexpr bool PA_CUBIC(int pair) { return pair % 5 == 1 || pair % 5 == 3; }
 constexpr float PA_RESCALE = 8.f;            // the running maximum is followed when it has grown by this many powers of two
 constexpr int PA_MAX_STAGES = 12;
-template <int CHUNKS> struct PromptShape {  // by the head's dimension in 64 elements, rounded up
-    static constexpr int STAGES = CHUNKS == 2 ? 5 : 12, STAGE_BYTES = CHUNKS * PA_CHUNK, Q_BYTES = 2 * CHUNKS * PA_CHUNK;
-    static constexpr int SMEM = Q_BYTES + STAGES * STAGE_BYTES + 1024;
-};
 
 // Two tiles of rows of one sequence and kv head.
 struct PromptItem {
@@ -126,33 +122,6 @@ __device__ __forceinline__ void tmem_wait_ld32(uint32_t* r) {
                  :
                  : "memory");
 }
-// 16 rows x 32 columns: a lane has the columns 8 x + 2 q and 8 x + 2 q + 1 (q = lane % 4, x = 0 .. 3) of the rows lane / 4 (r[4 x], r[4 x + 1]) and lane / 4 + 8
-// (r[4 x + 2], r[4 x + 3])
-__device__ __forceinline__ void tmem_ld_16x32(uint32_t taddr, uint32_t (&r)[16]) {
-    asm volatile("tcgen05.ld.sync.aligned.16x256b.x4.b32 {%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
-                 : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]), "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]),
-                   "=r"(r[12]), "=r"(r[13]), "=r"(r[14]), "=r"(r[15])
-                 : "r"(taddr)
-                 : "memory");
-}
-__device__ __forceinline__ void tmem_wait_ld16(uint32_t (&r)[16]) {
-    asm volatile("tcgen05.wait::ld.sync.aligned;"
-                 : "+r"(r[0]), "+r"(r[1]), "+r"(r[2]), "+r"(r[3]), "+r"(r[4]), "+r"(r[5]), "+r"(r[6]), "+r"(r[7]), "+r"(r[8]), "+r"(r[9]), "+r"(r[10]), "+r"(r[11]),
-                   "+r"(r[12]), "+r"(r[13]), "+r"(r[14]), "+r"(r[15])
-                 :
-                 : "memory");
-}
-// Lane q of four has word x of column x of a 4 x 4 matrix in w[x]; afterwards its row q.
-__device__ __forceinline__ void quad_transpose(uint32_t (&w)[4]) {
-    const bool odd = threadIdx.x & 1, high = threadIdx.x & 2;
-    // exchange with the neighbour, then two on: blocks of one, then of two
-    const uint32_t a = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[0] : w[1], 1), b = __shfl_xor_sync(0xFFFFFFFFu, odd ? w[2] : w[3], 1);
-    if (odd) w[0] = a, w[2] = b;
-    else w[1] = a, w[3] = b;
-    const uint32_t c = __shfl_xor_sync(0xFFFFFFFFu, high ? w[0] : w[2], 2), d = __shfl_xor_sync(0xFFFFFFFFu, high ? w[1] : w[3], 2);
-    if (high) w[0] = c, w[1] = d;
-    else w[2] = c, w[3] = d;
-}
 __device__ __forceinline__ void tmem_st32(uint32_t taddr, const uint32_t* r) {
     asm volatile(
         "tcgen05.st.sync.aligned.32x32b.x32.b32 [%0], "
@@ -178,6 +147,13 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 // integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a cubic on [-1/2, 1/2], 1 at 0, with the smallest largest relative error (1.0e-4, 1/38 of
 // what a weight may be off by its rounding to bf16), n added to the exponent.  0 from -127 on.
 __device__ __forceinline__ float2 add2(float2 a, float2 b);
+__device__ __forceinline__ float2 mul2(float2 a, float2 b) {
+    float2 d;
+    asm("{\n\t.reg .b64 x, y, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmul.rn.f32x2 w, x, y;\n\tmov.b64 {%0, %1}, w;\n\t}"
+        : "=f"(d.x), "=f"(d.y)
+        : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+    return d;
+}
 __device__ __forceinline__ float2 ex2_by_cubic(float2 x) {
     x.x = fmaxf(x.x, -127.f);
     x.y = fmaxf(x.y, -127.f);
@@ -202,13 +178,20 @@ __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) { return
 struct PromptShared {
     uint64_t q_full[2], q_empty[2];
     uint64_t s_full[2], p_half[2], p_full[2], o_full[2];  // scores; weights of the first 64 keys, of all; sums
-    uint64_t half_ready, half_taken;  // tree, one tile of rows: the second group's maxima and sums lie in half_max and half_sum; they and its O have been read
-    float half_max[PA_ROWS], half_sum[PA_ROWS];
+    uint64_t half_ready, half_taken;  // one tile of rows, two groups: their maxima and sums lie in half_max and half_sum; both O have been read
+    float half_max[2][PA_ROWS], half_sum[2][PA_ROWS];
+    uint32_t half_odd[4];  // rows that the second group has seen to be not finite
     uint64_t kv_full[PA_MAX_STAGES], kv_empty[PA_MAX_STAGES];
     uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
     PromptItem items[PA_ITEMS];
     int bad_page;  // an item of this number and before has pages outside the cache
     uint32_t tmem;
+};
+
+template <int CHUNKS> struct PromptShape {  // by the head's dimension in 64 elements, rounded up
+    static constexpr int STAGES = CHUNKS == 2 ? 5 : 12, STAGE_BYTES = CHUNKS * PA_CHUNK, Q_BYTES = 2 * CHUNKS * PA_CHUNK;
+    static constexpr int SMEM = Q_BYTES + STAGES * STAGE_BYTES + (int)sizeof(PromptShared);
+    static_assert(SMEM <= 227 * 1024, "shared memory");
 };
 
 // The next item of the ring; false: no more, or a wait ran out.
@@ -234,7 +217,7 @@ struct PromptSchedule {
     const PromptTiles& t;
     int block;       // tokens of an item
     int v;           // where the cursor is
-    int64_t before;  // items with a larger v
+    int before;      // items with a larger v
     int count;       // sequences that have this v
     PromptSeq mine;  // of the first 32 sequences, this lane's; the others are looked up when they are needed
     int mine_lo, mine_hi;
@@ -276,16 +259,16 @@ struct PromptSchedule {
         count = v >= 0 ? have(v) : 0;
     }
     // item i (they come in ascending order); false: there is none
-    __device__ __forceinline__ bool find(int64_t i, PromptItem& it) {
+    __device__ __forceinline__ bool find(int i, PromptItem& it) {
         const int heads = t.p.cache.kv_heads;
 #pragma unroll 1
-        while (v >= 0 && i >= before + (int64_t)count * heads) {
-            before += (int64_t)count * heads;
+        while (v >= 0 && i >= before + count * heads) {
+            before += count * heads;
             if (--v >= 0) count = have(v);
         }
         if (v < 0) return false;
-        int nth = (int)(i - before) / heads;
-        it.head = (int)(i - before) - nth * heads;
+        int nth = (i - before) / heads;
+        it.head = i - before - nth * heads;
 #pragma unroll 1
         for (int s0 = 0; s0 < t.p.seqs; s0 += 32) {
             int lo;
@@ -351,10 +334,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
     constexpr uint32_t IDESC = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(PA_ROWS / 16) << 24;  // fp32 += bf16 x bf16, 128 rows
     constexpr uint32_t IDESC_QK = IDESC | (uint32_t)(PA_KEYS / 8) << 17, IDESC_PV = IDESC | 1u << 16 | (uint32_t)(DIM / 8) << 17;
     constexpr uint32_t O_COLUMN = 2 * PA_KEYS;  // TMEM: S of tile 0, S of tile 1, O of tile 0, O of tile 1
-    extern __shared__ uint8_t raw[];
-    __shared__ PromptShared sh_;
-    PromptShared* const sh = &sh_;
-    const uint32_t smem = (g_smem_u32(raw) + 1023u) & ~1023u, kv_smem = smem + PromptShape<CHUNKS>::Q_BYTES;
+    extern __shared__ __align__(1024) uint8_t raw[];  // the kernel has no other shared memory: it begins where the swizzle wants it to
+    PromptShared* const sh = reinterpret_cast<PromptShared*>(raw + PromptShape<CHUNKS>::Q_BYTES + STAGES * STAGE_BYTES);
+    const uint32_t smem = g_smem_u32(raw), kv_smem = smem + PromptShape<CHUNKS>::Q_BYTES;
     const PromptParams& p = t.p;
     const int warp = __shfl_sync(0xFFFFFFFFu, (int)threadIdx.x >> 5, 0), lane = threadIdx.x & 31;
     if (warp == PA_LOAD_WARP && lane == 0) {
@@ -366,8 +348,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             g_mbar_init(&sh->p_full[g], 4);
             g_mbar_init(&sh->o_full[g], 1);
         }
-        g_mbar_init(&sh->half_ready, 4);
-        g_mbar_init(&sh->half_taken, 4);
+        g_mbar_init(&sh->half_ready, 8);
+        g_mbar_init(&sh->half_taken, 8);
         for (int i = 0; i < STAGES; i++) {
             g_mbar_init(&sh->kv_full[i], 1);
             g_mbar_init(&sh->kv_empty[i], 1);
@@ -511,121 +493,96 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             }
             if (failed) break;
             const int row = it.row0 + token, head = it.head * group + my_head;
-            bf16* const to = p.out + ((size_t)row * p.q_heads + head) * p.cache.dim;
             const int d = p.cache.dim;
             bool odd = false;  // something is not finite
             const bool halves = it.split && it.tiles(1) > 0;
-            if (n > 0 || (halves && g == 0)) {
+            if (n > 0) {
                 if (!pa_wait(&sh->o_full[g], o_phase[g])) {
                     failed = true;
                     break;
                 }
-                o_phase[g] ^= 1;
                 tc_fence_after();
             }
-            if (g == 0 && !halves && it.tiles(1) > 0) o_phase[1] ^= 1;  // the other group's
             if (TREE && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l = __uint_as_float(0x7FC00000u);
-            if (halves && g == 1) {  // the first group adds both halves up
-                sh->half_max[r] = m;
-                sh->half_sum[r] = l;
+            float keep = 1.f, take = 0.f, top = m;
+            if (halves) {  // both groups add both up, half of the columns each
+                sh->half_max[g][r] = m;
+                sh->half_sum[g][r] = l;
                 __syncwarp();
                 if (lane == 0) g_mbar_arrive(&sh->half_ready);
+                if (!pa_wait(&sh->half_ready, half_phase) || !pa_wait(&sh->o_full[g ^ 1], o_phase[g ^ 1])) {
+                    failed = true;
+                    break;
+                }
+                tc_fence_after();
+                const float other = sh->half_max[g ^ 1][r];
+                top = fmaxf(m, other);
+                const float ref = top == -INFINITY ? 0.f : top;
+                keep = ex2((m - ref) * scale), take = ex2((other - ref) * scale);
+                l = l * keep + sh->half_sum[g ^ 1][r] * take;
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) o_phase[e] ^= it.tiles(e) > 0;  // the other group's, too
+            const bool whole = !(TREE && it.piece);
+            if (n > 0) {
+                const float inv = l == 0.f ? 0.f : __frcp_rn(l);
+                const float2 f0 = make_float2(whole ? keep * inv : keep, whole ? keep * inv : keep), f1 = make_float2(whole ? take * inv : take, whole ? take * inv : take);
+                const int rows = t.c.piece_rows, at = it.split ? r : g * PA_ROWS + r;
+                float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
+                if (!whole && r < group * tile_tokens && !(halves && g)) {
+                    piece[rows * DIM + at] = top;
+                    piece[rows * (DIM + 1) + at] = l;
+                }
+                // Few instructions and a small loop: it runs once an item, by one warp a scheduler at about three cycles an instruction.  (Transposed among four lanes, so that
+                // a store touches 8 rows and not 32, it took twice as long.)
+                float2 finite = make_float2(0.f, 0.f);  // the sum: an Inf or a NaN stays in it
+                const uint32_t other_at = o_at + (uint32_t)(g ? -DIM : DIM);
+#pragma unroll 1
+                for (int c = halves && g ? DIM / 2 : 0; c < (halves && !g ? DIM / 2 : DIM); c += 32) {
+                    uint32_t o[32];
+                    tmem_ld32_start(o_at + c, o);
+                    tmem_wait_ld32(o);
+                    float2* const x = reinterpret_cast<float2*>(o);
+#pragma unroll
+                    for (int i = 0; i < 16; i++) x[i] = mul2(x[i], f0);
+                    if (halves) {
+                        uint32_t o1[32];
+                        tmem_ld32_start(other_at + c, o1);
+                        tmem_wait_ld32(o1);
+#pragma unroll
+                        for (int i = 0; i < 16; i++) x[i] = fma2(reinterpret_cast<float2*>(o1)[i], f1, x[i]);
+                    }
+                    if (TREE && !whole) {
+                        if (mine)
+#pragma unroll
+                            for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(piece + (size_t)at * DIM + c + 4 * i) = make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y);
+                        continue;
+                    }
+#pragma unroll
+                    for (int i = 0; i < 16; i++) {
+                        finite = add2(finite, x[i]);
+                        o[i] = pack_bf16(x[i].x, x[i].y);
+                    }
+                    bf16* const to = p.out + ((size_t)row * p.q_heads + head) * d + c;
+#pragma unroll
+                    for (int i = 0; i < 4; i++)
+                        if (mine && c + 8 * i < d) *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                }
+                odd = whole && (!(l < INFINITY) || scores_too_large(top, scale) || !(fabsf(finite.x + finite.y) < INFINITY));
+                tc_fence_before();
+            } else if (!TREE && mine && !(it.split && g)) {
+                for (int i = 0; i < d; i += 8) *reinterpret_cast<uint4*>(p.out + ((size_t)row * p.q_heads + head) * d + i) = make_uint4(0u, 0u, 0u, 0u);
+            }
+            if (halves) {
+                const uint32_t which = __ballot_sync(0xFFFFFFFFu, odd);
+                if (g && lane == 0) sh->half_odd[warp & 3] = which;
+                if (lane == 0) g_mbar_arrive(&sh->half_taken);
                 if (!pa_wait(&sh->half_taken, half_phase)) {
                     failed = true;
                     break;
                 }
                 half_phase ^= 1;
-                continue;
-            }
-            float keep = 1.f, take = 0.f, top = m;
-            if (halves) {
-                if (!pa_wait(&sh->half_ready, half_phase) || !pa_wait(&sh->o_full[1], o_phase[1])) {
-                    failed = true;
-                    break;
-                }
-                half_phase ^= 1;
-                o_phase[1] ^= 1;
-                tc_fence_after();
-                const float m1 = sh->half_max[r];
-                top = fmaxf(m, m1);
-                const float ref = top == -INFINITY ? 0.f : top;
-                keep = ex2((m - ref) * scale), take = ex2((m1 - ref) * scale);
-                l = l * keep + sh->half_sum[r] * take;
-            }
-            // The sums leave by 16 rows and 32 columns: a lane has rows 16 b + lane / 4 and 8 on, so that what four lanes store is contiguous.  (A thread
-            // storing its own row touches 32 rows with every store.)
-            const float inv = l == 0.f ? 0.f : __frcp_rn(l);
-            const bool whole = !(TREE && it.piece);
-            if (whole && n > 0) odd = !(l < INFINITY) || scores_too_large(top, scale);
-            const int rows = t.c.piece_rows, at = it.split ? 0 : g * PA_ROWS;
-            float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
-            if (!whole && n > 0 && r < group * tile_tokens) {
-                piece[rows * DIM + at + r] = top;
-                piece[rows * (DIM + 1) + at + r] = l;
-            }
-            if (n > 0) {
-                const float factor = whole ? inv : 1.f;  // of this thread's row
-                uint32_t strange = 0;                    // rows with something that is not finite: bit b * 2 + e, rows 16 b + 8 e + lane / 4
-#pragma unroll
-                for (int b = 0; b < 2; b++) {
-                    float f0[2], f1[2];
-                    bf16* out[2];
-                    float* part[2];
-#pragma unroll
-                    for (int e = 0; e < 2; e++) {
-                        const int from = 16 * b + 8 * e + (lane >> 2);  // the lane that has the row
-                        f0[e] = __shfl_sync(0xFFFFFFFFu, factor * (halves ? keep : 1.f), from);
-                        f1[e] = __shfl_sync(0xFFFFFFFFu, factor * take, from);
-                        const bool real = __shfl_sync(0xFFFFFFFFu, mine, from);
-                        const int row_at = __shfl_sync(0xFFFFFFFFu, row, from), head_at = __shfl_sync(0xFFFFFFFFu, head, from);
-                        out[e] = real && whole ? p.out + ((size_t)row_at * p.q_heads + head_at) * d : nullptr;
-                        part[e] = real && !whole ? piece + (size_t)(at + (warp & 3) * 32 + from) * DIM : nullptr;
-                    }
-#pragma unroll 1
-                    for (int c = 0; c < DIM; c += 32) {
-                        uint32_t o[16];
-                        tmem_ld_16x32(o_at + (uint32_t)(16 * b << 16) + c, o);
-                        tmem_wait_ld16(o);
-                        if (halves) {
-                            uint32_t o1[16];
-                            tmem_ld_16x32(o_at + (uint32_t)(16 * b << 16) + DIM + c, o1);
-                            tmem_wait_ld16(o1);
-#pragma unroll
-                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0[i >> 1 & 1] + __uint_as_float(o1[i]) * f1[i >> 1 & 1]);
-                        } else {
-#pragma unroll
-                            for (int i = 0; i < 16; i++) o[i] = __float_as_uint(__uint_as_float(o[i]) * f0[i >> 1 & 1]);
-                        }
-#pragma unroll
-                        for (int e = 0; e < 2; e++) {
-                            uint32_t largest = 0, w[4];
-#pragma unroll
-                            for (int x = 0; x < 4; x++) {
-                                const uint32_t u = o[4 * x + 2 * e], v = o[4 * x + 2 * e + 1];
-                                largest = max(largest, max(u & 0x7FFFFFFFu, v & 0x7FFFFFFFu));
-                                if (TREE && part[e]) *reinterpret_cast<uint2*>(part[e] + c + 8 * x + 2 * (lane & 3)) = make_uint2(u, v);
-                                w[x] = pack_bf16(__uint_as_float(u), __uint_as_float(v));
-                            }
-                            if (largest >= 0x7F800000u) strange |= 1u << (2 * b + e);
-                            quad_transpose(w);
-                            if (out[e] && c + 8 * (lane & 3) < d) *reinterpret_cast<uint4*>(out[e] + c + 8 * (lane & 3)) = make_uint4(w[0], w[1], w[2], w[3]);
-                        }
-                    }
-                }
-                tc_fence_before();
-                if (__any_sync(0xFFFFFFFFu, strange)) {  // to the lanes that have the rows
-#pragma unroll
-                    for (int k = 0; k < 4; k++) {
-                        const uint32_t by = __ballot_sync(0xFFFFFFFFu, strange >> k & 1);
-                        if (lane >> 3 == k && (by >> (4 * (lane & 7)) & 15)) odd = whole;
-                    }
-                }
-            } else if (!TREE && mine && !(it.split && g)) {
-                for (int i = 0; i < d; i += 8) *reinterpret_cast<uint4*>(to + i) = make_uint4(0u, 0u, 0u, 0u);
-            }
-            if (halves) {
-                __syncwarp();
-                if (lane == 0) g_mbar_arrive(&sh->half_taken);
+                odd = !g && (odd || (sh->half_odd[warp & 3] >> lane & 1));  // the first group's
             }
             // Rows with an Inf or a NaN in their sums, and rows whose pages are not in the cache, go key by key: the first may have
             // come from a key that the row does not see (0 x Inf), the second's keys were not read.
@@ -860,11 +817,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         } else {
             PromptSchedule schedule{t};
             schedule.begin();
-            for (int64_t i = blockIdx.x; schedule.find(i, it);) {
+            for (int i = blockIdx.x; schedule.find(i, it);) {
                 unsigned int ahead = 0;
                 if (lane == 0) ahead = atomicAdd(&t.sched[0], 1u);
                 if (!announce(it)) break;
-                i = (int64_t)gridDim.x + __shfl_sync(0xFFFFFFFFu, ahead, 0);
+                i = (int)(gridDim.x + __shfl_sync(0xFFFFFFFFu, ahead, 0));
             }
             __threadfence();
             if (lane == 0 && atomicAdd(&t.sched[1], 1u) == gridDim.x - 1) {  // the last one leaves the counters as it found them
