@@ -83,6 +83,7 @@ static int encode_cache(Context* c, CUtensorMap* map, const bf16* base, const Ca
     if (v.page_shift == 0) return encode_rows(c, map, base, v.dim, v.kv_heads, v.pages, v.dim, (int64_t)v.kv_heads * v.dim, 1, box_rows);
     return encode_rows(c, map, base, v.dim, 1, (v.pages * v.kv_heads) << v.page_shift, v.dim, v.dim, 1, box_rows);
 }
+static bool rows_of_sectors(const bf16* out, int dim) { return reinterpret_cast<uintptr_t>(out) % 32 == 0 && dim % 16 == 0; }
 static int dim_chunks(int dim) { return (dim + 63) / 64; }
 
 template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p, cudaStream_t s) {
@@ -106,6 +107,7 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     t.tile_tokens = PA_ROWS / p.group;
     t.box_rows = p.tables ? std::min(PA_KEYS, 1 << p.cache.page_shift) : PA_KEYS;
     t.sched = scratch.d_attn_sched.get();
+    t.wide_rows = rows_of_sectors(p.out, p.cache.dim);
     CUtensorMap q, k, v;
     int rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
@@ -180,6 +182,7 @@ template <int CHUNKS> static int launch_wide_tree(Context* c, const TreeParams& 
     t.p.status = p.status;
     t.tile_tokens = PA_ROWS / p.group;
     t.box_rows = std::min(PA_KEYS, 1 << p.cache.page_shift);
+    t.wide_rows = rows_of_sectors(p.out, p.cache.dim);
     const int64_t blocks = (p.max_drafts + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens), tiles = (p.max_context + p.max_drafts + PA_KEYS - 1) / PA_KEYS;
     t.c.may_cut = tiles > PA_WHOLE_TILES;
     t.c.piece_rows = p.max_drafts <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;

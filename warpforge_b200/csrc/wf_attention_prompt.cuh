@@ -46,6 +46,7 @@ struct PromptTiles {
     int tile_tokens;   // tokens of a tile: 128 / group
     int box_rows;      // rows of keys that one TMA load brings: those of a page, at most 128
     int split;         // prompt: items have one tile of rows
+    int wide_rows;     // rows of the output are made of aligned 32-byte pieces
     unsigned int* sched;  // prompt: [0] items taken beyond the first of each CTA, [1] CTAs that are done
     TreeParams tree;
     TreeCuts c;
@@ -174,6 +175,11 @@ __device__ __forceinline__ float2 add2(float2 a, float2 b) {
 
 // Waits for a barrier, the whole warp with one answer.
 __device__ __forceinline__ bool pa_wait(uint64_t* bar, uint32_t parity) { return __all_sync(0xFFFFFFFFu, g_mbar_wait(bar, parity)); }
+
+// 32 bytes, aligned: a sector in one store (a thread stores its own row: each of a warp's stores touches 32 lines, which is what it costs)
+__device__ __forceinline__ void store_32(void* to, const uint32_t* w) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(to), "r"(w[0]), "r"(w[1]), "r"(w[2]), "r"(w[3]), "r"(w[4]), "r"(w[5]), "r"(w[6]), "r"(w[7]) : "memory");
+}
 
 struct PromptShared {
     uint64_t q_full[2], q_empty[2];
@@ -555,7 +561,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     if (TREE && !whole) {
                         if (mine)
 #pragma unroll
-                            for (int i = 0; i < 8; i++) *reinterpret_cast<float4*>(piece + (size_t)at * DIM + c + 4 * i) = make_float4(x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y);
+                            for (int i = 0; i < 4; i++) store_32(piece + (size_t)at * DIM + c + 8 * i, o + 8 * i);
                         continue;
                     }
 #pragma unroll
@@ -564,9 +570,15 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                         o[i] = pack_bf16(x[i].x, x[i].y);
                     }
                     bf16* const to = p.out + ((size_t)row * p.q_heads + head) * d + c;
+                    if (t.wide_rows) {
 #pragma unroll
-                    for (int i = 0; i < 4; i++)
-                        if (mine && c + 8 * i < d) *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                        for (int i = 0; i < 2; i++)
+                            if (mine && c + 16 * i < d) store_32(to + 16 * i, o + 8 * i);
+                    } else {
+#pragma unroll
+                        for (int i = 0; i < 4; i++)
+                            if (mine && c + 8 * i < d) *reinterpret_cast<uint4*>(to + 8 * i) = make_uint4(o[4 * i], o[4 * i + 1], o[4 * i + 2], o[4 * i + 3]);
+                    }
                 }
                 odd = whole && (!(l < INFINITY) || scores_too_large(top, scale) || !(fabsf(finite.x + finite.y) < INFINITY));
                 tc_fence_before();
@@ -647,19 +659,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             int z = 0, z_before = 0, loads = 0, loads_before = 0;
             for (int j = 0; j < n && !failed; j++) {  // keys 0, keys 1, values 0, keys 2, values 1, ..
                 loads = find(it.from + j, z);
-                if (j == 0)
-                    for (int g = 0; g < 2; g++) {
-                        if (it.tiles(g) == 0) continue;
-                        if (!pa_wait(&sh->q_empty[g], q_phase[g])) failed = true;
-                        q_phase[g] ^= 1;
-                        if (failed) break;
-                        const uint32_t bar = g_smem_u32(&sh->q_full[g]);
-                        mbar_expect_if(bar, (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens), issue);
-                        const int first = it.row0 + it.token0 + (it.split ? 0 : g * t.tile_tokens);
+                auto queries = [&](int g) {
+                    if (it.tiles(g) == 0) return;
+                    if (!pa_wait(&sh->q_empty[g], q_phase[g])) failed = true;
+                    q_phase[g] ^= 1;
+                    if (failed) return;
+                    const uint32_t bar = g_smem_u32(&sh->q_full[g]);
+                    mbar_expect_if(bar, (uint32_t)(CHUNKS * 128 * p.group * t.tile_tokens), issue);
+                    const int first = it.row0 + it.token0 + (it.split ? 0 : g * t.tile_tokens);
 #pragma unroll
-                        for (int c = 0; c < CHUNKS; c++) tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, first, bar, issue);
-                    }
+                    for (int c = 0; c < CHUNKS; c++) tma_load_3d(smem + (uint32_t)((g * CHUNKS + c) * PA_CHUNK), &q_map, 64 * c, it.head * p.group, first, bar, issue);
+                };
+                if (j == 0) queries(0);
                 if (!failed) load(&k_map, z, loads);
+                if (j == 0 && !failed) queries(1);
                 if (j > 0 && !failed) load(&v_map, z_before, loads_before);
                 z_before = z;
                 loads_before = loads;
