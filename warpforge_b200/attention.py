@@ -286,6 +286,14 @@ class KvCache:
             self.copy_pages(DeviceTensor(self._pairs, (len(pairs), 2), "i32"), DeviceTensor(self._rows, (len(rows),), "i32"), stream)
         return out
 
+    def layer(self, i: int):
+        """keys and values of one layer, bf16 [pages, kv_heads, page_tokens, head_dim]."""
+        if not 0 <= i < self.layers:
+            raise ValueError(f"layer {i} of {self.layers}")
+        shape = self.keys.shape()[1:]
+        skip = i * int(np.prod(shape)) * 2
+        return tuple(DeviceTensor(t.ptr + skip, shape, "bf16", owner=t) for t in (self.keys, self.values))
+
     # ---- device
     def copy_pages(self, pairs: DeviceTensor, rows: Optional[DeviceTensor] = None, stream: int = 0) -> None:
         """In every layer page pairs[i][0] to page pairs[i][1] (i32 [n, 2]), the first rows[i] tokens of it (i32 [n]; None: all)."""
