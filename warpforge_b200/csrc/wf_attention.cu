@@ -140,12 +140,12 @@ static int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cu
 static int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
     return launch_attention(c, "tree_attention", tree_join_kernel, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
 }
-template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const TreeParams& p, cudaStream_t s) {
+template <int CHUNKS, int MT> static int launch_tree(Context* c, const TreeParams& p, cudaStream_t s) {
     const char* what = "tree_attention";
-    typedef TreeShape<CHUNKS, MT, WM> Shape;
+    typedef TreeShape<CHUNKS, MT> Shape;
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, WM>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
     const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
@@ -161,7 +161,7 @@ template <int CHUNKS, int MT, int WM> static int launch_tree(Context* c, const T
     if (rc != WF_OK) return rc;
     const int64_t units = p.seqs * blocks * p.cache.kv_heads, most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
     const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
-    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, WM>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
     return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, Shape::ROWS, s) : rc;
 }
 
@@ -284,8 +284,8 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     p.status = c->d_status;
     const int rows = a->max_drafts * p.group, chunks = dim_chunks(cache->head_dim);  // rows of a sequence and kv head
     if (rows > 32) return chunks == 1 ? launch_wide_tree<1>(c, p, s) : launch_wide_tree<2>(c, p, s);
-    if (chunks == 1) return rows <= 16 ? launch_tree<1, 1, 1>(c, p, s) : launch_tree<1, 2, 1>(c, p, s);
-    return rows <= 16 ? launch_tree<2, 1, 1>(c, p, s) : launch_tree<2, 2, 1>(c, p, s);
+    if (chunks == 1) return rows <= 16 ? launch_tree<1, 1>(c, p, s) : launch_tree<1, 2>(c, p, s);
+    return rows <= 16 ? launch_tree<2, 1>(c, p, s) : launch_tree<2, 2>(c, p, s);
 }
 
 }  // extern "C"

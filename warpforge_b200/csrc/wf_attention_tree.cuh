@@ -1,11 +1,11 @@
 // Attention of a few new tokens per sequence over a long cache.
 //
 // Bound by HBM: every key and value is read once, 4 dim bytes for 4 dim flops a row.  The rows of a sequence and kv head (its new tokens times the
-// heads of the group) are padded to 16 .. 64 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
-// one decoded token fills one to eight.
+// heads of the group) are padded to 16 or 32 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
+// one decoded token fills one to eight.  More than 32 rows go to the kernel of wf_attention_prompt.cuh.
 //
 // The units are cut as wf_attention_line.cuh says.  Inside a CTA four warps walk its share and have TMA fill a ring of tiles ahead, across the ends of
-// units too; teams of eight others take the tiles of a piece in turn.
+// units too; eight others take the tiles of a piece in turn.
 #pragma once
 #include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
@@ -22,19 +22,19 @@ constexpr int TA_SEGMENTS = 2;     // announced ahead
 constexpr int TA_UNIT_TILES = 8;   // what a unit costs beyond its tiles, in tiles
 constexpr int TA_WHOLE_TILES = 40; // units of no more tiles are never cut
 constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
-// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows a warp, WM warps a team
-template <int CHUNKS, int MT, int WM> struct TreeShape {
-    static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT * WM, TEAMS = TA_WARPS / WM;
+// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows
+template <int CHUNKS, int MT> struct TreeShape {
+    static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT;
     static constexpr int SLOT_BYTES = 2 * CHUNKS * TA_KEYS * 128;  // keys and values of a tile
     static constexpr int Q_BYTES = ROWS * DIM * 2;
     static constexpr int FIT = (227 * 1024 - TA_MERGE_BYTES - TA_SEGMENTS * Q_BYTES - 4 * 1024) / SLOT_BYTES;
-    // A slot belongs to one loader, and within a segment to one team, lap after lap: a barrier's parity tells the lap apart only for those that wait for every one.
-    static constexpr int TURN = TEAMS > TA_LOADERS ? TEAMS : TA_LOADERS, SLOTS = FIT > 32 ? 32 : FIT / TURN * TURN;
-    static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TEAMS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TEAMS;  // teams whose sums lie in shared memory at a time
+    // A slot belongs to one loader, and within a segment to one warp, lap after lap: a barrier's parity tells the laps apart only for those that wait for every one.
+    static constexpr int SLOTS = FIT > 32 ? 32 : FIT / TA_WARPS * TA_WARPS;
+    static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TA_WARPS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TA_WARPS;  // warps whose sums lie in shared memory at a time
     static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
     static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory
-    static_assert(SETS == TEAMS || 2 * SETS == TEAMS, "one round of folding");
-    static_assert(SLOTS >= TEAMS && SLOTS % TEAMS == 0 && SLOTS % TA_LOADERS == 0, "slots for every team and loader");
+    static_assert(SETS == TA_WARPS || 2 * SETS == TA_WARPS, "one round of folding");
+    static_assert(SLOTS >= TA_WARPS && SLOTS % TA_WARPS == 0 && SLOTS % TA_LOADERS == 0, "slots for every warp and loader");
 };
 // What a CTA has of a unit.
 struct alignas(16) TreeSegment {
@@ -82,21 +82,21 @@ __device__ __forceinline__ bool ta_sync_or(bool v) {  // the same answer for all
     return r != 0;
 }
 
-template <int CHUNKS, int MT, int WM> struct TreeShared {
-    typedef TreeShape<CHUNKS, MT, WM> Shape;
+template <int CHUNKS, int MT> struct TreeShared {
+    typedef TreeShape<CHUNKS, MT> Shape;
     uint64_t full[Shape::SLOTS], empty[Shape::SLOTS];
     uint64_t seg_full[TA_SEGMENTS], seg_empty[TA_SEGMENTS];
     TreeSegment segments[TA_SEGMENTS];
-    float team_max[Shape::SETS][Shape::ROWS], team_sum[Shape::SETS][Shape::ROWS];
+    float warp_max[Shape::SETS][Shape::ROWS], warp_sums[Shape::SETS][Shape::ROWS];
     unsigned long long odd_rows;
     int bad_page;  // the segment of this number and those before it have pages outside the cache
 };
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
-template <int CHUNKS, int MT, int WM>
-__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS, MT, WM>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
-    typedef TreeShape<CHUNKS, MT, WM> Shape;
+template <int CHUNKS, int MT>
+__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS, MT>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
+    typedef TreeShape<CHUNKS, MT> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
     const TreeParams& p = t.p;
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
@@ -169,22 +169,22 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
     return true;
 }
 
-template <int CHUNKS, int MT, int WM>
+template <int CHUNKS, int MT>
 __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
-    typedef TreeShape<CHUNKS, MT, WM> Shape;
-    constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, TEAMS = Shape::TEAMS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
+    typedef TreeShape<CHUNKS, MT> Shape;
+    constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
     constexpr bool Q_KEPT = MT * CHUNKS <= 2;  // queries stay in registers; else they are read again with every tile
     extern __shared__ uint8_t raw[];
-    __shared__ TreeShared<CHUNKS, MT, WM> sh_;
-    TreeShared<CHUNKS, MT, WM>* const sh = &sh_;
+    __shared__ TreeShared<CHUNKS, MT> sh_;
+    TreeShared<CHUNKS, MT>* const sh = &sh_;
     const TreeParams& p = t.p;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, quad = lane & 3;
     const uint32_t ring = (g_smem_u32(raw) + 1023u) & ~1023u, q_smem = ring + SLOTS * SLOT_BYTES;
     float* const merge = reinterpret_cast<float*>(raw + (ring - g_smem_u32(raw)) + SLOTS * SLOT_BYTES + TA_SEGMENTS * Shape::Q_BYTES);
     if (tid < SLOTS) {
         g_mbar_init(&sh->full[tid], 1);
-        g_mbar_init(&sh->empty[tid], WM);
+        g_mbar_init(&sh->empty[tid], 1);
     } else if (tid >= 32 && tid < 32 + TA_SEGMENTS) {
         g_mbar_init(&sh->seg_full[tid - 32], 32 * TA_LOADERS + 1);  // every lane's copies of queries, and the words
         g_mbar_init(&sh->seg_empty[tid - 32], TA_WARPS);
@@ -200,7 +200,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= TA_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_load<CHUNKS, MT, WM>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
+        if (!tree_load<CHUNKS, MT>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
@@ -208,13 +208,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     }
 
     asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_MULTIPLY_REGS));
-    const int team = warp / WM, part = warp % WM;  // the team, which rows of it
     const float scale = p.scale_log2;
     const int d = p.cache.dim, group = p.group;
     // ldmatrix: a lane's row and 16-byte piece, swizzled
     const int matrix = lane >> 3, mrow = lane & 7;
     const uint32_t k_row = (uint32_t)(((matrix >> 1) * 8 + mrow) * 128), v_row = (uint32_t)(((matrix & 1) * 8 + mrow) * 128) + CHUNKS * TA_KEYS * 128;
-    const uint32_t q_row = (uint32_t)((part * MT * 16 + (matrix & 1) * 8 + mrow) * DIM * 2);
+    const uint32_t q_row = (uint32_t)(((matrix & 1) * 8 + mrow) * DIM * 2);
     int seg = 0;
     uint32_t seg_phase = 0;
     bool failed = false;
@@ -244,11 +243,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll
             for (int n = 0; n < N_TILES; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
         }
-        int slot = w.slot + team;
+        int slot = w.slot + warp;
         uint32_t phase = (uint32_t)w.phase;
         if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
 #pragma unroll 1
-        for (int tile = w.from + team; tile < w.to; tile += TEAMS) {
+        for (int tile = w.from + warp; tile < w.to; tile += TA_WARPS) {
             if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->full[slot], phase))) {
                 failed = true;
                 break;
@@ -275,7 +274,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const int r = (part * MT + i) * 16 + g + 8 * e, token = p.token_of(w.first + r);
+                        const int r = 16 * i + g + 8 * e, token = p.token_of(w.first + r);
                         const uint64_t sees = r < count && keys > 0 ? ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows)) : 0;
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
@@ -346,7 +345,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) g_mbar_arrive(&sh->empty[slot]);
-            slot += TEAMS;
+            slot += TA_WARPS;
             if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
         }
         __syncwarp();
@@ -354,7 +353,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
         if (*reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l[0][0] = l[0][1] = l[MT - 1][0] = l[MT - 1][1] = __uint_as_float(0x7FC00000u);
 
-        // The teams' sums together.  Where they do not all fit shared memory the upper half hands its to the lower half first.
+        // The warps' sums together.  Where they do not all fit shared memory the upper half hands its to the lower half first.
         auto write_sums = [&](int set) {
 #pragma unroll
             for (int i = 0; i < MT; i++)
@@ -363,30 +362,30 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                     // the threads of a row have followed the same maximum
                     l[i][e] += __shfl_xor_sync(0xFFFFFFFFu, l[i][e], 1);
                     l[i][e] += __shfl_xor_sync(0xFFFFFFFFu, l[i][e], 2);
-                    const int r = (part * MT + i) * 16 + g + 8 * e;
+                    const int r = 16 * i + g + 8 * e;
                     if (quad == 0) {
-                        sh->team_max[set][r] = m[i][e];
-                        sh->team_sum[set][r] = l[i][e];
+                        sh->warp_max[set][r] = m[i][e];
+                        sh->warp_sums[set][r] = l[i][e];
                     }
                     float2* row = reinterpret_cast<float2*>(merge + (size_t)(set * ROWS + r) * DIM);
 #pragma unroll
                     for (int n = 0; n < N_TILES; n++) row[(n ^ (r & 3)) * 4 + quad] = make_float2(o[i][n][2 * e], o[i][n][2 * e + 1]);
                 }
         };
-        if (SETS < TEAMS) {
-            if (team >= SETS) write_sums(team - SETS);
+        if (SETS < TA_WARPS) {
+            if (warp >= SETS) write_sums(warp - SETS);
             ta_sync();
-            if (team < SETS) {
+            if (warp < SETS) {
 #pragma unroll
                 for (int i = 0; i < MT; i++)
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
-                        const int r = (part * MT + i) * 16 + g + 8 * e;
-                        const float other = sh->team_max[team][r], top = fmaxf(m[i][e], other), ref = top == -INFINITY ? 0.f : top;
+                        const int r = 16 * i + g + 8 * e;
+                        const float other = sh->warp_max[warp][r], top = fmaxf(m[i][e], other), ref = top == -INFINITY ? 0.f : top;
                         const float keep = line_ex2((m[i][e] - ref) * scale), take = line_ex2((other - ref) * scale);
                         m[i][e] = top;
-                        l[i][e] = l[i][e] * keep + (quad == 0 ? sh->team_sum[team][r] * take : 0.f);
-                        const float2* row = reinterpret_cast<const float2*>(merge + (size_t)(team * ROWS + r) * DIM);
+                        l[i][e] = l[i][e] * keep + (quad == 0 ? sh->warp_sums[warp][r] * take : 0.f);
+                        const float2* row = reinterpret_cast<const float2*>(merge + (size_t)(warp * ROWS + r) * DIM);
 #pragma unroll
                         for (int n = 0; n < N_TILES; n++) {
                             const float2 v = row[(n ^ (r & 3)) * 4 + quad];
@@ -397,7 +396,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             }
             ta_sync();
         }
-        if (team < SETS) write_sums(team);
+        if (warp < SETS) write_sums(warp);
         ta_sync();
         const bool whole = w.from == 0 && w.to == w.tiles;
         // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
@@ -418,12 +417,12 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             float top = -INFINITY, sum = 0.f, tops[SETS];
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
-            for (int c = 0; c < SETS; c++) top = fmaxf(top, tops[c] = sh->team_max[c][r]);
+            for (int c = 0; c < SETS; c++) top = fmaxf(top, tops[c] = sh->warp_max[c][r]);
             const float ref = top == -INFINITY ? 0.f : top;
 #pragma unroll
             for (int c = 0; c < SETS; c++) {
                 const float keep = line_ex2((tops[c] - ref) * scale);
-                sum += sh->team_sum[c][r] * keep;
+                sum += sh->warp_sums[c][r] * keep;
                 const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
                 x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
             }
