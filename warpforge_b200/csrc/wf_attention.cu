@@ -6,10 +6,6 @@
 #include "wf_attention_prompt.cuh"
 #include "wf_attention_tree.cuh"
 
-namespace wf {
-
-}  // namespace wf
-
 using namespace wf;
 
 static int check_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too) {
