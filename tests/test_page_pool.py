@@ -126,3 +126,73 @@ def test_rope_table():
     assert np.allclose(t[3, 1], [np.cos(3 * 100 ** -0.25), np.sin(3 * 100 ** -0.25)]) and np.allclose(t[3, 2, 0], np.cos(3 * 100 ** -0.5 / 2))
     with pytest.raises(ValueError):
         rope_table(5, 7)
+
+
+class HostContext:
+    """A context without a device: addresses are numbers, copies are kept, kernels are not launched."""
+
+    def __init__(self, lib):
+        self._lib, self.handle, self.freed, self.copies = lib, 0, [], []
+        self._next = 4096
+
+    def _ck(self, what, status):
+        pass
+
+    def allocate(self, n):
+        self._next += -(-n // 256) * 256
+        return self._next
+
+    def free(self, p):
+        self.freed.append(p)
+
+    def copy_to_device(self, dptr, host, stream=0, sync=True):
+        self.copies.append((dptr, host.tolist(), stream))
+
+
+@pytest.fixture
+def cache():
+    from warpforge_b200.attention import KvCache
+
+    made = KvCache(HostContext(LIB), layers=2, pages=12, page_tokens=16, kv_heads=1, head_dim=64)
+    yield made
+    made.close()
+
+
+def test_forks_of_two_streams_have_arrays_of_their_own(cache):
+    a = cache.sequence()
+    a.extend(20)
+    forks = [a.fork(stream) for stream in (7, 8, 7)]
+    assert [f.pages[0] for f in forks] == [a.pages[0]] * 3 and cache.holders(a.pages[0]) == 4
+    at = {stream: {p for p, _, s in cache.context.copies if s == stream} for stream in (7, 8)}
+    assert len(at[7]) == len(at[8]) == 2 and not at[7] & at[8]
+    pairs = [x for _, x, _ in cache.context.copies[::2]]
+    assert pairs == [[[a.pages[1], f.pages[1]]] for f in forks]
+
+
+def test_a_fork_that_cannot_be_changes_nothing(cache):
+    a, b = cache.sequence(), cache.sequence()
+    a.extend(20)
+    b.extend(20)
+    gone = list(b.pages)
+    cache._release(gone)  # b names pages that nobody holds
+    free = cache.free_pages()
+    with pytest.raises(Exception):
+        cache.fork([a, b])
+    assert cache.free_pages() == free and [cache.holders(p) for p in a.pages] == [1, 1]
+    b.pages, b.tokens = [], 0
+    c = cache.sequence()
+    c.extend(16 * cache.free_pages())  # no page is left for the part-full one
+    with pytest.raises(Exception):
+        a.fork()
+    assert cache.free_pages() == 0 and [cache.holders(p) for p in a.pages] == [1, 1]
+
+
+def test_a_sequence_forked_twice_in_one_call(cache):
+    a = cache.sequence()
+    a.extend(33)
+    one, two = cache.fork([a, a])
+    assert cache.holders(a.pages[0]) == cache.holders(a.pages[1]) == 3
+    assert len({a.pages[2], one.pages[2], two.pages[2]}) == 3
+    for s in (a, one, two):
+        s.free()
+    assert cache.free_pages() == 12

@@ -217,8 +217,7 @@ class KvCache:
         pool = ctypes.c_int64()
         N.check("wf_pages_create", context._lib.wf_pages_create(pages, ctypes.byref(pool)))
         self._pool = pool.value
-        self._pairs = self._rows = 0  # device arrays of fork()
-        self._forks = 0
+        self._fork_arrays = {}  # stream: device arrays of its forks (pairs, rows, how many fit)
 
     # ---- pages
     def _ids(self, ids: Seq[int]):
@@ -262,28 +261,34 @@ class KvCache:
     def fork(self, sequences: Seq[Sequence], stream: int = 0) -> List[Sequence]:
         """A second sequence for each, with the same tokens: whole pages shared, part-full last pages copied, all in one call on `stream`."""
         part = [s for s in sequences if s.tokens % self.page_tokens]
-        fresh = iter(self._take(len(part)))
+        shared = [p for s in sequences for p in s.pages[:s.tokens // self.page_tokens]]
+        self._share(shared)
+        try:
+            fresh = self._take(len(part))
+        except Exception:
+            self._release(shared)
+            raise
         out, pairs, rows = [], [], []
         for s in sequences:
             whole, rest = divmod(s.tokens, self.page_tokens)
-            self._share(s.pages[:whole])
             pages = s.pages[:whole]
             if rest:
-                pages = pages + [next(fresh)]
+                pages = pages + [fresh[len(pairs)]]
                 pairs.append((s.pages[whole], pages[-1]))
                 rows.append(rest)
             out.append(Sequence(self, pages, s.tokens))
         if pairs:
             ctx = self.context
-            if len(pairs) > self._forks:
-                for p in (self._pairs, self._rows):
+            to, counts, room = self._fork_arrays.get(stream, (0, 0, 0))
+            if len(pairs) > room:
+                for p in (to, counts):
                     if p:
                         ctx.free(p)
-                self._forks = max(16, 2 * len(pairs))
-                self._pairs, self._rows = ctx.allocate(self._forks * 8), ctx.allocate(self._forks * 4)
-            ctx.copy_to_device(self._pairs, np.array(pairs, np.int32), stream)
-            ctx.copy_to_device(self._rows, np.array(rows, np.int32), stream)
-            self.copy_pages(DeviceTensor(self._pairs, (len(pairs), 2), "i32"), DeviceTensor(self._rows, (len(rows),), "i32"), stream)
+                room = max(16, 2 * len(pairs))
+                to, counts, _ = self._fork_arrays[stream] = ctx.allocate(room * 8), ctx.allocate(room * 4), room
+            ctx.copy_to_device(to, np.array(pairs, np.int32), stream)
+            ctx.copy_to_device(counts, np.array(rows, np.int32), stream)
+            self.copy_pages(DeviceTensor(to, (len(pairs), 2), "i32"), DeviceTensor(counts, (len(rows),), "i32"), stream)
         return out
 
     def layer(self, i: int):
@@ -314,7 +319,7 @@ class KvCache:
         if self._pool:
             pool, self._pool = self._pool, 0
             N.check("wf_pages_destroy", self.context._lib.wf_pages_destroy(pool))
-            for p in self._owned + [p for p in (self._pairs, self._rows) if p]:
+            for p in self._owned + [p for arrays in self._fork_arrays.values() for p in arrays[:2]]:
                 if self.context.handle:
                     self.context.free(p)
-            self._owned, self._pairs, self._rows = [], 0, 0
+            self._owned, self._fork_arrays = [], {}
