@@ -291,6 +291,14 @@ def test_tree_many_units_of_many_rows(backend):
     run_tree(backend, [int(n) for n in rng.integers(0, 400, 60)], [int(n) for n in rng.integers(1, 65, 60)], 8, 2, 64, 16)
 
 
+@pytest.mark.parametrize("drafts", [1, 12])
+@pytest.mark.parametrize("seqs,longest", [(16, 1000), (20, 1400), (37, 900), (3, 1300)])
+def test_tree_whole_and_cut_units(backend, drafts, seqs, longest):
+    """About as many units as the device has SMs and more, alike and not, on both sides of the rule that cuts them."""
+    run_tree(backend, [longest - 7 * i for i in range(seqs)], [drafts] * seqs, 32, 8, 64, 32)
+    run_tree(backend, [longest] + [50] * (seqs - 1), [drafts] * seqs, 32, 8, 64, 32)
+
+
 def test_tree_defaults(backend):
     """Without offsets and words: every sequence has max_drafts tokens, a chain."""
     run_tree(backend, [100, 333, 5], [4, 4, 4], 4, 2, 64, 16, shape="chain", arrays=False)

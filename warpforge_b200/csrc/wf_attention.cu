@@ -147,7 +147,8 @@ template <int CHUNKS, int MT> static int launch_tree(Context* c, const TreeParam
     const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
     TreeTiles t{};
     t.p = p;
-    t.c.may_cut = tiles > TA_WHOLE_TILES;
+    const int64_t units = p.seqs * blocks * p.cache.kv_heads;
+    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
     t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
     t.c.dim = Shape::DIM;
     int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
@@ -155,7 +156,7 @@ template <int CHUNKS, int MT> static int launch_tree(Context* c, const TreeParam
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
     if (rc != WF_OK) return rc;
-    const int64_t units = p.seqs * blocks * p.cache.kv_heads, most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
     const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
     rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
     return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, Shape::ROWS, s) : rc;
@@ -180,7 +181,8 @@ template <int CHUNKS> static int launch_wide_tree(Context* c, const TreeParams& 
     t.box_rows = std::min(PA_KEYS, 1 << p.cache.page_shift);
     t.wide_rows = rows_of_sectors(p.out, p.cache.dim);
     const int64_t blocks = (p.max_drafts + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens), tiles = (p.max_context + p.max_drafts + PA_KEYS - 1) / PA_KEYS;
-    t.c.may_cut = tiles > PA_WHOLE_TILES;
+    const int64_t units = p.seqs * blocks * p.cache.kv_heads;
+    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, PA_CUT_TILES, PA_CUT_ANYWAY);
     t.c.piece_rows = p.max_drafts <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;
     t.c.tile_rows = t.tile_tokens * p.group;
     t.c.tile_room = PA_ROWS;
@@ -191,7 +193,7 @@ template <int CHUNKS> static int launch_wide_tree(Context* c, const TreeParams& 
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
     if (rc != WF_OK) return rc;
-    const int64_t units = p.seqs * blocks * p.cache.kv_heads, most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
     const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
     rc = launch_attention(c, "tree_attention", prompt_tiles_kernel<CHUNKS, true>, grid, PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
     return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, std::min(p.max_drafts, 2 * t.tile_tokens) * p.group, s) : rc;
@@ -279,6 +281,9 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     p.scale_log2 = a->scale * 1.44269504f;
     p.status = c->d_status;
     const int rows = a->max_drafts * p.group, chunks = dim_chunks(cache->head_dim);  // rows of a sequence and kv head
+    // Tiles of 128 rows on the 5th-generation tensor cores, or of 16 or 32 on mma.sync.  48 sequences of 1500 tokens, 8 heads of 128, 20 / 24 / 32 rows: 71.5 / 72.3 / 73.2 us
+    // against 65.1 / 66.1 / 67.8; 8 of 2000, 4 / 16 / 32 rows: 22.4 / 23.3 / 23.9 against 19.1 / 20.7 / 25.7; one of 600: 12.3 for all three against 9.5 / 10.1 / 13.4.  With more
+    // than 32 rows a row's sums no longer fit in the registers of the warps that multiply.
     if (rows > 32) return chunks == 1 ? launch_wide_tree<1>(c, p, s) : launch_wide_tree<2>(c, p, s);
     if (chunks == 1) return rows <= 16 ? launch_tree<1, 1>(c, p, s) : launch_tree<1, 2>(c, p, s);
     return rows <= 16 ? launch_tree<2, 1>(c, p, s) : launch_tree<2, 2>(c, p, s);

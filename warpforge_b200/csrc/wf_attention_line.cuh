@@ -24,6 +24,15 @@ struct TreeCuts {
     int may_cut;
 };
 
+// Whether units are cut, by what the host knows: how many there are and how many tiles the longest can have.  Cut, every CTA has the same share, but most
+// have parts of two units, and a second kernel joins them; that costs as much as `worth` tiles.  Whole, some CTAs have a unit more than the average.  Where
+// most sequences are shorter than the longest, whole units cost up to all of the longest one's tiles: from `anyway` tiles on, that is more than what cutting would
+// cost where they are alike.
+inline bool line_is_cut(int64_t units, int64_t tiles, int sms, int worth, int anyway) {
+    const int64_t rounds = (units + sms - 1) / sms;
+    return tiles > anyway || tiles * (rounds * sms - units) > (int64_t)worth * sms;
+}
+
 struct LineUnit {
     TreeSeq q;
     int seq, head, first;           // first: of the sequence's rows * group

@@ -311,7 +311,9 @@ struct PromptSchedule {
 // What a unit costs beyond its key tiles, in key tiles: with 0 / 1 / 2 / 3 / 4 / 6, eight sequences of 0 to 3000 tokens and up to 24 drafts take 27.5 / 24.3 / 24.2 / 22.9 /
 // 23.0 / 23.4 us.
 constexpr int PA_UNIT_TILES = 3;
-constexpr int PA_WHOLE_TILES = 5;   // units of no more key tiles are never cut
+// When units are cut (line_is_cut).  Microseconds whole / cut, 12 drafts of 32 / 8 heads of 128: 16 sequences with 700, 1000, 1400, 1800 tokens 16.3 / 23.9, 19.6 / 27.4,
+// 26.5 / 32.7, 31.2 / 37.7; 8 with 1000, 1400 17.0 / 19.2, 22.5 / 22.4; 20 with 1000, 1400 31.9 / 30.7, 42.8 / 37.9; 4 with 600, 1000 12.8 / 14.5, 15.9 / 15.7.
+constexpr int PA_CUT_TILES = 6, PA_CUT_ANYWAY = 15;
 template <class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
     const TreeParams& p = t.tree;
     bool cut = false;

@@ -20,7 +20,10 @@ constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
 constexpr int TA_MERGE_BYTES = 64 * 1024;
 constexpr int TA_SEGMENTS = 2;     // announced ahead
 constexpr int TA_UNIT_TILES = 8;   // what a unit costs beyond its tiles, in tiles
-constexpr int TA_WHOLE_TILES = 40; // units of no more tiles are never cut
+// When units are cut (line_is_cut).  Microseconds whole / cut, heads of 128: one sequence of 32 heads with 300, 600, 1000, 2000 tokens 7.2 / 8.7, 9.4 / 9.1, 11.9 / 10.7,
+// 20.3 / 12.8; 8, 16, 18, 20, 24 sequences of 8 heads with 1000 tokens 12.8 / 13.4, 15.5 / 20.1, 16.6 / 21.5, 24.9 / 22.5, 25.7 / 25.8; 16 with 1800 23.4 / 28.2; one with
+// 1250 beside 15 with 200 14.4 / 12.3.
+constexpr int TA_CUT_TILES = 40, TA_CUT_ANYWAY = 96;
 constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
 // CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows
 template <int CHUNKS, int MT> struct TreeShape {
