@@ -5,8 +5,13 @@
 //   O += P V    [128 rows x dim] fp32 in TMEM, P in TMEM, V in shared memory
 //
 // A CTA works on two tiles of rows of one kv head at a time, so that the tensor core has the one tile's products to do while the other
-// tile's exponentials are taken; where there is one tile of rows, on every other tile of keys of it in turn.  The rows of a tile are the heads of the group for some tokens, token by token: keys and values are read once
-// for the whole group.  A thread of the softmax warps has a row: its maximum and sum need no exchange.
+// tile's exponentials are taken; where there is one tile of rows, on every other tile of keys of it in turn.  The rows of a tile are the heads of the group for some tokens, token by
+// token: keys and values are read once for the whole group.  A thread of the softmax warps has a row: its maximum and sum need no exchange.
+//
+// Bound by the softmax warps' instructions beside the tensor cores' products: a pair of tiles takes about 3300 cycles, 2048 of them products at dim 128 and 1024 at dim 64.  8192
+// tokens, 32 / 8 heads of 128: 434 us in a burst (1.27 PFLOP/s of the products that the mask leaves, 0.77 of the measured rate), 502 over seconds under the power limit; of 64: 372 us.
+// 512 tokens, 32 / 32 heads: 12.2 us, a launch, 2 us until the first item is known (code and arguments come from memory), two pairs of tiles and the rows' way out.  Two threads a row
+// (16 softmax warps): 604 us where this takes 521.
 #pragma once
 #include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
@@ -21,7 +26,8 @@ constexpr int PA_THREADS = 12 * 32;
 constexpr int PA_SOFTMAX_REGS = 224, PA_OTHER_REGS = 56;
 constexpr int PA_CHUNK = PA_KEYS * 128;      // bytes of 128 rows x 64 elements
 constexpr int PA_ITEMS = 2;                  // items announced ahead
-// Which of the 32 pairs of weights of 64 keys are taken by the cubic: two in five, so that the special function unit and the fp32 units are through at about the same time.
+// Which of the 32 pairs of weights of 64 keys are taken by the cubic: two in five, so that the special function unit and the fp32 units are through at about the same time
+// (none / one in five / one in three / two in five: 449 / 433 / 431 / 435 us for 8192 tokens, 32 / 8 heads of 128; none / two in five: 429 / 372 of 64).
 __host__ __device__ constexpr bool PA_CUBIC(int pair) { return pair % 5 == 1 || pair % 5 == 3; }
 constexpr float PA_RESCALE = 8.f;            // the running maximum is followed when it has grown by this many powers of two
 constexpr int PA_MAX_STAGES = 12;

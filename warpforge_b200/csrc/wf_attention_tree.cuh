@@ -2,7 +2,8 @@
 //
 // Bound by HBM: every key and value is read once, 4 dim bytes for 4 dim flops a row.  The rows of a sequence and kv head (its new tokens times the
 // heads of the group) are padded to 16 or 32 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
-// one decoded token fills one to eight.  More than 32 rows go to the kernel of wf_attention_prompt.cuh.
+// one decoded token fills one to eight.  More than 32 rows go to the kernel of wf_attention_prompt.cuh.  (One token of 48 sequences of 31 to 4000 tokens, 64 / 8 heads of
+// 128: 419 MB in 73 us, 5.7 TB/s, 0.88 of a copy's rate.  One of 32 / 32 heads at 512 tokens: 9.2 us, of which 3.5 are a launch and the rest one SM's walk through 33 tiles.)
 //
 // The units are cut as wf_attention_line.cuh says.  Inside a CTA four warps walk its share and have TMA fill a ring of tiles ahead, across the ends of
 // units too; eight others take the tiles of a piece in turn.
@@ -19,7 +20,6 @@ constexpr int TA_THREADS = (TA_WARPS + TA_LOADERS) * 32;
 constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
 constexpr int TA_MERGE_BYTES = 64 * 1024;
 constexpr int TA_SEGMENTS = 2;     // announced ahead
-constexpr int TA_UNIT_TILES = 8;   // what a unit costs beyond its tiles, in tiles
 // When units are cut (line_is_cut).  Microseconds whole / cut, heads of 128: one sequence of 32 heads with 300, 600, 1000, 2000 tokens 7.2 / 8.7, 9.4 / 9.1, 11.9 / 10.7,
 // 20.3 / 12.8; 8, 16, 18, 20, 24 sequences of 8 heads with 1000 tokens 12.8 / 13.4, 15.5 / 20.1, 16.6 / 21.5, 24.9 / 22.5, 25.7 / 25.8; 16 with 1800 23.4 / 28.2; one with
 // 1250 beside 15 with 200 14.4 / 12.3.
@@ -36,6 +36,9 @@ template <int CHUNKS, int MT> struct TreeShape {
     static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TA_WARPS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TA_WARPS;  // warps whose sums lie in shared memory at a time
     static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
     static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory
+    // What a unit costs beyond its tiles, in tiles (queries, first tile's way, the fold over eight warps).  16 rows, with 2 / 4 / 8 / 12 / 16 / 24: 91 / 85 / 75 / 73 / 73 / 75 us
+    // for one token of 48 sequences of 31 to 4000 tokens; 32 rows of 30 sequences of 10 to 5000, with 16 / 24 / 32 / 48: 72 / 65 / 63 / 61, but 33.2 / 32.8 / 33.2 / 33.3 for 20 alike.
+    static constexpr int UNIT_TILES = 16 * MT;
     static_assert(SETS == TA_WARPS || 2 * SETS == TA_WARPS, "one round of folding");
     static_assert(SLOTS >= TA_WARPS && SLOTS % TA_WARPS == 0 && SLOTS % TA_LOADERS == 0, "slots for every warp and loader");
 };
@@ -107,7 +110,7 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
     bool cut = false;  // a unit that begins here goes on in the next share
-    const bool ok = walk_line<TA_KEYS>(p, ROWS, TA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+    const bool ok = walk_line<TA_KEYS>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
         const int keys = u.q.context < 0 ? 0 : u.q.context + u.q.rows, count = min(ROWS, u.q.rows * group - u.first);
         // the page of a lane's tile, asked for before anything is waited for
         const int* const table = u.q.place.table;
