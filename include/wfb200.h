@@ -39,7 +39,7 @@ extern "C" {
 #define WF_ERR_DEVICE_WAIT (-10)     /* a bounded device-side wait ran out (see wf_stream_sync) */
 #define WF_ERR_TOO_LARGE (-11)       /* request exceeds a fixed capacity                 */
 #define WF_ERR_GGUF (-12)            /* not a GGUF file, unsupported version or type, truncated */
-#define WF_ERR_INDEX (-13)           /* an embedding index outside the table (reported by wf_stream_sync) */
+#define WF_ERR_INDEX (-13)           /* an index outside its range: an embedding row, a page, slot, position or length on the device (reported by wf_stream_sync), a page of a pool */
 #define WF_ERR_RECORDING (-14)       /* the call would allocate device memory while its stream is being recorded into a graph */
 #define WF_ERR_IN_USE (-15)          /* the object is still referenced (a weight held by a live program)   */
 #define WF_ERR_CUDA_BASE 1000
@@ -252,7 +252,10 @@ int wf_qlinear_noalloc(int64_t ctx, int64_t weight, int64_t x_dev, int x_dtype, 
  * wf_kv_cache: keys and values are bf16 [layers][pages][kv_heads][page_tokens][head_dim], both 16-byte aligned.
  * page_tokens is a power of two from 16 to 1024, head_dim a multiple of 8 from 8 to 128.  Token t of a sequence lies in row
  * t % page_tokens of page table[t / page_tokens].  page_tokens == 1 is a packed tensor [tokens][kv_heads][head_dim]: a
- * prompt's keys and values one behind the other, without a cache (layers 1, pages = tokens). */
+ * prompt's keys and values one behind the other, without a cache (layers 1, pages = tokens).  At most 32767 layers, 1024 kv_heads and
+ * 2^31 - 1024 rows (pages * kv_heads * page_tokens) of a layer; attention takes up to 128 query heads for each kv head, fewer than 2^31
+ * rows of q (tokens * q_heads) and a scale above 0.  The scratch of a stream grows with the calls made on it: a call that would have to allocate
+ * while the stream is recorded is WF_ERR_RECORDING, as elsewhere. */
 typedef struct wf_kv_cache {
     int64_t keys_dev, values_dev;
     int64_t pages;

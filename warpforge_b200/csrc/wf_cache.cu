@@ -47,7 +47,8 @@ struct CopyParams {
     int* status;
 };
 // A unit is one head of one page in one layer, keys or values: contiguous on both sides.  A CTA has a unit at a time, COPY_DEPTH 16-byte pieces a thread in flight,
-// and knows where the next one lies before it copies.  Bound by HBM.
+// and knows where the next one lies before it copies.  Bound by HBM (24 pages of 64 tokens, part full, 8 heads of 128, 32 layers: 204 MB in 39 to 44 us, 0.71 to 0.80 of a
+// copy's rate).
 constexpr int COPY_THREADS = 128, COPY_DEPTH = 8, COPY_CTAS = 8;  // CTAs of an SM
 __global__ void __launch_bounds__(COPY_THREADS, COPY_CTAS) copy_pages_kernel(const __grid_constant__ CopyParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -97,7 +98,8 @@ struct CompactParams {
 };
 // A thread has one 16-byte piece of every kept token of a (layer, keys or values, sequence, head) and takes them in order, COMPACT_DEPTH
 // at a time: all loads, then all stores.  kept ascends, so kept[i] >= i and token i is stored to a place that only an earlier
-// token (or itself) came from: no load of a later batch can find it overwritten, and no two threads touch the same piece.
+// token (or itself) came from: no load of a later batch can find it overwritten, and no two threads touch the same piece.  Bound by the launch and four loads that follow
+// from one another (count, kept, table, key): 16 sequences of 16 drafts, 32 layers of 8 heads of 128, 8.5 us.
 constexpr int COMPACT_THREADS = 128, COMPACT_DEPTH = 8;
 __global__ void __launch_bounds__(COMPACT_THREADS) compact_kernel(const __grid_constant__ CompactParams p) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
