@@ -79,11 +79,10 @@ class Decoder:
         self.buf = {n: self._alloc(max_tokens * w * 4) for n, w in widths.items()}
         self.buf["qb"], self.buf["att"] = (self._alloc(max_tokens * s.q_heads * s.head_dim * 2) for _ in range(2))
         # what a call says about its tokens and sequences
-        for n, size in (("ids", 8), ("positions", 4), ("slots", 8), ("ancestors", 8)):
-            self.buf[n] = self._alloc(max_tokens * size)
-        for n in ("offsets", "lens", "counts"):
-            self.buf[n] = self._alloc((max_sequences + 1) * 4)
-        self.buf["tables"], self.buf["kept"] = self._alloc(max_sequences * self._table_width * 4), self._alloc(max_sequences * 64 * 4)
+        self._room = {n: max_tokens * size for n, size in (("ids", 8), ("positions", 4), ("slots", 8), ("ancestors", 8))}
+        self._room.update({n: (max_sequences + 1) * 4 for n in ("offsets", "lens", "counts")}, tables=max_sequences * self._table_width * 4, kept=max_sequences * 64 * 4)
+        self._room = {n: max(room, 16) for n, room in self._room.items()}
+        self.buf.update({n: self._alloc(room) for n, room in self._room.items()})
 
     def _alloc(self, nbytes: int) -> int:
         self._owned.append(self.ctx.allocate(max(nbytes, 16)))
@@ -99,6 +98,8 @@ class Decoder:
 
     def _send(self, name: str, a, dtype: str) -> DeviceTensor:
         a = np.ascontiguousarray(a, {"i32": np.int32, "i64": np.int64}[dtype])
+        if a.nbytes > self._room[name]:
+            raise ValueError(f"{name}: {a.nbytes} bytes, room for {self._room[name]}")
         if a.size:
             self.ctx.copy_to_device(self.buf[name], a)
         return DeviceTensor(self.buf[name], a.shape, dtype)
