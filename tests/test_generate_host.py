@@ -63,3 +63,69 @@ def test_a_copy_has_to_fit_its_buffer(model):
         assert model._send(name, np.zeros(room), dtype).shape() == (room,)
         with pytest.raises(ValueError):
             model._send(name, np.zeros(room + 1), dtype)
+
+
+def state(model, seqs):
+    return [s.tokens for s in seqs], [list(s.pages) for s in seqs], model.cache.free_pages(), model.ctx.copies
+
+
+def test_a_refused_call_changes_nothing(model):
+    a, b, c, d = seqs = [model.sequence() for _ in range(4)]
+    model.prefill([a, b], [np.arange(20), np.arange(5)])
+    for _ in range(3):
+        model.prefill([b], [np.arange(30)])  # 95 tokens of 100
+    before = state(model, seqs)
+    one = [0]
+    refused = [
+        lambda: model.prefill([a, c], [np.arange(20), np.arange(13)]),        # 33 tokens, room for 32
+        lambda: model.prefill([a, b], [one, np.arange(6)]),                   # position 100 of 100
+        lambda: model.prefill(seqs, [one] * 4),                               # four sequences, room for three
+        lambda: model.prefill([a, c], [one]),                                 # a prompt is missing
+        lambda: model.prefill([a, a], [one, one]),                            # named twice
+        lambda: model.step([a, c], [[0] * 16, [0] * 17]),
+        lambda: model.step([a, b], [one, [0] * 6]),
+        lambda: model.step([b], [[0] * 18], [[-1] * 18]),                     # few positions, but 113 tokens in pages for 112
+        lambda: model.step(seqs, [one] * 4),
+        lambda: model.step([a, c], [one]),
+        lambda: model.step([a, a], [one, one]),
+        lambda: model.step([a], [[0, 0]], [[0, 0]]),                          # its own parent
+    ]
+    for i, call in enumerate(refused):
+        with pytest.raises(ValueError):
+            call()
+        assert state(model, seqs) == before, i
+    model.step([b], [[0] * 17], [[-1] * 17])
+
+
+def test_no_more_drafts_than_a_word_has_bits():
+    from warpforge_b200.generate import Decoder, DecoderSpec
+    from warpforge_b200.quant import QuantizationType
+
+    m = Decoder(HostContext(), DecoderSpec(QuantizationType.Q8_0, 64, 2, 1, 32, 64, 1, 64, max_positions=100), pages=12, page_tokens=16, max_tokens=99)
+    s = m.sequence()
+    with pytest.raises(ValueError):
+        m.step([s], [[0] * 65])
+    assert s.tokens == 0 and m.cache.free_pages() == 12
+    m.step([s], [[0] * 64])
+    m.close()
+
+
+def test_a_call_that_fails_leaves_the_sequences_as_long_as_they_were(model):
+    a, b = model.sequence(), model.sequence()
+    model.prefill([a, b], [np.arange(17), np.arange(3)])
+    full = model.sequence()
+    full.extend(16 * (model.cache.free_pages() - 1))
+    before = state(model, [a, b])
+    for call in (lambda: model.prefill([a, b], [np.arange(16), np.arange(14)]), lambda: model.step([a, b], [[0] * 16, [0] * 14])):
+        with pytest.raises(N.WfError):  # one page is left, and each wants one
+            call()
+        assert state(model, [a, b]) == before
+
+    def fails(stream=0):
+        raise N.WfError("wf_stream_sync", N.WF_ERR_INDEX, "WF_ERR_INDEX")
+
+    model.ctx.synchronize = fails
+    for call in (lambda: model.prefill([a, b], [np.arange(15), [0]]), lambda: model.step([a, b], [[0] * 15, [0]])):
+        with pytest.raises(N.WfError):
+            call()
+        assert state(model, [a, b])[:3] == before[:3]

@@ -12,6 +12,7 @@ from __future__ import annotations
 
 import argparse
 import time
+from contextlib import contextmanager
 from dataclasses import dataclass
 from typing import Dict, List, Optional, Sequence as Seq
 
@@ -23,6 +24,7 @@ from . import quant as Q
 from .backend import CudaContext, DeviceTensor, QuantizedWeight
 
 SIZES = {"f32": 4, "bf16": 2, "i32": 4, "i64": 8}
+MAX_DRAFTS = 64  # of a sequence in a step: an ancestors word's bits
 
 
 @dataclass(frozen=True)
@@ -48,7 +50,8 @@ class DecoderSpec:
 
 
 class Decoder:
-    """Seeded synthetic weights; `max_tokens` rows of activations, a cache of `pages` pages."""
+    """Seeded synthetic weights; `max_tokens` rows of activations, a cache of `pages` pages.  A call that is refused or fails leaves the sequences as long
+    as they were."""
 
     def __init__(self, context: CudaContext, spec: DecoderSpec, pages: int, page_tokens: int = 64, max_tokens: int = 512, max_sequences: int = 16, seed: int = 1):
         self.ctx, self.spec, self.max_tokens, self.max_sequences = context, spec, max_tokens, max_sequences
@@ -80,7 +83,7 @@ class Decoder:
         self.buf["qb"], self.buf["att"] = (self._alloc(max_tokens * s.q_heads * s.head_dim * 2) for _ in range(2))
         # what a call says about its tokens and sequences
         self._room = {n: max_tokens * size for n, size in (("ids", 8), ("positions", 4), ("slots", 8), ("ancestors", 8))}
-        self._room.update({n: (max_sequences + 1) * 4 for n in ("offsets", "lens", "counts")}, tables=max_sequences * self._table_width * 4, kept=max_sequences * 64 * 4)
+        self._room.update({n: (max_sequences + 1) * 4 for n in ("offsets", "lens", "counts")}, tables=max_sequences * self._table_width * 4, kept=max_sequences * MAX_DRAFTS * 4)
         self._room = {n: max(room, 16) for n, room in self._room.items()}
         self.buf.update({n: self._alloc(room) for n, room in self._room.items()})
 
@@ -107,14 +110,35 @@ class Decoder:
     def sequence(self) -> A.Sequence:
         return self.cache.sequence()
 
+    # ---- what a call may be, before any of it has happened; what it leaves where it fails later
+    def _admit(self, sequences: Seq[A.Sequence], lens: Seq[int], positions: Seq[np.ndarray]) -> None:
+        if len(sequences) != len(lens) or len({id(s) for s in sequences}) != len(sequences):
+            raise ValueError(f"{len(lens)} entries for {len(sequences)} sequences, each of which is to be named once")
+        if len(sequences) > self.max_sequences:
+            raise ValueError(f"{len(sequences)} sequences, room for {self.max_sequences}")
+        if sum(lens) > self.max_tokens:
+            raise ValueError(f"{sum(lens)} tokens, room for {self.max_tokens}")
+        for s, n, at in zip(sequences, lens, positions):
+            if n and int(np.max(at)) >= self.spec.max_positions:
+                raise ValueError(f"position {int(np.max(at))} of {self.spec.max_positions}")
+            if s.tokens + n > self._table_width * self.cache.page_tokens:
+                raise ValueError(f"a sequence of {s.tokens + n} tokens in tables for {self._table_width * self.cache.page_tokens}")
+
+    @contextmanager
+    def _extended(self, sequences: Seq[A.Sequence], lens: Seq[int]):
+        """The slots of so many new tokens of each sequence; an exception inside makes the sequences as long as they were."""
+        before = [s.tokens for s in sequences]
+        try:
+            yield np.concatenate([np.array(s.extend(n), np.int64) for s, n in zip(sequences, lens)])
+        except BaseException:
+            for s, n in zip(sequences, before):
+                s.truncate(n)
+            raise
+
     # ---- the layers: `attend(layer, q, out)` is the attention of this call
     def _layers(self, ids: np.ndarray, positions: np.ndarray, slots: np.ndarray, attend) -> None:
         ctx, lib, s, b, h = self.ctx, self.ctx._lib, self.spec, self.buf, self.ctx.handle
         n = len(ids)
-        if n > self.max_tokens:
-            raise ValueError(f"{n} tokens, room for {self.max_tokens}")
-        if n and int(np.max(positions)) >= s.max_positions:
-            raise ValueError(f"position {int(np.max(positions))} of {s.max_positions}")
         tokens = self._send("ids", ids, "i64")
         pos, slot = self._send("positions", positions, "i32"), self._send("slots", slots, "i64")
         part = lambda name, heads, dtype: DeviceTensor(b[name], (n, heads, s.head_dim), dtype)  # noqa: E731
@@ -154,27 +178,28 @@ class Decoder:
         return out
 
     def _tables(self, sequences: Seq[A.Sequence]) -> DeviceTensor:
-        if len(sequences) > self.max_sequences:
-            raise ValueError(f"{len(sequences)} sequences, room for {self.max_sequences}")
         return self._send("tables", self.cache.tables(sequences, self._table_width), "i32")
 
     def prefill(self, sequences: Seq[A.Sequence], prompts: Seq[np.ndarray]) -> List[np.ndarray]:
         """The prompts behind what the sequences hold already; logits [len(prompt), vocab] of each."""
         lens = [len(p) for p in prompts]
         positions = [s.tokens + np.arange(n) for s, n in zip(sequences, lens)]
-        slots = [np.array(s.extend(n), np.int64) for s, n in zip(sequences, lens)]
+        self._admit(sequences, lens, positions)
         offsets = np.concatenate(([0], np.cumsum(lens)))
-        tables, off = self._tables(sequences), self._send("offsets", offsets, "i32")
-        total = self._send("lens", [s.tokens for s in sequences], "i32")
-        self._layers(np.concatenate(prompts), np.concatenate(positions), np.concatenate(slots),
-                     lambda q, k, v, out: A.PromptAttention(self.ctx, q, k, v, out, off, tables=tables, k_lens=total).run())
-        logits = self._logits(int(offsets[-1]))
+        with self._extended(sequences, lens) as slots:
+            tables, off = self._tables(sequences), self._send("offsets", offsets, "i32")
+            total = self._send("lens", [s.tokens for s in sequences], "i32")
+            self._layers(np.concatenate(prompts), np.concatenate(positions), slots,
+                         lambda q, k, v, out: A.PromptAttention(self.ctx, q, k, v, out, off, tables=tables, k_lens=total).run())
+            logits = self._logits(int(offsets[-1]))
         return [logits[a:b] for a, b in zip(offsets, offsets[1:])]
 
     def step(self, sequences: Seq[A.Sequence], tokens: Seq[Seq[int]], parents: Optional[Seq[Seq[int]]] = None) -> List[np.ndarray]:
         """New tokens of each sequence (one, or up to 64 drafted ones): parents[s][i] is the index of token i's parent among them, -1: the
         context; not given: a chain.  Logits [len(tokens[s]), vocab]; the tokens stay in the cache until ``keep`` says which of them remain."""
         lens = [len(t) for t in tokens]
+        if max(lens, default=0) > MAX_DRAFTS:
+            raise ValueError(f"{max(lens)} new tokens of a sequence, at most {MAX_DRAFTS}")
         context = [s.tokens for s in sequences]
         words, depth = [], []
         for s, n in enumerate(lens):
@@ -187,14 +212,15 @@ class Decoder:
             words += [w for w, _ in seen]
             depth.append(np.array([d for _, d in seen], np.int64))
         positions = [c + d for c, d in zip(context, depth)]
-        slots = [np.array(s.extend(n), np.int64) for s, n in zip(sequences, lens)]
+        self._admit(sequences, lens, positions)
         offsets = np.concatenate(([0], np.cumsum(lens)))
-        tables, off, ctx_lens = self._tables(sequences), self._send("offsets", offsets, "i32"), self._send("lens", context, "i32")
-        anc = self._send("ancestors", np.array(words, np.uint64).view(np.int64), "i64")
-        self._layers(np.concatenate([np.asarray(t) for t in tokens]), np.concatenate(positions), np.concatenate(slots),
-                     lambda q, k, v, out: A.TreeAttention(self.ctx, q, k, v, out, tables, ctx_lens, max_context=max(context), max_drafts=max(lens), q_offsets=off,
-                                                          ancestors=anc).run())
-        logits = self._logits(int(offsets[-1]))
+        with self._extended(sequences, lens) as slots:
+            tables, off, ctx_lens = self._tables(sequences), self._send("offsets", offsets, "i32"), self._send("lens", context, "i32")
+            anc = self._send("ancestors", np.array(words, np.uint64).view(np.int64), "i64")
+            self._layers(np.concatenate([np.asarray(t) for t in tokens]), np.concatenate(positions), slots,
+                         lambda q, k, v, out: A.TreeAttention(self.ctx, q, k, v, out, tables, ctx_lens, max_context=max(context), max_drafts=max(lens), q_offsets=off,
+                                                              ancestors=anc).run())
+            logits = self._logits(int(offsets[-1]))
         return [logits[a:b] for a, b in zip(offsets, offsets[1:])]
 
     def keep(self, sequences: Seq[A.Sequence], drafted: Seq[int], kept: Seq[Seq[int]]) -> None:
