@@ -129,3 +129,20 @@ def test_a_call_that_fails_leaves_the_sequences_as_long_as_they_were(model):
         with pytest.raises(N.WfError):
             call()
         assert state(model, [a, b])[:3] == before[:3]
+
+
+def test_what_is_kept_has_been_drafted(model):
+    a, b = model.sequence(), model.sequence()
+    model.prefill([a, b], [np.arange(10), np.arange(3)])
+    model.step([a, b], [[0] * 5, [0] * 5])
+    before = state(model, [a, b])
+    for drafted, kept in (([5, 5], [[0, 5], [0]]), ([5, 5], [[0], [-1]]), ([5, 5], [[2, 1], [0]]), ([5, 5], [[1, 1], [0]]), ([16, 5], [[15], [0]]), ([-1, 5], [[], [0]]),
+                          ([5, 5], [[0]]), ([5], [[0]]), ([5, 5], [[0], [0], [0]])):
+        with pytest.raises(ValueError):
+            model.keep([a, b], drafted, kept)
+        assert state(model, [a, b]) == before, (drafted, kept)
+    with pytest.raises(ValueError):
+        model.keep([a, a], [5, 5], [[0], [0]])
+    assert state(model, [a, b]) == before
+    model.keep([a, b], [5, 5], [[0, 2, 4], []])
+    assert (a.tokens, b.tokens) == (13, 3)

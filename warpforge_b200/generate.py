@@ -225,7 +225,12 @@ class Decoder:
 
     def keep(self, sequences: Seq[A.Sequence], drafted: Seq[int], kept: Seq[Seq[int]]) -> None:
         """After ``step`` with drafted[s] tokens: those of kept[s] (ascending, a path of the tree) remain, moved up to the end of the context."""
-        width = max(1, max(len(k) for k in kept))
+        if not len(sequences) == len(drafted) == len(kept) or len({id(s) for s in sequences}) != len(sequences):
+            raise ValueError(f"{len(drafted)} and {len(kept)} entries for {len(sequences)} sequences, each of which is to be named once")
+        for s, n, k in zip(sequences, drafted, kept):
+            if not 0 <= n <= s.tokens or any(not before < i < n for before, i in zip([-1, *k], k)):
+                raise ValueError(f"tokens {list(k)} of {n} drafted ones in a sequence of {s.tokens}")
+        width = max([1] + [len(k) for k in kept])
         rows = np.zeros((len(sequences), width), np.int32)
         for row, k in zip(rows, kept):
             row[:len(k)] = k
