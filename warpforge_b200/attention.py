@@ -279,17 +279,27 @@ class KvCache:
             out.append(Sequence(self, pages, s.tokens))
         if pairs:
             ctx = self.context
-            to, counts, room = self._fork_arrays.get(stream, (0, 0, 0))
-            if len(pairs) > room:
-                for p in (to, counts):
-                    if p:
-                        ctx.free(p)
-                room = max(16, 2 * len(pairs))
-                to, counts, _ = self._fork_arrays[stream] = ctx.allocate(room * 8), ctx.allocate(room * 4), room
+            to, counts = self._arrays(len(pairs), stream)
             ctx.copy_to_device(to, np.array(pairs, np.int32), stream)
             ctx.copy_to_device(counts, np.array(rows, np.int32), stream)
             self.copy_pages(DeviceTensor(to, (len(pairs), 2), "i32"), DeviceTensor(counts, (len(rows),), "i32"), stream)
         return out
+
+    def _arrays(self, n: int, stream: int):
+        """Device arrays for the pairs and rows of n copies on this stream; the old ones stay until larger ones are there."""
+        ctx, (to, counts, room) = self.context, self._fork_arrays.get(stream, (0, 0, 0))
+        if n > room:
+            old, room = [p for p in (to, counts) if p], max(16, 2 * n)
+            to = ctx.allocate(room * 8)
+            try:
+                counts = ctx.allocate(room * 4)
+            except BaseException:
+                ctx.free(to)
+                raise
+            self._fork_arrays[stream] = to, counts, room
+            for p in old:
+                ctx.free(p)
+        return to, counts
 
     def layer(self, i: int):
         """keys and values of one layer, bf16 [pages, kv_heads, page_tokens, head_dim]."""
