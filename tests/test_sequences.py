@@ -84,3 +84,20 @@ def test_arrays_of_forks_that_cannot_grow(cache, fail):
     assert cache.context.copied[-1] == ((a.pages[0], again.pages[0]), 5, 0)
     cache.context.fail = ()
     assert len({s.pages[0] for s in cache.fork([a] * 20) + [few, again]}) == 22
+
+
+@pytest.mark.parametrize("fail", ["allocate", "second allocate", "copy", "copy_pages"])
+def test_a_fork_that_fails_late_holds_nothing(cache, fail):
+    a, b = cache.sequence(), cache.sequence()
+    a.extend(40)
+    b.extend(33)
+    free, holders = cache.free_pages(), [cache.holders(p) for p in a.pages + b.pages]
+    cache.context.fail = (fail,)
+    with pytest.raises(MemoryError):
+        cache.fork([a, b, a])
+    assert cache.free_pages() == free and [cache.holders(p) for p in a.pages + b.pages] == holders
+    cache.context.fail = ()
+    c = a.fork()
+    for s in (a, b, c):
+        s.free()
+    assert cache.free_pages() == 60

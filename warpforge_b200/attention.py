@@ -265,7 +265,7 @@ class KvCache:
         self._share(shared)
         try:
             fresh = self._take(len(part))
-        except Exception:
+        except BaseException:
             self._release(shared)
             raise
         out, pairs, rows = [], [], []
@@ -277,13 +277,20 @@ class KvCache:
                 pairs.append((s.pages[whole], pages[-1]))
                 rows.append(rest)
             out.append(Sequence(self, pages, s.tokens))
-        if pairs:
-            ctx = self.context
-            to, counts = self._arrays(len(pairs), stream)
-            ctx.copy_to_device(to, np.array(pairs, np.int32), stream)
-            ctx.copy_to_device(counts, np.array(rows, np.int32), stream)
-            self.copy_pages(DeviceTensor(to, (len(pairs), 2), "i32"), DeviceTensor(counts, (len(rows),), "i32"), stream)
+        try:
+            self._copy_rows(pairs, rows, stream)
+        except BaseException:
+            self._release(shared + fresh)
+            raise
         return out
+
+    def _copy_rows(self, pairs, rows, stream: int) -> None:
+        """copy_pages of page numbers that the host has."""
+        if pairs:
+            to, counts = self._arrays(len(pairs), stream)
+            self.context.copy_to_device(to, np.array(pairs, np.int32), stream)
+            self.context.copy_to_device(counts, np.array(rows, np.int32), stream)
+            self.copy_pages(DeviceTensor(to, (len(pairs), 2), "i32"), DeviceTensor(counts, (len(rows),), "i32"), stream)
 
     def _arrays(self, n: int, stream: int):
         """Device arrays for the pairs and rows of n copies on this stream; the old ones stay until larger ones are there."""
