@@ -101,3 +101,113 @@ def test_a_fork_that_fails_late_holds_nothing(cache, fail):
     for s in (a, b, c):
         s.free()
     assert cache.free_pages() == 60
+
+
+def write(cache, s, slots, tokens):
+    """What a step does with the slots: the pages they lie in have to be this sequence's alone."""
+    size = cache.page_tokens
+    for slot, token in zip(slots, tokens):
+        assert slot // size in s.pages and cache.holders(slot // size) == 1
+        cache.memory[slot] = token
+
+
+def read(cache, s):
+    size = cache.page_tokens
+    apply_copies(cache)
+    return [cache.memory[s.pages[t // size] * size + t % size] for t in range(s.tokens)]
+
+
+def apply_copies(cache):
+    size = cache.page_tokens
+    for (a, b), rows, _ in cache.context.copied:
+        for r in range(size):
+            cache.memory.pop(b * size + r, None)
+        cache.memory.update({b * size + r: cache.memory[a * size + r] for r in range(rows)})
+    cache.context.copied.clear()
+
+
+@pytest.mark.parametrize("cut,more", [(20, 4), (17, 1), (31, 1), (31, 20), (5, 40), (32, 3), (16, 3)])
+def test_a_fork_that_is_cut_back_writes_to_pages_of_its_own(cache, cut, more):
+    cache.memory = {}
+    a = cache.sequence()
+    write(cache, a, a.extend(40), range(40))
+    b = a.fork(stream=3)
+    for s, name in ((a, 1000), (b, 2000)):  # the one that is cut first, then the other
+        s.truncate(cut)
+        slots = s.extend(more, stream=3)
+        apply_copies(cache)
+        write(cache, s, slots, range(name, name + more))
+        if s is a:
+            assert read(cache, b) == list(range(40))
+    assert read(cache, a) == [*range(cut), *range(1000, 1000 + more)] and read(cache, b) == [*range(cut), *range(2000, 2000 + more)]
+    for s in (a, b):
+        s.free()
+    assert cache.free_pages() == 60
+
+
+def test_the_last_holder_writes_in_place(cache):
+    a = cache.sequence()
+    a.extend(32)
+    b = a.fork()
+    a.truncate(20)
+    b.free()
+    page = a.pages[1]
+    assert a.extend(0) == [] and a.extend(2) == [page * 16 + 4, page * 16 + 5] and not cache.context.copied
+
+
+def test_an_extension_that_cannot_be_changes_nothing(cache):
+    a = cache.sequence()
+    a.extend(32)
+    b = a.fork()
+    a.truncate(20)
+    rest = cache.sequence()
+    rest.extend(16 * (cache.free_pages() - 1))
+    pages = list(a.pages)
+    with pytest.raises(N.WfError):
+        a.extend(13)  # a copy of the shared page and one more
+    assert a.pages == pages and a.tokens == 20 and cache.free_pages() == 1 and cache.holders(pages[1]) == 2
+    for fail in ("allocate", "copy", "copy_pages"):
+        cache.context.fail = (fail,)
+        with pytest.raises(MemoryError):
+            a.extend(12)
+        assert a.pages == pages and a.tokens == 20 and cache.free_pages() == 1 and cache.holders(pages[1]) == 2
+    cache.context.fail = ()
+    a.extend(12)
+    assert cache.free_pages() == 0 and a.pages[0] == b.pages[0] and a.pages[1] != b.pages[1]
+
+
+def test_sequences_against_lists(cache):
+    """Growing, cutting and forking at random: every sequence reads what was written to it."""
+    rng, cache.memory, live, number = random.Random(5), {}, [], 0
+    for _ in range(3000):
+        what = rng.random()
+        if not live or what < 0.05:
+            live.append((cache.sequence(), []))
+            continue
+        s, text = rng.choice(live)
+        try:
+            if what < 0.5:
+                n = rng.choice((0, 1, 1, 5, 16, 37))
+                slots = s.extend(n)
+                apply_copies(cache)
+                new = list(range(number, number + n))
+                number += n
+                write(cache, s, slots, new)
+                text += new
+            elif what < 0.7:
+                n = rng.randint(0, s.tokens)
+                s.truncate(n)
+                del text[n:]
+            elif what < 0.85:
+                live.append((s.fork(), list(text)))
+            else:
+                s.free()
+                live = [x for x in live if x[0] is not s]
+        except N.WfError as e:
+            assert e.status == N.WF_ERR_TOO_LARGE
+            live[0][0].free()
+            del live[0]
+        for t, want in live:
+            assert read(cache, t) == want
+        held = [p for t, _ in live for p in t.pages]
+        assert cache.free_pages() == 60 - len(set(held)) and all(cache.holders(p) == held.count(p) for p in set(held))

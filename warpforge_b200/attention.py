@@ -164,16 +164,16 @@ class Sequence:
     def __init__(self, cache: "KvCache", pages: List[int], tokens: int):
         self.cache, self.pages, self.tokens = cache, pages, tokens
 
-    def extend(self, n: int) -> List[int]:
-        """Room for n more tokens; their slots (page * page_tokens + row)."""
+    def extend(self, n: int, stream: int = 0) -> List[int]:
+        """Room for n more tokens; their slots (page * page_tokens + row), in pages that are this sequence's alone: a part-full last page that others hold
+        too is replaced by a copy of the rows in use (on `stream`, the one that the slots will be written on)."""
         if n < 0:
             raise ValueError(f"extend by {n} tokens")
         c, size = self.cache, self.cache.page_tokens
-        need = -(-(self.tokens + n) // size) - len(self.pages)
-        if need > 0:
-            self.pages += c._take(need)
-        slots = [self.pages[t // size] * size + t % size for t in range(self.tokens, self.tokens + n)]
-        self.tokens += n
+        end = self.tokens + n
+        self.pages += c._own([self], [(self.tokens, end)], max(0, -(-end // size) - len(self.pages)), stream)
+        slots = [self.pages[t // size] * size + t % size for t in range(self.tokens, end)]
+        self.tokens = end
         return slots
 
     def truncate(self, tokens: int) -> None:
@@ -283,6 +283,28 @@ class KvCache:
             self._release(shared + fresh)
             raise
         return out
+
+    def _own(self, sequences: Seq[Sequence], spans, more: int, stream: int) -> List[int]:
+        """Pages that hold tokens [spans[i][0], spans[i][1]) of a sequence and have other holders too are replaced by copies; `more` free pages besides, which
+        are returned.  All or nothing."""
+        size, places, left = self.page_tokens, [], {}
+        for s, (start, stop) in zip(sequences, spans):
+            for i in range(start // size, min(len(s.pages), -(-stop // size))) if start < stop else ():
+                page = s.pages[i]
+                left.setdefault(page, self.holders(page))
+                if left[page] > 1:
+                    left[page] -= 1
+                    places.append((s, i))
+        fresh = self._take(len(places) + more)
+        try:
+            self._copy_rows([(s.pages[i], page) for (s, i), page in zip(places, fresh)], [min(size, s.tokens - i * size) for s, i in places], stream)
+        except BaseException:
+            self._release(fresh)
+            raise
+        self._release([s.pages[i] for s, i in places])
+        for (s, i), page in zip(places, fresh):
+            s.pages[i] = page
+        return fresh[len(places):]
 
     def _copy_rows(self, pairs, rows, stream: int) -> None:
         """copy_pages of page numbers that the host has."""
