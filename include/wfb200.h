@@ -339,7 +339,8 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* args, const wf_
  * use, 0 (no array) = all.  No page may be the target of two pairs or source and target at once. */
 int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev, int64_t rows_dev, int64_t n, int64_t stream);
 /* After drafting: in every layer, token context[s] + kept[s][i] of sequence s becomes token context[s] + i, for i < counts[s].
- * kept int32 [seqs][kept_stride] ascending; counts int32 [seqs]; tables and context as in wf_tree_attention. */
+ * kept int32 [seqs][kept_stride] ascending; counts int32 [seqs]; tables and context as in wf_tree_attention.  A page that tokens
+ * move to, like one that wf_qk_norm_rope stores to, should have one holder: whoever else has it in a table reads what is written. */
 int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, int64_t table_stride, int64_t context_dev, int64_t kept_dev,
                      int64_t kept_stride, int64_t counts_dev, int64_t seqs, int64_t stream);
 

@@ -146,3 +146,22 @@ def test_what_is_kept_has_been_drafted(model):
     assert state(model, [a, b]) == before
     model.keep([a, b], [5, 5], [[0, 2, 4], []])
     assert (a.tokens, b.tokens) == (13, 3)
+
+
+def test_drafts_that_are_kept_do_not_move_in_shared_pages(model):
+    """A fork between step and keep shares the pages of the drafts; keep moves tokens in them."""
+    a, other = model.sequence(), model.sequence()
+    model.prefill([a], [np.arange(10)])
+    model.step([a], [[0] * 30], [[-1] * 30])
+    fork = a.fork()
+    shared = list(a.pages[:2])
+    assert [model.cache.holders(p) for p in shared] == [2, 2]
+    model.keep([a], [30], [list(range(20))])  # as they lie: nothing moves
+    assert a.pages[:2] == shared and fork.pages[:2] == shared
+    a.free()
+    a = fork.fork()
+    sent = {}
+    model.cache.compact = lambda tables, lens, kept, counts: sent.update(pages=list(a.pages))
+    model.keep([a], [30], [[0, 1, 5, 9]])  # rows 12 and 13 of page 0
+    assert sent["pages"][0] == a.pages[0] != fork.pages[0] and fork.pages[:2] == shared
+    assert a.tokens == 14 and model.cache.holders(a.pages[0]) == 1

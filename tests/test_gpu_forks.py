@@ -31,3 +31,29 @@ def test_a_fork_is_cut_back_and_goes_on(model):  # noqa: F811
     for s in (a, b, c):
         s.free()
     assert model.cache.free_pages() == 64
+
+
+def test_a_fork_between_drafts_and_what_is_kept(model):  # noqa: F811
+    """Two sequences keep different paths of the same drafts, which lie in pages that both hold."""
+    rng = np.random.default_rng(12)
+    for start in (10, 45):
+        text = list(map(int, rng.integers(0, 320, start)))
+        a = model.sequence()
+        model.prefill([a], [np.array(text)])
+        tree = [-1, 0, 0, 1, 2, 3, 4, 6, 7, 8, 9, 10, 5, 12] + [13 + i for i in range(12)]
+        draft = list(map(int, rng.integers(0, 320, len(tree))))
+        model.step([a], [draft], [tree])
+        b = a.fork()
+
+        def path(i):
+            return [] if i < 0 else path(tree[i]) + [i]
+
+        kept = [path(11), path(25)]
+        model.keep([a], [len(tree)], kept[:1])
+        model.keep([b], [len(tree)], kept[1:])
+        texts = [text + [draft[i] for i in k] for k in kept]
+        assert [a.tokens, b.tokens] == [len(t) for t in texts]
+        goes_on(model, rng, [a, b], texts)
+        for s in (a, b):
+            s.free()
+        assert model.cache.free_pages() == 64

@@ -211,3 +211,21 @@ def test_sequences_against_lists(cache):
             assert read(cache, t) == want
         held = [p for t, _ in live for p in t.pages]
         assert cache.free_pages() == 60 - len(set(held)) and all(cache.holders(p) == held.count(p) for p in set(held))
+
+
+def test_pages_are_made_private_before_tokens_move(cache):
+    a = cache.sequence()
+    a.extend(50)
+    b, c = cache.fork([a, a])
+    before = list(b.pages)
+    cache.context.copied.clear()
+    cache.own([a, b], [(20, 22), (33, 33)], stream=5)
+    assert cache.context.copied == [((before[1], a.pages[1]), 16, 5)]
+    assert a.pages[0] == b.pages[0] and a.pages[1] not in (before[1],) and a.pages[2] == before[2] and b.pages == before
+    cache.context.copied.clear()
+    cache.own([b, c], [(0, 48), (15, 33)])  # page 1 has two holders left: one copy is enough
+    moved = [pair for pair, _, _ in cache.context.copied]
+    assert len(moved) == 3 + 3 - 1 and not set(b.pages) & set(c.pages[:3])
+    for s in (a, b, c):
+        s.free()
+    assert cache.free_pages() == 60

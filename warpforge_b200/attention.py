@@ -13,7 +13,7 @@ from __future__ import annotations
 
 import ctypes
 import math
-from typing import List, Optional, Sequence as Seq
+from typing import List, Optional, Sequence as Seq, Tuple
 
 import numpy as np
 
@@ -284,6 +284,11 @@ class KvCache:
             raise
         return out
 
+    def own(self, sequences: Seq[Sequence], spans: Seq[Tuple[int, int]], stream: int = 0) -> None:
+        """Before tokens [start, stop) of each sequence are written to (``compact``): pages of them that other sequences hold too are replaced by copies of the
+        rows in use, all in one call on `stream`.  Tables made before this name the old pages."""
+        self._own(sequences, spans, 0, stream)
+
     def _own(self, sequences: Seq[Sequence], spans, more: int, stream: int) -> List[int]:
         """Pages that hold tokens [spans[i][0], spans[i][1]) of a sequence and have other holders too are replaced by copies; `more` free pages besides, which
         are returned.  All or nothing."""
@@ -347,7 +352,7 @@ class KvCache:
 
     def compact(self, tables: DeviceTensor, context_lens: DeviceTensor, kept: DeviceTensor, counts: DeviceTensor, stream: int = 0) -> None:
         """In every layer token context_lens[s] + kept[s][i] of sequence s becomes token context_lens[s] + i, i < counts[s]; kept i32
-        [seqs, most] ascending."""
+        [seqs, most] ascending.  The pages that tokens move to have to be the sequence's alone (``own``)."""
         seqs, most = kept.shape()
         ctx = self.context
         ctx._ck("wf_cache_compact", ctx._lib.wf_cache_compact(

@@ -235,6 +235,8 @@ class Decoder:
         for row, k in zip(rows, kept):
             row[:len(k)] = k
         context = [s.tokens - n for s, n in zip(sequences, drafted)]
+        still = [next((i for i, j in enumerate(k) if i != j), len(k)) for k in kept]  # tokens that lie where they belong
+        self.cache.own(sequences, [(c + n, c + len(k)) for c, n, k in zip(context, still, kept)])
         tables, lens = self._tables(sequences), self._send("lens", context, "i32")
         self.cache.compact(tables, lens, self._send("kept", rows, "i32"), self._send("counts", [len(k) for k in kept], "i32"))
         self.ctx.synchronize()
