@@ -229,3 +229,16 @@ def test_pages_are_made_private_before_tokens_move(cache):
     for s in (a, b, c):
         s.free()
     assert cache.free_pages() == 60
+
+
+@pytest.mark.parametrize("fail", ["allocate", "second allocate", "pool"])
+def test_a_cache_that_cannot_be_made_holds_no_memory(fail):
+    from warpforge_b200.attention import KvCache
+
+    ctx = Context()
+    ctx.fail = (fail,)
+    if fail == "pool":
+        ctx._lib.wf_pages_create = lambda pages, pool: N.WF_ERR_SHAPE
+    with pytest.raises((MemoryError, N.WfError)):
+        KvCache(ctx, layers=2, pages=60, page_tokens=16, kv_heads=1, head_dim=64)
+    assert not ctx.live

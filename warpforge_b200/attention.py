@@ -205,19 +205,24 @@ class KvCache:
         shape = (layers, pages, kv_heads, page_tokens, head_dim)
         self.context, self.layers, self.page_count, self.page_tokens, self.kv_heads, self.head_dim = context, layers, pages, page_tokens, kv_heads, head_dim
         self._owned, self._pool = [], 0
-        if keys is None:
-            for _ in range(2):
-                self._owned.append(context.allocate(int(np.prod(shape)) * 2))
-            keys, values = (DeviceTensor(p, shape, "bf16", owner=context) for p in self._owned)
-        self.keys, self.values = keys, values
-        for name, t in (("keys", keys), ("values", values)):
-            _typed(name, t, "bf16", *shape)
-        self._args = _cache_args(keys, values)
-        self._ref = ctypes.byref(self._args)
-        pool = ctypes.c_int64()
-        N.check("wf_pages_create", context._lib.wf_pages_create(pages, ctypes.byref(pool)))
-        self._pool = pool.value
         self._fork_arrays = {}  # stream: device arrays of its forks (pairs, rows, how many fit)
+        try:
+            if keys is None:
+                for _ in range(2):
+                    self._owned.append(context.allocate(int(np.prod(shape)) * 2))
+                keys, values = (DeviceTensor(p, shape, "bf16", owner=context) for p in self._owned)
+            self.keys, self.values = keys, values
+            for name, t in (("keys", keys), ("values", values)):
+                _typed(name, t, "bf16", *shape)
+            self._args = _cache_args(keys, values)
+            self._ref = ctypes.byref(self._args)
+            pool = ctypes.c_int64()
+            N.check("wf_pages_create", context._lib.wf_pages_create(pages, ctypes.byref(pool)))
+        except BaseException:
+            for p in self._owned:
+                context.free(p)
+            raise
+        self._pool = pool.value
 
     # ---- pages
     def _ids(self, ids: Seq[int]):
