@@ -1,0 +1,95 @@
+"""NaN and Inf that a row does see, at every place of a tile (bounds and helpers as in test_gpu_attention.py)."""
+import numpy as np
+import pytest
+from test_gpu_attention import backend, run_prompt, run_tree  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+VALUES = [float("nan"), float("inf")]
+
+
+def check_rows(out, q, bad, sees, value):
+    """Head h of a sequence's rows (out, q [rows, heads, dim]) is NaN in the rows that see its bad key, which has the value in element bad[h][1], and no others: a
+    score of NaN, or of plus infinity; with minus infinity the key has no weight.  sees: [rows, heads]."""
+    import torch
+
+    element = torch.tensor([e for _, e in bad], device="cuda")
+    factor = q.float().gather(2, element[None, :, None].expand(q.shape[0], -1, 1))[..., 0]
+    nan = sees & (factor > 0 if value == float("inf") else torch.ones_like(sees))
+    assert torch.equal(torch.isnan(out).all(-1), nan) and torch.equal(torch.isnan(out).any(-1), nan)
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads,rows,first", [(128, 201, 40), (128, 201, 0), (16, 300, 0), (16, 300, 16), (16, 300, 32), (16, 300, 48), (16, 300, 150), (16, 300, 171)])
+def test_prompt_a_bad_key_reaches_the_rows_that_see_it(backend, heads, rows, first, dim, value):  # noqa: F811
+    """Only the key is bad, its value is not; key first + h of head h.  128 heads: items of two tiles of rows; 16: of one, which two groups of warps share."""
+    import torch
+
+    bad, kept = [(first + h, h % dim) for h in range(heads)], {}
+
+    def edit(q, keys, values, tables):
+        for h, (t, e) in enumerate(bad):
+            keys[t, h, e] = value
+        kept["q"] = q
+
+    out = run_prompt(backend, [rows, 3], heads, heads, dim, edit=edit)
+    sees = torch.arange(rows, device="cuda")[:, None] >= torch.tensor([t for t, _ in bad], device="cuda")[None, :]
+    check_rows(out[:rows], kept["q"][:rows], bad, sees, value)
+    assert torch.isfinite(out[rows:]).all()
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("page,first", [(16, 64), (256, 1220)])
+def test_prompt_a_bad_key_of_the_past(backend, page, first, dim, value):  # noqa: F811
+    import torch
+
+    bad, kept = [(first + h, h % dim) for h in range(128)], {}
+
+    def edit(q, keys, values, tables):
+        for h, (t, e) in enumerate(bad):
+            keys[int(tables[0][t // page]), h, t % page, e] = value
+        kept["q"] = q
+
+    out = run_prompt(backend, [30], 128, 128, dim, page, [1310], edit=edit)
+    sees = torch.arange(1310, 1340, device="cuda")[:, None] >= torch.tensor([t for t, _ in bad], device="cuda")[None, :]
+    check_rows(out, kept["q"], bad, sees, value)
+
+
+def run_bad_tree(backend, contexts, drafts, q_heads, kv_heads, dim, page, place, value):  # noqa: F811
+    """place(s, h): the position of kv head h's bad key in sequence s, or None.  Chains."""
+    import torch
+
+    kept = {}
+
+    def edit(q, keys, values, tables):
+        for s in range(len(contexts)):
+            for h in range(kv_heads):
+                t = place(s, h)
+                if t is not None:
+                    keys[int(tables[s][t // page]), h, t % page, h % dim] = value
+        kept["q"] = q
+
+    out = run_tree(backend, contexts, [drafts] * len(contexts), q_heads, kv_heads, dim, page, shape="chain", edit=edit)
+    group = q_heads // kv_heads
+    for s, context in enumerate(contexts):
+        at = [place(s, h // group) for h in range(q_heads)]
+        rows = slice(s * drafts, (s + 1) * drafts)
+        sees = torch.arange(context, context + drafts, device="cuda")[:, None] >= torch.tensor([10**6 if t is None else t for t in at], device="cuda")[None, :]
+        check_rows(out[rows], kept["q"][rows], [(0, h // group % dim) for h in range(q_heads)], sees, value)
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("drafts,context", [(40, 100), (12, 400), (1, 100)])
+def test_tree_a_bad_key_reaches_the_rows_that_see_it(backend, drafts, context, dim, value):  # noqa: F811
+    """Rows on the 5th-generation tensor cores (160 and 48 of a kv head) and on mma.sync (4); keys of the context and drafted ones."""
+    run_bad_tree(backend, [context, context], drafts, 256, 64, dim, 16, lambda s, h: h + s * (context - 30) if h + s * (context - 30) < context + drafts else None, value)
+
+
+@pytest.mark.parametrize("value", VALUES)
+@pytest.mark.parametrize("drafts", [20, 1])
+def test_tree_a_bad_key_of_a_cut_unit(backend, drafts, value):  # noqa: F811
+    for first in range(0, 64, 8):
+        run_bad_tree(backend, [6000], drafts, 32, 8, 64, 64, lambda s, h: first + h + (3000 + 7 * first if h % 2 else 0), value)  # noqa: B023

@@ -143,6 +143,11 @@ __device__ __forceinline__ float ex2(float x) {
     asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
     return y;
 }
+__device__ __forceinline__ float max3_or_nan(float a, float b, float c) {  // the largest, or NaN where one of them is
+    float d;
+    asm("max.NaN.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
 __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
     float2 d;
     asm("{\n\t.reg .b64 x, y, z, w;\n\tmov.b64 x, {%2, %3};\n\tmov.b64 y, {%4, %5};\n\tmov.b64 z, {%6, %7};\n\tfma.rn.f32x2 w, x, y, z;\n\tmov.b64 {%0, %1}, w;\n\t}"
@@ -152,7 +157,7 @@ __device__ __forceinline__ float2 fma2(float2 a, float2 b, float2 c) {
 }
 // 2^x for x <= PA_RESCALE without the special function unit, which has 16 of them a cycle and would be what a tile waits for: x = n + f with n the nearest
 // integer (adding 1.5 * 2^23 leaves it in the low bits), 2^f by a cubic on [-1/2, 1/2], 1 at 0, with the smallest largest relative error (1.0e-4, 1/38 of
-// what a weight may be off by its rounding to bf16), n added to the exponent.  0 from -127 on.
+// what a weight may be off by its rounding to bf16), n added to the exponent.  0 from -127 on, and for NaN: a row that sees one is marked by its maxima.
 __device__ __forceinline__ float2 add2(float2 a, float2 b);
 __device__ __forceinline__ float2 mul2(float2 a, float2 b) {
     float2 d;
@@ -422,7 +427,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
 #pragma unroll
                     for (int i = 32 * c; i < 32 * c + 32; i += 8)
 #pragma unroll
-                        for (int e = 0; e < 4; e++) top[e] = fmaxf(fmaxf(top[e], __uint_as_float(s[i + 2 * e])), __uint_as_float(s[i + 2 * e + 1]));
+                        for (int e = 0; e < 4; e++) top[e] = max3_or_nan(top[e], __uint_as_float(s[i + 2 * e]), __uint_as_float(s[i + 2 * e + 1]));
                 };
                 tmem_ld32_start(s_at, s);
                 tmem_wait_ld32(s);
@@ -456,7 +461,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     for (int c = 0; c < 3; c++) maxima(c);
                 }
                 maxima(3);
-                const float tile_top = fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3]));
+                float tile_top = max3_or_nan(max3_or_nan(top[0], top[1], top[2]), top[3], -INFINITY);
+                if (tile_top != tile_top) {  // a score that the row sees is NaN: so is its sum from here on, whatever the cubic makes of it
+                    l = tile_top;
+                    tile_top = -INFINITY;
+                }
                 if (i_tile == 0) {
                     m = tile_top;
                 } else if (__any_sync(0xFFFFFFFFu, (tile_top - m) * scale > PA_RESCALE)) {
