@@ -93,3 +93,35 @@ def test_tree_a_bad_key_reaches_the_rows_that_see_it(backend, drafts, context, d
 def test_tree_a_bad_key_of_a_cut_unit(backend, drafts, value):  # noqa: F811
     for first in range(0, 64, 8):
         run_bad_tree(backend, [6000], drafts, 32, 8, 64, 64, lambda s, h: first + h + (3000 + 7 * first if h % 2 else 0), value)  # noqa: B023
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("pairs", ["half", "adjacent"])
+@pytest.mark.parametrize("dim,rot", [(64, 16), (80, 40), (96, 64), (128, 64), (128, 8)])
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_rope_an_element_that_is_not_rotated_stays_alone(backend, dim, rot, pairs, dtype, value):  # noqa: F811
+    """Token t has NaN or Inf in element rot + t of q and k: the other elements are as they are without it."""
+    import torch
+    from test_gpu_attention import held, i32
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(dim + rot)
+    tokens = dim - rot
+    kind = torch.float32 if dtype == "f32" else torch.bfloat16
+    fine = [torch.from_numpy(rng.standard_normal((tokens, h, dim)).astype(np.float32)).to(kind).cuda() for h in (3, 2, 2)]
+    table, positions, at = torch.from_numpy(A.rope_table(tokens, rot)).cuda(), i32(range(tokens)), torch.arange(tokens, device="cuda")
+
+    def run(q, k, v):
+        out, keys, values = (torch.zeros(tokens, h, dim, dtype=torch.bfloat16, device="cuda") for h in (3, 2, 2))
+        torch.cuda.synchronize()
+        A.QkNormRope(backend.cuda_context, held(q), held(k), held(v), held(out), held(keys), held(values), held(positions), held(table), pairs=pairs).run()
+        backend.synchronize_device()
+        return out, keys
+
+    want = run(*fine)
+    for x in fine[:2]:
+        x[at, :, rot + at] = value
+    for got, ref in zip(run(*fine), want):
+        ref[at, :, rot + at] = value
+        assert torch.equal(torch.nan_to_num(got.float(), 12345.0), torch.nan_to_num(ref.float(), 12345.0))

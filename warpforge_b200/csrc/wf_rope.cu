@@ -63,7 +63,9 @@ __device__ __forceinline__ float2 fma_pair(float2 a, float2 b, float2 c) {
 // is settled outside, and four elements are two operations on pairs.  (With the kinds mixed, a head took 121 instructions a lane and the kernel was bound by
 // them: 27.9 us at the size above, 8.6 instead of 6.0 us at 777 tokens of 28 + 2 x 4 bf16 heads of 96.)
 constexpr int ROPE_WARPS = 4, ROPE_UNROLL = 4, ROPE_WARPS_PER_SM = 64, ROPE_MOST_BATCHES = 5;
-template <class X, bool VEC, int LANES, int DIM>  // DIM: 4 * LANES, or 0: less than that
+// DIM: 4 * LANES where all of the head is rotated or nothing, else 0.  The test whether a lane turns costs registers: in the kernel for whole heads 26.4 instead of
+// 24.7 us at the size above; with half of each head rotated that size takes 27.3.
+template <class X, bool VEC, int LANES, int DIM>
 __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __grid_constant__ RopeParams p) {
     constexpr int SIDE = 32 / LANES, HEADS = ROPE_UNROLL * SIDE;  // heads beside one another in a warp, heads of a batch
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
@@ -100,7 +102,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __g
         slot = -1;
         pos = 0;
     }
-    float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);  // cosine and sine of the lane's two pairs: 16 bytes of the row either way
+    float4 cs = make_float4(1.f, 0.f, 1.f, 0.f);  // cosine and sine of the lane's two pairs, if they turn: 16 bytes of the row either way
     if (turns) cs = *reinterpret_cast<const float4*>(p.rope + (size_t)pos * (p.rot / 2) + 2 * lane);
     const int64_t place = slot < 0 ? 0 : (int64_t)p.cache.at(slot >> p.cache.page_shift, 0, (int)(slot & ((1 << p.cache.page_shift) - 1)));
 #pragma unroll 1
@@ -134,7 +136,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __g
                 x[u][1] = mul_pair(mul_pair(x[u][1], make_float2(inv, inv)), gb);
             }
         }
-        if (kind < 2 && p.rot) {
+        if (kind < 2 && (DIM ? p.rot != 0 : turns)) {  // a lane that does not turn is left alone: 0 x Inf would make a NaN of its others
             const float2 c = make_float2(cs.x, cs.z), s = make_float2(cs.y, cs.w), minus = make_float2(-cs.y, -cs.w);
 #pragma unroll
             for (int u = 0; u < ROPE_UNROLL; u++) {
@@ -142,7 +144,7 @@ __global__ void __launch_bounds__(ROPE_WARPS * 32) qk_norm_rope_kernel(const __g
                 if (p.adjacent) {
                     x[u][0] = make_float2(a.x * cs.x - a.y * cs.y, a.y * cs.x + a.x * cs.y);
                     x[u][1] = make_float2(b.x * cs.z - b.y * cs.w, b.y * cs.z + b.x * cs.w);
-                } else {  // lanes that do not turn have cosine 1 and sine 0
+                } else {
                     x[u][0] = fma_pair(b, minus, mul_pair(a, c));
                     x[u][1] = fma_pair(a, s, mul_pair(b, c));
                 }
@@ -219,7 +221,8 @@ extern "C" int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* a, const
     const int64_t grid = (a->tokens * p.sets + ROPE_WARPS - 1) / ROPE_WARPS;
     if (grid > (1LL << 31) - 1) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens of %d heads", what, (long long)a->tokens, p.q_heads + 2 * p.k_heads);
     void (*kernel)(RopeParams);
-#define WF_ROPE_DIM(X, V) (d == 128 ? qk_norm_rope_kernel<X, V, 32, 128> : d == 64 ? qk_norm_rope_kernel<X, V, 16, 64> : side == 2 ? qk_norm_rope_kernel<X, V, 16, 0> : qk_norm_rope_kernel<X, V, 32, 0>)
+    const int whole = p.rot == 0 || p.rot == d ? d : 0;
+#define WF_ROPE_DIM(X, V) (whole == 128 ? qk_norm_rope_kernel<X, V, 32, 128> : whole == 64 ? qk_norm_rope_kernel<X, V, 16, 64> : side == 2 ? qk_norm_rope_kernel<X, V, 16, 0> : qk_norm_rope_kernel<X, V, 32, 0>)
     if (size == 4) kernel = vec ? WF_ROPE_DIM(float, true) : WF_ROPE_DIM(float, false);
     else kernel = vec ? WF_ROPE_DIM(bf16, true) : WF_ROPE_DIM(bf16, false);
 #undef WF_ROPE_DIM
