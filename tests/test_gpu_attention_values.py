@@ -125,3 +125,81 @@ def test_rope_an_element_that_is_not_rotated_stays_alone(backend, dim, rot, pair
     for got, ref in zip(run(*fine), want):
         ref[at, :, rot + at] = value
         assert torch.equal(torch.nan_to_num(got.float(), 12345.0), torch.nan_to_num(ref.float(), 12345.0))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("drafts", [1, 3, 12])
+def test_tree_bad_pages_in_short_units(backend, drafts, dim):  # noqa: F811
+    """Many short sequences a CTA, every third of which names a page outside the cache: its keys are not seen, the status says so, the others are as they were."""
+    import torch
+    from test_gpu_attention import check, formula, held, i32, normal
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(drafts + dim)
+    seqs, page, pages = 700, 16, 64
+    contexts = [int(n) for n in rng.integers(0, 40, seqs)]
+    tables = rng.integers(0, pages, (seqs, 4)).astype(np.int32)
+    gone = {s: int(rng.integers(0, -(-(contexts[s] + drafts) // page))) for s in range(0, seqs, 3)}
+    for s, i in gone.items():
+        tables[s, i] = (pages, -1, 2**31 - 1)[s % 9 // 3]
+    q, keys, values = normal(rng, seqs * drafts, 4, dim), normal(rng, pages, 1, page, dim), normal(rng, pages, 1, page, dim)
+    out, tab, ctx = torch.zeros_like(q), torch.from_numpy(tables).cuda(), i32(contexts)
+    torch.cuda.synchronize()
+    op = A.TreeAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), max_context=40, max_drafts=drafts)
+    first = None
+    for _ in range(10):
+        op.run()
+        with pytest.raises(N.WfError) as e:
+            backend.synchronize_device()
+        assert e.value.status == N.WF_ERR_INDEX
+        first = out.clone() if first is None else first
+        assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+    host = [x.double().cpu() for x in (q, keys, values)]
+    for s in list(range(0, 60)) + list(range(660, 700)):
+        total, rows = contexts[s] + drafts, slice(s * drafts, (s + 1) * drafts)
+        t = np.arange(total)
+        named = np.where((tables[s] < 0) | (tables[s] >= pages), 0, tables[s])[t // page]
+        k, v = (x[named, 0, t % page] for x in host[1:])
+        seen = torch.from_numpy((t[None, :] <= np.arange(drafts)[:, None] + contexts[s]) & (t[None, :] // page != gone.get(s, -1)))
+        check(out[rows, 3], *formula(host[0][rows, 3], k, v, dim**-0.5, seen))
+
+
+@pytest.mark.parametrize("dim", [64, 128])
+@pytest.mark.parametrize("heads", [1, 5])
+def test_prompt_bad_pages_beside_good_ones(backend, heads, dim):  # noqa: F811
+    """The same for prompts: rows before the page that is not there, and other sequences, do not depend on when it is found."""
+    import torch
+    from test_gpu_attention import check, formula, held, i32, normal, offsets
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(heads + dim)
+    seqs, page, pages = 150, 32, 40
+    lens = [int(n) for n in rng.integers(1, 500 // heads, seqs)]
+    tables = rng.integers(0, pages, (seqs, 16)).astype(np.int32)
+    gone = {s: int(rng.integers(0, -(-lens[s] // page))) for s in range(0, seqs, 3)}
+    for s, i in gone.items():
+        tables[s, i] = (pages, -1, 2**31 - 1)[s % 9 // 3]
+    n, starts = sum(lens), offsets(lens)
+    q, keys, values = normal(rng, n, heads, dim), normal(rng, pages, 1, page, dim), normal(rng, pages, 1, page, dim)
+    out, tab, off, k_lens = torch.zeros_like(q), torch.from_numpy(tables).cuda(), i32(starts), i32(lens)
+    torch.cuda.synchronize()
+    op = A.PromptAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(off), tables=held(tab), k_lens=held(k_lens))
+    first = None
+    for _ in range(10):
+        op.run()
+        with pytest.raises(N.WfError) as e:
+            backend.synchronize_device()
+        assert e.value.status == N.WF_ERR_INDEX
+        first = out.clone() if first is None else first
+        assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+    host = [x.double().cpu() for x in (q, keys, values)]
+    for s in range(12):
+        rows, t = slice(starts[s], starts[s + 1]), np.arange(lens[s])
+        named = np.where((tables[s] < 0) | (tables[s] >= pages), 0, tables[s])[t // page]
+        k, v = (x[named, 0, t % page] for x in host[1:])
+        seen = torch.from_numpy((t[None, :] <= t[:, None]) & (t[None, :] // page != gone.get(s, -1)))
+        check(out[rows, 0], *formula(host[0][rows, 0], k, v, dim**-0.5, seen))

@@ -131,7 +131,7 @@ __device__ __forceinline__ uint32_t pack_bf16(float lo, float hi) {
 __device__ __forceinline__ bool scores_too_large(float m, float scale) { return m > -INFINITY && fabsf(m * scale) >= 1048576.f; }
 
 // One row by one warp, key by key: lane l has elements 4 l .. 4 l + 3.  softmax(s) v = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m) with the
-// running maximum m; keys that are not seen are not read.
+// running maximum m; keys that are not seen are not read, but all pages are looked at.
 template <class Seen>
 __device__ __noinline__ void attend_row(const CacheView& c, const KeyPlace& place, const bf16* q, bf16* out, int head, int keys, float scale_log2, int* status,
                                         Seen seen) {
@@ -140,12 +140,12 @@ __device__ __noinline__ void attend_row(const CacheView& c, const KeyPlace& plac
     float qf[4] = {}, o[4] = {}, m = -INFINITY, l = 0.f;
     if (mine) load4(q + 4 * lane, qf);
     for (int t = 0; t < keys; t++) {
-        if (!seen(t)) continue;
         const int64_t page = place.page_of(c, t);
         if (page < 0 || page >= c.pages) {
             if (lane == 0) report_status(status, STATUS_BAD_INDEX);
             continue;
         }
+        if (!seen(t)) continue;
         const size_t at = c.at(page, head, t & ((1 << c.page_shift) - 1)) + 4 * lane;
         float k[4] = {}, v[4] = {};
         if (mine) {

@@ -201,7 +201,7 @@ struct PromptShared {
     uint64_t kv_full[PA_MAX_STAGES], kv_empty[PA_MAX_STAGES];
     uint64_t item_full[PA_ITEMS], item_empty[PA_ITEMS];
     PromptItem items[PA_ITEMS];
-    int bad_page;  // an item of this number and before has pages outside the cache
+    int bad_pages[2][2 * PA_ITEMS];  // group g's key tiles of an item (ItemCursor::mark) have pages outside the cache
     uint32_t tmem;
 };
 
@@ -226,6 +226,8 @@ struct ItemCursor {
         if (++slot == PA_ITEMS) slot = 0, phase ^= 1;
         return it.last == 0;
     }
+    // A place for what the load warp finds out about the item.  It is at most PA_ITEMS items ahead of the softmax warps: twice as many places are enough.
+    __device__ __forceinline__ int mark() const { return slot + PA_ITEMS * (int)phase; }
 };
 
 // Which items there are, the longest first: tiles of a sequence count from where its past ends, v = block + past / block tokens, and v goes down
@@ -379,7 +381,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             g_mbar_init(&sh->item_full[i], 1);
             g_mbar_init(&sh->item_empty[i], PA_SOFTMAX_WARPS + 2);
         }
-        sh->bad_page = -1;
+        for (int i = 0; i < 2 * PA_ITEMS; i++) sh->bad_pages[0][i] = sh->bad_pages[1][i] = 0;
         asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
         prefetch_tensormap(&q_map);
         prefetch_tensormap(&k_map);
@@ -405,7 +407,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         const int my_token = r / group, my_head = r % group;
         const float scale = p.scale_log2;
         uint32_t s_phase = 0, o_phase[2] = {0, 0}, half_phase = 0;
-        for (int number = 0; items.next(sh, it, failed); number++) {
+        while (items.next(sh, it, failed)) {
             const int n = it.tiles(g), step = it.split ? 2 : 1;
             const int first = it.token0 + (it.split ? 0 : g * tile_tokens), token = first + my_token;
             const bool mine = r < group * tile_tokens && token < it.rows;
@@ -528,7 +530,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 }
                 tc_fence_after();
             }
-            if (TREE && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l = __uint_as_float(0x7FC00000u);
+            if (TREE && *reinterpret_cast<volatile int*>(&sh->bad_pages[g][items.mark()])) l = __uint_as_float(0x7FC00000u);
             float keep = 1.f, take = 0.f, top = m;
             if (halves) {  // both groups add both up, half of the columns each
                 sh->half_max[g][r] = m;
@@ -617,7 +619,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             }
             // Rows with an Inf or a NaN in their sums, and rows whose pages are not in the cache, go key by key: the first may have
             // come from a key that the row does not see (0 x Inf), the second's keys were not read.
-            if (!TREE) odd |= !(it.split && g) && *reinterpret_cast<volatile int*>(&sh->bad_page) >= number;
+            if (!TREE) odd |= !(it.split && g) && *reinterpret_cast<volatile int*>(&sh->bad_pages[g][items.mark()]);
             uint32_t again = __ballot_sync(0xFFFFFFFFu, mine && odd);
             while (again) {
                 const int l2 = __ffs(again) - 1;
@@ -639,7 +641,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         StageCursor ring;
         uint32_t q_phase[2] = {1, 1};
         const int boxes = PA_KEYS / t.box_rows;
-        for (int number = 0; items.next(sh, it, failed); number++) {
+        while (items.next(sh, it, failed)) {
             const int n = it.all();
             const int* table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
             // the rows of a key tile's boxes, a lane each, and how many there are
@@ -654,9 +656,11 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 if (valid && key < it.keys) page = table[key >> p.cache.page_shift];
                 if (page < 0 || page >= p.cache.pages) {  // never followed: these rows go key by key
                     report_status(p.status, STATUS_BAD_INDEX);
-                    *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                    for (int g = 0; g < 2; g++)
+                        if (it.split || j < (g ? it.n1 : it.n0)) *reinterpret_cast<volatile int*>(&sh->bad_pages[g][items.mark()]) = 1;
                     page = 0;
                 }
+                __syncwarp();  // the mark is there before a tile that this warp loads
                 z = (int)((((int64_t)page * p.cache.kv_heads + it.head) << p.cache.page_shift) + (key & ((1 << p.cache.page_shift) - 1)));
                 return __popc(__ballot_sync(0xFFFFFFFFu, valid));
             };
@@ -698,6 +702,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             }
             if (n > 0 && !failed) load(&v_map, z_before, loads_before);
             if (failed) break;
+            if (lane < 2) *reinterpret_cast<volatile int*>(&sh->bad_pages[lane][(items.mark() + 1) % (2 * PA_ITEMS)]) = 0;  // the next item's
+            __syncwarp();
         }
     } else if (warp == PA_MMA_WARP) {
         // Everything here is laid out for the pace of the issuing thread: the group is a constant in every place (as a variable the kernel lost 10 %).

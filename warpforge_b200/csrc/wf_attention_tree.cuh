@@ -95,7 +95,9 @@ template <int CHUNKS, int MT> struct TreeShared {
     TreeSegment segments[TA_SEGMENTS];
     float warp_max[Shape::SETS][Shape::ROWS], warp_sums[Shape::SETS][Shape::ROWS];
     unsigned long long odd_rows;
-    int bad_page;  // the segment of this number and those before it have pages outside the cache
+    // [number % ..] = number: the segment of that number has pages outside the cache; nobody is more than TA_SEGMENTS ahead of another
+    int bad_pages[2 * TA_SEGMENTS];
+    __device__ __forceinline__ volatile int& bad_page(int number) { return *reinterpret_cast<volatile int*>(&bad_pages[(unsigned)number % (2 * TA_SEGMENTS)]); }
 };
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
@@ -143,9 +145,10 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
                 page = tile < u.to && keys > 0 ? table[tile * TA_KEYS >> p.cache.page_shift] : 0;
             }
             if (page < 0 || page >= p.cache.pages) {  // never followed: the unit's rows go key by key
-                *reinterpret_cast<volatile int*>(&sh->bad_page) = number;
+                sh->bad_page(number) = number;
                 page = 0;
             }
+            __syncwarp();  // the mark is there before a tile that this warp has loaded
             const int z = ((page * heads + u.head) << p.cache.page_shift) + (tile * TA_KEYS & ((1 << p.cache.page_shift) - 1));  // below 2^31: check_cache
             const int n = min(32, u.to - t0);
 #pragma unroll 1
@@ -196,7 +199,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         g_mbar_init(&sh->seg_empty[tid - 32], TA_WARPS);
     } else if (tid == 64) {
         sh->odd_rows = 0;
-        sh->bad_page = -1;
+        for (int i = 0; i < 2 * TA_SEGMENTS; i++) sh->bad_pages[i] = -1;
         prefetch_tensormap(&k_map);
         prefetch_tensormap(&v_map);
     }
@@ -357,7 +360,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         __syncwarp();
         if (lane == 0) g_mbar_arrive(&sh->seg_empty[seg]);  // the queries
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
-        if (*reinterpret_cast<volatile int*>(&sh->bad_page) >= number) l[0][0] = l[0][1] = l[MT - 1][0] = l[MT - 1][1] = __uint_as_float(0x7FC00000u);
+        if (sh->bad_page(number) == number) l[0][0] = l[0][1] = l[MT - 1][0] = l[MT - 1][1] = __uint_as_float(0x7FC00000u);
 
         // The warps' sums together.  Where they do not all fit shared memory the upper half hands its to the lower half first.
         auto write_sums = [&](int set) {
