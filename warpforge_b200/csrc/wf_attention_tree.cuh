@@ -168,9 +168,9 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
         return true;
     });
+    if (t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
     if (!ok || !__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
     if (loader == 0 && lane == 0) {
-        if (t.c.may_cut && !cut) t.c.cuts[blockIdx.x].first_cta = -1;
         sh->segments[seg].last = 1;
         g_mbar_arrive(&sh->seg_full[seg]);
     }
