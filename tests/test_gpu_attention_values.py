@@ -203,3 +203,43 @@ def test_prompt_bad_pages_beside_good_ones(backend, heads, dim):  # noqa: F811
         k, v = (x[named, 0, t % page] for x in host[1:])
         seen = torch.from_numpy((t[None, :] <= t[:, None]) & (t[None, :] // page != gone.get(s, -1)))
         check(out[rows, 0], *formula(host[0][rows, 0], k, v, dim**-0.5, seen))
+
+
+def test_prompt_pasts_of_very_different_lengths(backend):  # noqa: F811
+    """Some with none beside some with much, more sequences than a warp has lanes; two or one tile of rows an item."""
+    rng = np.random.default_rng(21)
+    for q_heads, seqs in ((8, 70), (64, 40), (128, 5)):
+        past = [int(n) if i % 7 == 3 else 0 for i, n in enumerate(rng.integers(2000, 6000, seqs))]
+        run_prompt(backend, [int(n) for n in rng.integers(0, 9, seqs)], q_heads, 1, 64, 64, past)
+
+
+def test_prompt_time_does_not_grow_with_the_distance_of_pasts(backend):  # noqa: F811
+    """One token behind 60,000 others, beside 40 short prompts, with 128 query heads for the kv head, so that an item has two tokens: 30,000 places between the
+    first item and the others.  The token's 469 key tiles are one CTA's work, 1000 to 1700 cycles each with one or two groups of warps at them: below 1 ms, with the prompts
+beside it or without; twice that is allowed."""
+    import torch
+    from test_gpu_attention import held, i32, normal, offsets
+
+    from warpforge_b200 import attention as A
+
+    rng, ctx, page = np.random.default_rng(22), backend.cuda_context, 64
+    keys, values = normal(rng, 1024, 1, page, 64), normal(rng, 1024, 1, page, 64)
+    start, stop = ctx.create_event(), ctx.create_event()
+
+    def took(lens, past):
+        q = normal(rng, sum(lens), 128, 64)
+        out, tables = torch.zeros_like(q), torch.from_numpy(rng.integers(0, 1024, (len(lens), 1024)).astype(np.int32)).cuda()
+        off, k_lens = i32(offsets(lens)), i32([a + b for a, b in zip(lens, past)])
+        torch.cuda.synchronize()
+        op = A.PromptAttention(ctx, held(q), held(keys), held(values), held(out), held(off), tables=held(tables), k_lens=held(k_lens))
+        times = []
+        for _ in range(5):
+            ctx.record_event(start)
+            op.run()
+            ctx.record_event(stop)
+            backend.synchronize_device()
+            times.append(ctx.elapsed_ms(start, stop))
+        return min(times)
+
+    alone, both = took([1], [60000]), took([1] + [5] * 40, [60000] + [0] * 40)
+    assert alone <= 2.0 and both <= 2.0, (alone, both)
