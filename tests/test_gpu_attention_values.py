@@ -243,3 +243,21 @@ beside it or without; twice that is allowed."""
 
     alone, both = took([1], [60000]), took([1] + [5] * 40, [60000] + [0] * 40)
     assert alone <= 2.0 and both <= 2.0, (alone, both)
+
+
+def test_what_the_error_says(backend):  # noqa: F811
+    """A page outside the cache is not reported as an embedding's index."""
+    import torch
+    from test_gpu_attention import held, i32, normal
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(1)
+    q, pages = normal(rng, 1, 1, 64), normal(rng, 2, 1, 16, 64)
+    tables, context, out = i32([[2]]), i32([3]), torch.zeros(1, 1, 64, dtype=torch.bfloat16, device="cuda")
+    torch.cuda.synchronize()
+    A.TreeAttention(backend.cuda_context, held(q), held(pages), held(pages), held(out), held(tables), held(context), max_context=3).run()
+    with pytest.raises(N.WfError, match="a page") as e:
+        backend.synchronize_device()
+    assert e.value.status == N.WF_ERR_INDEX

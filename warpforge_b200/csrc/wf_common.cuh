@@ -22,7 +22,7 @@ constexpr uint32_t COMM_MAGIC = 0x5746434D;    // "WFCM"
 constexpr int STATUS_GEMV_FIXUP_TIMEOUT = 1;
 constexpr int STATUS_GEMM_PIPE_TIMEOUT = 2;
 constexpr int STATUS_PEER_WAIT_TIMEOUT = 4;
-constexpr int STATUS_BAD_INDEX = 8;  // an embedding index outside the table
+constexpr int STATUS_BAD_INDEX = 8;  // an index outside its range: an embedding row, a page, slot, position or length
 
 __device__ __forceinline__ uint32_t map_to_rank(uint32_t saddr, uint32_t rank) {
     uint32_t r;

@@ -464,7 +464,7 @@ int read_device_status(Context* c) {
     if (st != 0) {
         for (int b = 0; b < STATUS_BITS; b++) c->h_status[b] = 0;
         WF_CUDA(c, cudaMemset(c->d_status, 0, sizeof(int)));
-        if (st == STATUS_BAD_INDEX) return set_error(c, WF_ERR_INDEX, "an embedding index was outside the table (its row was written as zeros)");
+        if (st == STATUS_BAD_INDEX) return set_error(c, WF_ERR_INDEX, "an index on the device was outside its range: an embedding row, a page, slot, position or length (what it names was skipped, or written as zeros)");
         return set_error(c, WF_ERR_DEVICE_WAIT, "a device-side bounded wait expired (status bits 0x%x)", st);
     }
     return WF_OK;
