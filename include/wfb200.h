@@ -299,7 +299,8 @@ int wf_qk_norm_rope(int64_t ctx, const wf_qk_norm_rope_args* args, const wf_kv_c
  *   cache            with page_tokens == 1: packed keys and values, sequence s has the same rows of them as of q (tables_dev and k_lens_dev
  *                    are 0); else pages by tables_dev int32 [seqs][table_stride] and k_lens_dev int32 [seqs]
  * Products are bf16, scores, sums and the running maximum fp32; the weights exp(score - m) are rounded to bf16 for the second
- * product.  A key that a row does not see has no influence on it, whatever it and its value hold (Inf and NaN too). */
+ * product.  A key that a row does not see has no influence on it, whatever it and its value hold (Inf and NaN too); a score of NaN or of plus
+ * infinity that it does see makes it NaN. */
 typedef struct wf_prompt_attention_args {
     int64_t q_dev, out_dev;
     int64_t q_stride;

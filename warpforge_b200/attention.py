@@ -3,7 +3,8 @@
     QkNormRope       q, k, v of the projections: norms of q and k per head, rotation by position, rounding to bf16; k and v go into the cache
     PromptAttention  causal attention over whole prompts, packed one behind the other
     TreeAttention    attention of a decoded token, or of a chain or tree of drafted ones, over each sequence's cache
-    KvCache          pages of keys and values: sequences that grow, fork, are cut back and freed; drafts that are kept move up
+    KvCache          pages of keys and values: sequences that grow, fork, are cut back and freed; drafts that are kept move up.  Forks share pages until
+                     one of them is to write there
 
 The first three bind their buffers once (shapes and types are checked then) and are run once per step: ``op.run(stream)`` is one native
 call that only enqueues.  Lengths, tables and masks are device arrays read when the kernel runs, so a recorded step

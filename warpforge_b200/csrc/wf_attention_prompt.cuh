@@ -8,10 +8,12 @@
 // tile's exponentials are taken; where there is one tile of rows, on every other tile of keys of it in turn.  The rows of a tile are the heads of the group for some tokens, token by
 // token: keys and values are read once for the whole group.  A thread of the softmax warps has a row: its maximum and sum need no exchange.
 //
-// Bound by the softmax warps' instructions beside the tensor cores' products: a pair of tiles takes about 3300 cycles, 2048 of them products at dim 128 and 1024 at dim 64.  8192
-// tokens, 32 / 8 heads of 128: 434 us in a burst (1.27 PFLOP/s of the products that the mask leaves, 0.77 of the measured rate), 502 over seconds under the power limit; of 64: 372 us.
+// Bound by a chain: weights lie where the scores lay, so a group's next scores wait for its products, those for its exponentials, and a tile of keys is load of the scores, maxima,
+// exponentials, stores, products, scores one after the other, with the other group's beside it.  A pair of tiles takes about 3300 cycles at dim 128 (2048 of products; tensor
+// pipe 63 % busy, issue slots 52 %, special functions 40 %) and 3200 at dim 64 (1024; 33 %, 54 %, 42 %).  8192 tokens, 32 / 8 heads of 128: 440 us in a burst (1.25 PFLOP/s of
+// the products that the mask leaves, 0.76 of the measured rate), 505 to 515 over seconds under the power limit; of 64: 386 us in a burst.
 // 512 tokens, 32 / 32 heads: 12.2 us, a launch, 2 us until the first item is known (code and arguments come from memory), two pairs of tiles and the rows' way out.  Two threads a row
-// (16 softmax warps): 604 us where this takes 521.
+// (16 softmax warps): 604 us, where one took 521 at the time.
 #pragma once
 #include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
@@ -230,7 +232,8 @@ struct ItemCursor {
     __device__ __forceinline__ int mark() const { return slot + PA_ITEMS * (int)phase; }
 };
 
-// Which items there are, the longest first: tiles of a sequence count from where its past ends, v = block + past / block tokens, and v goes down
+// Which items there are, the longest first (a CTA's numbers are taken up to four items ahead, so the order evens out calls with many items a CTA, not those with
+// three): tiles of a sequence count from where its past ends, v = block + past / block tokens, and v goes down
 // over all sequences at once.  Every lane has every 32nd sequence.
 struct PromptSchedule {
     const PromptTiles& t;

@@ -3,7 +3,7 @@
 // Bound by HBM: every key and value is read once, 4 dim bytes for 4 dim flops a row.  The rows of a sequence and kv head (its new tokens times the
 // heads of the group) are padded to 16 or 32 and multiplied by mma.sync, 16 keys at a time; a tile of 5th-generation tensor cores has 128 rows, of which
 // one decoded token fills one to eight.  More than 32 rows go to the kernel of wf_attention_prompt.cuh.  (One token of 48 sequences of 31 to 4000 tokens, 64 / 8 heads of
-// 128: 419 MB in 73 us, 5.7 TB/s, 0.88 of a copy's rate.  One of 32 / 32 heads at 512 tokens: 9.2 us, of which 3.5 are a launch and the rest one SM's walk through 33 tiles.)
+// 128: 419 MB in 73 us, 5.7 TB/s, 0.88 of a copy's rate.  One of 32 / 32 heads at 512 tokens: 9.3 us, of which 3.5 are a launch and the rest one SM's walk through 33 tiles.)
 //
 // The units are cut as wf_attention_line.cuh says.  Inside a CTA four warps walk its share and have TMA fill a ring of tiles ahead, across the ends of
 // units too; eight others take the tiles of a piece in turn.
