@@ -345,6 +345,49 @@ int wf_cache_copy_pages(int64_t ctx, const wf_kv_cache* cache, int64_t pairs_dev
 int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, int64_t table_stride, int64_t context_dev, int64_t kept_dev,
                      int64_t kept_stride, int64_t counts_dev, int64_t seqs, int64_t stream);
 
+/* ---- attention that reads less than every key of every sequence --------------------------
+ * Pages that a token reads, chosen by what their keys promise (wf_page_bounds, wf_select_pages, wf_selected_attention), and keys that sequences have in
+ * common read once for all of them (wf_shared_prefix_attention).  (No counterpart in the reference, which has no cache.)
+ *
+ * wf_page_bounds: of every page that holds one of the tokens first[s] .. stop[s] - 1 of a sequence, in every layer and head, the bounds of the keys of its tokens below
+ * stop[s]:  codes = ceil(max_t k[t][d] / scale), floor(min_t k[t][d] / scale), scale the least power of two for which all are -127 .. 127 (2^-60 at least).  A page with an Inf
+ * or a NaN among its keys has the scale +Inf and codes 0.
+ *   codes_dev   int8 [layers][pages][kv_heads][2][head_dim], 16-byte aligned: upper bounds, lower bounds
+ *   scales_dev  fp32 [layers][pages][kv_heads]
+ *   tables_dev  int32 [seqs][table_stride]; first_dev, stop_dev int32 [seqs]
+ *   max_tokens  most tokens stop[s] - first[s] of a sequence; a longer range is WF_ERR_INDEX and left out
+ * Sequences that share a page should agree on how many of its tokens count: else the bounds are one or the other's. */
+int wf_page_bounds(int64_t ctx, const wf_kv_cache* cache, int64_t codes_dev, int64_t scales_dev, int64_t tables_dev, int64_t table_stride, int64_t first_dev, int64_t stop_dev,
+                   int64_t seqs, int64_t max_tokens, int64_t stream);
+
+/* For every new token and kv head the pages that it reads, at most `width` of them, in ascending order: the first `first` pages of its sequence, all from that of token
+ * context - recent on (those of the new tokens among them), and of those between the ones with the largest scores, as many as there is room for; of equal ones the earliest.
+ *     score = scale max over the heads of the group of f sum_d q_d (q_d > 0 ? hi_d : lo_d)     q rounded to whole numbers -127 .. 127 times f, the least power of two that allows it
+ * which is exact (whole numbers below 2^21 times a power of two).  A page with the scale +Inf comes before all others; a head with an Inf or a NaN among its elements scores 0
+ * everywhere.  Pages between have to be full, and their bounds up to date.
+ *   q_dev          bf16 [tokens][q_heads][head_dim], q_stride elements (a multiple of 8) from one token to the next, 16-byte aligned
+ *   codes_dev, scales_dev  those of wf_page_bounds for one layer: [pages][kv_heads][2][head_dim], [pages][kv_heads]
+ *   q_offsets_dev, tables_dev, context_dev, max_drafts, max_context   as in wf_tree_attention
+ *   pages_out_dev  int32 [tokens][kv_heads][width]: page numbers, -1 behind a list's end
+ *   lens_out_dev   int32 [tokens][kv_heads][2]: tokens of the context in the list; keys in all, which is as many new tokens more as the token may see: those up to itself, or
+ *                  with WF_SELECT_TREE all of its sequence (wf_selected_attention's ancestors say which).  New token j lies at place lens[0] + j of the list.
+ * A sequence whose context cannot be has empty lists, {0, 0}.  width must have room for the pages that are taken in any case; contexts of at most
+ * WF_SELECT_MAX_PAGES pages. */
+#define WF_SELECT_TREE 1
+#define WF_SELECT_MAX_PAGES 49152
+typedef struct wf_select_pages_args {
+    int64_t q_dev, q_stride;
+    int64_t codes_dev, scales_dev;
+    int64_t q_offsets_dev;
+    int64_t tables_dev, table_stride;
+    int64_t context_dev;
+    int64_t pages_out_dev, lens_out_dev;
+    int64_t tokens, max_context, pages;
+    int32_t seqs, q_heads, kv_heads, head_dim, page_tokens, max_drafts;
+    int32_t width, first, recent, flags;
+} wf_select_pages_args;
+int wf_select_pages(int64_t ctx, const wf_select_pages_args* args, int64_t stream);
+
 /* Who holds which page: a count of holders per page, in host memory.  Process-wide handles that need no device, any thread may call.
  * wf_pages_take: n free pages, each with one holder, lowest numbers first; all or none (WF_ERR_TOO_LARGE).  wf_pages_share: one
  * holder more for each (a fork reads the pages of what it was forked from).  wf_pages_release: one fewer; a page without holders

@@ -41,6 +41,12 @@ class TreeAttentionArgs(ctypes.Structure):  # wf_tree_attention_args
                                      "max_context")] + [("seqs", ctypes.c_int32), ("q_heads", ctypes.c_int32), ("max_drafts", ctypes.c_int32), ("scale", c_f32)]
 
 
+class SelectPagesArgs(ctypes.Structure):  # wf_select_pages_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "q_stride", "codes_dev", "scales_dev", "q_offsets_dev", "tables_dev", "table_stride", "context_dev", "pages_out_dev", "lens_out_dev",
+                                     "tokens", "max_context", "pages")] + [
+        (n, ctypes.c_int32) for n in ("seqs", "q_heads", "kv_heads", "head_dim", "page_tokens", "max_drafts", "width", "first", "recent", "flags")]
+
+
 c_i32 = ctypes.c_int32
 
 # name -> (restype, argtypes); must list every function declared in include/wfb200.h
@@ -89,6 +95,8 @@ SIGNATURES = {
     "wf_tree_attention": (c_int, [c_i64, P(TreeAttentionArgs), P(KvCacheArgs), c_int, c_i64]),
     "wf_cache_copy_pages": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64]),
     "wf_cache_compact": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "wf_page_bounds": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
+    "wf_select_pages": (c_int, [c_i64, P(SelectPagesArgs), c_i64]),
     "wf_pages_create": (c_int, [c_i64, P(c_i64)]),
     "wf_pages_destroy": (c_int, [c_i64]),
     "wf_pages_take": (c_int, [c_i64, c_i64, P(c_i32)]),
@@ -140,6 +148,7 @@ WF_Q4_0_ORDER_REFERENCE, WF_Q4_0_ORDER_GGML = 0, 1
 WF_DTYPE_F32, WF_DTYPE_BF16 = 0, 1
 WF_OP_NEW_X, WF_OP_DEPENDS = 1, 2
 WF_QK_NORM, WF_ROPE_ADJACENT = 1, 2
+WF_SELECT_TREE, WF_SELECT_MAX_PAGES = 1, 49152
 
 
 class NativeLibraryMissing(RuntimeError):

@@ -6,7 +6,12 @@
     KvCache          pages of keys and values: sequences that grow, fork, are cut back and freed; drafts that are kept move up.  Forks share pages until
                      one of them is to write there
 
-The first three bind their buffers once (shapes and types are checked then) and are run once per step: ``op.run(stream)`` is one native
+and, where reading every key of every sequence for each token takes too long,
+
+    PageBounds       the largest and smallest elements of the keys of every page, in 8 bits
+    SelectPages      the pages that a new token reads, by the scores that their bounds promise
+
+The operators bind their buffers once (shapes and types are checked then) and are run once per step: ``op.run(stream)`` is one native
 call that only enqueues.  Lengths, tables and masks are device arrays read when the kernel runs, so a recorded step
 (``CudaContext.graph_begin``) serves a growing cache.  All tensors are ``DeviceTensor``; the arithmetic is described in include/wfb200.h.
 """
@@ -73,13 +78,13 @@ def _cache_args(keys: DeviceTensor, values: DeviceTensor, layers: int = 1) -> N.
 class _Bound:
     """An operator with its buffers; they are kept alive with it."""
 
-    def __init__(self, context: CudaContext, function: str, args, cache: N.KvCacheArgs, layer: int, tensors):
+    def __init__(self, context: CudaContext, function: str, args, cache: Optional[N.KvCacheArgs], layer: int, tensors):
         self.context, self.args, self.cache, self.layer, self._tensors = context, args, cache, layer, tensors
         self._name, self._fn = function, getattr(context._lib, function)
-        self._args, self._cache = ctypes.byref(args), ctypes.byref(cache)
+        self._bound = (ctypes.byref(args),) if cache is None else (ctypes.byref(args), ctypes.byref(cache), layer)
 
     def run(self, stream: int = 0) -> None:
-        rc = self._fn(self.context.handle, self._args, self._cache, self.layer, stream)
+        rc = self._fn(self.context.handle, *self._bound, stream)
         if rc:
             self.context._ck(self._name, rc)
 
@@ -191,6 +196,28 @@ class Sequence:
 
     def free(self) -> None:
         self.truncate(0)
+
+
+class SelectPages(_Bound):
+    """The pages that new tokens read.  q bf16 [tokens, q_heads, dim]; codes i8 [pages, kv_heads, 2, dim] and scales f32 [pages, kv_heads] of one layer (``PageBounds.layer``);
+    tables, context_lens, q_offsets and the bounds max_context and max_drafts as in TreeAttention.  pages_out i32 [tokens, kv_heads, width]: for each token and kv head the first `first`
+    pages, those from token context - recent on, and of the others the ones that promise the largest scores, ascending, -1 behind them; lens_out i32 [tokens, kv_heads, 2]: tokens of
+    the context in the list, keys in all.  tree: a token's list counts all new tokens of its sequence (SelectedAttention is given the ancestors), else those up to itself."""
+
+    def __init__(self, context: CudaContext, q, codes, scales, tables, context_lens, pages_out, lens_out, *, page_tokens: int, max_context: int, first: int = 1, recent: int = 64,
+                 q_offsets=None, max_drafts: int = 1, tree: bool = False):
+        tokens, heads, dim = q.shape()
+        seqs, (pages, kv_heads) = context_lens.shape()[0], codes.shape()[:2]
+        a = N.SelectPagesArgs(tokens=tokens, q_heads=heads, seqs=seqs, max_drafts=max_drafts, max_context=max_context, pages=pages, kv_heads=kv_heads, head_dim=dim, page_tokens=page_tokens,
+                              first=first, recent=recent, width=pages_out.shape()[2], flags=N.WF_SELECT_TREE if tree else 0)
+        a.q_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _stride(q)
+        a.codes_dev, a.scales_dev = _typed("codes", codes, "i8", pages, kv_heads, 2, dim), _typed("scales", scales, "f32", pages, kv_heads)
+        a.q_offsets_dev = _typed("q_offsets", q_offsets, "i32", seqs + 1)
+        a.tables_dev, a.table_stride = _typed("tables", tables, "i32", seqs, None), tables.shape()[1]
+        a.context_dev = _typed("context_lens", context_lens, "i32", seqs)
+        a.pages_out_dev = _typed("pages_out", pages_out, "i32", tokens, kv_heads, None)
+        a.lens_out_dev = _typed("lens_out", lens_out, "i32", tokens, kv_heads, 2)
+        super().__init__(context, "wf_select_pages", a, None, 0, (q, codes, scales, tables, context_lens, pages_out, lens_out, q_offsets))
 
 
 class KvCache:
@@ -373,3 +400,46 @@ class KvCache:
                 if self.context.handle:
                     self.context.free(p)
             self._owned, self._fork_arrays = [], {}
+
+
+class PageBounds:
+    """What SelectPages knows of the keys of a cache: codes i8 [layers, pages, kv_heads, 2, head_dim] (the largest and the smallest element, times a power of two, rounded up and down) and
+    scales f32 [layers, pages, kv_heads], allocated here or given."""
+
+    def __init__(self, cache: KvCache, codes: Optional[DeviceTensor] = None, scales: Optional[DeviceTensor] = None):
+        if (codes is None) != (scales is None):
+            raise ValueError("codes and scales, or neither")
+        self.cache, self._owned = cache, []
+        shape = (cache.layers, cache.page_count, cache.kv_heads)
+        ctx = cache.context
+        try:
+            if codes is None:
+                for n in (2 * cache.head_dim, 4):
+                    self._owned.append(ctx.allocate(int(np.prod(shape)) * n))
+                codes, scales = DeviceTensor(self._owned[0], (*shape, 2, cache.head_dim), "i8", owner=ctx), DeviceTensor(self._owned[1], shape, "f32", owner=ctx)
+            self._addresses = _typed("codes", codes, "i8", *shape, 2, cache.head_dim), _typed("scales", scales, "f32", *shape)
+        except BaseException:
+            self.close()
+            raise
+        self.codes, self.scales = codes, scales
+
+    def update(self, tables: DeviceTensor, first: DeviceTensor, stop: DeviceTensor, *, max_tokens: int, stream: int = 0) -> None:
+        """In every layer, after tokens first[s] .. stop[s] - 1 (i32 [seqs]) of the sequences have been stored: the bounds of the pages that hold them.  max_tokens: most
+        tokens of a sequence."""
+        seqs, ctx = first.shape()[0], self.cache.context
+        ctx._ck("wf_page_bounds", ctx._lib.wf_page_bounds(
+            ctx.handle, self.cache._ref, *self._addresses, _typed("tables", tables, "i32", seqs, None), tables.shape()[1], _typed("first", first, "i32", seqs),
+            _typed("stop", stop, "i32", seqs), seqs, max_tokens, stream))
+
+    def layer(self, i: int):
+        """codes and scales of one layer."""
+        if not 0 <= i < self.cache.layers:
+            raise ValueError(f"layer {i} of {self.cache.layers}")
+        of = lambda t, size: DeviceTensor(t.ptr + i * int(np.prod(t.shape()[1:])) * size, t.shape()[1:], t.dtype, owner=t)  # noqa: E731
+        return of(self.codes, 1), of(self.scales, 4)
+
+    def close(self) -> None:
+        owned, self._owned = self._owned, []
+        for p in owned:
+            if self.cache.context.handle:
+                self.cache.context.free(p)
