@@ -388,6 +388,45 @@ typedef struct wf_select_pages_args {
 } wf_select_pages_args;
 int wf_select_pages(int64_t ctx, const wf_select_pages_args* args, int64_t stream);
 
+/* Attention of new tokens over lists of pages, one for each token and kv head.
+ *   q_dev, out_dev  as in wf_tree_attention
+ *   pages_dev, lens_dev  as wf_select_pages leaves them: int32 [tokens][kv_heads][width], int32 [tokens][kv_heads][2] (8-byte aligned).  Key t of a list lies in row t % page_tokens of page
+ *                   pages[t / page_tokens]; a token sees the first lens[0] keys, and of the lens[1] - lens[0] behind them (64 at most) those of its ancestors
+ *   ancestors_dev   uint64 [tokens]; 0 (no array) = all of them
+ * A list may name pages in any order, and one twice.  {0, 0} is an empty list, its rows are zeros; lengths that cannot be are WF_ERR_INDEX and rows of zeros. */
+typedef struct wf_selected_attention_args {
+    int64_t q_dev, out_dev;
+    int64_t q_stride;
+    int64_t pages_dev, lens_dev;
+    int64_t ancestors_dev;
+    int64_t tokens;
+    int32_t q_heads, width;
+    float scale;
+} wf_selected_attention_args;
+int wf_selected_attention(int64_t ctx, const wf_selected_attention_args* args, const wf_kv_cache* cache, int layer, int64_t stream);
+
+/* wf_tree_attention where sequences begin with the same tokens: sequences groups[g] .. groups[g + 1] - 1 have the first prefix[g] tokens in common, a multiple of page_tokens
+ * and not more than the context of any of them, in the same pages.  They are read once for all rows of the group, from the pages in the table of its first sequence.  The rest of the
+ * arguments are wf_tree_attention's.
+ *   groups_dev   int32 [n_groups + 1], ascending from 0 to seqs; prefix_dev int32 [n_groups], 0 = nothing in common
+ *   max_prefix   most tokens of a prefix; max_own: most context[s] - prefix of a sequence
+ * A group whose prefix or sequences cannot be, and a sequence with a context shorter than the prefix, are WF_ERR_INDEX and rows of zeros.  At most WF_SHARED_MAX_TOKENS
+ * tokens. */
+#define WF_SHARED_MAX_TOKENS 131072
+typedef struct wf_shared_prefix_attention_args {
+    int64_t q_dev, out_dev;
+    int64_t q_stride;
+    int64_t q_offsets_dev;
+    int64_t tables_dev, table_stride;
+    int64_t context_dev;
+    int64_t ancestors_dev;
+    int64_t groups_dev, prefix_dev;
+    int64_t tokens, max_prefix, max_own;
+    int32_t seqs, q_heads, max_drafts, n_groups;
+    float scale;
+} wf_shared_prefix_attention_args;
+int wf_shared_prefix_attention(int64_t ctx, const wf_shared_prefix_attention_args* args, const wf_kv_cache* cache, int layer, int64_t stream);
+
 /* Who holds which page: a count of holders per page, in host memory.  Process-wide handles that need no device, any thread may call.
  * wf_pages_take: n free pages, each with one holder, lowest numbers first; all or none (WF_ERR_TOO_LARGE).  wf_pages_share: one
  * holder more for each (a fork reads the pages of what it was forked from).  wf_pages_release: one fewer; a page without holders

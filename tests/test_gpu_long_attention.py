@@ -1,0 +1,501 @@
+"""Attention over lists of pages and attention of sequences that share a prefix, against the formula in 64 bits.  Tolerances as in test_gpu_attention.py: outputs are
+bf16 (2^-8 of a value at most), weights are rounded to bf16 before the second product (2^-8 of sum p |v|), scores are fp32; that sums come in parts which are
+joined in fp32 adds some 2^-22 of a value."""
+import math
+
+import numpy as np
+import pytest
+
+from test_gpu_attention import backend, check, formula, held, i32, normal, offsets, pages_for, tree_words  # noqa: F401
+
+pytestmark = pytest.mark.gpu
+
+
+def signed(words):
+    import torch
+
+    return torch.tensor([w - (1 << 64) if w >> 63 else w for w in words], dtype=torch.int64, device="cuda")
+
+
+def same_bits(op, out, backend, times=2):
+    import torch
+
+    first = out.clone()
+    for _ in range(times):
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        op.run()
+        backend.synchronize_device()
+        assert torch.equal(out.view(torch.int16), first.view(torch.int16))
+
+
+# ------------------------------------------------------------------------------------------------ lists
+def run_selected(backend, held_lens, news, q_heads, kv_heads, dim, page, width=None, words=None, seed=0, edit=None, pages=None, q_apart=0, heads=None):
+    """held_lens[t], news[t] of every token, the same for all kv heads but one page of the context less for odd ones."""
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(seed)
+    n = len(held_lens)
+    lens = np.zeros((n, kv_heads, 2), np.int32)
+    for t in range(n):
+        for h in range(kv_heads):
+            lens[t, h, 0] = max(0, held_lens[t] - (page if h & 1 else 0))
+            lens[t, h, 1] = lens[t, h, 0] + news[t]
+    width = width or max(1, -(-int(lens.max()) // page))
+    pages = pages or 3 * width + 5
+    lists = np.full((n, kv_heads, width), -1, np.int32)
+    for t in range(n):
+        for h in range(kv_heads):
+            used = -(-int(lens[t, h, 1]) // page)
+            lists[t, h, :used] = rng.permutation(pages)[:used]
+    wide = normal(rng, n, (q_heads + q_apart) * dim, scale=1.5)
+    q = wide[:, :q_heads * dim].unflatten(1, (q_heads, dim))
+    keys, values = normal(rng, pages, kv_heads, page, dim), normal(rng, pages, kv_heads, page, dim)
+    if edit:
+        edit(q, keys, values, lists, lens)
+    out = torch.full((n, q_heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    d_lists, d_lens, scale = torch.from_numpy(lists).cuda(), torch.from_numpy(lens).cuda(), 1 / math.sqrt(dim)
+    anc = signed(words) if words else None
+    torch.cuda.synchronize()
+    op = A.SelectedAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(d_lists), held(d_lens), ancestors=held(anc), scale=scale)
+    op.run()
+    backend.synchronize_device()
+    same_bits(op, out, backend)
+    group = q_heads // kv_heads
+    for t in range(n):
+        for h in heads or range(kv_heads):
+            context, total = map(int, lens[t, h])
+            k, v = (x[torch.from_numpy(lists[t, h, :-(-total // page)].astype(np.int64)).cuda(), h].flatten(0, 1)[:total].double().cpu() for x in (keys, values))
+            seen = torch.ones(1, total, dtype=torch.bool)
+            for j in range(total - context):
+                seen[0, context + j] = not words or bool(words[t] >> j & 1)
+            some = range(group) if group * total < 20000 else sorted({0, group - 1})
+            for g in some:
+                row = q[t, h * group + g][None].double().cpu()
+                want, spread = formula(row, k, v, scale, seen)
+                check(out[t, h * group + g][None], want, spread)
+    return out
+
+
+@pytest.mark.parametrize("dim", [8, 64, 72, 128])
+@pytest.mark.parametrize("q_heads,kv_heads", [(1, 1), (8, 1), (12, 4), (40, 2), (33, 1), (128, 1)])
+def test_selected(backend, q_heads, kv_heads, dim):
+    run_selected(backend, [0, 15, 16, 17, 130, 400, 33], [1, 1, 1, 1, 1, 1, 0], q_heads, kv_heads, dim, 16)
+
+
+@pytest.mark.parametrize("page", [16, 64, 128, 1024])
+def test_selected_pages(backend, page):
+    run_selected(backend, [3 * page, page + 5, 1], [5, 1, 64], 6, 2, 96, page, width=8)
+
+
+def test_selected_trees(backend):
+    rng = np.random.default_rng(2)
+    words = tree_words(24, rng, "tree") + tree_words(64, rng, "tree")
+    run_selected(backend, [500] * 24 + [37] * 64, [24] * 24 + [64] * 64, 6, 2, 64, 16, words=words)
+    run_selected(backend, [0, 16, 5], [9, 9, 9], 4, 2, 128, 16, words=[0, 0, 1 << 8])
+
+
+def test_selected_rows_that_see_nothing(backend):
+    import torch
+
+    out = run_selected(backend, [0, 0, 20], [0, 4, 1], 4, 1, 64, 16, words=[5, 0, 1], width=4)
+    assert torch.count_nonzero(out[:2]) == 0
+
+
+def test_selected_many_lists(backend):
+    """More lists than a CTA has lanes many times over, and few long ones that are cut."""
+    rng = np.random.default_rng(4)
+    run_selected(backend, [int(n) for n in rng.integers(0, 300, 700)], [1] * 700, 4, 2, 64, 16, pages=200)
+    run_selected(backend, [9000], [3], 8, 2, 128, 64, pages=160)
+    run_selected(backend, [2000] * 20, [1] * 20, 32, 8, 64, 32, pages=100, heads=[0, 7])
+
+
+def test_selected_one_page_many_times(backend):
+    def edit(q, keys, values, lists, lens):
+        lists[0, 0, :5] = [3, 3, 0, 3, 0]
+        lists[1, 0, :5] = lists[0, 0, 4::-1]
+
+    run_selected(backend, [70, 70], [3, 3], 2, 1, 64, 16, edit=edit)
+
+
+def test_selected_queries_with_gaps(backend):
+    run_selected(backend, [70, 200], [1, 1], 4, 2, 64, 16, q_apart=3)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+def test_selected_unseen_keys_have_no_influence(backend, value):
+    """Behind the end of a list, in pages that are not in it, and new tokens that are no ancestors; those that see it are what the formula says."""
+
+    def edit(q, keys, values, lists, lens):
+        for x in (keys, values):
+            x[int(lists[0, 0, 2]), :, 8:] = value   # 37 + 3 keys: rows 8 and on of the third page
+            x[int(lists[1, 0, 3]), 0, 4] = value    # place 52 of 50 + 9: new token 2
+            unused = sorted(set(range(len(keys))) - set(lists[:, 0].flatten().tolist()))
+            x[unused] = value
+
+    run_selected(backend, [37, 50], [3, 9], 4, 1, 64, 16, words=[7, 0b100000011], edit=edit)
+    run_selected(backend, [37, 50], [3, 9], 4, 1, 128, 16, words=[7, 0b100000111], edit=edit)
+
+
+def test_selected_values_of_every_size(backend):
+    def edit(q, keys, values, lists, lens):
+        keys[::2] *= 1e18
+        q[0] *= 1e18
+        q[1] *= 1e-30
+
+    run_selected(backend, [70, 300], [3, 9], 4, 1, 64, 16, edit=edit)
+
+
+def test_selected_outside(backend):
+    """Pages outside the cache are not followed, lengths that cannot be are rows of zeros; other rows keep their bits."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(3)
+    q, keys, values = normal(rng, 8, 4, 64), normal(rng, 12, 2, 16, 64), normal(rng, 12, 2, 16, 64)
+    lists = torch.from_numpy(rng.integers(0, 12, (8, 2, 5)).astype(np.int32)).cuda()
+    lens = torch.tensor([[[60, 61], [70, 71]]] * 8, dtype=torch.int32, device="cuda")
+    out, good = torch.empty_like(q), torch.empty_like(q)
+    run = lambda o: A.SelectedAttention(backend.cuda_context, held(q), held(keys), held(values), held(o), held(lists), held(lens)).run()  # noqa: E731
+    torch.cuda.synchronize()
+    run(good)
+    backend.synchronize_device()
+    lists[1, 0, 2], lists[2, 1, 4], lists[3, 0, 0] = -1, 12, 2**31 - 1
+    lens[4, 0], lens[5, 1], lens[6, 0], lens[7, 1] = i32([-1, 5]), i32([20, 19]), i32([3, 68]), i32([70, 81])
+    torch.cuda.synchronize()
+    run(out)
+    with pytest.raises(N.WfError) as e:
+        backend.synchronize_device()
+    assert e.value.status == N.WF_ERR_INDEX
+    differ = (out != good).any(-1).cpu()
+    want = torch.zeros(8, 4, dtype=torch.bool)
+    for t, h in ((1, 0), (2, 1), (3, 0), (4, 0), (5, 1), (6, 0), (7, 1)):
+        want[t, 2 * h:2 * h + 2] = True
+    assert torch.equal(differ, want)
+    for t, h in ((4, 0), (5, 1), (6, 0), (7, 1)):
+        assert torch.count_nonzero(out[t, 2 * h:2 * h + 2]) == 0
+    # without the keys of the page that is not there
+    for t, h, j in ((1, 0, 2), (2, 1, 4), (3, 0, 0)):
+        total = int(lens[t, h, 1])
+        kept = [i for i in range(total) if i // 16 != j]
+        at = torch.tensor(kept)
+        names = lists[t, h].cpu().long()[at // 16]
+        k, v = (x.cpu()[names, h, at % 16].double() for x in (keys, values))
+        for g in range(2):
+            w, spread = formula(q[t, 2 * h + g][None].double().cpu(), k, v, 1 / 8, torch.ones(1, len(kept), dtype=torch.bool))
+            check(out[t, 2 * h + g][None], w, spread)
+
+
+def test_selected_refusals(backend):
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    q, keys = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(9, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    lists, lens = torch.zeros(2, 2, 3, dtype=torch.int32, device="cuda"), torch.zeros(2, 2, 2, dtype=torch.int32, device="cuda")
+
+    def make(keys=keys, **more):
+        return A.SelectedAttention(backend.cuda_context, held(q), held(keys), held(keys), held(torch.empty_like(q)), held(lists), held(lens), **more)
+
+    make().run()
+    backend.synchronize_device()
+    for more, status in ((dict(scale=0.0), N.WF_ERR_INVALID_ARGUMENT), (dict(layer=1), N.WF_ERR_SHAPE), (dict(layer=-1), N.WF_ERR_SHAPE)):
+        with pytest.raises(N.WfError) as e:
+            make(**more).run()
+        assert e.value.status == status
+    op = make()
+    op.args.width = 0
+    with pytest.raises(N.WfError):
+        op.run()
+    with pytest.raises(ValueError):
+        make(ancestors=held(lists))
+    backend.synchronize_device()
+
+
+# ------------------------------------------------------------------------------------------------ shared prefixes
+def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, page, shape="tree", seed=0, edit=None, arrays=True, only=None, most=None, garbage=False):
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(seed)
+    n = sum(drafts)
+    of = [g for g, m in enumerate(members) for _ in range(m)]
+    q = normal(rng, n, q_heads, dim, scale=1.5)
+    first = offsets(members)
+    need = [-(-(a + b) // page) for a, b in zip(own, drafts)]
+    order = list(rng.permutation(sum(need) + sum(p // page for p in prefix) + 2).astype(np.int32))
+    pages = len(order)
+    common = [[order.pop() for _ in range(p // page)] for p in prefix]
+    width = max(len(common[g]) + m for g, m in zip(of, need)) or 1
+    tables = np.full((len(own), width), 2**31 - 1, np.int32)
+    for s, g in enumerate(of):
+        row = common[g] + [order.pop() for _ in range(need[s])]
+        tables[s, :len(row)] = row
+        if garbage and s != first[g]:
+            tables[s, :len(common[g])] = -5
+    keys, values = normal(rng, pages, kv_heads, page, dim), normal(rng, pages, kv_heads, page, dim)
+    words = [w for m in drafts for w in tree_words(m, rng, shape)]
+    if edit:
+        edit(q, keys, values, tables)
+    out = torch.full((n, q_heads, dim), 7.0, dtype=torch.bfloat16, device="cuda")
+    context = [prefix[g] + a for g, a in zip(of, own)]
+    tab, ctx, off, groups, pre, scale = torch.from_numpy(tables).cuda(), i32(context), i32(offsets(drafts)), i32(first), i32(prefix), 1 / math.sqrt(dim)
+    anc = signed(words) if words else torch.zeros(0, dtype=torch.int64, device="cuda")
+    torch.cuda.synchronize()
+    op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=most or max(prefix),
+                                 max_own=most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
+    op.run()
+    backend.synchronize_device()
+    same_bits(op, out, backend)
+    group, starts = q_heads // kv_heads, offsets(drafts)
+    for s, (g, new) in enumerate(zip(of, drafts)):
+        if only and s not in only:
+            continue
+        total, rows = context[s] + new, slice(starts[s], starts[s + 1])
+        t = np.arange(total)
+        names = np.where(t < prefix[g], tables[first[g]][np.minimum(t // page, width - 1)], tables[s][t // page])
+        where = torch.from_numpy(names.astype(np.int64)).cuda()
+        k, v = (x[where, :, torch.from_numpy(t % page).cuda()].double().cpu() for x in (keys, values))
+        seen = torch.ones(new, total, dtype=torch.bool)
+        for i in range(new):
+            for j in range(new):
+                seen[i, context[s] + j] = bool(words[starts[s] + i] >> j & 1)
+        heads = range(q_heads) if new * total * q_heads < 20000 else sorted({0, q_heads - 1})
+        for h in heads:
+            want, spread = formula(q[rows, h].double().cpu(), k[:, h // group], v[:, h // group], scale, seen)
+            check(out[rows, h], want, spread)
+    return out
+
+
+@pytest.mark.parametrize("dim", [8, 64, 72, 128])
+@pytest.mark.parametrize("q_heads,kv_heads", [(1, 1), (8, 2), (5, 1), (40, 1), (128, 1)])
+def test_shared(backend, q_heads, kv_heads, dim):
+    run_shared(backend, [3, 1, 4], [48, 0, 160], [5, 100, 0, 33, 16, 1, 64, 7], [1] * 8, q_heads, kv_heads, dim, 16)
+
+
+@pytest.mark.parametrize("page", [16, 64, 512])
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(6, 2, 128), (4, 4, 64), (16, 1, 96)])
+def test_shared_trees(backend, page, q_heads, kv_heads, dim):
+    run_shared(backend, [3, 2], [page, 3 * page], [37, 200, 0, 5, 77], [9, 1, 24, 7, 3], q_heads, kv_heads, dim, page)
+    run_shared(backend, [2, 1], [page, 0], [20, 3, 555], [2, 64, 5], q_heads, kv_heads, dim, page, shape="chain", garbage=True)
+
+
+def test_shared_defaults(backend):
+    """Without offsets and words: every sequence has max_drafts tokens, a chain; bounds far above the lengths."""
+    run_shared(backend, [3, 1], [64, 16], [100, 333, 5, 0], [4, 4, 4, 4], 4, 2, 64, 16, shape="chain", arrays=False)
+    run_shared(backend, [3, 1], [64, 16], [100, 333, 5, 0], [2, 4, 1, 4], 4, 2, 64, 16, most=5000)
+
+
+def test_shared_long_prefix(backend):
+    """Prefixes that many CTAs take a part of, by rows that fill several tiles, one, and a few of one."""
+    run_shared(backend, [40], [4096], [3 * i for i in range(40)], [1] * 40, 16, 2, 128, 64, only=[0, 17, 39])
+    run_shared(backend, [2], [20000], [300, 40], [1, 1], 8, 1, 64, 32, garbage=True)
+    run_shared(backend, [5, 7], [9008, 3200], [20, 700, 5, 0, 64, 3, 3, 3, 1500, 3, 3, 3], [1, 2, 1, 3, 1, 1, 1, 5, 1, 1, 1, 1], 24, 8, 64, 16, only=[0, 3, 8])
+
+
+def test_shared_long_own(backend):
+    """Own contexts that are cut, behind prefixes, by few rows and by many."""
+    run_shared(backend, [2, 1], [1024, 0], [9000, 10, 70], [1, 1, 1], 8, 2, 128, 64)
+    run_shared(backend, [2], [512], [5000, 3000], [40, 12], 8, 2, 64, 32, garbage=True)
+
+
+def test_shared_many_sequences(backend):
+    rng = np.random.default_rng(6)
+    members = [1 + int(n) for n in rng.integers(0, 7, 70)]
+    count = sum(members)
+    run_shared(backend, members, [16 * int(n) for n in rng.integers(0, 9, 70)], [int(n) for n in rng.integers(0, 60, count)], [1 + int(n) for n in rng.integers(0, 3, count)], 2, 1, 64, 16,
+               only=list(range(0, count, 5)))
+
+
+def test_shared_one_long_group(backend):
+    """More rows than two tiles: several units read the same prefix."""
+    run_shared(backend, [300], [256], [int(i % 40) for i in range(300)], [1] * 300, 4, 1, 64, 16, only=[0, 1, 128, 299])
+
+
+def test_shared_nothing_in_common(backend):
+    run_shared(backend, [1, 1, 1], [0, 0, 0], [100, 333, 5], [3, 1, 2], 4, 2, 64, 16)
+
+
+def test_shared_rows_that_see_nothing(backend):
+    import torch
+
+    out = run_shared(backend, [2], [0], [0, 20], [3, 2], 4, 2, 64, 16, shape="none")
+    assert torch.count_nonzero(out[:3]) == 0
+
+
+def test_shared_sequences_without_tokens(backend):
+    run_shared(backend, [3, 2], [48, 32], [5, 100, 0, 33, 16], [1, 0, 2, 0, 0], 4, 2, 64, 16)
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("drafts", [[2, 9, 1], [20, 9, 33]])
+def test_shared_unseen_keys_have_no_influence(backend, value, drafts):
+    """Behind the ends, in drafts that are no ancestors, in another group's prefix; a row that sees it has what the formula says."""
+
+    def edit(q, keys, values, tables):
+        for x in (keys, values):
+            x[int(tables[0][-(-(32 + 37 + drafts[0]) // 16) - 1]), :, (37 + drafts[0] - 1) % 16 + 1:] = value
+            x[int(tables[1][(32 + 50 + 2) // 16]), 1, 4] = value  # the third draft, seen by some
+            x[int(tables[2][1]), 0, 3] = value                    # the other group's prefix
+
+    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 4, 2, 64, 16, edit=edit, garbage=True)
+    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 12, 2, 128, 16, edit=edit, garbage=True)
+
+
+def test_shared_values_of_every_size(backend):
+    """Scores that leave the prefix or the own keys no weight at all, near the lowest and the largest fp32."""
+
+    def edit(q, keys, values, tables):
+        keys[int(tables[0][0])] *= 1e18
+        q[0] *= 1e18
+        q[1] *= 1e-30
+        keys[int(tables[1][3])] *= 30
+        q[2:] *= 10
+
+    run_shared(backend, [4], [48], [37, 50, 9, 16], [1, 1, 2, 1], 4, 2, 64, 16, edit=edit)
+
+
+def test_shared_outside(backend):
+    """Groups, prefixes, contexts and pages that cannot be: reported, rows of zeros or without those keys; the others keep their bits."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(3)
+    q, keys, values = normal(rng, 8, 4, 64), normal(rng, 40, 2, 16, 64), normal(rng, 40, 2, 16, 64)
+    tables = torch.arange(40, dtype=torch.int32, device="cuda").repeat(8, 1)
+    good_out = torch.empty_like(q)
+
+    def run(out, tables=tables, context=(40,) * 8, groups=(0, 2, 4, 6, 8), prefix=(32,) * 4, max_prefix=64, max_own=40):
+        tab, ctx, gr, pre = tables.contiguous(), i32(context), i32(groups), i32(prefix)
+        out.fill_(7.0)
+        torch.cuda.synchronize()
+        A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(gr), held(pre), max_prefix=max_prefix, max_own=max_own).run()
+
+    run(good_out)
+    backend.synchronize_device()
+    out = torch.empty_like(q)
+    zeros = lambda: [t for t in range(8) if torch.count_nonzero(out[t]) == 0]  # noqa: E731
+    same = lambda: [t for t in range(8) if torch.equal(out[t], good_out[t])]  # noqa: E731
+    for bad, at in ((dict(prefix=(32, 24, 32, 32)), [2, 3]), (dict(prefix=(32, 32, -16, 32)), [4, 5]), (dict(prefix=(80, 32, 32, 32)), [0, 1]),
+                    (dict(context=(40, 31, 40, 40, 40, 40, 73, 40)), [1, 6]), (dict(context=(40, 40, -1, 40, 40, 2**31 - 1, 40, 40)), [2, 5]),
+                    (dict(groups=(1, 2, 4, 6, 8)), [0]), (dict(groups=(0, 2, 4, 6, 7)), [7]), (dict(groups=(0, 2, 4, 6, 9)), [6, 7])):
+        run(out, **bad)
+        with pytest.raises(N.WfError) as e:
+            backend.synchronize_device()
+        assert e.value.status == N.WF_ERR_INDEX
+        assert zeros() == at and same() == [t for t in range(8) if t not in at], bad
+    for bad in ((0, 4, 2, 6, 8), (8, 6, 4, 2, 0), (-5, 2, 4, 6, 8)):  # which sequences are left, nothing says; no more than that
+        run(out, groups=bad)
+        with pytest.raises(N.WfError):
+            backend.synchronize_device()
+    wrong = tables.clone()
+    wrong[2, 1], wrong[5, 2] = -1, 40  # of a group's prefix, of a sequence's own
+    run(out, tables=wrong)
+    with pytest.raises(N.WfError) as e:
+        backend.synchronize_device()
+    assert e.value.status == N.WF_ERR_INDEX and same() == [0, 1, 4, 6, 7]
+    for t, gone in ((2, range(16, 32)), (3, range(16, 32)), (5, range(32, 48))):
+        at = torch.tensor([i for i in range(41) if i not in gone])
+        for h in range(4):
+            k, v = (x.cpu()[at // 16, h // 2, at % 16].double() for x in (keys, values))
+            w, spread = formula(q[t, h][None].double().cpu(), k, v, 1 / 8, torch.ones(1, len(at), dtype=torch.bool))
+            check(out[t, h][None], w, spread)
+
+
+def test_shared_is_what_trees_are(backend):
+    """The same call with and without a prefix, and by TreeAttention."""
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(8)
+    q, keys, values = normal(rng, 6, 8, 128), normal(rng, 30, 2, 64, 128), normal(rng, 30, 2, 64, 128)
+    rows = [list(range(9)) + [10 + 3 * s, 11 + 3 * s, 12 + 3 * s] for s in range(6)]
+    tables, context = i32(rows), i32([9 * 64 + 20 * s for s in range(6)])
+    outs = [torch.empty_like(q) for _ in range(3)]
+    args = [held(x) for x in (q, keys, values)]
+    torch.cuda.synchronize()
+    A.TreeAttention(backend.cuda_context, *args, held(outs[0]), held(tables), held(context), max_context=700).run()
+    for out, p in ((outs[1], 0), (outs[2], 9 * 64)):
+        groups, prefix = i32([0, 6]), i32([p])
+        torch.cuda.synchronize()
+        A.SharedPrefixAttention(backend.cuda_context, *args, held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=p, max_own=700 - p).run()
+        backend.synchronize_device()
+    assert torch.equal(outs[0], outs[1])
+    assert (outs[0].float() - outs[2].float()).abs().max() <= 2.0**-6 * outs[0].float().abs().max()
+
+
+def test_shared_refusals(backend):
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    q, keys = torch.zeros(2, 4, 64, dtype=torch.bfloat16, device="cuda"), torch.zeros(9, 2, 16, 64, dtype=torch.bfloat16, device="cuda")
+    tables, ctx, groups, prefix = torch.zeros(2, 4, dtype=torch.int32, device="cuda"), i32([0, 0]), i32([0, 2]), i32([0])
+
+    def make(groups=groups, prefix=prefix, **more):
+        args = dict(max_prefix=16, max_own=16) | more
+        return A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(keys), held(torch.empty_like(q)), held(tables), held(ctx), held(groups), held(prefix), **args)
+
+    make().run()
+    backend.synchronize_device()
+    for more, status in ((dict(max_prefix=-1), N.WF_ERR_SHAPE), (dict(max_own=-1), N.WF_ERR_SHAPE), (dict(max_drafts=0), N.WF_ERR_TOO_LARGE), (dict(max_drafts=65), N.WF_ERR_TOO_LARGE),
+                         (dict(max_drafts=2), N.WF_ERR_SHAPE), (dict(scale=-1.0), N.WF_ERR_INVALID_ARGUMENT), (dict(groups=i32([0]), prefix=i32([])), N.WF_ERR_SHAPE),
+                         (dict(groups=i32([0, 1, 2, 2]), prefix=i32([0, 0, 0])), N.WF_ERR_SHAPE)):
+        with pytest.raises(N.WfError) as e:
+            make(**more).run()
+        assert e.value.status == status, more
+    with pytest.raises(ValueError):
+        make(groups=i32([0, 1, 2]))
+    backend.synchronize_device()
+
+
+def test_shared_and_selected_recorded(backend):
+    """Recorded calls serve growing contexts, prefixes and lists; a call that would have to allocate while it is recorded is refused."""
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(11)
+    ctx = backend.cuda_context
+    q, keys, values = normal(rng, 3, 4, 64), normal(rng, 90, 2, 16, 64), normal(rng, 90, 2, 16, 64)
+    tables = torch.arange(90, dtype=torch.int32, device="cuda").repeat(3, 1)
+    context, groups, prefix = i32([0, 0, 0]), i32([0, 3]), i32([0])
+    lists, lens = torch.arange(40, dtype=torch.int32, device="cuda").repeat(3, 2, 1), torch.zeros(3, 2, 2, dtype=torch.int32, device="cuda")
+    outs = [torch.empty_like(q) for _ in range(4)]
+    args = [held(x) for x in (q, keys, values)]
+    stream = backend.create_stream()
+    torch.cuda.synchronize()
+    shared = A.SharedPrefixAttention(ctx, *args, held(outs[0]), held(tables), held(context), held(groups), held(prefix), max_prefix=1000, max_own=400)
+    selected = A.SelectedAttention(ctx, *args, held(outs[1]), held(lists), held(lens))
+    shared.run(stream)
+    ctx.synchronize(stream)
+    ctx.graph_begin(stream)
+    shared.run(stream)
+    selected.run(stream)
+    graph = ctx.graph_end(stream)
+    for p, own in ((0, 3), (160, 20), (992, 400)):
+        context.fill_(p + own)
+        prefix.fill_(p)
+        lens[..., 0], lens[..., 1] = own, own + 1
+        torch.cuda.synchronize()
+        ctx.graph_launch(graph, stream)
+        ctx.synchronize(stream)
+        A.TreeAttention(ctx, *args, held(outs[2]), held(tables), held(context), max_context=1400).run()
+        short = i32([own] * 3)
+        torch.cuda.synchronize()
+        A.TreeAttention(ctx, *args, held(outs[3]), held(tables), held(short), max_context=640).run()
+        backend.synchronize_device()
+        for got, want in zip(outs, outs[2:]):
+            assert (got.float() - want.float()).abs().max() <= 2.0**-6 * want.float().abs().max()
+    ctx.graph_destroy(graph)
+    backend.destroy_stream(stream)

@@ -47,6 +47,16 @@ class SelectPagesArgs(ctypes.Structure):  # wf_select_pages_args
         (n, ctypes.c_int32) for n in ("seqs", "q_heads", "kv_heads", "head_dim", "page_tokens", "max_drafts", "width", "first", "recent", "flags")]
 
 
+class SelectedAttentionArgs(ctypes.Structure):  # wf_selected_attention_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "out_dev", "q_stride", "pages_dev", "lens_dev", "ancestors_dev", "tokens")] + [
+        (n, ctypes.c_int32) for n in ("q_heads", "width")] + [("scale", c_f32)]
+
+
+class SharedPrefixAttentionArgs(ctypes.Structure):  # wf_shared_prefix_attention_args
+    _fields_ = [(n, c_i64) for n in ("q_dev", "out_dev", "q_stride", "q_offsets_dev", "tables_dev", "table_stride", "context_dev", "ancestors_dev", "groups_dev", "prefix_dev",
+                                     "tokens", "max_prefix", "max_own")] + [(n, ctypes.c_int32) for n in ("seqs", "q_heads", "max_drafts", "n_groups")] + [("scale", c_f32)]
+
+
 c_i32 = ctypes.c_int32
 
 # name -> (restype, argtypes); must list every function declared in include/wfb200.h
@@ -97,6 +107,8 @@ SIGNATURES = {
     "wf_cache_compact": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
     "wf_page_bounds": (c_int, [c_i64, P(KvCacheArgs), c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64, c_i64]),
     "wf_select_pages": (c_int, [c_i64, P(SelectPagesArgs), c_i64]),
+    "wf_selected_attention": (c_int, [c_i64, P(SelectedAttentionArgs), P(KvCacheArgs), c_int, c_i64]),
+    "wf_shared_prefix_attention": (c_int, [c_i64, P(SharedPrefixAttentionArgs), P(KvCacheArgs), c_int, c_i64]),
     "wf_pages_create": (c_int, [c_i64, P(c_i64)]),
     "wf_pages_destroy": (c_int, [c_i64]),
     "wf_pages_take": (c_int, [c_i64, c_i64, P(c_i32)]),

@@ -10,6 +10,8 @@ and, where reading every key of every sequence for each token takes too long,
 
     PageBounds       the largest and smallest elements of the keys of every page, in 8 bits
     SelectPages      the pages that a new token reads, by the scores that their bounds promise
+    SelectedAttention          attention over such lists of pages
+    SharedPrefixAttention      TreeAttention of sequences that have a prefix in common (forks): its keys are read once for all of them
 
 The operators bind their buffers once (shapes and types are checked then) and are run once per step: ``op.run(stream)`` is one native
 call that only enqueues.  Lengths, tables and masks are device arrays read when the kernel runs, so a recorded step
@@ -162,6 +164,44 @@ class TreeAttention(_Bound):
         a.tables_dev, a.table_stride = _typed("tables", tables, "i32", seqs, None), tables.shape()[1]
         a.context_dev, a.ancestors_dev = _typed("context_lens", context_lens, "i32", seqs), _typed("ancestors", ancestors, "i64", tokens)
         super().__init__(context, "wf_tree_attention", a, cache, layer, (q, keys, values, out, tables, context_lens, q_offsets, ancestors))
+
+
+class SharedPrefixAttention(_Bound):
+    """TreeAttention where sequences groups[g] .. groups[g + 1] - 1 have the first prefix_lens[g] tokens in common, in the same pages: those keys are read once for all of them.  groups i32
+    [n + 1] from 0 to the number of sequences, prefix_lens i32 [n], multiples of page_tokens (``KvCache.shared_prefixes`` finds both).  max_prefix and max_own, the most tokens of a prefix and
+    the most that the context of a sequence has behind it, are upper bounds; the rest as in TreeAttention."""
+
+    def __init__(self, context: CudaContext, q, keys, values, out, tables, context_lens, groups, prefix_lens, *, max_prefix: int, max_own: int, q_offsets=None, max_drafts: int = 1,
+                 ancestors=None, scale: Optional[float] = None, layer: int = 0):
+        cache = _cache_args(keys, values)
+        dim = cache.head_dim
+        tokens, heads = q.shape()[:2]
+        seqs, n = context_lens.shape()[0], prefix_lens.shape()[0]
+        a = N.SharedPrefixAttentionArgs(tokens=tokens, q_heads=heads, seqs=seqs, max_drafts=max_drafts, n_groups=n, max_prefix=max_prefix, max_own=max_own,
+                                        scale=1 / math.sqrt(dim) if scale is None else scale)
+        a.q_dev, a.out_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _typed("out", out, "bf16", tokens, heads, dim), _stride(q)
+        _dense("out", out)
+        a.q_offsets_dev = _typed("q_offsets", q_offsets, "i32", seqs + 1)
+        a.tables_dev, a.table_stride = _typed("tables", tables, "i32", seqs, None), tables.shape()[1]
+        a.context_dev, a.ancestors_dev = _typed("context_lens", context_lens, "i32", seqs), _typed("ancestors", ancestors, "i64", tokens)
+        a.groups_dev, a.prefix_dev = _typed("groups", groups, "i32", n + 1), _typed("prefix_lens", prefix_lens, "i32", n)
+        super().__init__(context, "wf_shared_prefix_attention", a, cache, layer, (q, keys, values, out, tables, context_lens, groups, prefix_lens, q_offsets, ancestors))
+
+
+class SelectedAttention(_Bound):
+    """q, out bf16 [tokens, q_heads, dim]; pages i32 [tokens, kv_heads, width] and lens i32 [tokens, kv_heads, 2] as SelectPages leaves them: which pages a token reads, how many keys of the
+    context they hold and how many keys in all.  ancestors i64 [tokens], bit j: sees new token j, the one behind those of the context (None: all that the lengths count)."""
+
+    def __init__(self, context: CudaContext, q, keys, values, out, pages, lens, *, ancestors=None, scale: Optional[float] = None, layer: int = 0):
+        cache = _cache_args(keys, values)
+        dim = cache.head_dim
+        tokens, heads = q.shape()[:2]
+        a = N.SelectedAttentionArgs(tokens=tokens, q_heads=heads, width=pages.shape()[2], scale=1 / math.sqrt(dim) if scale is None else scale)
+        a.q_dev, a.out_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _typed("out", out, "bf16", tokens, heads, dim), _stride(q)
+        _dense("out", out)
+        a.pages_dev, a.lens_dev = _typed("pages", pages, "i32", tokens, cache.kv_heads, None), _typed("lens", lens, "i32", tokens, cache.kv_heads, 2)
+        a.ancestors_dev = _typed("ancestors", ancestors, "i64", tokens)
+        super().__init__(context, "wf_selected_attention", a, cache, layer, (q, keys, values, out, pages, lens, ancestors))
 
 
 class Sequence:

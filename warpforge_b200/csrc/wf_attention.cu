@@ -3,8 +3,7 @@
 #include <algorithm>
 #include <atomic>
 
-#include "wf_attention_prompt.cuh"
-#include "wf_attention_tree.cuh"
+#include "wf_attention_launch.cuh"
 
 using namespace wf;
 
@@ -37,56 +36,11 @@ CacheView cache_layer(const wf_kv_cache& cache, int layer) {
 }
 int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too) { return check_cache(c, what, cache, layer, packed_too); }
 }  // namespace wf
-static int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
-    if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
-    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
-        return set_error(c, WF_ERR_SHAPE, "%s: bad shape tokens=%lld seqs=%d q_heads=%d", what, (long long)tokens, seqs, q_heads);
-    if (q_heads % cache->kv_heads) return set_error(c, WF_ERR_SHAPE, "%s: %d query heads over %d kv heads", what, q_heads, cache->kv_heads);
-    if (q_heads / cache->kv_heads > 128) return set_error(c, WF_ERR_TOO_LARGE, "%s: more than 128 query heads for each kv head", what);
-    if (q_stride < (int64_t)q_heads * cache->head_dim || q_stride % 8) return set_error(c, WF_ERR_SHAPE, "%s: q_stride %lld", what, (long long)q_stride);
-    return WF_OK;
-}
-template <class... Params, class... Args>
-static int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[1];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess) return cuda_status(c, e, what);
-    c->launches++;
-    return WF_OK;
-}
-
-// bf16 [z][y][x] with the given distances (elements) between y and z; boxes of 64 elements x by x bz, 128-byte swizzle, zeros outside
-static int encode_rows(Context* c, CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z, int64_t y_apart, int64_t z_apart, int by, int bz) {
-    const cuuint64_t dims[3] = {(cuuint64_t)x, (cuuint64_t)y, (cuuint64_t)z}, strides[2] = {(cuuint64_t)y_apart * 2, (cuuint64_t)z_apart * 2};
-    const cuuint32_t box[3] = {64, (cuuint32_t)by, (cuuint32_t)bz}, step[3] = {1, 1, 1};
-    const EncodeTiledFn encode = encode_tiled_fn();
-    if (!encode) return set_error(c, WF_ERR_NO_DEVICE, "the driver has no cuTensorMapEncodeTiled");
-    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
-                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
-    if (r != CUDA_SUCCESS) return set_error(c, WF_ERR_CUDA_BASE + (int)cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed: %d", (int)r);
-    return WF_OK;
-}
-static int encode_cache(Context* c, CUtensorMap* map, const bf16* base, const CacheView& v, int box_rows) {
-    if (v.page_shift == 0) return encode_rows(c, map, base, v.dim, v.kv_heads, v.pages, v.dim, (int64_t)v.kv_heads * v.dim, 1, box_rows);
-    return encode_rows(c, map, base, v.dim, 1, (v.pages * v.kv_heads) << v.page_shift, v.dim, v.dim, 1, box_rows);
-}
-static bool rows_of_sectors(const bf16* out, int dim) { return reinterpret_cast<uintptr_t>(out) % 32 == 0 && dim % 16 == 0; }
-static int dim_chunks(int dim) { return (dim + 63) / 64; }
-
 template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p, cudaStream_t s) {
     const char* what = "prompt_attention";
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, false>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
+        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, ATTEND_PROMPT>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
     GemvScratch& scratch = c->gemv_scratch[s];
@@ -115,98 +69,8 @@ template <int CHUNKS> static int launch_prompt(Context* c, const PromptParams& p
     if (pairs > (1LL << 31) - 65536) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens of %d heads", what, (long long)p.tokens, p.q_heads);
     t.split = 2 * pairs <= c->sm_count;
     const int64_t items = t.split ? (p.tokens + (int64_t)p.seqs * (t.tile_tokens - 1)) / t.tile_tokens * p.cache.kv_heads : pairs;
-    return launch_attention(c, what, prompt_tiles_kernel<CHUNKS, false>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
+    return launch_attention(c, what, prompt_tiles_kernel<CHUNKS, ATTEND_PROMPT>, (unsigned)std::min<int64_t>(items, c->sm_count), PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
 }
-
-// Where the pieces of cut units go.
-static int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cuts) {
-    GemvScratch& scratch = c->gemv_scratch[s];
-    const int64_t head = (c->sm_count * (int64_t)sizeof(TreeCut) + 255) & ~255LL, bytes = head + floats * (int64_t)sizeof(float);
-    if (bytes > scratch.attn_bytes) {
-        const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
-        if (rc != WF_OK) return rc;
-        scratch.d_attn.reset();
-        scratch.attn_bytes = 0;
-        WF_CUDA(c, make_shared_device(c, scratch.d_attn, (size_t)bytes));
-        scratch.attn_bytes = bytes;
-    }
-    cuts->cuts = reinterpret_cast<TreeCut*>(scratch.d_attn.get());
-    cuts->pieces = reinterpret_cast<float*>(scratch.d_attn.get() + head);
-    return WF_OK;
-}
-static int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
-    return launch_attention(c, "tree_attention", tree_join_kernel, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
-}
-template <int CHUNKS, int MT> static int launch_tree(Context* c, const TreeParams& p, cudaStream_t s) {
-    const char* what = "tree_attention";
-    typedef TreeShape<CHUNKS, MT> Shape;
-    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
-    if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
-        ready.fetch_or(1ull << (c->device & 63));
-    }
-    const int64_t blocks = ((int64_t)p.max_drafts * p.group + Shape::ROWS - 1) / Shape::ROWS, tiles = (p.max_context + p.max_drafts + TA_KEYS - 1) / TA_KEYS;
-    TreeTiles t{};
-    t.p = p;
-    const int64_t units = p.seqs * blocks * p.cache.kv_heads;
-    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
-    t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
-    t.c.dim = Shape::DIM;
-    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
-    CUtensorMap k, v;
-    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
-    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
-    if (rc != WF_OK) return rc;
-    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
-    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
-    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
-    return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, Shape::ROWS, s) : rc;
-}
-
-// The prompt kernel on the rows of trees.
-template <int CHUNKS> static int launch_wide_tree(Context* c, const TreeParams& p, cudaStream_t s) {
-    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
-    if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, true>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
-        ready.fetch_or(1ull << (c->device & 63));
-    }
-    PromptTiles t{};
-    t.tree = p;
-    t.p.cache = p.cache;
-    t.p.q = p.q, t.p.out = p.out, t.p.q_stride = p.q_stride;
-    t.p.tables = p.tables, t.p.table_stride = p.table_stride;
-    t.p.q_heads = p.q_heads, t.p.group = p.group;
-    t.p.scale_log2 = p.scale_log2;
-    t.p.status = p.status;
-    t.tile_tokens = PA_ROWS / p.group;
-    t.box_rows = std::min(PA_KEYS, 1 << p.cache.page_shift);
-    t.wide_rows = rows_of_sectors(p.out, p.cache.dim);
-    const int64_t blocks = (p.max_drafts + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens), tiles = (p.max_context + p.max_drafts + PA_KEYS - 1) / PA_KEYS;
-    const int64_t units = p.seqs * blocks * p.cache.kv_heads;
-    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, PA_CUT_TILES, PA_CUT_ANYWAY);
-    t.c.piece_rows = p.max_drafts <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;
-    t.c.tile_rows = t.tile_tokens * p.group;
-    t.c.tile_room = PA_ROWS;
-    t.c.dim = CHUNKS * 64;
-    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * t.c.piece_rows * (t.c.dim + 2) : 0, &t.c);
-    CUtensorMap q, k, v;
-    if (rc == WF_OK) rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
-    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
-    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
-    if (rc != WF_OK) return rc;
-    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
-    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
-    rc = launch_attention(c, "tree_attention", prompt_tiles_kernel<CHUNKS, true>, grid, PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
-    return rc == WF_OK && t.c.may_cut ? launch_join(c, p, t.c, grid, std::min(p.max_drafts, 2 * t.tile_tokens) * p.group, s) : rc;
-}
-
-#define ATTENTION_ENTER(ctxh)                                              \
-    Context* c = get_context(ctxh);                                        \
-    if (!c) return WF_ERR_INVALID_HANDLE;                                  \
-    ScopedLock _lk(c);                                                     \
-    if (!_lk.ok) return WF_ERR_BUSY;                                       \
-    WF_CUDA(c, cudaSetDevice(c->device));                                  \
-    cudaStream_t s = resolve_stream(c, stream)
 
 extern "C" {
 
@@ -285,9 +149,10 @@ int wf_tree_attention(int64_t ctx, const wf_tree_attention_args* a, const wf_kv_
     // Tiles of 128 rows on the 5th-generation tensor cores, or of 16 or 32 on mma.sync.  48 sequences of 1500 tokens, 8 heads of 128, 20 / 24 / 32 rows: 71.5 / 72.3 / 73.2 us
     // against 65.1 / 66.1 / 67.8; 8 of 2000, 4 / 16 / 32 rows: 22.4 / 23.3 / 23.9 against 19.1 / 20.7 / 25.7; one of 600: 12.3 for all three against 9.5 / 10.1 / 13.4.  With more
     // than 32 rows a row's sums no longer fit in the registers of the warps that multiply.
-    if (rows > 32) return chunks == 1 ? launch_wide_tree<1>(c, p, s) : launch_wide_tree<2>(c, p, s);
-    if (chunks == 1) return rows <= 16 ? launch_tree<1, 1>(c, p, s) : launch_tree<1, 2>(c, p, s);
-    return rows <= 16 ? launch_tree<2, 1>(c, p, s) : launch_tree<2, 2>(c, p, s);
+    const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, context = p.max_context + p.max_drafts;
+    if (rows > 32) return chunks == 1 ? launch_wide_tree<1, ATTEND_TREE>(c, p, units, a->max_drafts, context, s) : launch_wide_tree<2, ATTEND_TREE>(c, p, units, a->max_drafts, context, s);
+    if (chunks == 1) return rows <= 16 ? launch_tree<1, 1, ATTEND_TREE>(c, p, units, rows, context, s) : launch_tree<1, 2, ATTEND_TREE>(c, p, units, rows, context, s);
+    return rows <= 16 ? launch_tree<2, 1, ATTEND_TREE>(c, p, units, rows, context, s) : launch_tree<2, 2, ATTEND_TREE>(c, p, units, rows, context, s);
 }
 
 }  // extern "C"

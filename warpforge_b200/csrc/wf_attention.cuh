@@ -11,6 +11,10 @@ typedef __nv_bfloat16 bf16;
 constexpr int ATTN_MAX_DIM = 128;
 constexpr int TREE_MAX_DRAFTS = 64;  // a row's ancestors are one 64-bit word
 
+// What rows attend to: a prompt's past and itself; a sequence's context and new tokens; a list of pages for each token and kv head; where sequences have a prefix in
+// common, that prefix (the rows of all of them), and what a sequence has of its own behind it.
+enum AttentionKind { ATTEND_PROMPT, ATTEND_TREE, ATTEND_LISTS, ATTEND_PREFIX, ATTEND_OWN };
+
 // One layer of the cache, or packed keys and values (page_shift 0, a page a token).
 struct CacheView {
     bf16* keys;
@@ -62,7 +66,19 @@ struct TreeParams {
     uint32_t group_inverse;  // 2^32 / group, rounded up; 0 for a group of one
     float scale_log2;
     int* status;
+    // lists: tables is int32 [tokens][kv_heads][table_stride], and for each: tokens of the context in the list, keys in all
+    const int2* lens;
+    // prefixes: sequences groups[g] .. groups[g + 1] - 1 have prefix[g] tokens in common, whose pages the first one's table names
+    const int* groups;
+    const int* prefix;
+    int64_t max_prefix;
+    int n_groups;
+    int2* prefix_of;  // [seqs], made by the kernel that reads the prefixes: prefix (-1: cannot be) and first sequence of the group
+    float* state;     // of every row over its prefix: sums [tokens * q_heads][state_dim], then maxima, then sums of weights
+    int state_dim;
 #ifdef __CUDACC__
+    __device__ __forceinline__ float* state_maxima() const { return state + (size_t)tokens * q_heads * state_dim; }
+    __device__ __forceinline__ float* state_weights() const { return state_maxima() + (size_t)tokens * q_heads; }
     // row / group, for the rows of a sequence (64 x 128 at most)
     __device__ __forceinline__ int token_of(int row) const { return group_inverse ? (int)__umulhi((uint32_t)row, group_inverse) : row; }
 #endif
@@ -89,8 +105,17 @@ __device__ __forceinline__ PromptSeq prompt_seq(const PromptParams& p, int s) {
     q.place.first = q.row0;
     return q;
 }
+// Keys of a sequence behind a prefix that lies in another one's pages.
+struct SharedPlace {
+    const int* first;
+    int prefix;
+    const int* table;
+    __device__ __forceinline__ int64_t page_of(const CacheView& c, int t) const { return (t < prefix ? first : table)[t >> c.page_shift]; }
+};
 struct TreeSeq {
     int row0, rows, context;
+    int news;    // keys behind the context
+    int prefix;  // own keys: tokens before them, which other kernels have seen to
     KeyPlace place;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
@@ -103,10 +128,90 @@ __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
     const bool bad_keys = q.context < 0 || (int64_t)q.context > p.max_context || (int64_t)q.context + q.rows > (p.table_stride << p.cache.page_shift);
     if (bad_keys) q.context = -1;  // its rows are zeros
     if (bad || bad_keys) report_status(p.status, STATUS_BAD_INDEX);
+    q.news = q.rows;
     q.place.table = p.tables + (size_t)s * p.table_stride;
     q.place.first = 0;
     return q;
 }
+// A token's list for a kv head (s counts both): one row of the group.
+__device__ __forceinline__ TreeSeq list_seq(const TreeParams& p, int s) {
+    TreeSeq q;
+    const int2 lens = p.lens[s];
+    const bool bad = lens.x < 0 || lens.y < lens.x || lens.y - lens.x > TREE_MAX_DRAFTS || (int64_t)lens.y > p.table_stride << p.cache.page_shift;
+    if (bad) report_status(p.status, STATUS_BAD_INDEX);
+    q.row0 = s / p.cache.kv_heads;
+    q.rows = 1;
+    q.context = bad ? -1 : lens.x;  // its rows are zeros
+    q.news = bad ? 0 : lens.y - lens.x;
+    q.place.table = p.tables + (size_t)s * p.table_stride;
+    q.place.first = 0;
+    return q;
+}
+// The rows of a group of sequences, over the prefix that they share.  prefix: -1 where the group cannot be.
+struct GroupSeqs {
+    int first, stop, prefix;
+};
+__device__ __forceinline__ GroupSeqs group_seqs(const TreeParams& p, int g) {
+    GroupSeqs q;
+    q.first = p.groups[g], q.stop = p.groups[g + 1], q.prefix = p.prefix[g];
+    if (q.first < 0 || q.stop < q.first || q.stop > p.seqs || q.prefix < 0 || (int64_t)q.prefix > p.max_prefix || q.prefix & ((1 << p.cache.page_shift) - 1) ||
+        (int64_t)q.prefix > p.table_stride << p.cache.page_shift) {
+        report_status(p.status, STATUS_BAD_INDEX);
+        q.prefix = -1;
+        q.first = max(0, min(q.first, p.seqs));
+        q.stop = max(q.first, min(q.stop, p.seqs));
+    }
+    return q;
+}
+__device__ __forceinline__ TreeSeq prefix_seq(const TreeParams& p, int g) {
+    TreeSeq q;
+    const GroupSeqs of = group_seqs(p, g);
+    const bool some = of.prefix > 0 && of.stop > of.first;
+    int64_t a = 0, b = 0;
+    if (some) {
+        a = p.q_offsets ? p.q_offsets[of.first] : (int64_t)of.first * p.max_drafts;
+        b = p.q_offsets ? p.q_offsets[of.stop] : (int64_t)of.stop * p.max_drafts;
+    }
+    const bool bad = a < 0 || b < a || b > p.tokens;
+    if (bad) report_status(p.status, STATUS_BAD_INDEX);
+    q.row0 = bad ? 0 : (int)a;
+    q.rows = bad ? 0 : (int)(b - a);
+    q.context = max(0, of.prefix);
+    q.news = 0;
+    q.place.table = p.tables + (size_t)(some ? of.first : 0) * p.table_stride;
+    q.place.first = 0;
+    return q;
+}
+// What a sequence has behind its prefix.
+__device__ __forceinline__ TreeSeq own_seq(const TreeParams& p, int s) {
+    TreeSeq q;
+    const int64_t a = p.q_offsets ? p.q_offsets[s] : (int64_t)s * p.max_drafts, b = p.q_offsets ? p.q_offsets[s + 1] : a + p.max_drafts;
+    const bool bad = a < 0 || b < a || b > p.tokens || b - a > p.max_drafts;
+    q.row0 = bad ? 0 : (int)a;
+    q.rows = bad ? 0 : (int)(b - a);
+    q.prefix = p.prefix_of[s].x;
+    const int64_t context = p.context[s], own = context - q.prefix;
+    const bool bad_keys = q.prefix < 0 || own < 0 || own > p.max_context || context + q.rows > (p.table_stride << p.cache.page_shift);
+    q.context = bad_keys ? -1 : (int)own;  // its rows are zeros
+    if (bad_keys) q.prefix = 0;
+    if (bad || bad_keys) report_status(p.status, STATUS_BAD_INDEX);
+    q.news = q.rows;
+    q.place.table = p.tables + (size_t)s * p.table_stride + (q.prefix >> p.cache.page_shift);
+    q.place.first = 0;
+    return q;
+}
+template <int KIND> __device__ __forceinline__ TreeSeq seq_of(const TreeParams& p, int s) {
+    if (KIND == ATTEND_LISTS) return list_seq(p, s);
+    if (KIND == ATTEND_PREFIX) return prefix_seq(p, s);
+    if (KIND == ATTEND_OWN) return own_seq(p, s);
+    return tree_seq(p, s);
+}
+// Of a sequence, a segment or a cut unit: new keys, keys in all; context < 0: one that cannot be.
+template <int KIND, class Seq> __device__ __forceinline__ int news_of(const Seq& q) {
+    if constexpr (KIND == ATTEND_LISTS) return q.news;
+    return KIND == ATTEND_PREFIX ? 0 : q.rows;
+}
+template <int KIND, class Seq> __device__ __forceinline__ int keys_of(const Seq& q) { return q.context < 0 ? 0 : q.context + news_of<KIND>(q); }
 
 __device__ __forceinline__ float warp_sum(float v) {
 #pragma unroll
@@ -132,8 +237,8 @@ __device__ __forceinline__ bool scores_too_large(float m, float scale) { return 
 
 // One row by one warp, key by key: lane l has elements 4 l .. 4 l + 3.  softmax(s) v = sum_t 2^(s_t - m) v_t / sum_t 2^(s_t - m) with the
 // running maximum m; keys that are not seen are not read, but all pages are looked at.
-template <class Seen>
-__device__ __noinline__ void attend_row(const CacheView& c, const KeyPlace& place, const bf16* q, bf16* out, int head, int keys, float scale_log2, int* status,
+template <class Place, class Seen>
+__device__ __noinline__ void attend_row(const CacheView& c, const Place& place, const bf16* q, bf16* out, int head, int keys, float scale_log2, int* status,
                                         Seen seen) {
     const int lane = threadIdx.x & 31;
     const bool mine = 4 * lane < c.dim;
@@ -176,6 +281,29 @@ struct SeesAncestors {
 };
 __device__ __forceinline__ uint64_t ancestors_of(const TreeParams& p, int row, int i) {
     return p.ancestors ? p.ancestors[row] : (uint64_t)-1 >> (63 - i);
+}
+// The new keys that token i of a sequence (row `row` of q) sees, of the `news` that there are.
+template <int KIND> __device__ __forceinline__ uint64_t sees_of(const TreeParams& p, int row, int i, int news) {
+    if (KIND == ATTEND_PREFIX) return 0;
+    if (KIND == ATTEND_LISTS) return news == 0 ? 0 : (p.ancestors ? p.ancestors[row] : (uint64_t)-1) & ((uint64_t)-1 >> (64 - news));
+    return ancestors_of(p, row, i) & ((uint64_t)-1 >> (64 - news));
+}
+// A row key by key: token i of unit or segment w, whose list or table has the number w.seq.
+template <int KIND, class Unit>
+__device__ __forceinline__ void attend_again(const TreeParams& p, const Unit& w, int i, int head, const bf16* q, bf16* out) {
+    const uint64_t sees = sees_of<KIND>(p, w.row0 + i, i, news_of<KIND>(w));
+    const int keys = keys_of<KIND>(w);
+    if (KIND == ATTEND_OWN) {
+        const int2 prefix = p.prefix_of[w.seq];
+        const int before = w.context < 0 ? 0 : prefix.x;
+        const SharedPlace place = {p.tables + (size_t)(w.context < 0 ? 0 : prefix.y) * p.table_stride, before, p.tables + (size_t)w.seq * p.table_stride};
+        attend_row(p.cache, place, q, out, head, before + keys, p.scale_log2, p.status, SeesAncestors{before + w.context, sees});
+    } else {
+        KeyPlace place;
+        place.table = p.tables + (size_t)w.seq * p.table_stride;
+        place.first = 0;
+        attend_row(p.cache, place, q, out, head, keys, p.scale_log2, p.status, SeesAncestors{w.context, sees});
+    }
 }
 #endif
 

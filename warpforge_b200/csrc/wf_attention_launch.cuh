@@ -1,0 +1,154 @@
+// What the entry points of attention share: checks, tensor maps, scratch, launches.
+#pragma once
+#include <algorithm>
+#include <atomic>
+
+#include "wf_attention_prompt.cuh"
+#include "wf_attention_tree.cuh"
+
+namespace wf {
+
+CacheView cache_layer(const wf_kv_cache& cache, int layer);
+int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too);
+
+inline int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
+    if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
+    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
+        return set_error(c, WF_ERR_SHAPE, "%s: bad shape tokens=%lld seqs=%d q_heads=%d", what, (long long)tokens, seqs, q_heads);
+    if (q_heads % cache->kv_heads) return set_error(c, WF_ERR_SHAPE, "%s: %d query heads over %d kv heads", what, q_heads, cache->kv_heads);
+    if (q_heads / cache->kv_heads > 128) return set_error(c, WF_ERR_TOO_LARGE, "%s: more than 128 query heads for each kv head", what);
+    if (q_stride < (int64_t)q_heads * cache->head_dim || q_stride % 8) return set_error(c, WF_ERR_SHAPE, "%s: q_stride %lld", what, (long long)q_stride);
+    return WF_OK;
+}
+template <class... Params, class... Args>
+inline int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) return cuda_status(c, e, what);
+    c->launches++;
+    return WF_OK;
+}
+
+// bf16 [z][y][x] with the given distances (elements) between y and z; boxes of 64 elements x by x bz, 128-byte swizzle, zeros outside
+inline int encode_rows(Context* c, CUtensorMap* map, const void* base, int64_t x, int64_t y, int64_t z, int64_t y_apart, int64_t z_apart, int by, int bz) {
+    const cuuint64_t dims[3] = {(cuuint64_t)x, (cuuint64_t)y, (cuuint64_t)z}, strides[2] = {(cuuint64_t)y_apart * 2, (cuuint64_t)z_apart * 2};
+    const cuuint32_t box[3] = {64, (cuuint32_t)by, (cuuint32_t)bz}, step[3] = {1, 1, 1};
+    const EncodeTiledFn encode = encode_tiled_fn();
+    if (!encode) return set_error(c, WF_ERR_NO_DEVICE, "the driver has no cuTensorMapEncodeTiled");
+    const CUresult r = encode(map, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(base), dims, strides, box, step, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                              CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return set_error(c, WF_ERR_CUDA_BASE + (int)cudaErrorInvalidValue, "cuTensorMapEncodeTiled failed: %d", (int)r);
+    return WF_OK;
+}
+inline int encode_cache(Context* c, CUtensorMap* map, const bf16* base, const CacheView& v, int box_rows) {
+    if (v.page_shift == 0) return encode_rows(c, map, base, v.dim, v.kv_heads, v.pages, v.dim, (int64_t)v.kv_heads * v.dim, 1, box_rows);
+    return encode_rows(c, map, base, v.dim, 1, (v.pages * v.kv_heads) << v.page_shift, v.dim, v.dim, 1, box_rows);
+}
+inline bool rows_of_sectors(const bf16* out, int dim) { return reinterpret_cast<uintptr_t>(out) % 32 == 0 && dim % 16 == 0; }
+inline int dim_chunks(int dim) { return (dim + 63) / 64; }
+
+// Where the pieces of cut units go; `extra` bytes behind them, whose address *more is.
+inline int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cuts, int64_t extra = 0, uint8_t** more = nullptr) {
+    GemvScratch& scratch = c->gemv_scratch[s];
+    const int64_t head = (c->sm_count * (int64_t)sizeof(TreeCut) + 255) & ~255LL, pieces = head + ((floats * (int64_t)sizeof(float) + 255) & ~255LL), bytes = pieces + extra;
+    if (bytes > scratch.attn_bytes) {
+        const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
+        if (rc != WF_OK) return rc;
+        scratch.d_attn.reset();
+        scratch.attn_bytes = 0;
+        WF_CUDA(c, make_shared_device(c, scratch.d_attn, (size_t)bytes));
+        scratch.attn_bytes = bytes;
+    }
+    cuts->cuts = reinterpret_cast<TreeCut*>(scratch.d_attn.get());
+    cuts->pieces = reinterpret_cast<float*>(scratch.d_attn.get() + head);
+    if (more) *more = scratch.d_attn.get() + pieces;
+    return WF_OK;
+}
+template <int KIND> inline int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
+    return launch_attention(c, "tree_attention", tree_join_kernel<KIND>, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
+}
+// The kernel for few rows.  units: sequences (lists) times heads, with up to unit_rows rows and unit_keys keys each.
+template <int CHUNKS, int MT, int KIND> inline int launch_tree(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
+    const char* what = "tree_attention";
+    typedef TreeShape<CHUNKS, MT> Shape;
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    const int64_t tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
+    units *= (unit_rows + Shape::ROWS - 1) / Shape::ROWS;
+    TreeTiles t{};
+    t.p = p;
+    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
+    t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
+    t.c.dim = Shape::DIM;
+    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
+    CUtensorMap k, v;
+    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
+    if (rc != WF_OK) return rc;
+    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
+    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join<KIND>(c, p, t.c, grid, Shape::ROWS, s) : rc;
+}
+
+// The prompt kernel on the rows of trees.
+// units: sequences (groups) times heads, with up to unit_tokens tokens and unit_keys keys each.
+template <int CHUNKS, int KIND> inline int launch_wide_tree(Context* c, const TreeParams& p, int64_t units, int64_t unit_tokens, int64_t unit_keys, cudaStream_t s) {
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(prompt_tiles_kernel<CHUNKS, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, PromptShape<CHUNKS>::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    PromptTiles t{};
+    t.tree = p;
+    t.p.cache = p.cache;
+    t.p.q = p.q, t.p.out = p.out, t.p.q_stride = p.q_stride;
+    t.p.tables = p.tables, t.p.table_stride = p.table_stride;
+    t.p.q_heads = p.q_heads, t.p.group = p.group;
+    t.p.scale_log2 = p.scale_log2;
+    t.p.status = p.status;
+    t.tile_tokens = PA_ROWS / p.group;
+    t.box_rows = std::min(PA_KEYS, 1 << p.cache.page_shift);
+    t.wide_rows = rows_of_sectors(p.out, p.cache.dim);
+    const int64_t tiles = (unit_keys + PA_KEYS - 1) / PA_KEYS;
+    // groups: all of their tokens are p.tokens, and each may have a block that is not full
+    if (KIND == ATTEND_PREFIX) units += p.tokens / (2 * t.tile_tokens) * p.cache.kv_heads;
+    else units *= (unit_tokens + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens);
+    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, PA_CUT_TILES, PA_CUT_ANYWAY);
+    t.c.piece_rows = unit_tokens <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;
+    t.c.tile_rows = t.tile_tokens * p.group;
+    t.c.tile_room = PA_ROWS;
+    t.c.dim = CHUNKS * 64;
+    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * t.c.piece_rows * (t.c.dim + 2) : 0, &t.c);
+    CUtensorMap q, k, v;
+    if (rc == WF_OK) rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
+    if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, t.box_rows);
+    if (rc != WF_OK) return rc;
+    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
+    rc = launch_attention(c, "tree_attention", prompt_tiles_kernel<CHUNKS, KIND>, grid, PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join<KIND>(c, p, t.c, grid, (int)std::min<int64_t>(unit_tokens, 2 * t.tile_tokens) * p.group, s) : rc;
+}
+
+}  // namespace wf
+
+#define ATTENTION_ENTER(ctxh)                                              \
+    Context* c = get_context(ctxh);                                        \
+    if (!c) return WF_ERR_INVALID_HANDLE;                                  \
+    ScopedLock _lk(c);                                                     \
+    if (!_lk.ok) return WF_ERR_BUSY;                                       \
+    WF_CUDA(c, cudaSetDevice(c->device));                                  \
+    cudaStream_t s = resolve_stream(c, stream)

@@ -13,7 +13,8 @@ struct alignas(16) TreeCut {
     int first_cta, last_cta;       // that have pieces of it; first_cta < 0: none begins in this CTA
     int row0, rows, context, seq;  // of the sequence
     int head, first, count;        // kv head; which of the sequence's rows * group, row by row
-    int pad[3];
+    int news;                      // of a list
+    int pad[2];
 };
 struct TreeCuts {
     TreeCut* cuts;      // [CTAs]
@@ -42,13 +43,15 @@ struct LineUnit {
 
 #ifdef __CUDACC__
 // Walks the share of this CTA, the whole warp together: f(unit) for every unit that has tiles in it, until it answers false.
-template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, F f) {
-    const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
-    auto tiles_of = [&](const TreeSeq& q) { return max(1, (q.context + q.rows + KEYS - 1) / KEYS); };
+template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, F f) {
+    // a list is a kv head's
+    const int lane = threadIdx.x & 31, heads = KIND == ATTEND_LISTS ? 1 : p.cache.kv_heads, group = p.group;
+    const int seqs = KIND == ATTEND_LISTS ? (int)p.tokens * p.cache.kv_heads : KIND == ATTEND_PREFIX ? p.n_groups : p.seqs;
+    auto tiles_of = [&](const TreeSeq& q) { return max(1, (KIND == ATTEND_TREE ? q.context + q.rows + KEYS - 1 : keys_of<KIND>(q) + KEYS - 1) / KEYS); };
     auto blocks_of = [&](const TreeSeq& q) { return (q.rows * group + unit_rows - 1) / unit_rows; };
     auto info = [&](int s) {
         TreeSeq q{};
-        if (s < p.seqs) q = tree_seq(p, s);
+        if (s < seqs) q = seq_of<KIND>(p, s);
         return q;
     };
     auto line_of = [&](const TreeSeq& q) { return q.rows == 0 ? 0 : (int64_t)(tiles_of(q) + unit_tiles) * (heads * blocks_of(q)); };
@@ -56,7 +59,7 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const Tre
     TreeSeq mine = info(lane);
     int64_t line64 = line_of(mine), total64 = line64;
 #pragma unroll 1
-    for (int s0 = 32; s0 < p.seqs; s0 += 32) total64 += line_of(info(s0 + lane));
+    for (int s0 = 32; s0 < seqs; s0 += 32) total64 += line_of(info(s0 + lane));
 #pragma unroll
     for (int o = 16; o > 0; o >>= 1) total64 += __shfl_xor_sync(0xFFFFFFFFu, total64, o);
     if (total64 >= (1LL << 31)) {  // 3e10 keys: no cache holds them, some table says so
@@ -68,7 +71,7 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const Tre
     auto cta_of = [&](int x) { return x < more * (share + 1) ? x / (share + 1) : more + (x - more * (share + 1)) / share; };
     int at = 0;  // where the lanes' sequences begin on the line
 #pragma unroll 1
-    for (int s0 = 0; s0 < p.seqs && at < end; s0 += 32) {
+    for (int s0 = 0; s0 < seqs && at < end; s0 += 32) {
         if (s0) {
             mine = info(s0 + lane);
             line64 = line_of(mine);
@@ -92,6 +95,12 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const Tre
             u.q.context = __shfl_sync(0xFFFFFFFFu, mine.context, l);
             u.q.place.table = p.tables + (size_t)(s0 + l) * p.table_stride;
             u.q.place.first = 0;
+            if (KIND == ATTEND_LISTS) u.q.news = __shfl_sync(0xFFFFFFFFu, mine.news, l);
+            if (KIND == ATTEND_OWN) {
+                u.q.prefix = __shfl_sync(0xFFFFFFFFu, mine.prefix, l);
+                u.q.place.table += u.q.prefix >> p.cache.page_shift;
+            }
+            if (KIND == ATTEND_PREFIX) u.q.place.table = reinterpret_cast<const int*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(mine.place.table), l));
             u.seq = s0 + l;
             u.tiles = tiles_of(u.q);
             const int start = base + __shfl_sync(0xFFFFFFFFu, up_to - line, l), blocks = blocks_of(u.q), length = u.tiles + unit_tiles;
@@ -108,6 +117,7 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const Tre
                 if (u.to <= u.from) continue;
                 u.head = unit / blocks;
                 u.first = (unit - u.head * blocks) * unit_rows;
+                if (KIND == ATTEND_LISTS) u.head = u.seq % p.cache.kv_heads;
                 const bool whole = u.from == 0 && u.to == u.tiles;
                 u.first_cta = whole ? (int)blockIdx.x : cta_of(u_at + unit_tiles);
                 u.last_cta = whole ? (int)blockIdx.x : cta_of(u_at + length - 1);
@@ -119,11 +129,12 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_line(const Tre
 }
 
 // What a CTA leaves for tree_join_kernel: the unit that begins in its share and does not end there, if there is one.
-__device__ __forceinline__ void leave_cut(const TreeCuts& c, const LineUnit& u, int count) {
+template <int KIND> __device__ __forceinline__ void leave_cut(const TreeCuts& c, const LineUnit& u, int count) {
     TreeCut& cut = c.cuts[blockIdx.x];
     cut.first_cta = u.first_cta, cut.last_cta = u.last_cta;
     cut.row0 = u.q.row0, cut.rows = u.q.rows, cut.context = u.q.context, cut.seq = u.seq;
     cut.head = u.head, cut.first = u.first, cut.count = count;
+    if (KIND == ATTEND_LISTS) cut.news = u.q.news;
 }
 
 __device__ __forceinline__ float line_ex2(float x) {
@@ -137,7 +148,7 @@ __device__ __forceinline__ float line_ex2(float x) {
 // 12.4 / 13.0 / 12.8 us for one token of 32 heads at 2000 tokens (the kernel before it included), 25.2 / 22.8 / 22.0 / 23.1 / 23.0 of 8 heads at 20,000, 22.4 / 21.6 / 22.0 /
 // 21.8 / 22.9 for 8 sequences of 0 to 3000 with up to 24 drafts; CTAs of 2 / 8 / 16 warps, the last of these: 24.5 / 22.3 / 22.9.
 constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 4;
-__global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ TreeCuts c) {
+template <int KIND> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ TreeCuts c) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeCut cut = c.cuts[blockIdx.x];
@@ -172,20 +183,28 @@ __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid
             x.x += v[i].x * take, x.y += v[i].y * take, x.z += v[i].z * take, x.w += v[i].w * take;
         }
     }
-    const float inv = sum == 0.f ? 0.f : 1.f / sum;
     const int d = p.cache.dim, token = p.token_of(cut.first + row), head = cut.head * p.group + cut.first + row - token * p.group;
-    bf16* const to = p.out + ((size_t)(cut.row0 + token) * p.q_heads + head) * d;
+    const size_t place = (size_t)(cut.row0 + token) * p.q_heads + head;
+    if (KIND == ATTEND_PREFIX) {  // the keys behind the prefix are another kernel's
+        if (mine) *reinterpret_cast<float4*>(p.state + place * p.state_dim + 4 * lane) = x;
+        if (lane == 0) p.state_maxima()[place] = top, p.state_weights()[place] = sum;
+        return;
+    }
+    if (KIND == ATTEND_OWN && cut.context >= 0 && p.prefix_of[cut.seq].x > 0) {
+        const float4 v = mine ? ld_once(reinterpret_cast<const float4*>(p.state + place * p.state_dim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
+        const float m = ld_once(p.state_maxima() + place), l = ld_once(p.state_weights() + place);
+        const float grown = fmaxf(top, m), ref = grown == -INFINITY ? 0.f : grown, keep = line_ex2((top - ref) * p.scale_log2), take = line_ex2((m - ref) * p.scale_log2);
+        top = grown;
+        sum = sum * keep + l * take;
+        x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
+    }
+    const float inv = sum == 0.f ? 0.f : 1.f / sum;
+    bf16* const to = p.out + place * d;
     if (4 * lane < d) *reinterpret_cast<uint2*>(to + 4 * lane) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
     // Key by key where an Inf or a NaN may have come from a key that the row does not see, or from a page that is not in the cache.
     const float largest = fmaxf(fmaxf(fabsf(x.x), fabsf(x.y)), fmaxf(fabsf(x.z), fabsf(x.w)));
     const bool odd = !(sum < INFINITY) || scores_too_large(top, p.scale_log2) || !(largest < INFINITY) || x.x != x.x || x.y != x.y || x.z != x.z || x.w != x.w;
-    if (__any_sync(0xFFFFFFFFu, odd)) {
-        KeyPlace place;
-        place.table = p.tables + (size_t)cut.seq * p.table_stride;
-        place.first = 0;
-        attend_row(p.cache, place, p.q + (size_t)(cut.row0 + token) * p.q_stride + (size_t)head * d, to, cut.head, cut.context < 0 ? 0 : cut.context + cut.rows, p.scale_log2,
-                   p.status, SeesAncestors{cut.context, ancestors_of(p, cut.row0 + token, token) & ((uint64_t)-1 >> (64 - cut.rows))});
-    }
+    if (__any_sync(0xFFFFFFFFu, odd)) attend_again<KIND>(p, cut, token, cut.head, p.q + (size_t)(cut.row0 + token) * p.q_stride + (size_t)head * d, to);
 }
 #endif
 

@@ -44,6 +44,8 @@ struct PromptItem {
     int context;           // tree: tokens before the new ones, -1: a sequence that cannot be
     int piece;             // tree: the unit is cut; 1: this piece is not the one it begins with, 2: it is
     int last;              // no more work (1), or a wait ran out
+    int prefix;            // own keys: tokens before them
+    const int* table;      // prefixes and own keys: of the unit
     // key tiles of group g
     __device__ __forceinline__ int tiles(int g) const { return split ? (n0 - from - g + 1) >> 1 : max(0, (g ? n1 : n0) - from); }
     __device__ __forceinline__ int all() const { return max(n0, n1) - from; }
@@ -347,13 +349,27 @@ constexpr int PA_UNIT_TILES = 3;
 // When units are cut (line_is_cut).  Microseconds whole / cut, 12 drafts of 32 / 8 heads of 128: 16 sequences with 700, 1000, 1400, 1800 tokens 16.3 / 23.9, 19.6 / 27.4,
 // 26.5 / 32.7, 31.2 / 37.7; 8 with 1000, 1400 17.0 / 19.2, 22.5 / 22.4; 20 with 1000, 1400 31.9 / 30.7, 42.8 / 37.9; 4 with 600, 1000 12.8 / 14.5, 15.9 / 15.7.
 constexpr int PA_CUT_TILES = 6, PA_CUT_ANYWAY = 15;
-template <class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
+template <int KIND, class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
     const TreeParams& p = t.tree;
     bool cut = false;
-    const bool ok = walk_line<PA_KEYS>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+    if (KIND == ATTEND_PREFIX) {  // for the kernel behind this one: which prefix a sequence has
+        const int lane = threadIdx.x & 31;
+        for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
+            const GroupSeqs of = group_seqs(p, g);
+            for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(of.prefix, of.first);
+        }
+        if (blockIdx.x == 0) {  // those that no group has
+            const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
+            for (int s = lane; s < before; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+            for (int s = behind + lane; s < p.seqs; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+        }
+    }
+    const bool ok = walk_line<PA_KEYS, KIND>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
         PromptItem it{};
         it.seq = u.seq, it.head = u.head, it.row0 = u.q.row0, it.rows = u.q.rows, it.context = u.q.context;
-        it.keys = u.q.context < 0 ? 0 : u.q.context + u.q.rows;
+        it.keys = keys_of<KIND>(u.q);
+        if (KIND != ATTEND_TREE) it.table = u.q.place.table;
+        if (KIND == ATTEND_OWN) it.prefix = u.q.prefix;
         it.token0 = u.first / p.group;
         it.from = u.from;
         it.n0 = u.to;
@@ -362,7 +378,7 @@ template <class F> __device__ __forceinline__ bool tree_items(const PromptTiles&
         it.piece = u.from == 0 && u.to == u.tiles ? 0 : u.from == 0 ? 2 : 1;
         if (it.piece == 2) {
             cut = true;
-            if ((threadIdx.x & 31) == 0) leave_cut(t.c, u, min(2 * t.tile_tokens, it.rows - it.token0) * p.group);
+            if ((threadIdx.x & 31) == 0) leave_cut<KIND>(t.c, u, min(2 * t.tile_tokens, it.rows - it.token0) * p.group);
         }
         return f(it);
     });
@@ -370,9 +386,10 @@ template <class F> __device__ __forceinline__ bool tree_items(const PromptTiles&
     return ok;
 }
 
-template <int CHUNKS, bool TREE>
+template <int CHUNKS, int KIND>
 __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __grid_constant__ PromptTiles t, const __grid_constant__ CUtensorMap q_map,
                                                                     const __grid_constant__ CUtensorMap k_map, const __grid_constant__ CUtensorMap v_map) {
+    constexpr bool TREE = KIND != ATTEND_PROMPT, PREFIX = KIND == ATTEND_PREFIX;
     constexpr int DIM = CHUNKS * 64, STAGES = PromptShape<CHUNKS>::STAGES, STAGE_BYTES = PromptShape<CHUNKS>::STAGE_BYTES;
     constexpr uint32_t IDESC = 1u << 4 | 1u << 7 | 1u << 10 | (uint32_t)(PA_ROWS / 16) << 24;  // fp32 += bf16 x bf16, 128 rows
     constexpr uint32_t IDESC_QK = IDESC | (uint32_t)(PA_KEYS / 8) << 17, IDESC_PV = IDESC | 1u << 16 | (uint32_t)(DIM / 8) << 17;
@@ -433,7 +450,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             const bool mine = r < group * tile_tokens && token < it.rows;
             const int last_key = it.keys - it.rows + token;  // prompt: that the row sees
             const int all_see = TREE ? it.context - 1 : it.keys - it.rows + first + (warp & 3) * 32 / group;  // that every row of this warp sees
-            const uint64_t word = TREE && mine && it.keys > 0 ? ancestors_of(t.tree, it.row0 + token, token) & ((uint64_t)-1 >> (64 - it.rows)) : 0;
+            const uint64_t word = TREE && mine && it.keys > 0 ? sees_of<KIND>(t.tree, it.row0 + token, token, it.rows) : 0;
             float m = -INFINITY, l = 0.f;
             int j = it.from + (it.split ? g : 0);  // the key tile
             for (int i_tile = 0; i_tile < n; i_tile++, j += step) {
@@ -570,15 +587,34 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             }
 #pragma unroll
             for (int e = 0; e < 2; e++) o_phase[e] ^= it.tiles(e) > 0;  // the other group's, too
-            const bool whole = !(TREE && it.piece);
+            const bool whole = !(TREE && it.piece) && !PREFIX;  // rows go to the output
+            float before = 0.f;  // what the sums over the prefix count
+            const float* before_sums = nullptr;
+            if (KIND == ATTEND_OWN && whole && it.prefix > 0 && mine) {
+                const size_t at = (size_t)row * p.q_heads + head;
+                const float m_before = ld_once(t.tree.state_maxima() + at), l_before = ld_once(t.tree.state_weights() + at);
+                const float grown = fmaxf(top, m_before), ref = grown == -INFINITY ? 0.f : grown, less = ex2((top - ref) * scale);
+                before_sums = t.tree.state + at * t.tree.state_dim;
+                before = ex2((m_before - ref) * scale);
+                top = grown;
+                keep *= less, take *= less;
+                l = l * less + l_before * before;
+            }
             if (n > 0) {
                 const float inv = l == 0.f ? 0.f : __frcp_rn(l);
                 const float2 f0 = make_float2(whole ? keep * inv : keep, whole ? keep * inv : keep), f1 = make_float2(whole ? take * inv : take, whole ? take * inv : take);
                 const int rows = t.c.piece_rows, at = it.split ? r : g * PA_ROWS + r;
                 float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
+                const bool to_state = PREFIX && !it.piece;
+                float* const sums = to_state ? t.tree.state + ((size_t)row * p.q_heads + head) * DIM : piece + (size_t)at * DIM;
                 if (!whole && r < group * tile_tokens && !(halves && g)) {
-                    piece[rows * DIM + at] = top;
-                    piece[rows * (DIM + 1) + at] = l;
+                    if (!to_state) {
+                        piece[rows * DIM + at] = top;
+                        piece[rows * (DIM + 1) + at] = l;
+                    } else if (mine) {
+                        t.tree.state_maxima()[(size_t)row * p.q_heads + head] = top;
+                        t.tree.state_weights()[(size_t)row * p.q_heads + head] = l;
+                    }
                 }
                 // Few instructions and a small loop: it runs once an item, by one warp a scheduler at about three cycles an instruction.  (Transposed among four lanes, so that
                 // a store touches 8 rows and not 32, it took twice as long.)
@@ -602,8 +638,17 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     if (TREE && !whole) {
                         if (mine)
 #pragma unroll
-                            for (int i = 0; i < 4; i++) store_32(piece + (size_t)at * DIM + c + 8 * i, o + 8 * i);
+                            for (int i = 0; i < 4; i++) store_32(sums + c + 8 * i, o + 8 * i);
                         continue;
+                    }
+                    if (KIND == ATTEND_OWN && before_sums) {
+                        const float2 f2 = make_float2(before * inv, before * inv);
+#pragma unroll
+                        for (int i = 0; i < 8; i++) {
+                            const float4 v = ld_once(reinterpret_cast<const float4*>(before_sums + c) + i);
+                            x[2 * i] = fma2(make_float2(v.x, v.y), f2, x[2 * i]);
+                            x[2 * i + 1] = fma2(make_float2(v.z, v.w), f2, x[2 * i + 1]);
+                        }
                     }
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -650,10 +695,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 place.first = it.row0;
                 const bf16* q_row = p.q + (size_t)(it.row0 + tok) * p.q_stride + (size_t)hd * d;
                 bf16* out_row = p.out + ((size_t)(it.row0 + tok) * p.q_heads + hd) * d;
-                if (TREE)
-                    attend_row(p.cache, place, q_row, out_row, it.head, it.keys, p.scale_log2, p.status,
-                               SeesAncestors{it.context, ancestors_of(t.tree, it.row0 + tok, tok) & ((uint64_t)-1 >> (64 - it.rows))});
-                else attend_row(p.cache, place, q_row, out_row, it.head, min(it.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
+                if (TREE && !PREFIX) attend_again<KIND>(t.tree, it, tok, it.head, q_row, out_row);
+                else if (!TREE) attend_row(p.cache, place, q_row, out_row, it.head, min(it.keys, last + 1), p.scale_log2, p.status, SeesUpTo{last});
             }
         }
     } else if (warp == PA_LOAD_WARP) {
@@ -663,7 +706,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
         const int boxes = PA_KEYS / t.box_rows;
         while (items.next(sh, it, failed)) {
             const int n = it.all();
-            const int* table = p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
+            const int* table = KIND == ATTEND_PREFIX || KIND == ATTEND_OWN ? it.table : p.tables ? p.tables + (size_t)it.seq * p.table_stride : nullptr;
             // the rows of a key tile's boxes, a lane each, and how many there are
             auto find = [&](int j, int& z) {
                 if (!table) {
@@ -871,7 +914,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
             return true;
         };
         if (TREE) {
-            tree_items(t, announce);
+            tree_items<KIND>(t, announce);
         } else {
             PromptSchedule schedule{t};
             schedule.begin();

@@ -49,6 +49,7 @@ struct alignas(16) TreeSegment {
     int from, to, tiles;           // of the unit
     int slot, phase;               // of the first tile in the ring
     int last;                      // no more work
+    int news, prefix;              // lists; own keys
 };
 
 struct TreeTiles {
@@ -102,7 +103,7 @@ template <int CHUNKS, int MT> struct TreeShared {
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
-template <int CHUNKS, int MT>
+template <int CHUNKS, int MT, int KIND>
 __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS, MT>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
     typedef TreeShape<CHUNKS, MT> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
@@ -112,8 +113,8 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
     bool cut = false;  // a unit that begins here goes on in the next share
-    const bool ok = walk_line<TA_KEYS>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
-        const int keys = u.q.context < 0 ? 0 : u.q.context + u.q.rows, count = min(ROWS, u.q.rows * group - u.first);
+    const bool ok = walk_line<TA_KEYS, KIND>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+        const int keys = keys_of<KIND>(u.q), count = min(ROWS, u.q.rows * group - u.first);
         // the page of a lane's tile, asked for before anything is waited for
         const int* const table = u.q.place.table;
         int tile = u.from + lane, page = 0;
@@ -123,8 +124,10 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
             TreeSegment& d = sh->segments[seg];
             d.row0 = u.q.row0, d.rows = u.q.rows, d.context = u.q.context, d.seq = u.seq, d.head = u.head, d.first = u.first;
             d.from = u.from, d.to = u.to, d.tiles = u.tiles, d.slot = slot, d.phase = (int)phase ^ 1, d.last = 0;
+            if (KIND == ATTEND_LISTS) d.news = u.q.news;
+            if (KIND == ATTEND_OWN) d.prefix = u.q.prefix;
             g_mbar_arrive(&sh->seg_full[seg]);
-            if (u.from == 0 && u.to < u.tiles) leave_cut(t.c, u, count);
+            if (u.from == 0 && u.to < u.tiles) leave_cut<KIND>(t.c, u, count);
         }
         cut |= u.from == 0 && u.to < u.tiles;
         __syncwarp();
@@ -178,7 +181,7 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
     return true;
 }
 
-template <int CHUNKS, int MT>
+template <int CHUNKS, int MT, int KIND>
 __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
     typedef TreeShape<CHUNKS, MT> Shape;
@@ -209,7 +212,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= TA_WARPS) {
         asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_load<CHUNKS, MT>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
+        if (!tree_load<CHUNKS, MT, KIND>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
@@ -235,7 +238,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         }
         const TreeSegment w = sh->segments[seg];
         if (w.last) break;
-        const int keys = w.context < 0 ? 0 : w.context + w.rows, count = min(ROWS, w.rows * group - w.first);
+        const int keys = keys_of<KIND>(w), count = min(ROWS, w.rows * group - w.first);
         const uint32_t q_at = q_smem + (uint32_t)(seg * Shape::Q_BYTES) + q_row;
         auto load_q = [&](int i, int k, uint32_t(&a)[4]) { ldmatrix4(q_at + (uint32_t)(i * 16 * DIM * 2) + (uint32_t)(((2 * k + (matrix >> 1)) ^ mrow) << 4), a); };
         uint32_t q[MT][Q_KEPT ? DIM / 16 : 1][4];
@@ -284,7 +287,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll
                     for (int e = 0; e < 2; e++) {
                         const int r = 16 * i + g + 8 * e, token = p.token_of(w.first + r);
-                        const uint64_t sees = r < count && keys > 0 ? ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows)) : 0;
+                        const uint64_t sees = r < count && keys > 0 ? sees_of<KIND>(p, w.row0 + token, token, news_of<KIND>(w)) : 0;
 #pragma unroll
                         for (int c = 0; c < 4; c++) {
                             const int j = key0 + 8 * (c >> 1) + 2 * quad + (c & 1) - w.context;
@@ -435,6 +438,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                 const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
                 x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
             }
+            if (KIND == ATTEND_OWN && whole && w.prefix > 0) {
+                const int token = p.token_of(w.first + r);
+                const size_t place = (size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group;
+                const float4 v = ld_once(reinterpret_cast<const float4*>(p.state + place * p.state_dim) + n);
+                const float m_before = ld_once(p.state_maxima() + place), l_before = ld_once(p.state_weights() + place);
+                const float grown = fmaxf(top, m_before), ref2 = grown == -INFINITY ? 0.f : grown, keep = line_ex2((top - ref2) * scale), take = line_ex2((m_before - ref2) * scale);
+                top = grown;
+                sum = sum * keep + l_before * take;
+                x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
+            }
             if (whole) {
                 if (4 * n < d) store(r, 4 * n, x, sum, top);
             } else {
@@ -451,15 +464,11 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             // An Inf or a NaN in a row's sums may have come from a key that it does not see (0 x Inf), or from a page that is not in the cache: key by key.
             ta_sync();
             if (tid == 0) sh->odd_rows = 0;
-            KeyPlace place;
-            place.table = p.tables + (size_t)w.seq * p.table_stride;
-            place.first = 0;
 #pragma unroll 1
             for (int r = warp; r < count; r += TA_WARPS) {
                 if (!(odd >> r & 1)) continue;
                 const int token = p.token_of(w.first + r), h = w.head * group + (w.first + r) - token * group;
-                attend_row(p.cache, place, p.q + (size_t)(w.row0 + token) * p.q_stride + (size_t)h * d, p.out + ((size_t)(w.row0 + token) * p.q_heads + h) * d, w.head, keys,
-                           scale, p.status, SeesAncestors{w.context, ancestors_of(p, w.row0 + token, token) & ((uint64_t)-1 >> (64 - w.rows))});
+                attend_again<KIND>(p, w, token, w.head, p.q + (size_t)(w.row0 + token) * p.q_stride + (size_t)h * d, p.out + ((size_t)(w.row0 + token) * p.q_heads + h) * d);
             }
         }
     }
