@@ -331,6 +331,33 @@ class KvCache:
             row[:len(s.pages)] = s.pages
         return out
 
+    def shared_prefixes(self, sequences: Seq[Sequence], tokens: Optional[Seq[int]] = None) -> Tuple[np.ndarray, np.ndarray]:
+        """What SharedPrefixAttention is to be given for these sequences, in this order: groups i32 [n + 1] and prefix tokens i32 [n].  Neighbours that begin with the same pages
+        form a group; of all ways to cut the line of sequences into groups it is the one that leaves the fewest pages to be read.  tokens: the contexts (None: all tokens)."""
+        size, n = self.page_tokens, len(sequences)
+        tokens = [s.tokens for s in sequences] if tokens is None else tokens
+        whole = [min(len(s.pages), t // size) for s, t in zip(sequences, tokens)]
+        common = []  # whole pages that a sequence and the one before it begin with
+        for i in range(1, n):
+            m = min(whole[i - 1], whole[i])
+            a, b = np.array(sequences[i - 1].pages[:m]), np.array(sequences[i].pages[:m])
+            other = np.flatnonzero(a != b)
+            common.append(int(other[0]) if len(other) else m)
+        saved, begin = [0] * (n + 1), [0] * (n + 1)  # of the first i sequences; where the last group of them begins
+        for i in range(1, n + 1):
+            saved[i], begin[i], least = saved[i - 1], i - 1, None
+            for j in range(i - 2, -1, -1):
+                least = common[j] if least is None else min(least, common[j])
+                if least == 0:
+                    break
+                if saved[j] + least * (i - j - 1) > saved[i]:
+                    saved[i], begin[i] = saved[j] + least * (i - j - 1), j
+        groups = [n]
+        while groups[0]:
+            groups.insert(0, begin[groups[0]])
+        prefix = [min(common[a:b - 1]) * size if b - a > 1 else 0 for a, b in zip(groups, groups[1:])]
+        return np.array(groups, np.int32), np.array(prefix, np.int32)
+
     def fork(self, sequences: Seq[Sequence], stream: int = 0) -> List[Sequence]:
         """A second sequence for each, with the same tokens: whole pages shared, part-full last pages copied, all in one call on `stream`."""
         part = [s for s in sequences if s.tokens % self.page_tokens]
@@ -459,7 +486,8 @@ class PageBounds:
                 codes, scales = DeviceTensor(self._owned[0], (*shape, 2, cache.head_dim), "i8", owner=ctx), DeviceTensor(self._owned[1], shape, "f32", owner=ctx)
             self._addresses = _typed("codes", codes, "i8", *shape, 2, cache.head_dim), _typed("scales", scales, "f32", *shape)
         except BaseException:
-            self.close()
+            for p in self._owned:
+                ctx.free(p)
             raise
         self.codes, self.scales = codes, scales
 

@@ -5,7 +5,8 @@
     logits = Whead . rms_norm(h)
 
 Prompts of several sequences go through together (``prefill``: tensor-core GEMMs and PromptAttention), new tokens by ``step``: one for each sequence, or a
-tree of drafted ones of which ``keep`` retains a path (decode GEMVs, TreeAttention, compaction of the cache).  ``python -m
+tree of drafted ones of which ``keep`` retains a path (decode GEMVs, TreeAttention, compaction of the cache).  New tokens may read the prefix that neighbouring
+sequences share (forks) once for all of them (``share_prefixes``), or a few pages of a long context that promise the largest scores (``selected_pages``).  ``python -m
 warpforge_b200.generate`` runs it on seeded synthetic weights and prints tokens per second.
 """
 from __future__ import annotations
@@ -51,10 +52,19 @@ class DecoderSpec:
 
 class Decoder:
     """Seeded synthetic weights; `max_tokens` rows of activations, a cache of `pages` pages.  A call that is refused or fails leaves the sequences as long
-    as they were."""
+    as they were.
 
-    def __init__(self, context: CudaContext, spec: DecoderSpec, pages: int, page_tokens: int = 64, max_tokens: int = 512, max_sequences: int = 16, seed: int = 1):
+    share_prefixes: ``step`` reads what neighbours among its sequences have in common once for all of them.  selected_pages: in ``step`` a new token reads, for every kv head, so many pages
+    at most: the first `first_pages`, those of the last `recent_tokens` tokens, those of the new ones, and the ones between whose bounds promise the largest scores (0: all pages)."""
+
+    def __init__(self, context: CudaContext, spec: DecoderSpec, pages: int, page_tokens: int = 64, max_tokens: int = 512, max_sequences: int = 16, seed: int = 1,
+                 share_prefixes: bool = False, selected_pages: int = 0, first_pages: int = 1, recent_tokens: int = 64):
+        if selected_pages < 0 or first_pages < 0 or recent_tokens < 0 or (selected_pages and share_prefixes):
+            raise ValueError(f"selected_pages {selected_pages}, first_pages {first_pages}, recent_tokens {recent_tokens}; not together with share_prefixes")
         self.ctx, self.spec, self.max_tokens, self.max_sequences = context, spec, max_tokens, max_sequences
+        self.share_prefixes, self.selected_pages, self.first_pages, self.recent_tokens = share_prefixes, selected_pages, first_pages, recent_tokens
+        if selected_pages:
+            self._fits_lists(1, page_tokens)
         self.cache = A.KvCache(context, spec.layers, pages, page_tokens, spec.kv_heads, spec.head_dim)
         rng = np.random.default_rng(seed)
         self.host: Dict[str, np.ndarray] = {}
@@ -84,6 +94,11 @@ class Decoder:
         # what a call says about its tokens and sequences
         self._room = {n: max_tokens * size for n, size in (("ids", 8), ("positions", 4), ("slots", 8), ("ancestors", 8))}
         self._room.update({n: (max_sequences + 1) * 4 for n in ("offsets", "lens", "counts")}, tables=max_sequences * self._table_width * 4, kept=max_sequences * MAX_DRAFTS * 4)
+        if share_prefixes:
+            self._room.update(groups=(max_sequences + 1) * 4, prefixes=(max_sequences + 1) * 4)
+        self.bounds = A.PageBounds(self.cache) if selected_pages else None
+        if selected_pages:
+            self._room.update(before=(max_sequences + 1) * 4, lists=max_tokens * s.kv_heads * selected_pages * 4, list_lens=max_tokens * s.kv_heads * 8)
         self._room = {n: max(room, 16) for n, room in self._room.items()}
         self.buf.update({n: self._alloc(room) for n, room in self._room.items()})
 
@@ -135,7 +150,18 @@ class Decoder:
                 s.truncate(n)
             raise
 
-    # ---- the layers: `attend(layer, q, out)` is the attention of this call
+    # ---- pages that are selected
+    def _fits_lists(self, drafts: int, page_tokens: int) -> None:
+        need = self.first_pages + (self.recent_tokens + drafts + page_tokens - 2) // page_tokens + 1
+        if self.selected_pages < need:
+            raise ValueError(f"{drafts} new tokens of a sequence need {need} pages in any case, {self.selected_pages} are selected")
+
+    def _bound(self, tables: DeviceTensor, first: DeviceTensor, stop: DeviceTensor, most: int) -> None:
+        """The bounds of the pages that new tokens went to, in all layers."""
+        if self.bounds and most:
+            self.bounds.update(tables, first, stop, max_tokens=most)
+
+    # ---- the layers: `attend(layer, q, keys, values, out)` is the attention of this call
     def _layers(self, ids: np.ndarray, positions: np.ndarray, slots: np.ndarray, attend) -> None:
         ctx, lib, s, b, h = self.ctx, self.ctx._lib, self.spec, self.buf, self.ctx.handle
         n = len(ids)
@@ -158,7 +184,7 @@ class Decoder:
             gammas = {g: self._const(f"{g}_{layer}") for g in ("gamma_q", "gamma_k")} if s.qk_norm else {}
             A.QkNormRope(ctx, part("q", s.q_heads, "f32"), part("k", s.kv_heads, "f32"), part("v", s.kv_heads, "f32"), part("qb", s.q_heads, "bf16"), keys, values, pos,
                          self._const("rope"), slots=slot, norm=s.qk_norm, eps=s.eps, pairs=s.pairs, **gammas).run()
-            attend(part("qb", s.q_heads, "bf16"), keys, values, part("att", s.q_heads, "bf16"))
+            attend(layer, part("qb", s.q_heads, "bf16"), keys, values, part("att", s.q_heads, "bf16"))
             linear(w["wo"], b["att"], b["t"], N.WF_DTYPE_BF16)
             ctx._ck("wf_add", lib.wf_add(h, b["h"], b["t"], b["h"], n * s.d_model, 0))
             norm(self._const(f"gamma2_{layer}"))
@@ -190,7 +216,9 @@ class Decoder:
             tables, off = self._tables(sequences), self._send("offsets", offsets, "i32")
             total = self._send("lens", [s.tokens for s in sequences], "i32")
             self._layers(np.concatenate(prompts), np.concatenate(positions), slots,
-                         lambda q, k, v, out: A.PromptAttention(self.ctx, q, k, v, out, off, tables=tables, k_lens=total).run())
+                         lambda layer, q, k, v, out: A.PromptAttention(self.ctx, q, k, v, out, off, tables=tables, k_lens=total).run())
+            if self.bounds:
+                self._bound(tables, self._send("before", [s.tokens - n for s, n in zip(sequences, lens)], "i32"), total, max(lens, default=0))
             logits = self._logits(int(offsets[-1]))
         return [logits[a:b] for a, b in zip(offsets, offsets[1:])]
 
@@ -200,6 +228,8 @@ class Decoder:
         lens = [len(t) for t in tokens]
         if max(lens, default=0) > MAX_DRAFTS:
             raise ValueError(f"{max(lens)} new tokens of a sequence, at most {MAX_DRAFTS}")
+        if self.selected_pages and any(lens):
+            self._fits_lists(max(lens), self.cache.page_tokens)
         context = [s.tokens for s in sequences]
         words, depth = [], []
         for s, n in enumerate(lens):
@@ -217,11 +247,34 @@ class Decoder:
         with self._extended(sequences, lens) as slots:
             tables, off, ctx_lens = self._tables(sequences), self._send("offsets", offsets, "i32"), self._send("lens", context, "i32")
             anc = self._send("ancestors", np.array(words, np.uint64).view(np.int64), "i64")
-            self._layers(np.concatenate([np.asarray(t) for t in tokens]), np.concatenate(positions), slots,
-                         lambda q, k, v, out: A.TreeAttention(self.ctx, q, k, v, out, tables, ctx_lens, max_context=max(context), max_drafts=max(lens), q_offsets=off,
-                                                              ancestors=anc).run())
+            self._layers(np.concatenate([np.asarray(t) for t in tokens]), np.concatenate(positions), slots, self._attention(sequences, context, lens, tables, off, ctx_lens, anc))
+            if self.bounds:
+                self._bound(tables, ctx_lens, self._send("before", [s.tokens for s in sequences], "i32"), max(lens, default=0))
             logits = self._logits(int(offsets[-1]))
         return [logits[a:b] for a, b in zip(offsets, offsets[1:])]
+
+    def _attention(self, sequences: Seq[A.Sequence], context: List[int], lens: List[int], tables: DeviceTensor, off: DeviceTensor, ctx_lens: DeviceTensor, anc: DeviceTensor):
+        """What a step's new tokens do in every layer: attend to all that their sequences hold, with a common prefix read once, or to selected pages."""
+        ctx, drafts = self.ctx, dict(q_offsets=off, max_drafts=max(lens, default=1))
+        if self.selected_pages:
+            n = sum(lens)
+            lists = DeviceTensor(self.buf["lists"], (n, self.spec.kv_heads, self.selected_pages), "i32")
+            list_lens = DeviceTensor(self.buf["list_lens"], (n, self.spec.kv_heads, 2), "i32")
+
+            def selected(layer, q, k, v, out):
+                A.SelectPages(ctx, q, *self.bounds.layer(layer), tables, ctx_lens, lists, list_lens, page_tokens=self.cache.page_tokens, max_context=max(context, default=0), first=self.first_pages,
+                              recent=self.recent_tokens, tree=True, **drafts).run()
+                A.SelectedAttention(ctx, q, k, v, out, lists, list_lens, ancestors=anc).run()
+
+            return selected
+        if self.share_prefixes and sequences:
+            groups, prefix = self.cache.shared_prefixes(sequences, context)
+            if prefix.any():
+                d_groups, d_prefix = self._send("groups", groups, "i32"), self._send("prefixes", prefix, "i32")
+                own = max(c - int(p) for c, p in zip(context, np.repeat(prefix, np.diff(groups))))
+                return lambda layer, q, k, v, out: A.SharedPrefixAttention(ctx, q, k, v, out, tables, ctx_lens, d_groups, d_prefix, max_prefix=int(prefix.max()), max_own=own, ancestors=anc,
+                                                                           **drafts).run()
+        return lambda layer, q, k, v, out: A.TreeAttention(ctx, q, k, v, out, tables, ctx_lens, max_context=max(context), ancestors=anc, **drafts).run()
 
     def keep(self, sequences: Seq[A.Sequence], drafted: Seq[int], kept: Seq[Seq[int]]) -> None:
         """After ``step`` with drafted[s] tokens: those of kept[s] (ascending, a path of the tree) remain, moved up to the end of the context."""
@@ -239,6 +292,8 @@ class Decoder:
         self.cache.own(sequences, [(c + n, c + len(k)) for c, n, k in zip(context, still, kept)])
         tables, lens = self._tables(sequences), self._send("lens", context, "i32")
         self.cache.compact(tables, lens, self._send("kept", rows, "i32"), self._send("counts", [len(k) for k in kept], "i32"))
+        if self.bounds:
+            self._bound(tables, lens, self._send("before", [c + len(k) for c, k in zip(context, kept)], "i32"), max(len(k) for k in kept) if kept else 0)
         self.ctx.synchronize()
         for s, c, k in zip(sequences, context, kept):
             s.truncate(c + len(k))
@@ -249,6 +304,8 @@ class Decoder:
         for p in self._owned:
             self.ctx.free(p)
         self._owned = []
+        if self.bounds:
+            self.bounds.close()
         self.cache.close()
 
 
@@ -264,11 +321,15 @@ def main() -> None:
     ap.add_argument("--sequences", type=int, default=4)
     ap.add_argument("--prompt", type=int, default=512)
     ap.add_argument("--tokens", type=int, default=16)
+    ap.add_argument("--samples", type=int, default=1, help="continuations of each prompt, which share its pages")
+    ap.add_argument("--share-prefixes", action="store_true", help="read what they share once for all of them")
+    ap.add_argument("--selected-pages", type=int, default=0, help="pages that a new token reads (0: all)")
     a = ap.parse_args()
     spec = DecoderSpec(Q.QuantizationType[a.qtype], a.d_model, a.heads, a.kv_heads, a.d_model // a.heads, a.ffn, a.layers, a.vocab)
     ctx = CudaContext(0)
-    need = a.sequences * (-(-(a.prompt + a.tokens) // 64) + 1)
-    model = Decoder(ctx, spec, pages=need, max_tokens=a.sequences * a.prompt, max_sequences=a.sequences)
+    need = a.sequences * a.samples * (-(-(a.prompt + a.tokens) // 64) + 1)
+    model = Decoder(ctx, spec, pages=need, max_tokens=a.sequences * max(a.prompt, a.samples), max_sequences=a.sequences * a.samples, share_prefixes=a.share_prefixes,
+                    selected_pages=a.selected_pages)
     rng = np.random.default_rng(0)
     prompts = [rng.integers(0, a.vocab, a.prompt) for _ in range(a.sequences)]
     warm = [model.sequence() for _ in prompts]
@@ -279,13 +340,15 @@ def main() -> None:
     t0 = time.perf_counter()
     last = [int(np.argmax(x[-1])) for x in model.prefill(seqs, prompts)]
     t1 = time.perf_counter()
+    seqs = [s if i == 0 else s.fork() for s in seqs for i in range(a.samples)]
+    last = [(t + i) % a.vocab for t in last for i in range(a.samples)]  # each continues with another token
     out = [[t] for t in last]
     for _ in range(a.tokens - 1):
         last = [int(np.argmax(x[-1])) for x in model.step(seqs, [[t] for t in last])]
         for o, t in zip(out, last):
             o.append(t)
     t2 = time.perf_counter()
-    print(f"prompts: {a.sequences * a.prompt / (t1 - t0):.0f} tokens/s   decoding: {a.sequences * max(1, a.tokens - 1) / (t2 - t1):.0f} tokens/s   first tokens: {[o[:6] for o in out]}")
+    print(f"prompts: {a.sequences * a.prompt / (t1 - t0):.0f} tokens/s   decoding: {len(seqs) * max(1, a.tokens - 1) / (t2 - t1):.0f} tokens/s   first tokens: {[o[:6] for o in out]}")
     model.close()
     ctx.close()
 
