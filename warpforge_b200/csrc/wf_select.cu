@@ -141,11 +141,15 @@ struct SelectParams {
     int2* lens_out;
     int64_t tokens, max_context, pages;
     int kv_heads, dim, group, page_shift, max_drafts, width, first, recent, tree;
-    int room;  // pages whose scores a CTA can hold
+    int room;            // pages whose scores a token and kv head may have
+    uint32_t* scores;    // [tokens][kv_heads][room], where a kernel of its own makes them
+    int score_pages;     // of a CTA there
+    uint32_t group_inverse;  // 2^32 / group, rounded up; 0 for a group of one
     int* status;
+    __device__ __forceinline__ int token_of(int head) const { return group_inverse ? (int)__umulhi((uint32_t)head, group_inverse) : head; }  // head / group, below 64 x 128
 };
-constexpr int SELECT_WARPS = 16, SELECT_THREADS = SELECT_WARPS * 32;
-constexpr int SELECT_MAX_GROUP = 128, SELECT_BINS = 256;
+constexpr int SELECT_MAX_GROUP = 128, SELECT_BINS = 256, SELECT_FEW = 256;  // SELECT_FEW: no more than a CTA has threads
+constexpr int64_t SCORE_BYTES = 1LL << 30, SCORED_FROM = 1 << 16;  // of scores in memory, at most; scores of a call that go there
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -155,14 +159,251 @@ __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, ui
 __device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
+// What a sequence's new tokens choose from.  rows: its new tokens; context < 0: a sequence that cannot be.
+struct SelectSeq {
+    int64_t row0;
+    int rows, context;
+    int last, tail, first, between;  // pages in all, from where on all are taken, how many at the start are, how many lie between
+};
+__device__ __forceinline__ SelectSeq select_seq(const SelectParams& p, int s, bool report) {
+    SelectSeq q;
+    const int64_t a = p.q_offsets ? p.q_offsets[s] : (int64_t)s * p.max_drafts, b = p.q_offsets ? p.q_offsets[s + 1] : a + p.max_drafts;
+    const bool no_rows = a < 0 || b < a || b > p.tokens || b - a > p.max_drafts;
+    q.row0 = no_rows ? 0 : a;
+    q.rows = no_rows ? 0 : (int)(b - a);
+    q.context = p.context[s];
+    const bool bad = q.context < 0 || (int64_t)q.context > p.max_context || (int64_t)q.context + q.rows > p.table_stride << p.page_shift;
+    if ((no_rows || bad) && report) report_status(p.status, STATUS_BAD_INDEX);
+    if (bad) q.context = -1;
+    q.last = bad ? 0 : (q.context + q.rows + (1 << p.page_shift) - 1) >> p.page_shift;
+    q.tail = bad ? 0 : max(0, q.context - p.recent) >> p.page_shift;
+    q.first = min(p.first, q.tail);
+    q.between = q.tail - q.first;
+    return q;
+}
+
+// A head of q (4 elements a lane, zeros behind the last) in 8 bits: a word of those that are positive, one of those that are negative; the exponent of its scale, LEAST_SCALE to 122.
+__device__ __forceinline__ int quantized(uint2 w, uint32_t& plus, uint32_t& minus) {
+    const uint32_t x = w.x & 0x7FFF7FFFu, y = w.y & 0x7FFF7FFFu;
+    const uint32_t size = __reduce_max_sync(0xFFFFFFFFu, max(max(x & 0xFFFF, x >> 16), max(y & 0xFFFF, y >> 16)));
+    const bool fine = size < 0x7F80;  // a head with an Inf or a NaN has no preferences
+    const int exponent = fine ? scale_exponent(size) : 0;
+    const float by = power_of_two(-exponent);
+    int v[4];
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+        const uint32_t half = e & 2 ? w.y : w.x;
+        v[e] = __float2int_rn(__uint_as_float(e & 1 ? half & 0xFFFF0000u : half << 16) * by);
+    }
+    const uint32_t bytes = fine ? __byte_perm(__byte_perm(v[0], v[1], 0x0040), __byte_perm(v[2], v[3], 0x0040), 0x5410) : 0;
+    uint32_t negative;  // every byte's sign, eight times
+    asm("prmt.b32 %0, %1, 0, 0xBA98;" : "=r"(negative) : "r"(bytes));
+    plus = bytes & ~negative;
+    minus = bytes & negative;
+    return exponent;
+}
+// Puts a head's codes where the lanes of an MMA take them from: column `column` of [columns / 8][CHUNKS][32] vectors.
+template <int CHUNKS> __device__ __forceinline__ void place_codes(uint4* codes, int column, int dim, uint32_t plus, uint32_t minus) {
+    const int lane = threadIdx.x & 31;
+    if (4 * lane >= dim) return;
+    auto word = [](int k) { return k / 64 * 128 + (k & 63) / 16 * 4 + (k & 15) / 4; };  // of byte k of a page's codes
+    uint32_t* const to = reinterpret_cast<uint32_t*>(codes) + column / 8 * (CHUNKS * 128) + (column & 7) * 16;
+    to[word(4 * lane)] = plus;
+    to[word(dim + 4 * lane)] = minus;
+}
+// A score of a head is a whole number below 2^21 times its scale, 2^-60 to 2^122; less 2^SCORE_BASE that is a number that a float holds exactly.
+constexpr int SCORE_BASE = 16;
+__device__ __forceinline__ float score_scale(int exponent) { return power_of_two(exponent - SCORE_BASE); }
+
+// Sixteen pages, first + t * 16 .. of the table: lane g * 4 + quad has 16 codes of pages g and g + 8 in every chunk.  Which of them are called which k of the product does not matter, so
+// long as q has the same.
+template <int CHUNKS> struct PageTile {
+    uint4 codes[2][CHUNKS];
+    int scale[2];  // what a page's scale adds to a score; FIRST: the page comes before others, NOWHERE: it is not in the cache
+    static constexpr int NOWHERE = INT_MIN + 1, FIRST = INT_MIN;
+    // the pages' numbers; -1: a place behind the last
+    static __device__ __forceinline__ int2 find(const int* table, const SelectSeq& q, int t) {
+        const int n = t * 16 + ((threadIdx.x & 31) >> 2);
+        return make_int2(n < q.between ? table[q.first + n] : 0, n + 8 < q.between ? table[q.first + n + 8] : 0);
+    }
+    __device__ __forceinline__ void load(const SelectParams& p, int head, int2 pages) {
+        const int quad = threadIdx.x & 3, bytes = 2 * p.dim;
+#pragma unroll
+        for (int e = 0; e < 2; e++) {
+            const int page = e ? pages.y : pages.x;
+            const bool real = page >= 0 && page < p.pages;
+            const size_t entry = (size_t)(real ? page : 0) * p.kv_heads + head;
+#pragma unroll
+            for (int k = 0; k < CHUNKS; k++)
+                codes[e][k] = 64 * k + 16 * quad < bytes ? *reinterpret_cast<const uint4*>(p.codes + entry * bytes + 64 * k + 16 * quad) : make_uint4(0, 0, 0, 0);
+            const int exponent = (int)(__float_as_uint(p.scales[entry]) >> 23 & 0xFF);
+            scale[e] = !real ? NOWHERE : exponent == 0xFF ? FIRST : (exponent - 127 - LEAST_SCALE + SCORE_BASE - LEAST_SCALE) << 20;
+            if (!real) report_status(p.status, STATUS_BAD_INDEX);
+        }
+    }
+    // eight columns: sums of pages g (0, 1) and g + 8 (2, 3) with columns 2 quad, 2 quad + 1
+    __device__ __forceinline__ void multiply(const uint4* q, int (&sum)[4]) const {
+        sum[0] = sum[1] = sum[2] = sum[3] = 0;
+#pragma unroll
+        for (int k = 0; k < CHUNKS; k++) {
+            const uint4 b = q[k * 32 + (threadIdx.x & 31)];
+            mma_s8(sum, codes[0][k].x, codes[1][k].x, codes[0][k].y, codes[1][k].y, b.x, b.y);
+            mma_s8(sum, codes[0][k].z, codes[1][k].z, codes[0][k].w, codes[1][k].w, b.z, b.w);
+        }
+    }
+    // The largest score over the heads, of page g + 8 e, with that page's scale, as an unsigned number of the same order: the exponent (127 less LEAST_SCALE twice and more, so that no scale
+    // changes a sign) above 20 bits of significand, which such a number has.
+    static __device__ __forceinline__ uint32_t key(float best, int scale) {
+        const int size = (int)((__float_as_uint(best) & 0x7FFFFFFFu) >> 3) + scale;
+        const uint32_t key = 0x80000000u + (uint32_t)(best == 0.f ? 0 : best < 0.f ? -size : size);
+        return scale <= NOWHERE ? (scale == FIRST ? 0xFFFFFFFFu : 0u) : key;
+    }
+};
+
+// Scores of all new tokens of a sequence, a CTA a kv head and p.score_pages pages, a warp 16 pages at a time: the codes of a page are read once for all of them.  Columns of the product are
+// the heads of a token, padded to PADDED (0: to a multiple of eight above it), token by token; as many tokens at a time as SCORE_COLUMNS have room for.
+constexpr int SCORE_WARPS = 8, SCORE_PAGES = SCORE_WARPS * 16, SCORE_COLUMNS = 128, SCORE_HEADS = 4;  // heads asked for at a time
+template <int CHUNKS, int PADDED> __global__ void __launch_bounds__(SCORE_WARPS * 32, 2) score_pages_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int TILES = PADDED == 0 ? 1 : 2;  // of eight columns at a time
+    __shared__ uint4 q_codes[SCORE_COLUMNS / 8 * CHUNKS * 32];
+    __shared__ float q_scale[SCORE_COLUMNS];
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = lane >> 2, quad = lane & 3;
+    const int s = blockIdx.y / p.kv_heads, head = blockIdx.y - s * p.kv_heads, padded = PADDED ? PADDED : (p.group + 7) & ~7;
+    const SelectSeq q = select_seq(p, s, false);
+    const int begin = blockIdx.x * p.score_pages, end = min(begin + p.score_pages, q.between);
+    // where all pages are taken, the kernel behind this one does not look at the scores
+    if (q.rows == 0 || begin >= end || q.between <= p.width - q.first - (q.last - q.tail)) return;
+    const int* const table = p.tables + (size_t)s * p.table_stride;
+    const int tokens_at_once = SCORE_COLUMNS / padded;
+    const size_t apart = (size_t)p.kv_heads * p.room;  // scores of a token
+    for (int token0 = 0; token0 < q.rows; token0 += tokens_at_once) {
+        const int tokens = min(tokens_at_once, q.rows - token0), heads = tokens * p.group, column_tiles = (tokens * padded + 7) / 8;
+        int t = begin / 16 + warp;
+        const int last = (end - 1) / 16;
+        // two tiles ahead of the one that is multiplied: the numbers of one's pages, the codes of the next one
+        PageTile<CHUNKS> tile;
+        int2 pages = PageTile<CHUNKS>::find(table, q, t);
+        tile.load(p, head, pages);
+        pages = PageTile<CHUNKS>::find(table, q, t + SCORE_WARPS);
+        __syncthreads();
+        for (int n = threadIdx.x; n < SCORE_COLUMNS / 8 * CHUNKS * 32; n += SCORE_WARPS * 32) q_codes[n] = make_uint4(0, 0, 0, 0);
+        __syncthreads();
+        for (int n0 = warp; n0 < heads; n0 += SCORE_WARPS * SCORE_HEADS) {
+            uint2 w[SCORE_HEADS];
+#pragma unroll
+            for (int e = 0; e < SCORE_HEADS; e++) {
+                const int n = n0 + e * SCORE_WARPS, i = p.token_of(n), h = n - i * p.group;
+                w[e] = make_uint2(0, 0);
+                if (n < heads && 4 * lane < p.dim)
+                    w[e] = *reinterpret_cast<const uint2*>(p.q + (q.row0 + token0 + i) * p.q_stride + (size_t)(head * p.group + h) * p.dim + 4 * lane);
+            }
+#pragma unroll
+            for (int e = 0; e < SCORE_HEADS; e++) {
+                const int n = n0 + e * SCORE_WARPS, i = p.token_of(n), h = n - i * p.group;
+                if (n >= heads) break;
+                uint32_t plus, minus;
+                const int scale = quantized(w[e], plus, minus);
+                place_codes<CHUNKS>(q_codes, i * padded + h, p.dim, plus, minus);
+                if (lane == 0) q_scale[i * padded + h] = score_scale(scale);
+            }
+        }
+        __syncthreads();
+#pragma unroll 1
+        for (; t <= last; t += SCORE_WARPS) {
+            PageTile<CHUNKS> next;
+            next.load(p, head, pages);
+            pages = PageTile<CHUNKS>::find(table, q, t + 2 * SCORE_WARPS);
+            float best[2] = {-INFINITY, -INFINITY};
+            uint32_t* to = p.scores + ((size_t)(q.row0 + token0) * p.kv_heads + head) * p.room + t * 16 + g;  // page g, of the token that the columns have come to
+            const bool inside[2] = {t * 16 + g < q.between, t * 16 + g + 8 < q.between};
+            int left = tokens, h0 = 0;  // tokens from there on, heads of the first one that are done (PADDED 0)
+            // (PADDED 2, 4, 8) whether this lane's columns are heads, which of the tokens of eight columns it stores (none: TREE_MAX_DRAFTS), of which page
+            const bool one = (2 * quad & (PADDED - 1)) < p.group, two = (2 * quad & (PADDED - 1)) + 1 < p.group;
+            const int mine = PADDED == 8 && quad > 1 ? TREE_MAX_DRAFTS : PADDED == 4 ? quad >> 1 : PADDED == 2 ? quad : 0;
+            const bool mine_inside = quad & 1 ? inside[1] : inside[0];
+            if (PADDED > 1) to += PADDED == 2 ? quad * apart : PADDED == 4 ? (quad >> 1) * apart + 8 * (quad & 1) : 8 * (quad & 1);
+#pragma unroll 1
+            for (int n0 = 0; n0 < column_tiles; n0 += TILES) {  // (there are codes, if only zeros, for SCORE_COLUMNS)
+                int sum[TILES][4];
+#pragma unroll
+                for (int e = 0; e < TILES; e++) tile.multiply(q_codes + (n0 + e) * CHUNKS * 32, sum[e]);
+#pragma unroll
+                for (int i = 0; i < TILES; i++) {
+                    const float2 scales = *reinterpret_cast<const float2*>(q_scale + (n0 + i) * 8 + 2 * quad);
+                    float v[4];
+#pragma unroll
+                    for (int e = 0; e < 4; e++) v[e] = (float)sum[i][e] * (e & 1 ? scales.y : scales.x);
+                    if constexpr (PADDED == 1) {
+#pragma unroll
+                        for (int e = 0; e < 4; e++)
+                            if (2 * quad + (e & 1) < left && inside[e >> 1]) to[(2 * quad + (e & 1)) * apart + 8 * (e >> 1)] = tile.key(v[e], tile.scale[e >> 1]);
+                        to += 8 * apart, left -= 8;
+                    } else if constexpr (PADDED > 1) {
+                        // the largest over the columns of a token that this lane has and its neighbours have; 8 / PADDED tokens
+                        float top[2];
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            top[e] = fmaxf(two ? v[2 * e + 1] : -INFINITY, one ? v[2 * e] : -INFINITY);
+                            if (PADDED >= 4) top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 1));
+                            if (PADDED >= 8) top[e] = fmaxf(top[e], __shfl_xor_sync(0xFFFFFFFFu, top[e], 2));
+                        }
+                        if (PADDED == 2) {
+#pragma unroll
+                            for (int e = 0; e < 2; e++)
+                                if (quad < left && inside[e]) to[8 * e] = tile.key(top[e], tile.scale[e]);
+                        } else if (mine < left && mine_inside) {  // of two lanes that know both, one has page g and the other page g + 8
+                            *to = tile.key(quad & 1 ? top[1] : top[0], quad & 1 ? tile.scale[1] : tile.scale[0]);
+                        }
+                        to += 8 / PADDED * apart, left -= 8 / PADDED;
+                    } else {
+                        const int h = h0 + 2 * quad;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) best[e] = fmaxf(best[e], h + 1 < p.group ? fmaxf(v[2 * e], v[2 * e + 1]) : h < p.group ? v[2 * e] : -INFINITY);
+                        if ((h0 += 8) < padded) continue;
+#pragma unroll
+                        for (int e = 0; e < 2; e++) {
+                            best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 1));
+                            best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 2));
+                            if (quad == 0 && left > 0 && inside[e]) to[8 * e] = tile.key(best[e], tile.scale[e]);
+                            best[e] = -INFINITY;
+                        }
+                        to += apart, left--, h0 = 0;
+                    }
+                }
+            }
+            tile = next;
+        }
+    }
+}
+
+// Scores that the kernel before this one left (ld_once says why not by a plain load).
+__device__ __forceinline__ uint4 load_scores(const uint32_t* from) {
+    uint4 v;
+    asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
+    return v;
+}
+__device__ __forceinline__ uint2 load_scores2(const uint32_t* from) {
+    uint2 v;
+    asm volatile("ld.global.cs.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(from));
+    return v;
+}
+
 // A cluster has one new token and kv head.  Its CTAs score a part of the pages each, 16 pages by the heads of the group a warp at a time (mma.sync on the codes: [q+ | q-] . [hi | lo],
-// the positive elements of q in the one half and the negative ones in the other), and leave the scores in the first CTA's shared memory, which takes the largest.
-// CHUNKS of 64 codes of a page (hi and lo together).
-template <int CHUNKS> __global__ void __launch_bounds__(SELECT_THREADS) select_pages_kernel(const __grid_constant__ SelectParams p) {
-    extern __shared__ uint32_t keys[];  // [room] scores, as unsigned numbers of the same order
-    __shared__ uint4 q_codes[SELECT_MAX_GROUP / 8][CHUNKS][32];  // as the lanes of an MMA take them
-    __shared__ int q_scale[SELECT_MAX_GROUP];  // exponents as they are added to a score
-    __shared__ uint32_t bins[SELECT_BINS], warp_sums[SELECT_WARPS], warp_low[SELECT_WARPS], warp_high[SELECT_WARPS], found[3];
+// the positive elements of q in the one half and the negative ones in the other), and leave the scores in the first CTA's shared memory, which takes the largest.  SCORED: the scores lie in
+// memory.  CHUNKS of 64 codes of a page (hi and lo together).  RUN: scores of a thread, which it keeps in registers; 0: as many as there are, read again each time.
+template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_bounds__(WARPS * 32, WARPS <= 8 && RUN != 2 ? 2 : WARPS <= 8 ? 3 : SCORED ? 2 : 1) select_pages_kernel(const __grid_constant__ SelectParams p) {
+    constexpr int THREADS = WARPS * 32;
+    constexpr bool AHEAD = RUN != 2;  // (few pages: a warp has one or two tiles of them, and registers are worth more)
+    constexpr bool IN_MEMORY = SCORED && RUN > 0;  // registers take the scores from there
+    extern __shared__ uint4 dynamic[];  // scores [room], as unsigned numbers of the same order; codes of the heads; exponents of their scales
+    uint32_t* const keys = reinterpret_cast<uint32_t*>(dynamic);
+    uint4* const q_codes = dynamic + p.room / 4;
+    float* const q_scale = reinterpret_cast<float*>(q_codes + (p.group + 7) / 8 * CHUNKS * 32);
+    __shared__ uint32_t bins[SELECT_BINS], warp_low[WARPS], warp_high[WARPS], found[3];
+    __shared__ unsigned long long totals[WARPS];
+    __shared__ uint32_t few[SELECT_FEW], few_count;
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     uint32_t rank, ranks;
     asm("mov.u32 %0, %%cluster_ctarank;" : "=r"(rank));
@@ -172,159 +413,152 @@ template <int CHUNKS> __global__ void __launch_bounds__(SELECT_THREADS) select_p
     const unsigned unit = blockIdx.x / ranks, per_seq = (unsigned)p.max_drafts * p.kv_heads, s = unit / per_seq, of_seq = unit - s * per_seq;
     const int i = (int)(of_seq / p.kv_heads), head = (int)(of_seq - i * p.kv_heads);
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    const int64_t a = p.q_offsets ? p.q_offsets[s] : (int64_t)s * p.max_drafts, b = p.q_offsets ? p.q_offsets[s + 1] : a + p.max_drafts;
-    const bool no_rows = a < 0 || b < a || b > p.tokens || b - a > p.max_drafts;
-    if (no_rows && tid == 0 && rank == 0) report_status(p.status, STATUS_BAD_INDEX);
-    if (no_rows || i >= (int)(b - a)) {  // all of the cluster
+    const SelectSeq q = select_seq(p, (int)s, tid == 0 && rank == 0 && of_seq == 0);
+    if (i >= q.rows) {  // all of the cluster
         cluster_wait();
         return;
     }
-    const int rows = (int)(b - a), context = p.context[s], shift = p.page_shift, page_tokens = 1 << shift;
-    const int64_t row = a + i;
-    const bool bad = context < 0 || (int64_t)context > p.max_context || (int64_t)context + rows > p.table_stride << shift;
-    if (bad && tid == 0 && rank == 0) report_status(p.status, STATUS_BAD_INDEX);
+    const int64_t row = q.row0 + i;
     const int* const table = p.tables + (size_t)s * p.table_stride;
-    const int last = bad ? 0 : (context + rows + page_tokens - 1) >> shift;             // pages of the sequence
-    const int tail = bad ? 0 : max(0, context - p.recent) >> shift;                     // from here on all are taken
-    const int first = min(p.first, tail), between = tail - first, ends = first + last - tail;
-    const int take = min(between, p.width - ends), count = ends + take;                 // the host sees to it that the ends fit
+    const int first = q.first, between = q.between, ends = first + q.last - q.tail;
+    const int take = min(between, p.width - ends), count = ends + take;  // the host sees to it that the ends fit
     int* const list = p.pages_out + ((size_t)row * p.kv_heads + head) * p.width;
     if (rank == ranks - 1) {
-        for (int n = tid; n < p.width - take; n += SELECT_THREADS) {  // the places that the scores do not decide
-            const int at = n < first ? n : n + take, page = at < first ? at : tail + at - first - take;
+        for (int n = tid; n < p.width - take; n += THREADS) {  // the places that the scores do not decide
+            const int at = n < first ? n : n + take, page = at < first ? at : q.tail + at - first - take;
             list[at] = at < count ? table[page] : -1;
         }
         if (tid == 0) {
-            const int held = bad ? 0 : context - (between - take) * page_tokens;
-            p.lens_out[row * p.kv_heads + head] = make_int2(held, bad ? 0 : held + (p.tree ? rows : i + 1));
+            const int held = q.context < 0 ? 0 : q.context - ((between - take) << p.page_shift);
+            p.lens_out[row * p.kv_heads + head] = make_int2(held, q.context < 0 ? 0 : held + (p.tree ? q.rows : i + 1));
         }
     }
     if (take == between) {  // all of them
         if (rank == 0)
-            for (int n = tid; n < take; n += SELECT_THREADS) list[first + n] = table[first + n];
+            for (int n = tid; n < take; n += THREADS) list[first + n] = table[first + n];
         cluster_wait();
         return;
     }
 
-    // The heads of the group in 8 bits, a warp a head.
-    const int column_tiles = (p.group + 7) / 8;
-    for (int n = tid; n < column_tiles * CHUNKS * 32; n += SELECT_THREADS) (&q_codes[0][0][0])[n] = make_uint4(0, 0, 0, 0);
-    __syncthreads();
-    for (int h = warp; h < p.group; h += SELECT_WARPS) {
-        const bf16* q = p.q + row * p.q_stride + (size_t)(head * p.group + h) * p.dim + 4 * lane;
-        const bool mine = 4 * lane < p.dim;
-        const uint2 w = mine ? *reinterpret_cast<const uint2*>(q) : make_uint2(0, 0);
-        const uint32_t x = w.x & 0x7FFF7FFFu, y = w.y & 0x7FFF7FFFu;
-        const uint32_t size = __reduce_max_sync(0xFFFFFFFFu, max(max(x & 0xFFFF, x >> 16), max(y & 0xFFFF, y >> 16)));
-        const bool fine = size < 0x7F80;  // a head with an Inf or a NaN has no preferences
-        const int exponent = fine ? scale_exponent(size) : 0;
-        const float by = power_of_two(-exponent);
-        uint32_t plus = 0, minus = 0;
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-            const uint32_t half = e & 2 ? w.y : w.x;
-            const int v = fine ? __float2int_rn(__uint_as_float(e & 1 ? half & 0xFFFF0000u : half << 16) * by) : 0;
-            plus |= (uint32_t)(max(v, 0) & 0xFF) << 8 * e;
-            minus |= (uint32_t)(min(v, 0) & 0xFF) << 8 * e;
-        }
-        if (mine) {
-            const int k0 = 4 * lane, k1 = p.dim + 4 * lane;  // bytes of a page's codes
-            auto at = [&](int k) { return reinterpret_cast<uint32_t*>(&q_codes[h / 8][k / 64][(h & 7) * 4 + (k & 63) / 16]) + (k & 15) / 4; };
-            *at(k0) = plus;
-            *at(k1) = minus;
-        }
-        if (lane == 0) q_scale[h] = (exponent - LEAST_SCALE) << 20;
-    }
-    __syncthreads();
-    if (ranks > 1) cluster_wait();
-
-    // Scores.  Lane g * 4 + quad has 16 codes of pages g and g + 8 of a tile in every chunk; which of them are called which k of the product does not matter, so long as q has the same.
-    const uint32_t to = map_to_rank((uint32_t)__cvta_generic_to_shared(keys), 0);
-    const int tiles = (between + 15) / 16, mine0 = (int)((int64_t)tiles * rank / ranks), mine1 = (int)((int64_t)tiles * (rank + 1) / ranks);
-    const int codes = 2 * p.dim;
-    for (int t = mine0 + warp; t < mine1; t += SELECT_WARPS) {
-        int64_t entry[2];
-        bool real[2], inside[2];
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            const int n = t * 16 + g + 8 * e;
-            inside[e] = n < between;
-            const int64_t page = inside[e] ? table[first + n] : 0;
-            real[e] = page >= 0 && page < p.pages;
-            if (!real[e] && quad == 0) report_status(p.status, STATUS_BAD_INDEX);
-            entry[e] = (real[e] ? page : 0) * p.kv_heads + head;
-        }
-        uint4 c[2][CHUNKS];
-        uint32_t scale[2];  // exponent as in a float
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-#pragma unroll
-            for (int k = 0; k < CHUNKS; k++) {
-                const bool some = 64 * k + 16 * quad < codes;
-                c[e][k] = some ? *reinterpret_cast<const uint4*>(p.codes + entry[e] * codes + 64 * k + 16 * quad) : make_uint4(0, 0, 0, 0);
-            }
-            scale[e] = __float_as_uint(p.scales[entry[e]]) >> 23 & 0xFF;
-        }
-        int best[2] = {INT_MIN, INT_MIN};
-        for (int n = 0; n < column_tiles; n++) {
-            int sum[4] = {0, 0, 0, 0};
-#pragma unroll
-            for (int k = 0; k < CHUNKS; k++) {
-                const uint4 q = q_codes[n][k][lane];
-                mma_s8(sum, c[0][k].x, c[1][k].x, c[0][k].y, c[1][k].y, q.x, q.y);
-                mma_s8(sum, c[0][k].z, c[1][k].z, c[0][k].w, c[1][k].w, q.z, q.w);
-            }
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                const int h = n * 8 + 2 * quad + (e & 1);
-                // a float's exponent and the 20 bits of significand that such a number has, and the scale's exponent on top
-                const int size = sum[e] ? (__float_as_int((float)abs(sum[e])) >> 3) + q_scale[h] : 0;
-                if (h < p.group) best[e >> 1] = max(best[e >> 1], sum[e] < 0 ? -size : size);
-            }
-        }
-#pragma unroll
-        for (int e = 0; e < 2; e++) {
-            best[e] = max(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 1));
-            best[e] = max(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 2));
-            const int more = ((int)scale[e] - 127 - LEAST_SCALE) << 20;  // the page's scale (a size begins at 127 << 20: no sign changes)
-            const int score = best[e] > 0 ? best[e] + more : best[e] < 0 ? best[e] - more : 0;
-            const uint32_t key = !real[e] ? 0 : scale[e] == 0xFF ? 0xFFFFFFFFu : (uint32_t)score ^ 0x80000000u;
-            if (quad == 0 && inside[e]) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * (uint32_t)(t * 16 + g + 8 * e)), "r"(key) : "memory");
-        }
-    }
-    if (ranks > 1) {
-        cluster_arrive();
+    const uint32_t* const scores = SCORED ? p.scores + ((size_t)row * p.kv_heads + head) * p.room : nullptr;
+    if (SCORED) {
         cluster_wait();
-        if (rank) return;  // nothing is sent to the others
+        if (!IN_MEMORY) {
+            for (int n = 4 * tid; n < between; n += 4 * THREADS) *reinterpret_cast<uint4*>(keys + n) = load_scores(scores + n);
+            __syncthreads();
+        }
     } else {
-        cluster_wait();  // that of the start
+        // This warp's first pages are on their way while the heads of the group are brought to 8 bits, a warp a head.
+        const int tiles = (between + 15) / 16, mine0 = (int)((int64_t)tiles * rank / ranks), mine1 = (int)((int64_t)tiles * (rank + 1) / ranks);
+        PageTile<CHUNKS> tile;
+        int2 pages = PageTile<CHUNKS>::find(table, q, min(mine0 + warp, tiles - 1));
+        tile.load(p, head, pages);
+        if (AHEAD) pages = PageTile<CHUNKS>::find(table, q, mine0 + warp + WARPS);
+        const int column_tiles = (p.group + 7) / 8;
+        for (int n = tid; n < column_tiles * CHUNKS * 32; n += THREADS) q_codes[n] = make_uint4(0, 0, 0, 0);
         __syncthreads();
+        for (int h = warp; h < p.group; h += WARPS) {
+            const bf16* from = p.q + row * p.q_stride + (size_t)(head * p.group + h) * p.dim + 4 * lane;
+            uint32_t plus, minus;
+            const int scale = quantized(4 * lane < p.dim ? *reinterpret_cast<const uint2*>(from) : make_uint2(0, 0), plus, minus);
+            place_codes<CHUNKS>(q_codes, h, p.dim, plus, minus);
+            if (lane == 0) q_scale[h] = score_scale(scale);
+        }
+        __syncthreads();
+        if (ranks > 1) cluster_wait();
+
+        const uint32_t to = map_to_rank((uint32_t)__cvta_generic_to_shared(keys), 0);
+#pragma unroll 1
+        for (int t = mine0 + warp; t < mine1; t += WARPS) {
+            PageTile<CHUNKS> next;
+            if (AHEAD) {
+                next.load(p, head, pages);
+                pages = PageTile<CHUNKS>::find(table, q, t + 2 * WARPS);
+            }
+            float best[2] = {-INFINITY, -INFINITY};
+            for (int n = 0; n < column_tiles; n++) {
+                int sum[4];
+                tile.multiply(q_codes + n * CHUNKS * 32, sum);
+#pragma unroll
+                for (int e = 0; e < 4; e++) {
+                    const int h = n * 8 + 2 * quad + (e & 1);
+                    if (h < p.group) best[e >> 1] = fmaxf(best[e >> 1], (float)sum[e] * q_scale[h]);
+                }
+            }
+#pragma unroll
+            for (int e = 0; e < 2; e++) {
+                best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 1));
+                best[e] = fmaxf(best[e], __shfl_xor_sync(0xFFFFFFFFu, best[e], 2));
+                const int n = t * 16 + g + 8 * e;
+                if (quad == 0 && n < between) asm volatile("st.shared::cluster.u32 [%0], %1;" ::"r"(to + 4 * (uint32_t)n), "r"(tile.key(best[e], tile.scale[e])) : "memory");
+            }
+            if (AHEAD) tile = next;
+            else if (t + WARPS < mine1) tile.load(p, head, PageTile<CHUNKS>::find(table, q, t + WARPS));
+        }
+        if (ranks > 1) {
+            cluster_arrive();
+            cluster_wait();
+            if (rank) return;  // nothing is sent to the others
+        } else {
+            cluster_wait();  // that of the start
+            __syncthreads();
+        }
     }
+
+    // A thread has a run of pages: `run` of them from `from` on (of odd length where they lie in shared memory, for the sake of the banks).
+    const int run = RUN ? RUN : ((between + THREADS - 1) / THREADS) | 1, from = min(tid * run, between), valid = min(run, between - from);
+    uint32_t kept[RUN ? RUN : 1];
+    if constexpr (RUN > 0) {
+#pragma unroll
+        for (int e = 0; e < RUN; e += RUN < 4 ? 2 : 4) {
+            if constexpr (RUN < 4) {
+                const uint2 v = e < valid ? IN_MEMORY ? load_scores2(scores + from + e) : *reinterpret_cast<const uint2*>(keys + from + e) : make_uint2(0, 0);
+                kept[e] = v.x, kept[e + 1] = v.y;
+            } else {
+                const uint4 v = e < valid ? IN_MEMORY ? load_scores(scores + from + e) : *reinterpret_cast<const uint4*>(keys + from + e) : make_uint4(0, 0, 0, 0);
+                kept[e] = v.x, kept[e + 1] = v.y, kept[e + 2] = v.z, kept[e + 3] = v.w;
+            }
+        }
+    }
+    // f(score) for each of them
+    auto each = [&](auto f) {
+        if constexpr (RUN > 0) {
+#pragma unroll
+            for (int e = 0; e < RUN; e++)
+                if (e < valid) f(e, kept[e]);
+        } else {
+            for (int e = 0; e < valid; e++) f(e, keys[from + e]);
+        }
+    };
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+    each([&](int, uint32_t key) { low = min(low, key), high = max(high, key); });
 
     // The largest `take` of them: the key of the last one, by eight bits at a time of what is above the smallest key, and how many of that key.
-    uint32_t low = 0xFFFFFFFFu, high = 0;
-    for (int n = tid; n < between; n += SELECT_THREADS) low = min(low, keys[n]), high = max(high, keys[n]);
     low = __reduce_min_sync(0xFFFFFFFFu, low);
     high = __reduce_max_sync(0xFFFFFFFFu, high);
     if (lane == 0) warp_low[warp] = low, warp_high[warp] = high;
+    if (tid < SELECT_BINS) bins[tid] = 0;
+    if (tid == 0) few_count = 0;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < SELECT_WARPS; w++) low = min(low, warp_low[w]), high = max(high, warp_high[w]);
-    int bits = 32 - __clz(high - low);      // of the differences that are still open
+    for (int w = 0; w < WARPS; w++) low = min(low, warp_low[w]), high = max(high, warp_high[w]);
+    int bits = 32 - __clz(high - low);           // of the differences that are still open
     uint32_t prefix = 0, need = (uint32_t)take;  // what is decided of the difference; how many are still to be taken of those that begin so
     while (bits > 0) {
         const int less = max(0, bits - 8);
-        if (tid < SELECT_BINS) bins[tid] = 0;
-        __syncthreads();
-        for (int n = tid; n < between; n += SELECT_THREADS) {
-            const uint32_t d = keys[n] - low;
+        each([&](int, uint32_t key) {
+            const uint32_t d = key - low;
             if (bits == 32 || d >> bits == prefix >> bits) atomicAdd(&bins[d >> less & (SELECT_BINS - 1)], 1u);
-        }
+        });
         __syncthreads();
         if (warp == 0) {  // the bin of the last one, from above: a lane has eight bins
             uint32_t mine[8], sum = 0;
 #pragma unroll
-            for (int e = 0; e < 8; e++) sum += mine[e] = bins[SELECT_BINS - 1 - (lane * 8 + e)];
+            for (int e = 0; e < 8; e++) {
+                uint32_t& bin = bins[SELECT_BINS - 1 - (lane * 8 + e)];
+                sum += mine[e] = bin;
+                bin = 0;
+            }
             uint32_t before = sum;
 #pragma unroll
             for (int o = 1; o < 32; o <<= 1) {
@@ -343,35 +577,56 @@ template <int CHUNKS> __global__ void __launch_bounds__(SELECT_THREADS) select_p
         need = found[1];
         bits = less;
         if (found[2] == need) break;  // all that begin so
+        if (found[2] <= SELECT_FEW && bits > 0) {  // few begin so: the key of the last one is that of which fewer than `need` are larger and `need` or more are not smaller
+            each([&](int, uint32_t key) {
+                const uint32_t d = key - low;
+                if (d >> bits == prefix >> bits) few[atomicAdd(&few_count, 1u)] = d;
+            });
+            __syncthreads();
+            const uint32_t candidates = few_count, d = tid < candidates ? few[tid] : 0;
+            uint32_t larger = 0, same = 0;
+            if (tid < candidates)
+                for (uint32_t j = 0; j < candidates; j++) larger += few[j] > d, same += few[j] == d;
+            if (tid < candidates && larger < need && larger + same >= need) found[0] = d, found[1] = need - larger;  // (all that have it write the same)
+            __syncthreads();
+            prefix = found[0], need = found[1], bits = 0;
+            break;
+        }
         __syncthreads();
     }
-    // Those that begin above the prefix, and of those that begin like it the first `need`.  A thread has a run of pages, of odd length for the sake of the banks.
-    const int run = ((between + SELECT_THREADS - 1) / SELECT_THREADS) | 1, from = min(tid * run, between), end = min(from + run, between);
+    // Those that begin above the prefix, and of those that begin like it the first `need`.
     const uint32_t border = prefix >> bits;
     uint32_t mine = 0, alike = 0;  // of the run: above the border, on it
-    for (int n = from; n < end; n++) {
-        const uint32_t d = (keys[n] - low) >> bits;
+    each([&](int, uint32_t key) {
+        const uint32_t d = (key - low) >> bits;
         mine += d > border;
         alike += d == border;
-    }
-    unsigned long long both = (unsigned long long)alike << 32 | mine, sum = both;
+    });
+    const unsigned long long both = (unsigned long long)alike << 32 | mine;
+    unsigned long long sum = both;
 #pragma unroll
     for (int o = 1; o < 32; o <<= 1) {
         const unsigned long long v = __shfl_up_sync(0xFFFFFFFFu, sum, o);
         if (lane >= o) sum += v;
     }
-    __shared__ unsigned long long totals[SELECT_WARPS];
     if (lane == 31) totals[warp] = sum;
     __syncthreads();
     sum -= both;
     for (int w = 0; w < warp; w++) sum += totals[w];
     uint32_t above = (uint32_t)sum, like = (uint32_t)(sum >> 32);
-    for (int n = from; n < end; n++) {
-        const uint32_t d = (keys[n] - low) >> bits;
-        const bool taken = d > border || (d == border && like < need);
-        if (taken) list[first + above + min(like, need)] = table[first + n];
+    each([&](int e, uint32_t key) {
+        const uint32_t d = (key - low) >> bits;
+        if (d > border || (d == border && like < need)) {
+            const uint32_t at = above + min(like, need);
+            if (RUN > 0) keys[at] = (uint32_t)(from + e);  // the scores that lay there are in registers
+            else list[first + at] = table[first + from + e];
+        }
         above += d > border;
         like += d == border;
+    });
+    if (RUN > 0) {
+        __syncthreads();
+        for (int n = tid; n < take; n += THREADS) list[first + n] = table[first + keys[n]];
     }
 }
 
@@ -408,13 +663,54 @@ static int launch_select(Context* c, const char* what, void (*kernel)(Params), d
     return WF_OK;
 }
 
-template <int CHUNKS> static int launch_selection(Context* c, const SelectParams& p, int64_t units, unsigned cluster, cudaStream_t s) {
+template <int CHUNKS, int WARPS, int RUN, bool SCORED> static int launch_selection(Context* c, const SelectParams& p, int64_t units, unsigned cluster, cudaStream_t s) {
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    constexpr size_t HEADS = SCORED ? 0 : CHUNKS * 32 * sizeof(uint4) + 8 * sizeof(int);  // bytes for eight heads
+    const size_t smem = (size_t)p.room * 4 + (p.group + 7) / 8 * HEADS;
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(select_pages_kernel<CHUNKS>, cudaFuncAttributeMaxDynamicSharedMemorySize, WF_SELECT_MAX_PAGES * 4));
+        WF_CUDA(c, cudaFuncSetAttribute(select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(WF_SELECT_MAX_PAGES * 4 + SELECT_MAX_GROUP / 8 * HEADS)));
         ready.fetch_or(1ull << (c->device & 63));
     }
-    return launch_select(c, "select_pages", select_pages_kernel<CHUNKS>, dim3((unsigned)(units * cluster)), SELECT_THREADS, cluster, (size_t)p.room * 4, s, p);
+    return launch_select(c, "select_pages", select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, dim3((unsigned)(units * cluster)), WARPS * 32, cluster, smem, s, p);
+}
+template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, int seqs, cudaStream_t s) {
+    const int64_t units = (int64_t)seqs * p.max_drafts * p.kv_heads, bytes = p.tokens * p.kv_heads * p.room * 4;
+    // Several new tokens of a sequence read the same codes.  In one kernel each token's cluster reads them (microseconds: 5 tokens of 4 sequences with 250 pages, 32 / 8 heads, 10.4; of 16
+    // sequences 20.6; 21 tokens of one with 250, 1000, 8125 pages 10.3, 20.1, 97), in two kernels a CTA scores pages for all of them (10.6; 14.5; 14.2, 16.3, 41).
+    if (p.max_drafts > 1 && units * p.room >= SCORED_FROM && bytes <= SCORE_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
+        GemvScratch& scratch = c->gemv_scratch[s];
+        if (bytes > scratch.attn_bytes) {
+            const int rc = refuse_allocation_while_recording(c, s, "the scores of select_pages");
+            if (rc != WF_OK) return rc;
+            scratch.d_attn.reset();
+            scratch.attn_bytes = 0;
+            WF_CUDA(c, make_shared_device(c, scratch.d_attn, (size_t)bytes));
+            scratch.attn_bytes = bytes;
+        }
+        p.scores = reinterpret_cast<uint32_t*>(scratch.d_attn.get());
+        const int64_t lines = (int64_t)seqs * p.kv_heads, pieces = (p.room + SCORE_PAGES - 1) / SCORE_PAGES;
+        // two CTAs on every SM at once: what a CTA does before its first page, the queries, is done by as few as that
+        const int64_t each = (lines * pieces + 2 * c->sm_count - 1) / (2 * c->sm_count);  // pieces of a CTA
+        p.score_pages = (int)(each * SCORE_PAGES);
+        const dim3 grid((unsigned)((pieces + each - 1) / each), (unsigned)lines);
+        auto score = [&](auto kernel) { return launch_select(c, "select_pages", kernel, grid, SCORE_WARPS * 32, 1, 0, s, p); };
+        const int rc = p.group == 1   ? score(score_pages_kernel<CHUNKS, 1>)
+                       : p.group == 2 ? score(score_pages_kernel<CHUNKS, 2>)
+                       : p.group <= 4 ? score(score_pages_kernel<CHUNKS, 4>)
+                       : p.group <= 8 ? score(score_pages_kernel<CHUNKS, 8>)
+                                      : score(score_pages_kernel<CHUNKS, 0>);
+        if (rc != WF_OK) return rc;
+        if (p.room <= 512) return launch_selection<CHUNKS, 8, 2, true>(c, p, units, 1, s);
+        if (p.room <= 2048) return launch_selection<CHUNKS, 8, 8, true>(c, p, units, 1, s);
+        return p.room <= 8192 ? launch_selection<CHUNKS, 16, 16, true>(c, p, units, 1, s) : launch_selection<CHUNKS, 16, 0, true>(c, p, units, 1, s);
+    }
+    // As many CTAs a token and head as leave every CTA an SM and eight tiles of pages: one token of 8 heads at 250, 500, 1000, 8125 pages in clusters of 1 / 2 / 4 / 8: 7.2 / 7.0 / 6.7 / 6.7,
+    // 10.0 / 7.9 / 6.7 / 6.3, 14.0 / 11.3 / 9.6 / 9.0, 52 / 33 / 22 / 17 us; of 48 x 8 heads at 250 9.7 / 14.6 / 20 / 36.
+    unsigned cluster = 1;
+    while (cluster < 8 && units * cluster * 2 <= c->sm_count && p.room >= 128 * (int)cluster) cluster *= 2;
+    if (p.room <= 512) return launch_selection<CHUNKS, 8, 2, false>(c, p, units, cluster, s);
+    if (p.room <= 2048) return launch_selection<CHUNKS, 8, 8, false>(c, p, units, cluster, s);
+    return p.room <= 8192 ? launch_selection<CHUNKS, 16, 16, false>(c, p, units, cluster, s) : launch_selection<CHUNKS, 16, 0, false>(c, p, units, cluster, s);
 }
 
 extern "C" {
@@ -503,11 +799,10 @@ int wf_select_pages(int64_t ctx, const wf_select_pages_args* a, int64_t stream) 
     p.kv_heads = a->kv_heads, p.dim = a->head_dim, p.group = a->q_heads / a->kv_heads;
     p.page_shift = __builtin_ctz((unsigned)page);
     p.max_drafts = a->max_drafts, p.width = a->width, p.first = a->first, p.recent = a->recent, p.tree = a->flags & WF_SELECT_TREE;
+    p.group_inverse = p.group == 1 ? 0 : (uint32_t)(((1ull << 32) + p.group - 1) / p.group);
     p.room = (int)((most + 15) / 16 * 16);
     p.status = c->d_status;
-    unsigned cluster = 1;
-    while (cluster < 8 && units * cluster * 2 <= c->sm_count && most >= 256 * (int)cluster) cluster *= 2;
-    return 2 * a->head_dim <= 128 ? launch_selection<2>(c, p, units, cluster, s) : launch_selection<4>(c, p, units, cluster, s);
+    return 2 * a->head_dim <= 128 ? launch_selections<2>(c, p, a->seqs, s) : 2 * a->head_dim <= 192 ? launch_selections<3>(c, p, a->seqs, s) : launch_selections<4>(c, p, a->seqs, s);
 }
 
 }  // extern "C"
