@@ -411,7 +411,8 @@ def test_shared_outside(backend):
 
 
 def test_shared_is_what_trees_are(backend):
-    """The same call with and without a prefix, and by TreeAttention."""
+    """The same call with and without a prefix, and by TreeAttention: sums of the same products in other parts and orders.  Each is off by at most 2^-8 |out| + 2^-8 sum p |v| (check), and neither
+    of these is more than the largest |v|: two results differ by at most 2 (2^-8 + 2^-8) max |v| = 2^-6 max |v|."""
     import torch
 
     from warpforge_b200 import attention as A
@@ -429,8 +430,8 @@ def test_shared_is_what_trees_are(backend):
         torch.cuda.synchronize()
         A.SharedPrefixAttention(backend.cuda_context, *args, held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=p, max_own=700 - p).run()
         backend.synchronize_device()
-    assert torch.equal(outs[0], outs[1])
-    assert (outs[0].float() - outs[2].float()).abs().max() <= 2.0**-6 * outs[0].float().abs().max()
+    for out in outs[1:]:
+        assert (outs[0].float() - out.float()).abs().max() <= 2.0**-6 * values.float().abs().max()
 
 
 def test_shared_refusals(backend):
@@ -496,6 +497,6 @@ def test_shared_and_selected_recorded(backend):
         A.TreeAttention(ctx, *args, held(outs[3]), held(tables), held(short), max_context=640).run()
         backend.synchronize_device()
         for got, want in zip(outs, outs[2:]):
-            assert (got.float() - want.float()).abs().max() <= 2.0**-6 * want.float().abs().max()
+            assert (got.float() - want.float()).abs().max() <= 2.0**-6 * values.float().abs().max()  # as in test_shared_is_what_trees_are
     ctx.graph_destroy(graph)
     backend.destroy_stream(stream)

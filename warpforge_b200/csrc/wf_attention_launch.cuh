@@ -57,9 +57,9 @@ inline bool rows_of_sectors(const bf16* out, int dim) { return reinterpret_cast<
 inline int dim_chunks(int dim) { return (dim + 63) / 64; }
 
 // Where the pieces of cut units go; `extra` bytes behind them, whose address *more is.
-inline int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cuts, int64_t extra = 0, uint8_t** more = nullptr) {
+inline int tree_scratch(Context* c, cudaStream_t s, int64_t ctas, int64_t floats, TreeCuts* cuts, int64_t extra = 0, uint8_t** more = nullptr) {
     GemvScratch& scratch = c->gemv_scratch[s];
-    const int64_t head = (c->sm_count * (int64_t)sizeof(TreeCut) + 255) & ~255LL, pieces = head + ((floats * (int64_t)sizeof(float) + 255) & ~255LL), bytes = pieces + extra;
+    const int64_t head = (ctas * (int64_t)sizeof(TreeCut) + 255) & ~255LL, pieces = head + ((floats * (int64_t)sizeof(float) + 255) & ~255LL), bytes = pieces + extra;
     if (bytes > scratch.attn_bytes) {
         const int rc = refuse_allocation_while_recording(c, s, "the pieces of tree_attention");
         if (rc != WF_OK) return rc;
@@ -73,34 +73,43 @@ inline int tree_scratch(Context* c, cudaStream_t s, int64_t floats, TreeCuts* cu
     if (more) *more = scratch.d_attn.get() + pieces;
     return WF_OK;
 }
-template <int KIND> inline int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
-    return launch_attention(c, "tree_attention", tree_join_kernel<KIND>, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
+template <int KIND, bool PARTS> inline int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
+    return launch_attention(c, "tree_attention", tree_join_kernel<KIND, PARTS>, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
 }
 // The kernel for few rows.  units: sequences (lists) times heads, with up to unit_rows rows and unit_keys keys each.
-template <int CHUNKS, int MT, int KIND> inline int launch_tree(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
+template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS> inline int launch_tree(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
     const char* what = "tree_attention";
-    typedef TreeShape<CHUNKS, MT> Shape;
+    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, KIND, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
     const int64_t tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
-    units *= (unit_rows + Shape::ROWS - 1) / Shape::ROWS;
+    const int blocks = (unit_rows + Shape::ROWS - 1) / Shape::ROWS, ctas = c->sm_count * Shape::CTAS;
+    units *= blocks;
     TreeTiles t{};
     t.p = p;
-    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
+    if (Shape::MANY) {
+        t.c.may_cut = line_is_cut(units, tiles, ctas, TA_CUT_TILES, TA_CUT_ANYWAY);
+    } else {
+        t.c.blocks = blocks;
+        t.c.units = (int)units;
+        t.c.parts = unit_parts(units, tiles, ctas);
+        t.c.may_cut = t.c.parts > 1;
+    }
     t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
     t.c.dim = Shape::DIM;
-    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
+    const int64_t places = Shape::MANY ? 2 * ctas : units * t.c.parts;
+    int rc = tree_scratch(c, s, Shape::MANY || !t.c.may_cut ? ctas : std::max<int64_t>(units, ctas), t.c.may_cut ? places * Shape::PIECE : 0, &t.c);
     CUtensorMap k, v;
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
     if (rc != WF_OK) return rc;
-    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
-    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
-    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND>, grid, TA_THREADS, (size_t)Shape::SMEM, s, t, k, v);
-    return rc == WF_OK && t.c.may_cut ? launch_join<KIND>(c, p, t.c, grid, Shape::ROWS, s) : rc;
+    const int64_t most = Shape::MANY ? (t.c.may_cut ? std::min<int64_t>(units, ctas) * tiles : units) : units * t.c.parts;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, ctas);
+    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND, WARPS>, grid, Shape::THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join<KIND, !Shape::MANY>(c, p, t.c, Shape::MANY ? grid : (unsigned)units, Shape::ROWS, s) : rc;
 }
 
 // The prompt kernel on the rows of trees.
@@ -126,12 +135,16 @@ template <int CHUNKS, int KIND> inline int launch_wide_tree(Context* c, const Tr
     // groups: all of their tokens are p.tokens, and each may have a block that is not full
     if (KIND == ATTEND_PREFIX) units += p.tokens / (2 * t.tile_tokens) * p.cache.kv_heads;
     else units *= (unit_tokens + 2 * t.tile_tokens - 1) / (2 * t.tile_tokens);
-    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, PA_CUT_TILES, PA_CUT_ANYWAY);
+    constexpr bool PREFIX = KIND == ATTEND_PREFIX;
+    // a prefix is cut where there are fewer units than half of the CTAs' rounds; `cuts` has an entry for each unit, a piece a place for each CTA and round
+    t.c.may_cut = PREFIX ? tiles > 1 && units <= (PREFIX_ROUNDS - 1) * c->sm_count : line_is_cut(units, tiles, c->sm_count, PA_CUT_TILES, PA_CUT_ANYWAY);
+    t.c.units = (int)std::min<int64_t>(units, (PREFIX_ROUNDS - 1) * c->sm_count);
+    const int places = PREFIX ? PREFIX_ROUNDS * c->sm_count : 2 * c->sm_count;
     t.c.piece_rows = unit_tokens <= t.tile_tokens ? PA_ROWS : 2 * PA_ROWS;
     t.c.tile_rows = t.tile_tokens * p.group;
     t.c.tile_room = PA_ROWS;
     t.c.dim = CHUNKS * 64;
-    int rc = tree_scratch(c, s, t.c.may_cut ? (int64_t)c->sm_count * 2 * t.c.piece_rows * (t.c.dim + 2) : 0, &t.c);
+    int rc = tree_scratch(c, s, 2 * c->sm_count, t.c.may_cut ? (int64_t)places * t.c.piece_rows * (t.c.dim + 2) : 0, &t.c);
     CUtensorMap q, k, v;
     if (rc == WF_OK) rc = encode_rows(c, &q, p.q, p.cache.dim, p.q_heads, p.tokens, p.cache.dim, p.q_stride, p.group, t.tile_tokens);
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, t.box_rows);
@@ -140,7 +153,7 @@ template <int CHUNKS, int KIND> inline int launch_wide_tree(Context* c, const Tr
     const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
     const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
     rc = launch_attention(c, "tree_attention", prompt_tiles_kernel<CHUNKS, KIND>, grid, PA_THREADS, (size_t)PromptShape<CHUNKS>::SMEM, s, t, q, k, v);
-    return rc == WF_OK && t.c.may_cut ? launch_join<KIND>(c, p, t.c, grid, (int)std::min<int64_t>(unit_tokens, 2 * t.tile_tokens) * p.group, s) : rc;
+    return rc == WF_OK && t.c.may_cut ? launch_join<KIND, PREFIX>(c, p, t.c, PREFIX ? (unsigned)t.c.units : grid, (int)std::min<int64_t>(unit_tokens, 2 * t.tile_tokens) * p.group, s) : rc;
 }
 
 }  // namespace wf

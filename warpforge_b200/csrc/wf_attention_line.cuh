@@ -1,12 +1,23 @@
 // How attention over a cache is cut over the SMs, and how the pieces are joined.
 //
-// A unit is a block of rows of one sequence and kv head; it reads so many tiles of keys.  All units form one line, a unit `unit_tiles` positions (for
+// A unit is a block of rows of one sequence and kv head; it reads so many tiles of keys.  Where units are few and of unequal length, all of them form one line, a unit `unit_tiles` positions (for
 // what it costs in any case) and a position for each tile; the line is cut into even shares, one a CTA.  Where units may be cut, a CTA's pieces
 // of cut units go to memory and tree_join_kernel adds them up in the order of the line; where they may not, a unit belongs to the share that it begins in.
+// Where units are many (walk_units), each is cut into the same number of parts, or not at all, and a CTA finds its own without looking at the others; prefixes (walk_prefixes) are cut into
+// parts of at most so many tiles, that many that all CTAs have one.  Parts have a place in memory each.
 #pragma once
+#include <algorithm>
+
 #include "wf_attention.cuh"
 
 namespace wf {
+
+// Units by number: cut though they are more than the CTAs, up to so many times; places for their parts, a CTA.
+constexpr int UNIT_ROUNDS = 4, UNIT_PLACES = 8;
+constexpr int64_t UNIT_ITEMS = 1 << 18, UNIT_KEYS = 1 << 27;  // sequences (lists) times heads, of which each may be four blocks of rows, and keys of one: their tiles are numbers for quick_div
+
+// Parts of prefixes: as many as all CTAs have in so many rounds, at most.
+constexpr int PREFIX_ROUNDS = 3;
 
 // A cut unit, as the CTA that it begins in leaves it for tree_join_kernel.
 struct alignas(16) TreeCut {
@@ -23,6 +34,8 @@ struct TreeCuts {
     int tile_rows, tile_room;  // rows come in tiles of tile_rows, which have the room of tile_room
     int dim;            // floats of a row
     int may_cut;
+    int parts, blocks;  // units by number: parts of each, blocks of rows of a sequence and head
+    int units;          // by number, and prefixes: that `cuts` has an entry for
 };
 
 // Whether units are cut, by what the host knows: how many there are and how many tiles the longest can have.  Cut, every CTA has the same share, but most
@@ -34,11 +47,19 @@ inline bool line_is_cut(int64_t units, int64_t tiles, int sms, int worth, int an
     return tiles > anyway || tiles * (rounds * sms - units) > (int64_t)worth * sms;
 }
 
+// Parts of each unit, where units go by number: what leaves every CTA a part of eight tiles or more; where there are somewhat more units than CTAs, long ones are cut all the same, since the last
+// of them would be taken by few CTAs.
+inline int unit_parts(int64_t units, int64_t tiles, int ctas) {
+    const int64_t parts = units <= ctas ? ctas / std::max<int64_t>(units, 1) : units <= UNIT_ROUNDS * ctas ? tiles / 64 : 1;
+    return (int)std::max<int64_t>(1, std::min(std::min(parts, tiles / 8), std::max<int64_t>(1, UNIT_PLACES * ctas / units)));
+}
+
 struct LineUnit {
     TreeSeq q;
     int seq, head, first;           // first: of the sequence's rows * group
     int from, to, tiles;            // tiles of the unit that lie in the share
     int first_cta, last_cta;        // whose shares have tiles of it
+    int unit, part;                 // by number, and prefixes: the unit, the place of this part's sums
 };
 
 #ifdef __CUDACC__
@@ -128,9 +149,128 @@ template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_line
     return true;
 }
 
+// a / b for 0 <= a < 2^24 (or a < 2 b): by a float, which is off by one at most then, and put right.  Ten instructions where the exact division has thirty; what a CTA does before its
+// first load it does once, and waits for every line of its code.
+__device__ __forceinline__ int quick_div(int a, int b) {
+    int q = (int)__fdividef((float)a, (float)b);
+    const int rest = a - q * b;
+    return q + (rest >= b) - (rest < 0);
+}
+// The part'th of `parts` parts of so many tiles begins here.
+__device__ __forceinline__ int part_begins(int tiles, int parts, int part) {
+    const int each = quick_div(tiles, parts);
+    return part * each + min(part, tiles - parts * each);
+}
+
+// Walks the units that this CTA has by their number, the whole warp together.
+template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_units(const TreeParams& p, const TreeCuts& c, int unit_rows, F f) {
+    const int heads = p.cache.kv_heads, items = c.units * c.parts;  // below 2^20: launch_tree
+#pragma unroll 1
+    for (int item = blockIdx.x; item < items; item += gridDim.x) {
+        LineUnit u;
+        u.unit = quick_div(item, c.parts);
+        const int part = item - u.unit * c.parts, per_block = quick_div(u.unit, c.blocks), block = u.unit - per_block * c.blocks;  // per_block: a sequence's (token's) kv head
+        const int seq = quick_div(per_block, heads);
+        u.head = per_block - seq * heads;
+        u.seq = KIND == ATTEND_LISTS ? per_block : seq;
+        u.q = seq_of<KIND>(p, u.seq);
+        u.first = block * unit_rows;
+        u.tiles = max(1, (keys_of<KIND>(u.q) + KEYS - 1) / KEYS);
+        const int parts = u.first < u.q.rows * p.group ? min(c.parts, u.tiles) : 0;
+        u.first_cta = item - part, u.last_cta = u.first_cta + parts - 1, u.part = item;
+        if (c.parts > 1 && part == 0 && parts <= 1 && (threadIdx.x & 31) == 0) c.cuts[u.unit].first_cta = -1;
+        if (part >= parts) continue;
+        u.from = 0, u.to = u.tiles;
+        if (parts > 1) u.from = part_begins(u.tiles, parts, part), u.to = part_begins(u.tiles, parts, part + 1);
+        if (!f(u)) return false;
+    }
+    return true;
+}
+
+// Walks this CTA's parts of prefixes.  All CTAs have a part of `most` tiles at most in each of one, two or three rounds, whichever takes least: sum ceil(tiles / most) is not more than total /
+// most + units, so most = total / (rounds CTAs - units) is enough; where there is one group its units are alike, and rounds CTAs / units parts of each are exactly as many.  too_many: groups
+// that overlap have more units than there is room for; nothing is walked.
+template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, bool& too_many, F f) {
+    const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, ctas = (int)gridDim.x, unit_tokens = quick_div(unit_rows, p.group);
+    auto info = [&](int g) {
+        TreeSeq q{};
+        if (g < p.n_groups) q = prefix_seq(p, g);
+        return q;
+    };
+    auto blocks_of = [&](const TreeSeq& q) { return quick_div(q.rows + unit_tokens - 1, unit_tokens); };
+    auto units_of = [&](const TreeSeq& q) { return blocks_of(q) * heads; };
+    auto tiles_of = [&](const TreeSeq& q) { return (q.context + KEYS - 1) / KEYS; };
+    const TreeSeq first = info(lane);
+    int units = units_of(first), total = units * tiles_of(first);
+#pragma unroll 1
+    for (int g0 = 32; g0 < p.n_groups; g0 += 32) {
+        const TreeSeq q = info(g0 + lane);
+        units += units_of(q), total += units_of(q) * tiles_of(q);
+    }
+    units = __reduce_add_sync(0xFFFFFFFFu, units);
+    total = __reduce_add_sync(0xFFFFFFFFu, total);
+    too_many = c.may_cut && units > c.units;
+    if (units == 0 || too_many) {
+        if (c.may_cut && blockIdx.x == 0)
+            for (int i = lane; i < c.units; i += 32) c.cuts[i].first_cta = -1;
+        return true;
+    }
+    int most = 1 << 28;  // tiles of a part
+    TreeSeq first0 = first;  // the first group's, for all lanes
+    first0.context = __shfl_sync(0xFFFFFFFFu, first.context, 0);
+    if (c.may_cut) {
+        int least = 1 << 30;
+#pragma unroll 1
+        for (int rounds = 1; rounds <= PREFIX_ROUNDS; rounds++) {
+            const int room = rounds * ctas;
+            if (units >= room) continue;
+            const int each = quick_div(room, units), t = p.n_groups == 1 ? quick_div(tiles_of(first0) + each - 1, each) : (int)((unsigned)(total + room - units - 1) / (unsigned)(room - units));
+            if (rounds * (t + unit_tiles) < least) least = rounds * (t + unit_tiles), most = t;
+        }
+    }
+    int at = 0, unit_at = 0;  // items and units of the groups before the lanes'
+    int item = (int)blockIdx.x;
+#pragma unroll 1
+    for (int g0 = 0; g0 < p.n_groups; g0 += 32) {
+        TreeSeq mine = first;
+        if (g0) mine = info(g0 + lane);
+        const int my_units = units_of(mine), my_parts = my_units ? quick_div(tiles_of(mine) + most - 1, most) : 0, my_items = my_units * my_parts;
+        int up_to = my_items, units_to = my_units;
+#pragma unroll
+        for (int o = 1; o < 32; o <<= 1) {
+            const int v = __shfl_up_sync(0xFFFFFFFFu, up_to, o), w = __shfl_up_sync(0xFFFFFFFFu, units_to, o);
+            if (lane >= o) up_to += v, units_to += w;
+        }
+        const int all = __shfl_sync(0xFFFFFFFFu, up_to, 31);
+#pragma unroll 1
+        for (; item < at + all; item += ctas) {
+            const int l = __ffs(__ballot_sync(0xFFFFFFFFu, at + up_to > item)) - 1;  // the group
+            LineUnit u;
+            u.q.row0 = __shfl_sync(0xFFFFFFFFu, mine.row0, l), u.q.rows = __shfl_sync(0xFFFFFFFFu, mine.rows, l), u.q.context = __shfl_sync(0xFFFFFFFFu, mine.context, l);
+            u.q.place.table = reinterpret_cast<const int*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(mine.place.table), l));
+            u.q.place.first = 0;
+            u.seq = g0 + l;
+            u.tiles = tiles_of(u.q);
+            const int parts = __shfl_sync(0xFFFFFFFFu, my_parts, l), begin = at + __shfl_sync(0xFFFFFFFFu, up_to - my_items, l), unit = quick_div(item - begin, parts), part = item - begin - unit * parts;
+            u.unit = unit_at + __shfl_sync(0xFFFFFFFFu, units_to - my_units, l) + unit;
+            const int blocks = blocks_of(u.q);
+            u.head = quick_div(unit, blocks);
+            u.first = (unit - u.head * blocks) * unit_rows;
+            u.from = part_begins(u.tiles, parts, part), u.to = part_begins(u.tiles, parts, part + 1);
+            u.first_cta = item - part, u.last_cta = u.first_cta + parts - 1, u.part = item;
+            if (c.may_cut && parts == 1 && lane == 0) c.cuts[u.unit].first_cta = -1;
+            if (!f(u)) return false;
+        }
+        at += all;
+        unit_at += __shfl_sync(0xFFFFFFFFu, units_to, 31);
+    }
+    if (c.may_cut && blockIdx.x == 0)
+        for (int i = unit_at + lane; i < c.units; i += 32) c.cuts[i].first_cta = -1;  // there are no more
+    return true;
+}
+
 // What a CTA leaves for tree_join_kernel: the unit that begins in its share and does not end there, if there is one.
-template <int KIND> __device__ __forceinline__ void leave_cut(const TreeCuts& c, const LineUnit& u, int count) {
-    TreeCut& cut = c.cuts[blockIdx.x];
+template <int KIND> __device__ __forceinline__ void leave_cut(TreeCut& cut, const LineUnit& u, int count) {
     cut.first_cta = u.first_cta, cut.last_cta = u.last_cta;
     cut.row0 = u.q.row0, cut.rows = u.q.rows, cut.context = u.q.context, cut.seq = u.seq;
     cut.head = u.head, cut.first = u.first, cut.count = count;
@@ -147,8 +287,9 @@ __device__ __forceinline__ float line_ex2(float x) {
 // the unit begins in.  Bound by the latency of cut, pieces and row one after the other, and by how many rows an SM has at a time.  Pieces ahead 2 / 3 / 4 / 5 / 8: 13.3 / 12.5 /
 // 12.4 / 13.0 / 12.8 us for one token of 32 heads at 2000 tokens (the kernel before it included), 25.2 / 22.8 / 22.0 / 23.1 / 23.0 of 8 heads at 20,000, 22.4 / 21.6 / 22.0 /
 // 21.8 / 22.9 for 8 sequences of 0 to 3000 with up to 24 drafts; CTAs of 2 / 8 / 16 warps, the last of these: 24.5 / 22.3 / 22.9.
+// PARTS: the pieces are parts of units by number, one place each; blockIdx.x is the unit.
 constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 4;
-template <int KIND> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ TreeCuts c) {
+template <int KIND, bool PARTS> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ TreeCuts c) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     const TreeCut cut = c.cuts[blockIdx.x];
@@ -164,7 +305,7 @@ template <int KIND> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join
 #pragma unroll
         for (int i = 0; i < JOIN_AHEAD; i++) {
             const bool real = c0 + i <= cut.last_cta;
-            const float* from = c.pieces + ((size_t)(c0 + i) * 2 + (c0 + i == cut.first_cta)) * piece_floats;
+            const float* from = c.pieces + (PARTS ? (size_t)(c0 + i) : (size_t)(c0 + i) * 2 + (c0 + i == cut.first_cta)) * piece_floats;
             v[i] = real && mine ? ld_once(reinterpret_cast<const float4*>(from + (size_t)at * c.dim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
             m[i] = real ? ld_once(from + c.piece_rows * c.dim + at) : -INFINITY;
             l[i] = real ? ld_once(from + c.piece_rows * (c.dim + 1) + at) : 0.f;
@@ -189,14 +330,6 @@ template <int KIND> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join
         if (mine) *reinterpret_cast<float4*>(p.state + place * p.state_dim + 4 * lane) = x;
         if (lane == 0) p.state_maxima()[place] = top, p.state_weights()[place] = sum;
         return;
-    }
-    if (KIND == ATTEND_OWN && cut.context >= 0 && p.prefix_of[cut.seq].x > 0) {
-        const float4 v = mine ? ld_once(reinterpret_cast<const float4*>(p.state + place * p.state_dim) + lane) : make_float4(0.f, 0.f, 0.f, 0.f);
-        const float m = ld_once(p.state_maxima() + place), l = ld_once(p.state_weights() + place);
-        const float grown = fmaxf(top, m), ref = grown == -INFINITY ? 0.f : grown, keep = line_ex2((top - ref) * p.scale_log2), take = line_ex2((m - ref) * p.scale_log2);
-        top = grown;
-        sum = sum * keep + l * take;
-        x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
     }
     const float inv = sum == 0.f ? 0.f : 1.f / sum;
     bf16* const to = p.out + place * d;

@@ -30,19 +30,25 @@ static TreeParams attention_params(Context* c, const wf_kv_cache& cache, int lay
     return p;
 }
 
-// Lists.  More than 32 heads of a group are taken 32 at a time.
+// Lists.  More than 32 heads of a group are taken 32 at a time.  Many lists go to small CTAs by number, up to one an SM to large ones that share them out evenly.  Microseconds of the
+// large / the small, 32 / 8 heads of 128, lists of 256, 1024, 4096 keys: 8 lists 6.9 / 10.2, 11.0 / 10.2, 12.6 / 16.8; 128 9.3 / 10.2, 18.3 / 19.4, 53 / 50; 160 13.2 / 10.7, 25.8 / 22.0,
+// 64 / 59; 384 23.5 / 13.7, 45.8 / 36.6, 133 / 125; 800 44 / 26, 88 / 75, 264 / 262.
 template <int CHUNKS> static int launch_lists(Context* c, const TreeParams& p, cudaStream_t s) {
     const int64_t units = p.tokens * p.cache.kv_heads, keys = p.table_stride << p.cache.page_shift;
+    if (units * ((p.group + 31) / 32) > c->sm_count && units < UNIT_ITEMS && keys < UNIT_KEYS)
+        return p.group <= 16 ? launch_tree<CHUNKS, 1, ATTEND_LISTS, TA_FEW_WARPS>(c, p, units, p.group, keys, s) : launch_tree<CHUNKS, 2, ATTEND_LISTS, TA_FEW_WARPS>(c, p, units, p.group, keys, s);
     return p.group <= 16 ? launch_tree<CHUNKS, 1, ATTEND_LISTS>(c, p, units, p.group, keys, s) : launch_tree<CHUNKS, 2, ATTEND_LISTS>(c, p, units, p.group, keys, s);
 }
 
-// Prefixes, then what the sequences have of their own; the second kernel adds the first one's sums to its rows.
+// Prefixes, then what the sequences have of their own, which begins with the first one's sums.
 template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStream_t s) {
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
-    const int64_t pieces = (int64_t)c->sm_count * 2 * 2 * PA_ROWS * (CHUNKS * 64 + 2);  // the most that any of the kernels leaves
+    // the most cut units and pieces of them that any of the kernels leaves (16: CTAs of an SM times rounds)
+    const int64_t most_cuts = 16 * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
+    static_assert(4 * UNIT_ROUNDS <= 16 && UNIT_PLACES * 4 * 16 <= PREFIX_ROUNDS * 2 * PA_ROWS, "pieces of small CTAs");
     TreeCuts cuts{};
     uint8_t* more = nullptr;
-    int rc = tree_scratch(c, s, pieces, &cuts, sums + p.seqs * (int64_t)sizeof(int2), &more);
+    int rc = tree_scratch(c, s, most_cuts, pieces, &cuts, sums + p.seqs * (int64_t)sizeof(int2), &more);
     if (rc != WF_OK) return rc;
     p.state = reinterpret_cast<float*>(more);
     p.state_dim = CHUNKS * 64;
@@ -51,7 +57,12 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     if (rc != WF_OK) return rc;
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_context + p.max_drafts;
     const int unit_rows = p.max_drafts * p.group;
-    if (unit_rows > 32) return launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
+    // Tiles of 128 rows where sequences have more than 32; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of
+    // 24 / 8 heads of 64 48 / 39; 4, 16, 48 with 12 tokens of 32 / 8 heads of 128 and 400 keys 29.8 / 28.7, 38 / 43, 66 / 85.
+    if (unit_rows > 32 && p.tokens * p.group > 20 * (int64_t)p.seqs) return launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
+    // Small CTAs for many sequences with few rows.  Large / small, one token of 32 / 8 heads of 128 behind 512 in common: 128 units of 50, 400, 2000 keys 18.9 / 18.5, 22.6 / 25.4, 41 / 40; 384 27.9 /
+    // 22.8, 37 / 34, 82 / 81; with 20 rows (two small CTAs an SM) 384 43 / 39, 53 / 56, 93 / 136.
+    if (unit_rows <= 16 && 2 * units >= 5 * c->sm_count && units < UNIT_ITEMS && keys < UNIT_KEYS) return launch_tree<CHUNKS, 1, ATTEND_OWN, TA_FEW_WARPS>(c, p, units, unit_rows, keys, s);
     return unit_rows <= 16 ? launch_tree<CHUNKS, 1, ATTEND_OWN>(c, p, units, unit_rows, keys, s) : launch_tree<CHUNKS, 2, ATTEND_OWN>(c, p, units, unit_rows, keys, s);
 }
 
@@ -90,7 +101,7 @@ int wf_shared_prefix_attention(int64_t ctx, const wf_shared_prefix_attention_arg
     if (!a->q_offsets_dev && a->tokens != (int64_t)a->seqs * a->max_drafts)
         return set_error(c, WF_ERR_SHAPE, "%s: %lld tokens are not %d for each of %d sequences", what, (long long)a->tokens, a->max_drafts, a->seqs);
     if (a->tokens > WF_SHARED_MAX_TOKENS) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens, at most %d", what, (long long)a->tokens, WF_SHARED_MAX_TOKENS);
-    if (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1 || a->max_prefix < 0 || a->max_prefix > (1LL << 31) - 1024 || a->max_own < 0 ||
+    if (a->table_stride < 1 || a->table_stride > (1LL << 31) / cache->page_tokens - 1 || a->max_prefix < 0 || a->max_prefix > 1LL << 28 || a->max_own < 0 ||
         a->max_own > (1LL << 31) - 1024)
         return set_error(c, WF_ERR_SHAPE, "%s: table_stride %lld, max_prefix %lld, max_own %lld", what, (long long)a->table_stride, (long long)a->max_prefix, (long long)a->max_own);
     TreeParams p = attention_params(c, *cache, layer, a->q_dev, a->out_dev, a->q_stride, a->tokens, a->q_heads, a->scale);

@@ -45,6 +45,7 @@ struct PromptItem {
     int piece;             // tree: the unit is cut; 1: this piece is not the one it begins with, 2: it is
     int last;              // no more work (1), or a wait ran out
     int prefix;            // own keys: tokens before them
+    int part;              // prefixes: the place of the sums of a cut unit's part
     const int* table;      // prefixes and own keys: of the unit
     // key tiles of group g
     __device__ __forceinline__ int tiles(int g) const { return split ? (n0 - from - g + 1) >> 1 : max(0, (g ? n1 : n0) - from); }
@@ -66,6 +67,12 @@ struct PromptTiles {
 __device__ __forceinline__ void tma_load_3d(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar, uint32_t issue) {
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
                  "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(y), "r"(z), "r"(bar), "r"(issue)
+                 : "memory");
+}
+__device__ __forceinline__ void tma_load_3d_once(uint32_t dst, const CUtensorMap* map, int x, int y, int z, uint32_t bar, uint32_t issue) {
+    asm volatile("{\n\t.reg .pred e;\n\t.reg .b64 p;\n\tsetp.ne.b32 e, %6, 0;\n\tcreatepolicy.fractional.L2::evict_first.b64 p, 1.0;\n\t"
+                 "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], p;\n\t}" ::"r"(dst), "l"(map),
                  "r"(x), "r"(y), "r"(z), "r"(bar), "r"(issue)
                  : "memory");
 }
@@ -352,19 +359,7 @@ constexpr int PA_CUT_TILES = 6, PA_CUT_ANYWAY = 15;
 template <int KIND, class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
     const TreeParams& p = t.tree;
     bool cut = false;
-    if (KIND == ATTEND_PREFIX) {  // for the kernel behind this one: which prefix a sequence has
-        const int lane = threadIdx.x & 31;
-        for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
-            const GroupSeqs of = group_seqs(p, g);
-            for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(of.prefix, of.first);
-        }
-        if (blockIdx.x == 0) {  // those that no group has
-            const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
-            for (int s = lane; s < before; s += 32) p.prefix_of[s] = make_int2(-1, 0);
-            for (int s = behind + lane; s < p.seqs; s += 32) p.prefix_of[s] = make_int2(-1, 0);
-        }
-    }
-    const bool ok = walk_line<PA_KEYS, KIND>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+    auto unit = [&](const LineUnit& u) {
         PromptItem it{};
         it.seq = u.seq, it.head = u.head, it.row0 = u.q.row0, it.rows = u.q.rows, it.context = u.q.context;
         it.keys = keys_of<KIND>(u.q);
@@ -378,10 +373,29 @@ template <int KIND, class F> __device__ __forceinline__ bool tree_items(const Pr
         it.piece = u.from == 0 && u.to == u.tiles ? 0 : u.from == 0 ? 2 : 1;
         if (it.piece == 2) {
             cut = true;
-            if ((threadIdx.x & 31) == 0) leave_cut<KIND>(t.c, u, min(2 * t.tile_tokens, it.rows - it.token0) * p.group);
+            if ((threadIdx.x & 31) == 0) leave_cut<KIND>(t.c.cuts[KIND == ATTEND_PREFIX ? u.unit : (int)blockIdx.x], u, min(2 * t.tile_tokens, it.rows - it.token0) * p.group);
         }
+        if (KIND == ATTEND_PREFIX) it.part = u.part;
         return f(it);
-    });
+    };
+    if constexpr (KIND == ATTEND_PREFIX) {
+        bool too_many;
+        const bool well = walk_prefixes<PA_KEYS>(p, t.c, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, too_many, unit);
+        // for the kernel behind this one: which prefix a sequence has
+        const int lane = threadIdx.x & 31;
+        if (too_many) report_status(p.status, STATUS_BAD_INDEX);
+        for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
+            const GroupSeqs of = group_seqs(p, g);
+            for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(too_many ? -1 : of.prefix, of.first);
+        }
+        if (blockIdx.x == 0) {  // those that no group has
+            const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
+            for (int s = lane; s < before; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+            for (int s = behind + lane; s < p.seqs; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+        }
+        return well;
+    }
+    const bool ok = walk_line<PA_KEYS, KIND>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, unit);
     if (t.c.may_cut && !cut && (threadIdx.x & 31) == 0) t.c.cuts[blockIdx.x].first_cta = -1;
     return ok;
 }
@@ -588,9 +602,9 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
 #pragma unroll
             for (int e = 0; e < 2; e++) o_phase[e] ^= it.tiles(e) > 0;  // the other group's, too
             const bool whole = !(TREE && it.piece) && !PREFIX;  // rows go to the output
-            float before = 0.f;  // what the sums over the prefix count
+            float before = 0.f;  // what the sums over the prefix count, in the part that has the first keys
             const float* before_sums = nullptr;
-            if (KIND == ATTEND_OWN && whole && it.prefix > 0 && mine) {
+            if (KIND == ATTEND_OWN && it.piece != 1 && it.prefix > 0 && mine && n > 0) {
                 const size_t at = (size_t)row * p.q_heads + head;
                 const float m_before = ld_once(t.tree.state_maxima() + at), l_before = ld_once(t.tree.state_weights() + at);
                 const float grown = fmaxf(top, m_before), ref = grown == -INFINITY ? 0.f : grown, less = ex2((top - ref) * scale);
@@ -604,7 +618,7 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                 const float inv = l == 0.f ? 0.f : __frcp_rn(l);
                 const float2 f0 = make_float2(whole ? keep * inv : keep, whole ? keep * inv : keep), f1 = make_float2(whole ? take * inv : take, whole ? take * inv : take);
                 const int rows = t.c.piece_rows, at = it.split ? r : g * PA_ROWS + r;
-                float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
+                float* const piece = t.c.pieces + (PREFIX ? (size_t)it.part : (size_t)blockIdx.x * 2 + (it.piece == 2)) * rows * (DIM + 2);
                 const bool to_state = PREFIX && !it.piece;
                 float* const sums = to_state ? t.tree.state + ((size_t)row * p.q_heads + head) * DIM : piece + (size_t)at * DIM;
                 if (!whole && r < group * tile_tokens && !(halves && g)) {
@@ -635,20 +649,20 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
 #pragma unroll
                         for (int i = 0; i < 16; i++) x[i] = fma2(reinterpret_cast<float2*>(o1)[i], f1, x[i]);
                     }
-                    if (TREE && !whole) {
-                        if (mine)
-#pragma unroll
-                            for (int i = 0; i < 4; i++) store_32(sums + c + 8 * i, o + 8 * i);
-                        continue;
-                    }
                     if (KIND == ATTEND_OWN && before_sums) {
-                        const float2 f2 = make_float2(before * inv, before * inv);
+                        const float2 f2 = make_float2(whole ? before * inv : before, whole ? before * inv : before);
 #pragma unroll
                         for (int i = 0; i < 8; i++) {
                             const float4 v = ld_once(reinterpret_cast<const float4*>(before_sums + c) + i);
                             x[2 * i] = fma2(make_float2(v.x, v.y), f2, x[2 * i]);
                             x[2 * i + 1] = fma2(make_float2(v.z, v.w), f2, x[2 * i + 1]);
                         }
+                    }
+                    if (TREE && !whole) {
+                        if (mine)
+#pragma unroll
+                            for (int i = 0; i < 4; i++) store_32(sums + c + 8 * i, o + 8 * i);
+                        continue;
                     }
 #pragma unroll
                     for (int i = 0; i < 16; i++) {
@@ -738,7 +752,8 @@ __global__ void __launch_bounds__(PA_THREADS, 1) prompt_tiles_kernel(const __gri
                     const int row = __shfl_sync(0xFFFFFFFFu, z, i);
 #pragma unroll
                     for (int c = 0; c < CHUNKS; c++)
-                        tma_load_3d(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + i * t.box_rows * 128), map, 64 * c, table ? 0 : it.head, row, bar, issue);
+                        if (KIND == ATTEND_PROMPT || KIND == ATTEND_TREE) tma_load_3d(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + i * t.box_rows * 128), map, 64 * c, table ? 0 : it.head, row, bar, issue);
+                        else tma_load_3d_once(kv_smem + (uint32_t)(ring.s * STAGE_BYTES + c * PA_CHUNK + i * t.box_rows * 128), map, 64 * c, table ? 0 : it.head, row, bar, issue);
                 }
                 ring.advance(STAGES);
             };

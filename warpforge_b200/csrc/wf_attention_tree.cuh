@@ -14,33 +14,37 @@
 namespace wf {
 
 constexpr int TA_KEYS = 16;  // of a tile
-constexpr int TA_WARPS = 8, TA_LOADERS = 4;  // warps that multiply, warps that walk and load
-constexpr int TA_THREADS = (TA_WARPS + TA_LOADERS) * 32;
+// Warps that multiply; warps that walk and load.  Eight and four: an SM has one CTA, and a unit's tiles are shared out among eight warps, which is what a few long units want.  Two and one:
+// an SM has four CTAs (two for 32 rows), each with a unit of its own, which is what many short ones want: what a unit costs beyond its tiles is paid beside other units' tiles.
+constexpr int TA_WARPS = 8, TA_FEW_WARPS = 2;
 // Registers: 168 a thread at launch; the warps that multiply take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
-constexpr int TA_MERGE_BYTES = 64 * 1024;
 constexpr int TA_SEGMENTS = 2;     // announced ahead
 // When units are cut (line_is_cut).  Microseconds whole / cut, heads of 128: one sequence of 32 heads with 300, 600, 1000, 2000 tokens 7.2 / 8.7, 9.4 / 9.1, 11.9 / 10.7,
 // 20.3 / 12.8; 8, 16, 18, 20, 24 sequences of 8 heads with 1000 tokens 12.8 / 13.4, 15.5 / 20.1, 16.6 / 21.5, 24.9 / 22.5, 25.7 / 25.8; 16 with 1800 23.4 / 28.2; one with
 // 1250 beside 15 with 200 14.4 / 12.3.
 constexpr int TA_CUT_TILES = 40, TA_CUT_ANYWAY = 96;
 constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
-// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows
-template <int CHUNKS, int MT> struct TreeShape {
-    static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT;
+// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows; WARPS that multiply
+template <int CHUNKS, int MT, int WARPS = TA_WARPS> struct TreeShape {
+    static constexpr bool MANY = WARPS == TA_WARPS;
+    static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT, LOADERS = MANY ? 4 : 1, THREADS = (WARPS + LOADERS) * 32;
+    static constexpr int CTAS = MANY ? 1 : 4 / MT;  // of an SM
+    static constexpr int MERGE_BYTES = MANY ? 64 * 1024 : ROWS * DIM * 4;
     static constexpr int SLOT_BYTES = 2 * CHUNKS * TA_KEYS * 128;  // keys and values of a tile
     static constexpr int Q_BYTES = ROWS * DIM * 2;
-    static constexpr int FIT = (227 * 1024 - TA_MERGE_BYTES - TA_SEGMENTS * Q_BYTES - 4 * 1024) / SLOT_BYTES;
+    // (a CTA of several takes 1 KB of its SM beside its own)
+    static constexpr int FIT = ((MANY ? 227 : 228 / CTAS - 1) * 1024 - MERGE_BYTES - TA_SEGMENTS * Q_BYTES - (MANY ? 4 : 2) * 1024) / SLOT_BYTES;
     // A slot belongs to one loader, and within a segment to one warp, lap after lap: a barrier's parity tells the laps apart only for those that wait for every one.
-    static constexpr int SLOTS = FIT > 32 ? 32 : FIT / TA_WARPS * TA_WARPS;
-    static constexpr int SETS = TA_MERGE_BYTES / (ROWS * DIM * 4) < TA_WARPS ? TA_MERGE_BYTES / (ROWS * DIM * 4) : TA_WARPS;  // warps whose sums lie in shared memory at a time
-    static constexpr int SMEM = SLOTS * SLOT_BYTES + TA_MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
+    static constexpr int SLOTS = FIT > 32 ? 32 : FIT / WARPS * WARPS;
+    static constexpr int SETS = MERGE_BYTES / (ROWS * DIM * 4) < WARPS ? MERGE_BYTES / (ROWS * DIM * 4) : WARPS;  // warps whose sums lie in shared memory at a time
+    static constexpr int SMEM = SLOTS * SLOT_BYTES + MERGE_BYTES + TA_SEGMENTS * Q_BYTES + 1024;
     static constexpr int PIECE = ROWS * (DIM + 2);  // floats of a piece in memory
     // What a unit costs beyond its tiles, in tiles (queries, first tile's way, the fold over eight warps).  16 rows, with 2 / 4 / 8 / 12 / 16 / 24: 91 / 85 / 75 / 73 / 73 / 75 us
     // for one token of 48 sequences of 31 to 4000 tokens; 32 rows of 30 sequences of 10 to 5000, with 16 / 24 / 32 / 48: 72 / 65 / 63 / 61, but 33.2 / 32.8 / 33.2 / 33.3 for 20 alike.
     static constexpr int UNIT_TILES = 16 * MT;
-    static_assert(SETS == TA_WARPS || 2 * SETS == TA_WARPS, "one round of folding");
-    static_assert(SLOTS >= TA_WARPS && SLOTS % TA_WARPS == 0 && SLOTS % TA_LOADERS == 0, "slots for every warp and loader");
+    static_assert(SETS == WARPS || 2 * SETS == WARPS, "one round of folding");
+    static_assert(SLOTS >= WARPS && SLOTS % WARPS == 0 && SLOTS % LOADERS == 0, "slots for every warp and loader");
 };
 // What a CTA has of a unit.
 struct alignas(16) TreeSegment {
@@ -50,6 +54,7 @@ struct alignas(16) TreeSegment {
     int slot, phase;               // of the first tile in the ring
     int last;                      // no more work
     int news, prefix;              // lists; own keys
+    int part;                      // units by number: the place of its sums
 };
 
 struct TreeTiles {
@@ -63,6 +68,18 @@ __device__ __forceinline__ void ta_load(uint32_t dst, const CUtensorMap* map, in
     asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
                  "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes [%0], [%1, {%2, %3, %4}], [%5];\n\t}" ::"r"(dst), "l"(map),
                  "r"(x), "r"(0), "r"(z), "r"(bar), "r"(issue)
+                 : "memory");
+}
+// ... of keys and values that are read once: they leave the L2 before what else lies there, the code of the next kernel and the tables among it
+__device__ __forceinline__ uint64_t read_once_policy() {
+    uint64_t p;
+    asm("createpolicy.fractional.L2::evict_first.b64 %0, 1.0;" : "=l"(p));
+    return p;
+}
+__device__ __forceinline__ void ta_load_once(uint32_t dst, const CUtensorMap* map, int x, int z, uint32_t bar, uint32_t issue, uint64_t policy) {
+    asm volatile("{\n\t.reg .pred e;\n\tsetp.ne.b32 e, %6, 0;\n\t"
+                 "@e cp.async.bulk.tensor.3d.shared::cluster.global.tile.mbarrier::complete_tx::bytes.L2::cache_hint [%0], [%1, {%2, %3, %4}], [%5], %7;\n\t}" ::"r"(dst), "l"(map),
+                 "r"(x), "r"(0), "r"(z), "r"(bar), "r"(issue), "l"(policy)
                  : "memory");
 }
 __device__ __forceinline__ void ta_expect(uint32_t bar, uint32_t bytes, uint32_t issue) {
@@ -82,15 +99,15 @@ __device__ __forceinline__ void mma_bf16(float (&d)[4], const uint32_t (&a)[4], 
 __device__ __forceinline__ void ta_copy16(uint32_t dst, const void* src, bool real) {  // zeros where there is nothing
     asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(real ? 16 : 0) : "memory");
 }
-__device__ __forceinline__ void ta_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(TA_WARPS * 32) : "memory"); }
-__device__ __forceinline__ bool ta_sync_or(bool v) {  // the same answer for all warps that multiply
+template <int WARPS> __device__ __forceinline__ void ta_sync() { asm volatile("barrier.cta.sync 1, %0;" ::"n"(WARPS * 32) : "memory"); }
+template <int WARPS> __device__ __forceinline__ bool ta_sync_or(bool v) {  // the same answer for all warps that multiply
     uint32_t r;
-    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)v), "n"(TA_WARPS * 32) : "memory");
+    asm volatile("{\n\t.reg .pred p, q;\n\tsetp.ne.u32 p, %1, 0;\n\tbarrier.cta.red.or.pred q, 1, %2, p;\n\tselp.u32 %0, 1, 0, q;\n\t}" : "=r"(r) : "r"((uint32_t)v), "n"(WARPS * 32) : "memory");
     return r != 0;
 }
 
-template <int CHUNKS, int MT> struct TreeShared {
-    typedef TreeShape<CHUNKS, MT> Shape;
+template <class S> struct TreeShared {
+    typedef S Shape;
     uint64_t full[Shape::SLOTS], empty[Shape::SLOTS];
     uint64_t seg_full[TA_SEGMENTS], seg_empty[TA_SEGMENTS];
     TreeSegment segments[TA_SEGMENTS];
@@ -103,17 +120,18 @@ template <int CHUNKS, int MT> struct TreeShared {
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
-template <int CHUNKS, int MT, int KIND>
-__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS, MT>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
-    typedef TreeShape<CHUNKS, MT> Shape;
-    constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM;
+template <int CHUNKS, int MT, int KIND, int WARPS>
+__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeShape<CHUNKS, MT, WARPS>>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
+    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+    constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM, LOADERS = Shape::LOADERS;
     const TreeParams& p = t.p;
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
     const uint32_t issue = elect_one();
+    const uint64_t policy = KIND == ATTEND_OWN ? read_once_policy() : 0;
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
     bool cut = false;  // a unit that begins here goes on in the next share
-    const bool ok = walk_line<TA_KEYS, KIND>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, [&](const LineUnit& u) {
+    auto unit = [&](const LineUnit& u) {
         const int keys = keys_of<KIND>(u.q), count = min(ROWS, u.q.rows * group - u.first);
         // the page of a lane's tile, asked for before anything is waited for
         const int* const table = u.q.place.table;
@@ -127,14 +145,15 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
             if (KIND == ATTEND_LISTS) d.news = u.q.news;
             if (KIND == ATTEND_OWN) d.prefix = u.q.prefix;
             g_mbar_arrive(&sh->seg_full[seg]);
-            if (u.from == 0 && u.to < u.tiles) leave_cut<KIND>(t.c, u, count);
+            if (!Shape::MANY) d.part = u.part;
+            if (u.from == 0 && u.to < u.tiles) leave_cut<KIND>(t.c.cuts[Shape::MANY ? (int)blockIdx.x : u.unit], u, count);
         }
         cut |= u.from == 0 && u.to < u.tiles;
         __syncwarp();
         // the queries: rows of 16-byte pieces, swizzled by the row
         const bf16* q0 = p.q + (size_t)u.q.row0 * p.q_stride + (size_t)u.head * group * p.cache.dim;
 #pragma unroll 1
-        for (int i = loader * 32 + lane; i < ROWS * (DIM / 8); i += 32 * TA_LOADERS) {
+        for (int i = loader * 32 + lane; i < ROWS * (DIM / 8); i += 32 * LOADERS) {
             const int r = i / (DIM / 8), piece = i % (DIM / 8), token = p.token_of(u.first + r);
             const bool real = r < count && piece * 8 < p.cache.dim;
             ta_copy16(q_smem + (uint32_t)(seg * Shape::Q_BYTES + r * DIM * 2 + ((piece ^ (r & 7)) << 4)),
@@ -157,12 +176,15 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
 #pragma unroll 1
             for (int i = 0; i < n; i++) {
                 const int row = __shfl_sync(0xFFFFFFFFu, z, i);
-                if (slot % TA_LOADERS == loader) {
+                if (slot % LOADERS == loader) {
                     if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->empty[slot], phase))) return false;
                     const uint32_t bar = g_smem_u32(&sh->full[slot]), to_slot = ring + (uint32_t)(slot * Shape::SLOT_BYTES);
                     ta_expect(bar, Shape::SLOT_BYTES, issue);
 #pragma unroll
-                    for (int c = 0; c < 2 * CHUNKS; c++) ta_load(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue);
+                    for (int c = 0; c < 2 * CHUNKS; c++) {
+                        if (KIND != ATTEND_OWN) ta_load(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue);
+                        else ta_load_once(to_slot + (uint32_t)(c * TA_KEYS * 128), c < CHUNKS ? k_map : v_map, 64 * (c % CHUNKS), row, bar, issue, policy);
+                    }
                 }
                 if (++slot == Shape::SLOTS) slot = 0, phase ^= 1;
             }
@@ -170,8 +192,11 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
         number++;
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
         return true;
-    });
-    if (t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
+    };
+    bool ok;
+    if constexpr (Shape::MANY) ok = walk_line<TA_KEYS, KIND>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, unit);
+    else ok = walk_units<TA_KEYS, KIND>(p, t.c, ROWS, unit);
+    if (Shape::MANY && t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
     if (!ok || !__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
     if (loader == 0 && lane == 0) {
         sh->segments[seg].last = 1;
@@ -181,15 +206,15 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<CHUNKS,
     return true;
 }
 
-template <int CHUNKS, int MT, int KIND>
-__global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
+template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS>
+__global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeShape<CHUNKS, MT, WARPS>::CTAS) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
-    typedef TreeShape<CHUNKS, MT> Shape;
+    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
     constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
     constexpr bool Q_KEPT = MT * CHUNKS <= 2;  // queries stay in registers; else they are read again with every tile
     extern __shared__ uint8_t raw[];
-    __shared__ TreeShared<CHUNKS, MT> sh_;
-    TreeShared<CHUNKS, MT>* const sh = &sh_;
+    __shared__ TreeShared<Shape> sh_;
+    TreeShared<Shape>* const sh = &sh_;
     const TreeParams& p = t.p;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, quad = lane & 3;
     const uint32_t ring = (g_smem_u32(raw) + 1023u) & ~1023u, q_smem = ring + SLOTS * SLOT_BYTES;
@@ -198,8 +223,8 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         g_mbar_init(&sh->full[tid], 1);
         g_mbar_init(&sh->empty[tid], 1);
     } else if (tid >= 32 && tid < 32 + TA_SEGMENTS) {
-        g_mbar_init(&sh->seg_full[tid - 32], 32 * TA_LOADERS + 1);  // every lane's copies of queries, and the words
-        g_mbar_init(&sh->seg_empty[tid - 32], TA_WARPS);
+        g_mbar_init(&sh->seg_full[tid - 32], 32 * Shape::LOADERS + 1);  // every lane's copies of queries, and the words
+        g_mbar_init(&sh->seg_empty[tid - 32], WARPS);
     } else if (tid == 64) {
         sh->odd_rows = 0;
         for (int i = 0; i < 2 * TA_SEGMENTS; i++) sh->bad_pages[i] = -1;
@@ -210,16 +235,16 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
     __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
-    if (warp >= TA_WARPS) {
-        asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_load<CHUNKS, MT, KIND>(t, sh, &k_map, &v_map, ring, q_smem, warp - TA_WARPS)) {
+    if (warp >= WARPS) {
+        if (Shape::MANY) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
+        if (!tree_load<CHUNKS, MT, KIND, WARPS>(t, sh, &k_map, &v_map, ring, q_smem, warp - WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
         return;
     }
 
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_MULTIPLY_REGS));
+    if (Shape::MANY) asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(TA_MULTIPLY_REGS));
     const float scale = p.scale_log2;
     const int d = p.cache.dim, group = p.group;
     // ldmatrix: a lane's row and 16-byte piece, swizzled
@@ -232,7 +257,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll 1
     for (int number = 0;; number++) {
         failed |= !g_mbar_wait(&sh->seg_full[seg], seg_phase);
-        if (ta_sync_or(failed)) {  // `merge` is free again, too
+        if (ta_sync_or<WARPS>(failed)) {  // `merge` is free again, too
             failed = true;
             break;
         }
@@ -255,11 +280,28 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
 #pragma unroll
             for (int n = 0; n < N_TILES; n++) o[i][n][0] = o[i][n][1] = o[i][n][2] = o[i][n][3] = 0.f;
         }
+        // What the prefix has given the rows is where the last warp begins, in the part that has the first keys.
+        if (KIND == ATTEND_OWN && warp == WARPS - 1 && w.prefix > 0 && w.from == 0) {
+#pragma unroll
+            for (int i = 0; i < MT; i++)
+#pragma unroll
+                for (int e = 0; e < 2; e++) {
+                    const int r = 16 * i + g + 8 * e;
+                    if (r >= count) continue;
+                    const int token = p.token_of(w.first + r);
+                    const size_t place = (size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group;
+                    m[i][e] = ld_once(p.state_maxima() + place);
+                    l[i][e] = quad == 0 ? ld_once(p.state_weights() + place) : 0.f;
+                    const float* const from = p.state + place * p.state_dim + 2 * quad;
+#pragma unroll
+                    for (int n = 0; n < N_TILES; n++) asm volatile("ld.global.cs.v2.f32 {%0, %1}, [%2];" : "=f"(o[i][n][2 * e]), "=f"(o[i][n][2 * e + 1]) : "l"(from + 8 * n));
+                }
+        }
         int slot = w.slot + warp;
         uint32_t phase = (uint32_t)w.phase;
         if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
 #pragma unroll 1
-        for (int tile = w.from + warp; tile < w.to; tile += TA_WARPS) {
+        for (int tile = w.from + warp; tile < w.to; tile += WARPS) {
             if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->full[slot], phase))) {
                 failed = true;
                 break;
@@ -357,7 +399,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
             }
             __syncwarp();
             if (lane == 0) g_mbar_arrive(&sh->empty[slot]);
-            slot += TA_WARPS;
+            slot += WARPS;
             if (slot >= SLOTS) slot -= SLOTS, phase ^= 1;
         }
         __syncwarp();
@@ -384,9 +426,9 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                     for (int n = 0; n < N_TILES; n++) row[(n ^ (r & 3)) * 4 + quad] = make_float2(o[i][n][2 * e], o[i][n][2 * e + 1]);
                 }
         };
-        if (SETS < TA_WARPS) {
+        if (SETS < WARPS) {
             if (warp >= SETS) write_sums(warp - SETS);
-            ta_sync();
+            ta_sync<WARPS>();
             if (warp < SETS) {
 #pragma unroll
                 for (int i = 0; i < MT; i++)
@@ -406,13 +448,13 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                         }
                     }
             }
-            ta_sync();
+            ta_sync<WARPS>();
         }
         if (warp < SETS) write_sums(warp);
-        ta_sync();
+        ta_sync<WARPS>();
         const bool whole = w.from == 0 && w.to == w.tiles;
         // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
-        float* const piece = t.c.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
+        float* const piece = t.c.pieces + (Shape::MANY ? (size_t)blockIdx.x * 2 + (w.from == 0) : (size_t)w.part) * Shape::PIECE;
         auto store = [&](int r, int col, const float4& x, float sum, float top) {  // four elements of a row, or zeros where it sees nothing
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             uint32_t largest = sum < INFINITY && !scores_too_large(top, scale) ? 0 : 0x7F800000u;
@@ -424,7 +466,7 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
         };
         constexpr int PER_ROW = DIM / 4;  // threads of a row
 #pragma unroll 1
-        for (int i = tid; i < count * PER_ROW; i += TA_WARPS * 32) {
+        for (int i = tid; i < count * PER_ROW; i += WARPS * 32) {
             const int r = i / PER_ROW, n = i % PER_ROW;
             float top = -INFINITY, sum = 0.f, tops[SETS];
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -438,16 +480,6 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                 const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
                 x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
             }
-            if (KIND == ATTEND_OWN && whole && w.prefix > 0) {
-                const int token = p.token_of(w.first + r);
-                const size_t place = (size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group;
-                const float4 v = ld_once(reinterpret_cast<const float4*>(p.state + place * p.state_dim) + n);
-                const float m_before = ld_once(p.state_maxima() + place), l_before = ld_once(p.state_weights() + place);
-                const float grown = fmaxf(top, m_before), ref2 = grown == -INFINITY ? 0.f : grown, keep = line_ex2((top - ref2) * scale), take = line_ex2((m_before - ref2) * scale);
-                top = grown;
-                sum = sum * keep + l_before * take;
-                x.x = x.x * keep + v.x * take, x.y = x.y * keep + v.y * take, x.z = x.z * keep + v.z * take, x.w = x.w * keep + v.w * take;
-            }
             if (whole) {
                 if (4 * n < d) store(r, 4 * n, x, sum, top);
             } else {
@@ -458,14 +490,14 @@ __global__ void __launch_bounds__(TA_THREADS, 1) tree_tiles_kernel(const __grid_
                 }
             }
         }
-        ta_sync();
+        ta_sync<WARPS>();
         const unsigned long long odd = sh->odd_rows;
         if (odd) {
             // An Inf or a NaN in a row's sums may have come from a key that it does not see (0 x Inf), or from a page that is not in the cache: key by key.
-            ta_sync();
+            ta_sync<WARPS>();
             if (tid == 0) sh->odd_rows = 0;
 #pragma unroll 1
-            for (int r = warp; r < count; r += TA_WARPS) {
+            for (int r = warp; r < count; r += WARPS) {
                 if (!(odd >> r & 1)) continue;
                 const int token = p.token_of(w.first + r), h = w.head * group + (w.first + r) - token * group;
                 attend_again<KIND>(p, w, token, w.head, p.q + (size_t)(w.row0 + token) * p.q_stride + (size_t)h * d, p.out + ((size_t)(w.row0 + token) * p.q_heads + h) * d);
