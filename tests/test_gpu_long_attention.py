@@ -112,6 +112,15 @@ def test_selected_many_lists(backend):
     run_selected(backend, [2000] * 20, [1] * 20, 32, 8, 64, 32, pages=100, heads=[0, 7])
 
 
+def test_selected_on_every_way(backend):
+    """Lists by number and on a line, in clusters of large CTAs and of small ones, whole: as many lists, and of such lengths, as lead there."""
+    run_selected(backend, [2100] * 76, [1] * 76, 16, 8, 64, 16, pages=140, heads=[0, 7])                    # 608 long ones: a line
+    run_selected(backend, [700 + 9 * i for i in range(10)], [1] * 10, 160, 8, 128, 16, pages=140, heads=[7])  # 80 with 20 rows: a line
+    run_selected(backend, [700 + 9 * i for i in range(9)], [1] * 9, 160, 8, 128, 16, pages=140, heads=[0])    # 72 with 20 rows: clusters of 2
+    for tokens in (1, 3, 9, 12, 17, 24, 40):
+        run_selected(backend, [1 + (37 * i) % 600 for i in range(tokens)], [1] * tokens, 16, 8, 128, 16, width=38, pages=60, heads=[0, 3])
+
+
 def test_selected_one_page_many_times(backend):
     def edit(q, keys, values, lists, lens):
         lists[0, 0, :5] = [3, 3, 0, 3, 0]
@@ -218,7 +227,11 @@ def test_selected_refusals(backend):
 
 
 # ------------------------------------------------------------------------------------------------ shared prefixes
-def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, page, shape="tree", seed=0, edit=None, arrays=True, only=None, most=None, garbage=False):
+# A bound of the prefix far above it: as much might be read again, if every sequence were to read it, that the prefixes have a kernel of their own.
+FAR = 1 << 24
+
+
+def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, page, shape="tree", seed=0, edit=None, arrays=True, only=None, most=None, garbage=False, several=False):
     import torch
 
     from warpforge_b200 import attention as A
@@ -248,7 +261,7 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     tab, ctx, off, groups, pre, scale = torch.from_numpy(tables).cuda(), i32(context), i32(offsets(drafts)), i32(first), i32(prefix), 1 / math.sqrt(dim)
     anc = signed(words) if words else torch.zeros(0, dtype=torch.int64, device="cuda")
     torch.cuda.synchronize()
-    op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=most or max(prefix),
+    op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=FAR if several else most or max(prefix),
                                  max_own=most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
     op.run()
     backend.synchronize_device()
@@ -273,69 +286,95 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     return out
 
 
+several = pytest.mark.parametrize("several", [False, True])
+
+
+@several
 @pytest.mark.parametrize("dim", [8, 64, 72, 128])
 @pytest.mark.parametrize("q_heads,kv_heads", [(1, 1), (8, 2), (5, 1), (40, 1), (128, 1)])
-def test_shared(backend, q_heads, kv_heads, dim):
-    run_shared(backend, [3, 1, 4], [48, 0, 160], [5, 100, 0, 33, 16, 1, 64, 7], [1] * 8, q_heads, kv_heads, dim, 16)
+def test_shared(backend, q_heads, kv_heads, dim, several):
+    run_shared(backend, [3, 1, 4], [48, 0, 160], [5, 100, 0, 33, 16, 1, 64, 7], [1] * 8, q_heads, kv_heads, dim, 16, several=several)
 
 
+@several
 @pytest.mark.parametrize("page", [16, 64, 512])
 @pytest.mark.parametrize("q_heads,kv_heads,dim", [(6, 2, 128), (4, 4, 64), (16, 1, 96)])
-def test_shared_trees(backend, page, q_heads, kv_heads, dim):
-    run_shared(backend, [3, 2], [page, 3 * page], [37, 200, 0, 5, 77], [9, 1, 24, 7, 3], q_heads, kv_heads, dim, page)
-    run_shared(backend, [2, 1], [page, 0], [20, 3, 555], [2, 64, 5], q_heads, kv_heads, dim, page, shape="chain", garbage=True)
+def test_shared_trees(backend, page, q_heads, kv_heads, dim, several):
+    run_shared(backend, [3, 2], [page, 3 * page], [37, 200, 0, 5, 77], [9, 1, 24, 7, 3], q_heads, kv_heads, dim, page, several=several)
+    run_shared(backend, [2, 1], [page, 0], [20, 3, 555], [2, 64, 5], q_heads, kv_heads, dim, page, shape="chain", garbage=True, several=several)
 
 
-def test_shared_defaults(backend):
+@several
+def test_shared_few_rows(backend, several):
+    """Up to 16 and 32 rows in all; prefixes in clusters and on a line; tokens of a long sequence among short ones, 32 rows at a time."""
+    run_shared(backend, [2, 2], [320, 48], [5, 100, 0, 33], [1, 1, 1, 1], 8, 2, 64, 16, several=several)
+    run_shared(backend, [2], [640], [5, 100], [1, 2], 20, 2, 128, 16, several=several, garbage=True)
+    run_shared(backend, [2, 2, 2, 1, 1], [320, 48, 160, 0, 0], [5, 100, 0, 33, 7, 8, 9, 1], [1] * 8, 48, 16, 64, 16, several=several, only=[0, 3, 7])
+    run_shared(backend, [9], [64], [5, 100, 0, 33, 7, 8, 9, 1, 60], [1, 1, 1, 12, 1, 1, 1, 1, 1], 8, 2, 64, 16, several=several)
+
+
+@several
+def test_shared_defaults(backend, several):
     """Without offsets and words: every sequence has max_drafts tokens, a chain; bounds far above the lengths."""
-    run_shared(backend, [3, 1], [64, 16], [100, 333, 5, 0], [4, 4, 4, 4], 4, 2, 64, 16, shape="chain", arrays=False)
+    run_shared(backend, [3, 1], [64, 16], [100, 333, 5, 0], [4, 4, 4, 4], 4, 2, 64, 16, shape="chain", arrays=False, several=several)
     run_shared(backend, [3, 1], [64, 16], [100, 333, 5, 0], [2, 4, 1, 4], 4, 2, 64, 16, most=5000)
 
 
-def test_shared_long_prefix(backend):
+@several
+def test_shared_long_prefix(backend, several):
     """Prefixes that many CTAs take a part of, by rows that fill several tiles, one, and a few of one."""
-    run_shared(backend, [40], [4096], [3 * i for i in range(40)], [1] * 40, 16, 2, 128, 64, only=[0, 17, 39])
-    run_shared(backend, [2], [20000], [300, 40], [1, 1], 8, 1, 64, 32, garbage=True)
-    run_shared(backend, [5, 7], [9008, 3200], [20, 700, 5, 0, 64, 3, 3, 3, 1500, 3, 3, 3], [1, 2, 1, 3, 1, 1, 1, 5, 1, 1, 1, 1], 24, 8, 64, 16, only=[0, 3, 8])
+    run_shared(backend, [40], [4096], [3 * i for i in range(40)], [1] * 40, 16, 2, 128, 64, only=[0, 17, 39], several=several)
+    run_shared(backend, [2], [20000], [300, 40], [1, 1], 8, 1, 64, 32, garbage=True, several=several)
+    run_shared(backend, [5, 7], [9008, 3200], [20, 700, 5, 0, 64, 3, 3, 3, 1500, 3, 3, 3], [1, 2, 1, 3, 1, 1, 1, 5, 1, 1, 1, 1], 24, 8, 64, 16, only=[0, 3, 8], several=several)
 
 
-def test_shared_long_own(backend):
+@several
+def test_shared_long_own(backend, several):
     """Own contexts that are cut, behind prefixes, by few rows and by many."""
-    run_shared(backend, [2, 1], [1024, 0], [9000, 10, 70], [1, 1, 1], 8, 2, 128, 64)
-    run_shared(backend, [2], [512], [5000, 3000], [40, 12], 8, 2, 64, 32, garbage=True)
+    run_shared(backend, [2, 1], [1024, 0], [9000, 10, 70], [1, 1, 1], 8, 2, 128, 64, several=several)
+    run_shared(backend, [2], [512], [5000, 3000], [40, 12], 8, 2, 64, 32, garbage=True, several=several)
+    run_shared(backend, [20], [64], [1500] * 10 + [30] * 10, [1] * 20, 8, 8, 64, 32, garbage=True, several=several, only=[0, 19])
 
 
-def test_shared_many_sequences(backend):
+@several
+def test_shared_many_sequences(backend, several):
     rng = np.random.default_rng(6)
     members = [1 + int(n) for n in rng.integers(0, 7, 70)]
     count = sum(members)
     run_shared(backend, members, [16 * int(n) for n in rng.integers(0, 9, 70)], [int(n) for n in rng.integers(0, 60, count)], [1 + int(n) for n in rng.integers(0, 3, count)], 2, 1, 64, 16,
-               only=list(range(0, count, 5)))
+               only=list(range(0, count, 5)), several=several)
 
 
-def test_shared_one_long_group(backend):
-    """More rows than two tiles: several units read the same prefix."""
-    run_shared(backend, [300], [256], [int(i % 40) for i in range(300)], [1] * 300, 4, 1, 64, 16, only=[0, 1, 128, 299])
+@several
+def test_shared_one_long_group(backend, several):
+    """More rows than two tiles: several units read the same prefix.  (On one kv head 300 sequences are few units for the SMs, on eight more than their CTAs.)"""
+    run_shared(backend, [300], [256], [int(i % 40) for i in range(300)], [1] * 300, 4, 1, 64, 16, only=[0, 1, 128, 299], several=several)
+    run_shared(backend, [100], [256], [int(i % 40) for i in range(100)], [1] * 100, 16, 8, 64, 16, only=[0, 1, 99], several=several)
 
 
-def test_shared_nothing_in_common(backend):
-    run_shared(backend, [1, 1, 1], [0, 0, 0], [100, 333, 5], [3, 1, 2], 4, 2, 64, 16)
+@several
+def test_shared_nothing_in_common(backend, several):
+    run_shared(backend, [1, 1, 1], [0, 0, 0], [100, 333, 5], [3, 1, 2], 4, 2, 64, 16, several=several)
+    run_shared(backend, [2, 1], [0, 0], [100, 333, 5], [3, 1, 2], 4, 2, 64, 16, several=several)
 
 
-def test_shared_rows_that_see_nothing(backend):
+@several
+def test_shared_rows_that_see_nothing(backend, several):
     import torch
 
-    out = run_shared(backend, [2], [0], [0, 20], [3, 2], 4, 2, 64, 16, shape="none")
+    out = run_shared(backend, [2], [0], [0, 20], [3, 2], 4, 2, 64, 16, shape="none", several=several)
     assert torch.count_nonzero(out[:3]) == 0
 
 
-def test_shared_sequences_without_tokens(backend):
-    run_shared(backend, [3, 2], [48, 32], [5, 100, 0, 33, 16], [1, 0, 2, 0, 0], 4, 2, 64, 16)
+@several
+def test_shared_sequences_without_tokens(backend, several):
+    run_shared(backend, [3, 2], [48, 32], [5, 100, 0, 33, 16], [1, 0, 2, 0, 0], 4, 2, 64, 16, several=several)
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf"), -float("inf")])
 @pytest.mark.parametrize("drafts", [[2, 9, 1], [20, 9, 33]])
-def test_shared_unseen_keys_have_no_influence(backend, value, drafts):
+@several
+def test_shared_unseen_keys_have_no_influence(backend, value, drafts, several):
     """Behind the ends, in drafts that are no ancestors, in another group's prefix; a row that sees it has what the formula says."""
 
     def edit(q, keys, values, tables):
@@ -344,11 +383,12 @@ def test_shared_unseen_keys_have_no_influence(backend, value, drafts):
             x[int(tables[1][(32 + 50 + 2) // 16]), 1, 4] = value  # the third draft, seen by some
             x[int(tables[2][1]), 0, 3] = value                    # the other group's prefix
 
-    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 4, 2, 64, 16, edit=edit, garbage=True)
-    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 12, 2, 128, 16, edit=edit, garbage=True)
+    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 4, 2, 64, 16, edit=edit, garbage=True, several=several)
+    run_shared(backend, [2, 1], [32, 48], [37, 50, 9], drafts, 12, 2, 128, 16, edit=edit, garbage=True, several=several)
 
 
-def test_shared_values_of_every_size(backend):
+@several
+def test_shared_values_of_every_size(backend, several):
     """Scores that leave the prefix or the own keys no weight at all, near the lowest and the largest fp32."""
 
     def edit(q, keys, values, tables):
@@ -358,10 +398,12 @@ def test_shared_values_of_every_size(backend):
         keys[int(tables[1][3])] *= 30
         q[2:] *= 10
 
-    run_shared(backend, [4], [48], [37, 50, 9, 16], [1, 1, 2, 1], 4, 2, 64, 16, edit=edit)
+    run_shared(backend, [4], [48], [37, 50, 9, 16], [1, 1, 2, 1], 4, 2, 64, 16, edit=edit, several=several)
+    run_shared(backend, [4], [48], [37, 50, 9, 16], [9, 11, 20, 1], 4, 2, 64, 16, edit=edit, several=several)
 
 
-def test_shared_outside(backend):
+@several
+def test_shared_outside(backend, several):
     """Groups, prefixes, contexts and pages that cannot be: reported, rows of zeros or without those keys; the others keep their bits."""
     import torch
 
@@ -373,7 +415,7 @@ def test_shared_outside(backend):
     tables = torch.arange(40, dtype=torch.int32, device="cuda").repeat(8, 1)
     good_out = torch.empty_like(q)
 
-    def run(out, tables=tables, context=(40,) * 8, groups=(0, 2, 4, 6, 8), prefix=(32,) * 4, max_prefix=64, max_own=40):
+    def run(out, tables=tables, context=(40,) * 8, groups=(0, 2, 4, 6, 8), prefix=(32,) * 4, max_prefix=FAR if several else 64, max_own=40):
         tab, ctx, gr, pre = tables.contiguous(), i32(context), i32(groups), i32(prefix)
         out.fill_(7.0)
         torch.cuda.synchronize()
@@ -384,7 +426,7 @@ def test_shared_outside(backend):
     out = torch.empty_like(q)
     zeros = lambda: [t for t in range(8) if torch.count_nonzero(out[t]) == 0]  # noqa: E731
     same = lambda: [t for t in range(8) if torch.equal(out[t], good_out[t])]  # noqa: E731
-    for bad, at in ((dict(prefix=(32, 24, 32, 32)), [2, 3]), (dict(prefix=(32, 32, -16, 32)), [4, 5]), (dict(prefix=(80, 32, 32, 32)), [0, 1]),
+    for bad, at in ((dict(prefix=(32, 24, 32, 32)), [2, 3]), (dict(prefix=(32, 32, -16, 32)), [4, 5]), (dict(prefix=(FAR + 16 if several else 80, 32, 32, 32)), [0, 1]),
                     (dict(context=(40, 31, 40, 40, 40, 40, 73, 40)), [1, 6]), (dict(context=(40, 40, -1, 40, 40, 2**31 - 1, 40, 40)), [2, 5]),
                     (dict(groups=(1, 2, 4, 6, 8)), [0]), (dict(groups=(0, 2, 4, 6, 7)), [7]), (dict(groups=(0, 2, 4, 6, 9)), [6, 7])):
         run(out, **bad)
@@ -425,10 +467,11 @@ def test_shared_is_what_trees_are(backend):
     args = [held(x) for x in (q, keys, values)]
     torch.cuda.synchronize()
     A.TreeAttention(backend.cuda_context, *args, held(outs[0]), held(tables), held(context), max_context=700).run()
-    for out, p in ((outs[1], 0), (outs[2], 9 * 64)):
+    outs.append(torch.empty_like(q))
+    for out, p, most in ((outs[1], 0, 0), (outs[2], 9 * 64, 9 * 64), (outs[3], 9 * 64, FAR)):
         groups, prefix = i32([0, 6]), i32([p])
         torch.cuda.synchronize()
-        A.SharedPrefixAttention(backend.cuda_context, *args, held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=p, max_own=700 - p).run()
+        A.SharedPrefixAttention(backend.cuda_context, *args, held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=most, max_own=700 - p).run()
         backend.synchronize_device()
     for out in outs[1:]:
         assert (outs[0].float() - out.float()).abs().max() <= 2.0**-6 * values.float().abs().max()
@@ -476,7 +519,7 @@ def test_shared_and_selected_recorded(backend):
     args = [held(x) for x in (q, keys, values)]
     stream = backend.create_stream()
     torch.cuda.synchronize()
-    shared = A.SharedPrefixAttention(ctx, *args, held(outs[0]), held(tables), held(context), held(groups), held(prefix), max_prefix=1000, max_own=400)
+    shared = A.SharedPrefixAttention(ctx, *args, held(outs[0]), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR, max_own=400)
     selected = A.SelectedAttention(ctx, *args, held(outs[1]), held(lists), held(lens))
     shared.run(stream)
     ctx.synchronize(stream)

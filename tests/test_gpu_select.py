@@ -250,6 +250,28 @@ def test_select_long(backend, pages):
     run_select(backend, [16 * pages], [2], 4, 1, 128, 16, pages // 2, repeat=2)
 
 
+@pytest.mark.parametrize("q_heads,kv_heads,dim", [(4, 4, 64), (8, 4, 128), (12, 4, 96), (28, 4, 8), (48, 4, 72)])
+def test_select_many_tokens(backend, q_heads, kv_heads, dim):
+    """As many scores as have a kernel of their own, with groups of 1, 2, 3, 7 and 12 heads; a sequence with few pages and one without a context among them."""
+    run_select(backend, [16 * 600 + 5, 700, 0, 300], [20, 3, 9, 0], q_heads, kv_heads, dim, 16, 30, tree=True, repeat=2)
+
+
+@pytest.mark.parametrize("pages,tokens", [(1500, 12), (8150, 8), (8200, 8), (9000, 1)])
+def test_select_many_pages(backend, pages, tokens):
+    """Runs of pages in registers and, where there are more, in shared memory."""
+    run_select(backend, [16 * pages + 3], [tokens], 8, 4 if pages == 1500 else 1, 64, 16, 100)
+
+
+def test_select_ties_of_many_tokens(backend):
+    def two(q, codes, scales, tables):
+        codes[:] = codes[0, 0, 0, 0]
+        scales[:] = 0.25
+        scales[::3] = 0.5
+
+    run_select(backend, [16 * 1100], [16], 8, 4, 64, 16, 50, edit=two)
+    run_select(backend, [16 * 1100], [16], 8, 4, 64, 16, 700, edit=two)
+
+
 def test_select_batch(backend):
     rng = np.random.default_rng(7)
     run_select(backend, [int(n) for n in rng.integers(0, 9000, 60)], [1] * 60, 16, 4, 128, 64, 20, 1, 128)

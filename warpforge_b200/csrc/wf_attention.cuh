@@ -12,8 +12,8 @@ constexpr int ATTN_MAX_DIM = 128;
 constexpr int TREE_MAX_DRAFTS = 64;  // a row's ancestors are one 64-bit word
 
 // What rows attend to: a prompt's past and itself; a sequence's context and new tokens; a list of pages for each token and kv head; where sequences have a prefix in
-// common, that prefix (the rows of all of them), and what a sequence has of its own behind it.
-enum AttentionKind { ATTEND_PROMPT, ATTEND_TREE, ATTEND_LISTS, ATTEND_PREFIX, ATTEND_OWN };
+// common, that prefix (the rows of all of them), and what a sequence has of its own behind it; or both, a sequence at a time.
+enum AttentionKind { ATTEND_PROMPT, ATTEND_TREE, ATTEND_LISTS, ATTEND_PREFIX, ATTEND_OWN, ATTEND_WHOLE };
 
 // One layer of the cache, or packed keys and values (page_shift 0, a page a token).
 struct CacheView {
@@ -115,7 +115,8 @@ struct SharedPlace {
 struct TreeSeq {
     int row0, rows, context;
     int news;    // keys behind the context
-    int prefix;  // own keys: tokens before them, which other kernels have seen to
+    int prefix;  // own keys: tokens before them, which other kernels have seen to; whole sequences: tokens in the pages of another one
+    int first;   // whole sequences: that one
     KeyPlace place;
 };
 __device__ __forceinline__ TreeSeq tree_seq(const TreeParams& p, int s) {
@@ -200,10 +201,41 @@ __device__ __forceinline__ TreeSeq own_seq(const TreeParams& p, int s) {
     q.place.first = 0;
     return q;
 }
+// The prefix of a sequence and whose pages hold it; -1 where its group cannot be.
+__device__ __forceinline__ int2 prefix_of_seq(const TreeParams& p, int s) {
+    int lo = 0, hi = p.n_groups - 1;  // the last group that begins at s or before it
+#pragma unroll 1
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.groups[mid] <= s) lo = mid;
+        else hi = mid - 1;
+    }
+    const GroupSeqs of = group_seqs(p, lo);
+    return make_int2(s < of.first || s >= of.stop ? -1 : of.prefix, of.first);
+}
+__device__ __forceinline__ TreeSeq whole_seq(const TreeParams& p, int s) {
+    TreeSeq q;
+    const int64_t a = p.q_offsets ? p.q_offsets[s] : (int64_t)s * p.max_drafts, b = p.q_offsets ? p.q_offsets[s + 1] : a + p.max_drafts;
+    const bool bad = a < 0 || b < a || b > p.tokens || b - a > p.max_drafts;
+    q.row0 = bad ? 0 : (int)a;
+    q.rows = bad ? 0 : (int)(b - a);
+    const int64_t context = p.context[s];
+    const int2 prefix = prefix_of_seq(p, s);
+    const bool bad_keys = prefix.x < 0 || context < prefix.x || context - prefix.x > p.max_context || context + q.rows > (p.table_stride << p.cache.page_shift);
+    q.context = bad_keys ? -1 : (int)context;  // its rows are zeros
+    q.prefix = bad_keys ? 0 : prefix.x;
+    q.first = bad_keys ? 0 : prefix.y;
+    if (bad || bad_keys) report_status(p.status, STATUS_BAD_INDEX);
+    q.news = q.rows;
+    q.place.table = p.tables + (size_t)s * p.table_stride;
+    q.place.first = 0;
+    return q;
+}
 template <int KIND> __device__ __forceinline__ TreeSeq seq_of(const TreeParams& p, int s) {
     if (KIND == ATTEND_LISTS) return list_seq(p, s);
     if (KIND == ATTEND_PREFIX) return prefix_seq(p, s);
     if (KIND == ATTEND_OWN) return own_seq(p, s);
+    if (KIND == ATTEND_WHOLE) return whole_seq(p, s);
     return tree_seq(p, s);
 }
 // Of a sequence, a segment or a cut unit: new keys, keys in all; context < 0: one that cannot be.
@@ -293,10 +325,11 @@ template <int KIND, class Unit>
 __device__ __forceinline__ void attend_again(const TreeParams& p, const Unit& w, int i, int head, const bf16* q, bf16* out) {
     const uint64_t sees = sees_of<KIND>(p, w.row0 + i, i, news_of<KIND>(w));
     const int keys = keys_of<KIND>(w);
-    if (KIND == ATTEND_OWN) {
-        const int2 prefix = p.prefix_of[w.seq];
-        const int before = w.context < 0 ? 0 : prefix.x;
-        const SharedPlace place = {p.tables + (size_t)(w.context < 0 ? 0 : prefix.y) * p.table_stride, before, p.tables + (size_t)w.seq * p.table_stride};
+    if (KIND == ATTEND_OWN || KIND == ATTEND_WHOLE) {
+        int2 prefix = make_int2(0, 0);
+        if (w.context >= 0) prefix = KIND == ATTEND_OWN ? p.prefix_of[w.seq] : prefix_of_seq(p, w.seq);
+        const int before = KIND == ATTEND_OWN ? prefix.x : 0;
+        const SharedPlace place = {p.tables + (size_t)prefix.y * p.table_stride, prefix.x, p.tables + (size_t)w.seq * p.table_stride};
         attend_row(p.cache, place, q, out, head, before + keys, p.scale_log2, p.status, SeesAncestors{before + w.context, sees});
     } else {
         KeyPlace place;

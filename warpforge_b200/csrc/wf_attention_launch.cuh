@@ -21,21 +21,29 @@ inline int check_queries(Context* c, const char* what, int64_t q, int64_t out, i
     return WF_OK;
 }
 template <class... Params, class... Args>
-inline int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
+inline int launch_clusters(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, unsigned cluster, size_t smem, cudaStream_t s, const Args&... args) {
     cudaLaunchConfig_t cfg = {};
     cfg.gridDim = grid;
     cfg.blockDim = dim3(threads);
     cfg.dynamicSmemBytes = smem;
     cfg.stream = s;
-    cudaLaunchAttribute attr[1];
+    cudaLaunchAttribute attr[2];
     attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
     attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
     cfg.attrs = attr;
-    cfg.numAttrs = 1;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
     const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
     if (e != cudaSuccess) return cuda_status(c, e, what);
     c->launches++;
     return WF_OK;
+}
+
+template <class... Params, class... Args>
+inline int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
+    return launch_clusters(c, what, kernel, grid, threads, 1, smem, s, args...);
 }
 
 // bf16 [z][y][x] with the given distances (elements) between y and z; boxes of 64 elements x by x bz, 128-byte swizzle, zeros outside
@@ -76,40 +84,97 @@ inline int tree_scratch(Context* c, cudaStream_t s, int64_t ctas, int64_t floats
 template <int KIND, bool PARTS> inline int launch_join(Context* c, const TreeParams& p, const TreeCuts& cuts, unsigned ctas, int rows, cudaStream_t s) {
     return launch_attention(c, "tree_attention", tree_join_kernel<KIND, PARTS>, dim3(ctas, (unsigned)((rows + JOIN_WARPS - 1) / JOIN_WARPS)), JOIN_WARPS * 32, 0, s, p, cuts);
 }
-// The kernel for few rows.  units: sequences (lists) times heads, with up to unit_rows rows and unit_keys keys each.
-template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS> inline int launch_tree(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
+// The kernel for few rows, units on a line.  units: sequences (lists) times heads, with up to unit_rows rows and unit_keys keys each.
+template <int CHUNKS, int MT, int KIND> inline int launch_tree(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
     const char* what = "tree_attention";
-    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+    typedef TreeShape<CHUNKS, MT> Shape;
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
-        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, KIND, WARPS>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        WF_CUDA(c, cudaFuncSetAttribute(tree_tiles_kernel<CHUNKS, MT, KIND>, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
         ready.fetch_or(1ull << (c->device & 63));
     }
     const int64_t tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
-    const int blocks = (unit_rows + Shape::ROWS - 1) / Shape::ROWS, ctas = c->sm_count * Shape::CTAS;
-    units *= blocks;
+    units *= (unit_rows + Shape::ROWS - 1) / Shape::ROWS;
     TreeTiles t{};
     t.p = p;
-    if (Shape::MANY) {
-        t.c.may_cut = line_is_cut(units, tiles, ctas, TA_CUT_TILES, TA_CUT_ANYWAY);
-    } else {
-        t.c.blocks = blocks;
-        t.c.units = (int)units;
-        t.c.parts = unit_parts(units, tiles, ctas);
-        t.c.may_cut = t.c.parts > 1;
-    }
+    t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
     t.c.piece_rows = t.c.tile_rows = t.c.tile_room = Shape::ROWS;
     t.c.dim = Shape::DIM;
-    const int64_t places = Shape::MANY ? 2 * ctas : units * t.c.parts;
-    int rc = tree_scratch(c, s, Shape::MANY || !t.c.may_cut ? ctas : std::max<int64_t>(units, ctas), t.c.may_cut ? places * Shape::PIECE : 0, &t.c);
+    int rc = tree_scratch(c, s, c->sm_count, t.c.may_cut ? (int64_t)c->sm_count * 2 * Shape::PIECE : 0, &t.c);
     CUtensorMap k, v;
     if (rc == WF_OK) rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
     if (rc != WF_OK) return rc;
-    const int64_t most = Shape::MANY ? (t.c.may_cut ? std::min<int64_t>(units, ctas) * tiles : units) : units * t.c.parts;  // CTAs that can have work
-    const unsigned grid = (unsigned)std::min<int64_t>(most, ctas);
-    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND, WARPS>, grid, Shape::THREADS, (size_t)Shape::SMEM, s, t, k, v);
-    return rc == WF_OK && t.c.may_cut ? launch_join<KIND, !Shape::MANY>(c, p, t.c, Shape::MANY ? grid : (unsigned)units, Shape::ROWS, s) : rc;
+    const int64_t most = t.c.may_cut ? std::min<int64_t>(units, c->sm_count) * tiles : units;  // CTAs that can have work
+    const unsigned grid = (unsigned)std::min<int64_t>(most, c->sm_count);
+    rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND>, grid, Shape::THREADS, (size_t)Shape::SMEM, s, t, k, v);
+    return rc == WF_OK && t.c.may_cut ? launch_join<KIND, false>(c, p, t.c, grid, Shape::ROWS, s) : rc;
+}
+// Units by number: each in a CTA, or in a cluster's.
+template <int CHUNKS, int MT, int KIND, int WARPS, bool CLUSTER> inline int launch_numbered(Context* c, const TreeParams& p, int64_t units, int parts, int64_t blocks, cudaStream_t s) {
+    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+    auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, WARPS, true, CLUSTER>;
+    static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
+    if (!(ready.load() >> (c->device & 63) & 1)) {
+        WF_CUDA(c, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
+        ready.fetch_or(1ull << (c->device & 63));
+    }
+    TreeTiles t{};
+    t.p = p;
+    t.c.blocks = (int)blocks;
+    t.c.units = (int)units;
+    t.c.parts = parts;
+    CUtensorMap k, v;
+    int rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
+    if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
+    if (rc != WF_OK) return rc;
+    const unsigned grid = CLUSTER ? (unsigned)(units * parts) : (unsigned)std::min<int64_t>(units, c->sm_count * Shape::CTAS);
+    return launch_clusters(c, "tree_attention", kernel, dim3(grid), Shape::THREADS, (unsigned)parts, (size_t)Shape::SMEM, s, t, k, v);
+}
+// Clusters of so many CTAs that the device has at a time.
+template <int CHUNKS, int MT, int KIND, int WARPS> inline int clusters_at_once(Context* c, int size) {
+    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+    static std::atomic<int> known[64][MAX_CLUSTER + 1];  // and one more; 0: not asked
+    std::atomic<int>& held = known[c->device & 63][size];
+    if (held.load() == 0) {
+        auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, WARPS, true, true>;
+        cudaLaunchConfig_t cfg = {};
+        cfg.gridDim = dim3((unsigned)size * 1024);
+        cfg.blockDim = dim3(Shape::THREADS);
+        cfg.dynamicSmemBytes = Shape::SMEM;
+        cudaLaunchAttribute attr[1];
+        attr[0].id = cudaLaunchAttributeClusterDimension;
+        attr[0].val.clusterDim.x = (unsigned)size;
+        attr[0].val.clusterDim.y = attr[0].val.clusterDim.z = 1;
+        cfg.attrs = attr;
+        cfg.numAttrs = 1;
+        int n = 0;
+        if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM) != cudaSuccess || cudaOccupancyMaxActiveClusters(&n, kernel, &cfg) != cudaSuccess) {
+            n = 0;
+            cudaGetLastError();
+        }
+        held.store(n + 1);
+    }
+    return held.load() - 1;
+}
+// How units with few rows go to the SMs.  Up to one an SM, the parts of a unit go to a cluster of large CTAs, as many as let all units be there at once; then to clusters of small CTAs, of
+// which an SM has four; then each to a small CTA of its own; where those are not enough and units are long, to large CTAs that share a line of them.  Microseconds for lists of 256 / 4096 keys, 32 / 8
+// heads of 128, on the line and as chosen here: 8 units 7.0 / 12.6 and 6.6 / 9.2 (clusters of 8), 24 7.1 / 16.6 and 6.8 / 14.3 (4), 72 8.4 / 34 and 6.9 / 28.6 (2), 128 9.1 / 53 and 8.0 / 46.6 (4
+// small), 192 14.1 / 73 and 9.2 / 66 (2 small), 320 21.6 / 115 and 12.4 / 108, 640 36 / 215 and 23 / 249.  With 17 to 32 rows an SM has two small CTAs, and the line is quicker: 64 units of 2048 keys
+// 24.4 and 20.6 (2 large), 80 27.9 against 33 (3 small), 192 49 against 69.
+template <int CHUNKS, int MT, int KIND> inline int launch_units(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
+    const int64_t blocks = (unit_rows + 16 * MT - 1) / (16 * MT), all = units * blocks, tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
+    if (units < UNIT_ITEMS && unit_keys < UNIT_KEYS) {
+        for (int parts = MAX_CLUSTER; parts > 1; parts /= 2)
+            if (tiles >= 8 * parts && all <= clusters_at_once<CHUNKS, MT, KIND, TA_WARPS>(c, parts)) return launch_numbered<CHUNKS, MT, KIND, TA_WARPS, true>(c, p, all, parts, blocks, s);
+        if constexpr (MT == 1) {
+            for (int parts = MAX_CLUSTER / 2; parts > 1; parts--)
+                if (tiles >= 4 * parts && all <= clusters_at_once<CHUNKS, MT, KIND, TA_FEW_WARPS>(c, parts))
+                    return launch_numbered<CHUNKS, MT, KIND, TA_FEW_WARPS, true>(c, p, all, parts, blocks, s);
+            if (all <= c->sm_count * TreeShape<CHUNKS, MT, TA_FEW_WARPS>::CTAS || tiles <= 128) return launch_numbered<CHUNKS, MT, KIND, TA_FEW_WARPS, false>(c, p, all, 1, blocks, s);
+        }
+    }
+    return launch_tree<CHUNKS, MT, KIND>(c, p, units, unit_rows, unit_keys, s);
 }
 
 // The prompt kernel on the rows of trees.

@@ -3,8 +3,8 @@
 // A unit is a block of rows of one sequence and kv head; it reads so many tiles of keys.  Where units are few and of unequal length, all of them form one line, a unit `unit_tiles` positions (for
 // what it costs in any case) and a position for each tile; the line is cut into even shares, one a CTA.  Where units may be cut, a CTA's pieces
 // of cut units go to memory and tree_join_kernel adds them up in the order of the line; where they may not, a unit belongs to the share that it begins in.
-// Where units are many (walk_units), each is cut into the same number of parts, or not at all, and a CTA finds its own without looking at the others; prefixes (walk_prefixes) are cut into
-// parts of at most so many tiles, that many that all CTAs have one.  Parts have a place in memory each.
+// Where units go by number (walk_units), a CTA or a cluster finds its own without looking at the others, and a cluster's CTAs add their parts up among themselves.  Prefixes (walk_prefixes) are
+// cut into parts of at most so many tiles, that many that all CTAs have one; each has a place in memory, and tree_join_kernel adds them up.
 #pragma once
 #include <algorithm>
 
@@ -12,8 +12,8 @@
 
 namespace wf {
 
-// Units by number: cut though they are more than the CTAs, up to so many times; places for their parts, a CTA.
-constexpr int UNIT_ROUNDS = 4, UNIT_PLACES = 8;
+constexpr int MAX_CLUSTER = 8;
+enum UnitWay { UNITS_ON_A_LINE, UNITS_BY_NUMBER, UNITS_IN_PARTS };
 constexpr int64_t UNIT_ITEMS = 1 << 18, UNIT_KEYS = 1 << 27;  // sequences (lists) times heads, of which each may be four blocks of rows, and keys of one: their tiles are numbers for quick_div
 
 // Parts of prefixes: as many as all CTAs have in so many rounds, at most.
@@ -34,8 +34,8 @@ struct TreeCuts {
     int tile_rows, tile_room;  // rows come in tiles of tile_rows, which have the room of tile_room
     int dim;            // floats of a row
     int may_cut;
-    int parts, blocks;  // units by number: parts of each, blocks of rows of a sequence and head
-    int units;          // by number, and prefixes: that `cuts` has an entry for
+    int parts, blocks;  // units by number: parts of each (CTAs of a cluster), blocks of rows of a sequence and head
+    int units;          // by number, how many; prefixes: that `cuts` has an entry for
 };
 
 // Whether units are cut, by what the host knows: how many there are and how many tiles the longest can have.  Cut, every CTA has the same share, but most
@@ -47,24 +47,17 @@ inline bool line_is_cut(int64_t units, int64_t tiles, int sms, int worth, int an
     return tiles > anyway || tiles * (rounds * sms - units) > (int64_t)worth * sms;
 }
 
-// Parts of each unit, where units go by number: what leaves every CTA a part of eight tiles or more; where there are somewhat more units than CTAs, long ones are cut all the same, since the last
-// of them would be taken by few CTAs.
-inline int unit_parts(int64_t units, int64_t tiles, int ctas) {
-    const int64_t parts = units <= ctas ? ctas / std::max<int64_t>(units, 1) : units <= UNIT_ROUNDS * ctas ? tiles / 64 : 1;
-    return (int)std::max<int64_t>(1, std::min(std::min(parts, tiles / 8), std::max<int64_t>(1, UNIT_PLACES * ctas / units)));
-}
-
 struct LineUnit {
     TreeSeq q;
     int seq, head, first;           // first: of the sequence's rows * group
     int from, to, tiles;            // tiles of the unit that lie in the share
     int first_cta, last_cta;        // whose shares have tiles of it
-    int unit, part;                 // by number, and prefixes: the unit, the place of this part's sums
+    int unit, part;                 // prefixes: the unit, the place of this part's sums
 };
 
 #ifdef __CUDACC__
 // Walks the share of this CTA, the whole warp together: f(unit) for every unit that has tiles in it, until it answers false.
-template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, F f) {
+template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_share(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, F f) {
     // a list is a kv head's
     const int lane = threadIdx.x & 31, heads = KIND == ATTEND_LISTS ? 1 : p.cache.kv_heads, group = p.group;
     const int seqs = KIND == ATTEND_LISTS ? (int)p.tokens * p.cache.kv_heads : KIND == ATTEND_PREFIX ? p.n_groups : p.seqs;
@@ -121,6 +114,7 @@ template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_line
                 u.q.prefix = __shfl_sync(0xFFFFFFFFu, mine.prefix, l);
                 u.q.place.table += u.q.prefix >> p.cache.page_shift;
             }
+            if (KIND == ATTEND_WHOLE) u.q.prefix = __shfl_sync(0xFFFFFFFFu, mine.prefix, l), u.q.first = __shfl_sync(0xFFFFFFFFu, mine.first, l);
             if (KIND == ATTEND_PREFIX) u.q.place.table = reinterpret_cast<const int*>(__shfl_sync(0xFFFFFFFFu, reinterpret_cast<uint64_t>(mine.place.table), l));
             u.seq = s0 + l;
             u.tiles = tiles_of(u.q);
@@ -163,34 +157,49 @@ __device__ __forceinline__ int part_begins(int tiles, int parts, int part) {
 }
 
 // Walks the units that this CTA has by their number, the whole warp together.
+// In a cluster every CTA has a part, if only one without tiles.
 template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_units(const TreeParams& p, const TreeCuts& c, int unit_rows, F f) {
-    const int heads = p.cache.kv_heads, items = c.units * c.parts;  // below 2^20: launch_tree
+    const int heads = p.cache.kv_heads, items = c.units * c.parts;  // below 2^23: launch_units
 #pragma unroll 1
     for (int item = blockIdx.x; item < items; item += gridDim.x) {
         LineUnit u;
-        u.unit = quick_div(item, c.parts);
-        const int part = item - u.unit * c.parts, per_block = quick_div(u.unit, c.blocks), block = u.unit - per_block * c.blocks;  // per_block: a sequence's (token's) kv head
+        const int unit = quick_div(item, c.parts), part = item - unit * c.parts;
+        const int per_block = quick_div(unit, c.blocks), block = unit - per_block * c.blocks;  // per_block: a sequence's (token's) kv head
         const int seq = quick_div(per_block, heads);
         u.head = per_block - seq * heads;
         u.seq = KIND == ATTEND_LISTS ? per_block : seq;
         u.q = seq_of<KIND>(p, u.seq);
         u.first = block * unit_rows;
+        if (u.first >= u.q.rows * p.group) continue;
         u.tiles = max(1, (keys_of<KIND>(u.q) + KEYS - 1) / KEYS);
-        const int parts = u.first < u.q.rows * p.group ? min(c.parts, u.tiles) : 0;
-        u.first_cta = item - part, u.last_cta = u.first_cta + parts - 1, u.part = item;
-        if (c.parts > 1 && part == 0 && parts <= 1 && (threadIdx.x & 31) == 0) c.cuts[u.unit].first_cta = -1;
-        if (part >= parts) continue;
         u.from = 0, u.to = u.tiles;
-        if (parts > 1) u.from = part_begins(u.tiles, parts, part), u.to = part_begins(u.tiles, parts, part + 1);
+        if (c.parts > 1) {
+            const int parts = min(c.parts, u.tiles);
+            u.from = part < parts ? part_begins(u.tiles, parts, part) : u.tiles, u.to = part < parts ? part_begins(u.tiles, parts, part + 1) : u.tiles;
+        }
         if (!f(u)) return false;
     }
     return true;
 }
 
+// For the kernel behind the one that reads the prefixes: which prefix a sequence has.  By a warp of every CTA.
+__device__ __forceinline__ void leave_prefixes(const TreeParams& p, bool none) {
+    const int lane = threadIdx.x & 31;
+    for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
+        const GroupSeqs of = group_seqs(p, g);
+        for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(none ? -1 : of.prefix, of.first);
+    }
+    if (blockIdx.x == 0) {  // those that no group has
+        const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
+        for (int s = lane; s < before; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+        for (int s = behind + lane; s < p.seqs; s += 32) p.prefix_of[s] = make_int2(-1, 0);
+    }
+}
+
 // Walks this CTA's parts of prefixes.  All CTAs have a part of `most` tiles at most in each of one, two or three rounds, whichever takes least: sum ceil(tiles / most) is not more than total /
-// most + units, so most = total / (rounds CTAs - units) is enough; where there is one group its units are alike, and rounds CTAs / units parts of each are exactly as many.  too_many: groups
-// that overlap have more units than there is room for; nothing is walked.
-template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, bool& too_many, F f) {
+// most + units, so most = total / (rounds CTAs - units) is enough; where there is one group its units are alike, and rounds CTAs / units parts of each are exactly as many.  Groups
+// that overlap may have more units than there is room for: nothing is walked then.  Every unit's entry of `cuts` is written, where a wait ran out, too.
+template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, F f) {
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, ctas = (int)gridDim.x, unit_tokens = quick_div(unit_rows, p.group);
     auto info = [&](int g) {
         TreeSeq q{};
@@ -209,12 +218,15 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const
     }
     units = __reduce_add_sync(0xFFFFFFFFu, units);
     total = __reduce_add_sync(0xFFFFFFFFu, total);
-    too_many = c.may_cut && units > c.units;
+    const bool too_many = c.may_cut && units > c.units;
     if (units == 0 || too_many) {
         if (c.may_cut && blockIdx.x == 0)
             for (int i = lane; i < c.units; i += 32) c.cuts[i].first_cta = -1;
+        if (too_many) report_status(p.status, STATUS_BAD_INDEX);
+        leave_prefixes(p, too_many);
         return true;
     }
+    bool well = true;
     int most = 1 << 28;  // tiles of a part
     TreeSeq first0 = first;  // the first group's, for all lanes
     first0.context = __shfl_sync(0xFFFFFFFFu, first.context, 0);
@@ -258,15 +270,23 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const
             u.first = (unit - u.head * blocks) * unit_rows;
             u.from = part_begins(u.tiles, parts, part), u.to = part_begins(u.tiles, parts, part + 1);
             u.first_cta = item - part, u.last_cta = u.first_cta + parts - 1, u.part = item;
-            if (c.may_cut && parts == 1 && lane == 0) c.cuts[u.unit].first_cta = -1;
-            if (!f(u)) return false;
+            if (c.may_cut && lane == 0 && (parts == 1 || (part == 0 && !well))) c.cuts[u.unit].first_cta = -1;
+            if (well) well = f(u);
         }
         at += all;
         unit_at += __shfl_sync(0xFFFFFFFFu, units_to, 31);
     }
     if (c.may_cut && blockIdx.x == 0)
         for (int i = unit_at + lane; i < c.units; i += 32) c.cuts[i].first_cta = -1;  // there are no more
-    return true;
+    leave_prefixes(p, false);
+    return well;
+}
+
+// f(unit) for every unit, or part of one, that this CTA has, the whole warp together, until it answers false.
+template <int KEYS, int KIND, UnitWay WAY, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, F f) {
+    if constexpr (WAY == UNITS_BY_NUMBER) return walk_units<KEYS, KIND>(p, c, unit_rows, f);
+    else if constexpr (WAY == UNITS_IN_PARTS) return walk_prefixes<KEYS>(p, c, unit_rows, unit_tiles, f);
+    else return walk_share<KEYS, KIND>(p, unit_rows, unit_tiles, c.may_cut, f);
 }
 
 // What a CTA leaves for tree_join_kernel: the unit that begins in its share and does not end there, if there is one.

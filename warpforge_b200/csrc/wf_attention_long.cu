@@ -30,22 +30,31 @@ static TreeParams attention_params(Context* c, const wf_kv_cache& cache, int lay
     return p;
 }
 
-// Lists.  More than 32 heads of a group are taken 32 at a time.  Many lists go to small CTAs by number, up to one an SM to large ones that share them out evenly.  Microseconds of the
-// large / the small, 32 / 8 heads of 128, lists of 256, 1024, 4096 keys: 8 lists 6.9 / 10.2, 11.0 / 10.2, 12.6 / 16.8; 128 9.3 / 10.2, 18.3 / 19.4, 53 / 50; 160 13.2 / 10.7, 25.8 / 22.0,
-// 64 / 59; 384 23.5 / 13.7, 45.8 / 36.6, 133 / 125; 800 44 / 26, 88 / 75, 264 / 262.
+// Lists.  More than 32 heads of a group are taken 32 at a time.
 template <int CHUNKS> static int launch_lists(Context* c, const TreeParams& p, cudaStream_t s) {
     const int64_t units = p.tokens * p.cache.kv_heads, keys = p.table_stride << p.cache.page_shift;
-    if (units * ((p.group + 31) / 32) > c->sm_count && units < UNIT_ITEMS && keys < UNIT_KEYS)
-        return p.group <= 16 ? launch_tree<CHUNKS, 1, ATTEND_LISTS, TA_FEW_WARPS>(c, p, units, p.group, keys, s) : launch_tree<CHUNKS, 2, ATTEND_LISTS, TA_FEW_WARPS>(c, p, units, p.group, keys, s);
-    return p.group <= 16 ? launch_tree<CHUNKS, 1, ATTEND_LISTS>(c, p, units, p.group, keys, s) : launch_tree<CHUNKS, 2, ATTEND_LISTS>(c, p, units, p.group, keys, s);
+    return p.group <= 16 ? launch_units<CHUNKS, 1, ATTEND_LISTS>(c, p, units, p.group, keys, s) : launch_units<CHUNKS, 2, ATTEND_LISTS>(c, p, units, p.group, keys, s);
 }
+
+// Tiles of 128 rows where sequences have more than 32 each; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of 24 / 8
+// heads of 64 48 / 39; 4, 16, 48 with 12 tokens of 32 / 8 heads of 128 and 400 keys 29.8 / 28.7, 38 / 43, 66 / 85.
+static bool few_rows(const TreeParams& p) { return p.max_drafts * p.group <= 32 || p.tokens * p.group <= 20 * (int64_t)p.seqs; }
+constexpr double AGAIN_BYTES = 192e6;
 
 // Prefixes, then what the sequences have of their own, which begins with the first one's sums.
 template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStream_t s) {
+    // Where little would be read again, most of it out of the L2, a sequence reads its prefix itself, and there is one kernel.  Microseconds by several kernels / by one, one token each with 100 keys of
+    // its own, (sequences - groups) x prefix in MB: 64 / 8 heads of 128, 4 sequences behind 1024 in common (12) 17.8 / 8.4, 4096 (48) 20.7 / 12.4, 16384 (192) 33.0 / 28.9; 16 behind 4096 (240) 29.4 / 26.9,
+    // 16384 (960) 36.5 / 83; 48 behind 1024 (188) 28.8 / 28.4; 32 / 32 heads, 4 behind 1024 (48) 15.2 / 13.0, 4096 (192) 24.8 / 28.2; 16 behind 1024 (240) 18.0 / 29.3.
+    const double again = (double)(p.seqs - p.n_groups) * (double)p.max_prefix * p.cache.kv_heads * p.cache.dim * 4;
+    if (again <= AGAIN_BYTES && few_rows(p)) {
+        const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_prefix + p.max_context + p.max_drafts;
+        const int rows = p.max_drafts * p.group;
+        return rows <= 16 ? launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, rows, keys, s) : launch_units<CHUNKS, 2, ATTEND_WHOLE>(c, p, units, rows, keys, s);
+    }
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
-    // the most cut units and pieces of them that any of the kernels leaves (16: CTAs of an SM times rounds)
-    const int64_t most_cuts = 16 * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
-    static_assert(4 * UNIT_ROUNDS <= 16 && UNIT_PLACES * 4 * 16 <= PREFIX_ROUNDS * 2 * PA_ROWS, "pieces of small CTAs");
+    // the most cut units and pieces of them that any of the kernels leaves
+    const int64_t most_cuts = (PREFIX_ROUNDS - 1) * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
     TreeCuts cuts{};
     uint8_t* more = nullptr;
     int rc = tree_scratch(c, s, most_cuts, pieces, &cuts, sums + p.seqs * (int64_t)sizeof(int2), &more);
@@ -53,17 +62,16 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     p.state = reinterpret_cast<float*>(more);
     p.state_dim = CHUNKS * 64;
     p.prefix_of = reinterpret_cast<int2*>(more + sums);
-    rc = launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, (int64_t)p.n_groups * p.cache.kv_heads, p.tokens, p.max_prefix, s);
+    // Up to 32 rows in all go to the kernel for few rows.  Microseconds of the call, 4 sequences with one token of 32 / 8 heads of 128 behind 1024 in common: 19.7 by tiles of 128 rows, 15.3 by tiles of 16.
+    const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads, prefix_rows = p.tokens * p.group;
+    rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s)
+         : prefix_rows > 16 ? launch_units<CHUNKS, 2, ATTEND_PREFIX>(c, p, prefixes, (int)prefix_rows, p.max_prefix, s)
+                            : launch_units<CHUNKS, 1, ATTEND_PREFIX>(c, p, prefixes, (int)prefix_rows, p.max_prefix, s);
     if (rc != WF_OK) return rc;
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_context + p.max_drafts;
     const int unit_rows = p.max_drafts * p.group;
-    // Tiles of 128 rows where sequences have more than 32; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of
-    // 24 / 8 heads of 64 48 / 39; 4, 16, 48 with 12 tokens of 32 / 8 heads of 128 and 400 keys 29.8 / 28.7, 38 / 43, 66 / 85.
-    if (unit_rows > 32 && p.tokens * p.group > 20 * (int64_t)p.seqs) return launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
-    // Small CTAs for many sequences with few rows.  Large / small, one token of 32 / 8 heads of 128 behind 512 in common: 128 units of 50, 400, 2000 keys 18.9 / 18.5, 22.6 / 25.4, 41 / 40; 384 27.9 /
-    // 22.8, 37 / 34, 82 / 81; with 20 rows (two small CTAs an SM) 384 43 / 39, 53 / 56, 93 / 136.
-    if (unit_rows <= 16 && 2 * units >= 5 * c->sm_count && units < UNIT_ITEMS && keys < UNIT_KEYS) return launch_tree<CHUNKS, 1, ATTEND_OWN, TA_FEW_WARPS>(c, p, units, unit_rows, keys, s);
-    return unit_rows <= 16 ? launch_tree<CHUNKS, 1, ATTEND_OWN>(c, p, units, unit_rows, keys, s) : launch_tree<CHUNKS, 2, ATTEND_OWN>(c, p, units, unit_rows, keys, s);
+    if (!few_rows(p)) return launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
+    return unit_rows <= 16 ? launch_units<CHUNKS, 1, ATTEND_OWN>(c, p, units, unit_rows, keys, s) : launch_units<CHUNKS, 2, ATTEND_OWN>(c, p, units, unit_rows, keys, s);
 }
 
 extern "C" {

@@ -359,7 +359,7 @@ constexpr int PA_CUT_TILES = 6, PA_CUT_ANYWAY = 15;
 template <int KIND, class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
     const TreeParams& p = t.tree;
     bool cut = false;
-    auto unit = [&](const LineUnit& u) {
+    const bool ok = walk_line<PA_KEYS, KIND, KIND == ATTEND_PREFIX ? UNITS_IN_PARTS : UNITS_ON_A_LINE>(p, t.c, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, [&](const LineUnit& u) {
         PromptItem it{};
         it.seq = u.seq, it.head = u.head, it.row0 = u.q.row0, it.rows = u.q.rows, it.context = u.q.context;
         it.keys = keys_of<KIND>(u.q);
@@ -377,26 +377,8 @@ template <int KIND, class F> __device__ __forceinline__ bool tree_items(const Pr
         }
         if (KIND == ATTEND_PREFIX) it.part = u.part;
         return f(it);
-    };
-    if constexpr (KIND == ATTEND_PREFIX) {
-        bool too_many;
-        const bool well = walk_prefixes<PA_KEYS>(p, t.c, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, too_many, unit);
-        // for the kernel behind this one: which prefix a sequence has
-        const int lane = threadIdx.x & 31;
-        if (too_many) report_status(p.status, STATUS_BAD_INDEX);
-        for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
-            const GroupSeqs of = group_seqs(p, g);
-            for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(too_many ? -1 : of.prefix, of.first);
-        }
-        if (blockIdx.x == 0) {  // those that no group has
-            const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
-            for (int s = lane; s < before; s += 32) p.prefix_of[s] = make_int2(-1, 0);
-            for (int s = behind + lane; s < p.seqs; s += 32) p.prefix_of[s] = make_int2(-1, 0);
-        }
-        return well;
-    }
-    const bool ok = walk_line<PA_KEYS, KIND>(p, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, t.c.may_cut, unit);
-    if (t.c.may_cut && !cut && (threadIdx.x & 31) == 0) t.c.cuts[blockIdx.x].first_cta = -1;
+    });
+    if (KIND != ATTEND_PREFIX && t.c.may_cut && !cut && (threadIdx.x & 31) == 0) t.c.cuts[blockIdx.x].first_cta = -1;
     return ok;
 }
 

@@ -20,6 +20,7 @@ constexpr int TA_WARPS = 8, TA_FEW_WARPS = 2;
 // Registers: 168 a thread at launch; the warps that multiply take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
 constexpr int TA_SEGMENTS = 2;     // announced ahead
+constexpr int CLUSTER_AHEAD = 4;   // CTAs of a cluster whose sums are asked for before the first are added up
 // When units are cut (line_is_cut).  Microseconds whole / cut, heads of 128: one sequence of 32 heads with 300, 600, 1000, 2000 tokens 7.2 / 8.7, 9.4 / 9.1, 11.9 / 10.7,
 // 20.3 / 12.8; 8, 16, 18, 20, 24 sequences of 8 heads with 1000 tokens 12.8 / 13.4, 15.5 / 20.1, 16.6 / 21.5, 24.9 / 22.5, 25.7 / 25.8; 16 with 1800 23.4 / 28.2; one with
 // 1250 beside 15 with 200 14.4 / 12.3.
@@ -54,7 +55,6 @@ struct alignas(16) TreeSegment {
     int slot, phase;               // of the first tile in the ring
     int last;                      // no more work
     int news, prefix;              // lists; own keys
-    int part;                      // units by number: the place of its sums
 };
 
 struct TreeTiles {
@@ -106,13 +106,44 @@ template <int WARPS> __device__ __forceinline__ bool ta_sync_or(bool v) {  // th
     return r != 0;
 }
 
-template <class S> struct TreeShared {
+// Waits for a barrier that other CTAs of the cluster arrive at, and sees what they wrote before.
+__device__ __forceinline__ bool ta_cluster_wait(void* bar, uint32_t parity) {
+    uint32_t ok = 0;
+#pragma unroll 1
+    for (uint32_t n = 0; n < (uint32_t)GEMM_WAIT_SPINS && !ok; n++)
+        asm volatile("{\n\t.reg .pred p;\n\tmbarrier.try_wait.parity.acquire.cluster.shared::cta.b64 p, [%1], %2;\n\tselp.u32 %0, 1, 0, p;\n\t}"
+                     : "=r"(ok)
+                     : "r"(g_smem_u32(bar)), "r"(parity)
+                     : "memory");
+    return ok != 0;
+}
+__device__ __forceinline__ void ta_cluster_arrive(uint32_t bar) {  // an address of map_to_rank
+    asm volatile("mbarrier.arrive.release.cluster.shared::cluster.b64 _, [%0];" ::"r"(bar) : "memory");
+}
+__device__ __forceinline__ float ta_cluster_float(uint32_t at) {
+    float v;
+    asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ float4 ta_cluster_float4(uint32_t at) {
+    float4 v;
+    asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(at) : "memory");
+    return v;
+}
+__device__ __forceinline__ void ta_cluster_sync() {  // all threads of all CTAs
+    asm volatile("barrier.cluster.arrive.release;\n\tbarrier.cluster.wait.acquire;" ::: "memory");
+}
+
+template <class S, bool CLUSTER> struct TreeShared {
     typedef S Shape;
     uint64_t full[Shape::SLOTS], empty[Shape::SLOTS];
     uint64_t seg_full[TA_SEGMENTS], seg_empty[TA_SEGMENTS];
     TreeSegment segments[TA_SEGMENTS];
     float warp_max[Shape::SETS][Shape::ROWS], warp_sums[Shape::SETS][Shape::ROWS];
     unsigned long long odd_rows;
+    // clusters: the sums of all of its CTAs lie in their shared memory; maxima and sums of weights of this one's rows
+    uint64_t joined;
+    float row_max[CLUSTER ? Shape::ROWS : 1], row_sums[CLUSTER ? Shape::ROWS : 1];
     // [number % ..] = number: the segment of that number has pages outside the cache; nobody is more than TA_SEGMENTS ahead of another
     int bad_pages[2 * TA_SEGMENTS];
     __device__ __forceinline__ volatile int& bad_page(int number) { return *reinterpret_cast<volatile int*>(&bad_pages[(unsigned)number % (2 * TA_SEGMENTS)]); }
@@ -120,8 +151,8 @@ template <class S> struct TreeShared {
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
-template <int CHUNKS, int MT, int KIND, int WARPS>
-__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeShape<CHUNKS, MT, WARPS>>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
+template <int CHUNKS, int MT, int KIND, int WARPS, bool BY_NUMBER, bool CLUSTER>
+__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeShape<CHUNKS, MT, WARPS>, CLUSTER>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
     typedef TreeShape<CHUNKS, MT, WARPS> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM, LOADERS = Shape::LOADERS;
     const TreeParams& p = t.p;
@@ -131,12 +162,14 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
     bool cut = false;  // a unit that begins here goes on in the next share
-    auto unit = [&](const LineUnit& u) {
+    const bool ok = walk_line<TA_KEYS, KIND, BY_NUMBER ? UNITS_BY_NUMBER : UNITS_ON_A_LINE>(p, t.c, ROWS, Shape::UNIT_TILES, [&](const LineUnit& u) {
         const int keys = keys_of<KIND>(u.q), count = min(ROWS, u.q.rows * group - u.first);
         // the page of a lane's tile, asked for before anything is waited for
         const int* const table = u.q.place.table;
+        const int* const shared = KIND == ATTEND_WHOLE ? p.tables + (size_t)u.q.first * p.table_stride : nullptr;
+        auto page_of = [&](int tile) { return (KIND == ATTEND_WHOLE && tile * TA_KEYS < u.q.prefix ? shared : table)[tile * TA_KEYS >> p.cache.page_shift]; };
         int tile = u.from + lane, page = 0;
-        if (tile < u.to && keys > 0) page = table[tile * TA_KEYS >> p.cache.page_shift];
+        if (tile < u.to && keys > 0) page = page_of(tile);
         if (!__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
         if (loader == 0 && lane == 0) {
             TreeSegment& d = sh->segments[seg];
@@ -145,8 +178,7 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
             if (KIND == ATTEND_LISTS) d.news = u.q.news;
             if (KIND == ATTEND_OWN) d.prefix = u.q.prefix;
             g_mbar_arrive(&sh->seg_full[seg]);
-            if (!Shape::MANY) d.part = u.part;
-            if (u.from == 0 && u.to < u.tiles) leave_cut<KIND>(t.c.cuts[Shape::MANY ? (int)blockIdx.x : u.unit], u, count);
+            if (!BY_NUMBER && u.from == 0 && u.to < u.tiles) leave_cut<KIND>(t.c.cuts[blockIdx.x], u, count);
         }
         cut |= u.from == 0 && u.to < u.tiles;
         __syncwarp();
@@ -164,7 +196,7 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
         for (int t0 = u.from; t0 < u.to; t0 += 32) {
             if (t0 > u.from) {
                 tile = t0 + lane;
-                page = tile < u.to && keys > 0 ? table[tile * TA_KEYS >> p.cache.page_shift] : 0;
+                page = tile < u.to && keys > 0 ? page_of(tile) : 0;
             }
             if (page < 0 || page >= p.cache.pages) {  // never followed: the unit's rows go key by key
                 sh->bad_page(number) = number;
@@ -192,11 +224,11 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
         number++;
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
         return true;
-    };
-    bool ok;
-    if constexpr (Shape::MANY) ok = walk_line<TA_KEYS, KIND>(p, ROWS, Shape::UNIT_TILES, t.c.may_cut, unit);
-    else ok = walk_units<TA_KEYS, KIND>(p, t.c, ROWS, unit);
-    if (Shape::MANY && t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
+    });
+    if (KIND == ATTEND_PREFIX && loader == 0) leave_prefixes(p, false);
+    if (KIND == ATTEND_WHOLE && loader == 0 && blockIdx.x == 0)
+        for (int g = lane; g < p.n_groups; g += 32) group_seqs(p, g);  // groups that no sequence's search has come to are looked at, too
+    if (!BY_NUMBER && t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
     if (!ok || !__all_sync(0xFFFFFFFFu, g_mbar_wait(&sh->seg_empty[seg], seg_phase))) return false;
     if (loader == 0 && lane == 0) {
         sh->segments[seg].last = 1;
@@ -206,15 +238,17 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
     return true;
 }
 
-template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS>
+// BY_NUMBER: a CTA finds its units by their number; else on the line.
+// CLUSTER: the CTAs of a cluster have a unit's parts, one each, and add their rows up from one another's shared memory; so there is no second kernel to join them.
+template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS, bool BY_NUMBER = false, bool CLUSTER = false>
 __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeShape<CHUNKS, MT, WARPS>::CTAS) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
     typedef TreeShape<CHUNKS, MT, WARPS> Shape;
     constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
     constexpr bool Q_KEPT = MT * CHUNKS <= 2;  // queries stay in registers; else they are read again with every tile
     extern __shared__ uint8_t raw[];
-    __shared__ TreeShared<Shape> sh_;
-    TreeShared<Shape>* const sh = &sh_;
+    __shared__ TreeShared<Shape, CLUSTER> sh_;
+    TreeShared<Shape, CLUSTER>* const sh = &sh_;
     const TreeParams& p = t.p;
     const int tid = threadIdx.x, warp = __shfl_sync(0xFFFFFFFFu, tid >> 5, 0), lane = tid & 31, g = lane >> 2, quad = lane & 3;
     const uint32_t ring = (g_smem_u32(raw) + 1023u) & ~1023u, q_smem = ring + SLOTS * SLOT_BYTES;
@@ -227,20 +261,23 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
         g_mbar_init(&sh->seg_empty[tid - 32], WARPS);
     } else if (tid == 64) {
         sh->odd_rows = 0;
+        if (CLUSTER) g_mbar_init(&sh->joined, t.c.parts);
         for (int i = 0; i < 2 * TA_SEGMENTS; i++) sh->bad_pages[i] = -1;
         prefetch_tensormap(&k_map);
         prefetch_tensormap(&v_map);
     }
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
-    __syncthreads();
+    if (CLUSTER) ta_cluster_sync();
+    else __syncthreads();
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= WARPS) {
         if (Shape::MANY) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_load<CHUNKS, MT, KIND, WARPS>(t, sh, &k_map, &v_map, ring, q_smem, warp - WARPS)) {
+        if (!tree_load<CHUNKS, MT, KIND, WARPS, BY_NUMBER, CLUSTER>(t, sh, &k_map, &v_map, ring, q_smem, warp - WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }
+        if (CLUSTER) ta_cluster_sync();  // that of the end
         return;
     }
 
@@ -454,8 +491,16 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
         ta_sync<WARPS>();
         const bool whole = w.from == 0 && w.to == w.tiles;
         // a CTA has at most two pieces of cut units: one that began before its share, one that begins in it
-        float* const piece = t.c.pieces + (Shape::MANY ? (size_t)blockIdx.x * 2 + (w.from == 0) : (size_t)w.part) * Shape::PIECE;
+        float* const piece = BY_NUMBER ? nullptr : t.c.pieces + ((size_t)blockIdx.x * 2 + (w.from == 0)) * Shape::PIECE;
         auto store = [&](int r, int col, const float4& x, float sum, float top) {  // four elements of a row, or zeros where it sees nothing
+            if (KIND == ATTEND_PREFIX) {  // the keys behind the prefix are another kernel's
+                const int token = p.token_of(w.first + r);
+                const size_t at = (size_t)(w.row0 + token) * p.q_heads + w.head * group + (w.first + r) - token * group;
+                *reinterpret_cast<float4*>(p.state + at * p.state_dim + col) = x;
+                if (col == 0) p.state_maxima()[at] = top, p.state_weights()[at] = sum;
+                return;
+            }
+            if (col >= d) return;
             const float inv = sum == 0.f ? 0.f : 1.f / sum;
             uint32_t largest = sum < INFINITY && !scores_too_large(top, scale) ? 0 : 0x7F800000u;
             largest = max(max(largest, __float_as_uint(x.x) & 0x7FFFFFFFu), max(__float_as_uint(x.y) & 0x7FFFFFFFu, max(__float_as_uint(x.z) & 0x7FFFFFFFu, __float_as_uint(x.w) & 0x7FFFFFFFu)));
@@ -465,8 +510,10 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
             *reinterpret_cast<uint2*>(to) = make_uint2(pack_bf16(x.x * inv, x.y * inv), pack_bf16(x.z * inv, x.w * inv));
         };
         constexpr int PER_ROW = DIM / 4;  // threads of a row
+        auto place = [&](int set, int r, int n) { return merge + (size_t)(set * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4; };
+        // the sums of this CTA's warps
 #pragma unroll 1
-        for (int i = tid; i < count * PER_ROW; i += WARPS * 32) {
+        for (int i = CLUSTER && SETS == 1 ? count * PER_ROW : tid; i < count * PER_ROW; i += WARPS * 32) {
             const int r = i / PER_ROW, n = i % PER_ROW;
             float top = -INFINITY, sum = 0.f, tops[SETS];
             float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
@@ -477,11 +524,14 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
             for (int c = 0; c < SETS; c++) {
                 const float keep = line_ex2((tops[c] - ref) * scale);
                 sum += sh->warp_sums[c][r] * keep;
-                const float4 v = *reinterpret_cast<const float4*>(merge + (size_t)(c * ROWS + r) * DIM + ((n >> 1) ^ (r & 3)) * 8 + (n & 1) * 4);
+                const float4 v = *reinterpret_cast<const float4*>(place(c, r, n));
                 x.x += v.x * keep, x.y += v.y * keep, x.z += v.z * keep, x.w += v.w * keep;
             }
-            if (whole) {
-                if (4 * n < d) store(r, 4 * n, x, sum, top);
+            if (CLUSTER) {
+                *reinterpret_cast<float4*>(place(0, r, n)) = x;
+                if (n == 0) sh->row_max[r] = top, sh->row_sums[r] = sum;
+            } else if (BY_NUMBER || whole) {
+                store(r, 4 * n, x, sum, top);
             } else {
                 *reinterpret_cast<float4*>(piece + r * DIM + 4 * n) = x;
                 if (n == 0) {
@@ -490,9 +540,53 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
                 }
             }
         }
+        if (CLUSTER) {
+            // Every CTA has its rows' sums where the others find them; a row is added up by the CTA with its number, modulo the CTAs there are.
+            const int ranks = t.c.parts, rank = (int)cluster_rank();
+            ta_sync<WARPS>();
+            if (tid < ranks) ta_cluster_arrive(map_to_rank(g_smem_u32(&sh->joined), (uint32_t)tid));
+            if (ta_sync_or<WARPS>(!ta_cluster_wait(&sh->joined, 0))) {
+                failed = true;
+                break;
+            }
+            const uint32_t maxima = g_smem_u32(SETS == 1 ? sh->warp_max[0] : sh->row_max), weights = g_smem_u32(SETS == 1 ? sh->warp_sums[0] : sh->row_sums);
+#pragma unroll 1
+            for (int i = tid; i < (count - rank + ranks - 1) / ranks * PER_ROW; i += WARPS * 32) {
+                const int r = rank + i / PER_ROW * ranks, n = i % PER_ROW;
+                float top = -INFINITY, sum = 0.f;
+                float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll 1
+                for (int c0 = 0; c0 < ranks; c0 += CLUSTER_AHEAD) {
+                    float4 v[CLUSTER_AHEAD];
+                    float m_of[CLUSTER_AHEAD], l_of[CLUSTER_AHEAD];
+#pragma unroll
+                    for (int e = 0; e < CLUSTER_AHEAD; e++) {
+                        const uint32_t from = (uint32_t)min(c0 + e, ranks - 1);
+                        v[e] = ta_cluster_float4(map_to_rank(g_smem_u32(place(0, r, n)), from));
+                        m_of[e] = ta_cluster_float(map_to_rank(maxima + 4 * r, from));
+                        l_of[e] = ta_cluster_float(map_to_rank(weights + 4 * r, from));
+                    }
+                    float grown = top;
+#pragma unroll
+                    for (int e = 0; e < CLUSTER_AHEAD; e++) grown = c0 + e < ranks ? fmaxf(grown, m_of[e]) : grown;
+                    const float ref = grown == -INFINITY ? 0.f : grown, keep = line_ex2((top - ref) * scale);
+                    top = grown;
+                    sum *= keep;
+                    x.x *= keep, x.y *= keep, x.z *= keep, x.w *= keep;
+#pragma unroll
+                    for (int e = 0; e < CLUSTER_AHEAD; e++) {
+                        if (c0 + e >= ranks) break;
+                        const float take = line_ex2((m_of[e] - ref) * scale);
+                        sum += l_of[e] * take;
+                        x.x += v[e].x * take, x.y += v[e].y * take, x.z += v[e].z * take, x.w += v[e].w * take;
+                    }
+                }
+                store(r, 4 * n, x, sum, top);
+            }
+        }
         ta_sync<WARPS>();
         const unsigned long long odd = sh->odd_rows;
-        if (odd) {
+        if (KIND != ATTEND_PREFIX && odd) {
             // An Inf or a NaN in a row's sums may have come from a key that it does not see (0 x Inf), or from a page that is not in the cache: key by key.
             ta_sync<WARPS>();
             if (tid == 0) sh->odd_rows = 0;
@@ -508,6 +602,7 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
         if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
         drain_after_abort();
     }
+    if (CLUSTER) ta_cluster_sync();  // no CTA goes while another may read from it or arrive at its barrier
 }
 
 }  // namespace wf
