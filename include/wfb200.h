@@ -355,7 +355,7 @@ int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, 
  *   codes_dev   int8 [layers][pages][kv_heads][2][head_dim], 16-byte aligned: upper bounds, lower bounds
  *   scales_dev  fp32 [layers][pages][kv_heads]
  *   tables_dev  int32 [seqs][table_stride]; first_dev, stop_dev int32 [seqs]
- *   max_tokens  most tokens stop[s] - first[s] of a sequence; a longer range is WF_ERR_INDEX and left out
+ *   max_tokens  most tokens stop[s] - first[s] of a sequence; a range of more pages than so many tokens can touch is WF_ERR_INDEX and left out
  * Sequences that share a page should agree on how many of its tokens count: else the bounds are one or the other's. */
 int wf_page_bounds(int64_t ctx, const wf_kv_cache* cache, int64_t codes_dev, int64_t scales_dev, int64_t tables_dev, int64_t table_stride, int64_t first_dev, int64_t stop_dev,
                    int64_t seqs, int64_t max_tokens, int64_t stream);

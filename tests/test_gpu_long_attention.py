@@ -543,3 +543,98 @@ def test_shared_and_selected_recorded(backend):
             assert (got.float() - want.float()).abs().max() <= 2.0**-6 * values.float().abs().max()  # as in test_shared_is_what_trees_are
     ctx.graph_destroy(graph)
     backend.destroy_stream(stream)
+
+
+@several
+def test_shared_queries_with_gaps_and_rows_behind(backend, several):
+    """Tokens that lie further apart than they are long, on another stream; rows behind the last sequence stay as they were."""
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(12)
+    wide = normal(rng, 5, 7 * 64)
+    q, keys, values = wide[:, :4 * 64].unflatten(1, (4, 64)), normal(rng, 40, 2, 16, 64), normal(rng, 40, 2, 16, 64)
+    tables, context, groups, prefix, off = torch.arange(40, dtype=torch.int32, device="cuda").repeat(3, 1), i32([70, 64, 64]), i32([0, 3]), i32([64]), i32([0, 2, 2, 3])
+    out = torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
+    stream = backend.create_stream()
+    torch.cuda.synchronize()
+    A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR if several else 64, max_own=6,
+                            q_offsets=held(off), max_drafts=2).run(stream)
+    backend.synchronize_stream(stream)
+    assert (out[3:] == 7).all()
+    for row, n in ((0, 71), (1, 72), (2, 65)):
+        k, v = (x.transpose(1, 2).flatten(0, 1)[:n].double().cpu() for x in (keys, values))
+        for h in range(4):
+            want, spread = formula(q[row, h][None].double().cpu(), k[:, h // 2], v[:, h // 2], 1 / 8, torch.ones(1, n, dtype=torch.bool))
+            check(out[row, h][None], want, spread)
+    backend.destroy_stream(stream)
+
+
+def test_a_step_as_it_is_used(backend):
+    """Keys into the cache, bounds, selection, attention over the lists, on one stream with nothing between, three layers one after the other: every layer's attention is that of the pages that
+    were selected for it."""
+    import torch
+
+    from test_gpu_select import plain_list
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(13)
+    ctx, layers, pages, page, heads, dim, width = backend.cuda_context, 3, 60, 16, 2, 64, 8
+    lens, drafts = [300, 100, 17], [5, 1, 3]
+    n = sum(drafts)
+    tables, _ = pages_for([a + b for a, b in zip(lens, drafts)], page, rng, spare=20)
+    tables[tables > 1000] = 0
+    cache = A.KvCache(ctx, layers, pages, page, heads, dim)
+    bounds = A.PageBounds(cache)
+    tab, off, context = torch.from_numpy(tables).cuda(), i32(offsets(drafts)), i32(lens)
+    past = [t for m in lens for t in range(m)]
+    past_slots = torch.tensor([int(tables[s][t // page]) * page + t % page for s, m in enumerate(lens) for t in range(m)], dtype=torch.int64, device="cuda")
+    slots = torch.tensor([int(tables[s][(m + i) // page]) * page + (m + i) % page for s, (m, d) in enumerate(zip(lens, drafts)) for i in range(d)], dtype=torch.int64, device="cuda")
+    zero, total = i32([0] * 3), i32([a + b for a, b in zip(lens, drafts)])
+    outs = [torch.zeros(n, 4, dim, dtype=torch.bfloat16, device="cuda") for _ in range(layers)]
+    lists = [torch.zeros(n, heads, width, dtype=torch.int32, device="cuda") for _ in range(layers)]
+    list_lens = [torch.zeros(n, heads, 2, dtype=torch.int32, device="cuda") for _ in range(layers)]
+    qb = [torch.zeros(n, 4, dim, dtype=torch.bfloat16, device="cuda") for _ in range(layers)]
+    q, k, v = (torch.from_numpy(rng.standard_normal((layers, n, h, dim)).astype(np.float32)).cuda() for h in (4, heads, heads))
+    pk, pv = (torch.from_numpy(rng.standard_normal((layers, len(past), heads, dim)).astype(np.float32)).cuda() for _ in range(2))
+    words = signed([w for m in drafts for w in tree_words(m, rng, "tree")])
+    torch.cuda.synchronize()
+    for layer in range(layers):
+        A.QkNormRope(ctx, None, held(pk[layer]), held(pv[layer]), None, *cache.layer(layer), None, None, slots=held(past_slots)).run()
+    bounds.update(held(tab), held(zero), held(context), max_tokens=300)
+    for layer in range(layers):
+        keys, values = cache.layer(layer)
+        A.QkNormRope(ctx, held(q[layer]), held(k[layer]), held(v[layer]), held(qb[layer]), keys, values, None, None, slots=held(slots)).run()
+        A.SelectPages(ctx, held(qb[layer]), *bounds.layer(layer), held(tab), held(context), held(lists[layer]), held(list_lens[layer]), page_tokens=page, max_context=300, recent=20,
+                      q_offsets=held(off), max_drafts=5, tree=True).run()
+        A.SelectedAttention(ctx, held(qb[layer]), keys, values, held(outs[layer]), held(lists[layer]), held(list_lens[layer]), ancestors=held(words)).run()
+    bounds.update(held(tab), held(context), held(total), max_tokens=5)
+    backend.synchronize_device()
+
+    def host(t, dtype):
+        a = np.empty(t.shape(), dtype)
+        ctx.copy_to_host(a, t.ptr)
+        return a
+
+    all_k, all_v = (torch.from_numpy((host(t, np.uint16).astype(np.uint32) << 16).view(np.float32)).double() for t in (cache.keys, cache.values))
+    codes, scales = host(bounds.codes, np.int8).astype(np.float64), host(bounds.scales, np.float32).astype(np.float64)
+    for layer in range(layers):
+        for s, (m, d) in enumerate(zip(lens, drafts)):
+            for i in range(d):
+                row = offsets(drafts)[s] + i
+                for h in range(heads):
+                    got, got_lens = lists[layer][row, h].tolist(), list_lens[layer][row, h].tolist()
+                    # (full pages' bounds are the same before and after the new tokens)
+                    assert (got, got_lens) == plain_list(qb[layer][row, 2 * h:2 * h + 2].double().cpu().numpy(), codes[layer, :, h], scales[layer, :, h], tables[s], m, d, i, True, page, width, 1, 20)
+                    t = np.arange(got_lens[1])
+                    names = torch.tensor(got)[torch.from_numpy(t // page)]
+                    kk, vv = all_k[layer, names, h, torch.from_numpy(t % page)], all_v[layer, names, h, torch.from_numpy(t % page)]
+                    seen = torch.ones(1, len(t), dtype=torch.bool)
+                    for j in range(d):
+                        seen[0, got_lens[0] + j] = bool(int(words[row]) >> j & 1)
+                    for g in range(2):
+                        want, spread = formula(qb[layer][row, 2 * h + g][None].double().cpu(), kk, vv, 1 / 8, seen)
+                        check(outs[layer][row, 2 * h + g][None], want, spread)
+    bounds.close()
+    cache.close()

@@ -262,6 +262,17 @@ def test_select_many_pages(backend, pages, tokens):
     run_select(backend, [16 * pages + 3], [tokens], 8, 4 if pages == 1500 else 1, 64, 16, 100)
 
 
+def test_select_most_pages(backend):
+    """As many pages as a call may have, by as many heads as a group may have; one more is refused."""
+    from warpforge_b200 import _native as N
+
+    run_select(backend, [16 * N.WF_SELECT_MAX_PAGES], [1], 128, 1, 8, 16, 60)
+    run_select(backend, [16 * N.WF_SELECT_MAX_PAGES], [2], 2, 1, 128, 16, 60)
+    with pytest.raises(N.WfError) as e:
+        run_select(backend, [16 * N.WF_SELECT_MAX_PAGES + 1], [1], 2, 1, 8, 16, 60)
+    assert e.value.status == N.WF_ERR_TOO_LARGE
+
+
 def test_select_ties_of_many_tokens(backend):
     def two(q, codes, scales, tables):
         codes[:] = codes[0, 0, 0, 0]
