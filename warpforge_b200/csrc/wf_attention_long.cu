@@ -30,10 +30,12 @@ static TreeParams attention_params(Context* c, const wf_kv_cache& cache, int lay
     return p;
 }
 
-// Lists.  More than 32 heads of a group are taken 32 at a time.
-template <int CHUNKS> static int launch_lists(Context* c, const TreeParams& p, cudaStream_t s) {
-    const int64_t units = p.tokens * p.cache.kv_heads, keys = p.table_stride << p.cache.page_shift;
-    return p.group <= 16 ? launch_units<CHUNKS, 1, ATTEND_LISTS>(c, p, units, p.group, keys, s) : launch_units<CHUNKS, 2, ATTEND_LISTS>(c, p, units, p.group, keys, s);
+// Units of up to `rows` rows, 16 or 32 of them at a time.  17 to 32 go 16 at a time, and read their keys twice, where that is little, or where it keeps many short units off the line.  Microseconds 32 / 16 at
+// a time, 20 rows of 8 heads of 128: 32 units of 300, 750 keys 11.4 / 7.8, 11.2 / 8.9; 128 12.0 / 12.2, 17.0 / 17.9; 320 28.8 / 22.9, 39 / 42.
+template <int CHUNKS, int KIND> static int launch_rows(Context* c, const TreeParams& p, int64_t units, int64_t rows, int64_t keys, cudaStream_t s) {
+    const int64_t tiles = (keys + TA_KEYS - 1) / TA_KEYS;
+    const bool twice = rows <= 32 && (2.0 * units * tiles <= 48.0 * c->sm_count || (2 * units > c->sm_count && tiles <= 32));
+    return rows <= 16 || twice ? launch_units<CHUNKS, 1, KIND>(c, p, units, (int)rows, keys, s) : launch_units<CHUNKS, 2, KIND>(c, p, units, (int)rows, keys, s);
 }
 
 // Tiles of 128 rows where sequences have more than 32 each; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of 24 / 8
@@ -49,8 +51,7 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     const double again = (double)(p.seqs - p.n_groups) * (double)p.max_prefix * p.cache.kv_heads * p.cache.dim * 4;
     if (again <= AGAIN_BYTES && few_rows(p)) {
         const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_prefix + p.max_context + p.max_drafts;
-        const int rows = p.max_drafts * p.group;
-        return rows <= 16 ? launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, rows, keys, s) : launch_units<CHUNKS, 2, ATTEND_WHOLE>(c, p, units, rows, keys, s);
+        return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, p.max_drafts * p.group, keys, s);
     }
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
     // the most cut units and pieces of them that any of the kernels leaves
@@ -64,14 +65,10 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     p.prefix_of = reinterpret_cast<int2*>(more + sums);
     // Up to 32 rows in all go to the kernel for few rows.  Microseconds of the call, 4 sequences with one token of 32 / 8 heads of 128 behind 1024 in common: 19.7 by tiles of 128 rows, 15.3 by tiles of 16.
     const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads, prefix_rows = p.tokens * p.group;
-    rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s)
-         : prefix_rows > 16 ? launch_units<CHUNKS, 2, ATTEND_PREFIX>(c, p, prefixes, (int)prefix_rows, p.max_prefix, s)
-                            : launch_units<CHUNKS, 1, ATTEND_PREFIX>(c, p, prefixes, (int)prefix_rows, p.max_prefix, s);
+    rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s) : launch_rows<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, prefix_rows, p.max_prefix, s);
     if (rc != WF_OK) return rc;
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_context + p.max_drafts;
-    const int unit_rows = p.max_drafts * p.group;
-    if (!few_rows(p)) return launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
-    return unit_rows <= 16 ? launch_units<CHUNKS, 1, ATTEND_OWN>(c, p, units, unit_rows, keys, s) : launch_units<CHUNKS, 2, ATTEND_OWN>(c, p, units, unit_rows, keys, s);
+    return few_rows(p) ? launch_rows<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts * p.group, keys, s) : launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
 }
 
 extern "C" {
@@ -91,7 +88,9 @@ int wf_selected_attention(int64_t ctx, const wf_selected_attention_args* a, cons
     p.table_stride = a->width;
     p.lens = reinterpret_cast<const int2*>(a->lens_dev);
     p.ancestors = reinterpret_cast<const uint64_t*>(a->ancestors_dev);
-    return dim_chunks(cache->head_dim) == 1 ? launch_lists<1>(c, p, s) : launch_lists<2>(c, p, s);
+    // (more than 32 heads of a group are taken 32 at a time)
+    const int64_t units = p.tokens * cache->kv_heads, keys = p.table_stride << p.cache.page_shift;
+    return dim_chunks(cache->head_dim) == 1 ? launch_rows<1, ATTEND_LISTS>(c, p, units, p.group, keys, s) : launch_rows<2, ATTEND_LISTS>(c, p, units, p.group, keys, s);
 }
 
 int wf_shared_prefix_attention(int64_t ctx, const wf_shared_prefix_attention_args* a, const wf_kv_cache* cache, int layer, int64_t stream) {
