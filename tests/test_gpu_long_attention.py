@@ -452,6 +452,36 @@ def test_shared_outside(backend, several):
             check(out[t, h][None], w, spread)
 
 
+@pytest.mark.parametrize("groups", [[0, 40] * 20, list(range(0, 41, 4)) + list(range(0, 37, 4)), list(range(0, 41, 2)) + list(range(0, 39, 2))])
+def test_shared_groups_that_overlap(backend, groups):
+    """More rows in groups than there are tokens: reported, and no more work than a batch that can be has (as many groups as sequences: each sequence reads for itself, and may find a group
+    that it is in); the next call is as ever."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(4)
+    q, keys, values = normal(rng, 40, 8, 64), normal(rng, 30, 2, 16, 64), normal(rng, 30, 2, 16, 64)
+    tables, context = torch.arange(30, dtype=torch.int32, device="cuda").repeat(40, 1), i32([470] * 40)
+
+    def run(groups):
+        out, gr, pre = torch.full_like(q, 7.0), i32(groups), i32([320] * (len(groups) - 1))
+        torch.cuda.synchronize()
+        A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(gr), held(pre), max_prefix=FAR, max_own=200).run()
+        return out
+
+    good = run([0, 40])
+    backend.synchronize_device()
+    out = run(groups)
+    with pytest.raises(N.WfError) as e:
+        backend.synchronize_device()
+    assert e.value.status == N.WF_ERR_INDEX and (len(groups) == 41 or torch.count_nonzero(out) == 0)
+    again = run([0, 40])
+    backend.synchronize_device()
+    assert torch.equal(again, good)
+
+
 def test_shared_is_what_trees_are(backend):
     """The same call with and without a prefix, and by TreeAttention: sums of the same products in other parts and orders.  Each is off by at most 2^-8 |out| + 2^-8 sum p |v| (check), and neither
     of these is more than the largest |v|: two results differ by at most 2 (2^-8 + 2^-8) max |v| = 2^-6 max |v|."""

@@ -198,7 +198,7 @@ __device__ __forceinline__ void leave_prefixes(const TreeParams& p, bool none) {
 
 // Walks this CTA's parts of prefixes.  All CTAs have a part of `most` tiles at most in each of one, two or three rounds, whichever takes least: sum ceil(tiles / most) is not more than total /
 // most + units, so most = total / (rounds CTAs - units) is enough; where there is one group its units are alike, and rounds CTAs / units parts of each are exactly as many.  Groups
-// that overlap may have more units than there is room for: nothing is walked then.  Every unit's entry of `cuts` is written, where a wait ran out, too.
+// that overlap may have more rows than there are tokens, and more units than there is room for: nothing is walked then.  Every unit's entry of `cuts` is written, where a wait ran out, too.
 template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, F f) {
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, ctas = (int)gridDim.x, unit_tokens = quick_div(unit_rows, p.group);
     auto info = [&](int g) {
@@ -210,15 +210,16 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const
     auto units_of = [&](const TreeSeq& q) { return blocks_of(q) * heads; };
     auto tiles_of = [&](const TreeSeq& q) { return (q.context + KEYS - 1) / KEYS; };
     const TreeSeq first = info(lane);
-    int units = units_of(first), total = units * tiles_of(first);
+    int units = units_of(first), total = units * tiles_of(first), rows = first.rows;
 #pragma unroll 1
     for (int g0 = 32; g0 < p.n_groups; g0 += 32) {
         const TreeSeq q = info(g0 + lane);
         units += units_of(q), total += units_of(q) * tiles_of(q);
+        rows = min(rows + q.rows, 1 << 18);  // (there are 2^17 tokens at most)
     }
     units = __reduce_add_sync(0xFFFFFFFFu, units);
     total = __reduce_add_sync(0xFFFFFFFFu, total);
-    const bool too_many = c.may_cut && units > c.units;
+    const bool too_many = __reduce_add_sync(0xFFFFFFFFu, rows) > p.tokens || (c.may_cut && units > c.units);
     if (units == 0 || too_many) {
         if (c.may_cut && blockIdx.x == 0)
             for (int i = lane; i < c.units; i += 32) c.cuts[i].first_cta = -1;
