@@ -117,7 +117,7 @@ def test_selected_on_every_way(backend):
     run_selected(backend, [2100] * 76, [1] * 76, 16, 8, 64, 16, pages=140, heads=[0, 7])                    # 608 long ones: a line
     run_selected(backend, [700 + 9 * i for i in range(10)], [1] * 10, 160, 8, 128, 16, pages=140, heads=[7])  # 80 with 20 rows: a line
     run_selected(backend, [700 + 9 * i for i in range(9)], [1] * 9, 160, 8, 128, 16, pages=140, heads=[0])    # 72 with 20 rows: clusters of 2
-    for tokens in (1, 3, 9, 12, 17, 24, 40):
+    for tokens in (1, 3, 9, 12, 17, 24, 40, 60, 80):
         run_selected(backend, [1 + (37 * i) % 600 for i in range(tokens)], [1] * tokens, 16, 8, 128, 16, width=38, pages=60, heads=[0, 3])
 
 

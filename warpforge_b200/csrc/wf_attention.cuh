@@ -340,4 +340,29 @@ __device__ __forceinline__ void attend_again(const TreeParams& p, const Unit& w,
 }
 #endif
 
+CacheView cache_layer(const wf_kv_cache& cache, int layer);
+int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too);
+
+// A launch that may begin before the kernel in front of it ends.
+template <class... Params, class... Args>
+inline int launch_clusters(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, unsigned cluster, size_t smem, cudaStream_t s, const Args&... args) {
+    cudaLaunchConfig_t cfg = {};
+    cfg.gridDim = grid;
+    cfg.blockDim = dim3(threads);
+    cfg.dynamicSmemBytes = smem;
+    cfg.stream = s;
+    cudaLaunchAttribute attr[2];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    attr[1].id = cudaLaunchAttributeClusterDimension;
+    attr[1].val.clusterDim.x = cluster;
+    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = cluster > 1 ? 2 : 1;
+    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
+    if (e != cudaSuccess) return cuda_status(c, e, what);
+    c->launches++;
+    return WF_OK;
+}
+
 }  // namespace wf

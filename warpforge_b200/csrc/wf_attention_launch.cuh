@@ -8,9 +8,6 @@
 
 namespace wf {
 
-CacheView cache_layer(const wf_kv_cache& cache, int layer);
-int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too);
-
 inline int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
     if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
     if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
@@ -20,27 +17,6 @@ inline int check_queries(Context* c, const char* what, int64_t q, int64_t out, i
     if (q_stride < (int64_t)q_heads * cache->head_dim || q_stride % 8) return set_error(c, WF_ERR_SHAPE, "%s: q_stride %lld", what, (long long)q_stride);
     return WF_OK;
 }
-template <class... Params, class... Args>
-inline int launch_clusters(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, unsigned cluster, size_t smem, cudaStream_t s, const Args&... args) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, args...);
-    if (e != cudaSuccess) return cuda_status(c, e, what);
-    c->launches++;
-    return WF_OK;
-}
-
 template <class... Params, class... Args>
 inline int launch_attention(Context* c, const char* what, void (*kernel)(Params...), dim3 grid, unsigned threads, size_t smem, cudaStream_t s, const Args&... args) {
     return launch_clusters(c, what, kernel, grid, threads, 1, smem, s, args...);
@@ -110,10 +86,10 @@ template <int CHUNKS, int MT, int KIND> inline int launch_tree(Context* c, const
     rc = launch_attention(c, what, tree_tiles_kernel<CHUNKS, MT, KIND>, grid, Shape::THREADS, (size_t)Shape::SMEM, s, t, k, v);
     return rc == WF_OK && t.c.may_cut ? launch_join<KIND, false>(c, p, t.c, grid, Shape::ROWS, s) : rc;
 }
-// Units by number: each in a CTA, or in a cluster's.
-template <int CHUNKS, int MT, int KIND, int WARPS, bool CLUSTER> inline int launch_numbered(Context* c, const TreeParams& p, int64_t units, int parts, int64_t blocks, cudaStream_t s) {
-    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
-    auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, WARPS, true, CLUSTER>;
+// Units by number, each in a CTA or a cluster.  CTAS of an SM.
+template <int CHUNKS, int MT, int KIND, int CTAS, bool CLUSTER> inline int launch_numbered(Context* c, const TreeParams& p, int64_t units, int parts, int64_t blocks, cudaStream_t s) {
+    typedef TreeShape<CHUNKS, MT, CTAS> Shape;
+    auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, CTAS, true, CLUSTER>;
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     if (!(ready.load() >> (c->device & 63) & 1)) {
         WF_CUDA(c, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, Shape::SMEM));
@@ -128,16 +104,16 @@ template <int CHUNKS, int MT, int KIND, int WARPS, bool CLUSTER> inline int laun
     int rc = encode_cache(c, &k, p.cache.keys, p.cache, TA_KEYS);
     if (rc == WF_OK) rc = encode_cache(c, &v, p.cache.values, p.cache, TA_KEYS);
     if (rc != WF_OK) return rc;
-    const unsigned grid = CLUSTER ? (unsigned)(units * parts) : (unsigned)std::min<int64_t>(units, c->sm_count * Shape::CTAS);
+    const unsigned grid = CLUSTER ? (unsigned)(units * parts) : (unsigned)std::min<int64_t>(units, c->sm_count * CTAS);
     return launch_clusters(c, "tree_attention", kernel, dim3(grid), Shape::THREADS, (unsigned)parts, (size_t)Shape::SMEM, s, t, k, v);
 }
 // Clusters of so many CTAs that the device has at a time.
-template <int CHUNKS, int MT, int KIND, int WARPS> inline int clusters_at_once(Context* c, int size) {
-    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+template <int CHUNKS, int MT, int KIND, int CTAS> inline int clusters_at_once(Context* c, int size) {
+    typedef TreeShape<CHUNKS, MT, CTAS> Shape;
     static std::atomic<int> known[64][MAX_CLUSTER + 1];  // and one more; 0: not asked
     std::atomic<int>& held = known[c->device & 63][size];
     if (held.load() == 0) {
-        auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, WARPS, true, true>;
+        auto* const kernel = tree_tiles_kernel<CHUNKS, MT, KIND, CTAS, true, true>;
         cudaLaunchConfig_t cfg = {};
         cfg.gridDim = dim3((unsigned)size * 1024);
         cfg.blockDim = dim3(Shape::THREADS);
@@ -157,21 +133,26 @@ template <int CHUNKS, int MT, int KIND, int WARPS> inline int clusters_at_once(C
     }
     return held.load() - 1;
 }
-// How units with few rows go to the SMs.  Up to one an SM, the parts of a unit go to a cluster of large CTAs, as many as let all units be there at once; then to clusters of small CTAs, of
-// which an SM has four; then each to a small CTA of its own; where those are not enough and units are long, to large CTAs that share a line of them.  Microseconds for lists of 256 / 4096 keys, 32 / 8
-// heads of 128, on the line and as chosen here: 8 units 7.0 / 12.6 and 6.6 / 9.2 (clusters of 8), 24 7.1 / 16.6 and 6.8 / 14.3 (4), 72 8.4 / 34 and 6.9 / 28.6 (2), 128 9.1 / 53 and 8.0 / 46.6 (4
-// small), 192 14.1 / 73 and 9.2 / 66 (2 small), 320 21.6 / 115 and 12.4 / 108, 640 36 / 215 and 23 / 249.  With 17 to 32 rows an SM has two small CTAs, and the line is quicker: 64 units of 2048 keys
-// 24.4 and 20.6 (2 large), 80 27.9 against 33 (3 small), 192 49 against 69.
+// How units with few rows go to the SMs.  Up to one an SM, the parts of a unit go to a cluster of large CTAs, as many as let all units be there at once; then to clusters of small CTAs; then
+// each to a small CTA of its own.  An SM has three of them (a fourth where that spares a second round of units); where there are more and they are long, large CTAs share a line of them, since of
+// units that a CTA takes one after the other two may be long.  Microseconds for lists of 256 / 4096 keys, 32 / 8 heads of 128, on the line and in clusters: 8 units 7.0 / 12.6 and 6.6 / 9.2
+// (clusters of 8), 24 7.1 / 16.6 and 6.8 / 14.3 (4), 72 8.4 / 34 and 6.9 / 28.6 (2), 128 9.1 / 53 and 8.0 / 46.6 (4 small), 192 14.1 / 73 and 8.8 / 66 (2 small).  Of 256 / 2048 keys, with four
+// small CTAs and with three: 352 units 13.2 / 63 and 12.3 / 61, 480 15.9 / 79 and 20.2 / 102, 576 17.6 / 94 and 21 / 105, 640 24.2 / 130 and 21.4 / 109, 1200 35 / 209 and 31 / 193 (36 / 215 on the line for
+// 640 of 256 / 4096 keys).  800 units of 2560, 4096 keys, alike: 177, 267 on the line, 161, 248 in threes; 640 of 200 to 6000: 158 and 177; 800, most of 30 keys, one in eight of 6000: 77 and 185.
+// Of 17 to 32 rows an SM would have two small CTAs, and the line is quicker: 80 units of 2048 keys 27.9 against 33, 192 49 against 69.
 template <int CHUNKS, int MT, int KIND> inline int launch_units(Context* c, const TreeParams& p, int64_t units, int unit_rows, int64_t unit_keys, cudaStream_t s) {
     const int64_t blocks = (unit_rows + 16 * MT - 1) / (16 * MT), all = units * blocks, tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
     if (units < UNIT_ITEMS && unit_keys < UNIT_KEYS) {
         for (int parts = MAX_CLUSTER; parts > 1; parts /= 2)
-            if (tiles >= 8 * parts && all <= clusters_at_once<CHUNKS, MT, KIND, TA_WARPS>(c, parts)) return launch_numbered<CHUNKS, MT, KIND, TA_WARPS, true>(c, p, all, parts, blocks, s);
+            if (tiles >= 8 * parts && all <= clusters_at_once<CHUNKS, MT, KIND, 1>(c, parts)) return launch_numbered<CHUNKS, MT, KIND, 1, true>(c, p, all, parts, blocks, s);
         if constexpr (MT == 1) {
             for (int parts = MAX_CLUSTER / 2; parts > 1; parts--)
-                if (tiles >= 4 * parts && all <= clusters_at_once<CHUNKS, MT, KIND, TA_FEW_WARPS>(c, parts))
-                    return launch_numbered<CHUNKS, MT, KIND, TA_FEW_WARPS, true>(c, p, all, parts, blocks, s);
-            if (all <= c->sm_count * TreeShape<CHUNKS, MT, TA_FEW_WARPS>::CTAS || tiles <= 128) return launch_numbered<CHUNKS, MT, KIND, TA_FEW_WARPS, false>(c, p, all, 1, blocks, s);
+                if (tiles >= 4 * parts) {
+                    if (all <= clusters_at_once<CHUNKS, MT, KIND, 3>(c, parts)) return launch_numbered<CHUNKS, MT, KIND, 3, true>(c, p, all, parts, blocks, s);
+                    if (all <= clusters_at_once<CHUNKS, MT, KIND, 4>(c, parts)) return launch_numbered<CHUNKS, MT, KIND, 4, true>(c, p, all, parts, blocks, s);
+                }
+            if (all > c->sm_count * 3 && all <= c->sm_count * 4) return launch_numbered<CHUNKS, MT, KIND, 4, false>(c, p, all, 1, blocks, s);
+            if (all <= c->sm_count * 3 || tiles <= 128) return launch_numbered<CHUNKS, MT, KIND, 3, false>(c, p, all, 1, blocks, s);
         }
     }
     return launch_tree<CHUNKS, MT, KIND>(c, p, units, unit_rows, unit_keys, s);

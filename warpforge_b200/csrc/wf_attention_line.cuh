@@ -308,7 +308,7 @@ __device__ __forceinline__ float line_ex2(float x) {
 // the unit begins in.  Bound by the latency of cut, pieces and row one after the other, and by how many rows an SM has at a time.  Pieces ahead 2 / 3 / 4 / 5 / 8: 13.3 / 12.5 /
 // 12.4 / 13.0 / 12.8 us for one token of 32 heads at 2000 tokens (the kernel before it included), 25.2 / 22.8 / 22.0 / 23.1 / 23.0 of 8 heads at 20,000, 22.4 / 21.6 / 22.0 /
 // 21.8 / 22.9 for 8 sequences of 0 to 3000 with up to 24 drafts; CTAs of 2 / 8 / 16 warps, the last of these: 24.5 / 22.3 / 22.9.
-// PARTS: the pieces are parts of units by number, one place each; blockIdx.x is the unit.
+// PARTS: the pieces are parts of prefixes, one place each; blockIdx.x is the unit.  (64 rows of 8 heads and one prefix in 18 parts, 22 MB of pieces out of the L2: 6 us.)
 constexpr int JOIN_WARPS = 4, JOIN_AHEAD = 4;
 template <int KIND, bool PARTS> __global__ void __launch_bounds__(JOIN_WARPS * 32) tree_join_kernel(const __grid_constant__ TreeParams p, const __grid_constant__ TreeCuts c) {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");

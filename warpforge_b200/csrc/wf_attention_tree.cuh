@@ -7,6 +7,10 @@
 //
 // The units are cut as wf_attention_line.cuh says.  Inside a CTA four warps walk its share and have TMA fill a ring of tiles ahead, across the ends of
 // units too; eight others take the tiles of a piece in turn.
+//
+// Lists, shared prefixes and what lies behind them are the same work on other units (KIND); a list or a sequence that is one of few goes to a cluster, one of many to a small CTA
+// (launch_units).  One token of 8 heads over lists of 4096 keys 9.0 us (16.8 MB, clusters of 8: launch, list, pages and tiles one after the other); of 48 sequences over lists of up to 2048
+// (384 MB) 63.4 us, 6.1 TB/s, 0.92 of a copy's rate; 48 drafted tokens of 4 heads over lists of 1536 keys, from the L2: 19.6 us, of which a warp's 24 tiles are half.
 #pragma once
 #include "wf_attention_line.cuh"
 #include "wf_gemm_core.cuh"
@@ -15,7 +19,8 @@ namespace wf {
 
 constexpr int TA_KEYS = 16;  // of a tile
 // Warps that multiply; warps that walk and load.  Eight and four: an SM has one CTA, and a unit's tiles are shared out among eight warps, which is what a few long units want.  Two and one:
-// an SM has four CTAs (two for 32 rows), each with a unit of its own, which is what many short ones want: what a unit costs beyond its tiles is paid beside other units' tiles.
+// an SM has three CTAs or four, each with a unit of its own (or a part of one), which is what many short ones want: what a unit costs beyond its tiles is paid beside other units' tiles.
+// Three have room for three tiles a warp, four for two; a warp waits for its tiles and not for its products (two tiles at a time, for the sake of those, took 10 to 30 % longer).
 constexpr int TA_WARPS = 8, TA_FEW_WARPS = 2;
 // Registers: 168 a thread at launch; the warps that multiply take what the others give back (256 x 216 + 128 x 72 = 384 x 168).
 constexpr int TA_MULTIPLY_REGS = 216, TA_WALK_REGS = 72;
@@ -26,11 +31,11 @@ constexpr int CLUSTER_AHEAD = 4;   // CTAs of a cluster whose sums are asked for
 // 1250 beside 15 with 200 14.4 / 12.3.
 constexpr int TA_CUT_TILES = 40, TA_CUT_ANYWAY = 96;
 constexpr float TA_RESCALE = 8.f;  // the running maximum is followed when it has grown by this many powers of two
-// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows; WARPS that multiply
-template <int CHUNKS, int MT, int WARPS = TA_WARPS> struct TreeShape {
-    static constexpr bool MANY = WARPS == TA_WARPS;
+// CHUNKS of 64 elements of the head's dimension; MT blocks of 16 rows; CTAS that an SM has: one large one, or three or four small ones
+template <int CHUNKS, int MT, int CTAS = 1> struct TreeShape {
+    static constexpr bool MANY = CTAS == 1;
+    static constexpr int WARPS = MANY ? TA_WARPS : TA_FEW_WARPS;
     static constexpr int DIM = CHUNKS * 64, ROWS = 16 * MT, LOADERS = MANY ? 4 : 1, THREADS = (WARPS + LOADERS) * 32;
-    static constexpr int CTAS = MANY ? 1 : 4 / MT;  // of an SM
     static constexpr int MERGE_BYTES = MANY ? 64 * 1024 : ROWS * DIM * 4;
     static constexpr int SLOT_BYTES = 2 * CHUNKS * TA_KEYS * 128;  // keys and values of a tile
     static constexpr int Q_BYTES = ROWS * DIM * 2;
@@ -44,6 +49,7 @@ template <int CHUNKS, int MT, int WARPS = TA_WARPS> struct TreeShape {
     // What a unit costs beyond its tiles, in tiles (queries, first tile's way, the fold over eight warps).  16 rows, with 2 / 4 / 8 / 12 / 16 / 24: 91 / 85 / 75 / 73 / 73 / 75 us
     // for one token of 48 sequences of 31 to 4000 tokens; 32 rows of 30 sequences of 10 to 5000, with 16 / 24 / 32 / 48: 72 / 65 / 63 / 61, but 33.2 / 32.8 / 33.2 / 33.3 for 20 alike.
     static constexpr int UNIT_TILES = 16 * MT;
+    static_assert(MANY || MT == 1, "small CTAs have 16 rows");
     static_assert(SETS == WARPS || 2 * SETS == WARPS, "one round of folding");
     static_assert(SLOTS >= WARPS && SLOTS % WARPS == 0 && SLOTS % LOADERS == 0, "slots for every warp and loader");
 };
@@ -151,9 +157,9 @@ template <class S, bool CLUSTER> struct TreeShared {
 
 // The warps that walk the line: the first announces this CTA's segments, all fetch their queries and have their tiles loaded, by turns.  True: all went
 // well.
-template <int CHUNKS, int MT, int KIND, int WARPS, bool BY_NUMBER, bool CLUSTER>
-__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeShape<CHUNKS, MT, WARPS>, CLUSTER>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
-    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
+template <int CHUNKS, int MT, int KIND, int CTAS, bool BY_NUMBER, bool CLUSTER>
+__device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeShape<CHUNKS, MT, CTAS>, CLUSTER>* sh, const CUtensorMap* k_map, const CUtensorMap* v_map, uint32_t ring, uint32_t q_smem, int loader) {
+    typedef TreeShape<CHUNKS, MT, CTAS> Shape;
     constexpr int ROWS = Shape::ROWS, DIM = Shape::DIM, LOADERS = Shape::LOADERS;
     const TreeParams& p = t.p;
     const int lane = threadIdx.x & 31, heads = p.cache.kv_heads, group = p.group;
@@ -240,11 +246,11 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
 
 // BY_NUMBER: a CTA finds its units by their number; else on the line.
 // CLUSTER: the CTAs of a cluster have a unit's parts, one each, and add their rows up from one another's shared memory; so there is no second kernel to join them.
-template <int CHUNKS, int MT, int KIND, int WARPS = TA_WARPS, bool BY_NUMBER = false, bool CLUSTER = false>
-__global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeShape<CHUNKS, MT, WARPS>::CTAS) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
+template <int CHUNKS, int MT, int KIND, int CTAS = 1, bool BY_NUMBER = false, bool CLUSTER = false>
+__global__ void __launch_bounds__(TreeShape<CHUNKS, MT, CTAS>::THREADS, CTAS) tree_tiles_kernel(const __grid_constant__ TreeTiles t, const __grid_constant__ CUtensorMap k_map,
                                                                    const __grid_constant__ CUtensorMap v_map) {
-    typedef TreeShape<CHUNKS, MT, WARPS> Shape;
-    constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS;
+    typedef TreeShape<CHUNKS, MT, CTAS> Shape;
+    constexpr int DIM = Shape::DIM, ROWS = Shape::ROWS, SLOTS = Shape::SLOTS, SLOT_BYTES = Shape::SLOT_BYTES, N_TILES = DIM / 8, SETS = Shape::SETS, WARPS = Shape::WARPS;
     constexpr bool Q_KEPT = MT * CHUNKS <= 2;  // queries stay in registers; else they are read again with every tile
     extern __shared__ uint8_t raw[];
     __shared__ TreeShared<Shape, CLUSTER> sh_;
@@ -273,7 +279,7 @@ __global__ void __launch_bounds__(TreeShape<CHUNKS, MT, WARPS>::THREADS, TreeSha
     asm volatile("griddepcontrol.wait;" ::: "memory");
     if (warp >= WARPS) {
         if (Shape::MANY) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(TA_WALK_REGS));
-        if (!tree_load<CHUNKS, MT, KIND, WARPS, BY_NUMBER, CLUSTER>(t, sh, &k_map, &v_map, ring, q_smem, warp - WARPS)) {
+        if (!tree_load<CHUNKS, MT, KIND, CTAS, BY_NUMBER, CLUSTER>(t, sh, &k_map, &v_map, ring, q_smem, warp - WARPS)) {
             if (lane == 0) report_status(p.status, STATUS_GEMM_PIPE_TIMEOUT);
             drain_after_abort();
         }

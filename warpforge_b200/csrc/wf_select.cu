@@ -12,9 +12,6 @@
 
 namespace wf {
 
-int check_kv_cache(Context* c, const char* what, const wf_kv_cache* cache, int layer, bool packed_too);
-CacheView cache_layer(const wf_kv_cache& cache, int layer);
-
 constexpr int LEAST_SCALE = -60;  // exponent: products of two scales are normal numbers
 
 // The exponent of the scale for a largest magnitude of these bf16 bits (finite ones): 127 x 2^e >= size.  size = m 2^x, 127 = 1.984375 x 2^6, and of the
@@ -642,27 +639,6 @@ using namespace wf;
     WF_CUDA(c, cudaSetDevice(c->device));                                  \
     cudaStream_t s = resolve_stream(c, stream)
 
-template <class Params>
-static int launch_select(Context* c, const char* what, void (*kernel)(Params), dim3 grid, unsigned threads, unsigned cluster, size_t smem, cudaStream_t s, const Params& p) {
-    cudaLaunchConfig_t cfg = {};
-    cfg.gridDim = grid;
-    cfg.blockDim = dim3(threads);
-    cfg.dynamicSmemBytes = smem;
-    cfg.stream = s;
-    cudaLaunchAttribute attr[2];
-    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-    attr[0].val.programmaticStreamSerializationAllowed = 1;
-    attr[1].id = cudaLaunchAttributeClusterDimension;
-    attr[1].val.clusterDim.x = cluster;
-    attr[1].val.clusterDim.y = attr[1].val.clusterDim.z = 1;
-    cfg.attrs = attr;
-    cfg.numAttrs = cluster > 1 ? 2 : 1;
-    const cudaError_t e = cudaLaunchKernelEx(&cfg, kernel, p);
-    if (e != cudaSuccess) return cuda_status(c, e, what);
-    c->launches++;
-    return WF_OK;
-}
-
 template <int CHUNKS, int WARPS, int RUN, bool SCORED> static int launch_selection(Context* c, const SelectParams& p, int64_t units, unsigned cluster, cudaStream_t s) {
     static std::atomic<uint64_t> ready{0};  // devices whose attribute is set
     constexpr size_t HEADS = SCORED ? 0 : CHUNKS * 32 * sizeof(uint4) + 8 * sizeof(int);  // bytes for eight heads
@@ -671,7 +647,7 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> static int launch_selecti
         WF_CUDA(c, cudaFuncSetAttribute(select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)(WF_SELECT_MAX_PAGES * 4 + SELECT_MAX_GROUP / 8 * HEADS)));
         ready.fetch_or(1ull << (c->device & 63));
     }
-    return launch_select(c, "select_pages", select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, dim3((unsigned)(units * cluster)), WARPS * 32, cluster, smem, s, p);
+    return launch_clusters(c, "select_pages", select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, dim3((unsigned)(units * cluster)), WARPS * 32, cluster, smem, s, p);
 }
 template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, int seqs, cudaStream_t s) {
     const int64_t units = (int64_t)seqs * p.max_drafts * p.kv_heads, bytes = p.tokens * p.kv_heads * p.room * 4;
@@ -693,7 +669,7 @@ template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, i
         const int64_t each = (lines * pieces + 2 * c->sm_count - 1) / (2 * c->sm_count);  // pieces of a CTA
         p.score_pages = (int)(each * SCORE_PAGES);
         const dim3 grid((unsigned)((pieces + each - 1) / each), (unsigned)lines);
-        auto score = [&](auto kernel) { return launch_select(c, "select_pages", kernel, grid, SCORE_WARPS * 32, 1, 0, s, p); };
+        auto score = [&](auto kernel) { return launch_clusters(c, "select_pages", kernel, grid, SCORE_WARPS * 32, 1, 0, s, p); };
         const int rc = p.group == 1   ? score(score_pages_kernel<CHUNKS, 1>)
                        : p.group == 2 ? score(score_pages_kernel<CHUNKS, 2>)
                        : p.group <= 4 ? score(score_pages_kernel<CHUNKS, 4>)
@@ -745,7 +721,7 @@ int wf_page_bounds(int64_t ctx, const wf_kv_cache* cache, int64_t codes_dev, int
     const int64_t units = touched * cache->kv_heads;
     if (units > (1LL << 31) - 1) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld tokens of %d heads", what, (long long)max_tokens, cache->kv_heads);
     p.units = (unsigned)units;
-    return launch_select(c, what, page_bounds_kernel, dim3((unsigned)((units + BOUNDS_WARPS - 1) / BOUNDS_WARPS), (unsigned)std::min<int64_t>(seqs, 65535), (unsigned)cache->layers),
+    return launch_clusters(c, what, page_bounds_kernel, dim3((unsigned)((units + BOUNDS_WARPS - 1) / BOUNDS_WARPS), (unsigned)std::min<int64_t>(seqs, 65535), (unsigned)cache->layers),
                          BOUNDS_WARPS * 32, 1, 0, s, p);
 }
 
