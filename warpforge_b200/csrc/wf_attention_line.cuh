@@ -196,7 +196,8 @@ __device__ __forceinline__ void leave_prefixes(const TreeParams& p, bool none) {
     }
 }
 
-// Walks this CTA's parts of prefixes.  All CTAs have a part of `most` tiles at most in each of one, two or three rounds, whichever takes least: sum ceil(tiles / most) is not more than total /
+// Walks this CTA's parts of prefixes.  (64 tokens of 8 x 8 heads behind 16384: 16 units in 18 parts of 7 or 8 tiles of 128 keys, two rounds of 148 CTAs.  On a line most CTAs have pieces of two units
+// in one round, of which each waits for its queries, first tile and way out.)  All CTAs have a part of `most` tiles at most in each of one, two or three rounds, whichever takes least: sum ceil(tiles / most) is not more than total /
 // most + units, so most = total / (rounds CTAs - units) is enough; where there is one group its units are alike, and rounds CTAs / units parts of each are exactly as many.  Groups
 // that overlap may have more rows than there are tokens, and more units than there is room for: nothing is walked then.  Every unit's entry of `cuts` is written, where a wait ran out, too.
 template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, F f) {

@@ -36,7 +36,9 @@ struct BoundsParams {
     int* status;
 };
 
-// A warp has one head of one page in one layer, contiguous in memory: a lane has 8 elements of a row, 32 / (dim / 8) rows go with one load, BOUNDS_DEPTH loads are in flight.
+// A warp has one head of one page in one layer, contiguous in memory: a lane has 8 elements of a row, 32 / (dim / 8) rows go with one load, BOUNDS_DEPTH loads are in flight.  Every key of the
+// pages is read once and nothing is left to wait for but HBM: 8192 tokens of 32 layers x 8 heads of 128 (537 MB and 9 of bounds) 75 us, as fast as a plain read; 48 decoded tokens, whose pages of
+// up to 64 tokens are read again in all of 32 layers (39 MB), 6.3 us, half of it a launch and the two loads before the first key (the table, the page).
 constexpr int BOUNDS_WARPS = 4, BOUNDS_DEPTH = 8;
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // NaN where one of them is
     uint32_t r;
@@ -259,6 +261,8 @@ template <int CHUNKS> struct PageTile {
 
 // Scores of all new tokens of a sequence, a CTA a kv head and p.score_pages pages, a warp 16 pages at a time: the codes of a page are read once for all of them.  Columns of the product are
 // the heads of a token, padded to PADDED (0: to a multiple of eight above it), token by token; as many tokens at a time as SCORE_COLUMNS have room for.
+// Bound by instructions: a tile of 16 pages by 8 columns has 4 to 8 products of the tensor cores and several times as many instructions on what comes out.  21 tokens of 24 / 8 heads of 96 over 8189 pages: 13 MB of
+// codes (2 us), 12 to 17 us, of which 3 bring the 63 heads that a CTA has to 8 bits; in the kernel below, without tiles of several tokens, 97.
 constexpr int SCORE_WARPS = 8, SCORE_PAGES = SCORE_WARPS * 16, SCORE_COLUMNS = 128, SCORE_HEADS = 4;  // heads asked for at a time
 template <int CHUNKS, int PADDED> __global__ void __launch_bounds__(SCORE_WARPS * 32, 2) score_pages_kernel(const __grid_constant__ SelectParams p) {
     constexpr int TILES = PADDED == 0 ? 1 : 2;  // of eight columns at a time
@@ -390,6 +394,8 @@ __device__ __forceinline__ uint2 load_scores2(const uint32_t* from) {
 // A cluster has one new token and kv head.  Its CTAs score a part of the pages each, 16 pages by the heads of the group a warp at a time (mma.sync on the codes: [q+ | q-] . [hi | lo],
 // the positive elements of q in the one half and the negative ones in the other), and leave the scores in the first CTA's shared memory, which takes the largest.  SCORED: the scores lie in
 // memory.  CHUNKS of 64 codes of a page (hi and lo together).  RUN: scores of a thread, which it keeps in registers; 0: as many as there are, read again each time.
+// Bound by latencies: launch, context, table, codes, and some six barriers of the selection.  One token of 8 heads over 250 pages 6.3 us, of 48 sequences with up to 250 pages 9.7 (13 MB, 1.4 TB/s).
+// The largest are found by two or three histograms of eight bits instead of a sort: what is left in a bin of the second, at most 256 scores, is ranked by comparing all with all.
 template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_bounds__(WARPS * 32, WARPS <= 8 && RUN != 2 ? 2 : WARPS <= 8 ? 3 : SCORED ? 2 : 1) select_pages_kernel(const __grid_constant__ SelectParams p) {
     constexpr int THREADS = WARPS * 32;
     constexpr bool AHEAD = RUN != 2;  // (few pages: a warp has one or two tiles of them, and registers are worth more)
