@@ -273,6 +273,29 @@ def test_select_most_pages(backend):
     assert e.value.status == N.WF_ERR_TOO_LARGE
 
 
+@pytest.mark.parametrize("pages", [3, 100, 128, 129, 400, 512])
+@pytest.mark.parametrize("what", ["scores", "ties", "one", "odd"])
+def test_select_many_lists_of_few_pages(backend, pages, what):
+    """Lists that a warp has, with contexts from none to `pages` pages: scores of all sizes, of two sizes, all alike, and pages that come before all others or are nowhere."""
+    rng = np.random.default_rng(pages)
+
+    def edit(q, codes, scales, tables):
+        if what in ("ties", "one"):
+            codes[:] = codes[0, 0, 0, 0]
+            scales[:] = 0.25
+        if what == "ties":
+            scales[::3] = 0.5
+        if what == "odd":
+            scales[::5] = float("inf")
+            q[::7, 1] = float("nan")
+            q[::11] = 0.0
+
+    lens = [16 * pages] + [int(n) for n in rng.integers(0, 16 * pages + 1, 10)]
+    drafts = [24] + [int(n) for n in rng.integers(0, 25, 10)]
+    run_select(backend, lens, drafts, 16, 8, 64, 16, 11 + pages // 9, first=2, recent=20, tree=True, edit=edit, most=16 * max(pages, 500 if pages > 128 else 120), repeat=2)
+    run_select(backend, [16 * pages] * 40, [24] * 40, 2, 1, 8, 16, 9, edit=edit, arrays=False, most=16 * max(pages, 500 if pages > 128 else 120))
+
+
 def test_select_ties_of_many_tokens(backend):
     def two(q, codes, scales, tables):
         codes[:] = codes[0, 0, 0, 0]

@@ -143,6 +143,7 @@ struct SelectParams {
     int room;            // pages whose scores a token and kv head may have
     uint32_t* scores;    // [tokens][kv_heads][room], where a kernel of its own makes them
     int score_pages;     // of a CTA there
+    unsigned lists;      // sequences times max_drafts times heads
     uint32_t group_inverse;  // 2^32 / group, rounded up; 0 for a group of one
     int* status;
     __device__ __forceinline__ int token_of(int head) const { return group_inverse ? (int)__umulhi((uint32_t)head, group_inverse) : head; }  // head / group, below 64 x 128
@@ -385,10 +386,87 @@ __device__ __forceinline__ uint4 load_scores(const uint32_t* from) {
     asm volatile("ld.global.cs.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(from));
     return v;
 }
-__device__ __forceinline__ uint2 load_scores2(const uint32_t* from) {
-    uint2 v;
-    asm volatile("ld.global.cs.v2.u32 {%0, %1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(from));
-    return v;
+
+// What a list has in any case, by `lanes` threads of which this is number `lane`: the places that the scores do not decide, the lengths.
+__device__ __forceinline__ void write_ends(const SelectParams& p, const SelectSeq& q, int64_t line, int i, int take, const int* table, int* list, int lane, int lanes) {
+    const int first = q.first, count = first + q.last - q.tail + take;
+    for (int n = lane; n < p.width - take; n += lanes) {
+        const int at = n < first ? n : n + take, page = at < first ? at : q.tail + at - first - take;
+        list[at] = at < count ? table[page] : -1;
+    }
+    if (lane == 0) {
+        const int held = q.context < 0 ? 0 : q.context - ((q.between - take) << p.page_shift);
+        p.lens_out[line] = make_int2(held, q.context < 0 ? 0 : held + (p.tree ? q.rows : i + 1));
+    }
+}
+
+// The pages of a new token and kv head by a warp, where their scores lie in memory and are few: a lane keeps RUN of them.  The largest are those from T on, the largest number for which there are
+// enough of them, found bit by bit; no barrier and no shared memory.  (4152 lists of some 70 pages, their scores included: 17 us; by CTAs of eight warps, sixteen rounds of them, 36.)
+constexpr int FEW_WARPS = 4;
+template <int RUN> __global__ void __launch_bounds__(FEW_WARPS * 32) select_few_kernel(const __grid_constant__ SelectParams p) {
+    asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+    asm volatile("griddepcontrol.wait;" ::: "memory");
+    const unsigned unit = blockIdx.x * FEW_WARPS + (threadIdx.x >> 5), per_seq = (unsigned)p.max_drafts * p.kv_heads, s = unit / per_seq, of_seq = unit - s * per_seq;
+    if (unit >= p.lists) return;
+    const int lane = threadIdx.x & 31, i = (int)(of_seq / p.kv_heads), head = (int)(of_seq - i * p.kv_heads);
+    const SelectSeq q = select_seq(p, (int)s, lane == 0 && of_seq == 0);
+    if (i >= q.rows) return;
+    const int64_t line = (q.row0 + i) * p.kv_heads + head;
+    const int* const table = p.tables + (size_t)s * p.table_stride;
+    int* const list = p.pages_out + (size_t)line * p.width;
+    const int take = min(q.between, p.width - q.first - (q.last - q.tail));
+    const int from = lane * RUN, valid = max(0, min(RUN, q.between - from));
+    uint32_t d[RUN];
+    if (take < q.between) {
+        const uint32_t* const scores = p.scores + (size_t)line * p.room;
+#pragma unroll
+        for (int e = 0; e < RUN; e += 4) {
+            const uint4 v = e < valid ? load_scores(scores + from + e) : make_uint4(0, 0, 0, 0);
+            d[e] = v.x, d[e + 1] = v.y, d[e + 2] = v.z, d[e + 3] = v.w;
+        }
+    }
+    write_ends(p, q, line, i, take, table, list, lane, 32);
+    if (take == q.between) {  // all of them
+        for (int n = lane; n < take; n += 32) list[q.first + n] = table[q.first + n];
+        return;
+    }
+    uint32_t low = 0xFFFFFFFFu, high = 0;
+#pragma unroll
+    for (int e = 0; e < RUN; e++)
+        if (e < valid) low = min(low, d[e]), high = max(high, d[e]);
+    low = __reduce_min_sync(0xFFFFFFFFu, low);
+    high = __reduce_max_sync(0xFFFFFFFFu, high);
+#pragma unroll
+    for (int e = 0; e < RUN; e++) d[e] = e < valid ? d[e] - low : 0;  // (what is above 0 is a page's)
+    uint32_t border = 0;
+    for (int bit = 31 - __clz(high - low); bit >= 0; bit--) {
+        const uint32_t next = border | 1u << bit;
+        int enough = 0;
+#pragma unroll
+        for (int e = 0; e < RUN; e++) enough += d[e] >= next;
+        enough = __reduce_add_sync(0xFFFFFFFFu, enough);
+        if (enough >= take) border = next;
+        if (enough == take) break;
+    }
+    // Those above the border, and of those on it the first ones: how many of each there are up to this lane, in one word.
+    uint32_t both = 0;
+#pragma unroll
+    for (int e = 0; e < RUN; e++) both += d[e] > border ? 1u : e < valid && d[e] == border ? 1u << 16 : 0;
+    uint32_t up_to = both;
+#pragma unroll
+    for (int o = 1; o < 32; o <<= 1) {
+        const uint32_t v = __shfl_up_sync(0xFFFFFFFFu, up_to, o);
+        if (lane >= o) up_to += v;
+    }
+    const int need = take - (int)(__shfl_sync(0xFFFFFFFFu, up_to, 31) & 0xFFFF);
+    int above = (int)((up_to - both) & 0xFFFF), like = (int)((up_to - both) >> 16);
+#pragma unroll
+    for (int e = 0; e < RUN; e++) {
+        const bool on = e < valid && d[e] == border;
+        if (d[e] > border || (on && like < need)) list[q.first + above + min(like, need)] = table[q.first + from + e];
+        above += d[e] > border;
+        like += on;
+    }
 }
 
 // A cluster has one new token and kv head.  Its CTAs score a part of the pages each, 16 pages by the heads of the group a warp at a time (mma.sync on the codes: [q+ | q-] . [hi | lo],
@@ -400,6 +478,7 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_
     constexpr int THREADS = WARPS * 32;
     constexpr bool AHEAD = RUN != 2;  // (few pages: a warp has one or two tiles of them, and registers are worth more)
     constexpr bool IN_MEMORY = SCORED && RUN > 0;  // registers take the scores from there
+    static_assert(!SCORED || RUN != 2, "few scores in memory: select_few_kernel");
     extern __shared__ uint4 dynamic[];  // scores [room], as unsigned numbers of the same order; codes of the heads; exponents of their scales
     uint32_t* const keys = reinterpret_cast<uint32_t*>(dynamic);
     uint4* const q_codes = dynamic + p.room / 4;
@@ -423,19 +502,10 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_
     }
     const int64_t row = q.row0 + i;
     const int* const table = p.tables + (size_t)s * p.table_stride;
-    const int first = q.first, between = q.between, ends = first + q.last - q.tail;
-    const int take = min(between, p.width - ends), count = ends + take;  // the host sees to it that the ends fit
+    const int first = q.first, between = q.between;
+    const int take = min(between, p.width - first - (q.last - q.tail));  // the host sees to it that the ends fit
     int* const list = p.pages_out + ((size_t)row * p.kv_heads + head) * p.width;
-    if (rank == ranks - 1) {
-        for (int n = tid; n < p.width - take; n += THREADS) {  // the places that the scores do not decide
-            const int at = n < first ? n : n + take, page = at < first ? at : q.tail + at - first - take;
-            list[at] = at < count ? table[page] : -1;
-        }
-        if (tid == 0) {
-            const int held = q.context < 0 ? 0 : q.context - ((between - take) << p.page_shift);
-            p.lens_out[row * p.kv_heads + head] = make_int2(held, q.context < 0 ? 0 : held + (p.tree ? q.rows : i + 1));
-        }
-    }
+    if (rank == ranks - 1) write_ends(p, q, row * p.kv_heads + head, i, take, table, list, tid, THREADS);
     if (take == between) {  // all of them
         if (rank == 0)
             for (int n = tid; n < take; n += THREADS) list[first + n] = table[first + n];
@@ -515,7 +585,7 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_
 #pragma unroll
         for (int e = 0; e < RUN; e += RUN < 4 ? 2 : 4) {
             if constexpr (RUN < 4) {
-                const uint2 v = e < valid ? IN_MEMORY ? load_scores2(scores + from + e) : *reinterpret_cast<const uint2*>(keys + from + e) : make_uint2(0, 0);
+                const uint2 v = e < valid ? *reinterpret_cast<const uint2*>(keys + from + e) : make_uint2(0, 0);
                 kept[e] = v.x, kept[e + 1] = v.y;
             } else {
                 const uint4 v = e < valid ? IN_MEMORY ? load_scores(scores + from + e) : *reinterpret_cast<const uint4*>(keys + from + e) : make_uint4(0, 0, 0, 0);
@@ -656,7 +726,8 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> static int launch_selecti
     return launch_clusters(c, "select_pages", select_pages_kernel<CHUNKS, WARPS, RUN, SCORED>, dim3((unsigned)(units * cluster)), WARPS * 32, cluster, smem, s, p);
 }
 template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, int seqs, cudaStream_t s) {
-    const int64_t units = (int64_t)seqs * p.max_drafts * p.kv_heads, bytes = p.tokens * p.kv_heads * p.room * 4;
+    p.lists = (unsigned)((int64_t)seqs * p.max_drafts * p.kv_heads);
+    const int64_t units = p.lists, bytes = p.tokens * p.kv_heads * p.room * 4;
     // Several new tokens of a sequence read the same codes.  In one kernel each token's cluster reads them (microseconds: 5 tokens of 4 sequences with 250 pages, 32 / 8 heads, 10.4; of 16
     // sequences 20.6; 21 tokens of one with 250, 1000, 8125 pages 10.3, 20.1, 97), in two kernels a CTA scores pages for all of them (10.6; 14.5; 14.2, 16.3, 41).
     if (p.max_drafts > 1 && units * p.room >= SCORED_FROM && bytes <= SCORE_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
@@ -682,7 +753,9 @@ template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, i
                        : p.group <= 8 ? score(score_pages_kernel<CHUNKS, 8>)
                                       : score(score_pages_kernel<CHUNKS, 0>);
         if (rc != WF_OK) return rc;
-        if (p.room <= 512) return launch_selection<CHUNKS, 8, 2, true>(c, p, units, 1, s);
+        const dim3 few((unsigned)((units + FEW_WARPS - 1) / FEW_WARPS));
+        if (p.room <= 128) return launch_clusters(c, "select_pages", select_few_kernel<4>, few, FEW_WARPS * 32, 1, 0, s, p);
+        if (p.room <= 512) return launch_clusters(c, "select_pages", select_few_kernel<16>, few, FEW_WARPS * 32, 1, 0, s, p);
         if (p.room <= 2048) return launch_selection<CHUNKS, 8, 8, true>(c, p, units, 1, s);
         return p.room <= 8192 ? launch_selection<CHUNKS, 16, 16, true>(c, p, units, 1, s) : launch_selection<CHUNKS, 16, 0, true>(c, p, units, 1, s);
     }
