@@ -115,8 +115,11 @@ def test_selected_many_lists(backend):
 def test_selected_on_every_way(backend):
     """Lists by number and on a line, in clusters of large CTAs and of small ones, whole: as many lists, and of such lengths, as lead there."""
     run_selected(backend, [2100] * 76, [1] * 76, 16, 8, 64, 16, pages=140, heads=[0, 7])                    # 608 long ones: a line
-    run_selected(backend, [700 + 9 * i for i in range(10)], [1] * 10, 160, 8, 128, 16, pages=140, heads=[7])  # 80 with 20 rows: a line
-    run_selected(backend, [700 + 9 * i for i in range(9)], [1] * 9, 160, 8, 128, 16, pages=140, heads=[0])    # 72 with 20 rows: clusters of 2
+    run_selected(backend, [700 + 9 * i for i in range(10)], [1] * 10, 160, 8, 128, 16, pages=140, heads=[7])   # 80 with 20 rows
+    run_selected(backend, [700 + 9 * i for i in range(9)], [1] * 9, 160, 8, 128, 16, pages=140, heads=[0])
+    run_selected(backend, [2100 + 9 * i for i in range(10)], [1] * 10, 160, 8, 128, 16, pages=160, heads=[7])  # longer ones, 32 rows at a time: a line
+    run_selected(backend, [2100 + 9 * i for i in range(9)], [1] * 9, 160, 8, 128, 16, pages=160, heads=[0])    # clusters of 2
+    run_selected(backend, [2100 + 9 * i for i in range(5)], [1] * 5, 320, 8, 64, 16, pages=160, heads=[3])     # 40 rows
     for tokens in (1, 3, 9, 12, 17, 24, 40, 60, 80):
         run_selected(backend, [1 + (37 * i) % 600 for i in range(tokens)], [1] * tokens, 16, 8, 128, 16, width=38, pages=60, heads=[0, 3])
 
@@ -227,7 +230,8 @@ def test_selected_refusals(backend):
 
 
 # ------------------------------------------------------------------------------------------------ shared prefixes
-# A bound of the prefix far above it: as much might be read again, if every sequence were to read it, that the prefixes have a kernel of their own.
+# A bound of the prefix far above it: as much might be read again, if every sequence were to read it, that the prefixes have a kernel of their own (several = 1).  A bound of what a sequence has behind
+# it as well (2): as much might lie there that its rows go 32 or 128 at a time.
 FAR = 1 << 24
 
 
@@ -262,7 +266,7 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     anc = signed(words) if words else torch.zeros(0, dtype=torch.int64, device="cuda")
     torch.cuda.synchronize()
     op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=FAR if several else most or max(prefix),
-                                 max_own=most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
+                                 max_own=FAR if several == 2 else most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
     op.run()
     backend.synchronize_device()
     same_bits(op, out, backend)
@@ -286,7 +290,7 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     return out
 
 
-several = pytest.mark.parametrize("several", [False, True])
+several = pytest.mark.parametrize("several", [0, 1, 2])
 
 
 @several
@@ -589,7 +593,7 @@ def test_shared_queries_with_gaps_and_rows_behind(backend, several):
     out = torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
     stream = backend.create_stream()
     torch.cuda.synchronize()
-    A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR if several else 64, max_own=6,
+    A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR if several else 64, max_own=FAR if several == 2 else 6,
                             q_offsets=held(off), max_drafts=2).run(stream)
     backend.synchronize_stream(stream)
     assert (out[3:] == 7).all()

@@ -30,18 +30,32 @@ static TreeParams attention_params(Context* c, const wf_kv_cache& cache, int lay
     return p;
 }
 
-// Units of up to `rows` rows, 16 or 32 of them at a time.  17 to 32 go 16 at a time, and read their keys twice, where that is little, or where it keeps many short units off the line.  Microseconds 32 / 16 at
-// a time, 20 rows of 8 heads of 128: 32 units of 300, 750 keys 11.4 / 7.8, 11.2 / 8.9; 128 12.0 / 12.2, 17.0 / 17.9; 320 28.8 / 22.9, 39 / 42.
+// What rows, 16 at a time in small CTAs, take of an SM: in tiles of 16 keys, eight more for what a block of rows costs in any case.
+static double share_of_rows(const Context* c, int64_t units, int64_t rows, int64_t keys) { return (double)units * ((rows + 15) / 16) * ((keys + TA_KEYS - 1) / TA_KEYS + 8) / c->sm_count; }
+
+// Units of more than 16 rows, 16 or 32 of them at a time.  16 read the keys twice as often, out of the L2, but go to clusters and to small CTAs of their own; where that is much, a line is quicker, and where
+// units are long and not alike (lists are), too.  Microseconds 32 / 16 at a time: lists of 512, 2048, 4096 keys, 64 heads of 128 for one kv head, one token (share of an SM: 1 to 7) 9.9 / 7.5, 11.5 / 8.7,
+// 13.5 / 9.9; 8 (9, 29, 57) 10.2 / 7.8, 13.2 / 9.7, 17.0 / 12.6; 32 (35, 118, 228) 11.5 / 10.4, 17.8 / 18.3, 25.4 / 28.6; 96 (104, 353, 685) 24.3 / 16.2, 44.6 / 41.3, 69 / 74; 256 (277, 941, 1827)
+// 48 / 41, 102 / 113, 177 / 331; 40 / 2 heads, 96 tokens (104, 353, 685) 27.6 / 16.8, 48.3 / 43.3, 76.6 / 77.2.  17 sequences of 1 to 1777 keys of their own, 36 rows of 8 heads (331): 39.7 / 47.3.
+constexpr double SHARE_LITTLE = 60, SHARE_OF_SHORT = 600;
 template <int CHUNKS, int KIND> static int launch_rows(Context* c, const TreeParams& p, int64_t units, int64_t rows, int64_t keys, cudaStream_t s) {
-    const int64_t tiles = (keys + TA_KEYS - 1) / TA_KEYS;
-    const bool twice = rows <= 32 && (2.0 * units * tiles <= 48.0 * c->sm_count || (2 * units > c->sm_count && tiles <= 32));
-    return rows <= 16 || twice ? launch_units<CHUNKS, 1, KIND>(c, p, units, (int)rows, keys, s) : launch_units<CHUNKS, 2, KIND>(c, p, units, (int)rows, keys, s);
+    const double share = share_of_rows(c, units, rows, keys);
+    const bool sixteen = rows <= 16 || share <= SHARE_LITTLE || (keys <= (KIND == ATTEND_LISTS ? 2048 : 512) && share <= SHARE_OF_SHORT);
+    return sixteen ? launch_units<CHUNKS, 1, KIND>(c, p, units, (int)rows, keys, s) : launch_units<CHUNKS, 2, KIND>(c, p, units, (int)rows, keys, s);
 }
 
 // Tiles of 128 rows where sequences have more than 32 each; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of 24 / 8
 // heads of 64 48 / 39; 4, 16, 48 with 12 tokens of 32 / 8 heads of 128 and 400 keys 29.8 / 28.7, 38 / 43, 66 / 85.
 static bool few_rows(const TreeParams& p) { return p.max_drafts * p.group <= 32 || p.tokens * p.group <= 20 * (int64_t)p.seqs; }
 constexpr double AGAIN_BYTES = 192e6;
+// More than 32 rows go 16 at a time, too, where that is little: the tiles of 128 rows wait longer for the little that they have to do.  Sequences behind a prefix of 4096, 32 / 8 heads of 128, own keys by
+// 128 rows / by 16: 8 with 12 tokens and 20, 400, 1500 keys (share 13, 44, 133) 40.6 / 33.5, 43.2 / 38.5, 50.6 / 48.5; 24 with 20, 400 (39, 132) 59.0 / 45.8, 66.0 / 54.7; 48 with 20, 400, 1500 (78, 265, 800)
+// 78.0 / 66.5, 90.8 / 87.8, 122 / 146.  With 24 tokens, 96 rows: 8 with 400 (91) 47.2 / 44.6; 24 with 100, 400 (125, 272) 72.3 / 71.5, 80.7 / 87.3; 48 with 20 (171) 109.5 / 111.6.
+constexpr double SHARE_48_ROWS = 270, SHARE_MORE_ROWS = 110;
+// The same where each sequence reads the prefix itself, by several kernels (the quicker way) / by one, 12 and 24 tokens with 100 keys of their own: 2 sequences behind 512 (15, 31) 21.8 / 8.9, 25.4 / 11.4; 8
+// behind 1024 (102, 207) 28.5 / 19.1, 30.6 / 28.5; 32 behind 512 (244) 38.3 / 34.1; 4 behind 4096 (176, 353) 32.0 / 27.5, 35.8 / 47.6; 16 / 2 heads, 32 with 24 behind 512 (248) 38.6 / 34.9; 32 / 16 heads of 64,
+// 16 behind 512 (248) 30.4 / 22.9.
+constexpr double SHARE_AGAIN = 280;
 
 // Prefixes, then what the sequences have of their own, which begins with the first one's sums.
 template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStream_t s) {
@@ -49,10 +63,9 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     // its own, (sequences - groups) x prefix in MB: 64 / 8 heads of 128, 4 sequences behind 1024 in common (12) 17.8 / 8.4, 4096 (48) 20.7 / 12.4, 16384 (192) 33.0 / 28.9; 16 behind 4096 (240) 29.4 / 26.9,
     // 16384 (960) 36.5 / 83; 48 behind 1024 (188) 28.8 / 28.4; 32 / 32 heads, 4 behind 1024 (48) 15.2 / 13.0, 4096 (192) 24.8 / 28.2; 16 behind 1024 (240) 18.0 / 29.3.
     const double again = (double)(p.seqs - p.n_groups) * (double)p.max_prefix * p.cache.kv_heads * p.cache.dim * 4;
-    if (again <= AGAIN_BYTES && few_rows(p)) {
-        const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_prefix + p.max_context + p.max_drafts;
-        return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, p.max_drafts * p.group, keys, s);
-    }
+    const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, unit_rows = p.max_drafts * p.group, own_keys = p.max_context + p.max_drafts, all_keys = p.max_prefix + own_keys;
+    if (unit_rows > 32 && share_of_rows(c, units, unit_rows, all_keys) <= SHARE_AGAIN) return launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, (int)unit_rows, all_keys, s);
+    if (again <= AGAIN_BYTES && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
     // the most cut units and pieces of them that any of the kernels leaves
     const int64_t most_cuts = (PREFIX_ROUNDS - 1) * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
@@ -67,8 +80,9 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads, prefix_rows = p.tokens * p.group;
     rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s) : launch_rows<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, prefix_rows, p.max_prefix, s);
     if (rc != WF_OK) return rc;
-    const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, keys = p.max_context + p.max_drafts;
-    return few_rows(p) ? launch_rows<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts * p.group, keys, s) : launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, keys, s);
+    if (unit_rows > 32 && share_of_rows(c, units, unit_rows, own_keys) <= (unit_rows <= 48 ? SHARE_48_ROWS : SHARE_MORE_ROWS))
+        return launch_units<CHUNKS, 1, ATTEND_OWN>(c, p, units, (int)unit_rows, own_keys, s);
+    return few_rows(p) ? launch_rows<CHUNKS, ATTEND_OWN>(c, p, units, unit_rows, own_keys, s) : launch_wide_tree<CHUNKS, ATTEND_OWN>(c, p, units, p.max_drafts, own_keys, s);
 }
 
 extern "C" {
