@@ -47,7 +47,7 @@ template <int CHUNKS, int KIND> static int launch_rows(Context* c, const TreePar
 // Tiles of 128 rows where sequences have more than 32 each; where only the longest of them do, 32 at a time.  Microseconds of the call, tiles of 128 / of 32: 17 sequences with 1 to 12 tokens of 24 / 8
 // heads of 64 48 / 39; 4, 16, 48 with 12 tokens of 32 / 8 heads of 128 and 400 keys 29.8 / 28.7, 38 / 43, 66 / 85.
 static bool few_rows(const TreeParams& p) { return p.max_drafts * p.group <= 32 || p.tokens * p.group <= 20 * (int64_t)p.seqs; }
-constexpr double AGAIN_BYTES = 192e6;
+constexpr double AGAIN_BYTES = 270e6, AGAIN_FEW_BYTES = 110e6;
 // More than 32 rows go 16 at a time, too, where that is little: the tiles of 128 rows wait longer for the little that they have to do.  Sequences behind a prefix of 4096, 32 / 8 heads of 128, own keys by
 // 128 rows / by 16: 8 with 12 tokens and 20, 400, 1500 keys (share 13, 44, 133) 40.6 / 33.5, 43.2 / 38.5, 50.6 / 48.5; 24 with 20, 400 (39, 132) 59.0 / 45.8, 66.0 / 54.7; 48 with 20, 400, 1500 (78, 265, 800)
 // 78.0 / 66.5, 90.8 / 87.8, 122 / 146.  With 24 tokens, 96 rows: 8 with 400 (91) 47.2 / 44.6; 24 with 100, 400 (125, 272) 72.3 / 71.5, 80.7 / 87.3; 48 with 20 (171) 109.5 / 111.6.
@@ -59,13 +59,15 @@ constexpr double SHARE_AGAIN = 280;
 
 // Prefixes, then what the sequences have of their own, which begins with the first one's sums.
 template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStream_t s) {
-    // Where little would be read again, most of it out of the L2, a sequence reads its prefix itself, and there is one kernel.  Microseconds by several kernels / by one, one token each with 100 keys of
-    // its own, (sequences - groups) x prefix in MB: 64 / 8 heads of 128, 4 sequences behind 1024 in common (12) 17.8 / 8.4, 4096 (48) 20.7 / 12.4, 16384 (192) 33.0 / 28.9; 16 behind 4096 (240) 29.4 / 26.9,
-    // 16384 (960) 36.5 / 83; 48 behind 1024 (188) 28.8 / 28.4; 32 / 32 heads, 4 behind 1024 (48) 15.2 / 13.0, 4096 (192) 24.8 / 28.2; 16 behind 1024 (240) 18.0 / 29.3.
+    // Where little would be read again, most of it out of the L2, a sequence reads its prefix itself, and there is one kernel; less where a prefix has up to 32 rows in all, whose kernel is quick.  Microseconds
+    // by several kernels / by one, one token each with 100 keys of its own, (sequences - groups) x prefix in MB: 64 / 8 heads of 128, 4 sequences behind 1024 in common (13) 15.6 / 8.6; 8 behind 8192 (235)
+    // 31.7 / 29.3; 16 behind 4096, 8192 (252, 503) 29.9 / 27.3, 33.3 / 46.3; 64 behind 1024 (264) 30.3 / 29.7; 16 / 2 heads, 32 behind 8192 (260) 41.6 / 28.0; 32 / 8 heads, 64 behind 1024 (264) 28.8 / 28.9.  Up to 32
+    // rows: 32 / 8 heads, 8 behind 4096, 8192 (117, 235) 19.7 / 18.0, 25.6 / 29.0; 32 / 32 heads, 4 behind 2048, 4096 (101, 201) 18.0 / 18.4, 24.1 / 28.4; 8 behind 512, 1024 (59, 117) 14.9 / 13.4, 15.9 / 18.6.
     const double again = (double)(p.seqs - p.n_groups) * (double)p.max_prefix * p.cache.kv_heads * p.cache.dim * 4;
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, unit_rows = p.max_drafts * p.group, own_keys = p.max_context + p.max_drafts, all_keys = p.max_prefix + own_keys;
+    const int64_t prefix_rows = p.tokens * p.group;
     if (unit_rows > 32 && share_of_rows(c, units, unit_rows, all_keys) <= SHARE_AGAIN) return launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, (int)unit_rows, all_keys, s);
-    if (again <= AGAIN_BYTES && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
+    if (again <= (prefix_rows > 32 ? AGAIN_BYTES : AGAIN_FEW_BYTES) && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
     // the most cut units and pieces of them that any of the kernels leaves
     const int64_t most_cuts = (PREFIX_ROUNDS - 1) * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
@@ -77,7 +79,7 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     p.state_dim = CHUNKS * 64;
     p.prefix_of = reinterpret_cast<int2*>(more + sums);
     // Up to 32 rows in all go to the kernel for few rows.  Microseconds of the call, 4 sequences with one token of 32 / 8 heads of 128 behind 1024 in common: 19.7 by tiles of 128 rows, 15.3 by tiles of 16.
-    const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads, prefix_rows = p.tokens * p.group;
+    const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads;
     rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s) : launch_rows<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, prefix_rows, p.max_prefix, s);
     if (rc != WF_OK) return rc;
     if (unit_rows > 32 && share_of_rows(c, units, unit_rows, own_keys) <= (unit_rows <= 48 ? SHARE_48_ROWS : SHARE_MORE_ROWS))
