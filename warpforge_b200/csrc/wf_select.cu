@@ -149,7 +149,7 @@ struct SelectParams {
     __device__ __forceinline__ int token_of(int head) const { return group_inverse ? (int)__umulhi((uint32_t)head, group_inverse) : head; }  // head / group, below 64 x 128
 };
 constexpr int SELECT_MAX_GROUP = 128, SELECT_BINS = 256, SELECT_FEW = 256;  // SELECT_FEW: no more than a CTA has threads
-constexpr int64_t SCORE_BYTES = 1LL << 30, SCORED_FROM = 1 << 16;  // of scores in memory, at most; scores of a call that go there
+constexpr int64_t SCORE_BYTES = 1LL << 30;  // of scores in memory, at most
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -400,7 +400,7 @@ __device__ __forceinline__ void write_ends(const SelectParams& p, const SelectSe
     }
 }
 
-// The pages of a new token and kv head by a warp, where their scores lie in memory and are few: a lane keeps RUN of them.  The largest are those from T on, the largest number for which there are
+// The pages of a new token and kv head by a warp, where their scores lie in memory and are few, or none is left out: a lane keeps RUN of them.  The largest are those from T on, the largest number for which there are
 // enough of them, found bit by bit; no barrier and no shared memory.  (4152 lists of some 70 pages, their scores included: 17 us; by CTAs of eight warps, sixteen rounds of them, 36.)
 constexpr int FEW_WARPS = 4;
 template <int RUN> __global__ void __launch_bounds__(FEW_WARPS * 32) select_few_kernel(const __grid_constant__ SelectParams p) {
@@ -728,9 +728,17 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> static int launch_selecti
 template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, int seqs, cudaStream_t s) {
     p.lists = (unsigned)((int64_t)seqs * p.max_drafts * p.kv_heads);
     const int64_t units = p.lists, bytes = p.tokens * p.kv_heads * p.room * 4;
-    // Several new tokens of a sequence read the same codes.  In one kernel each token's cluster reads them (microseconds: 5 tokens of 4 sequences with 250 pages, 32 / 8 heads, 10.4; of 16
-    // sequences 20.6; 21 tokens of one with 250, 1000, 8125 pages 10.3, 20.1, 97), in two kernels a CTA scores pages for all of them (10.6; 14.5; 14.2, 16.3, 41).
-    if (p.max_drafts > 1 && units * p.room >= SCORED_FROM && bytes <= SCORE_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
+    const dim3 few((unsigned)((units + FEW_WARPS - 1) / FEW_WARPS));
+    // Lists that have room for all pages of the longest context: nothing is scored.  (24 tokens x 16 heads over 7 to 16 pages 3.3 us, by CTAs 4.9.)
+    if (p.room <= 512 && (std::min(p.max_context + p.max_drafts, p.table_stride << p.page_shift) + (1 << p.page_shift) - 1) >> p.page_shift <= p.width)
+        return launch_clusters(c, "select_pages", select_few_kernel<4>, few, FEW_WARPS * 32, 1, 0, s, p);
+    // Several new tokens of a sequence read the same codes.  In one kernel each token's cluster reads them, in two a CTA scores pages for all of them: that begins later, and by the more, the more heads each
+    // of its CTAs brings to 8 bits.  Microseconds by one / by two, tokens x sequences with pages of 16: 32 / 8 heads (20 to 84 heads of a CTA), 64 pages, 5 x 4, 5 x 16, 21 x 4, 21 x 16 (160 to 2688 lists)
+    // 7.0 / 8.5, 12.3 / 9.5, 12.3 / 11.7, 35.6 / 15.2; 500 pages 13.2 / 11.5, 23.6 / 16.9, 24.4 / 20.8, 77 / 29; 16 / 2 heads (168), 21 x 4, 21 x 16, 21 x 48: 7.1 / 17.8, 12.6 / 17.8, 28.4 / 18.6.  More pages: 32 / 8
+    // heads, 1000, 2 x 1, 5 x 1, 21 x 1: 9.8 / 10.7, 13.4 / 12.1, 18.3 / 15.3; 4000: 20.7 / 16.1, 22.3 / 15.7, 60 / 22.6; 16 / 2 heads, 21 x 1, 21 x 4 of 4000: 22.2 / 28.3, 60 / 32.
+    const int64_t heads = (int64_t)p.max_drafts * p.group, lists = p.tokens * p.kv_heads;
+    const bool scored = p.room <= 512 ? lists >= 200 + 11 * heads / 2 : lists * p.room >= 20480 + 1024 * heads;
+    if (p.max_drafts > 1 && scored && bytes <= SCORE_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
         GemvScratch& scratch = c->gemv_scratch[s];
         if (bytes > scratch.attn_bytes) {
             const int rc = refuse_allocation_while_recording(c, s, "the scores of select_pages");
@@ -753,7 +761,6 @@ template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, i
                        : p.group <= 8 ? score(score_pages_kernel<CHUNKS, 8>)
                                       : score(score_pages_kernel<CHUNKS, 0>);
         if (rc != WF_OK) return rc;
-        const dim3 few((unsigned)((units + FEW_WARPS - 1) / FEW_WARPS));
         if (p.room <= 128) return launch_clusters(c, "select_pages", select_few_kernel<4>, few, FEW_WARPS * 32, 1, 0, s, p);
         if (p.room <= 512) return launch_clusters(c, "select_pages", select_few_kernel<16>, few, FEW_WARPS * 32, 1, 0, s, p);
         if (p.room <= 2048) return launch_selection<CHUNKS, 8, 8, true>(c, p, units, 1, s);
