@@ -273,6 +273,21 @@ def test_select_most_pages(backend):
     assert e.value.status == N.WF_ERR_TOO_LARGE
 
 
+@pytest.mark.parametrize("group,dim", [(1, 8), (2, 128), (3, 96), (4, 64), (7, 72), (12, 80)])
+def test_select_many_tokens_of_many_sequences(backend, group, dim):
+    """Trees of so many sequences that their scores have a kernel of their own, in groups of all widths, with tokens in several parts."""
+    rng = np.random.default_rng(group)
+    drafts = [24] * 9 + [1, 0, 7, 24]
+    run_select(backend, [int(n) for n in rng.integers(300, 16 * 60, 13)], drafts, 8 * group, 8, dim, 16, 12, tree=True)
+
+
+@pytest.mark.parametrize("pages", [520, 2040, 2060, 8150, 8200])
+def test_select_long_runs_of_several_tokens(backend, pages):
+    run_select(backend, [16 * pages + 3, 700], [8, 7], 2, 2, 64, 16, 60, repeat=2)
+    if pages < 2100:
+        run_select(backend, [16 * pages, 16 * pages - 100], [13, 12], 10, 2, 128, 16, 30)
+
+
 @pytest.mark.parametrize("pages", [3, 100, 128, 129, 400, 512])
 @pytest.mark.parametrize("what", ["scores", "ties", "one", "odd"])
 def test_select_many_lists_of_few_pages(backend, pages, what):
