@@ -231,7 +231,7 @@ def test_selected_refusals(backend):
 
 # ------------------------------------------------------------------------------------------------ shared prefixes
 # A bound of the prefix far above it: as much might be read again, if every sequence were to read it, that the prefixes have a kernel of their own (several = 1).  A bound of what a sequence has behind
-# it as well (2): as much might lie there that its rows go 32 or 128 at a time.
+# it as well (2): as much might lie there that its rows go 32 or 128 at a time.  Of the latter alone (3): prefixes that are known to be short.
 FAR = 1 << 24
 
 
@@ -265,8 +265,8 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     tab, ctx, off, groups, pre, scale = torch.from_numpy(tables).cuda(), i32(context), i32(offsets(drafts)), i32(first), i32(prefix), 1 / math.sqrt(dim)
     anc = signed(words) if words else torch.zeros(0, dtype=torch.int64, device="cuda")
     torch.cuda.synchronize()
-    op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=FAR if several else most or max(prefix),
-                                 max_own=FAR if several == 2 else most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
+    op = A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tab), held(ctx), held(groups), held(pre), max_prefix=FAR if several in (1, 2) else most or max(prefix),
+                                 max_own=FAR if several >= 2 else most or max(own), q_offsets=held(off) if arrays else None, max_drafts=max(drafts), ancestors=held(anc) if arrays else None, scale=scale)
     op.run()
     backend.synchronize_device()
     same_bits(op, out, backend)
@@ -290,7 +290,7 @@ def run_shared(backend, members, prefix, own, drafts, q_heads, kv_heads, dim, pa
     return out
 
 
-several = pytest.mark.parametrize("several", [0, 1, 2])
+several = pytest.mark.parametrize("several", [0, 1, 2, 3])
 
 
 @several
@@ -419,7 +419,7 @@ def test_shared_outside(backend, several):
     tables = torch.arange(40, dtype=torch.int32, device="cuda").repeat(8, 1)
     good_out = torch.empty_like(q)
 
-    def run(out, tables=tables, context=(40,) * 8, groups=(0, 2, 4, 6, 8), prefix=(32,) * 4, max_prefix=FAR if several else 64, max_own=40):
+    def run(out, tables=tables, context=(40,) * 8, groups=(0, 2, 4, 6, 8), prefix=(32,) * 4, max_prefix=FAR if several in (1, 2) else 64, max_own=40):
         tab, ctx, gr, pre = tables.contiguous(), i32(context), i32(groups), i32(prefix)
         out.fill_(7.0)
         torch.cuda.synchronize()
@@ -430,7 +430,7 @@ def test_shared_outside(backend, several):
     out = torch.empty_like(q)
     zeros = lambda: [t for t in range(8) if torch.count_nonzero(out[t]) == 0]  # noqa: E731
     same = lambda: [t for t in range(8) if torch.equal(out[t], good_out[t])]  # noqa: E731
-    for bad, at in ((dict(prefix=(32, 24, 32, 32)), [2, 3]), (dict(prefix=(32, 32, -16, 32)), [4, 5]), (dict(prefix=(FAR + 16 if several else 80, 32, 32, 32)), [0, 1]),
+    for bad, at in ((dict(prefix=(32, 24, 32, 32)), [2, 3]), (dict(prefix=(32, 32, -16, 32)), [4, 5]), (dict(prefix=(FAR + 16 if several in (1, 2) else 80, 32, 32, 32)), [0, 1]),
                     (dict(context=(40, 31, 40, 40, 40, 40, 73, 40)), [1, 6]), (dict(context=(40, 40, -1, 40, 40, 2**31 - 1, 40, 40)), [2, 5]),
                     (dict(groups=(1, 2, 4, 6, 8)), [0]), (dict(groups=(0, 2, 4, 6, 7)), [7]), (dict(groups=(0, 2, 4, 6, 9)), [6, 7])):
         run(out, **bad)
@@ -593,7 +593,7 @@ def test_shared_queries_with_gaps_and_rows_behind(backend, several):
     out = torch.full((5, 4, 64), 7.0, dtype=torch.bfloat16, device="cuda")
     stream = backend.create_stream()
     torch.cuda.synchronize()
-    A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR if several else 64, max_own=FAR if several == 2 else 6,
+    A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=FAR if several in (1, 2) else 64, max_own=FAR if several >= 2 else 6,
                             q_offsets=held(off), max_drafts=2).run(stream)
     backend.synchronize_stream(stream)
     assert (out[3:] == 7).all()

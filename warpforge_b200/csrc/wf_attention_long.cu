@@ -52,10 +52,13 @@ constexpr double AGAIN_BYTES = 270e6, AGAIN_FEW_BYTES = 110e6;
 // 128 rows / by 16: 8 with 12 tokens and 20, 400, 1500 keys (share 13, 44, 133) 40.6 / 33.5, 43.2 / 38.5, 50.6 / 48.5; 24 with 20, 400 (39, 132) 59.0 / 45.8, 66.0 / 54.7; 48 with 20, 400, 1500 (78, 265, 800)
 // 78.0 / 66.5, 90.8 / 87.8, 122 / 146.  With 24 tokens, 96 rows: 8 with 400 (91) 47.2 / 44.6; 24 with 100, 400 (125, 272) 72.3 / 71.5, 80.7 / 87.3; 48 with 20 (171) 109.5 / 111.6.
 constexpr double SHARE_48_ROWS = 270, SHARE_MORE_ROWS = 110;
-// The same where each sequence reads the prefix itself, by several kernels (the quicker way) / by one, 12 and 24 tokens with 100 keys of their own: 2 sequences behind 512 (15, 31) 21.8 / 8.9, 25.4 / 11.4; 8
-// behind 1024 (102, 207) 28.5 / 19.1, 30.6 / 28.5; 32 behind 512 (244) 38.3 / 34.1; 4 behind 4096 (176, 353) 32.0 / 27.5, 35.8 / 47.6; 16 / 2 heads, 32 with 24 behind 512 (248) 38.6 / 34.9; 32 / 16 heads of 64,
-// 16 behind 512 (248) 30.4 / 22.9.
-constexpr double SHARE_AGAIN = 280;
+// Prefixes of more than 32 rows in all 16 rows at a time: one token each behind a prefix, tiles of 128 rows / 16 at a time.  32 / 8 heads of 128, 16 sequences behind 1024, 4096, 16384 (share 16, 57, 223)
+// 20.1 / 14.5, 26.9 / 19.0, 34.7 / 35.9; 32 (31, 114, 446) 22.1 / 15.8, 28.3 / 24.2, 36.4 / 56.3; 64 (62, 228) 27.0 / 20.6, 32.4 / 34.0; 16 / 2 heads, 16 behind 4096, 16384 (29, 112) 24.7 / 18.4, 41.6 / 33.9.
+constexpr double SHARE_OF_PREFIX = 140;
+// Each sequence reads the prefix itself, in one kernel, by what that takes of an SM, where a prefix has more than 32 rows.  Microseconds by several kernels / by one.  Where the prefix is read 16 rows at a time, by
+// its share and that: 32 / 8 heads of 128, 16 and 32 sequences behind 1024 (16, 68; 31, 135) 14.5 / 12.5, 15.8 / 17.4; 16 / 2 heads, 32 and 64 behind 4096 (57, 116; 114, 232) 18.7 / 17.5, 23.9 / 26.8.  Where it is
+// not, sequences with more than 32 rows each (12 and 24 tokens): 32 behind 512 (244) 38.3 / 34.1; 4 behind 4096 (176, 353) 32.0 / 27.5, 35.8 / 47.6; 16 / 2 heads, 32 with 24 behind 512 (248) 38.6 / 34.9.
+constexpr double SHARE_MORE_AGAIN = 80, SHARE_AGAIN = 280;
 
 // Prefixes, then what the sequences have of their own, which begins with the first one's sums.
 template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStream_t s) {
@@ -66,8 +69,11 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     const double again = (double)(p.seqs - p.n_groups) * (double)p.max_prefix * p.cache.kv_heads * p.cache.dim * 4;
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, unit_rows = p.max_drafts * p.group, own_keys = p.max_context + p.max_drafts, all_keys = p.max_prefix + own_keys;
     const int64_t prefix_rows = p.tokens * p.group;
-    if (unit_rows > 32 && share_of_rows(c, units, unit_rows, all_keys) <= SHARE_AGAIN) return launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, (int)unit_rows, all_keys, s);
-    if (again <= (prefix_rows > 32 ? AGAIN_BYTES : AGAIN_FEW_BYTES) && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
+    const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads;
+    const double share = share_of_rows(c, units, unit_rows, all_keys), share_of_prefix = share_of_rows(c, prefixes, prefix_rows, p.max_prefix);
+    const bool sixteen = prefix_rows > 32 && share_of_prefix <= SHARE_OF_PREFIX;
+    if (sixteen ? share <= SHARE_MORE_AGAIN + share_of_prefix : unit_rows > 32 && share <= SHARE_AGAIN) return launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, (int)unit_rows, all_keys, s);
+    if (!sixteen && again <= (prefix_rows > 32 ? AGAIN_BYTES : AGAIN_FEW_BYTES) && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
     const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
     // the most cut units and pieces of them that any of the kernels leaves
     const int64_t most_cuts = (PREFIX_ROUNDS - 1) * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
@@ -78,9 +84,9 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     p.state = reinterpret_cast<float*>(more);
     p.state_dim = CHUNKS * 64;
     p.prefix_of = reinterpret_cast<int2*>(more + sums);
-    // Up to 32 rows in all go to the kernel for few rows.  Microseconds of the call, 4 sequences with one token of 32 / 8 heads of 128 behind 1024 in common: 19.7 by tiles of 128 rows, 15.3 by tiles of 16.
-    const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads;
-    rc = prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s) : launch_rows<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, prefix_rows, p.max_prefix, s);
+    rc = sixteen             ? launch_units<CHUNKS, 1, ATTEND_PREFIX>(c, p, prefixes, (int)prefix_rows, p.max_prefix, s)
+         : prefix_rows > 32 ? launch_wide_tree<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, p.tokens, p.max_prefix, s)
+                            : launch_rows<CHUNKS, ATTEND_PREFIX>(c, p, prefixes, prefix_rows, p.max_prefix, s);
     if (rc != WF_OK) return rc;
     if (unit_rows > 32 && share_of_rows(c, units, unit_rows, own_keys) <= (unit_rows <= 48 ? SHARE_48_ROWS : SHARE_MORE_ROWS))
         return launch_units<CHUNKS, 1, ATTEND_OWN>(c, p, units, (int)unit_rows, own_keys, s);
