@@ -454,3 +454,49 @@ def test_select_replayed(backend):
             assert (out[0, h].tolist(), lens[0, h].tolist()) == want
     ctx.graph_destroy(graph)
     backend.destroy_stream(stream)
+
+
+def test_select_of_several_tokens_recorded(backend):
+    """Scores of several tokens lie in the scratch of the stream: it has to be there before the call is recorded; replayed beside a larger call on the same stream the graph keeps its own."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(13)
+    ctx = backend.cuda_context
+
+    def make(tokens, pages, most):
+        q = normal(rng, tokens, 4, 64)
+        codes, scales = torch.from_numpy(rng.integers(-60, 60, (pages, 2, 2, 64)).astype(np.int8)).cuda(), torch.ones(pages, 2, device="cuda")
+        tables, context = torch.arange(pages, dtype=torch.int32, device="cuda")[None], i32([0])
+        out, lens = torch.zeros(tokens, 2, 20, dtype=torch.int32, device="cuda"), torch.zeros(tokens, 2, 2, dtype=torch.int32, device="cuda")
+        torch.cuda.synchronize()
+        op = A.SelectPages(ctx, held(q), held8(codes), held8(scales), held(tables), held(context), held(out), held(lens), page_tokens=16, max_context=most, recent=16, max_drafts=tokens, tree=True)
+        return op, q, codes, scales, context, out, lens
+
+    op, q, codes, scales, context, out, lens = make(24, 2000, 16 * 1990)
+    larger = make(24, 4000, 16 * 3990)
+    stream = backend.create_stream()
+    ctx.graph_begin(stream)
+    with pytest.raises(N.WfError) as e:
+        op.run(stream)
+    assert e.value.status == N.WF_ERR_RECORDING
+    ctx.graph_destroy(ctx.graph_end(stream))
+    op.run(stream)
+    ctx.graph_begin(stream)
+    op.run(stream)
+    graph = ctx.graph_end(stream)
+    larger[0].run(stream)
+    for n in (5, 600, 16 * 1990):
+        context.fill_(n)
+        torch.cuda.synchronize()
+        ctx.graph_launch(graph, stream)
+        larger[0].run(stream)
+        ctx.synchronize(stream)
+        for t in (0, 23):
+            for h in range(2):
+                want = plain_list(q[t, 2 * h:2 * h + 2].double().cpu().numpy(), codes[:, h].double().cpu().numpy(), scales[:, h].double().cpu().numpy(), list(range(2000)), n, 24, t, True, 16, 20, 1, 16)
+                assert (out[t, h].tolist(), lens[t, h].tolist()) == want
+    ctx.graph_destroy(graph)
+    backend.destroy_stream(stream)
