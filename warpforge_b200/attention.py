@@ -343,15 +343,15 @@ class KvCache:
             a, b = np.array(sequences[i - 1].pages[:m]), np.array(sequences[i].pages[:m])
             other = np.flatnonzero(a != b)
             common.append(int(other[0]) if len(other) else m)
-        saved, begin = [0] * (n + 1), [0] * (n + 1)  # of the first i sequences; where the last group of them begins
-        for i in range(1, n + 1):
-            saved[i], begin[i], least = saved[i - 1], i - 1, None
-            for j in range(i - 2, -1, -1):
-                least = common[j] if least is None else min(least, common[j])
-                if least == 0:
-                    break
-                if saved[j] + least * (i - j - 1) > saved[i]:
-                    saved[i], begin[i] = saved[j] + least * (i - j - 1), j
+        shared = np.array(common, np.int64)
+        saved, begin = np.zeros(n + 1, np.int64), list(range(-1, n))  # pages, of the first i sequences; where the last group of them begins
+        for i in range(2, n + 1):
+            before = np.arange(i - 2, -1, -1)  # where that may be, if it is more than one sequence
+            gain = saved[before] + np.minimum.accumulate(shared[before]) * (i - 1 - before)
+            best = int(np.argmax(gain))
+            saved[i] = max(gain[best], saved[i - 1])
+            if gain[best] > saved[i - 1]:
+                begin[i] = int(before[best])
         groups = [n]
         while groups[0]:
             groups.insert(0, begin[groups[0]])
