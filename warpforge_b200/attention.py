@@ -260,6 +260,40 @@ class SelectPages(_Bound):
         super().__init__(context, "wf_select_pages", a, None, 0, (q, codes, scales, tables, context_lens, pages_out, lens_out, q_offsets))
 
 
+def _common(a: List[int], b: List[int], n: int) -> int:
+    """How many of their first n pages two lists have in common, at the start."""
+    if a[:n] == b[:n]:
+        return n
+    lo, hi = 0, n  # the first other one lies there
+    while hi - lo > 1:
+        mid = (lo + hi) // 2
+        if a[lo:mid] == b[lo:mid]:
+            lo = mid
+        else:
+            hi = mid
+    return lo
+
+
+def _fewest_pages(common: Seq[int]) -> List[int]:
+    """Where groups of a run of sequences end; common: what each has in common with the next one."""
+    n = len(common) + 1
+    if n == 1 or min(common) == max(common):
+        return [n]
+    shared = np.array(common, np.int64)
+    saved, begin = np.zeros(n + 1, np.int64), list(range(-1, n))  # pages, of the first i sequences; where the last group of them begins
+    for i in range(2, n + 1):
+        before = np.arange(i - 2, -1, -1)  # where that may be, if it is more than one sequence
+        gain = saved[before] + np.minimum.accumulate(shared[before]) * (i - 1 - before)
+        best = int(np.argmax(gain))
+        saved[i] = max(gain[best], saved[i - 1])
+        if gain[best] > saved[i - 1]:
+            begin[i] = int(before[best])
+    ends = [n]
+    while begin[ends[0]]:
+        ends.insert(0, begin[ends[0]])
+    return ends
+
+
 class KvCache:
     """`pages` pages of page_tokens tokens for every layer: keys and values bf16 [layers, pages, kv_heads, page_tokens, head_dim], allocated here or
     given.  Page numbers are handed out by the native pool (wf_pages_*), which counts the sequences that hold each."""
@@ -337,25 +371,16 @@ class KvCache:
         size, n = self.page_tokens, len(sequences)
         tokens = [s.tokens for s in sequences] if tokens is None else tokens
         whole = [min(len(s.pages), t // size) for s, t in zip(sequences, tokens)]
-        common = []  # whole pages that a sequence and the one before it begin with
-        for i in range(1, n):
-            m = min(whole[i - 1], whole[i])
-            a, b = np.array(sequences[i - 1].pages[:m]), np.array(sequences[i].pages[:m])
-            other = np.flatnonzero(a != b)
-            common.append(int(other[0]) if len(other) else m)
-        shared = np.array(common, np.int64)
-        saved, begin = np.zeros(n + 1, np.int64), list(range(-1, n))  # pages, of the first i sequences; where the last group of them begins
-        for i in range(2, n + 1):
-            before = np.arange(i - 2, -1, -1)  # where that may be, if it is more than one sequence
-            gain = saved[before] + np.minimum.accumulate(shared[before]) * (i - 1 - before)
-            best = int(np.argmax(gain))
-            saved[i] = max(gain[best], saved[i - 1])
-            if gain[best] > saved[i - 1]:
-                begin[i] = int(before[best])
-        groups = [n]
-        while groups[0]:
-            groups.insert(0, begin[groups[0]])
-        prefix = [min(common[a:b - 1]) * size if b - a > 1 else 0 for a, b in zip(groups, groups[1:])]
+        common = [_common(sequences[i - 1].pages, sequences[i].pages, min(whole[i - 1], whole[i])) for i in range(1, n)]  # whole pages that a sequence and the one before it begin with
+        groups, prefix = [0], []
+        while groups[-1] < n:
+            first = stop = groups[-1]  # a run of sequences that have something in common with the next
+            while stop + 1 < n and common[stop]:
+                stop += 1
+            for end in _fewest_pages(common[first:stop]):
+                a, b = groups[-1], first + end
+                groups.append(b)
+                prefix.append(min(common[a:b - 1], default=0) * size)
         return np.array(groups, np.int32), np.array(prefix, np.int32)
 
     def fork(self, sequences: Seq[Sequence], stream: int = 0) -> List[Sequence]:

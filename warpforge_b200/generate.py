@@ -332,15 +332,18 @@ def main() -> None:
                     selected_pages=a.selected_pages)
     rng = np.random.default_rng(0)
     prompts = [rng.integers(0, a.vocab, a.prompt) for _ in range(a.sequences)]
+    samples = lambda seqs: [s if i == 0 else s.fork() for s in seqs for i in range(a.samples)]  # noqa: E731
     warm = [model.sequence() for _ in prompts]
     model.prefill(warm, prompts)
+    warm = samples(warm)
+    model.step(warm, [[0]] * len(warm))
     for s in warm:
         s.free()
     seqs = [model.sequence() for _ in prompts]
     t0 = time.perf_counter()
     last = [int(np.argmax(x[-1])) for x in model.prefill(seqs, prompts)]
     t1 = time.perf_counter()
-    seqs = [s if i == 0 else s.fork() for s in seqs for i in range(a.samples)]
+    seqs = samples(seqs)
     last = [(t + i) % a.vocab for t in last for i in range(a.samples)]  # each continues with another token
     out = [[t] for t in last]
     for _ in range(a.tokens - 1):
