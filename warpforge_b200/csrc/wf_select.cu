@@ -164,6 +164,8 @@ struct SelectSeq {
     int64_t row0;
     int rows, context;
     int last, tail, first, between;  // pages in all, from where on all are taken, how many at the start are, how many lie between
+    int take;                        // how many of those between a list has room for (0 or more: the host sees to it that the ends fit)
+    __device__ __forceinline__ bool scored() const { return take > 0 && take < between; }  // else a list has all of them, or none
 };
 __device__ __forceinline__ SelectSeq select_seq(const SelectParams& p, int s, bool report) {
     SelectSeq q;
@@ -179,6 +181,7 @@ __device__ __forceinline__ SelectSeq select_seq(const SelectParams& p, int s, bo
     q.tail = bad ? 0 : max(0, q.context - p.recent) >> p.page_shift;
     q.first = min(p.first, q.tail);
     q.between = q.tail - q.first;
+    q.take = min(q.between, p.width - q.first - (q.last - q.tail));
     return q;
 }
 
@@ -275,8 +278,8 @@ template <int CHUNKS, int PADDED> __global__ void __launch_bounds__(SCORE_WARPS 
     const int s = blockIdx.y / p.kv_heads, head = blockIdx.y - s * p.kv_heads, padded = PADDED ? PADDED : (p.group + 7) & ~7;
     const SelectSeq q = select_seq(p, s, false);
     const int begin = blockIdx.x * p.score_pages, end = min(begin + p.score_pages, q.between);
-    // where all pages are taken, the kernel behind this one does not look at the scores
-    if (q.rows == 0 || begin >= end || q.between <= p.width - q.first - (q.last - q.tail)) return;
+    // the kernel behind this one does not look at the scores where all pages are taken, or none
+    if (q.rows == 0 || begin >= end || !q.scored()) return;
     const int* const table = p.tables + (size_t)s * p.table_stride;
     const int tokens_at_once = SCORE_COLUMNS / padded;
     const size_t apart = (size_t)p.kv_heads * p.room;  // scores of a token
@@ -388,8 +391,8 @@ __device__ __forceinline__ uint4 load_scores(const uint32_t* from) {
 }
 
 // What a list has in any case, by `lanes` threads of which this is number `lane`: the places that the scores do not decide, the lengths.
-__device__ __forceinline__ void write_ends(const SelectParams& p, const SelectSeq& q, int64_t line, int i, int take, const int* table, int* list, int lane, int lanes) {
-    const int first = q.first, count = first + q.last - q.tail + take;
+__device__ __forceinline__ void write_ends(const SelectParams& p, const SelectSeq& q, int64_t line, int i, const int* table, int* list, int lane, int lanes) {
+    const int first = q.first, take = q.take, count = first + q.last - q.tail + take;
     for (int n = lane; n < p.width - take; n += lanes) {
         const int at = n < first ? n : n + take, page = at < first ? at : q.tail + at - first - take;
         list[at] = at < count ? table[page] : -1;
@@ -414,10 +417,10 @@ template <int RUN> __global__ void __launch_bounds__(FEW_WARPS * 32) select_few_
     const int64_t line = (q.row0 + i) * p.kv_heads + head;
     const int* const table = p.tables + (size_t)s * p.table_stride;
     int* const list = p.pages_out + (size_t)line * p.width;
-    const int take = min(q.between, p.width - q.first - (q.last - q.tail));
+    const int take = q.take;
     const int from = lane * RUN, valid = max(0, min(RUN, q.between - from));
     uint32_t d[RUN];
-    if (take < q.between) {
+    if (q.scored()) {
         const uint32_t* const scores = p.scores + (size_t)line * p.room;
 #pragma unroll
         for (int e = 0; e < RUN; e += 4) {
@@ -425,8 +428,8 @@ template <int RUN> __global__ void __launch_bounds__(FEW_WARPS * 32) select_few_
             d[e] = v.x, d[e + 1] = v.y, d[e + 2] = v.z, d[e + 3] = v.w;
         }
     }
-    write_ends(p, q, line, i, take, table, list, lane, 32);
-    if (take == q.between) {  // all of them
+    write_ends(p, q, line, i, table, list, lane, 32);
+    if (!q.scored()) {
         for (int n = lane; n < take; n += 32) list[q.first + n] = table[q.first + n];
         return;
     }
@@ -502,11 +505,10 @@ template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_
     }
     const int64_t row = q.row0 + i;
     const int* const table = p.tables + (size_t)s * p.table_stride;
-    const int first = q.first, between = q.between;
-    const int take = min(between, p.width - first - (q.last - q.tail));  // the host sees to it that the ends fit
+    const int first = q.first, between = q.between, take = q.take;
     int* const list = p.pages_out + ((size_t)row * p.kv_heads + head) * p.width;
-    if (rank == ranks - 1) write_ends(p, q, row * p.kv_heads + head, i, take, table, list, tid, THREADS);
-    if (take == between) {  // all of them
+    if (rank == ranks - 1) write_ends(p, q, row * p.kv_heads + head, i, table, list, tid, THREADS);
+    if (!q.scored()) {
         if (rank == 0)
             for (int n = tid; n < take; n += THREADS) list[first + n] = table[first + n];
         cluster_wait();
