@@ -1,9 +1,10 @@
 """Page bounds, selection of pages and shared prefixes where a call has just no room, numbers are at the end of their range, or offsets cannot be.  Bounds and lists are exact and
 compared for equality; attention is held against 64 bits with the tolerance of test_gpu_attention.py."""
+import numpy as np
 import pytest
 
-from test_gpu_attention import backend  # noqa: F401
-from test_gpu_select import run_select
+from test_gpu_attention import backend, held, i32, normal  # noqa: F401
+from test_gpu_select import bounds_of, held8, run_select
 
 pytestmark = pytest.mark.gpu
 
@@ -17,3 +18,36 @@ def test_select_no_room_between(backend, pages, tokens):
         lens = [16 * pages + rest, 700, 0]
         run_select(backend, lens, [tokens, 1, tokens], 8, 2, 64, 16, width, first, recent, tree=True, repeat=2)
     run_select(backend, [16 * pages + 3] * (40 if pages <= 400 else 2), [1] * (40 if pages <= 400 else 2), 4, 4, 128, 16, 1, 0, 0)
+
+
+@pytest.mark.parametrize("page,first,stop,most", [(1024, 1 << 30, (1 << 30) + 5, (1 << 31) - 1024), (1024, 2**31 - 2048, 2**31 - 1030, 2**31 - 2048), (1024, 5, 1030, (1 << 31) - 1024)])
+def test_bounds_at_the_end_of_long_tables(backend, page, first, stop, most):
+    """Tables for as many tokens as there may be, and a call with room for as many again behind the first one: its pages' numbers pass 2^31 tokens.  All but the two pages of the range
+    lie outside the cache, where nothing is to be looked at."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(page)
+    keys = normal(rng, 1, 3, 1, page, 8)
+    codes, scales = torch.full((1, 3, 1, 2, 8), 77, dtype=torch.int8, device="cuda"), torch.full((1, 3, 1), 77.0, device="cuda")
+    cache = A.KvCache(backend.cuda_context, 1, 3, page, 1, 8, keys=held(keys), values=held(keys))
+    bounds = A.PageBounds(cache, held8(codes), held8(scales))
+    tables = torch.full((1, 2**31 // page - 1), -7, dtype=torch.int32, device="cuda")
+    tables[0, first // page], tables[0, (stop - 1) // page] = 0, 2
+    at, to = i32([first]), i32([stop])
+    torch.cuda.synchronize()
+    bounds.update(held(tables), held(at), held(to), max_tokens=most)
+    backend.synchronize_device()
+    done = {2: stop - (stop - 1) // page * page}
+    if first // page != (stop - 1) // page:
+        done[0] = page
+    for name in range(3):
+        want = bounds_of(keys[0, name, 0, :done[name]]) if name in done else (np.full((2, 8), 77, np.int8), 77.0)
+        assert np.array_equal(codes[0, name, 0].cpu().numpy(), want[0]) and scales[0, name, 0].item() == want[1]
+    with pytest.raises(N.WfError) as e:
+        bounds.update(held(tables), held(at), held(to), max_tokens=2**31)
+    assert e.value.status == N.WF_ERR_SHAPE
+    bounds.close()
+    cache.close()

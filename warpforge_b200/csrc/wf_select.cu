@@ -66,7 +66,8 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) page_bounds_kernel(const __
             if (lane == 0) report_status(p.status, STATUS_BAD_INDEX);
             continue;
         }
-        const int j = (first >> shift) + index, begin = j << shift;
+        const int j = (first >> shift) + index;
+        const int64_t begin = (int64_t)j << shift;  // of a range whose call has room for more: behind 2^31, too
         if (first == stop || begin >= stop) continue;
         const int64_t page = p.tables[s * p.table_stride + j];
         if (page < 0 || page >= p.cache.pages) {
@@ -74,7 +75,7 @@ __global__ void __launch_bounds__(BOUNDS_WARPS * 32) page_bounds_kernel(const __
             continue;
         }
         const uint4* from = reinterpret_cast<const uint4*>(keys + p.cache.at(page, head, 0)) + lane;
-        const int all = lane < active ? min(page_tokens, stop - begin) * pieces - lane : 0;  // this lane's pieces: 0, active, 2 active .. below it
+        const int all = lane < active ? (int)min((int64_t)page_tokens, stop - begin) * pieces - lane : 0;  // this lane's pieces: 0, active, 2 active .. below it
         uint32_t hi[4], lo[4];
 #pragma unroll
         for (int e = 0; e < 4; e++) hi[e] = 0xFF80FF80u, lo[e] = 0x7F807F80u;  // -Inf, +Inf
