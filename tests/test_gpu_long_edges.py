@@ -4,6 +4,7 @@ import numpy as np
 import pytest
 
 from test_gpu_attention import backend, held, i32, normal  # noqa: F401
+from test_gpu_generate_long import check_bounds, closed, make
 from test_gpu_select import bounds_of, held8, run_select
 
 pytestmark = pytest.mark.gpu
@@ -51,3 +52,23 @@ def test_bounds_at_the_end_of_long_tables(backend, page, first, stop, most):
     assert e.value.status == N.WF_ERR_SHAPE
     bounds.close()
     cache.close()
+
+
+def test_bounds_of_pages_whose_drafts_are_kept_by_others():
+    """Forks between step and keep: one keeps a part of a page at its place, one all of it, one moves tokens.  Bounds of full pages are those of their keys."""
+    m = make(2, selected_pages=20, recent_tokens=0)
+    rng = np.random.default_rng(11)
+    a = m.sequence()
+    m.prefill([a], [rng.integers(0, 320, 42)])
+    m.step([a], [list(map(int, rng.integers(0, 320, 25)))])
+    b, c = a.fork(), a.fork()
+    check_bounds(m, [a, b, c])
+    m.keep([a, b, c], [25] * 3, [[0, 1], list(range(25)), [0, 4, 5, 6, 7, 9]])
+    assert a.pages[2] == b.pages[2] != c.pages[2] and (a.tokens, b.tokens, c.tokens) == (44, 67, 48)
+    check_bounds(m, [a, b, c])
+    m.step([a, b, c], [list(map(int, rng.integers(0, 320, n))) for n in (5, 1, 17)])
+    m.keep([a, b, c], [5, 1, 17], [[0, 1, 2, 3], [0], [1, 2]])
+    check_bounds(m, [a, b, c])
+    for s in (a, b, c):
+        s.free()
+    closed(m)

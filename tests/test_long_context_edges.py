@@ -1,0 +1,101 @@
+"""A decoder that selects pages, as far as it needs no device: which bounds it asks for, which memory it holds."""
+import numpy as np
+
+from test_long_context_host import HostContext
+
+from warpforge_b200.generate import Decoder, DecoderSpec
+from warpforge_b200.quant import QuantizationType
+
+
+class Watched(HostContext):
+    """... that knows what was copied where."""
+
+    def __init__(self):
+        super().__init__()
+        self.sent = {}
+
+    def copy_to_device(self, dptr, host, stream=0, sync=True):
+        super().copy_to_device(dptr, host, stream, sync)
+        self.sent[dptr] = host.copy()
+
+
+def decoder(max_tokens=64, max_sequences=4, **more):
+    spec = DecoderSpec(QuantizationType.Q8_0, 64, 2, 1, 32, 64, 1, 64, max_positions=200)
+    return Decoder(Watched(), spec, pages=30, page_tokens=16, max_tokens=max_tokens, max_sequences=max_sequences, selected_pages=12, recent_tokens=0, **more)
+
+
+def watch_bounds(m):
+    """Pages and rows of every update that follows."""
+    seen = []
+
+    def update(tables, first, stop, *, max_tokens):
+        table, first, stop = (m.ctx.sent[x.ptr].reshape(x.shape()) for x in (tables, first, stop))
+        now = []
+        for row, a, b in zip(table, first, stop):
+            assert 0 <= a <= b and b - a <= max_tokens
+            now += [(int(row[j]), min(16, int(b) - 16 * j)) for j in range(a // 16, -(-b // 16))] if a < b else []
+        assert len({page for page, _ in now}) == len(now), "a page by two sequences"
+        for page, rows in now:
+            assert rows == 16 or m.cache.holders(page) == 1, f"{rows} rows of page {page}, which others hold too"
+        seen.append(now)
+
+    m.bounds.update = update
+    return seen
+
+
+def test_kept_drafts_leave_the_bounds_of_pages_that_others_hold():
+    """A fork between step and keep holds a page whole of which keep retains a part, at its place."""
+    m = decoder()
+    a = m.sequence()
+    m.prefill([a], [np.arange(10)])
+    seen = watch_bounds(m)
+    m.step([a], [[0] * 6])
+    assert seen == [[(a.pages[0], 16)]]
+    b = a.fork()
+    m.keep([a], [6], [[0, 1]])
+    assert a.pages == b.pages and (a.tokens, b.tokens) == (12, 16) and [x for now in seen[1:] for x in now] == []
+    m.step([a, b], [[0], [0]])
+    assert a.pages[0] != b.pages[0] and seen[-1] == [(a.pages[0], 13), (b.pages[1], 1)]
+    m.keep([a, b], [1, 1], [[0], [0]])
+    # both branches in one call: one keeps what lies at its place, the other one moves tokens
+    c = m.sequence()
+    m.prefill([c], [np.arange(10)])
+    m.step([c], [[0] * 22], [[-1] * 22])
+    d, e = c.fork(), c.fork()
+    m.keep([c, d, e], [22] * 3, [[0, 1], list(range(22)), [0, 3, 4]])
+    assert c.pages[0] == d.pages[0] != e.pages[0] and seen[-1] == [(e.pages[0], 13)]
+    m.step([c, d, e], [[0]] * 3)
+    for s in (a, b, c, d, e):
+        s.free()
+    assert m.cache.free_pages() == 30
+    m.close()
+
+
+def test_full_pages_have_bounds_of_all_their_rows():
+    """Steps, forks and keeps at random: what the last update of a page says is what a sequence that holds it full has."""
+    rng = np.random.default_rng(5)
+    for _ in range(30):
+        m = decoder()
+        seqs, rows = [m.sequence()], {}
+        seen = watch_bounds(m)
+        m.prefill(seqs, [np.arange(int(rng.integers(1, 50)))])
+        for _ in range(12):
+            n = [int(rng.integers(0, 12)) for _ in seqs]
+            m.step(seqs, [[0] * k for k in n], [[-1] * k for k in n])
+            if len(seqs) < 4 and rng.random() < 0.5:
+                i = int(rng.integers(len(seqs)))
+                seqs.append(seqs[i].fork())
+                n.append(n[i])
+            kept = [sorted(rng.choice(k, int(rng.integers(0, k + 1)), replace=False).tolist()) if rng.random() < 0.5 else list(range(int(rng.integers(0, k + 1)))) for k in n]
+            m.keep(seqs, n, kept)
+            for now in seen:
+                rows.update(now)
+            seen.clear()
+            for s in seqs:
+                for page in s.pages[:s.tokens // 16]:
+                    assert rows[page] == 16
+                if s.tokens > 100:
+                    s.truncate(int(rng.integers(1, 40)))
+        for s in seqs:
+            s.free()
+        m.close()

@@ -98,7 +98,7 @@ class Decoder:
             self._room.update(groups=(max_sequences + 1) * 4, prefixes=(max_sequences + 1) * 4)
         self.bounds = A.PageBounds(self.cache) if selected_pages else None
         if selected_pages:
-            self._room.update(before=(max_sequences + 1) * 4, lists=max_tokens * s.kv_heads * selected_pages * 4, list_lens=max_tokens * s.kv_heads * 8)
+            self._room.update(before=(max_sequences + 1) * 4, moved=(max_sequences + 1) * 4, lists=max_tokens * s.kv_heads * selected_pages * 4, list_lens=max_tokens * s.kv_heads * 8)
         self._room = {n: max(room, 16) for n, room in self._room.items()}
         self.buf.update({n: self._alloc(room) for n, room in self._room.items()})
 
@@ -289,11 +289,12 @@ class Decoder:
             row[:len(k)] = k
         context = [s.tokens - n for s, n in zip(sequences, drafted)]
         still = [next((i for i, j in enumerate(k) if i != j), len(k)) for k in kept]  # tokens that lie where they belong
-        self.cache.own(sequences, [(c + n, c + len(k)) for c, n, k in zip(context, still, kept)])
+        moved = [(c + n, c + len(k)) for c, n, k in zip(context, still, kept)]
+        self.cache.own(sequences, moved)
         tables, lens = self._tables(sequences), self._send("lens", context, "i32")
         self.cache.compact(tables, lens, self._send("kept", rows, "i32"), self._send("counts", [len(k) for k in kept], "i32"))
-        if self.bounds:
-            self._bound(tables, lens, self._send("before", [c + len(k) for c, k in zip(context, kept)], "i32"), max(len(k) for k in kept) if kept else 0)
+        if self.bounds:  # of the pages that tokens moved to.  Where none did, others may hold more of a page than is kept here, and ``step`` has left the bounds of all of it
+            self._bound(tables, self._send("moved", [a for a, _ in moved], "i32"), self._send("before", [b for _, b in moved], "i32"), max((b - a for a, b in moved), default=0))
         self.ctx.synchronize()
         for s, c, k in zip(sequences, context, kept):
             s.truncate(c + len(k))
