@@ -3,8 +3,9 @@ compared for equality; attention is held against 64 bits with the tolerance of t
 import numpy as np
 import pytest
 
-from test_gpu_attention import backend, held, i32, normal  # noqa: F401
+from test_gpu_attention import backend, held, i32, normal, offsets  # noqa: F401
 from test_gpu_generate_long import check_bounds, closed, make
+from test_gpu_long_attention import FAR, several
 from test_gpu_select import bounds_of, held8, run_select
 
 pytestmark = pytest.mark.gpu
@@ -72,3 +73,55 @@ def test_bounds_of_pages_whose_drafts_are_kept_by_others():
     for s in (a, b, c):
         s.free()
     closed(m)
+
+
+def run_offsets(backend, offs, several, group, n, members, prefix):
+    """What a call with these offsets leaves, its scratch full of another call's sums before; and what it leaves where they are one token each."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(n)
+    q, keys, values = normal(rng, n, 2 * group, 64), normal(rng, 40, 2, 16, 64), normal(rng, 40, 2, 16, 64)
+    groups, tables, context = i32(offsets(members)), torch.arange(40, dtype=torch.int32, device="cuda").repeat(n, 1), i32([p + 9 for p, m in zip(prefix, members) for _ in range(m)])
+    pre, outs = i32(prefix), []
+    for at, v in ((list(range(n + 1)), values * 1000), (list(range(n + 1)), values), (list(range(n + 1)), values * 1000), (offs, values)):
+        out, off = torch.full_like(q, 7.0), i32(at)
+        torch.cuda.synchronize()
+        A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(v), held(out), held(tables), held(context), held(groups), held(pre), q_offsets=held(off), max_drafts=3,
+                                max_prefix=FAR if several in (1, 2) else max(prefix), max_own=FAR if several >= 2 else 9).run()
+        if at is offs:
+            with pytest.raises(N.WfError) as e:
+                backend.synchronize_device()
+            assert e.value.status == N.WF_ERR_INDEX
+        else:
+            backend.synchronize_device()
+        outs.append(out)
+    return outs[3], outs[1]
+
+
+@several
+@pytest.mark.parametrize("group,members", [(2, [3, 2, 1, 2]), (4, [10, 13, 1, 16])])
+def test_shared_offsets_that_cannot_be(backend, several, group, members):
+    """Where a group's offsets leave the tokens, or one of its sequences has rows outside them, that group's sequences have zeros, as far as their own rows are rows; the other groups keep
+    their bits, and no sum is used that this call has not made."""
+    import torch
+
+    n, first = sum(members), offsets(members)
+    prefix = [160, 96, 0, 128]
+    same = list(range(n + 1))
+    # the last group's last offset behind the tokens; the second group's last sequence ends before it begins, and those before it lie behind the group's end
+    last = same[:-1] + [n + 1]
+    got, good = run_offsets(backend, last, several, group, n, members, prefix)
+    assert torch.equal(got[:first[3]], good[:first[3]]) and torch.count_nonzero(got[first[3]:n - 1]) == 0 and (got[n - 1] == 7).all()
+    swapped = list(same)
+    swapped[first[1] + 1] = first[2] + 1  # the second group's first sequence: as many rows as reach behind its group
+    if first[2] + 1 - first[1] <= 3:  # (no more than max_drafts)
+        got, good = run_offsets(backend, swapped, several, group, n, members, prefix)
+        others = list(range(first[1])) + list(range(first[3], n))
+        assert torch.equal(got[others], good[others])
+        assert torch.isfinite(got.float()).all() and got[first[1]:first[2]].float().abs().max() == 0
+    before = [-1] + same[1:]
+    got, good = run_offsets(backend, before, several, group, n, members, prefix)
+    assert torch.equal(got[first[1]:], good[first[1]:]) and torch.count_nonzero(got[1:first[1]]) == 0 and (got[0] == 7).all()

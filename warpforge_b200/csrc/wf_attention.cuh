@@ -73,7 +73,7 @@ struct TreeParams {
     const int* prefix;
     int64_t max_prefix;
     int n_groups;
-    int2* prefix_of;  // [seqs], made by the kernel that reads the prefixes: prefix (-1: cannot be) and first sequence of the group
+    int2* prefix_of;  // [seqs], made by the kernel that reads the prefixes: prefix (-1: cannot be, or has no sums for these rows) and first sequence of the group
     float* state;     // of every row over its prefix: sums [tokens * q_heads][state_dim], then maxima, then sums of weights
     int state_dim;
 #ifdef __CUDACC__
@@ -164,6 +164,12 @@ __device__ __forceinline__ GroupSeqs group_seqs(const TreeParams& p, int g) {
     }
     return q;
 }
+// Whether a sequence's rows lie among those of its group: the others have no sums over the prefix.
+__device__ __forceinline__ bool rows_in_group(const TreeParams& p, const GroupSeqs& g, int s) {
+    if (!p.q_offsets || g.prefix <= 0) return true;
+    const int from = p.q_offsets[g.first], to = p.q_offsets[g.stop], a = p.q_offsets[s], b = p.q_offsets[s + 1];
+    return from >= 0 && from <= a && a <= b && b <= to && to <= p.tokens;
+}
 __device__ __forceinline__ TreeSeq prefix_seq(const TreeParams& p, int g) {
     TreeSeq q;
     const GroupSeqs of = group_seqs(p, g);
@@ -201,7 +207,7 @@ __device__ __forceinline__ TreeSeq own_seq(const TreeParams& p, int s) {
     q.place.first = 0;
     return q;
 }
-// The prefix of a sequence and whose pages hold it; -1 where its group cannot be.
+// The prefix of a sequence and whose pages hold it; -1 where its group cannot be, or cannot have its rows.
 __device__ __forceinline__ int2 prefix_of_seq(const TreeParams& p, int s) {
     int lo = 0, hi = p.n_groups - 1;  // the last group that begins at s or before it
 #pragma unroll 1
@@ -211,7 +217,7 @@ __device__ __forceinline__ int2 prefix_of_seq(const TreeParams& p, int s) {
         else hi = mid - 1;
     }
     const GroupSeqs of = group_seqs(p, lo);
-    return make_int2(s < of.first || s >= of.stop ? -1 : of.prefix, of.first);
+    return make_int2(s < of.first || s >= of.stop || !rows_in_group(p, of, s) ? -1 : of.prefix, of.first);
 }
 __device__ __forceinline__ TreeSeq whole_seq(const TreeParams& p, int s) {
     TreeSeq q;

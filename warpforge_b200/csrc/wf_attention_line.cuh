@@ -187,7 +187,7 @@ __device__ __forceinline__ void leave_prefixes(const TreeParams& p, bool none) {
     const int lane = threadIdx.x & 31;
     for (int g = blockIdx.x; g < p.n_groups; g += gridDim.x) {
         const GroupSeqs of = group_seqs(p, g);
-        for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(none ? -1 : of.prefix, of.first);
+        for (int s = of.first + lane; s < of.stop; s += 32) p.prefix_of[s] = make_int2(none || !rows_in_group(p, of, s) ? -1 : of.prefix, of.first);
     }
     if (blockIdx.x == 0) {  // those that no group has
         const int before = max(0, min(p.groups[0], p.seqs)), behind = max(0, min(p.groups[p.n_groups], p.seqs));
