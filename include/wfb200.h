@@ -412,7 +412,8 @@ int wf_selected_attention(int64_t ctx, const wf_selected_attention_args* args, c
  *   groups_dev   int32 [n_groups + 1], ascending from 0 to seqs; prefix_dev int32 [n_groups], 0 = nothing in common
  *   max_prefix   most tokens of a prefix; max_own: most context[s] - prefix of a sequence
  * A group whose prefix, sequences or offsets cannot be, a sequence with a context shorter than the prefix, and one with rows outside those of its group
- * (q_offsets[groups[g]] .. q_offsets[groups[g + 1]]) are WF_ERR_INDEX and rows of zeros.  At most WF_SHARED_MAX_TOKENS tokens. */
+ * (q_offsets[groups[g]] .. q_offsets[groups[g + 1]]) are WF_ERR_INDEX and rows of zeros.  So is a call whose prefixes, 16 keys at a time, are 2^31 or more for all heads together;
+ * where the other keys are that many, WF_ERR_INDEX and rows as they were.  At most WF_SHARED_MAX_TOKENS tokens. */
 #define WF_SHARED_MAX_TOKENS 131072
 typedef struct wf_shared_prefix_attention_args {
     int64_t q_dev, out_dev;

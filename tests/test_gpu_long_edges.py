@@ -125,3 +125,32 @@ def test_shared_offsets_that_cannot_be(backend, several, group, members):
     before = [-1] + same[1:]
     got, good = run_offsets(backend, before, several, group, n, members, prefix)
     assert torch.equal(got[first[1]:], good[first[1]:]) and torch.count_nonzero(got[1:first[1]]) == 0 and (got[0] == 7).all()
+
+
+def test_shared_prefixes_of_more_tiles_than_a_line_has(backend):
+    """128 heads behind 2^28 tokens (one page, over and over) are more tiles than the CTAs' shares are counted in: reported, and no sums are used that were not made."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(21)
+    q, keys, values = normal(rng, 2, 128, 8), normal(rng, 2, 128, 1024, 8), normal(rng, 2, 128, 1024, 8) * 1000
+    tables = torch.zeros(2, 2**18 + 1, dtype=torch.int32, device="cuda")
+    groups = i32([0, 2])
+
+    def run(prefix):
+        out, context, pre = torch.full_like(q, 7.0), i32([prefix] * 2), i32([prefix])
+        torch.cuda.synchronize()
+        A.SharedPrefixAttention(backend.cuda_context, held(q), held(keys), held(values), held(out), held(tables), held(context), held(groups), held(pre), max_prefix=1 << 28, max_own=0).run()
+        if prefix < 1 << 28:
+            backend.synchronize_device()
+            return out
+        with pytest.raises(N.WfError) as e:
+            backend.synchronize_device()
+        assert e.value.status == N.WF_ERR_INDEX
+        return out
+
+    for _ in range(2):
+        assert torch.count_nonzero(run(2048)) > 0  # sums in the scratch
+        assert torch.count_nonzero(run(1 << 28)) == 0

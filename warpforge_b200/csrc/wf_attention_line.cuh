@@ -56,8 +56,8 @@ struct LineUnit {
 };
 
 #ifdef __CUDACC__
-// Walks the share of this CTA, the whole warp together: f(unit) for every unit that has tiles in it, until it answers false.
-template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_share(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, F f) {
+// Walks the share of this CTA, the whole warp together: f(unit) for every unit that has tiles in it, until it answers false.  none: there are more tiles than a line has, and no unit is walked.
+template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_share(const TreeParams& p, int unit_rows, int unit_tiles, bool may_cut, bool& none, F f) {
     // a list is a kv head's
     const int lane = threadIdx.x & 31, heads = KIND == ATTEND_LISTS ? 1 : p.cache.kv_heads, group = p.group;
     const int seqs = KIND == ATTEND_LISTS ? (int)p.tokens * p.cache.kv_heads : KIND == ATTEND_PREFIX ? p.n_groups : p.seqs;
@@ -78,6 +78,7 @@ template <int KEYS, int KIND, class F> __device__ __forceinline__ bool walk_shar
     for (int o = 16; o > 0; o >>= 1) total64 += __shfl_xor_sync(0xFFFFFFFFu, total64, o);
     if (total64 >= (1LL << 31)) {  // 3e10 keys: no cache holds them, some table says so
         report_status(p.status, STATUS_BAD_INDEX);
+        none = true;
         return true;
     }
     const int total = (int)total64, share = total / (int)gridDim.x, more = total - share * (int)gridDim.x;  // the first `more` CTAs have a position more
@@ -284,11 +285,11 @@ template <int KEYS, class F> __device__ __forceinline__ bool walk_prefixes(const
     return well;
 }
 
-// f(unit) for every unit, or part of one, that this CTA has, the whole warp together, until it answers false.
-template <int KEYS, int KIND, UnitWay WAY, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, F f) {
+// f(unit) for every unit, or part of one, that this CTA has, the whole warp together, until it answers false.  none: set where a line is too long.
+template <int KEYS, int KIND, UnitWay WAY, class F> __device__ __forceinline__ bool walk_line(const TreeParams& p, const TreeCuts& c, int unit_rows, int unit_tiles, bool& none, F f) {
     if constexpr (WAY == UNITS_BY_NUMBER) return walk_units<KEYS, KIND>(p, c, unit_rows, f);
     else if constexpr (WAY == UNITS_IN_PARTS) return walk_prefixes<KEYS>(p, c, unit_rows, unit_tiles, f);
-    else return walk_share<KEYS, KIND>(p, unit_rows, unit_tiles, c.may_cut, f);
+    else return walk_share<KEYS, KIND>(p, unit_rows, unit_tiles, c.may_cut, none, f);
 }
 
 // What a CTA leaves for tree_join_kernel: the unit that begins in its share and does not end there, if there is one.

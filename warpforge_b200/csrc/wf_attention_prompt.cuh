@@ -361,8 +361,8 @@ constexpr int PA_UNIT_TILES = 3;
 constexpr int PA_CUT_TILES = 6, PA_CUT_ANYWAY = 15;
 template <int KIND, class F> __device__ __forceinline__ bool tree_items(const PromptTiles& t, F f) {
     const TreeParams& p = t.tree;
-    bool cut = false;
-    const bool ok = walk_line<PA_KEYS, KIND, KIND == ATTEND_PREFIX ? UNITS_IN_PARTS : UNITS_ON_A_LINE>(p, t.c, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, [&](const LineUnit& u) {
+    bool cut = false, none = false;
+    const bool ok = walk_line<PA_KEYS, KIND, KIND == ATTEND_PREFIX ? UNITS_IN_PARTS : UNITS_ON_A_LINE>(p, t.c, 2 * t.tile_tokens * p.group, PA_UNIT_TILES, none, [&](const LineUnit& u) {
         PromptItem it{};
         it.seq = u.seq, it.head = u.head, it.row0 = u.q.row0, it.rows = u.q.rows, it.context = u.q.context;
         it.keys = keys_of<KIND>(u.q);

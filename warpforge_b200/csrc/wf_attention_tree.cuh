@@ -167,8 +167,8 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
     const uint64_t policy = KIND == ATTEND_OWN ? read_once_policy() : 0;
     int seg = 0, slot = 0, number = 0;
     uint32_t seg_phase = 1, phase = 1;
-    bool cut = false;  // a unit that begins here goes on in the next share
-    const bool ok = walk_line<TA_KEYS, KIND, BY_NUMBER ? UNITS_BY_NUMBER : UNITS_ON_A_LINE>(p, t.c, ROWS, Shape::UNIT_TILES, [&](const LineUnit& u) {
+    bool cut = false, none = false;  // a unit that begins here goes on in the next share; no unit is walked
+    const bool ok = walk_line<TA_KEYS, KIND, BY_NUMBER ? UNITS_BY_NUMBER : UNITS_ON_A_LINE>(p, t.c, ROWS, Shape::UNIT_TILES, none, [&](const LineUnit& u) {
         const int keys = keys_of<KIND>(u.q), count = min(ROWS, u.q.rows * group - u.first);
         // the page of a lane's tile, asked for before anything is waited for
         const int* const table = u.q.place.table;
@@ -231,7 +231,7 @@ __device__ __forceinline__ bool tree_load(const TreeTiles& t, TreeShared<TreeSha
         if (++seg == TA_SEGMENTS) seg = 0, seg_phase ^= 1;
         return true;
     });
-    if (KIND == ATTEND_PREFIX && loader == 0) leave_prefixes(p, false);
+    if (KIND == ATTEND_PREFIX && loader == 0) leave_prefixes(p, none);
     if (KIND == ATTEND_WHOLE && loader == 0 && blockIdx.x == 0)
         for (int g = lane; g < p.n_groups; g += 32) group_seqs(p, g);  // groups that no sequence's search has come to are looked at, too
     if (!BY_NUMBER && t.c.may_cut && !cut && loader == 0 && lane == 0) t.c.cuts[blockIdx.x].first_cta = -1;  // where a wait ran out, too: tree_join_kernel follows it
