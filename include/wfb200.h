@@ -394,7 +394,9 @@ int wf_select_pages(int64_t ctx, const wf_select_pages_args* args, int64_t strea
  *   pages_dev, lens_dev  as wf_select_pages leaves them: int32 [tokens][kv_heads][width], int32 [tokens][kv_heads][2] (8-byte aligned).  Key t of a list lies in row t % page_tokens of page
  *                   pages[t / page_tokens]; a token sees the first lens[0] keys, and of the lens[1] - lens[0] behind them (64 at most) those of its ancestors
  *   ancestors_dev   uint64 [tokens]; 0 (no array) = all of them
- * A list may name pages in any order, and one twice.  {0, 0} is an empty list, its rows are zeros; lengths that cannot be are WF_ERR_INDEX and rows of zeros. */
+ * A list may name pages in any order, and one twice.  {0, 0} is an empty list, its rows are zeros; lengths that cannot be are WF_ERR_INDEX and rows of zeros.  Lists for groups of
+ * up to 16 heads count 17 each, of more heads 33 for every 32 of them: 2^31 or more are WF_ERR_TOO_LARGE, and where their keys, 16 at a time, make as many of them, WF_ERR_INDEX and rows as
+ * they were. */
 typedef struct wf_selected_attention_args {
     int64_t q_dev, out_dev;
     int64_t q_stride;

@@ -154,3 +154,31 @@ def test_shared_prefixes_of_more_tiles_than_a_line_has(backend):
     for _ in range(2):
         assert torch.count_nonzero(run(2048)) > 0  # sums in the scratch
         assert torch.count_nonzero(run(1 << 28)) == 0
+
+
+def test_selected_more_lists_than_a_line_has(backend):
+    """2^27 lists, each of which is a place on the CTAs' line and 16 more for what it costs: refused before anything is read; as many as have room are done."""
+    import torch
+
+    from warpforge_b200 import _native as N
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(22)
+    tokens, few = 1 << 24, 1 << 16
+    q, out, keys = (torch.empty(n, 8, 16, 8, dtype=torch.bfloat16, device="cuda") for n in (tokens // 16, tokens // 16, 1))
+    q, out = q.view(tokens, 8, 8), out.view(tokens, 8, 8)
+    lists, lens = torch.zeros(tokens, 8, 1, dtype=torch.int32, device="cuda"), torch.zeros(tokens, 8, 2, dtype=torch.int32, device="cuda")
+    keys.copy_(normal(rng, 1, 8, 16, 8))
+    lens[:few] = 1  # a key each
+    out.fill_(7.0)
+    torch.cuda.synchronize()
+    with pytest.raises(N.WfError) as e:
+        A.SelectedAttention(backend.cuda_context, held(q), held(keys), held(keys), held(out), held(lists), held(lens)).run()
+    assert e.value.status == N.WF_ERR_TOO_LARGE
+    backend.synchronize_device()
+    assert (out == 7).all()
+    q[:few] = normal(rng, few, 8, 8)
+    torch.cuda.synchronize()
+    A.SelectedAttention(backend.cuda_context, held(q[:few]), held(keys), held(keys), held(out[:few]), held(lists[:few]), held(lens[:few])).run()
+    backend.synchronize_device()
+    assert torch.equal(out[:few], keys[0, :, 0].expand(few, 8, 8)) and (out[few:] == 7).all()

@@ -10,7 +10,7 @@ namespace wf {
 
 inline int check_queries(Context* c, const char* what, int64_t q, int64_t out, int64_t q_stride, int64_t tokens, int seqs, int q_heads, const wf_kv_cache* cache) {
     if (!q || !out || (q | out) & 15) return set_error(c, WF_ERR_INVALID_ARGUMENT, "%s: q and out must be 16-byte aligned device addresses", what);
-    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
+    if (tokens < 0 || tokens > (1LL << 31) - 1024 || seqs < 0 || seqs > (1LL << 31) - 1024 || q_heads < 1 || q_heads > 8192 || tokens * q_heads >= (1LL << 31))
         return set_error(c, WF_ERR_SHAPE, "%s: bad shape tokens=%lld seqs=%d q_heads=%d", what, (long long)tokens, seqs, q_heads);
     if (q_heads % cache->kv_heads) return set_error(c, WF_ERR_SHAPE, "%s: %d query heads over %d kv heads", what, q_heads, cache->kv_heads);
     if (q_heads / cache->kv_heads > 128) return set_error(c, WF_ERR_TOO_LARGE, "%s: more than 128 query heads for each kv head", what);
@@ -71,6 +71,8 @@ template <int CHUNKS, int MT, int KIND> inline int launch_tree(Context* c, const
     }
     const int64_t tiles = (unit_keys + TA_KEYS - 1) / TA_KEYS;
     units *= (unit_rows + Shape::ROWS - 1) / Shape::ROWS;
+    // every list is a tile on the line, and what a unit costs beside it
+    if (KIND == ATTEND_LISTS && units * (1 + Shape::UNIT_TILES) >= 1LL << 31) return set_error(c, WF_ERR_TOO_LARGE, "%s: %lld lists, rows %d at a time", what, (long long)units, Shape::ROWS);
     TreeTiles t{};
     t.p = p;
     t.c.may_cut = line_is_cut(units, tiles, c->sm_count, TA_CUT_TILES, TA_CUT_ANYWAY);
