@@ -348,7 +348,9 @@ int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, 
 /* ---- attention that reads less than every key of every sequence --------------------------
  * Pages that a token reads, chosen by what their keys promise (wf_page_bounds, wf_select_pages, wf_selected_attention), and keys that sequences have in
  * common read once for all of them (wf_shared_prefix_attention).  (No counterpart in the reference, which has no cache.)
- * The last three work in their stream's scratch, as the operators above do: WF_ERR_RECORDING where a recorded call would have to enlarge it.
+ * The last three work in their stream's scratch, as the operators above do: WF_ERR_RECORDING where a recorded call would have to enlarge it.  The largest call yet says how large it is:
+ * up to 1 GiB for the scores of several new tokens of a sequence (4 bytes for each token, kv head and page of max_context), up to 1 GiB and 60 MB for rows' sums over prefixes (264
+ * bytes for each token and query head, 520 where heads have more than 64 elements) and pieces of them; calls that would want more do without.
  *
  * wf_page_bounds: of every page that holds one of the tokens first[s] .. stop[s] - 1 of a sequence, in every layer and head, the bounds of the keys of its tokens below
  * stop[s]:  codes = ceil(max_t k[t][d] / scale), floor(min_t k[t][d] / scale), scale the least power of two for which all are -127 .. 127 (2^-60 at least).  A page with an Inf

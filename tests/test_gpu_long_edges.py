@@ -182,3 +182,32 @@ def test_selected_more_lists_than_a_line_has(backend):
     A.SelectedAttention(backend.cuda_context, held(q[:few]), held(keys), held(keys), held(out[:few]), held(lists[:few]), held(lens[:few])).run()
     backend.synchronize_device()
     assert torch.equal(out[:few], keys[0, :, 0].expand(few, 8, 8)) and (out[few:] == 7).all()
+
+
+def test_shared_sums_of_no_more_than_a_call_may_have(backend):
+    """Rows whose sums over a prefix would take more than 1 GiB: the call does without, in far less memory.  Both it and the one beside it, with fewer rows, are what TreeAttention
+    gives, to 2^-6 of the largest value (as in test_shared_is_what_trees_are)."""
+    import torch
+
+    from warpforge_b200 import attention as A
+
+    rng = np.random.default_rng(23)
+    heads, dim, drafts = 128, 72, 64
+    keys, values = normal(rng, 600, 1, 32, dim), normal(rng, 600, 1, 32, dim)
+    groups, prefix = None, i32([64])
+    for seqs in (254, 200):
+        n = seqs * drafts
+        assert (n * heads * 130 * 4 > 1 << 30) == (seqs == 254)
+        q = torch.randn(n, heads, dim, device="cuda", dtype=torch.bfloat16, generator=torch.Generator(device="cuda").manual_seed(seqs))
+        tables, context, groups = i32([[0, 1, 2 + 2 * s, 3 + 2 * s] for s in range(seqs)]), i32([64] * seqs), i32([0, seqs])
+        want, out = torch.empty_like(q), torch.full_like(q, 7.0)
+        args = [held(x) for x in (q, keys, values)]
+        torch.cuda.synchronize()
+        A.TreeAttention(backend.cuda_context, *args, held(want), held(tables), held(context), max_context=64, max_drafts=drafts).run()
+        backend.synchronize_device()
+        free = torch.cuda.mem_get_info()[0]
+        A.SharedPrefixAttention(backend.cuda_context, *args, held(out), held(tables), held(context), held(groups), held(prefix), max_prefix=64, max_own=0, max_drafts=drafts).run()
+        backend.synchronize_device()
+        if seqs == 254:
+            assert free - torch.cuda.mem_get_info()[0] < 256 << 20
+        assert (out.float() - want.float()).abs().max() <= 2.0**-6 * values.float().abs().max()

@@ -10,6 +10,7 @@ typedef __nv_bfloat16 bf16;
 
 constexpr int ATTN_MAX_DIM = 128;
 constexpr int TREE_MAX_DRAFTS = 64;  // a row's ancestors are one 64-bit word
+constexpr int64_t ATTN_CALL_BYTES = 1LL << 30;  // of a selection's scores, or of rows' sums over a prefix, that a call may have in its stream's scratch
 
 // What rows attend to: a prompt's past and itself; a sequence's context and new tokens; a list of pages for each token and kv head; where sequences have a prefix in
 // common, that prefix (the rows of all of them), and what a sequence has of its own behind it; or both, a sequence at a time.

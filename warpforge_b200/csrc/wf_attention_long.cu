@@ -70,11 +70,13 @@ template <int CHUNKS> static int launch_shared(Context* c, TreeParams p, cudaStr
     const int64_t units = (int64_t)p.seqs * p.cache.kv_heads, unit_rows = p.max_drafts * p.group, own_keys = p.max_context + p.max_drafts, all_keys = p.max_prefix + own_keys;
     const int64_t prefix_rows = p.tokens * p.group;
     const int64_t prefixes = (int64_t)p.n_groups * p.cache.kv_heads;
+    const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
     const double share = share_of_rows(c, units, unit_rows, all_keys), share_of_prefix = share_of_rows(c, prefixes, prefix_rows, p.max_prefix);
     const bool sixteen = prefix_rows > 32 && share_of_prefix <= SHARE_OF_PREFIX;
     if (sixteen ? share <= SHARE_MORE_AGAIN + share_of_prefix : unit_rows > 32 && share <= SHARE_AGAIN) return launch_units<CHUNKS, 1, ATTEND_WHOLE>(c, p, units, (int)unit_rows, all_keys, s);
     if (!sixteen && again <= (prefix_rows > 32 ? AGAIN_BYTES : AGAIN_FEW_BYTES) && few_rows(p)) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
-    const int64_t rows = p.tokens * p.q_heads, sums = (rows * (CHUNKS * 64 + 2) * (int64_t)sizeof(float) + 255) & ~255LL;
+    // more sums than a call may have: without any
+    if (sums > ATTN_CALL_BYTES) return launch_rows<CHUNKS, ATTEND_WHOLE>(c, p, units, unit_rows, all_keys, s);
     // the most cut units and pieces of them that any of the kernels leaves
     const int64_t most_cuts = (PREFIX_ROUNDS - 1) * c->sm_count, pieces = (int64_t)c->sm_count * PREFIX_ROUNDS * 2 * PA_ROWS * (CHUNKS * 64 + 2);
     TreeCuts cuts{};

@@ -150,7 +150,6 @@ struct SelectParams {
     __device__ __forceinline__ int token_of(int head) const { return group_inverse ? (int)__umulhi((uint32_t)head, group_inverse) : head; }  // head / group, below 64 x 128
 };
 constexpr int SELECT_MAX_GROUP = 128, SELECT_BINS = 256, SELECT_FEW = 256;  // SELECT_FEW: no more than a CTA has threads
-constexpr int64_t SCORE_BYTES = 1LL << 30;  // of scores in memory, at most
 
 __device__ __forceinline__ void mma_s8(int (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0, uint32_t b1) {
     asm("mma.sync.aligned.m16n8k32.row.col.s32.s8.s8.s32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, {%0, %1, %2, %3};"
@@ -741,7 +740,7 @@ template <int CHUNKS> static int launch_selections(Context* c, SelectParams p, i
     // heads, 1000, 2 x 1, 5 x 1, 21 x 1: 9.8 / 10.7, 13.4 / 12.1, 18.3 / 15.3; 4000: 20.7 / 16.1, 22.3 / 15.7, 60 / 22.6; 16 / 2 heads, 21 x 1, 21 x 4 of 4000: 22.2 / 28.3, 60 / 32.
     const int64_t heads = (int64_t)p.max_drafts * p.group, lists = p.tokens * p.kv_heads;
     const bool scored = p.room <= 512 ? lists >= 200 + 11 * heads / 2 : lists * p.room >= 20480 + 1024 * heads;
-    if (p.max_drafts > 1 && scored && bytes <= SCORE_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
+    if (p.max_drafts > 1 && scored && bytes <= ATTN_CALL_BYTES && (int64_t)seqs * p.kv_heads <= 65535) {
         GemvScratch& scratch = c->gemv_scratch[s];
         if (bytes > scratch.attn_bytes) {
             const int rc = refuse_allocation_while_recording(c, s, "the scores of select_pages");
