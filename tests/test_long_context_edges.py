@@ -99,3 +99,13 @@ def test_full_pages_have_bounds_of_all_their_rows():
         for s in seqs:
             s.free()
         m.close()
+
+
+def test_lists_have_room_for_the_tokens_of_a_step():
+    """... which are no more than 64 for each sequence, however long prompts are."""
+    for max_tokens, max_sequences, tokens in ((4096, 2, 128), (50, 2, 50), (128, 2, 128)):
+        m = decoder(max_tokens=max_tokens, max_sequences=max_sequences)
+        assert (m.ctx.room[m.buf["lists"]], m.ctx.room[m.buf["list_lens"]]) == (tokens * 12 * 4, tokens * 8)
+        seqs = [m.sequence() for _ in range(max_sequences)]
+        m.step(seqs, [[0] * (tokens // max_sequences)] * max_sequences, [[-1] * (tokens // max_sequences)] * max_sequences)
+        m.close()

@@ -98,7 +98,9 @@ class Decoder:
             self._room.update(groups=(max_sequences + 1) * 4, prefixes=(max_sequences + 1) * 4)
         self.bounds = A.PageBounds(self.cache) if selected_pages else None
         if selected_pages:
-            self._room.update(before=(max_sequences + 1) * 4, moved=(max_sequences + 1) * 4, lists=max_tokens * s.kv_heads * selected_pages * 4, list_lens=max_tokens * s.kv_heads * 8)
+            self._room.update(before=(max_sequences + 1) * 4, moved=(max_sequences + 1) * 4)
+            new = min(max_tokens, max_sequences * MAX_DRAFTS) * s.kv_heads  # lists of a step
+            self._room.update(lists=new * selected_pages * 4, list_lens=new * 8)
         self._room = {n: max(room, 16) for n, room in self._room.items()}
         self.buf.update({n: self._alloc(room) for n, room in self._room.items()})
 
