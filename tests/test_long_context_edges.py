@@ -1,8 +1,10 @@
-"""A decoder that selects pages, as far as it needs no device: which bounds it asks for, which memory it holds."""
+"""A decoder that selects pages or shares prefixes, as far as it needs no device: which bounds it asks for, which memory it holds, what its command takes."""
 import numpy as np
+import pytest
 
 from test_long_context_host import HostContext
 
+from warpforge_b200 import generate
 from warpforge_b200.generate import Decoder, DecoderSpec
 from warpforge_b200.quant import QuantizationType
 
@@ -109,3 +111,18 @@ def test_lists_have_room_for_the_tokens_of_a_step():
         seqs = [m.sequence() for _ in range(max_sequences)]
         m.step(seqs, [[0] * (tokens // max_sequences)] * max_sequences, [[-1] * (tokens // max_sequences)] * max_sequences)
         m.close()
+
+
+@pytest.mark.parametrize("more", [[], ["--samples", "3", "--share-prefixes"], ["--selected-pages", "66"]])
+def test_the_command_takes_prompts_as_long_as_there_are_positions(monkeypatch, capsys, more):
+    """... where nothing is decoded behind them; where something is, one less."""
+    class Closed(HostContext):
+        def close(self):
+            assert not self.room
+
+    monkeypatch.setattr(generate, "CudaContext", lambda device: Closed())
+    small = ["x", "--qtype", "Q8_0", "--layers", "1", "--d-model", "64", "--heads", "2", "--kv-heads", "1", "--ffn", "64", "--vocab", "64", "--sequences", "1"]
+    for prompt, tokens in ((4096, 1), (4095, 2), (7, 3)):
+        monkeypatch.setattr("sys.argv", small + ["--prompt", str(prompt), "--tokens", str(tokens)] + more)
+        generate.main()
+        assert "tokens/s" in capsys.readouterr().out

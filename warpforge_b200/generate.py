@@ -339,7 +339,8 @@ def main() -> None:
     warm = [model.sequence() for _ in prompts]
     model.prefill(warm, prompts)
     warm = samples(warm)
-    model.step(warm, [[0]] * len(warm))
+    if a.tokens > 1:  # else nothing is decoded, and a prompt may have every position that there is
+        model.step(warm, [[0]] * len(warm))
     for s in warm:
         s.free()
     seqs = [model.sequence() for _ in prompts]
