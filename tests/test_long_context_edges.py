@@ -2,9 +2,11 @@
 import numpy as np
 import pytest
 
-from test_long_context_host import HostContext
+from test_long_context_host import HostContext, dev
 
+from warpforge_b200 import attention as A
 from warpforge_b200 import generate
+from warpforge_b200.backend import DeviceTensor
 from warpforge_b200.generate import Decoder, DecoderSpec
 from warpforge_b200.quant import QuantizationType
 
@@ -126,3 +128,47 @@ def test_the_command_takes_prompts_as_long_as_there_are_positions(monkeypatch, c
         monkeypatch.setattr("sys.argv", small + ["--prompt", str(prompt), "--tokens", str(tokens)] + more)
         generate.main()
         assert "tokens/s" in capsys.readouterr().out
+
+
+def test_operators_refuse_gaps_ranks_and_numbers():
+    """Only queries may have gaps; arrays of other ranks are refused like those of other sizes; what 32 bits do not hold is not cut down to what they do."""
+    ctx = HostContext()
+    gaps = lambda t: DeviceTensor(t.ptr, t.shape(), t.dtype, row_stride=int(np.prod(t.shape()[1:])) + 8)  # noqa: E731
+    q, kv, table, n = dev("bf16", 3, 4, 64), dev("bf16", 9, 2, 16, 64), dev("i32", 3, 5), dev("i32", 3)
+    codes, scales, lists, lens = dev("i8", 9, 2, 2, 64), dev("f32", 9, 2), dev("i32", 3, 2, 6), dev("i32", 3, 2, 2)
+    gap, wrong = A.UnsupportedOperationError, ValueError
+
+    def select(q=q, codes=codes, scales=scales, table=table, lists=lists, lens=lens, page_tokens=16, **more):
+        return A.SelectPages(ctx, q, codes, scales, table, n, lists, lens, page_tokens=page_tokens, max_context=50, **more)
+
+    assert select().args.width == 6 and select(q=gaps(q)).args.q_stride == 264
+    for error, bad in ((gap, dict(codes=gaps(codes))), (gap, dict(scales=gaps(scales))), (gap, dict(table=gaps(table))), (gap, dict(lists=gaps(lists))), (gap, dict(lens=gaps(lens))),
+                       (wrong, dict(lists=dev("i32", 3, 2))), (wrong, dict(lists=dev("i32", 18))), (wrong, dict(codes=dev("i8", 9))), (wrong, dict(q=dev("bf16", 3, 256))),
+                       (wrong, dict(recent=2**32)), (wrong, dict(first=2**32 + 1)), (wrong, dict(max_drafts=2**32 + 1)), (wrong, dict(page_tokens=2**32 + 16))):
+        with pytest.raises(error):
+            select(**bad)
+
+    def selected(q=q, lists=lists, lens=lens):
+        return A.SelectedAttention(ctx, q, kv, kv, q, lists, lens)
+
+    assert selected().args.width == 6
+    for error, bad in ((gap, dict(lists=gaps(lists))), (gap, dict(lens=gaps(lens))), (wrong, dict(lists=dev("i32", 3, 2))), (wrong, dict(lists=dev("i32", 36)))):
+        with pytest.raises(error):
+            selected(**bad)
+
+    def shared(table=table, **more):
+        return A.SharedPrefixAttention(ctx, q, kv, kv, q, table, n, dev("i32", 2), dev("i32", 1), max_prefix=16, max_own=16, **more)
+
+    shared()
+    for error, bad in ((gap, dict(table=gaps(table))), (wrong, dict(table=dev("i32", 15))), (wrong, dict(max_drafts=2**32 + 1))):
+        with pytest.raises(error):
+            shared(**bad)
+
+    cache = A.KvCache(ctx, 2, 9, 16, 2, 64)
+    codes, scales = dev("i8", 2, 9, 2, 2, 64), dev("f32", 2, 9, 2)
+    for bad in ((gaps(codes), scales), (codes, gaps(scales))):
+        with pytest.raises(gap):
+            A.PageBounds(cache, *bad)
+    with pytest.raises(gap):
+        A.PageBounds(cache, codes, scales).update(gaps(table), n, n, max_tokens=1)
+    cache.close()

@@ -58,6 +58,21 @@ def _dense(name: str, t: DeviceTensor) -> None:
         raise UnsupportedOperationError(f"{name} must be without gaps")
 
 
+def _rows(name: str, t: DeviceTensor, dtype: str, *dims) -> int:
+    """The address of `t`, which has this type and these dimensions (None: any) and no gaps."""
+    at = _typed(name, t, dtype, *dims)
+    _dense(name, t)
+    return at
+
+
+def _counts(**values: int) -> dict:
+    """Numbers for 32-bit arguments, which would cut others down without a word."""
+    for name, n in values.items():
+        if not -(2**31) <= n < 2**31:
+            raise ValueError(f"{name} {n}")
+    return values
+
+
 def _stride(t: DeviceTensor) -> int:
     return t.row_stride or int(np.prod(t.shape()[1:]))
 
@@ -177,12 +192,12 @@ class SharedPrefixAttention(_Bound):
         dim = cache.head_dim
         tokens, heads = q.shape()[:2]
         seqs, n = context_lens.shape()[0], prefix_lens.shape()[0]
-        a = N.SharedPrefixAttentionArgs(tokens=tokens, q_heads=heads, seqs=seqs, max_drafts=max_drafts, n_groups=n, max_prefix=max_prefix, max_own=max_own,
+        a = N.SharedPrefixAttentionArgs(tokens=tokens, q_heads=heads, seqs=seqs, n_groups=n, max_prefix=max_prefix, max_own=max_own, **_counts(max_drafts=max_drafts),
                                         scale=1 / math.sqrt(dim) if scale is None else scale)
         a.q_dev, a.out_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _typed("out", out, "bf16", tokens, heads, dim), _stride(q)
         _dense("out", out)
         a.q_offsets_dev = _typed("q_offsets", q_offsets, "i32", seqs + 1)
-        a.tables_dev, a.table_stride = _typed("tables", tables, "i32", seqs, None), tables.shape()[1]
+        a.tables_dev, a.table_stride = _rows("tables", tables, "i32", seqs, None), tables.shape()[1]
         a.context_dev, a.ancestors_dev = _typed("context_lens", context_lens, "i32", seqs), _typed("ancestors", ancestors, "i64", tokens)
         a.groups_dev, a.prefix_dev = _typed("groups", groups, "i32", n + 1), _typed("prefix_lens", prefix_lens, "i32", n)
         super().__init__(context, "wf_shared_prefix_attention", a, cache, layer, (q, keys, values, out, tables, context_lens, groups, prefix_lens, q_offsets, ancestors))
@@ -196,10 +211,11 @@ class SelectedAttention(_Bound):
         cache = _cache_args(keys, values)
         dim = cache.head_dim
         tokens, heads = q.shape()[:2]
-        a = N.SelectedAttentionArgs(tokens=tokens, q_heads=heads, width=pages.shape()[2], scale=1 / math.sqrt(dim) if scale is None else scale)
+        a = N.SelectedAttentionArgs(tokens=tokens, q_heads=heads, scale=1 / math.sqrt(dim) if scale is None else scale)
         a.q_dev, a.out_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _typed("out", out, "bf16", tokens, heads, dim), _stride(q)
         _dense("out", out)
-        a.pages_dev, a.lens_dev = _typed("pages", pages, "i32", tokens, cache.kv_heads, None), _typed("lens", lens, "i32", tokens, cache.kv_heads, 2)
+        a.pages_dev, a.lens_dev = _rows("pages", pages, "i32", tokens, cache.kv_heads, None), _rows("lens", lens, "i32", tokens, cache.kv_heads, 2)
+        a.width = pages.shape()[2]
         a.ancestors_dev = _typed("ancestors", ancestors, "i64", tokens)
         super().__init__(context, "wf_selected_attention", a, cache, layer, (q, keys, values, out, pages, lens, ancestors))
 
@@ -248,15 +264,15 @@ class SelectPages(_Bound):
                  q_offsets=None, max_drafts: int = 1, tree: bool = False):
         tokens, heads, dim = q.shape()
         seqs, (pages, kv_heads) = context_lens.shape()[0], codes.shape()[:2]
-        a = N.SelectPagesArgs(tokens=tokens, q_heads=heads, seqs=seqs, max_drafts=max_drafts, max_context=max_context, pages=pages, kv_heads=kv_heads, head_dim=dim, page_tokens=page_tokens,
-                              first=first, recent=recent, width=pages_out.shape()[2], flags=N.WF_SELECT_TREE if tree else 0)
+        a = N.SelectPagesArgs(tokens=tokens, q_heads=heads, seqs=seqs, max_context=max_context, pages=pages, kv_heads=kv_heads, head_dim=dim, flags=N.WF_SELECT_TREE if tree else 0,
+                              **_counts(max_drafts=max_drafts, page_tokens=page_tokens, first=first, recent=recent))
         a.q_dev, a.q_stride = _typed("q", q, "bf16", tokens, heads, dim), _stride(q)
-        a.codes_dev, a.scales_dev = _typed("codes", codes, "i8", pages, kv_heads, 2, dim), _typed("scales", scales, "f32", pages, kv_heads)
+        a.codes_dev, a.scales_dev = _rows("codes", codes, "i8", pages, kv_heads, 2, dim), _rows("scales", scales, "f32", pages, kv_heads)
         a.q_offsets_dev = _typed("q_offsets", q_offsets, "i32", seqs + 1)
-        a.tables_dev, a.table_stride = _typed("tables", tables, "i32", seqs, None), tables.shape()[1]
+        a.tables_dev, a.table_stride = _rows("tables", tables, "i32", seqs, None), tables.shape()[1]
         a.context_dev = _typed("context_lens", context_lens, "i32", seqs)
-        a.pages_out_dev = _typed("pages_out", pages_out, "i32", tokens, kv_heads, None)
-        a.lens_out_dev = _typed("lens_out", lens_out, "i32", tokens, kv_heads, 2)
+        a.pages_out_dev = _rows("pages_out", pages_out, "i32", tokens, kv_heads, None)
+        a.lens_out_dev, a.width = _rows("lens_out", lens_out, "i32", tokens, kv_heads, 2), pages_out.shape()[2]
         super().__init__(context, "wf_select_pages", a, None, 0, (q, codes, scales, tables, context_lens, pages_out, lens_out, q_offsets))
 
 
@@ -509,7 +525,7 @@ class PageBounds:
                 for n in (2 * cache.head_dim, 4):
                     self._owned.append(ctx.allocate(int(np.prod(shape)) * n))
                 codes, scales = DeviceTensor(self._owned[0], (*shape, 2, cache.head_dim), "i8", owner=ctx), DeviceTensor(self._owned[1], shape, "f32", owner=ctx)
-            self._addresses = _typed("codes", codes, "i8", *shape, 2, cache.head_dim), _typed("scales", scales, "f32", *shape)
+            self._addresses = _rows("codes", codes, "i8", *shape, 2, cache.head_dim), _rows("scales", scales, "f32", *shape)
         except BaseException:
             for p in self._owned:
                 ctx.free(p)
@@ -521,7 +537,7 @@ class PageBounds:
         tokens of a sequence."""
         seqs, ctx = first.shape()[0], self.cache.context
         ctx._ck("wf_page_bounds", ctx._lib.wf_page_bounds(
-            ctx.handle, self.cache._ref, *self._addresses, _typed("tables", tables, "i32", seqs, None), tables.shape()[1], _typed("first", first, "i32", seqs),
+            ctx.handle, self.cache._ref, *self._addresses, _rows("tables", tables, "i32", seqs, None), tables.shape()[1], _typed("first", first, "i32", seqs),
             _typed("stop", stop, "i32", seqs), seqs, max_tokens, stream))
 
     def layer(self, i: int):
