@@ -359,7 +359,8 @@ int wf_cache_compact(int64_t ctx, const wf_kv_cache* cache, int64_t tables_dev, 
  *   scales_dev  fp32 [layers][pages][kv_heads]
  *   tables_dev  int32 [seqs][table_stride]; first_dev, stop_dev int32 [seqs]
  *   max_tokens  most tokens stop[s] - first[s] of a sequence; a range of more pages than so many tokens can touch is WF_ERR_INDEX and left out
- * Sequences that share a page should agree on how many of its tokens count: else the bounds are one or the other's. */
+ * Sequences that share a page have to agree on how many of its tokens count, or a page has to be in one range only: its bounds are written by each of them, in three stores that
+ * nothing orders, and could be the codes of one with the scale of another. */
 int wf_page_bounds(int64_t ctx, const wf_kv_cache* cache, int64_t codes_dev, int64_t scales_dev, int64_t tables_dev, int64_t table_stride, int64_t first_dev, int64_t stop_dev,
                    int64_t seqs, int64_t max_tokens, int64_t stream);
 
@@ -416,8 +417,8 @@ int wf_selected_attention(int64_t ctx, const wf_selected_attention_args* args, c
  *   groups_dev   int32 [n_groups + 1], ascending from 0 to seqs; prefix_dev int32 [n_groups], 0 = nothing in common
  *   max_prefix   most tokens of a prefix; max_own: most context[s] - prefix of a sequence
  * A group whose prefix, sequences or offsets cannot be, a sequence with a context shorter than the prefix, and one with rows outside those of its group
- * (q_offsets[groups[g]] .. q_offsets[groups[g + 1]]) are WF_ERR_INDEX and rows of zeros.  So is a call whose prefixes, 16 keys at a time, are 2^31 or more for all heads together;
- * where the other keys are that many, WF_ERR_INDEX and rows as they were.  At most WF_SHARED_MAX_TOKENS tokens. */
+ * (q_offsets[groups[g]] .. q_offsets[groups[g + 1]]) are WF_ERR_INDEX and rows of zeros.  A call whose prefixes, 16 keys at a time, are 2^31 or more for all heads together may be so,
+ * too; where the other keys are that many, WF_ERR_INDEX and rows as they were.  At most WF_SHARED_MAX_TOKENS tokens. */
 #define WF_SHARED_MAX_TOKENS 131072
 typedef struct wf_shared_prefix_attention_args {
     int64_t q_dev, out_dev;

@@ -37,8 +37,9 @@ struct BoundsParams {
 };
 
 // A warp has one head of one page in one layer, contiguous in memory: a lane has 8 elements of a row, 32 / (dim / 8) rows go with one load, BOUNDS_DEPTH loads are in flight.  Every key of the
-// pages is read once and nothing is left to wait for but HBM: 8192 tokens of 32 layers x 8 heads of 128 (537 MB and 9 of bounds) 75 us, as fast as a plain read; 48 decoded tokens, whose pages of
-// up to 64 tokens are read again in all of 32 layers (39 MB), 6.3 us, half of it a launch and the two loads before the first key (the table, the page).
+// pages is read once and nothing is left to wait for but HBM: 8192 tokens of 32 layers x 8 heads of 128 (537 MB and 9 of bounds) 75 us, as fast as a plain read; 16 decoded tokens, whose pages of
+// up to 64 tokens are read again in all of 32 layers (39 MB), 6.3 us where the L2 has them, half of it a launch and the two loads before the first key (the table, the page), and 15 out of HBM: a launch, those
+// loads and one round of warps, each of which waits for all of its keys once.
 constexpr int BOUNDS_WARPS = 4, BOUNDS_DEPTH = 8;
 __device__ __forceinline__ uint32_t max2(uint32_t a, uint32_t b) {  // NaN where one of them is
     uint32_t r;
@@ -224,7 +225,7 @@ template <int CHUNKS> struct PageTile {
     uint4 codes[2][CHUNKS];
     int scale[2];  // what a page's scale adds to a score; FIRST: the page comes before others, NOWHERE: it is not in the cache
     static constexpr int NOWHERE = INT_MIN + 1, FIRST = INT_MIN;
-    // the pages' numbers; -1: a place behind the last
+    // the pages' numbers; behind the last place page 0, whose score goes nowhere
     static __device__ __forceinline__ int2 find(const int* table, const SelectSeq& q, int t) {
         const int n = t * 16 + ((threadIdx.x & 31) >> 2);
         return make_int2(n < q.between ? table[q.first + n] : 0, n + 8 < q.between ? table[q.first + n + 8] : 0);
@@ -475,7 +476,7 @@ template <int RUN> __global__ void __launch_bounds__(FEW_WARPS * 32) select_few_
 // A cluster has one new token and kv head.  Its CTAs score a part of the pages each, 16 pages by the heads of the group a warp at a time (mma.sync on the codes: [q+ | q-] . [hi | lo],
 // the positive elements of q in the one half and the negative ones in the other), and leave the scores in the first CTA's shared memory, which takes the largest.  SCORED: the scores lie in
 // memory.  CHUNKS of 64 codes of a page (hi and lo together).  RUN: scores of a thread, which it keeps in registers; 0: as many as there are, read again each time.
-// Bound by latencies: launch, context, table, codes, and some six barriers of the selection.  One token of 8 heads over 250 pages 6.3 us, of 48 sequences with up to 250 pages 9.7 (13 MB, 1.4 TB/s).
+// Bound by latencies: launch, context, table, codes, and some six barriers of the selection.  One token of 8 kv heads over 497 pages 6.4 us, of 48 sequences with up to 250 pages 9.7 (13 MB, 1.4 TB/s).
 // The largest are found by two or three histograms of eight bits instead of a sort: what is left in a bin of the second, at most 256 scores, is ranked by comparing all with all.
 template <int CHUNKS, int WARPS, int RUN, bool SCORED> __global__ void __launch_bounds__(WARPS * 32, WARPS <= 8 && RUN != 2 ? 2 : WARPS <= 8 ? 3 : SCORED ? 2 : 1) select_pages_kernel(const __grid_constant__ SelectParams p) {
     constexpr int THREADS = WARPS * 32;
