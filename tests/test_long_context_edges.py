@@ -172,3 +172,18 @@ def test_operators_refuse_gaps_ranks_and_numbers():
     with pytest.raises(gap):
         A.PageBounds(cache, codes, scales).update(gaps(table), n, n, max_tokens=1)
     cache.close()
+
+
+def test_bounds_that_are_closed_are_not_written():
+    ctx = HostContext()
+    cache = A.KvCache(ctx, 2, 9, 16, 2, 64)
+    bounds = A.PageBounds(cache)
+    held = len(ctx.room)
+    bounds.update(dev("i32", 3, 4), dev("i32", 3), dev("i32", 3), max_tokens=1)
+    for _ in range(2):
+        bounds.close()
+        assert len(ctx.room) == held - 2
+        for call in (lambda: bounds.update(dev("i32", 3, 4), dev("i32", 3), dev("i32", 3), max_tokens=1), lambda: bounds.layer(0)):
+            with pytest.raises(ValueError):
+                call()
+    cache.close()

@@ -535,6 +535,8 @@ class PageBounds:
     def update(self, tables: DeviceTensor, first: DeviceTensor, stop: DeviceTensor, *, max_tokens: int, stream: int = 0) -> None:
         """In every layer, after tokens first[s] .. stop[s] - 1 (i32 [seqs]) of the sequences have been stored: the bounds of the pages that hold them.  max_tokens: most
         tokens of a sequence."""
+        if self._addresses is None:
+            raise ValueError("bounds that have been closed")
         seqs, ctx = first.shape()[0], self.cache.context
         ctx._ck("wf_page_bounds", ctx._lib.wf_page_bounds(
             ctx.handle, self.cache._ref, *self._addresses, _rows("tables", tables, "i32", seqs, None), tables.shape()[1], _typed("first", first, "i32", seqs),
@@ -542,6 +544,8 @@ class PageBounds:
 
     def layer(self, i: int):
         """codes and scales of one layer."""
+        if self._addresses is None:
+            raise ValueError("bounds that have been closed")
         if not 0 <= i < self.cache.layers:
             raise ValueError(f"layer {i} of {self.cache.layers}")
         of = lambda t, size: DeviceTensor(t.ptr + i * int(np.prod(t.shape()[1:])) * size, t.shape()[1:], t.dtype, owner=t)  # noqa: E731
@@ -549,6 +553,7 @@ class PageBounds:
 
     def close(self) -> None:
         owned, self._owned = self._owned, []
+        self._addresses = None  # the memory may be another's from here on
         for p in owned:
             if self.cache.context.handle:
                 self.cache.context.free(p)
